@@ -212,20 +212,21 @@ def prepare(case, seed):
     num_pages = sum(-(-n // page) for n in after) + 5
     tables, storage = _page_tables(rows, num_pages, page, max_pages, cached, gen, heads)
     state = {"case": c, "tables": tables, "storage": storage, "saved": storage.clone(), "counts": _int32(counts), "total": sum(counts),
-             "longest": max(after)}
+             "longest": max(after), "most": max(counts)}
     if c["kind"] == "tables":
         return state
     # the step's plan is made once and serves every layer
     h, d = heads, c["dim"]
     groups = h if c["per_head"] else 1
     if own:
-        step = _framework()[0].append_tokens(tables, state["counts"], state["total"], max_length=state["longest"])
+        step = _framework()[0].append_tokens(tables, state["counts"], state["total"], max_length=state["longest"],
+                                                max_count=state["most"])
     else:
         step = _plain_append(tables, state["counts"], state["total"])
     cache = {"k": _normal(gen, (num_pages, h, page, d), c["scale"]), "v": _normal(gen, (num_pages, h, page, d)),
              "selected": _history(c, cached, rows, groups, max_pages * page, gen)}
     qkv = tuple(_normal(gen, (state["total"], h, d), s) for s in (c["scale"], c["scale"], 1.0))
-    return dict(state, step=step, cache=cache, history=cache["selected"].clone(), qkv=qkv, most=max(counts))
+    return dict(state, step=step, cache=cache, history=cache["selected"].clone(), qkv=qkv)
 
 
 # ---- the plain forms ---------------------------------------------------------------------------------------------------------
@@ -327,14 +328,12 @@ def _plain_reorder(tables, cache, parents):
     stays = new >= 0
     stays[row, full.clamp_max(max_pages - 1)] &= ~fresh
     had = block < held[:, None]
+    held_before = refs > 0
     refs.scatter_add_(0, old.clamp_min(0).reshape(-1).long(), -had.reshape(-1).to(torch.int32))
     refs.scatter_add_(0, new.clamp_min(0).reshape(-1).long(), stays.reshape(-1).to(torch.int32))
-    # pages that no row has any more go to the end of the free list, in the order of their first place in the old tables
-    place = torch.full((refs.numel(),), rows * max_pages, device=device)
-    place.scatter_reduce_(0, old.clamp_min(0).reshape(-1).long(),
-                          torch.where(had, row[:, None] * max_pages + block, rows * max_pages).reshape(-1), "amin")
-    gone = (refs == 0) & (place < rows * max_pages)
-    rank = (torch.where(gone, place, rows * max_pages)).argsort(stable=True)
+    # pages that no row has any more go to the end of the free list, lowest first
+    gone = (refs == 0) & held_before
+    rank = (~gone).to(torch.uint8).argsort(stable=True)
     n_gone = gone.sum()
     at = torch.arange(rank.numel(), device=device)
     target = torch.where(at < n_gone, count.long() + at, free_pages.numel())
@@ -375,7 +374,8 @@ def run(state):
         if c["kind"] == "tables":                              # one more step from the same state: it goes back, then on
             state["storage"].copy_(state["saved"])
             if own:
-                step = _framework()[0].append_tokens(tables, state["counts"], state["total"], max_length=state["longest"])
+                step = _framework()[0].append_tokens(tables, state["counts"], state["total"], max_length=state["longest"],
+                                                max_count=state["most"])
             else:
                 step = _plain_append(tables, state["counts"], state["total"])
             return [step["query_start"], step["cached"], step["slots"], state["storage"]]
