@@ -338,6 +338,104 @@ int sa_prefill_rows(const sa_problem* p, int cached, const void* q, const void* 
 int sa_cache_store(int dtype, int batch, int heads, int groups, int seq, int capacity, int head_dim, int at, int begin,
                    const sa_tensor* k, const sa_tensor* v, void* k_cache, void* v_cache, float* selected, void* stream);
 
+/* ---- serving many requests: a paged cache, and beams ------------------------------------------------------------------
+ * No counterpart in the reference (one contiguous cache for sequences of one length, mixers.py:105-130).
+ *
+ * Rows (requests, or beams of one) own pages of `page_size` tokens.  The tables are shared by every layer; a layer has its pools of
+ * pages and its history sums.  The numbers of tokens stay on the device, so a step can be captured in a graph. */
+typedef struct sa_page_tables {
+  int32_t struct_bytes;   /* sizeof(sa_page_tables)                                                    */
+  int32_t rows;           /* at most 4096                                                              */
+  int32_t max_pages;      /* of a row                                                                  */
+  int32_t num_pages;      /* of the pools                                                              */
+  int32_t page_size;      /* 16, 32, 64, 128 or 256 tokens                                             */
+  int32_t heads;          /* of the layers that share the tables, at most 256                          */
+  int32_t* block_tables;  /* (rows, max_pages): page of a row's block, -1 where it has none            */
+  int32_t* lengths;       /* (rows): tokens                                                            */
+  int32_t* free_pages;    /* (num_pages): the first free_count entries are free; taken from their end  */
+  int32_t* free_count;    /* (1)                                                                       */
+  int32_t* page_refs;     /* (num_pages): rows that hold a page                                        */
+} sa_page_tables;
+
+/* Row r gets counts[r] (device; below 0: none) new tokens: its pages, its length, and what the step's attention needs.
+ *   total        tokens of the step, in row order, as q, k, v hold them
+ *   max_length   no row has more tokens after the step; max_count: no row gets more
+ *   query_start  (rows + 1): first token of a row; the last entry is where the last row ends (both cut at total)
+ *   cached       (rows): tokens before the step; -1: the row is left as it was (it does not fit `total`, max_length, max_count, its
+ *                table, or the pool -- then nor does any later row that needs a page)
+ *   slots        (total) int64: page * page_size + offset of a token; -1: no row's, or a row that is left as it was
+ *   work         sa_page_step_words() int32 words, 16-byte aligned: the plan of the step's attention
+ * The k-th page that is needed, in row order, is free_pages[free_count - 1 - k]. */
+size_t sa_page_step_words(int rows, int total, int heads);
+int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int total, int max_length, int max_count, int32_t* query_start,
+                   int32_t* cached, int64_t* slots, int32_t* work, void* stream);
+
+/* Selective Attention of a step's new tokens over the pages of their rows (bf16, head_dim 64 or 128; one selector for all heads,
+ * or every head its own).  Stores k and v in their pages, moves the histories on.
+ *   k_pages, v_pages  (num_pages, heads, page_size, head_dim)
+ *   selected          (rows, groups, max_pages * page_size) fp32
+ *   q, k, v           (total, heads, head_dim) with token and head strides, multiples of 8 elements
+ *   y                 (total, heads, head_dim) contiguous; zeros for tokens without a slot
+ *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream); 0: the call
+ *                     clears tickets of its own
+ * A page outside the pool reads as zeros. */
+typedef struct sa_paged_attention {
+  int32_t struct_bytes;   /* sizeof(sa_paged_attention) */
+  int32_t groups, head_dim, exempt, total, max_length, max_count, plan_tickets;
+  const sa_page_tables* tables;
+  const int32_t *query_start, *cached;
+  const int64_t* slots;
+  int32_t* work;
+  void *k_pages, *v_pages;
+  float* selected;
+  const void *q, *k, *v;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  void* y;
+  void* workspace;        /* sa_paged_workspace_bytes(), 256-byte aligned */
+  uint64_t workspace_bytes;
+  void* stream;
+} sa_paged_attention;
+/* 0 while nothing is captured on the stream, else a number of the capture: calls with the plan_tickets of a step have the same one
+ * (and the same stream) as its sa_page_append. */
+unsigned long long sa_stream_capture(void* stream);
+size_t sa_paged_workspace_bytes(const sa_paged_attention* p);
+int sa_paged_run(const sa_paged_attention* p);
+
+/* Row r becomes a copy of row parents[r] (device; outside [0, rows): an empty row, its pages go back).  Full pages are shared; the
+ * page that is being filled stays with the lowest row that has the parent, the others get one of their own.
+ *   copies   (rows, 2): the page to copy and the one that receives it, or -1 -1
+ *   work     sa_page_reorder_words() int32 words, 16-byte aligned; sa_page_move reads it
+ * Pages that no row holds any more go to the end of the free list, lowest first, before the new ones are taken off it.  A row for
+ * which there is none becomes empty.
+ * sa_page_move: the tokens of those pages and the histories of the rows, for one layer.  Behind a row's last token everything is
+ * left as it was. */
+size_t sa_page_reorder_words(int rows, int max_pages, int num_pages);
+int sa_page_reorder(const sa_page_tables* tables, const int32_t* parents, int32_t* copies, int32_t* work, void* stream);
+int sa_page_move(const sa_page_tables* tables, const int32_t* copies, const int32_t* work, int groups, int head_dim, void* k_pages,
+                 void* v_pages, float* selected, void* stream);
+
+/* The `width` (at most 32) best continuations of every group of beams (at most 256): scores[k] + logits[k][v] - log sum_u
+ * exp(logits[k][u]), largest first, equal ones by the lowest k * vocab + v.  A score that is not finite (a beam whose score is
+ * -inf, or whose logits hold a NaN or +inf or nothing but -inf) counts as -inf.
+ *   logits      (groups, beams, vocab) at group and beam strides, contiguous along the vocabulary
+ *   scores      (groups, beams) fp32
+ *   out_scores, out_rows, out_tokens   (groups, width): fp32; int32 group * beams + beam; int64 */
+typedef struct sa_beam {
+  int32_t struct_bytes;   /* sizeof(sa_beam) */
+  int32_t dtype, groups, beams, vocab, width;
+  const void* logits;
+  int64_t group_stride, beam_stride;
+  const float* scores;
+  float* out_scores;
+  int32_t* out_rows;
+  int64_t* out_tokens;
+  void* workspace;        /* sa_beam_workspace_bytes(), 16-byte aligned */
+  uint64_t workspace_bytes;
+  void* stream;
+} sa_beam;
+size_t sa_beam_workspace_bytes(int dtype, int groups, int beams, int vocab, int width);
+int sa_beam_select(const sa_beam* p);
+
 /* Per-kernel device timing for benchmarks.  sa_profile_enable(id) makes every later launch of that
  * kernel record a CUDA event pair on its stream (id 0 disables); sa_profile_collect waits for the
  * recorded pairs, writes their durations in milliseconds (launch order) to ms_host, forgets them and

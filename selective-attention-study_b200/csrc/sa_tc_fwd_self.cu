@@ -29,8 +29,6 @@ namespace sa {
 namespace tc {
 namespace {
 
-constexpr int kTile = 128;          // query rows per CTA; also the carry checkpoint spacing
-constexpr int kRowTile = 16384;     // bytes of a [128][64] bf16 operand tile
 constexpr int kThreads = 512;       // two softmax warpgroups, the selection, four single warps (one idle)
 constexpr int kRing = 3;            // tiles in flight
 // Registers: 512 x 128 at launch; the softmax keeps 128 logits: 256 x 168 + 256 x 88.

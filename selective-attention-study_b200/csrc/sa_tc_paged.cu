@@ -1,0 +1,350 @@
+// Tensor-core engine over a paged cache: rows (requests) of any length, each with the tokens that the step gives it (sm_100a).
+//
+//   store_kernel          new keys and values into their pages; zeros for tokens that no row was given
+//   colsum_pages_kernel   selection pass: column sums of a query tile's relu'd, masked logits, key tile by key tile
+//   scan_pages_kernel     their running sum over the tiles of a row, from the row's history on (-> what the tiles start from), and
+//                         the history moved on
+//   forward_pair_kernel, forward_wide_kernel (PAGED)   sa_tc_fwd_pair.cuh, sa_tc_fwd_wide.cuh
+//
+// The plan of the step (sa_paged.cu) says which tiles there are; the host knows bounds, so a grid covers those and CTAs without
+// a tile return at once.  A query tile is 128 positions of one row, counted from its token 0, as the key tiles are: the
+// triangular running sum needs both to start at the same places.  A key tile is 128 / page_size TMA boxes (or one), which land
+// one behind the other as the rows of one swizzled operand tile.
+//
+// Rows of a tile that are other sequences' queries, and keys behind a row's last token (in its own page, where an earlier row's
+// data stands, or in none), must not reach anything: they are left out of the selection and the logits by selection, not by
+// multiplication, and the values among them are zeroed in shared memory.
+#include "sa_tc_fwd_pair.cuh"
+#include "sa_tc_fwd_wide.cuh"
+
+namespace sa {
+namespace tc {
+namespace {
+
+using paged::Attention;
+using paged::TileItem;
+
+// ---- new rows -----------------------------------------------------------------------------------------------------------------
+struct TokenRows {
+  const uint4* ptr;
+  int64_t token, head;               // strides in 16-byte units
+};
+// A unit is 16 bytes of one token's K or V; heads * units of a token are neighbours.
+__global__ void __launch_bounds__(256) store_kernel(TokenRows k, TokenRows v, uint4* k_pages, uint4* v_pages, uint4* y,
+                                                    const int64_t* __restrict__ slots, int total, int heads, int row_units, int num_pages,
+                                                    int page_shift, unsigned int* tickets, int n_tickets) {
+  after_previous_kernel();
+  const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  if (tickets != nullptr)
+    for (int64_t i = first; i < n_tickets; i += step) tickets[i] = 0u;
+  const int per_token = heads * row_units;
+  const int64_t n = (int64_t)total * per_token, slots_end = (int64_t)num_pages << page_shift;
+  for (int64_t i = first; i < n; i += step) {
+    const int token = (int)(i / per_token), u = (int)(i - (int64_t)token * per_token), h = u / row_units, c = u - h * row_units;
+    const int64_t slot = slots[token];
+    if (slot < 0) y[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (slot < 0 || slot >= slots_end) continue;
+    const int64_t row = ((((slot >> page_shift) * heads + h) << page_shift) + (slot & ((1 << page_shift) - 1))) * row_units + c;
+    k_pages[row] = k.ptr[token * k.token + h * k.head + c];
+    v_pages[row] = v.ptr[token * v.token + h * v.head + c];
+  }
+}
+
+// ---- selection column sums --------------------------------------------------------------------------------------------------
+// As colsum_kernel (sa_tc_fwd.cu), with the loops the other way round: a CTA keeps one query tile and takes a run of `chunk` key
+// tiles, since rows have few query tiles.  128 threads own a key each, a fifth warp loads and issues, one tile ahead.
+template <int D>
+__global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                           float* __restrict__ carry, int exempt, float scale, WaitCtx status, int chunk,
+                                                           const TileItem* __restrict__ tiles, const __grid_constant__ PagedWalk paged) {
+  constexpr int DK = D / 64;
+  after_previous_kernel();
+  if ((int)blockIdx.x >= paged.header[paged::kTiles]) return;
+  const TileItem w = tiles[blockIdx.x];
+  const int nj0 = blockIdx.y * chunk, h = blockIdx.z;
+  if (nj0 > w.mi) return;
+  const int count = min(chunk, w.mi + 1 - nj0);
+  const int i0 = w.mi * kTile;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q0s = smem;                               // DK tiles [128 queries][64]
+  uint8_t* k0s = smem + DK * kRowTile;               // 2 stages x DK tiles [128 keys][64]
+  __shared__ uint64_t bar_q, bar_k[2], bar_mma[2], bar_read[2];
+  __shared__ uint32_t tmem_base_s;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&bar_q, 1);
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(&bar_k[u], 1);
+      mbar_init(&bar_mma[u], 1);
+      mbar_init(&bar_read[u], 4);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 0) tmem_alloc(&tmem_base_s, 256);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_base_s;
+
+  if (warp == 4) {
+    Waiter wait;
+    wait.begin(status);
+    auto await = [&](uint64_t* bar, uint32_t parity, int site) { wait.left = wait_call(smem_u32(bar), parity, site, wait.left); };
+    const PageBoxes boxes{paged.tables + (int64_t)w.row * paged.max_pages, paged.page_shift, paged.box_rows};
+    int page = boxes.page(nj0 * kTile, w.length, lane);
+    const uint32_t idesc = instr_desc_bf16(128, 128, false, false);
+    const uint32_t k_low = desc_low(smem_u32(k0s), 16), q_low = desc_low(smem_u32(q0s), 16);
+    auto load_k = [&](int it) {
+      const int j0 = (nj0 + it) * kTile, used = boxes.count(j0, w.length);
+      uint64_t* bar = &bar_k[it & 1];
+      if (elect_one()) mbar_expect_tx(bar, DK * used * paged.box_rows * 128);
+      __syncwarp();
+      if (lane < used)
+        for (int s = 0; s < DK; ++s)
+          tma_load_4d(k0s + ((it & 1) * DK + s) * kRowTile + lane * paged.box_rows * 128, &map_k, bar, s * 64, boxes.at(j0, lane), h, page);
+      __syncwarp();
+      page = boxes.page(j0 + kTile, w.length, lane);
+    };
+    if (elect_one()) {
+      mbar_expect_tx(&bar_q, DK * kRowTile);
+      for (int s = 0; s < DK; ++s) tma_load_4d(q0s + s * kRowTile, &map_q, &bar_q, s * 64, w.token + i0 - w.cached, h, 0);
+    }
+    __syncwarp();
+    load_k(0);
+    if (count > 1) load_k(1);
+    await(&bar_q, 0, 211);
+#pragma unroll 1
+    for (int it = 0; it < count; ++it) {
+      const int st = it & 1;
+      const uint32_t ph = (uint32_t)((it >> 1) & 1);
+      if (it >= 2) await(&bar_read[st], ph ^ 1u, 213);                   // the columns' last tile has been read
+      await(&bar_k[st], ph, 210);
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < 4 * DK; ++ks) {
+          const uint32_t off = (uint32_t)((ks >> 2) * kRowTile + (ks & 3) * 32) >> 4;
+          const uint32_t kl = k_low + (uint32_t)(st * DK * kRowTile >> 4) + off;
+          if (ks == 0) mma_ss_low<false>(tmem + st * 128, kl, q_low + off, idesc);
+          else mma_ss_low<true>(tmem + st * 128, kl, q_low + off, idesc);
+        }
+        mma_commit(&bar_mma[st]);
+      }
+      __syncwarp();
+      if (it >= 1 && it + 1 < count) {                                   // the other stage: its MMA has completed
+        await(&bar_mma[st ^ 1], (uint32_t)(((it - 1) >> 1) & 1), 214);
+        load_k(it + 1);
+      }
+    }
+    if (lane == 0) wait.end(status);
+    __syncwarp();
+  } else {
+    const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
+    const int lo = max(w.cached - i0, 0), hi = min(w.length - i0, kTile);  // the tile's queries that are the row's
+    float* dst = carry + ((int64_t)blockIdx.x * gridDim.z + h) * paged.key_stride;
+#pragma unroll 1
+    for (int it = 0; it < count; ++it) {
+      mbar_wait(&bar_mma[it & 1], (uint32_t)((it >> 1) & 1), status, 212);
+      tc_fence_after_sync();
+      const bool diag = nj0 + it == w.mi;
+      const bool masked = diag || lo > 0 || hi < kTile;
+      const int from = diag ? max(lo, tid + 1) : lo;                      // (key and query count from the same position)
+      float2 acc[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld32(lane_base + (it & 1) * 128 + c0, r);
+        tmem_ld_wait();
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c0 + e < from || c0 + e >= hi) r[e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          acc[(e >> 1) & 3] = __fadd2_rn(acc[(e >> 1) & 3], make_float2(fmaxf(__uint_as_float(r[e]), 0.f),
+                                                                        fmaxf(__uint_as_float(r[e + 1]), 0.f)));
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_read[it & 1]);
+      const float2 s2 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+      const int j = (nj0 + it) * kTile + tid;
+      if (j < w.length) dst[j] = (j < exempt) ? 0.f : (s2.x + s2.y) * scale;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 256);
+}
+
+// One thread per key and group of a row that has tiles: carry[tile][group][j] = what the key has received before the tile, in
+// place, and `selected` moved on.  A new key has received nothing before the step, whatever an earlier row left there.
+__global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t key_stride, const int* __restrict__ tile_start,
+                                                         const TileItem* __restrict__ tiles, int groups, float* selected,
+                                                         int64_t sel_stride) {
+  after_previous_kernel();
+  const int r = blockIdx.z, g = blockIdx.y;
+  const int t0 = tile_start[r], n = tile_start[r + 1] - t0;
+  if (n == 0) return;
+  const TileItem w = tiles[t0];                                 // the row's first tile
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  if (j >= w.length) return;
+  const int64_t pitch = groups * key_stride;
+  float* col = carry + ((int64_t)t0 * groups + g) * key_stride + j;
+  float* sel = selected + ((int64_t)r * groups + g) * sel_stride + j;
+  float run = j < w.cached ? *sel : 0.f;
+  int t = max(j / kTile - w.mi, 0);
+  for (; t + 8 <= n; t += 8) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = col[(t + u) * pitch];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      col[(t + u) * pitch] = run;
+      run += x[u];
+    }
+  }
+  for (; t < n; ++t) {
+    const float x = col[t * pitch];
+    col[t * pitch] = run;
+    run += x;
+  }
+  *sel = run;
+}
+
+template <typename... Args>
+int launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t s, Args... args) {
+  SA_CUDA_CHECK(allow_smem(kernel, smem));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  config.attrs = &attr;
+  config.numAttrs = overlap ? 1 : 0;
+  count_launch();
+  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+  return SA_OK;
+}
+
+template <int D>
+int tiles_impl(const Attention& a, cudaStream_t s) {
+  constexpr int DK = D / 64;
+  const paged::StepLayout l = paged::step_layout(a.rows, a.total, a.heads);
+  const paged::AttentionScratch w = paged::attention_scratch(a);
+  const int page = 1 << a.page_shift, box_rows = min(page, kTile);
+  const bool self = a.groups == a.heads;
+  CUtensorMap map_q, map_k, map_v;
+  int st = make_map_16bit(&map_q, a.q, D, a.total, a.heads, 1, a.q_stride[0], a.q_stride[1], 0, kTile);
+  if (st != SA_OK) return st;
+  st = make_pool_map(&map_k, a.k_pages, D, page, a.heads, a.num_pages, 64, box_rows, true);
+  if (st != SA_OK) return st;
+  st = make_pool_map(&map_v, a.v_pages, D, page, a.heads, a.num_pages, 64, box_rows, true);
+  if (st != SA_OK) return st;
+  WaitCtx status;
+  st = wait_ctx(&status);
+  if (st != SA_OK) return st;
+
+  unsigned int* const walk_tickets = reinterpret_cast<unsigned int*>(a.workspace + w.tickets);
+  // store: also clears the walks' tickets
+  const int n_walk = l.tiles_max * a.heads;
+  {
+    const TokenRows k{static_cast<const uint4*>(a.k), a.k_stride[0] / 8, a.k_stride[1] / 8};
+    const TokenRows v{static_cast<const uint4*>(a.v), a.v_stride[0] / 8, a.v_stride[1] / 8};
+    const int64_t units = (int64_t)a.total * a.heads * (D / 8);
+    const unsigned blocks = (unsigned)max((int64_t)1, min((units + 255) / 256, (int64_t)8 * kSms));
+    st = launch(store_kernel, dim3(blocks), 256, 0, true, s, k, v, static_cast<uint4*>(a.k_pages), static_cast<uint4*>(a.v_pages),
+                static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk);
+    if (st != SA_OK) return st;
+  }
+  PagedWalk walk{};
+  walk.header = a.work;
+  walk.items = reinterpret_cast<const TileItem*>(a.work + l.tile_items);
+  walk.tables = a.block_tables;
+  walk.max_pages = a.max_pages; walk.page_shift = a.page_shift; walk.box_rows = box_rows;
+  walk.key_stride = w.key_stride;
+  walk.tickets = walk_tickets;
+  walk.part = a.workspace + w.part;
+  walk.lse = a.workspace + w.lse;
+  const TileItem* tiles = reinterpret_cast<const TileItem*>(a.work + l.tiles);
+  float* carry = a.workspace + w.carry;
+  const float scale = 1.0f / sqrtf((float)D);
+  const int key_tiles = (a.max_length + kTile - 1) / kTile;
+  {
+    // key tiles per CTA: 8, or 32 where that still gives every SM several CTAs (the query tile and the set-up are paid per CTA)
+    const int chunk = (int64_t)l.tiles_max * key_tiles * a.groups >= 32 * 16 * kSms ? 32 : 8;
+    ProfileScope prof(SA_KERNEL_TC_COLSUM, s);
+    st = launch(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, true, s,
+                map_q, map_k, carry, a.exempt, scale, status, chunk, tiles, walk);
+    if (st != SA_OK) return st;
+  }
+  {
+    ProfileScope prof(SA_KERNEL_TC_SCAN, s);
+    st = launch(scan_pages_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, true, s, carry, w.key_stride,
+                (const int*)(a.work + l.tile_start), tiles, a.groups, a.selected, a.sel_stride);
+    if (st != SA_OK) return st;
+  }
+  // Two heads a CTA, or one: as over contiguous caches (sa_tc_fwd.cu), by the tiles that there are at least, since the plan's
+  // number is on the device.  Where there may be few, the plan may have cut their walks.
+  const int tiles_min = (a.total - (a.rows - 1) + kTile - 1) / kTile;
+  ProfileScope prof(SA_KERNEL_TC_FORWARD, s);
+  __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
+  const RowLayout y_rows{0, D, (int64_t)a.heads * D};
+  if constexpr (D == 64) {
+    if (!self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
+      return launch(forward_pair_kernel<false, true>, dim3((unsigned)l.tile_items_max * (a.heads / 2)), kThreads, PairSmem::total, true, s,
+                    map_q, map_k, map_v, map_q, map_k, (const float*)carry, (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale,
+                    status, y, y_rows, 0, (const uint8_t*)nullptr, walk);
+  }
+  const dim3 grid((unsigned)l.tile_items_max * a.heads);
+  auto wide = [&](auto kernel) {
+    return launch(kernel, grid, kWideThreads, WideSmem<D>::total + 1024, true, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
+                  (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
+                  SplitWalk{}, walk);
+  };
+  const bool whole = (int64_t)2 * tiles_min > paged::tile_wave(a.heads);
+  if (self) return whole ? wide(forward_wide_kernel<D, true, false, false, true>) : wide(forward_wide_kernel<D, true, false, true, true>);
+  return whole ? wide(forward_wide_kernel<D, false, false, false, true>) : wide(forward_wide_kernel<D, false, false, true, true>);
+}
+
+}  // namespace
+}  // namespace tc
+
+namespace paged {
+
+AttentionScratch attention_scratch(const Attention& a) {
+  const StepLayout l = step_layout(a.rows, a.total, a.heads);
+  AttentionScratch w{};
+  w.key_stride = ((int64_t)a.max_length + 127) / 128 * 128;
+  auto take = [&](size_t n) {
+    const size_t at = w.floats;
+    w.floats += (n + 63) / 64 * 64;
+    return at;
+  };
+  w.own_tickets = take((size_t)l.tickets_count);
+  w.partial = take((size_t)l.decode_items_max * a.heads * (a.head_dim + 2));
+  w.sel_new = take(a.groups < a.heads ? (size_t)a.rows * a.groups * w.key_stride : 0);
+  if (a.max_count > 1 && l.tiles_max > 0) {
+    w.carry = take((size_t)l.tiles_max * a.groups * w.key_stride);
+    const size_t cut = (size_t)tile_wave(a.heads) * a.heads * kTile;        // the plan cuts no more than a wave of walks
+    w.part = take(cut * a.head_dim);
+    w.lse = take(cut);
+    w.tickets = take((size_t)l.tiles_max * a.heads);
+  }
+  return w;
+}
+
+int tiles(const Attention& a, cudaStream_t s) {
+  return a.head_dim == 64 ? tc::tiles_impl<64>(a, s) : a.head_dim == 128 ? tc::tiles_impl<128>(a, s) : SA_ERR_UNSUPPORTED;
+}
+
+}  // namespace paged
+}  // namespace sa

@@ -148,6 +148,13 @@ __device__ __forceinline__ float load_ahead(const float* p) {
   return v;
 }
 
+// First in a kernel that is launched while the one before it still runs (programmatic stream serialization): the next one may be
+// launched, and everything that the kernels before have written is there.
+__device__ __forceinline__ void after_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- fences -------------------------------------------------------------------------------------------
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }

@@ -377,6 +377,185 @@ pybind11::tuple decode(const Tensor& kc, const Tensor& vc, const Tensor& selecte
   return pybind11::make_tuple(y, keep);
 }
 
+// ---- a paged cache, and beams ------------------------------------------------------------------------------------------------
+
+struct PageTables {                               // paged.begin_tables
+  Tensor block_tables, lengths, free_pages, free_count, page_refs;
+  int64_t page_size, heads;
+};
+
+sa_page_tables tables_of(const PageTables& t) {
+  TORCH_CHECK_VALUE(t.block_tables.dim() == 2 && t.lengths.dim() == 1 && t.free_pages.dim() == 1 && t.page_refs.dim() == 1 &&
+                        t.block_tables.size(0) == t.lengths.size(0) && t.free_pages.size(0) == t.page_refs.size(0) && t.free_count.numel() == 1,
+                    "page tables must be block_tables (rows, max_pages), lengths (rows,), free_pages and page_refs (num_pages,), free_count (1,)");
+  for (const Tensor* x : {&t.block_tables, &t.lengths, &t.free_pages, &t.free_count, &t.page_refs})
+    TORCH_CHECK_VALUE(x->is_cuda() && x->device() == t.block_tables.device() && x->scalar_type() == at::kInt && x->is_contiguous(),
+                      "page tables must be contiguous int32 CUDA tensors on one device");
+  TORCH_CHECK_VALUE(t.page_size == 16 || t.page_size == 32 || t.page_size == 64 || t.page_size == 128 || t.page_size == 256,
+                    "page_size must be one of (16, 32, 64, 128, 256); got ", t.page_size);
+  TORCH_CHECK_VALUE(t.lengths.size(0) >= 1 && t.lengths.size(0) <= 4096 && t.heads >= 1 && t.heads <= 256,
+                    "page tables have 1 to 4096 rows and 1 to 256 heads");
+  sa_page_tables p{};
+  p.struct_bytes = sizeof(sa_page_tables);
+  p.rows = (int32_t)t.block_tables.size(0);
+  p.max_pages = (int32_t)t.block_tables.size(1);
+  p.num_pages = (int32_t)t.free_pages.size(0);
+  p.page_size = (int32_t)t.page_size;
+  p.heads = (int32_t)t.heads;
+  p.block_tables = t.block_tables.data_ptr<int32_t>();
+  p.lengths = t.lengths.data_ptr<int32_t>();
+  p.free_pages = t.free_pages.data_ptr<int32_t>();
+  p.free_count = t.free_count.data_ptr<int32_t>();
+  p.page_refs = t.page_refs.data_ptr<int32_t>();
+  return p;
+}
+
+void check_int32(const Tensor& x, const PageTables& t, int64_t n, const char* what) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.device() == t.block_tables.device() && x.scalar_type() == at::kInt && x.is_contiguous() && x.numel() == n,
+                    what, " must be a contiguous int32 CUDA tensor of ", n, " numbers on the tables' device");
+}
+
+// (query_start, cached, slots, work, max_length, max_count, stream, capture): the step, its bounds, and where it was made
+pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t total, int64_t max_length, int64_t max_count) {
+  const sa_page_tables p = tables_of(t);
+  check_int32(counts, t, p.rows, "counts");
+  TORCH_CHECK_VALUE(total >= 0 && total <= (1 << 30), "total must be the number of the step's tokens; got ", total);
+  TORCH_CHECK_VALUE(max_length >= 1 && max_count >= 1, "max_length and max_count must be at least 1");
+  const c10::cuda::CUDAGuard guard(t.block_tables.device());
+  const int64_t capacity = (int64_t)p.max_pages * p.page_size;
+  max_length = std::min(max_length, capacity);
+  max_count = std::min({max_count, max_length, std::max<int64_t>(total, 1)});
+  const int64_t words = (int64_t)sa_page_step_words(p.rows, (int)total, p.heads);
+  const Tensor ints = at::empty({words + 2 * p.rows + 1}, t.lengths.options());
+  const Tensor slots = at::empty({total}, t.lengths.options().dtype(at::kLong));
+  const Tensor work = ints.narrow(0, 0, words), query_start = ints.narrow(0, words, p.rows + 1), cached = ints.narrow(0, words + p.rows + 1, p.rows);
+  void* const stream = stream_of(t.lengths);
+  check("sa_page_append", sa_page_append(&p, counts.data_ptr<int32_t>(), (int)total, (int)max_length, (int)max_count,
+                                         query_start.data_ptr<int32_t>(), cached.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
+                                         work.data_ptr<int32_t>(), stream));
+  return pybind11::make_tuple(query_start, cached, slots, work, max_length, max_count, reinterpret_cast<uint64_t>(stream),
+                              (uint64_t)sa_stream_capture(stream));
+}
+
+struct PageStep {                                  // paged.append_tokens
+  Tensor query_start, cached, slots, work;
+  int64_t max_length, max_count;
+  uint64_t stream, capture;
+};
+
+void check_pools(const PageTables& t, const sa_page_tables& p, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
+  TORCH_CHECK_VALUE(kc.dim() == 4 && kc.size(0) == p.num_pages && kc.size(1) == p.heads && kc.size(2) == p.page_size && vc.sizes() == kc.sizes(),
+                    "cache['k'] and cache['v'] must be (num_pages, H, page_size, D) as the tables have them; got ", kc.sizes(), " and ", vc.sizes());
+  TORCH_CHECK_VALUE(selected.dim() == 3 && selected.size(0) == p.rows && selected.size(2) == (int64_t)p.max_pages * p.page_size &&
+                        (selected.size(1) == 1 || selected.size(1) == p.heads),
+                    "cache['selected'] must be (rows, 1 or H, max_pages * page_size); got ", selected.sizes());
+  for (const Tensor* x : {&kc, &vc, &selected})
+    TORCH_CHECK_VALUE(x->is_cuda() && x->device() == t.block_tables.device() && x->is_contiguous() &&
+                          x->scalar_type() == (x == &selected ? at::kFloat : at::kBFloat16),
+                      "a paged cache is contiguous CUDA tensors on the tables' device: k and v bf16, `selected` fp32");
+  TORCH_CHECK_VALUE(kc.size(3) == 64 || kc.size(3) == 128, "head_dim must be 64 or 128 in a paged cache; got ", kc.size(3));
+}
+
+Tensor paged_attention(const PageTables& t, const PageStep& step, const Tensor& kc, const Tensor& vc, const Tensor& selected, const Tensor& q_in,
+                       const Tensor& k_in, const Tensor& v_in, int64_t exempt) {
+  const sa_page_tables p = tables_of(t);
+  check_pools(t, p, kc, vc, selected);
+  const int64_t total = step.slots.numel(), h = p.heads, d = kc.size(3);
+  check_int32(step.query_start, t, p.rows + 1, "the step's query_start");
+  check_int32(step.cached, t, p.rows, "the step's cached");
+  check_int32(step.work, t, (int64_t)sa_page_step_words(p.rows, (int)total, p.heads), "the step's plan");
+  TORCH_CHECK_VALUE(step.slots.is_cuda() && step.slots.device() == kc.device() && step.slots.scalar_type() == at::kLong && step.slots.is_contiguous(),
+                    "the step's slots must be a contiguous int64 CUDA tensor on the tables' device");
+  for (const Tensor* x : {&q_in, &k_in, &v_in}) {
+    TORCH_CHECK_VALUE(x->dim() == 3 && x->size(0) == total && x->size(1) == h && x->size(2) == d, "q, k, v must all be (", total, ", ", h, ", ", d,
+                      "): the step's tokens; got ", x->sizes());
+    TORCH_CHECK_VALUE(x->device() == kc.device() && code_of(*x) >= 0, "q, k, v must be float16, bfloat16 or float32 CUDA tensors on the cache's device");
+  }
+  const at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard guard(kc.device());
+  const Tensor y = at::empty({total, h, d}, kc.options());
+  if (total == 0) return y;
+  auto prepare = [&](const Tensor& x) {
+    const Tensor c = x.scalar_type() == at::kBFloat16 ? x : x.to(at::kBFloat16);
+    const bool ok = c.stride(2) == 1 && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 && c.stride(0) % 8 == 0 && c.stride(1) % 8 == 0;
+    return ok ? c : c.clone(at::MemoryFormat::Contiguous);
+  };
+  const Tensor q = prepare(q_in), k = prepare(k_in), v = prepare(v_in);
+  void* const stream = stream_of(kc);
+  sa_paged_attention a{};
+  a.struct_bytes = sizeof(sa_paged_attention);
+  a.groups = (int32_t)selected.size(1); a.head_dim = (int32_t)d; a.exempt = (int32_t)exempt; a.total = (int32_t)total;
+  a.max_length = (int32_t)step.max_length; a.max_count = (int32_t)step.max_count;
+  // calls on the stream that made the plan, outside any capture or in the same one, run one after the other
+  a.plan_tickets = step.stream == reinterpret_cast<uint64_t>(stream) && step.capture == (uint64_t)sa_stream_capture(stream);
+  a.tables = &p;
+  a.query_start = step.query_start.data_ptr<int32_t>(); a.cached = step.cached.data_ptr<int32_t>();
+  a.slots = step.slots.data_ptr<int64_t>(); a.work = step.work.data_ptr<int32_t>();
+  a.k_pages = kc.data_ptr(); a.v_pages = vc.data_ptr(); a.selected = selected.data_ptr<float>();
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    a.q_stride[i] = q.stride(i);
+    a.k_stride[i] = k.stride(i);
+    a.v_stride[i] = v.stride(i);
+  }
+  a.y = y.data_ptr();
+  a.workspace_bytes = sa_paged_workspace_bytes(&a);
+  const Tensor workspace = bytes_on(kc, a.workspace_bytes);
+  a.workspace = workspace.data_ptr();
+  a.stream = stream;
+  check("sa_paged_run", sa_paged_run(&a));
+  return y;
+}
+
+pybind11::tuple reorder_rows(const PageTables& t, const Tensor& parents) {
+  const sa_page_tables p = tables_of(t);
+  check_int32(parents, t, p.rows, "parents");
+  const c10::cuda::CUDAGuard guard(t.block_tables.device());
+  const Tensor copies = at::empty({p.rows, 2}, t.lengths.options());
+  const Tensor work = at::empty({(int64_t)sa_page_reorder_words(p.rows, p.max_pages, p.num_pages)}, t.lengths.options());
+  check("sa_page_reorder", sa_page_reorder(&p, parents.data_ptr<int32_t>(), copies.data_ptr<int32_t>(), work.data_ptr<int32_t>(), stream_of(t.lengths)));
+  return pybind11::make_tuple(copies, work);
+}
+
+void move_rows(const PageTables& t, const Tensor& copies, const Tensor& work, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
+  const sa_page_tables p = tables_of(t);
+  check_pools(t, p, kc, vc, selected);
+  check_int32(copies, t, 2 * (int64_t)p.rows, "the moves' copies");
+  check_int32(work, t, (int64_t)sa_page_reorder_words(p.rows, p.max_pages, p.num_pages), "the moves' plan");
+  const c10::cuda::CUDAGuard guard(kc.device());
+  check("sa_page_move", sa_page_move(&p, copies.data_ptr<int32_t>(), work.data_ptr<int32_t>(), (int)selected.size(1), (int)kc.size(3), kc.data_ptr(),
+                                     vc.data_ptr(), selected.data_ptr<float>(), stream_of(kc)));
+}
+
+pybind11::tuple beam_select(const Tensor& logits_in, const Tensor& scores_in, int64_t width) {
+  TORCH_CHECK_VALUE(logits_in.dim() == 3 && scores_in.dim() == 2 && scores_in.size(0) == logits_in.size(0) && scores_in.size(1) == logits_in.size(1),
+                    "logits must be (groups, beams, vocab) and scores (groups, beams); got ", logits_in.sizes(), " and ", scores_in.sizes());
+  const int64_t g = logits_in.size(0), k = logits_in.size(1), vocab = logits_in.size(2);
+  TORCH_CHECK_VALUE(logits_in.is_cuda() && scores_in.device() == logits_in.device() && code_of(logits_in) >= 0,
+                    "logits must be a float16, bfloat16 or float32 CUDA tensor with scores on its device");
+  TORCH_CHECK_VALUE(g >= 1 && k >= 1 && k <= 256 && vocab >= 1 && vocab < (1ll << 31) && g * k <= (1 << 20), "1 to 256 beams of a non-empty vocabulary");
+  TORCH_CHECK_VALUE(width >= 1 && width <= 32 && width <= k * vocab, "width must be 1 to 32, and no more than beams * vocab; got ", width);
+  const at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard guard(logits_in.device());
+  const Tensor logits = logits_in.stride(2) == 1 || vocab == 1 ? logits_in : logits_in.contiguous();
+  const Tensor scores = (scores_in.scalar_type() == at::kFloat ? scores_in : scores_in.to(at::kFloat)).contiguous();
+  const Tensor out = at::empty({g, width}, scores.options()), rows = at::empty({g, width}, scores.options().dtype(at::kInt)),
+               tokens = at::empty({g, width}, scores.options().dtype(at::kLong));
+  sa_beam a{};
+  a.struct_bytes = sizeof(sa_beam);
+  a.dtype = code_of(logits); a.groups = (int32_t)g; a.beams = (int32_t)k; a.vocab = (int32_t)vocab; a.width = (int32_t)width;
+  a.logits = logits.data_ptr();
+  a.group_stride = logits.stride(0); a.beam_stride = logits.stride(1);
+  a.scores = scores.data_ptr<float>();
+  a.out_scores = out.data_ptr<float>(); a.out_rows = rows.data_ptr<int32_t>(); a.out_tokens = tokens.data_ptr<int64_t>();
+  a.workspace_bytes = sa_beam_workspace_bytes(a.dtype, a.groups, a.beams, a.vocab, a.width);
+  const Tensor workspace = bytes_on(logits, a.workspace_bytes);
+  a.workspace = workspace.data_ptr();
+  a.stream = stream_of(logits);
+  check("sa_beam_select", sa_beam_select(&a));
+  return pybind11::make_tuple(out, rows, tokens);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -386,4 +565,13 @@ PYBIND11_MODULE(_native, m) {
   m.def("prefill_rows", &prefill_rows, nogil());
   m.def("store_rows", &store_rows, nogil());
   m.def("decode", &decode);
+  pybind11::class_<PageTables>(m, "PageTables")
+      .def(pybind11::init<Tensor, Tensor, Tensor, Tensor, Tensor, int64_t, int64_t>());
+  pybind11::class_<PageStep>(m, "PageStep")
+      .def(pybind11::init<Tensor, Tensor, Tensor, Tensor, int64_t, int64_t, uint64_t, uint64_t>());
+  m.def("append_tokens", &append_tokens);
+  m.def("paged_attention", &paged_attention, nogil());
+  m.def("reorder_rows", &reorder_rows);
+  m.def("move_rows", &move_rows, nogil());
+  m.def("beam_select", &beam_select);
 }

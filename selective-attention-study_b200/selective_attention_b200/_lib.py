@@ -25,7 +25,9 @@ EXPORTS = ("sa_abi_version", "sa_status_string", "sa_last_cuda_error", "sa_engin
            "sa_profile_collect", "sa_static_scratch_floats", "sa_forward_static_scratch", "sa_forward_selector",
            "sa_backward_selector", "sa_forward_fused", "sa_backward_fused", "sa_prefill_extend", "sa_selection_carry", "sa_launch_count", "sa_selftest_wait_timeout", "sa_selftest_wait_tries",
            "sa_tile_table_bytes", "sa_forward_live_tiles", "sa_backward_live_tiles", "sa_prefill_extend_live_tiles", "sa_decode_step_live_keys",
-           "sa_decode_run", "sa_prefill_scratch_bytes", "sa_prefill_rows", "sa_cache_store")
+           "sa_decode_run", "sa_prefill_scratch_bytes", "sa_prefill_rows", "sa_cache_store", "sa_page_step_words", "sa_page_append",
+           "sa_paged_workspace_bytes", "sa_paged_run", "sa_page_reorder_words", "sa_page_reorder", "sa_page_move", "sa_stream_capture",
+           "sa_beam_workspace_bytes", "sa_beam_select")
 
 
 class Problem(ctypes.Structure):
@@ -45,6 +47,30 @@ class Tensor(ctypes.Structure):
     """sa_tensor: rows of head_dim contiguous elements at batch / head / token strides."""
     _fields_ = [("ptr", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
                 ("stride", ctypes.c_int64 * 3)]
+
+
+class PageTables(ctypes.Structure):
+    """sa_page_tables"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "rows", "max_pages", "num_pages", "page_size", "heads")] + \
+               [(n, ctypes.c_void_p) for n in ("block_tables", "lengths", "free_pages", "free_count", "page_refs")]
+
+
+class PagedAttention(ctypes.Structure):
+    """sa_paged_attention"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "groups", "head_dim", "exempt", "total", "max_length", "max_count",
+                                              "plan_tickets")] + \
+               [("tables", ctypes.POINTER(PageTables))] + \
+               [(n, ctypes.c_void_p) for n in ("query_start", "cached", "slots", "work", "k_pages", "v_pages", "selected", "q", "k", "v")] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [("y", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
+
+
+class Beam(ctypes.Structure):
+    """sa_beam"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "dtype", "groups", "beams", "vocab", "width")] + \
+               [("logits", ctypes.c_void_p), ("group_stride", ctypes.c_int64), ("beam_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("scores", "out_scores", "out_rows", "out_tokens", "workspace")] + \
+               [("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
 
 
 class LibraryError(RuntimeError):
@@ -143,6 +169,27 @@ def load() -> ctypes.CDLL:
     lib.sa_prefill_rows.argtypes = [pp, i32, vp, vp, vp, f32p, ctypes.c_int64, tp, f32p, f32p, vp, sz, vp, sz, vp]
     lib.sa_cache_store.restype = i32
     lib.sa_cache_store.argtypes = [i32] * 9 + [tp, tp, vp, vp, f32p, vp]
+    i64, tabs = ctypes.c_int64, ctypes.POINTER(PageTables)
+    lib.sa_page_step_words.restype = sz
+    lib.sa_page_step_words.argtypes = [i32] * 3
+    lib.sa_page_append.restype = i32
+    lib.sa_page_append.argtypes = [tabs, vp, i32, i32, i32, vp, vp, vp, vp, vp]
+    lib.sa_paged_workspace_bytes.restype = sz
+    lib.sa_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttention)]
+    lib.sa_paged_run.restype = i32
+    lib.sa_paged_run.argtypes = [ctypes.POINTER(PagedAttention)]
+    lib.sa_page_reorder_words.restype = sz
+    lib.sa_page_reorder_words.argtypes = [i32] * 3
+    lib.sa_page_reorder.restype = i32
+    lib.sa_page_reorder.argtypes = [tabs, vp, vp, vp, vp]
+    lib.sa_page_move.restype = i32
+    lib.sa_page_move.argtypes = [tabs, vp, vp, i32, i32, vp, vp, vp, vp]
+    lib.sa_stream_capture.restype = ctypes.c_ulonglong
+    lib.sa_stream_capture.argtypes = [vp]
+    lib.sa_beam_workspace_bytes.restype = sz
+    lib.sa_beam_workspace_bytes.argtypes = [i32] * 5
+    lib.sa_beam_select.restype = i32
+    lib.sa_beam_select.argtypes = [ctypes.POINTER(Beam)]
     lib.sa_device_status.restype = i32
     lib.sa_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint), i32]
     lib.sa_selftest_tcgen05.restype = i32

@@ -7,6 +7,7 @@ the reference's layer can call it after ``_split_heads`` and before ``_merge_hea
     _attend      -> attend(q, k, v, want_total)            (reference :76-98)
     begin_cache  -> begin_cache(q, k, v, capacity)         (reference :105-113 with model.py:76-83)
     (none)       -> extend_cache(q, k, v, cache)           a further prompt chunk; the reference prefills once
+    (none)       -> begin_pages, attend_pages              many requests of different lengths over a paged cache (paged.py)
     step_cache   -> step_cache(q1, k1, v1, cache)          (reference :115-130 with model.py:86-93)
 
 Variants as in the reference (:16-22): "selective" (head 0 selects, <BOS> exempt), "selective_x16"
@@ -17,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from . import kernels
+from . import kernels, paged
 
 VARIANTS = {"selective": (1, False), "selective_x16": (16, False), "selective_perhead": (1, True)}
 MIXER_TYPES = tuple(VARIANTS)
@@ -103,6 +104,20 @@ class SelectiveAttentionSlot:
         part of the cache whose probabilities are all exactly zero for these queries is not read (same rows)."""
         out_dtype = torch.bfloat16 if v.dtype == torch.bfloat16 else torch.float32
         y = kernels._extend(cache, q, k, v, self.exempt, skip_dead_tiles, out_dtype)
+        return y if y.dtype == v.dtype else y.to(v.dtype)
+
+    def begin_pages(self, tables: dict, head_dim: int):
+        """The layer's part of a paged cache over ``paged.begin_tables``."""
+        if tables["heads"] != self.n_heads:
+            raise ValueError(f"the tables are for {tables['heads']} heads, the layer has {self.n_heads}")
+        return paged.begin_pages(tables, head_dim, per_head=self.groups > 1)
+
+    def attend_pages(self, q, k, v, cache: dict, tables: dict, step: dict):
+        """The new tokens of a step (``paged.append_tokens``), (total, H, D), row after row: prompts, chunks of them and single
+        tokens of many requests at once.  (total, H, D) outputs in v's dtype; the pages and histories move on."""
+        if cache["selected"].shape[1] != self.groups:
+            raise ValueError(f"the cache has {cache['selected'].shape[1]} histories a row, the layer {self.groups} selectors")
+        y = paged.paged_attention(cache, tables, step, q, k, v, exempt=self.exempt)
         return y if y.dtype == v.dtype else y.to(v.dtype)
 
     def step_cache(self, q1, k1, v1, cache: dict):
