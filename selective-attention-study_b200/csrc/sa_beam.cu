@@ -3,15 +3,16 @@
 //   score[k][v] = scores[k] + logits[k][v] - log sum_u exp(logits[k][u]);   the WIDTH largest over (k, v) of a group, in order,
 //   equal ones by the lowest k V + v.
 //
-// Two launches.  candidates_kernel reads the logits once: a CTA keeps a chunk of one beam's vocabulary in registers, and leaves
-// the chunk's maximum, its sum of exponentials and its WIDTH largest logits.  choose_kernel (a CTA a group) makes the beams'
-// log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
+// Two launches.  candidates_kernel: a CTA takes a run of one beam's vocabulary and leaves the run's maximum, its sum of exponentials
+// and its WIDTH largest logits.  The run is read twice, for the sum and for the candidates, the second time from L2 (kept in
+// registers, runs are short: 8,192 logits a CTA, 1,792 CTAs for 256 beams of 50,304, took 43 us).  choose_kernel (a CTA a group) makes the
+// beams' log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
 // Bound by memory where there are many beams, else by the latency of the two launches.
 //
-// The largest of a set, without sorting it: every thread's own maximum is ranked among those of the CTA; the WIDTH-th of them
-// bounds the WIDTH-th of the set from below, and the few elements that reach it are ranked among themselves.  Where more than
-// kList reach it (equal or masked logits) they are taken one by one.
+// The largest of a set, without sorting it: each of the eight warps gives the ceil(WIDTH / 8)-th largest of its lanes' own maxima;
+// WIDTH elements at least reach the least of the eight, and not many more do (about 25 for 8 of 8,192 random ones).  Those are
+// ranked among themselves.  Where more than kList reach it (equal or masked logits) they are taken one by one.
 #include "sa_common.cuh"
 #include "sa_beam.cuh"
 #include "sa_tc_ptx.cuh"
@@ -23,82 +24,84 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kList = 256;
 
-template <typename V>
+template <typename V, typename I>
 struct Entry {
   V value;
-  long long index;           // below 0: none
+  I index;                   // below 0: none
 };
 // a comes before b
-template <typename V>
-__device__ __forceinline__ bool before(const V a, const long long ia, const V b, const long long ib) {
-  return a > b || (a == b && ia < ib);
+template <typename V, typename I>
+__device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& b) {
+  return a.value > b.value || (a.value == b.value && a.index < b.index);
 }
 
-template <typename V>
+template <typename V, typename I>
 struct Shared {
-  V top[kThreads];
-  Entry<V> list[kList];
-  V threshold;
+  V bound[kThreads / 32];
+  Entry<V, I> list[kList];
   int count;
-  Entry<V> warp_best[kThreads / 32];
+  Entry<V, I> warp_best[kThreads / 32];
 };
 
-// Calls emit(rank, value, index) for the `width` first of the CTA's elements.  each(f) calls f(value, index) for every element
-// of the calling thread (no value a NaN); the same ones each time.  All threads call this; emit is called by any.
-template <typename V, typename Each, typename Emit>
-__device__ __forceinline__ void largest(Shared<V>& sh, int width, const Each& each, const Emit& emit) {
-  const int tid = threadIdx.x;
+// Calls emit(rank, value, index) for the `width` first of the CTA's elements.  `mine` is the largest value of the calling thread's
+// elements (-inf: none); reach(bound, f) calls f(value, index) for those of them that are not below `bound` (no value a NaN).
+// All threads call this; emit is called by any.
+template <typename V, typename I, typename Reach, typename Emit>
+__device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, const Reach& reach, const Emit& emit) {
+  const int tid = threadIdx.x, lane = tid & 31;
   constexpr V kNone = -INFINITY;
-  V mine = kNone;
-  bool any = false;
-  each([&](V x, long long) {
-    mine = any ? (x > mine ? x : mine) : x;
-    any = true;
-  });
-  sh.top[tid] = mine;                                       // a thread without elements: -inf bounds as well
+  V top = kNone;
+  for (int left = (width + kThreads / 32 - 1) / (kThreads / 32); left > 0; --left) {
+    top = mine;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+      const V o = __shfl_xor_sync(0xffffffffu, top, s);
+      top = o > top ? o : top;
+    }
+    const unsigned at = __ballot_sync(0xffffffffu, mine == top);
+    if (lane == __ffs(at) - 1) mine = kNone;                // one of them is done with
+  }
+  if (lane == 0) sh.bound[tid >> 5] = top;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  int rank = 0;
-  for (int u = 0; u < kThreads; ++u) rank += before(sh.top[u], (long long)u, mine, (long long)tid) ? 1 : 0;
-  if (rank == width - 1) sh.threshold = mine;
-  __syncthreads();
-  const V bound = sh.threshold;
-  each([&](V x, long long i) {
-    if (x >= bound) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kList) sh.list[at] = Entry<V>{x, i};
-    }
+  V bound = sh.bound[0];
+#pragma unroll
+  for (int u = 1; u < kThreads / 32; ++u) bound = sh.bound[u] < bound ? sh.bound[u] : bound;
+  reach(bound, [&](V x, I i) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kList) sh.list[at] = Entry<V, I>{x, i};
   });
   __syncthreads();
   const int n = sh.count;
   if (n <= kList) {
     if (tid < n) {
-      const Entry<V> e = sh.list[tid];
+      const Entry<V, I> e = sh.list[tid];
       int at = 0;
-      for (int u = 0; u < n; ++u) at += before(sh.list[u].value, sh.list[u].index, e.value, e.index) ? 1 : 0;
+#pragma unroll 4
+      for (int u = 0; u < n; ++u) at += before(sh.list[u], e) ? 1 : 0;
       if (at < width) emit(at, e.value, e.index);
     }
-    for (int u = n + tid; u < width; u += kThreads) emit(u, kNone, -1LL);     // fewer elements than that
+    for (int u = n + tid; u < width; u += kThreads) emit(u, kNone, (I)-1);     // fewer elements than that
     return;
   }
-  Entry<V> last{INFINITY, -1};                               // one by one
+  Entry<V, I> last{INFINITY, -1};                            // one by one
   for (int w = 0; w < width; ++w) {
-    Entry<V> best{kNone, -1};
-    each([&](V x, long long i) {
-      const bool left = w == 0 || before(last.value, last.index, x, i);
-      if (left && (best.index < 0 || before(x, i, best.value, best.index))) best = Entry<V>{x, i};
-    });
-    auto better = [&](const Entry<V>& o) {
-      if (o.index >= 0 && (best.index < 0 || before(o.value, o.index, best.value, best.index))) best = o;
+    Entry<V, I> best{kNone, -1};
+    auto better = [&](const Entry<V, I>& o) {
+      if (o.index >= 0 && (best.index < 0 || before(o, best))) best = o;
     };
+    reach(bound, [&](V x, I i) {
+      const Entry<V, I> e{x, i};
+      if (w == 0 || before(last, e)) better(e);
+    });
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
-      Entry<V> o;
+      Entry<V, I> o;
       o.value = __shfl_xor_sync(0xffffffffu, best.value, s);
       o.index = __shfl_xor_sync(0xffffffffu, best.index, s);
       better(o);
     }
-    if ((tid & 31) == 0) sh.warp_best[tid >> 5] = best;
+    if (lane == 0) sh.warp_best[tid >> 5] = best;
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < kThreads / 32; ++u) better(sh.warp_best[u]);
@@ -108,53 +111,109 @@ __device__ __forceinline__ void largest(Shared<V>& sh, int width, const Each& ea
   }
 }
 
+// Two logits of a 32-bit word, or one.
+template <typename T> struct Word;
+template <> struct Word<float> {
+  static constexpr int kPer = 1;
+  static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t none() { return 0xff800000u; }
+};
+template <> struct Word<__nv_bfloat16> {
+  static constexpr int kPer = 2;
+  static __device__ __forceinline__ float at(uint32_t w, int e) { return __uint_as_float(e ? w & 0xffff0000u : w << 16); }
+  static __device__ __forceinline__ uint32_t none() { return 0xff80u; }
+};
+template <> struct Word<__half> {
+  static constexpr int kPer = 2;
+  static __device__ __forceinline__ float at(uint32_t w, int e) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return e ? __high2float(h) : __low2float(h);
+  }
+  static __device__ __forceinline__ uint32_t none() { return 0xfc00u; }
+};
+
 // Elements are taken in units of 16 bytes from a 16-byte boundary on: a row that begins elsewhere has `lead` elements fewer in
-// its first unit.  Ends of a row are read element by element.
-template <typename T, int UNITS>
-__global__ void __launch_bounds__(kThreads) candidates_kernel(const T* __restrict__ logits, int64_t group_stride, int64_t beam_stride,
-                                                              int beams, int vocab, int width, int chunks, float2* __restrict__ sums,
-                                                              float* __restrict__ values, int* __restrict__ tokens) {
+// its first unit.  Units that stick out of the row are read element by element.
+constexpr int kAhead = 4;            // units in flight a thread: 64 KB an SM with four CTAs
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __restrict__ logits, int64_t group_stride, int64_t beam_stride,
+                                                                 int beams, int vocab, int width, int chunks, int units,
+                                                                 float2* __restrict__ sums, float* __restrict__ values,
+                                                                 int* __restrict__ tokens) {
+  using W = Word<T>;
   constexpr int kPer = 16 / (int)sizeof(T);
-  __shared__ Shared<float> sh;
+  asm volatile("griddepcontrol.launch_dependents;");
+  __shared__ Shared<float, int> sh;
   __shared__ float red[2][kThreads / 32];
   const int n = blockIdx.x / chunks, chunk = blockIdx.x - n * chunks;      // n: beam over all groups
   const int g = n / beams;
   const T* row = logits + g * group_stride + (int64_t)(n - g * beams) * beam_stride;
   const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int tid = threadIdx.x;
-  float x[UNITS * kPer];
-  int first[UNITS];
+  // this CTA's units: [unit0, unit1) of the row's
+  const int total = (int)(((int64_t)vocab + lead + kPer - 1) / kPer);
+  const int unit0 = chunk * units, unit1 = min(unit0 + units, total);
+  auto load = [&](int unit) {
+    const int64_t v = (int64_t)unit * kPer - lead;
+    if (unit < unit1 && v >= 0 && v + kPer <= vocab) return *reinterpret_cast<const uint4*>(row + v);
+    uint32_t x[4];
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    const int64_t v64 = ((int64_t)chunk * UNITS + u) * kThreads * kPer + (int64_t)tid * kPer - lead;
-    const int v = (int)min(v64, (int64_t)vocab);
-    first[u] = v;
-    if (v >= 0 && v64 + kPer <= vocab) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(row + v);
-      const T* e = reinterpret_cast<const T*>(&raw);
+    for (int i = 0; i < 4; ++i) {
+      x[i] = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[u * kPer + i] = to_float<T>(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) x[u * kPer + i] = v + i >= 0 && v64 + i < vocab ? to_float<T>(row[v + i]) : -INFINITY;
+      for (int e = 0; e < W::kPer; ++e) {
+        const int64_t at = v + i * W::kPer + e;
+        uint32_t one = W::none();
+        if (unit < unit1 && at >= 0 && at < vocab) {
+          if constexpr (sizeof(T) == 4) one = __float_as_uint(row[at]);
+          else one = *reinterpret_cast<const uint16_t*>(row + at);
+        }
+        x[i] |= one << (16 * e);
+      }
     }
-  }
-  // the chunk's maximum (NaNs aside) and its sum of exponentials (with them)
-  float top = -INFINITY;
+    return make_uint4(x[0], x[1], x[2], x[3]);
+  };
+  // The run's maximum (NaNs aside) and its sum of exponentials (with them), by thread with a maximum of its own.
+  // +inf: inf - inf, a NaN as a NaN among the logits: the beam has no finite sum.
+  float mine = -INFINITY, sum = 0.f;
+  for (int base = unit0; base < unit1; base += kThreads * kAhead) {
+    uint4 raw[kAhead];
 #pragma unroll
-  for (int i = 0; i < UNITS * kPer; ++i) top = fmaxf(top, x[i]);
+    for (int u = 0; u < kAhead; ++u) raw[u] = load(base + u * kThreads + tid);
+    float x[kAhead][kPer], top = mine;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        x[u][i] = W::at(w[i / W::kPer], i % W::kPer);
+        top = fmaxf(top, x[u][i]);
+      }
+    }
+    const float from = top == -INFINITY ? 0.f : top;
+    if (top > mine) sum *= tc::ex2((mine - from) * kLog2e);
+    mine = top;
+    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    const float2 shift = make_float2(-from, -from), scale = make_float2(kLog2e, kLog2e);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[u][i], x[u][i + 1]), shift), scale);
+        part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], make_float2(tc::ex2(d.x), tc::ex2(d.y)));
+      }
+    const float2 both = __fadd2_rn(part[0], part[1]);
+    sum += both.x + both.y;
+  }
+  float top = mine;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
   if ((tid & 31) == 0) red[0][tid >> 5] = top;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kThreads / 32; ++u) top = fmaxf(top, red[0][u]);
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < UNITS * kPer; ++i) {
-    sum += x[i] == -INFINITY ? 0.f : exp2f((x[i] - top) * kLog2e);         // +inf: inf - inf, the beam has no finite sum
-    if (isnan(x[i])) x[i] = -INFINITY;
-  }
+  if (top != -INFINITY) sum *= tc::ex2((mine - top) * kLog2e);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   if ((tid & 31) == 0) red[1][tid >> 5] = sum;
@@ -163,18 +222,33 @@ __global__ void __launch_bounds__(kThreads) candidates_kernel(const T* __restric
     for (int u = 1; u < kThreads / 32; ++u) sum += red[1][u];
     sums[blockIdx.x] = make_float2(top, sum);
   }
-  auto each = [&](auto f) {
+  auto reach = [&](float bound, auto f) {
+    for (int base = unit0; base < unit1; base += kThreads * kAhead) {
+      uint4 raw[kAhead];
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u)
+      for (int u = 0; u < kAhead; ++u) raw[u] = load(base + u * kThreads + tid);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (first[u] + i >= 0 && first[u] + i < vocab) f(x[u * kPer + i], (long long)(first[u] + i));
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) most = fmaxf(most, W::at(w[i / W::kPer], i % W::kPer));
+        if (most < bound) continue;
+#pragma unroll 1
+        for (int i = 0; i < kPer; ++i) {
+          const int64_t at = ((int64_t)base + u * kThreads + tid) * kPer - lead + i;
+          if (base + u * kThreads + tid >= unit1 || at < 0 || at >= vocab) continue;
+          const float v = fmaxf(to_float<T>(row[at]), -INFINITY);          // a NaN is never chosen
+          if (v >= bound) f(v, (int)at);
+        }
+      }
+    }
   };
   float* out_v = values + (int64_t)blockIdx.x * width;
   int* out_t = tokens + (int64_t)blockIdx.x * width;
-  largest(sh, width, each, [&](int at, float v, long long i) {
+  largest(sh, width, mine, reach, [&](int at, float v, int i) {
     out_v[at] = v;
-    out_t[at] = (int)i;
+    out_t[at] = i;
   });
 }
 
@@ -183,9 +257,20 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
                                                           const int* __restrict__ tokens, float* __restrict__ out_scores,
                                                           int* __restrict__ out_rows, long long* __restrict__ out_tokens) {
   tc::after_previous_kernel();
-  __shared__ Shared<double> sh;
+  __shared__ Shared<double, long long> sh;
   __shared__ double base[kMaxBeams];                         // score - log-sum-exp of a beam; NaN: all of its scores are -inf
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  const int per_beam = chunks * width, n = beams * per_beam;
+  const int64_t first = (int64_t)g * n;
+  constexpr int kKept = 4;                                   // candidates of a thread that are on their way meanwhile
+  float kept_v[kKept];
+  int kept_t[kKept];
+#pragma unroll
+  for (int u = 0; u < kKept; ++u) {
+    const int i = tid + u * kThreads;
+    kept_v[u] = i < n ? values[first + i] : 0.f;
+    kept_t[u] = i < n ? tokens[first + i] : -1;
+  }
   for (int k = tid >> 5; k < beams; k += kThreads / 32) {
     const float2* part = sums + ((int64_t)g * beams + k) * chunks;
     float top = -INFINITY;
@@ -195,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
     double sum = 0.0;
     for (int c = lane; c < chunks; c += 32) {
       const float2 p = part[c];
-      if (p.y != 0.f) sum += (double)p.y * exp((double)p.x - (double)top);      // 0: nothing but -inf; a NaN stays
+      if (p.y != 0.f) sum += (double)p.y * exp2f((p.x - top) * kLog2e);         // 0: nothing but -inf; a NaN stays
     }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -205,77 +290,68 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
     }
   }
   __syncthreads();
-  const int per_beam = chunks * width;
-  const int64_t first = (int64_t)g * beams * per_beam;
-  auto each = [&](auto f) {
-    for (int i = tid; i < beams * per_beam; i += kThreads) {
-      const int k = i / per_beam;
-      if (isnan(base[k])) {                                   // equal ones: the lowest tokens stand for all
-        const int v = i - k * per_beam;
-        if (v < width && v < vocab) f(-(double)INFINITY, (long long)k * vocab + v);
-        continue;
-      }
-      const int v = tokens[first + i];
-      if (v >= 0) f(base[k] + (double)values[first + i], (long long)k * vocab + v);
+  auto one = [&](int i, float value, int token, auto f) {    // f(score, place): beam in the upper half of the place, token in the lower
+    const int k = i / per_beam;
+    if (isnan(base[k])) {                                     // equal ones: the lowest tokens stand for all
+      const int v = i - k * per_beam;
+      if (v < width && v < vocab) f(-(double)INFINITY, ((long long)k << 32) | v);
+    } else if (token >= 0) {
+      f(base[k] + (double)value, ((long long)k << 32) | token);
     }
   };
-  largest(sh, width, each, [&](int at, double v, long long i) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+      if (tid + u * kThreads < n) one(tid + u * kThreads, kept_v[u], kept_t[u], f);
+    for (int i = tid + kKept * kThreads; i < n; i += kThreads) one(i, values[first + i], tokens[first + i], f);
+  };
+  double mine = -INFINITY;
+  each([&](double x, long long) { mine = x > mine ? x : mine; });
+  auto reach = [&](double bound, auto f) {
+    each([&](double x, long long i) {
+      if (x >= bound) f(x, i);
+    });
+  };
+  largest(sh, width, mine, reach, [&](int at, double v, long long i) {
     const int64_t o = (int64_t)g * width + at;
-    const int k = (int)(i / vocab);
     out_scores[o] = (float)v;
-    out_rows[o] = g * beams + k;
-    out_tokens[o] = i - (long long)k * vocab;
+    out_rows[o] = g * beams + (int)(i >> 32);
+    out_tokens[o] = i & 0xffffffffLL;
   });
 }
 
-template <typename T>
-int units_of(int rows, int vocab) {
-  // 8,192 logits a CTA where that still gives every SM several, else 2,048 (of 32 bits half as many)
-  constexpr int kPer = 16 / (int)sizeof(T);
-  const int64_t large = (int64_t)rows * ((vocab + 4 * kThreads * kPer - 1) / (4 * kThreads * kPer));
-  return large >= 4 * kSms ? 4 : 1;
-}
-int units_for(int dtype, int rows, int vocab) {
-  return dtype == SA_F32 ? units_of<float>(rows, vocab) : units_of<__half>(rows, vocab);
-}
-int chunks_for(int dtype, int rows, int vocab) {
-  const int per = dtype == SA_F32 ? 4 : 8, chunk = units_for(dtype, rows, vocab) * kThreads * per;
-  return (int)(((int64_t)vocab + per - 1 + chunk - 1) / chunk);             // a row may begin up to per - 1 elements into a unit
+// Runs of a beam's vocabulary, a CTA each: as many as make one wave of four CTAs an SM, none shorter than a unit a thread.
+struct Runs { int chunks, units; };
+Runs runs_of(int dtype, int rows, int vocab) {
+  const int per = dtype == SA_F32 ? 4 : 8;
+  const int total = (int)(((int64_t)vocab + per - 1 + per - 1) / per);      // a row may begin up to per - 1 elements into a unit
+  const int most = (total + kThreads - 1) / kThreads, wave = max(1, 4 * kSms / rows);
+  const int chunks = min(most, wave);
+  const int units = (total + chunks - 1) / chunks;
+  return Runs{(total + units - 1) / units, units};
 }
 
 }  // namespace
 
 size_t workspace_bytes(int dtype, int groups, int beams, int vocab, int width) {
-  return (size_t)groups * beams * chunks_for(dtype, groups * beams, vocab) * (8 + 8 * (size_t)width);
+  return (size_t)groups * beams * runs_of(dtype, groups * beams, vocab).chunks * (8 + 8 * (size_t)width);
 }
 
 int select(const Select& p, cudaStream_t s) {
-  const int rows = p.groups * p.beams, chunks = chunks_for(p.dtype, rows, p.vocab);
+  const int rows = p.groups * p.beams;
+  const Runs r = runs_of(p.dtype, rows, p.vocab);
   float2* sums = static_cast<float2*>(p.workspace);
-  float* values = reinterpret_cast<float*>(sums + (size_t)rows * chunks);
-  int* tokens = reinterpret_cast<int*>(values + (size_t)rows * chunks * p.width);
+  float* values = reinterpret_cast<float*>(sums + (size_t)rows * r.chunks);
+  int* tokens = reinterpret_cast<int*>(values + (size_t)rows * r.chunks * p.width);
   auto launch = [&](auto kernel, auto ptr) {
     count_launch();
-    kernel<<<(unsigned)rows * chunks, kThreads, 0, s>>>(ptr, p.group_stride, p.beam_stride, p.beams, p.vocab, p.width, chunks, sums, values,
-                                                        tokens);
+    kernel<<<(unsigned)rows * r.chunks, kThreads, 0, s>>>(ptr, p.group_stride, p.beam_stride, p.beams, p.vocab, p.width, r.chunks, r.units,
+                                                          sums, values, tokens);
   };
-  const bool four = units_for(p.dtype, rows, p.vocab) == 4;
   switch (p.dtype) {
-    case SA_F32: {
-      const float* x = static_cast<const float*>(p.logits);
-      four ? launch(candidates_kernel<float, 4>, x) : launch(candidates_kernel<float, 1>, x);
-      break;
-    }
-    case SA_BF16: {
-      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.logits);
-      four ? launch(candidates_kernel<__nv_bfloat16, 4>, x) : launch(candidates_kernel<__nv_bfloat16, 1>, x);
-      break;
-    }
-    case SA_F16: {
-      const __half* x = static_cast<const __half*>(p.logits);
-      four ? launch(candidates_kernel<__half, 4>, x) : launch(candidates_kernel<__half, 1>, x);
-      break;
-    }
+    case SA_F32: launch(candidates_kernel<float>, static_cast<const float*>(p.logits)); break;
+    case SA_BF16: launch(candidates_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(p.logits)); break;
+    case SA_F16: launch(candidates_kernel<__half>, static_cast<const __half*>(p.logits)); break;
     default: return SA_ERR_BAD_ARGUMENT;
   }
   SA_CUDA_CHECK(cudaGetLastError());
@@ -289,7 +365,7 @@ int select(const Select& p, cudaStream_t s) {
   config.attrs = &attr;
   config.numAttrs = 1;
   count_launch();
-  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, choose_kernel, p.scores, p.beams, p.vocab, p.width, chunks, (const float2*)sums,
+  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, choose_kernel, p.scores, p.beams, p.vocab, p.width, r.chunks, (const float2*)sums,
                                    (const float*)values, (const int*)tokens, p.out_scores, p.out_rows, p.out_tokens));
   return SA_OK;
 }

@@ -6,6 +6,8 @@
 // end.  Nothing depends on the order in which threads run.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "sa_paged.cuh"
 #include "sa_tc_ptx.cuh"
 
@@ -15,39 +17,34 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-// Exclusive sums of N numbers over the threads of a CTA; `total` receives the sums of all.  `warp_sums`: N x 32 in shared memory.
-template <int N>
-__device__ __forceinline__ void block_scan(long long (&x)[N], long long (&total)[N], long long (*warp_sums)[32]) {
+// Exclusive sums of N numbers over the threads of a CTA; `total` receives the sums of all.  `warp_sums`: 32 of each in shared
+// memory.
+template <int N, typename S>
+__device__ __forceinline__ void block_scan(S (&x)[N], S (&total)[N], S (*warp_sums)[32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  long long own[N];
+  S own[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     own[n] = x[n];
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x[n], s);
+      const S y = __shfl_up_sync(0xffffffffu, x[n], s);
       if (lane >= s) x[n] += y;
     }
     if (lane == 31) warp_sums[n][warp] = x[n];
   }
   __syncthreads();
-  if (warp == 0) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      long long v = lane < warps ? warp_sums[n][lane] : 0;
+  for (int n = 0; n < N; ++n) {                                 // every warp adds up the warps before it
+    S v = lane < warps ? warp_sums[n][lane] : 0;
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, v, s);
-        if (lane >= s) v += y;
-      }
-      warp_sums[n][lane] = v;
+    for (int s = 1; s < 32; s <<= 1) {
+      const S y = __shfl_up_sync(0xffffffffu, v, s);
+      if (lane >= s) v += y;
     }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    total[n] = warp_sums[n][31];
-    x[n] += (warp > 0 ? warp_sums[n][warp - 1] : 0) - own[n];
+    total[n] = __shfl_sync(0xffffffffu, v, 31);
+    const S before = __shfl_sync(0xffffffffu, v, max(warp - 1, 0));
+    x[n] += (warp > 0 ? before : 0) - own[n];
   }
   __syncthreads();                                              // warp_sums may be written again
 }
@@ -64,235 +61,225 @@ __device__ __forceinline__ int row_of(P first, int n, int x) {
   return lo;
 }
 
-__device__ __forceinline__ int64_t slot_of(const Tables& t, int row, int position) {
-  const int page = t.block_tables[(int64_t)row * t.max_pages + (position >> t.page_shift)];
-  return ((int64_t)page << t.page_shift) + (position & ((1 << t.page_shift) - 1));
-}
-
 struct Append {
   Tables t;
   const int* counts;
-  int total, max_length, max_count, least_tokens, wave_tiles, wave_decode, slots_inside;
+  int total, max_length, max_count, least_tokens, wave_tiles, wave_decode, inside;
   int *query_start, *cached;
   int64_t* slots;
   int* work;
   StepLayout layout;
 };
+// Sums over the rows before a row (rows + 1 each): tokens, pages that they take, tiles, pieces of single tokens; and the tokens that
+// a row has (-1: it is left as it is).
+struct RowSums {
+  int *start, *page, *tile, *piece, *before;
+  __device__ __forceinline__ RowSums(int* at, int rows)
+      : start(at), page(at + rows + 1), tile(at + 2 * (rows + 1)), piece(at + 3 * (rows + 1)), before(at + 4 * (rows + 1)) {}
+};
 
-// One CTA: PER rows a thread, a handful of prefix sums over the rows (tokens, pages, tiles, pieces), and everything that is
-// per page, per tile or per token spread over the threads by a search in those sums.  What it takes is the chain of dependent
-// loads, sums and barriers.  Slots of a long step are written by a second kernel
-// (slots_kernel): one SM stores about 60 GB/s of them.
-template <int PER>
+// Everything that is per page, per tile or per token, by a search in the sums: the caller takes every `step`-th from `first` on.
+__device__ __forceinline__ void spread(const Append& a, const RowSums& s, const int* header, int first, int step) {
+  const Tables& t = a.t;
+  const int page_mask = (1 << t.page_shift) - 1;
+  const int free_before = header[kFreeBefore], wanted = header[kPagesWanted], n_tiles = header[kTiles], n_single = header[kDecodeItems];
+  const int piece_keys = header[kPieceKeys];
+  const bool cut = header[kCut] != 0;
+  for (int i = first; i < a.layout.tickets_count; i += step) a.work[a.layout.tickets + i] = 0;
+  for (int k = first; k < wanted; k += step) {                    // off the end of the free list
+    const int r = row_of(s.page, t.rows, k);
+    if (s.before[r] < 0) continue;                                // the first row that did not fit
+    const int block = ((s.before[r] + page_mask) >> t.page_shift) + k - s.page[r];
+    const int page = t.free_pages[free_before - 1 - k];
+    t.block_tables[(int64_t)r * t.max_pages + block] = page;
+    if (page >= 0 && page < t.num_pages) atomicAdd(t.page_refs + page, 1);
+  }
+  for (int i = first; i < a.total; i += step) {
+    const int r = row_of(s.start, t.rows, i);
+    int64_t slot = -1;
+    if (i < s.start[t.rows] && s.before[r] >= 0) {
+      const int position = s.before[r] + i - s.start[r], block = position >> t.page_shift;
+      const int fresh = block - ((s.before[r] + page_mask) >> t.page_shift);    // of the row's new pages
+      const int page = fresh >= 0 ? t.free_pages[free_before - 1 - (s.page[r] + fresh)] : t.block_tables[(int64_t)r * t.max_pages + block];
+      slot = ((int64_t)page << t.page_shift) + (position & page_mask);
+    }
+    a.slots[i] = slot;
+  }
+  // tiles (a row's first tile first) and walks over their keys (the longest of a row first)
+  for (int i = first; i < n_tiles && !cut; i += step) {
+    const int r = row_of(s.tile, t.rows, i);
+    const TileItem x{r, s.start[r], s.before[r] / kTile + i - s.tile[r], i, 0, 1, s.before[r], s.before[r] + s.start[r + 1] - s.start[r]};
+    reinterpret_cast<TileItem*>(a.work + a.layout.tiles)[i] = x;
+    reinterpret_cast<TileItem*>(a.work + a.layout.tile_items)[n_tiles - 1 - i] = x;
+  }
+  for (int i = first; i < n_single; i += step) {
+    const int r = row_of(s.piece, t.rows, i);
+    DecodeItem x;
+    x.row = r; x.token = s.start[r];
+    x.first = s.piece[r];
+    x.piece = i - x.first;
+    x.pieces = s.piece[r + 1] - x.first;
+    x.length = s.before[r] + 1;
+    x.c0 = x.piece * piece_keys;
+    x.c1 = min(x.c0 + piece_keys, x.length);
+    reinterpret_cast<DecodeItem*>(a.work + a.layout.decode_items)[i] = x;
+  }
+}
+
+// One CTA: PER rows a thread and four prefix sums over the rows; what is per page, tile or token (spread) here too where that is
+// little, else in a second kernel of many CTAs (a quarter of a million slots and 16,800 pages: 48 us in one CTA).  What a small
+// step takes is the chain of dependent loads, sums and barriers.  S: 32 bits where no sum can pass them.
+template <int PER, typename S>
 __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Append a) {
   const Tables& t = a.t;
   extern __shared__ int rows_s[];
-  __shared__ long long warp_sums[4][32];
-  int* start_s = rows_s;                       // rows + 1: first token
-  int* page_s = start_s + t.rows + 1;          // rows + 1: pages that the rows before take
-  int* tile_s = page_s + t.rows + 1;           // rows + 1: tiles
-  int* piece_s = tile_s + t.rows + 1;          // rows + 1: pieces of single tokens
-  int* before_s = piece_s + t.rows + 1;        // rows: tokens before the step; -1 where the row is left as it is
-  const int tid = threadIdx.x, step = blockDim.x;
+  __shared__ S warp_sums[5][32];
+  __shared__ int header[kHeaderWords];
+  const RowSums sums(rows_s, t.rows);
+  const int tid = threadIdx.x;
   const int r0 = tid * PER;
   const int64_t limit = min((int64_t)t.max_pages << t.page_shift, (int64_t)a.max_length);
   const int page_mask = (1 << t.page_shift) - 1;
 
-  for (int i = tid; i < a.layout.tickets_count; i += step) a.work[a.layout.tickets + i] = 0;
   int count[PER], before[PER];
-  long long sum[1] = {0}, total[1];
+  S sum[1] = {0}, total[1];
+  const int free_count = min(max(*t.free_count, 0), t.num_pages);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int r = r0 + u;
-    count[u] = r < t.rows ? max(a.counts[r], 0) : 0;
+    count[u] = r < t.rows ? min(max(a.counts[r], 0), a.total + 1) : 0;
     before[u] = r < t.rows ? t.lengths[r] : 0;
     sum[0] += count[u];
   }
-  block_scan<1>(sum, total, warp_sums);
+  block_scan(sum, total, warp_sums);
   // ---- which rows fit, and the pages that they need -----------------------------------------------------------------------
   bool fits[PER];
   int need[PER];
-  long long pages[1] = {0}, pages_total[1];
+  S pages[1] = {0}, pages_total[1];
   {
-    long long at = sum[0];
+    S at = sum[0];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int r = r0 + u;
-      if (r < t.rows) start_s[r] = (int)min(at, (long long)a.total);
+      if (r < t.rows) sums.start[r] = (int)min(at, (S)a.total);
       at += count[u];
       fits[u] = r < t.rows && at <= a.total && count[u] <= a.max_count && before[u] >= 0 && (int64_t)before[u] + count[u] <= limit;
       need[u] = fits[u] ? ((before[u] + count[u] + page_mask) >> t.page_shift) - ((before[u] + page_mask) >> t.page_shift) : 0;
       pages[0] += need[u];
     }
   }
-  const int free_count = min(max(*t.free_count, 0), t.num_pages);
-  block_scan<1>(pages, pages_total, warp_sums);
-  long long next[4] = {0, 0, 0, 0}, next_total[4];    // tiles, key tiles of their walks, single tokens, their keys
+  block_scan(pages, pages_total, warp_sums);
+  S next[5] = {0, 0, 0, 0, 0}, next_total[5];    // tiles, key tiles of their walks, single tokens, their keys, pages taken
   {
-    long long upto = pages[0];
+    S upto = pages[0];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int r = r0 + u;
-      if (r < t.rows) page_s[r] = (int)min(upto, (long long)t.num_pages + 1);
+      if (r < t.rows) sums.page[r] = (int)min(upto, (S)t.num_pages + 1);
       upto += need[u];
       if (need[u] > 0 && upto > free_count) fits[u] = false;    // and every later row that needs a page
       if (r < t.rows) {
-        before_s[r] = fits[u] ? before[u] : -1;
+        sums.before[r] = fits[u] ? before[u] : -1;
         a.cached[r] = fits[u] ? before[u] : -1;
         if (fits[u] && count[u] > 0) t.lengths[r] = before[u] + count[u];
       }
       if (!fits[u]) count[u] = 0;
+      else next[4] += need[u];
       if (count[u] > 0 && count[u] < a.least_tokens) {
         next[2] += 1;
         next[3] += before[u] + 1;
       } else if (count[u] > 0) {
-        const long long first = before[u] / kTile, last = (before[u] + count[u] - 1) / kTile;
+        const S first = before[u] / kTile, last = (before[u] + count[u] - 1) / kTile;
         next[0] += last - first + 1;
         next[1] += (last - first + 1) * (first + last + 2) / 2;
       }
     }
   }
-  if (tid == 0) {
-    start_s[t.rows] = (int)min(total[0], (long long)a.total);
-    page_s[t.rows] = (int)min(pages_total[0], (long long)t.num_pages + 1);
-  }
-  block_scan<4>(next, next_total, warp_sums);
-  const int n_tiles = (int)next_total[0];
-  {
-    int at = (int)next[0];
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int r = r0 + u;
-      if (r < t.rows) {
-        tile_s[r] = at;
-        a.work[a.layout.tile_start + r] = at;
-      }
-      if (count[u] >= a.least_tokens) at += (before[u] + count[u] - 1) / kTile - before[u] / kTile + 1;
-    }
-    if (tid == 0) {
-      tile_s[t.rows] = n_tiles;
-      a.work[a.layout.tile_start + t.rows] = n_tiles;
-    }
-  }
-  // ---- pieces of single tokens: about one wave of CTAs over all heads, or several where rows alone are more than that --------
-  const int singles = (int)next_total[2];
+  block_scan(next, next_total, warp_sums);
+  const int n_tiles = (int)next_total[0], singles = (int)next_total[2];
+  // pieces of single tokens: about one wave of CTAs over all heads, or several where rows alone are more than that
   int piece_keys = kTile;
   if (singles > 0) {
-    const int spread = 2 * singles <= a.wave_decode ? a.wave_decode - singles : kDecodeWaves * a.wave_decode;
-    const long long keys = (next_total[3] + spread - 1) / spread;
-    piece_keys = (int)max((long long)kTile, (keys + kTile - 1) / kTile * kTile);
+    const int spread_over = 2 * singles <= a.wave_decode ? a.wave_decode - singles : kDecodeWaves * a.wave_decode;
+    const S keys = (next_total[3] + spread_over - 1) / spread_over;
+    piece_keys = (int)max((S)kTile, (keys + kTile - 1) / kTile * kTile);
   }
-  long long pieces[1] = {0}, pieces_total[1] = {0};
+  S pieces[1] = {0}, pieces_total[1] = {0};
   if (singles > 0) {
 #pragma unroll
     for (int u = 0; u < PER; ++u)
       if (count[u] > 0 && count[u] < a.least_tokens) pieces[0] += before[u] / piece_keys + 1;
-    block_scan<1>(pieces, pieces_total, warp_sums);
-    int at = (int)pieces[0];
+    block_scan(pieces, pieces_total, warp_sums);
+  }
+  // Few tiles: their walks are cut so that all heads together fill the GPU.
+  const bool cut = n_tiles > 0 && 2 * n_tiles <= a.wave_tiles;
+  {
+    int tile_at = (int)next[0], piece_at = (int)pieces[0];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int r = r0 + u;
-      if (r < t.rows) piece_s[r] = at;
-      if (count[u] > 0 && count[u] < a.least_tokens) at += before[u] / piece_keys + 1;
+      if (r < t.rows) {
+        sums.tile[r] = tile_at;
+        sums.piece[r] = piece_at;
+        a.work[a.layout.tile_start + r] = tile_at;
+        a.query_start[r] = sums.start[r];
+      }
+      if (count[u] >= a.least_tokens) tile_at += (before[u] + count[u] - 1) / kTile - before[u] / kTile + 1;
+      else if (count[u] > 0) piece_at += before[u] / piece_keys + 1;
     }
-    if (tid == 0) piece_s[t.rows] = (int)pieces_total[0];
+    if (tid == 0) {
+      sums.start[t.rows] = a.query_start[t.rows] = (int)min(total[0], (S)a.total);
+      sums.page[t.rows] = (int)min(pages_total[0], (S)t.num_pages + 1);
+      sums.tile[t.rows] = a.work[a.layout.tile_start + t.rows] = n_tiles;
+      sums.piece[t.rows] = (int)pieces_total[0];
+      header[kTiles] = n_tiles;
+      header[kTileItems] = n_tiles;
+      header[kDecodeItems] = (int)pieces_total[0];
+      header[kPieceKeys] = piece_keys;
+      header[kPagesWanted] = min(sums.page[t.rows], free_count);     // of the rows that are served: those up to the first that is not
+      header[kFreeBefore] = free_count;
+      header[kCut] = cut;
+      *t.free_count = free_count - (int)next_total[4];
+    }
   }
-  for (int i = tid; i <= t.rows; i += step) a.query_start[i] = start_s[i];
   __syncthreads();                                               // the sums, and who is served
-  // ---- pages, off the end of the free list -------------------------------------------------------------------------------------
-  const int wanted = min(page_s[t.rows], free_count);             // of the rows that are served: those up to the first that is not
-  int taken = 0;
-  for (int k = tid; k < wanted; k += step) {
-    const int r = row_of(page_s, t.rows, k);
-    if (before_s[r] < 0) continue;
-    const int block = ((before_s[r] + page_mask) >> t.page_shift) + k - page_s[r];
-    const int page = t.free_pages[free_count - 1 - k];
-    t.block_tables[(int64_t)r * t.max_pages + block] = page;
-    if (page >= 0 && page < t.num_pages) atomicAdd(t.page_refs + page, 1);
-    ++taken;
-  }
-  taken = __reduce_add_sync(0xffffffffu, taken);
-  if ((tid & 31) == 0 && taken > 0) atomicSub(t.free_count, taken);
-  // ---- the plan: tiles (a row's first tile first), walks over their keys (the longest of a row first), pieces ------------------
-  TileItem* tiles = reinterpret_cast<TileItem*>(a.work + a.layout.tiles);
-  TileItem* items = reinterpret_cast<TileItem*>(a.work + a.layout.tile_items);
-  DecodeItem* singles_out = reinterpret_cast<DecodeItem*>(a.work + a.layout.decode_items);
-  auto tile_at = [&](int i, TileItem* x) {
-    const int r = row_of(tile_s, t.rows, i);
-    x->row = r; x->token = start_s[r];
-    x->mi = before_s[r] / kTile + i - tile_s[r];
-    x->tile = i;
-    x->cached = before_s[r];
-    x->length = before_s[r] + start_s[r + 1] - start_s[r];
-    return r;
-  };
-  // Few tiles: their walks are cut so that all heads together fill the GPU.  A piece takes at least four key tiles.
-  const bool cut = n_tiles > 0 && 2 * n_tiles <= a.wave_tiles;
-  int n_items = n_tiles;
-  if (cut) {
-    const long long per = (next_total[1] + (a.wave_tiles - n_tiles) - 1) / (a.wave_tiles - n_tiles);
-    const int piece_tiles = (int)max(4LL, per);
+  if (cut) {                                                     // at most half a wave of 148 tiles; a piece takes at least four key tiles
+    const S per = (next_total[1] + (a.wave_tiles - n_tiles) - 1) / (a.wave_tiles - n_tiles);
+    const int piece_tiles = (int)max((S)4, per);
     TileItem x{};
-    long long parts[1] = {0}, parts_total[1];
-    if (tid < n_tiles) {                                          // at most half a wave of 148
-      tile_at(tid, &x);
-      tiles[tid] = x;
+    S parts[1] = {0}, parts_total[1];
+    if (tid < n_tiles) {
+      const int r = row_of(sums.tile, t.rows, tid);
+      x = TileItem{r, sums.start[r], sums.before[r] / kTile + tid - sums.tile[r], tid, 0, 1, sums.before[r],
+                   sums.before[r] + sums.start[r + 1] - sums.start[r]};
+      reinterpret_cast<TileItem*>(a.work + a.layout.tiles)[tid] = x;
       x.pieces = (x.mi + piece_tiles) / piece_tiles;
       parts[0] = x.pieces;
     }
-    block_scan<1>(parts, parts_total, warp_sums);
-    n_items = (int)parts_total[0];
+    block_scan(parts, parts_total, warp_sums);
     if (tid < n_tiles)
-      for (x.piece = 0; x.piece < x.pieces; ++x.piece) items[parts[0] + x.piece] = x;
+      for (x.piece = 0; x.piece < x.pieces; ++x.piece) reinterpret_cast<TileItem*>(a.work + a.layout.tile_items)[(int)parts[0] + x.piece] = x;
+    if (tid == 0) header[kTileItems] = (int)parts_total[0];
+    __syncthreads();
+  }
+  if (tid < kHeaderWords) a.work[tid] = header[tid];
+  if (a.inside) {
+    spread(a, sums, header, tid, blockDim.x);
   } else {
-    for (int i = tid; i < n_tiles; i += step) {
-      TileItem x{};
-      tile_at(i, &x);
-      tiles[i] = x;
-      x.pieces = 1;
-      items[n_tiles - 1 - i] = x;
-    }
-  }
-  const int n_single = (int)pieces_total[0];
-  for (int i = tid; i < n_single; i += step) {
-    const int r = row_of(piece_s, t.rows, i);
-    DecodeItem x;
-    x.row = r; x.token = start_s[r];
-    x.first = piece_s[r];
-    x.piece = i - x.first;
-    x.pieces = piece_s[r + 1] - x.first;
-    x.length = before_s[r] + 1;
-    x.c0 = x.piece * piece_keys;
-    x.c1 = min(x.c0 + piece_keys, x.length);
-    singles_out[i] = x;
-  }
-  if (tid == 0) {
-    a.work[kTiles] = n_tiles;
-    a.work[kTileItems] = n_items;
-    a.work[kDecodeItems] = n_single;
-  }
-  if (!a.slots_inside) return;
-  __syncthreads();                                               // the new pages are in the tables
-  for (int i = tid; i < a.total; i += step) {
-    const int r = row_of(start_s, t.rows, i);
-    const bool in = i < start_s[t.rows] && before_s[r] >= 0;
-    a.slots[i] = in ? slot_of(t, r, before_s[r] + i - start_s[r]) : -1;
+    for (int i = tid; i < 5 * (t.rows + 1) - 1; i += blockDim.x) a.work[a.layout.sums + i] = rows_s[i];
   }
 }
 
-__global__ void __launch_bounds__(256) slots_kernel(Tables t, int total, const int* __restrict__ query_start,
-                                                    const int* __restrict__ cached, int64_t* __restrict__ slots) {
+__global__ void __launch_bounds__(256) spread_kernel(const __grid_constant__ Append a) {
   tc::after_previous_kernel();
-  extern __shared__ int rows_s[];                                // query_start
-  for (int i = threadIdx.x; i <= t.rows; i += blockDim.x) rows_s[i] = query_start[i];
+  extern __shared__ int rows_s[];
+  __shared__ int header[kHeaderWords];
+  for (int i = threadIdx.x; i < 5 * (a.t.rows + 1) - 1; i += blockDim.x) rows_s[i] = __ldcg(a.work + a.layout.sums + i);
+  if (threadIdx.x < kHeaderWords) header[threadIdx.x] = __ldcg(a.work + threadIdx.x);
   __syncthreads();
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
-    const int r = row_of(rows_s, t.rows, i);
-    const int before = cached[r];
-    slots[i] = i < rows_s[t.rows] && before >= 0 ? slot_of(t, r, before + i - rows_s[r]) : -1;
-  }
+  spread(a, RowSums(rows_s, a.t.rows), header, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
-constexpr int kSlotsInside = 2048;
+constexpr int kInside = 2048;         // tokens of a step that one CTA writes by itself
 
 // ---- rows that become copies of other rows ------------------------------------------------------------------------------------
 // Row r becomes a copy of row parents[r] (outside [0, rows): an empty row).  Full pages are shared.  The page that is being
@@ -326,7 +313,7 @@ struct ReorderWork {
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThreads)
     reorder_kernel(Tables t, const int* __restrict__ parents, int* copies, int* moved, int* info, unsigned* marks, int* scratch) {
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ long long warp_sums[2][32];
+  __shared__ int warp_sums[2][32];
   const int tid = threadIdx.x, cta = (int)cluster.block_rank();
   const int all = kCluster * kReorderThreads, me = cta * kReorderThreads + tid;
   const int lane = tid & 31, warp = me >> 5, warps = all >> 5;
@@ -385,8 +372,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
     for (int w0 = 0; w0 < words; w0 += kReorderThreads) {
       const int w = w0 + tid;
       unsigned bits = w < words ? __ldcg(marks + w) : 0u;
-      long long n[1] = {__popc(bits)}, total[1];
-      block_scan<1>(n, total, warp_sums);
+      int n[1] = {__popc(bits)}, total[1];
+      block_scan(n, total, warp_sums);
       for (int at = count + (int)n[0]; bits != 0u && at < t.num_pages; bits &= bits - 1u, ++at) t.free_pages[at] = w * 32 + __ffs(bits) - 1;
       count = min(count + (int)total[0], t.num_pages);
     }
@@ -398,8 +385,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
       const int len = p >= 0 ? length_of(p) : 0, full = len >> t.page_shift;
       const bool fresh = r < t.rows && __ldcg(info + r) != 0;
       const bool changes = len > 0 && (p != r || fresh);
-      long long n[2] = {fresh ? 1 : 0, changes ? 1 : 0}, total[2];
-      block_scan<2>(n, total, warp_sums);
+      int n[2] = {fresh ? 1 : 0, changes ? 1 : 0}, total[2];
+      block_scan(n, total, warp_sums);
       int src = -1, dst = -1;
       bool dropped = false;
       if (fresh) {
@@ -520,10 +507,10 @@ int append(const Tables& t, const int* counts, int total, int max_length, int ma
   a.least_tokens = tile_tokens(t.rows, total, max_count);
   a.wave_tiles = tile_wave(t.heads);
   a.wave_decode = decode_wave(t.heads);
-  a.slots_inside = total <= kSlotsInside;
+  a.inside = total <= kInside;
   a.query_start = query_start; a.cached = cached; a.slots = slots; a.work = work;
   a.layout = step_layout(t.rows, total, t.heads);
-  const size_t smem = (5 * (size_t)t.rows + 4) * 4;
+  const size_t smem = 5 * ((size_t)t.rows + 1) * 4;
   auto launch = [&](auto kernel, int threads) -> int {
     SA_CUDA_CHECK(allow_smem(kernel, smem));
     count_launch();
@@ -531,13 +518,22 @@ int append(const Tables& t, const int* counts, int total, int max_length, int ma
     SA_CUDA_CHECK(cudaGetLastError());
     return SA_OK;
   };
+  const int64_t most = (int64_t)t.rows * max(total + 1, min(max_length, t.max_pages << t.page_shift) + 1);
+  const int64_t walks = ((int64_t)total / kTile + 2 * t.rows) * (((int64_t)t.max_pages << t.page_shift) / kTile + 2);
+  const bool narrow = most < (1LL << 31) && 2 * walks < (1LL << 31);
+  auto by_width = [&](auto per, int threads) {
+    constexpr int kPer = decltype(per)::value;
+    return narrow ? launch(append_kernel<kPer, int>, threads) : launch(append_kernel<kPer, long long>, threads);
+  };
+  using One = std::integral_constant<int, 1>;
   // 256 threads where they cover rows and tokens: barriers and sums over eight warps are shorter than over thirty-two
-  const int st = t.rows <= 256 && total <= 256 ? launch(append_kernel<1>, 256)
-                 : t.rows <= 1024              ? launch(append_kernel<1>, 1024)
-                                               : launch(append_kernel<kMaxRows / 1024>, 1024);
-  if (st != SA_OK || a.slots_inside) return st;
-  const unsigned blocks = (unsigned)min((total + 255) / 256, 4 * kSms);
-  return launch_after(slots_kernel, dim3(blocks), 256, ((size_t)t.rows + 1) * 4, s, t, total, (const int*)query_start, (const int*)cached, slots);
+  const int st = t.rows <= 256 && total <= 256 ? by_width(One{}, 256)
+                 : t.rows <= 1024              ? by_width(One{}, 1024)
+                                               : by_width(std::integral_constant<int, kMaxRows / 1024>{}, 1024);
+  if (st != SA_OK || a.inside) return st;
+  const unsigned blocks = (unsigned)min((total + 255) / 256, 2 * kSms);
+  SA_CUDA_CHECK(allow_smem(spread_kernel, smem));
+  return launch_after(spread_kernel, dim3(blocks), 256, smem, s, a);
 }
 
 size_t reorder_work_words(int rows, int max_pages, int num_pages) { return ReorderWork(rows, max_pages, num_pages).words; }

@@ -16,8 +16,8 @@ struct Tables {
 };
 
 // ---- the plan of a step: int32 words that sa_page_append writes and the attention over pages reads ------------------------
-// header | first tile of every row | tiles | tile items | decode items | tickets (zero between launches)
-enum : int { kTiles = 0, kTileItems = 1, kDecodeItems = 2, kHeaderWords = 16 };
+// header | sums over the rows | first tile of every row | tiles | tile items | decode items | tickets (zero between launches)
+enum : int { kTiles = 0, kTileItems = 1, kDecodeItems = 2, kPieceKeys = 3, kPagesWanted = 4, kFreeBefore = 5, kCut = 6, kHeaderWords = 16 };
 
 // One walk over the keys of a 128-query tile: key tiles from the diagonal back, cut into `pieces` (which stand together).
 struct TileItem {
@@ -40,7 +40,7 @@ inline int tile_tokens(int rows, int total, int max_count) { return rows == 1 &&
 
 struct StepLayout {
   int tiles_max, tile_items_max, decode_items_max;
-  size_t tile_start, tiles, tile_items, decode_items, tickets, words;   // offsets in words
+  size_t sums, tile_start, tiles, tile_items, decode_items, tickets, words;   // offsets in words
   int tickets_count;
 };
 inline int decode_wave(int heads) { const int w = kSms * kDecodeCtas / heads; return w > 1 ? w : 1; }
@@ -59,6 +59,7 @@ inline StepLayout step_layout(int rows, int total, int heads) {
     at += (n + 7) / 8 * 8;
     return x;
   };
+  l.sums = take(5 * ((size_t)rows + 1));
   l.tile_start = take((size_t)rows + 1);
   l.tiles = take(8 * (size_t)l.tiles_max);
   l.tile_items = take(8 * (size_t)l.tile_items_max);

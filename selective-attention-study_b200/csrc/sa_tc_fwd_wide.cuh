@@ -349,6 +349,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           const uint4 v4 = *reinterpret_cast<const uint4*>(src + (chunk >> 3) * kRowTile + swz_off(row, chunk & 7));
           w[4 * c] = v4.x; w[4 * c + 1] = v4.y; w[4 * c + 2] = v4.z; w[4 * c + 3] = v4.w;
         }
+        // PAGED: the tile's other rows are queries of other sequences: zeros, which select nothing (a NaN of theirs would reach
+        // every row through the running sum)
+        if (PAGED && (i0 + row < q_offset || i0 + row >= seq)) {
+#pragma unroll
+          for (int e = 0; e < kChunks * 4; ++e) w[e] = 0u;
+        }
         tmem_st_n<kChunks * 4>(lane_base + (m == 0 ? kColQ : kColQ0) + wg * (kChunks * 4), w);
       }
     }
@@ -385,10 +391,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const float* carry_row = carry + (PAGED ? ((int64_t)item.tile * (SELF ? heads : 1) + (SELF ? h : 0)) * paged.key_stride
                                             : ((int64_t)b * (ntiles + 1) + mi) * seq);
     const int i = i0 + row;
-    // PAGED: the tile's other rows are queries of other sequences, which select nothing here (a NaN of theirs would reach every
-    // row through the running sum)
     const bool mine = !PAGED || (i >= q_offset && i < seq);
-    const bool ragged = PAGED && (i0 < q_offset || i0 + kTile > seq);
     const int cw = wg * NC;                                    // this warpgroup's key columns within a step
 
     // The carry of a step's keys is fetched from global memory a step before it is staged, so the load's latency
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       if (tid < kTile) carry_s[it & 1][tid] = -carry_value * kLog2e;   // negated: the logits pass adds it in an FMA
       mbar_wait(&bar_l0, it & 1, status, 313);
       tc_fence_after_sync();
-      const bool masked = (j0 + kTile > i0) || (j0 < exempt) || ragged;
+      const bool masked = (j0 + kTile > i0) || (j0 < exempt);
       uint32_t r32[32];
       tmem_ld32(lane_base + kColL + cw, r32);                 // one load and one wait for the step's 32 columns
       tmem_ld_wait();

@@ -48,26 +48,11 @@ inline int make_map_16bit(CUtensorMap* map, const void* base, int head_dim, int 
   return SA_OK;
 }
 
-// 4-D map over (d, token of the page, head, page) of a bf16 pool of pages, (pages, heads, page_size, head_dim) contiguous; box =
-// (box_d elements, box_rows tokens, 1, 1).  A page outside the pool reads as zeros.
-inline int make_pool_map(CUtensorMap* map, const void* base, int head_dim, int page_size, int heads, int pages, int box_d, int box_rows,
-                         bool swizzled) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return SA_ERR_CUDA;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return SA_ERR_ALIGNMENT;
-  const cuuint64_t row = (cuuint64_t)head_dim * 2;
-  cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {row, row * page_size, row * page_size * heads};
-  cuuint32_t box[4] = {(cuuint32_t)box_d, (cuuint32_t)box_rows, 1, 1};
-  cuuint32_t elem[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, elem,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_last_cuda_error(10000 + (int)r);
-    return SA_ERR_CUDA;
-  }
-  return SA_OK;
+// The same over (d, token of the page, head, page) of a pool of pages, (pages, heads, page_size, head_dim) contiguous.  A page
+// outside the pool reads as zeros.
+inline int make_pool_map(CUtensorMap* map, const void* base, int head_dim, int page_size, int heads, int pages, int box_rows) {
+  const int64_t row = head_dim, head = row * page_size;
+  return make_map_16bit(map, base, head_dim, page_size, heads, pages, row, head, head * heads, box_rows);
 }
 
 // 4-D map over (d, token, row, 1) of a contiguous fp32 tensor (rows x seq x dim); box = (32 floats, 32 tokens, 1, 1): the

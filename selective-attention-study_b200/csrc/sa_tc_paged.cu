@@ -70,12 +70,13 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q0s = smem;                               // DK tiles [128 queries][64]
   uint8_t* k0s = smem + DK * kRowTile;               // 2 stages x DK tiles [128 keys][64]
-  __shared__ uint64_t bar_q, bar_k[2], bar_mma[2], bar_read[2];
+  __shared__ uint64_t bar_q, bar_zero, bar_k[2], bar_mma[2], bar_read[2];
   __shared__ uint32_t tmem_base_s;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&bar_q, 1);
+    mbar_init(&bar_zero, 4);
     for (int u = 0; u < 2; ++u) {
       mbar_init(&bar_k[u], 1);
       mbar_init(&bar_mma[u], 1);
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
     load_k(0);
     if (count > 1) load_k(1);
     await(&bar_q, 0, 211);
+    await(&bar_zero, 0, 215);
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
       const int st = it & 1;
@@ -144,13 +146,20 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
     const int lo = max(w.cached - i0, 0), hi = min(w.length - i0, kTile);  // the tile's queries that are the row's
     float* dst = carry + ((int64_t)blockIdx.x * gridDim.z + h) * paged.key_stride;
+    if (lo > 0 || hi < kTile) {                                            // the others select nothing: zeros
+      mbar_wait(&bar_q, 0, status, 216);
+      if (tid < lo || tid >= hi)
+        for (int u = 0; u < 8 * DK; ++u) *reinterpret_cast<uint4*>(q0s + (u >> 3) * kRowTile + tid * 128 + (u & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      fence_async_smem();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar_zero);
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
       mbar_wait(&bar_mma[it & 1], (uint32_t)((it >> 1) & 1), status, 212);
       tc_fence_after_sync();
       const bool diag = nj0 + it == w.mi;
-      const bool masked = diag || lo > 0 || hi < kTile;
-      const int from = diag ? max(lo, tid + 1) : lo;                      // (key and query count from the same position)
+      const int from = max(lo, tid + 1);                                  // (key and query count from the same position)
       float2 acc[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
@@ -159,7 +168,7 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
         uint32_t r[32];
         tmem_ld32(lane_base + (it & 1) * 128 + c0, r);
         tmem_ld_wait();
-        if (masked) {
+        if (diag) {                                                        // and where keys behind the row stand
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (c0 + e < from || c0 + e >= hi) r[e] = 0u;
@@ -245,9 +254,9 @@ int tiles_impl(const Attention& a, cudaStream_t s) {
   CUtensorMap map_q, map_k, map_v;
   int st = make_map_16bit(&map_q, a.q, D, a.total, a.heads, 1, a.q_stride[0], a.q_stride[1], 0, kTile);
   if (st != SA_OK) return st;
-  st = make_pool_map(&map_k, a.k_pages, D, page, a.heads, a.num_pages, 64, box_rows, true);
+  st = make_pool_map(&map_k, a.k_pages, D, page, a.heads, a.num_pages, box_rows);
   if (st != SA_OK) return st;
-  st = make_pool_map(&map_v, a.v_pages, D, page, a.heads, a.num_pages, 64, box_rows, true);
+  st = make_pool_map(&map_v, a.v_pages, D, page, a.heads, a.num_pages, box_rows);
   if (st != SA_OK) return st;
   WaitCtx status;
   st = wait_ctx(&status);
