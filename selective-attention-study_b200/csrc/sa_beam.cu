@@ -3,16 +3,15 @@
 //   score[k][v] = scores[k] + logits[k][v] - log sum_u exp(logits[k][u]);   the WIDTH largest over (k, v) of a group, in order,
 //   equal ones by the lowest k V + v.
 //
-// Two launches.  candidates_kernel: a CTA takes a run of one beam's vocabulary and leaves the run's maximum, its sum of exponentials
-// and its WIDTH largest logits.  The run is read twice, for the sum and for the candidates, the second time from L2 (kept in
-// registers, runs are short: 8,192 logits a CTA, 1,792 CTAs for 256 beams of 50,304, took 43 us).  choose_kernel (a CTA a group) makes the
+// Two launches.  candidates_kernel: a CTA takes a run of one beam's vocabulary into shared memory and leaves the run's maximum, its
+// sum of exponentials and its WIDTH largest logits.  choose_kernel (a CTA a group) makes the
 // beams' log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
 // Bound by memory where there are many beams, else by the latency of the two launches.
 //
-// The largest of a set, without sorting it: each of the eight warps gives the ceil(WIDTH / 8)-th largest of its lanes' own maxima;
-// WIDTH elements at least reach the least of the eight, and not many more do (about 25 for 8 of 8,192 random ones).  Those are
-// ranked among themselves.  Where more than kList reach it (equal or masked logits) they are taken one by one.
+// The largest of a set, without sorting it: each of the eight warps gives the largest of its lanes' own maxima, about two times
+// WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among
+// themselves.  Where more than kList reach it (equal or masked logits) they are taken one by one.
 #include "sa_common.cuh"
 #include "sa_beam.cuh"
 #include "sa_tc_ptx.cuh"
@@ -37,7 +36,8 @@ __device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& 
 
 template <typename V, typename I>
 struct Shared {
-  V bound[kThreads / 32];
+  V tops[kThreads / 4];
+  V bound;
   Entry<V, I> list[kList];
   int count;
   Entry<V, I> warp_best[kThreads / 32];
@@ -50,9 +50,10 @@ template <typename V, typename I, typename Reach, typename Emit>
 __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, const Reach& reach, const Emit& emit) {
   const int tid = threadIdx.x, lane = tid & 31;
   constexpr V kNone = -INFINITY;
-  V top = kNone;
-  for (int left = (width + kThreads / 32 - 1) / (kThreads / 32); left > 0; --left) {
-    top = mine;
+  constexpr int kWarps = kThreads / 32;
+  const int each = 2 * ((width + kWarps - 1) / kWarps), given = each * kWarps;      // 2 to 8 a warp, at most 64
+  for (int u = 0; u < each; ++u) {
+    V top = mine;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
       const V o = __shfl_xor_sync(0xffffffffu, top, s);
@@ -60,13 +61,18 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, con
     }
     const unsigned at = __ballot_sync(0xffffffffu, mine == top);
     if (lane == __ffs(at) - 1) mine = kNone;                // one of them is done with
+    if (lane == 0) sh.tops[u * kWarps + (tid >> 5)] = top;
   }
-  if (lane == 0) sh.bound[tid >> 5] = top;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  V bound = sh.bound[0];
-#pragma unroll
-  for (int u = 1; u < kThreads / 32; ++u) bound = sh.bound[u] < bound ? sh.bound[u] : bound;
+  if (tid < given) {
+    const V own = sh.tops[tid];
+    int rank = 0;
+    for (int u = 0; u < given; ++u) rank += sh.tops[u] > own || (sh.tops[u] == own && u < tid) ? 1 : 0;
+    if (rank == width - 1) sh.bound = own;
+  }
+  __syncthreads();
+  const V bound = sh.bound;
   reach(bound, [&](V x, I i) {
     const int at = atomicAdd(&sh.count, 1);
     if (at < kList) sh.list[at] = Entry<V, I>{x, i};
@@ -133,17 +139,21 @@ template <> struct Word<__half> {
 };
 
 // Elements are taken in units of 16 bytes from a 16-byte boundary on: a row that begins elsewhere has `lead` elements fewer in
-// its first unit.  Units that stick out of the row are read element by element.
-constexpr int kAhead = 4;            // units in flight a thread: 64 KB an SM with four CTAs
+// its first unit.  A unit that sticks out of the row is put together element by element; the others come by bulk copies in
+// kParts parts, so that the first is worked on while the last is on its way.
+constexpr int kParts = 4;
+constexpr int kMostUnits = 3328;     // of a CTA: 52 KB, four CTAs an SM
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __restrict__ logits, int64_t group_stride, int64_t beam_stride,
                                                                  int beams, int vocab, int width, int chunks, int units,
                                                                  float2* __restrict__ sums, float* __restrict__ values,
-                                                                 int* __restrict__ tokens) {
+                                                                 int* __restrict__ tokens, tc::WaitCtx status) {
   using W = Word<T>;
   constexpr int kPer = 16 / (int)sizeof(T);
   asm volatile("griddepcontrol.launch_dependents;");
+  extern __shared__ __align__(128) uint4 run[];
+  __shared__ uint64_t arrived[kParts];
   __shared__ Shared<float, int> sh;
   __shared__ float red[2][kThreads / 32];
   const int n = blockIdx.x / chunks, chunk = blockIdx.x - n * chunks;      // n: beam over all groups
@@ -151,61 +161,71 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
   const T* row = logits + g * group_stride + (int64_t)(n - g * beams) * beam_stride;
   const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int tid = threadIdx.x;
-  // this CTA's units: [unit0, unit1) of the row's
+  // this CTA's units: [unit0, unit0 + count) of the row's, of which [whole0, whole1) lie inside the row
   const int total = (int)(((int64_t)vocab + lead + kPer - 1) / kPer);
-  const int unit0 = chunk * units, unit1 = min(unit0 + units, total);
-  auto load = [&](int unit) {
-    const int64_t v = (int64_t)unit * kPer - lead;
-    if (unit < unit1 && v >= 0 && v + kPer <= vocab) return *reinterpret_cast<const uint4*>(row + v);
+  const int unit0 = chunk * units, count = max(0, min(units, total - unit0));
+  const int whole0 = unit0 == 0 && lead > 0 ? 1 : 0, whole1 = max(whole0, min(count, (int)(((int64_t)vocab + lead) / kPer) - unit0));
+  const int part_units = (whole1 - whole0 + kParts - 1) / kParts;
+  if (tid == 0) {
+    for (int p = 0; p < kParts; ++p) tc::mbar_init(&arrived[p], 1);
+    tc::mbar_init_fence();
+    for (int p = 0; p < kParts; ++p) {
+      const int u0 = whole0 + p * part_units, u1 = min(u0 + part_units, whole1);
+      tc::mbar_expect_tx(&arrived[p], u1 > u0 ? (uint32_t)(u1 - u0) * 16u : 0u);
+      if (u1 > u0) tc::bulk_load(run + u0, row + (int64_t)(unit0 + u0) * kPer - lead, (uint32_t)(u1 - u0) * 16u, &arrived[p]);
+    }
+  }
+  for (int u = tid; u < whole0 + count - whole1; u += kThreads) {          // at most two
+    const int at = u < whole0 ? u : whole1 + u - whole0;
+    const int64_t v = (int64_t)(unit0 + at) * kPer - lead;
     uint32_t x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[i] = 0;
 #pragma unroll
       for (int e = 0; e < W::kPer; ++e) {
-        const int64_t at = v + i * W::kPer + e;
+        const int64_t j = v + i * W::kPer + e;
         uint32_t one = W::none();
-        if (unit < unit1 && at >= 0 && at < vocab) {
-          if constexpr (sizeof(T) == 4) one = __float_as_uint(row[at]);
-          else one = *reinterpret_cast<const uint16_t*>(row + at);
+        if (j >= 0 && j < vocab) {
+          if constexpr (sizeof(T) == 4) one = __float_as_uint(row[j]);
+          else one = *reinterpret_cast<const uint16_t*>(row + j);
         }
         x[i] |= one << (16 * e);
       }
     }
-    return make_uint4(x[0], x[1], x[2], x[3]);
-  };
+    run[at] = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+  __syncthreads();
   // The run's maximum (NaNs aside) and its sum of exponentials (with them), by thread with a maximum of its own.
   // +inf: inf - inf, a NaN as a NaN among the logits: the beam has no finite sum.
   float mine = -INFINITY, sum = 0.f;
-  for (int base = unit0; base < unit1; base += kThreads * kAhead) {
-    uint4 raw[kAhead];
+  auto take = [&](int u) {
+    const uint4 raw = run[u];
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[kPer], top = mine;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) raw[u] = load(base + u * kThreads + tid);
-    float x[kAhead][kPer], top = mine;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        x[u][i] = W::at(w[i / W::kPer], i % W::kPer);
-        top = fmaxf(top, x[u][i]);
-      }
+    for (int i = 0; i < kPer; ++i) {
+      x[i] = W::at(w[i / W::kPer], i % W::kPer);
+      top = fmaxf(top, x[i]);
     }
     const float from = top == -INFINITY ? 0.f : top;
     if (top > mine) sum *= tc::ex2((mine - from) * kLog2e);
     mine = top;
-    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     const float2 shift = make_float2(-from, -from), scale = make_float2(kLog2e, kLog2e);
+    float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-      for (int i = 0; i < kPer; i += 2) {
-        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[u][i], x[u][i + 1]), shift), scale);
-        part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], make_float2(tc::ex2(d.x), tc::ex2(d.y)));
-      }
-    const float2 both = __fadd2_rn(part[0], part[1]);
-    sum += both.x + both.y;
+    for (int i = 0; i < kPer; i += 2) {
+      const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), shift), scale);
+      part = __fadd2_rn(part, make_float2(tc::ex2(d.x), tc::ex2(d.y)));
+    }
+    sum += part.x + part.y;
+  };
+  int here = whole0, part = 0;                              // units below `here` have arrived
+  for (int u = tid; u < count; u += kThreads) {
+    for (; u >= here && part < kParts; here = min(here + part_units, whole1)) tc::mbar_wait(&arrived[part++], 0, status, 700);
+    take(u);
   }
+  for (; part < kParts; ++part) tc::mbar_wait(&arrived[part], 0, status, 700);
   float top = mine;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
@@ -222,26 +242,26 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
     for (int u = 1; u < kThreads / 32; ++u) sum += red[1][u];
     sums[blockIdx.x] = make_float2(top, sum);
   }
+  // Few threads have anything to give: each one's units are looked through by its whole warp.
   auto reach = [&](float bound, auto f) {
-    for (int base = unit0; base < unit1; base += kThreads * kAhead) {
-      uint4 raw[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) raw[u] = load(base + u * kThreads + tid);
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    for (unsigned left = __ballot_sync(0xffffffffu, mine >= bound); left != 0u; left &= left - 1u) {
+      const int first = (tid & ~31) + __ffs(left) - 1;
+      for (int u = first + (tid & 31) * kThreads; u < count; u += 32 * kThreads) {
+        const uint4 raw = run[u];
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) most = fmaxf(most, W::at(w[i / W::kPer], i % W::kPer));
         if (most < bound) continue;
+        const int64_t v = (int64_t)(unit0 + u) * kPer - lead;
 #pragma unroll 1
         for (int i = 0; i < kPer; ++i) {
-          const int64_t at = ((int64_t)base + u * kThreads + tid) * kPer - lead + i;
-          if (base + u * kThreads + tid >= unit1 || at < 0 || at >= vocab) continue;
-          const float v = fmaxf(to_float<T>(row[at]), -INFINITY);          // a NaN is never chosen
-          if (v >= bound) f(v, (int)at);
+          if (v + i < 0 || v + i >= vocab) continue;
+          const float x = fmaxf(to_float<T>(reinterpret_cast<const T*>(run)[u * kPer + i]), -INFINITY);      // a NaN is never chosen
+          if (x >= bound) f(x, (int)(v + i));
         }
       }
+      __syncwarp();
     }
   };
   float* out_v = values + (int64_t)blockIdx.x * width;
@@ -260,6 +280,9 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
   __shared__ Shared<double, long long> sh;
   __shared__ double base[kMaxBeams];                         // score - log-sum-exp of a beam; NaN: all of its scores are -inf
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  // candidate of this thread in every 256: a warp has every eighth, of all beams (of a poor beam alone, its maximum would let
+  // all of the others' candidates pass)
+  const int place = lane * (kThreads / 32) + (tid >> 5);
   const int per_beam = chunks * width, n = beams * per_beam;
   const int64_t first = (int64_t)g * n;
   constexpr int kKept = 4;                                   // candidates of a thread that are on their way meanwhile
@@ -267,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
   int kept_t[kKept];
 #pragma unroll
   for (int u = 0; u < kKept; ++u) {
-    const int i = tid + u * kThreads;
+    const int i = place + u * kThreads;
     kept_v[u] = i < n ? values[first + i] : 0.f;
     kept_t[u] = i < n ? tokens[first + i] : -1;
   }
@@ -302,8 +325,8 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
   auto each = [&](auto f) {
 #pragma unroll
     for (int u = 0; u < kKept; ++u)
-      if (tid + u * kThreads < n) one(tid + u * kThreads, kept_v[u], kept_t[u], f);
-    for (int i = tid + kKept * kThreads; i < n; i += kThreads) one(i, values[first + i], tokens[first + i], f);
+      if (place + u * kThreads < n) one(place + u * kThreads, kept_v[u], kept_t[u], f);
+    for (int i = place + kKept * kThreads; i < n; i += kThreads) one(i, values[first + i], tokens[first + i], f);
   };
   double mine = -INFINITY;
   each([&](double x, long long) { mine = x > mine ? x : mine; });
@@ -320,13 +343,14 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
   });
 }
 
-// Runs of a beam's vocabulary, a CTA each: as many as make one wave of four CTAs an SM, none shorter than a unit a thread.
+// Runs of a beam's vocabulary, a CTA each: as many as make one wave of four CTAs an SM where they fit, none shorter than kLeastUnits.
+constexpr int kLeastUnits = 512;
 struct Runs { int chunks, units; };
 Runs runs_of(int dtype, int rows, int vocab) {
   const int per = dtype == SA_F32 ? 4 : 8;
   const int total = (int)(((int64_t)vocab + per - 1 + per - 1) / per);      // a row may begin up to per - 1 elements into a unit
-  const int most = (total + kThreads - 1) / kThreads, wave = max(1, 4 * kSms / rows);
-  const int chunks = min(most, wave);
+  const int most = (total + kLeastUnits - 1) / kLeastUnits, least = (total + kMostUnits - 1) / kMostUnits;
+  const int chunks = max(least, min(most, max(1, 4 * kSms / rows)));
   const int units = (total + chunks - 1) / chunks;
   return Runs{(total + units - 1) / units, units};
 }
@@ -343,18 +367,25 @@ int select(const Select& p, cudaStream_t s) {
   float2* sums = static_cast<float2*>(p.workspace);
   float* values = reinterpret_cast<float*>(sums + (size_t)rows * r.chunks);
   int* tokens = reinterpret_cast<int*>(values + (size_t)rows * r.chunks * p.width);
-  auto launch = [&](auto kernel, auto ptr) {
+  tc::WaitCtx status;
+  int st = tc::wait_ctx(&status);
+  if (st != SA_OK) return st;
+  auto launch = [&](auto kernel, auto ptr) -> int {
+    const size_t smem = (size_t)r.units * 16;
+    SA_CUDA_CHECK(allow_smem(kernel, smem));
     count_launch();
-    kernel<<<(unsigned)rows * r.chunks, kThreads, 0, s>>>(ptr, p.group_stride, p.beam_stride, p.beams, p.vocab, p.width, r.chunks, r.units,
-                                                          sums, values, tokens);
+    kernel<<<(unsigned)rows * r.chunks, kThreads, smem, s>>>(ptr, p.group_stride, p.beam_stride, p.beams, p.vocab, p.width, r.chunks, r.units,
+                                                             sums, values, tokens, status);
+    SA_CUDA_CHECK(cudaGetLastError());
+    return SA_OK;
   };
   switch (p.dtype) {
-    case SA_F32: launch(candidates_kernel<float>, static_cast<const float*>(p.logits)); break;
-    case SA_BF16: launch(candidates_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(p.logits)); break;
-    case SA_F16: launch(candidates_kernel<__half>, static_cast<const __half*>(p.logits)); break;
+    case SA_F32: st = launch(candidates_kernel<float>, static_cast<const float*>(p.logits)); break;
+    case SA_BF16: st = launch(candidates_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(p.logits)); break;
+    case SA_F16: st = launch(candidates_kernel<__half>, static_cast<const __half*>(p.logits)); break;
     default: return SA_ERR_BAD_ARGUMENT;
   }
-  SA_CUDA_CHECK(cudaGetLastError());
+  if (st != SA_OK) return st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;

@@ -105,12 +105,23 @@ __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const 
     }
     a.slots[i] = slot;
   }
-  // tiles (a row's first tile first) and walks over their keys (the longest of a row first)
-  for (int i = first; i < n_tiles && !cut; i += step) {
+  // tiles (a row's first tile first), and walks over their keys, the longest of all rows first: a CTA each, taken in this order
+  // (a warp a tile: its place is the number of longer walks, and of equal ones of earlier rows)
+  for (int i = first >> 5; i < n_tiles && !cut; i += step >> 5) {
     const int r = row_of(s.tile, t.rows, i);
-    const TileItem x{r, s.start[r], s.before[r] / kTile + i - s.tile[r], i, 0, 1, s.before[r], s.before[r] + s.start[r + 1] - s.start[r]};
+    const int mi = s.before[r] / kTile + i - s.tile[r];
+    int at = 0;
+    for (int u = first & 31; u < t.rows; u += 32) {
+      const int n = s.tile[u + 1] - s.tile[u];
+      if (n == 0) continue;
+      const int from = s.before[u] / kTile, beyond = from + n - 1 - mi;      // tiles of row u behind tile mi of its own
+      at += max(0, min(n, beyond)) + (u < r && from <= mi && beyond >= 0 ? 1 : 0);
+    }
+    at = __reduce_add_sync(0xffffffffu, at);
+    if ((first & 31) != 0) continue;
+    const TileItem x{r, s.start[r], mi, i, 0, 1, s.before[r], s.before[r] + s.start[r + 1] - s.start[r]};
     reinterpret_cast<TileItem*>(a.work + a.layout.tiles)[i] = x;
-    reinterpret_cast<TileItem*>(a.work + a.layout.tile_items)[n_tiles - 1 - i] = x;
+    reinterpret_cast<TileItem*>(a.work + a.layout.tile_items)[at] = x;
   }
   for (int i = first; i < n_single; i += step) {
     const int r = row_of(s.piece, t.rows, i);
@@ -290,7 +301,7 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // each page of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first,
 // and takes the pages for the copies off its end, in row order; (4) the tables.  A row for which there is none becomes empty (its
 // full pages are shared with the lowest child, so nothing else is freed).
-constexpr int kCluster = 8, kReorderThreads = 512;
+constexpr int kCluster = 8, kReorderThreads = 1024;
 
 // The work of a reordering, int32 words: how many rows change, then (row, parent, tokens, tokens of the page being filled) of
 // each | a word a row | a bit a page | the new tables.
@@ -313,33 +324,35 @@ struct ReorderWork {
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThreads)
     reorder_kernel(Tables t, const int* __restrict__ parents, int* copies, int* moved, int* info, unsigned* marks, int* scratch) {
   cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ int rows_s[];
   __shared__ int warp_sums[2][32];
+  int *parent_s = rows_s, *length_s = rows_s + t.rows;            // -1: none; in tokens
   const int tid = threadIdx.x, cta = (int)cluster.block_rank();
   const int all = kCluster * kReorderThreads, me = cta * kReorderThreads + tid;
   const int lane = tid & 31, warp = me >> 5, warps = all >> 5;
   const int page_mask = (1 << t.page_shift) - 1;
   const int words = (t.num_pages + 31) / 32;
-  auto length_of = [&](int r) { return min(max(t.lengths[r], 0), t.max_pages << t.page_shift); };
-  auto parent_of = [&](int r) {
-    const int p = parents[r];
-    return p >= 0 && p < t.rows ? p : -1;
-  };
   auto real = [&](int page) { return page >= 0 && page < t.num_pages; };
 
+  for (int r = tid; r < t.rows; r += kReorderThreads) {
+    const int p = parents[r];
+    parent_s[r] = p >= 0 && p < t.rows ? p : -1;
+    length_s[r] = min(max(t.lengths[r], 0), t.max_pages << t.page_shift);
+  }
   for (int i = me; i < words; i += all) marks[i] = 0u;
+  __syncthreads();
   // (1) a warp a row
   for (int r = warp; r < t.rows; r += warps) {
-    const int p = parent_of(r);
-    const int len = p >= 0 ? length_of(p) : 0, full = len >> t.page_shift;
+    const int p = parent_s[r];
+    const int len = p >= 0 ? length_s[p] : 0, full = len >> t.page_shift;
     const bool part = (len & page_mask) != 0;
-    bool fresh = false;
-    if (part) {                                                   // a lower child of the same parent has the page already
-      for (int c0 = 0; c0 < r && !fresh; c0 += 32) fresh = __any_sync(0xffffffffu, c0 + lane < r && parents[c0 + lane] == p);
-    }
     const int* from = t.block_tables + (int64_t)max(p, 0) * t.max_pages;
     const int* was = t.block_tables + (int64_t)r * t.max_pages;
-    const int held = (length_of(r) + page_mask) >> t.page_shift;
+    const int held = (length_s[r] + page_mask) >> t.page_shift;
     int* to = scratch + (int64_t)r * t.max_pages;
+    bool fresh = false;                                           // a lower child of the same parent has the page already
+    if (part)
+      for (int c0 = 0; c0 < r && !fresh; c0 += 32) fresh = __any_sync(0xffffffffu, c0 + lane < r && parent_s[c0 + lane] == p);
     const int blocks = full + (part ? 1 : 0);
     for (int b = lane; b < t.max_pages; b += 32) {
       const int page = b < blocks ? from[b] : -1;
@@ -353,8 +366,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
   cluster.sync();
   // (2)
   for (int r = warp; r < t.rows; r += warps) {
-    const int held = (length_of(r) + page_mask) >> t.page_shift;
-    const int p = parent_of(r), len = p >= 0 ? length_of(p) : 0, full = len >> t.page_shift;
+    const int held = (length_s[r] + page_mask) >> t.page_shift;
+    const int p = parent_s[r], len = p >= 0 ? length_s[p] : 0, full = len >> t.page_shift;
     const int blocks = full + ((len & page_mask) != 0 && __ldcg(info + r) == 0 ? 1 : 0);
     const int* was = t.block_tables + (int64_t)r * t.max_pages;
     const int* now = scratch + (int64_t)r * t.max_pages;
@@ -381,8 +394,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
     int used = 0, n_moved = 0;
     for (int c0 = 0; c0 < t.rows; c0 += kReorderThreads) {
       const int r = c0 + tid;
-      const int p = r < t.rows ? parent_of(r) : -1;
-      const int len = p >= 0 ? length_of(p) : 0, full = len >> t.page_shift;
+      const int p = r < t.rows ? parent_s[r] : -1;
+      const int len = p >= 0 ? length_s[p] : 0, full = len >> t.page_shift;
       const bool fresh = r < t.rows && __ldcg(info + r) != 0;
       const bool changes = len > 0 && (p != r || fresh);
       int n[2] = {fresh ? 1 : 0, changes ? 1 : 0}, total[2];
@@ -429,50 +442,56 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
   for (int64_t i = me; i < n; i += all) t.block_tables[i] = __ldcg(scratch + i);
 }
 
-// The history of the rows of `moved`: a CTA gathers 4 UNITS keys of one group over all rows, through shared memory, since a row
-// can be read and written: first everything is read, then everything is written.
+// The rows of `moved` in one layer.  The first history_ctas CTAs gather the history, 4 UNITS keys of one group over all rows, through shared
+// memory, since a row can be read and written: first everything is read, then everything is written.  The others copy the tokens
+// of the pages that are being filled into the pages that the copies got: kPagePieces CTAs a row and pool.
+// Bound by memory: 256 rows, half of them with a page of 64 tokens x 16 heads, two thirds with 16 histories of 1,500 keys.
+constexpr int kPagePieces = 4;
 template <int UNITS>
-__global__ void __launch_bounds__(256) move_history_kernel(const int4* __restrict__ moved, float* selected, int groups, int64_t capacity) {
+__global__ void __launch_bounds__(256) move_kernel(const int4* __restrict__ moved, const int2* __restrict__ copies, float* selected, int groups,
+                                                   int64_t capacity, int chunks, int history_ctas, uint4* k_pages, uint4* v_pages, int heads,
+                                                   int num_pages, int64_t head_units, int row_units) {
   tc::after_previous_kernel();
   extern __shared__ float4 keep[];
-  const int n = moved[0].x, g = blockIdx.y, unit = threadIdx.x % UNITS;
-  const int64_t j = ((int64_t)blockIdx.x * UNITS + unit) * 4;       // capacity is a multiple of 16: whole units
-  for (int m = threadIdx.x / UNITS; m < n; m += 256 / UNITS) {
-    const int4 x = moved[1 + m];
-    if (j < x.z && j < capacity) keep[m * UNITS + unit] = *reinterpret_cast<const float4*>(selected + ((int64_t)x.y * groups + g) * capacity + j);
-  }
-  __syncthreads();
-  for (int m = threadIdx.x / UNITS; m < n; m += 256 / UNITS) {
-    const int4 x = moved[1 + m];
-    if (j >= x.z || j >= capacity) continue;
-    const float4 v = keep[m * UNITS + unit];
-    float* to = selected + ((int64_t)x.x * groups + g) * capacity + j;
-    if (j + 4 <= x.z) {
-      *reinterpret_cast<float4*>(to) = v;
-    } else {                                                      // behind the row's last token nothing is written
-      to[0] = v.x;
-      if (j + 1 < x.z) to[1] = v.y;
-      if (j + 2 < x.z) to[2] = v.z;
-    }
-  }
-}
-
-// The tokens of the pages that are being filled, into the pages that their copies got.
-__global__ void __launch_bounds__(256) move_pages_kernel(const int4* __restrict__ moved, const int2* __restrict__ copies, uint4* k_pages,
-                                                         uint4* v_pages, int heads, int num_pages, int64_t head_units, int row_units) {
-  tc::after_previous_kernel();
   const int n = moved[0].x;
+  if ((int)blockIdx.x < history_ctas) {
+    const int g = blockIdx.x / chunks, unit = threadIdx.x % UNITS;
+    const int64_t j = ((int64_t)(blockIdx.x - g * chunks) * UNITS + unit) * 4;       // capacity is a multiple of 16: whole units
+#pragma unroll 4
+    for (int m = threadIdx.x / UNITS; m < n; m += 256 / UNITS) {
+      const int4 x = moved[1 + m];
+      if (j < x.z && j < capacity) keep[m * UNITS + unit] = *reinterpret_cast<const float4*>(selected + ((int64_t)x.y * groups + g) * capacity + j);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int m = threadIdx.x / UNITS; m < n; m += 256 / UNITS) {
+      const int4 x = moved[1 + m];
+      if (j >= x.z || j >= capacity) continue;
+      const float4 v = keep[m * UNITS + unit];
+      float* to = selected + ((int64_t)x.x * groups + g) * capacity + j;
+      if (j + 4 <= x.z) {
+        *reinterpret_cast<float4*>(to) = v;
+      } else {                                                      // behind the row's last token nothing is written
+        to[0] = v.x;
+        if (j + 1 < x.z) to[1] = v.y;
+        if (j + 2 < x.z) to[2] = v.z;
+      }
+    }
+    return;
+  }
   const int64_t page_units = head_units * heads;
-  for (int m = blockIdx.x; m < n; m += gridDim.x) {
+  const int piece = (blockIdx.x - history_ctas) % (2 * kPagePieces), ctas = (gridDim.x - history_ctas) / (2 * kPagePieces);
+  uint4* pool = piece < kPagePieces ? k_pages : v_pages;
+  for (int m = (blockIdx.x - history_ctas) / (2 * kPagePieces); m < n; m += ctas) {
     const int4 x = moved[1 + m];
     if (x.w == 0) continue;
     const int2 c = copies[x.x];
     if (c.x < 0 || c.x >= num_pages || c.y < 0 || c.y >= num_pages) continue;
     const int units = x.w * row_units;                            // of one head
-    uint4* pool = blockIdx.y == 0 ? k_pages : v_pages;
-    const uint4* from = pool + c.x * page_units;
-    uint4* to = pool + c.y * page_units;
-    for (int i = blockIdx.z * blockDim.x + threadIdx.x; i < units * heads; i += gridDim.z * blockDim.x) {
+    const uint4* __restrict__ from = pool + c.x * page_units;
+    uint4* __restrict__ to = pool + c.y * page_units;
+#pragma unroll 4
+    for (int i = piece % kPagePieces * 256 + threadIdx.x; i < units * heads; i += kPagePieces * 256) {
       const int h = i / units, u = i - h * units;
       to[h * head_units + u] = from[h * head_units + u];
     }
@@ -541,28 +560,28 @@ size_t reorder_work_words(int rows, int max_pages, int num_pages) { return Reord
 int reorder(const Tables& t, const int* parents, int* copies, int* work, cudaStream_t s) {
   const ReorderWork w(t.rows, t.max_pages, t.num_pages);
   count_launch();
-  reorder_kernel<<<kCluster, kReorderThreads, 0, s>>>(t, parents, copies, work + w.moved, work + w.info,
-                                                      reinterpret_cast<unsigned*>(work + w.marks), work + w.scratch);
+  const size_t smem = 2 * (size_t)t.rows * 4;
+  SA_CUDA_CHECK(allow_smem(reorder_kernel, smem));
+  reorder_kernel<<<kCluster, kReorderThreads, smem, s>>>(t, parents, copies, work + w.moved, work + w.info,
+                                                         reinterpret_cast<unsigned*>(work + w.marks), work + w.scratch);
   SA_CUDA_CHECK(cudaGetLastError());
   return SA_OK;
 }
 
 int move_rows(const Tables& t, const int* copies, const int* work, int groups, int head_dim, int elem_bytes, int64_t capacity, void* k_pages,
               void* v_pages, float* selected, cudaStream_t s) {
-  const int4* moved = reinterpret_cast<const int4*>(work);
+  const int row_units = head_dim * elem_bytes / 16;
   // 32 keys a CTA (a line of every row), or 8 where the rows would not fit the shared memory
-  auto history = [&](auto kernel, int units) -> int {
+  auto move = [&](auto kernel, int units) -> int {
     const size_t smem = (size_t)t.rows * units * sizeof(float4);
     SA_CUDA_CHECK(allow_smem(kernel, smem));
-    const unsigned chunks = (unsigned)((capacity + 4 * units - 1) / (4 * units));
-    return launch_after(kernel, dim3(chunks, groups), 256, smem, s, moved, selected, groups, capacity);
+    const int chunks = (int)((capacity + 4 * units - 1) / (4 * units));
+    const unsigned history = (unsigned)chunks * groups, pages = (unsigned)min(t.rows, 256) * 2 * kPagePieces;
+    return launch_after(kernel, dim3(history + pages), 256, smem, s, reinterpret_cast<const int4*>(work), reinterpret_cast<const int2*>(copies),
+                        selected, groups, capacity, chunks, (int)history, static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), t.heads,
+                        t.num_pages, (int64_t)row_units << t.page_shift, row_units);
   };
-  int st = t.rows <= 1024 ? history(move_history_kernel<8>, 8) : history(move_history_kernel<2>, 2);
-  if (st != SA_OK) return st;
-  const int row_units = head_dim * elem_bytes / 16;
-  return launch_after(move_pages_kernel, dim3(min(t.rows, 512), 2, 2), 256, 0, s, moved, reinterpret_cast<const int2*>(copies),
-                      static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), t.heads, t.num_pages,
-                      (int64_t)row_units << t.page_shift, row_units);
+  return t.rows <= 1024 ? move(move_kernel<8>, 8) : move(move_kernel<2>, 2);
 }
 
 }  // namespace paged

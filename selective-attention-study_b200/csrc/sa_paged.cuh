@@ -92,7 +92,8 @@ struct AttentionScratch {
   int64_t key_stride;                 // keys of a checkpoint row
 };
 AttentionScratch attention_scratch(const Attention& a);
-int decode(const Attention& a, cudaStream_t s);
+// `beside`: launched behind tiles() of the same call, and runs while that still does.
+int decode(const Attention& a, bool beside, cudaStream_t s);
 int tiles(const Attention& a, cudaStream_t s);
 
 // ---- launches (sa_paged.cu) ---------------------------------------------------------------------------------------------

@@ -131,11 +131,10 @@ int sa_paged_run(const sa_paged_attention* in) {
   cudaStream_t s = static_cast<cudaStream_t>(in->stream);
   // Rows of two tokens or more go through the tile kernels, rows of one through the single-token kernel; the step's bounds say
   // where there can be none of either.
-  if (a.max_count > 1) {
-    st = paged::tiles(a, s);
-    if (st != SA_OK || paged::tile_tokens(a.rows, a.total, a.max_count) == 1) return st;
-  }
-  return paged::decode(a, s);
+  if (a.max_count == 1) return paged::decode(a, false, s);
+  st = paged::tiles(a, s);
+  if (st != SA_OK || paged::tile_tokens(a.rows, a.total, a.max_count) == 1) return st;
+  return paged::decode(a, true, s);
 }
 
 unsigned long long sa_stream_capture(void* stream) {
@@ -161,6 +160,7 @@ int sa_beam_select(const sa_beam* in) {
   if (!in->logits || !in->scores || !in->out_scores || !in->out_rows || !in->out_tokens || !in->workspace) return SA_ERR_BAD_ARGUMENT;
   if (!aligned(in->logits, in->dtype == SA_F32 ? 4 : 2) || !aligned(in->workspace, 16) || !aligned(in->out_tokens, 8)) return SA_ERR_ALIGNMENT;
   if (in->workspace_bytes < beam::workspace_bytes(in->dtype, in->groups, in->beams, in->vocab, in->width)) return SA_ERR_WORKSPACE;
+  if (tc::timeout_pending()) return SA_ERR_DEVICE_TIMEOUT;
   const beam::Select p{in->dtype, in->groups, in->beams, in->vocab, in->width, in->logits, in->group_stride, in->beam_stride, in->scores,
                        in->out_scores, in->out_rows, reinterpret_cast<long long*>(in->out_tokens), in->workspace};
   return beam::select(p, static_cast<cudaStream_t>(in->stream));

@@ -60,10 +60,20 @@ __global__ void __launch_bounds__(kAllThreads) decode_pages_kernel(
     __nv_bfloat16* k_pages, __nv_bfloat16* v_pages, float* selected, int64_t sel_stride, const int* __restrict__ tables, int max_pages,
     int num_pages, int page_shift, int box_rows, const int* __restrict__ header, const DecodeItem* __restrict__ items, int items_max,
     float* __restrict__ partial, float* __restrict__ sel_new, int64_t new_stride, unsigned int* tickets, int heads, int groups, int exempt,
-    float scale, const int64_t* __restrict__ slots, int total, __nv_bfloat16* __restrict__ y, tc::WaitCtx status) {
+    float scale, const int64_t* __restrict__ slots, int total, __nv_bfloat16* __restrict__ y, tc::WaitCtx status, bool beside) {
   constexpr int DK = D / 64, KB = D / 16;
   constexpr int kStageBytes = 2 * DK * kTileBytes;                // K, then V
-  tc::after_previous_kernel();
+  if (!beside) {
+    tc::after_previous_kernel();
+  } else {
+    // The kernel before is that of the same call's tiles, which this one needs nothing of: it has let this one begin once
+    // everything before it was there.  One block more waits for its end, so that what comes after both waits for both.
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (blockIdx.x == (unsigned)items_max * heads) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      return;
+    }
+  }
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kStages], empty[kStages];
@@ -73,7 +83,7 @@ __global__ void __launch_bounds__(kAllThreads) decode_pages_kernel(
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // tokens that no row was given: zeros
-  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+  for (int i = blockIdx.x; i < total && !beside; i += gridDim.x) {
     if (slots[i] >= 0) continue;
     for (int u = tid; u < heads * D / 8; u += kAllThreads) reinterpret_cast<uint4*>(y + (int64_t)i * heads * D)[u] = make_uint4(0u, 0u, 0u, 0u);
   }
@@ -317,7 +327,7 @@ __global__ void __launch_bounds__(kAllThreads) decode_pages_kernel(
 }
 
 template <int D>
-int decode_impl(const Attention& a, cudaStream_t s) {
+int decode_impl(const Attention& a, bool beside, cudaStream_t s) {
   const StepLayout l = step_layout(a.rows, a.total, a.heads);
   const AttentionScratch w = attention_scratch(a);
   const int page = 1 << a.page_shift, box_rows = min(page, kStageKeys);
@@ -330,14 +340,14 @@ int decode_impl(const Attention& a, cudaStream_t s) {
   st = tc::wait_ctx(&status);
   if (st != SA_OK) return st;
   int* tickets = a.plan_tickets ? a.work + l.tickets : reinterpret_cast<int*>(a.workspace + w.own_tickets);
-  if (!a.plan_tickets) SA_CUDA_CHECK(cudaMemsetAsync(tickets, 0, (size_t)l.tickets_count * 4, s));
+  if (!a.plan_tickets && !beside) SA_CUDA_CHECK(cudaMemsetAsync(tickets, 0, (size_t)l.tickets_count * 4, s));
   auto kernel = decode_pages_kernel<D>;
   SA_CUDA_CHECK(allow_smem(kernel, smem_bytes<D>()));
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)l.decode_items_max * a.heads);
+  config.gridDim = dim3((unsigned)l.decode_items_max * a.heads + (beside ? 1 : 0));
   config.blockDim = dim3(kAllThreads);
   config.dynamicSmemBytes = smem_bytes<D>();
   config.stream = s;
@@ -352,14 +362,14 @@ int decode_impl(const Attention& a, cudaStream_t s) {
       static_cast<bf16*>(a.k_pages), static_cast<bf16*>(a.v_pages), a.selected, a.sel_stride, a.block_tables, a.max_pages, a.num_pages,
       a.page_shift, box_rows, (const int*)a.work, reinterpret_cast<const DecodeItem*>(a.work + l.decode_items), l.decode_items_max,
       a.workspace + w.partial, a.workspace + w.sel_new, w.key_stride, reinterpret_cast<unsigned*>(tickets), a.heads, a.groups, a.exempt,
-      1.0f / sqrtf((float)D), a.slots, a.total, static_cast<bf16*>(a.y), status));
+      1.0f / sqrtf((float)D), a.slots, a.total, static_cast<bf16*>(a.y), status, beside));
   return SA_OK;
 }
 
 }  // namespace
 
-int decode(const Attention& a, cudaStream_t s) {
-  return a.head_dim == 64 ? decode_impl<64>(a, s) : a.head_dim == 128 ? decode_impl<128>(a, s) : SA_ERR_UNSUPPORTED;
+int decode(const Attention& a, bool beside, cudaStream_t s) {
+  return a.head_dim == 64 ? decode_impl<64>(a, beside, s) : a.head_dim == 128 ? decode_impl<128>(a, beside, s) : SA_ERR_UNSUPPORTED;
 }
 
 }  // namespace paged

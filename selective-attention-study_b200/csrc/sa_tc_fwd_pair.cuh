@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
   constexpr int D = 64;
   paged::TileItem item{};
   if constexpr (PAGED) {
-    after_previous_kernel();
+    after_previous_kernel_first();
     if ((int)(blockIdx.x / (unsigned)(heads / 2)) >= paged.header[paged::kTileItems]) return;
     item = paged.items[blockIdx.x / (unsigned)(heads / 2)];
     seq = item.length;
@@ -141,11 +141,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
     if (warp == 13) {
       // ============================================ TMA loads =============================================
       if (PAGED || lane == 0) {
-        // PAGED: a lane a box of the tile; its page of the tile after is fetched with each load (`page`: of the next tile of K,
-        // V or K0, which two heads share), so that no load waits for the table.
+        // PAGED: a lane a box of the tile; its page of the tile after is fetched with each load (`page`: of the next tile of K
+        // or V, which two heads share), so that no load waits for the table.
         const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
-        int page_k = -1, page_v = -1, page_k0 = -1;
-        if constexpr (PAGED) page_k = page_v = page_k0 = boxes.page(i0, seq, lane);
+        int page_k = -1, page_v = -1;
+        if constexpr (PAGED) page_k = page_v = boxes.page(i0, seq, lane);
         auto load = [&](int off, const CUtensorMap* map, int id, int row, int head, int page) {
           if constexpr (PAGED) {
             const int used = boxes.count(row, seq);
@@ -168,8 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
           tma_load_4d(smem + L::q, &map_q, &bars[QF], 0, q_row, h0, b);
           tma_load_4d(smem + L::q + kRowTile, &map_q, &bars[QF], 0, q_row, h0 + 1, b);
         }
-        load(L::k0, &map_k0, LDK0, i0, 0, page_k0);
-        next_page(page_k0, mi - 1);
+        if (!PAGED) load(L::k0, &map_k0, LDK0, i0, 0, -1);
         // Tile n of the K and V rings: step n / 2 of head n & 1.  K runs one tile ahead of V.
         const int tiles = 2 * steps;
         int nj_k = mi, nj_v = mi, nj_k0 = mi;
@@ -194,11 +193,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
               next_page(page_v, nj_v);
             }
           }
-          if ((n & 1) && (n >> 1) + 1 < steps) {               // K0 of the next step, once this step's L0 is done
+          if (!PAGED && (n & 1) && (n >> 1) + 1 < steps) {     // K0 of the next step, once this step's L0 is done
             wait(bar(L0F), (uint32_t)((n >> 1) & 1), 503);
             nj_k0 = step_back(nj_k0);
-            load(L::k0, &map_k0, LDK0, nj_k0 * kTile, 0, page_k0);
-            next_page(page_k0, nj_k0 - 1);
+            load(L::k0, &map_k0, LDK0, nj_k0 * kTile, 0, -1);
           }
         }
       }
@@ -268,6 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
           mma_commit(bar(FF));
         }
         __syncwarp();
+      }
+    } else if (PAGED && warp == 15) {
+      // ===================== K0 in pages: not behind the boxes of K and V, which a step waits for less ===================
+      const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
+      int page = boxes.page(i0, seq, lane);
+#pragma unroll 1
+      for (int t = 0; t < steps; ++t) {
+        const int j0 = i0 - t * kTile, used = boxes.count(j0, seq);
+        if (t > 0) wait(bar(L0F), (uint32_t)((t - 1) & 1), 504);     // L0 of the step before is done
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(&bars[LDK0], used * paged.box_rows * 128);
+        __syncwarp();
+        if (lane < used) tma_load_4d(smem + L::k0 + lane * paged.box_rows * 128, &map_k0, &bars[LDK0], 0, boxes.at(j0, lane), 0, page);
+        page = boxes.page(j0 - kTile, seq, lane);
       }
     } else if (warp < 12) {
       // ================================= selection: relu(L0) under the mask, the carry ========================

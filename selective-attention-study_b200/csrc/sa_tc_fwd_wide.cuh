@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 
   paged::TileItem item{};
   if constexpr (PAGED) {
-    after_previous_kernel();
+    after_previous_kernel_first();
     if ((int)(blockIdx.x / (unsigned)heads) >= paged.header[paged::kTileItems]) return;
     item = paged.items[blockIdx.x / (unsigned)heads];
     seq = item.length;

@@ -32,11 +32,12 @@ struct TokenRows {
 // A unit is 16 bytes of one token's K or V; heads * units of a token are neighbours.
 __global__ void __launch_bounds__(256) store_kernel(TokenRows k, TokenRows v, uint4* k_pages, uint4* v_pages, uint4* y,
                                                     const int64_t* __restrict__ slots, int total, int heads, int row_units, int num_pages,
-                                                    int page_shift, unsigned int* tickets, int n_tickets) {
+                                                    int page_shift, unsigned int* tickets, int n_tickets, unsigned int* more_tickets,
+                                                    int n_more) {
   after_previous_kernel();
   const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
-  if (tickets != nullptr)
-    for (int64_t i = first; i < n_tickets; i += step) tickets[i] = 0u;
+  for (int64_t i = first; i < n_tickets; i += step) tickets[i] = 0u;
+  for (int64_t i = first; i < n_more; i += step) more_tickets[i] = 0u;
   const int per_token = heads * row_units;
   const int64_t n = (int64_t)total * per_token, slots_end = (int64_t)num_pages << page_shift;
   for (int64_t i = first; i < n; i += step) {
@@ -263,7 +264,7 @@ int tiles_impl(const Attention& a, cudaStream_t s) {
   if (st != SA_OK) return st;
 
   unsigned int* const walk_tickets = reinterpret_cast<unsigned int*>(a.workspace + w.tickets);
-  // store: also clears the walks' tickets
+  // store: also clears the tickets of this call, the walks' and (where they are not the plan's) the single tokens'
   const int n_walk = l.tiles_max * a.heads;
   {
     const TokenRows k{static_cast<const uint4*>(a.k), a.k_stride[0] / 8, a.k_stride[1] / 8};
@@ -271,7 +272,8 @@ int tiles_impl(const Attention& a, cudaStream_t s) {
     const int64_t units = (int64_t)a.total * a.heads * (D / 8);
     const unsigned blocks = (unsigned)max((int64_t)1, min((units + 255) / 256, (int64_t)8 * kSms));
     st = launch(store_kernel, dim3(blocks), 256, 0, true, s, k, v, static_cast<uint4*>(a.k_pages), static_cast<uint4*>(a.v_pages),
-                static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk);
+                static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk,
+                reinterpret_cast<unsigned int*>(a.workspace + w.own_tickets), a.plan_tickets ? 0 : l.tickets_count);
     if (st != SA_OK) return st;
   }
   PagedWalk walk{};

@@ -155,6 +155,13 @@ __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The same in the other order: the next kernel may be launched once this one has everything before it, so a kernel that needs
+// nothing from this one has it too.
+__device__ __forceinline__ void after_previous_kernel_first() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+
 // ---- fences -------------------------------------------------------------------------------------------
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }

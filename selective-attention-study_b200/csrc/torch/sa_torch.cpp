@@ -422,7 +422,13 @@ void check_int32(const Tensor& x, const PageTables& t, int64_t n, const char* wh
                     what, " must be a contiguous int32 CUDA tensor of ", n, " numbers on the tables' device");
 }
 
-// (query_start, cached, slots, work, max_length, max_count, stream, capture): the step, its bounds, and where it was made
+// A step as paged.append_tokens made it: its plan, its bounds, and the stream and capture that it was made on.
+struct PageStep {
+  Tensor query_start, cached, slots, work;
+  int64_t max_length, max_count;
+  uint64_t stream, capture;
+};
+
 pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t total, int64_t max_length, int64_t max_count) {
   const sa_page_tables p = tables_of(t);
   check_int32(counts, t, p.rows, "counts");
@@ -439,15 +445,10 @@ pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t
   check("sa_page_append", sa_page_append(&p, counts.data_ptr<int32_t>(), (int)total, (int)max_length, (int)max_count,
                                          query_start.data_ptr<int32_t>(), cached.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
                                          work.data_ptr<int32_t>(), stream));
-  return pybind11::make_tuple(query_start, cached, slots, work, max_length, max_count, reinterpret_cast<uint64_t>(stream),
-                              (uint64_t)sa_stream_capture(stream));
+  return pybind11::make_tuple(query_start, cached, slots,
+                              PageStep{query_start, cached, slots, work, max_length, max_count, reinterpret_cast<uint64_t>(stream),
+                                       (uint64_t)sa_stream_capture(stream)});
 }
-
-struct PageStep {                                  // paged.append_tokens
-  Tensor query_start, cached, slots, work;
-  int64_t max_length, max_count;
-  uint64_t stream, capture;
-};
 
 void check_pools(const PageTables& t, const sa_page_tables& p, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
   TORCH_CHECK_VALUE(kc.dim() == 4 && kc.size(0) == p.num_pages && kc.size(1) == p.heads && kc.size(2) == p.page_size && vc.sizes() == kc.sizes(),
@@ -572,8 +573,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("decode", &decode);
   pybind11::class_<PageTables>(m, "PageTables")
       .def(pybind11::init<Tensor, Tensor, Tensor, Tensor, Tensor, int64_t, int64_t>());
-  pybind11::class_<PageStep>(m, "PageStep")
-      .def(pybind11::init<Tensor, Tensor, Tensor, Tensor, int64_t, int64_t, uint64_t, uint64_t>());
+  pybind11::class_<PageStep>(m, "PageStep");
   m.def("append_tokens", &append_tokens);
   m.def("paged_attention", &paged_attention, nogil());
   m.def("reorder_rows", &reorder_rows);

