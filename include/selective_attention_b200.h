@@ -365,7 +365,8 @@ typedef struct sa_page_tables {
  *                table, or the pool -- then nor does any later row that needs a page)
  *   slots        (total) int64: page * page_size + offset of a token; -1: no row's, or a row that is left as it was
  *   work         sa_page_step_words() int32 words, 16-byte aligned: the plan of the step's attention
- * The k-th page that is needed, in row order, is free_pages[free_count - 1 - k]. */
+ * The k-th page that is needed, in row order, is free_pages[free_count - 1 - k].  A call that returns an error leaves the tables as
+ * they were. */
 size_t sa_page_step_words(int rows, int total, int heads);
 int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int total, int max_length, int max_count, int32_t* query_start,
                    int32_t* cached, int64_t* slots, int32_t* work, void* stream);
@@ -378,7 +379,7 @@ int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int tota
  *   y                 (total, heads, head_dim) contiguous; zeros for tokens without a slot
  *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream); 0: the call
  *                     clears tickets of its own
- * A page outside the pool reads as zeros. */
+ * A page outside the pool reads as zeros.  A call that returns an error leaves the histories as they were. */
 typedef struct sa_paged_attention {
   int32_t struct_bytes;   /* sizeof(sa_paged_attention) */
   int32_t groups, head_dim, exempt, total, max_length, max_count, plan_tickets;

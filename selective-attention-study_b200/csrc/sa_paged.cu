@@ -78,13 +78,19 @@ struct RowSums {
       : start(at), page(at + rows + 1), tile(at + 2 * (rows + 1)), piece(at + 3 * (rows + 1)), before(at + 4 * (rows + 1)) {}
 };
 
-// Everything that is per page, per tile or per token, by a search in the sums: the caller takes every `step`-th from `first` on.
+// Everything that is per page, per tile or per token, by a search in the sums, and all that changes the tables (a step whose second
+// launch fails leaves them as they were): the caller takes every `step`-th from `first` on.
 __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const int* header, int first, int step) {
   const Tables& t = a.t;
   const int page_mask = (1 << t.page_shift) - 1;
   const int free_before = header[kFreeBefore], wanted = header[kPagesWanted], n_tiles = header[kTiles], n_single = header[kDecodeItems];
   const int piece_keys = header[kPieceKeys];
   const bool cut = header[kCut] != 0;
+  if (first == 0) *t.free_count = header[kFreeAfter];
+  for (int r = first; r < t.rows; r += step) {
+    const int count = s.start[r + 1] - s.start[r];
+    if (s.before[r] >= 0 && count > 0) t.lengths[r] = s.before[r] + count;
+  }
   for (int i = first; i < a.layout.tickets_count; i += step) a.work[a.layout.tickets + i] = 0;
   for (int k = first; k < wanted; k += step) {                    // off the end of the free list
     const int r = row_of(s.page, t.rows, k);
@@ -192,7 +198,6 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       if (r < t.rows) {
         sums.before[r] = fits[u] ? before[u] : -1;
         a.cached[r] = fits[u] ? before[u] : -1;
-        if (fits[u] && count[u] > 0) t.lengths[r] = before[u] + count[u];
       }
       if (!fits[u]) count[u] = 0;
       else next[4] += need[u];
@@ -249,8 +254,8 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       header[kPieceKeys] = piece_keys;
       header[kPagesWanted] = min(sums.page[t.rows], free_count);     // of the rows that are served: those up to the first that is not
       header[kFreeBefore] = free_count;
+      header[kFreeAfter] = free_count - (int)next_total[4];
       header[kCut] = cut;
-      *t.free_count = free_count - (int)next_total[4];
     }
   }
   __syncthreads();                                               // the sums, and who is served

@@ -17,7 +17,8 @@ struct Tables {
 
 // ---- the plan of a step: int32 words that sa_page_append writes and the attention over pages reads ------------------------
 // header | sums over the rows | first tile of every row | tiles | tile items | decode items | tickets (zero between launches)
-enum : int { kTiles = 0, kTileItems = 1, kDecodeItems = 2, kPieceKeys = 3, kPagesWanted = 4, kFreeBefore = 5, kCut = 6, kHeaderWords = 16 };
+enum : int { kTiles = 0, kTileItems = 1, kDecodeItems = 2, kPieceKeys = 3, kPagesWanted = 4, kFreeBefore = 5, kFreeAfter = 6, kCut = 7,
+             kHeaderWords = 16 };
 
 // One walk over the keys of a 128-query tile: key tiles from the diagonal back, cut into `pieces` (which stand together).
 struct TileItem {
@@ -94,7 +95,9 @@ struct AttentionScratch {
 AttentionScratch attention_scratch(const Attention& a);
 // `beside`: launched behind tiles() of the same call, and runs while that still does.
 int decode(const Attention& a, bool beside, cudaStream_t s);
-int tiles(const Attention& a, cudaStream_t s);
+// `moved` is set once the histories have been moved on; a call that fails after that puts them back.
+int tiles(const Attention& a, bool* moved, cudaStream_t s);
+int restore_histories(const Attention& a, cudaStream_t s);
 
 // ---- launches (sa_paged.cu) ---------------------------------------------------------------------------------------------
 int append(const Tables& t, const int* counts, int total, int max_length, int max_count, int* query_start, int* cached, int64_t* slots,

@@ -132,9 +132,14 @@ int sa_paged_run(const sa_paged_attention* in) {
   // Rows of two tokens or more go through the tile kernels, rows of one through the single-token kernel; the step's bounds say
   // where there can be none of either.
   if (a.max_count == 1) return paged::decode(a, false, s);
-  st = paged::tiles(a, s);
-  if (st != SA_OK || paged::tile_tokens(a.rows, a.total, a.max_count) == 1) return st;
-  return paged::decode(a, true, s);
+  bool moved = false;
+  st = paged::tiles(a, &moved, s);
+  if (st == SA_OK && paged::tile_tokens(a.rows, a.total, a.max_count) > 1) st = paged::decode(a, true, s);
+  if (st != SA_OK && moved) {            // a call that fails leaves the histories as they were
+    const int back = paged::restore_histories(a, s);
+    if (back != SA_OK) return back;
+  }
+  return st;
 }
 
 unsigned long long sa_stream_capture(void* stream) {

@@ -227,6 +227,15 @@ __global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t k
   *sel = run;
 }
 
+// The histories of the rows that have tiles as they were before scan_pages_kernel: what their first tile starts from.
+__global__ void __launch_bounds__(256) restore_kernel(const float* __restrict__ carry, int64_t key_stride, const int* __restrict__ tile_start,
+                                                      const TileItem* __restrict__ tiles, int groups, float* selected, int64_t sel_stride) {
+  const int r = blockIdx.z, g = blockIdx.y, t0 = tile_start[r];
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  if (tile_start[r + 1] == t0 || j >= tiles[t0].cached) return;
+  selected[((int64_t)r * groups + g) * sel_stride + j] = carry[((int64_t)t0 * groups + g) * key_stride + j];
+}
+
 template <typename... Args>
 int launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t s, Args... args) {
   SA_CUDA_CHECK(allow_smem(kernel, smem));
@@ -246,7 +255,7 @@ int launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, bool ov
 }
 
 template <int D>
-int tiles_impl(const Attention& a, cudaStream_t s) {
+int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   constexpr int DK = D / 64;
   const paged::StepLayout l = paged::step_layout(a.rows, a.total, a.heads);
   const paged::AttentionScratch w = paged::attention_scratch(a);
@@ -302,6 +311,7 @@ int tiles_impl(const Attention& a, cudaStream_t s) {
     st = launch(scan_pages_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, true, s, carry, w.key_stride,
                 (const int*)(a.work + l.tile_start), tiles, a.groups, a.selected, a.sel_stride);
     if (st != SA_OK) return st;
+    *moved = true;
   }
   // Two heads a CTA, or one: as over contiguous caches (sa_tc_fwd.cu), by the tiles that there are at least, since the plan's
   // number is on the device.  Where there may be few, the plan may have cut their walks.
@@ -353,8 +363,16 @@ AttentionScratch attention_scratch(const Attention& a) {
   return w;
 }
 
-int tiles(const Attention& a, cudaStream_t s) {
-  return a.head_dim == 64 ? tc::tiles_impl<64>(a, s) : a.head_dim == 128 ? tc::tiles_impl<128>(a, s) : SA_ERR_UNSUPPORTED;
+int tiles(const Attention& a, bool* moved, cudaStream_t s) {
+  return a.head_dim == 64 ? tc::tiles_impl<64>(a, moved, s) : a.head_dim == 128 ? tc::tiles_impl<128>(a, moved, s) : SA_ERR_UNSUPPORTED;
+}
+
+int restore_histories(const Attention& a, cudaStream_t s) {
+  const StepLayout l = step_layout(a.rows, a.total, a.heads);
+  const AttentionScratch w = attention_scratch(a);
+  return tc::launch(tc::restore_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, false, s,
+                    (const float*)(a.workspace + w.carry), w.key_stride, (const int*)(a.work + l.tile_start),
+                    reinterpret_cast<const TileItem*>(a.work + l.tiles), a.groups, a.selected, a.sel_stride);
 }
 
 }  // namespace paged

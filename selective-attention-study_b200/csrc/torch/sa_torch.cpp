@@ -425,7 +425,7 @@ void check_int32(const Tensor& x, const PageTables& t, int64_t n, const char* wh
 // A step as paged.append_tokens made it: its plan, its bounds, and the stream and capture that it was made on.
 struct PageStep {
   Tensor query_start, cached, slots, work;
-  int64_t max_length, max_count;
+  int64_t max_pages, num_pages, page_size, max_length, max_count;
   uint64_t stream, capture;
 };
 
@@ -446,7 +446,7 @@ pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t
                                          query_start.data_ptr<int32_t>(), cached.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
                                          work.data_ptr<int32_t>(), stream));
   return pybind11::make_tuple(query_start, cached, slots,
-                              PageStep{query_start, cached, slots, work, max_length, max_count, reinterpret_cast<uint64_t>(stream),
+                              PageStep{query_start, cached, slots, work, p.max_pages, p.num_pages, p.page_size, max_length, max_count, reinterpret_cast<uint64_t>(stream),
                                        (uint64_t)sa_stream_capture(stream)});
 }
 
@@ -468,11 +468,10 @@ Tensor paged_attention(const PageTables& t, const PageStep& step, const Tensor& 
   const sa_page_tables p = tables_of(t);
   check_pools(t, p, kc, vc, selected);
   const int64_t total = step.slots.numel(), h = p.heads, d = kc.size(3);
-  check_int32(step.query_start, t, p.rows + 1, "the step's query_start");
-  check_int32(step.cached, t, p.rows, "the step's cached");
-  check_int32(step.work, t, (int64_t)sa_page_step_words(p.rows, (int)total, p.heads), "the step's plan");
-  TORCH_CHECK_VALUE(step.slots.is_cuda() && step.slots.device() == kc.device() && step.slots.scalar_type() == at::kLong && step.slots.is_contiguous(),
-                    "the step's slots must be a contiguous int64 CUDA tensor on the tables' device");
+  TORCH_CHECK_VALUE(step.cached.device() == kc.device() && step.cached.numel() == p.rows && step.max_pages == p.max_pages &&
+                        step.num_pages == p.num_pages && step.page_size == p.page_size &&
+                        step.work.numel() == (int64_t)sa_page_step_words(p.rows, (int)total, p.heads),
+                    "the step was made with other tables");
   for (const Tensor* x : {&q_in, &k_in, &v_in}) {
     TORCH_CHECK_VALUE(x->dim() == 3 && x->size(0) == total && x->size(1) == h && x->size(2) == d, "q, k, v must all be (", total, ", ", h, ", ", d,
                       "): the step's tokens; got ", x->sizes());

@@ -278,6 +278,9 @@ def test_arguments_that_are_refused():
         paged.paged_attention(dict(cache, selected=cache["selected"][:, :, :64]), t, step, x, x, x)
     with pytest.raises(ValueError, match="bf16"):
         paged.paged_attention(dict(cache, k=cache["k"].half()), t, step, x, x, x)
+    other = paged.begin_tables(2, 16, 16, 9, 2)
+    with pytest.raises(ValueError, match="other tables"):
+        paged.paged_attention(paged.begin_pages(other, 64), other, step, x, x, x)
     with pytest.raises(ValueError, match="counts"):
         paged.append_tokens(t, _ints([3, 4]).long(), 7)
     with pytest.raises(ValueError, match="counts"):
@@ -413,3 +416,93 @@ def test_histories_behind_the_last_token_stay():
     paged.move_rows(cache, paged.reorder_rows(t, _ints([2, 0, 1])))
     for r, (p, n) in enumerate(((2, 50), (0, 21), (1, 3))):
         assert torch.equal(cache["selected"][r, :, :n], was[p, :, :n]) and torch.equal(cache["selected"][r, :, n:], was[r, :, n:])
+
+
+_REFUSED_LAUNCH = """
+#define _GNU_SOURCE
+#include <dlfcn.h>
+typedef struct { unsigned x, y, z; } dim3_t;
+static int left = -1, failed = 0;             /* launches until one is refused */
+void refuse_launch(int n) { left = n; failed = 0; }
+int cudaLaunchKernel(const void* f, dim3_t g, dim3_t b, void** a, unsigned long smem, void* s) {
+  if (left >= 0 && left-- == 0) return failed = 2;                       /* cudaErrorMemoryAllocation */
+  return ((int (*)(const void*, dim3_t, dim3_t, void**, unsigned long, void*))dlsym(RTLD_NEXT, "cudaLaunchKernel"))(f, g, b, a, smem, s);
+}
+int cudaLaunchKernelExC(const void* c, const void* f, void** a) {
+  if (left >= 0 && left-- == 0) return failed = 2;
+  return ((int (*)(const void*, const void*, void**))dlsym(RTLD_NEXT, "cudaLaunchKernelExC"))(c, f, a);
+}
+int cudaGetLastError(void) {
+  const int e = failed;
+  failed = 0;
+  return e ? e : ((int (*)(void))dlsym(RTLD_NEXT, "cudaGetLastError"))();
+}
+"""
+
+_RETRIED_STEP = """
+import ctypes, sys
+import torch
+from selective_attention_b200 import _lib, paged
+shim = ctypes.CDLL(sys.argv[1])
+g = torch.Generator("cpu").manual_seed(3)
+ints = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+t = paged.begin_tables(3, 1200, 16, 400, 4)
+cache = paged.begin_pages(t, 64, per_head=sys.argv[2] == "per_head")
+tokens = lambda n: [torch.randn(n, 4, 64, generator=g).bfloat16().cuda() for _ in range(3)]
+first = [300, 5, 40]
+paged.paged_attention(cache, t, paged.append_tokens(t, ints(first), sum(first)), *tokens(sum(first)))
+for counts in ([200, 1, 1], [1, 1, 1], [3000, 1, 1]):
+    total, most = sum(counts), max(counts)
+    tables = {k: x.clone() for k, x in t.items() if torch.is_tensor(x)}
+
+    def tried(call, unchanged):
+        before, n = _lib.launch_count(), 0
+        while True:
+            shim.refuse_launch(n)
+            try:
+                out = call()
+                shim.refuse_launch(-1)
+                torch.cuda.synchronize()
+                return out, n
+            except _lib.LibraryError as e:
+                shim.refuse_launch(-1)
+                assert e.status == 5, e
+                torch.cuda.synchronize()
+                unchanged(n)
+                n += 1
+
+    def same_tables(n):
+        assert all(torch.equal(t[k], x) for k, x in tables.items()), n
+
+    step, launches = tried(lambda: paged.append_tokens(t, ints(counts), total, max_count=most), same_tables)
+    assert launches == (2 if total > 2048 else 1), launches
+    history, old = cache["selected"].clone(), step["cached"].tolist()
+
+    def same_history(n):
+        assert all(torch.equal(cache["selected"][r, :, :c], history[r, :, :c]) for r, c in enumerate(old)), n
+
+    x = tokens(total)
+    want = {k: v.clone() for k, v in cache.items()}
+    y = paged.paged_attention(want, t, step, *x)
+    got, launches = tried(lambda: paged.paged_attention(cache, t, step, *x), same_history)
+    assert torch.equal(got, y) and torch.equal(cache["selected"], want["selected"]), counts
+    assert launches == (1 if most == 1 else 5), launches
+print("all tried")
+"""
+
+
+@pytest.mark.parametrize("selectors", ["shared", "per_head"])
+def test_a_step_whose_call_fails_can_be_tried_again(selectors, tmp_path):
+    """Whichever of its launches is refused (by a stand-in for the runtime's launch functions, in a process of its own), the
+    tables and the histories are what they were, and the step counts once when it goes through."""
+    import os
+    import subprocess
+    import sys
+
+    source, shim = tmp_path / "refuse.c", tmp_path / "refuse.so"
+    source.write_text(_REFUSED_LAUNCH)
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(shim), str(source), "-ldl"])
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "selective-attention-study_b200")
+    env = dict(os.environ, LD_PRELOAD=str(shim), PYTHONPATH=os.pathsep.join([package, os.environ.get("PYTHONPATH", "")]))
+    run = subprocess.run([sys.executable, "-c", _RETRIED_STEP, str(shim), selectors], env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "all tried" in run.stdout, run.stdout + run.stderr
