@@ -9,9 +9,10 @@
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
 // Bound by memory where there are many beams, else by the latency of the two launches.
 //
-// The largest of a set, without sorting it: each of the eight warps gives the largest of its lanes' own maxima, about two times
+// The largest of a set, without sorting it: each warp that has elements gives the largest of its lanes' own maxima, about two times
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among
-// themselves.  Where more than kList reach it (equal or masked logits) they are taken one by one.
+// themselves.  Where more than kList reach it, because many are equal to it (masked logits, most often), those above it are ranked
+// and the first of the equal ones are found in order; where that is not so either, they are taken one by one.
 #include "sa_common.cuh"
 #include "sa_beam.cuh"
 #include "sa_tc_ptx.cuh"
@@ -36,32 +37,43 @@ __device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& 
 
 template <typename V, typename I>
 struct Shared {
-  V tops[kThreads / 4];
+  V tops[2 * kMaxWidth];
   V bound;
   Entry<V, I> list[kList];
   int count;
   Entry<V, I> warp_best[kThreads / 32];
 };
 
-// Calls emit(rank, value, index) for the `width` first of the CTA's elements.  `mine` is the largest value of the calling thread's
-// elements (-inf: none); reach(bound, f) calls f(value, index) for those of them that are not below `bound` (no value a NaN).
-// All threads call this; emit is called by any.
-template <typename V, typename I, typename Reach, typename Emit>
-__device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, const Reach& reach, const Emit& emit) {
+__device__ __forceinline__ float warp_max(float x) {
+  float top;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(x));
+  return top;
+}
+__device__ __forceinline__ double warp_max(double x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const double o = __shfl_xor_sync(0xffffffffu, x, s);
+    x = o > x ? o : x;
+  }
+  return x;
+}
+
+// Calls emit(rank, value, index) for the `width` first of the CTA's elements, which the first `warps` warps have.  `mine` is the
+// largest value of the calling thread's (-inf: none).  reach(bound, above, f) calls f(value, index) for the CTA's elements that are
+// not below `bound` (`above`: that are above it), until that says no, one(f) for the calling thread's (no value a NaN).  equal(x, n, f) calls f(k, index) for the first n
+// of the elements that are x, or returns false.  All threads call this; emit is called by any.
+template <typename V, typename I, typename Reach, typename One, typename Equal, typename Emit>
+__device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, V mine, const Reach& reach, const One& one, const Equal& equal,
+                                        const Emit& emit) {
   const int tid = threadIdx.x, lane = tid & 31;
   constexpr V kNone = -INFINITY;
-  constexpr int kWarps = kThreads / 32;
-  const int each = 2 * ((width + kWarps - 1) / kWarps), given = each * kWarps;      // 2 to 8 a warp, at most 64
-  for (int u = 0; u < each; ++u) {
-    V top = mine;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      const V o = __shfl_xor_sync(0xffffffffu, top, s);
-      top = o > top ? o : top;
-    }
+  // of w warps all but the last have 32 lanes' elements (or every lane of all has one): 2 ceil(width / w) of each are enough
+  const int each = min(32, 2 * ((width + warps - 1) / warps)), given = each * warps;      // at most 64 in all
+  for (int u = 0; u < each && (tid >> 5) < warps; ++u) {
+    const V top = warp_max(mine);
     const unsigned at = __ballot_sync(0xffffffffu, mine == top);
     if (lane == __ffs(at) - 1) mine = kNone;                // one of them is done with
-    if (lane == 0) sh.tops[u * kWarps + (tid >> 5)] = top;
+    if (lane == 0) sh.tops[u * warps + (tid >> 5)] = top;
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
@@ -73,12 +85,30 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, con
   }
   __syncthreads();
   const V bound = sh.bound;
-  reach(bound, [&](V x, I i) {
+  reach(bound, false, [&](V x, I i) {
     const int at = atomicAdd(&sh.count, 1);
     if (at < kList) sh.list[at] = Entry<V, I>{x, i};
+    return at <= kList;
   });
   __syncthreads();
-  const int n = sh.count;
+  int n = sh.count;
+  int ties = 0;                                              // of the first `width`, those that are equal to the bound
+  if (n > kList) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    reach(bound, true, [&](V x, I i) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kList) sh.list[at] = Entry<V, I>{x, i};
+      return at <= kList;
+    });
+    __syncthreads();
+    n = sh.count;
+    if (n < width) {
+      ties = width - n;
+      if (!equal(bound, ties, [&](int k, I i) { emit(n + k, bound, i); })) n = kList + 1;
+    }
+  }
   if (n <= kList) {
     if (tid < n) {
       const Entry<V, I> e = sh.list[tid];
@@ -87,7 +117,7 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, con
       for (int u = 0; u < n; ++u) at += before(sh.list[u], e) ? 1 : 0;
       if (at < width) emit(at, e.value, e.index);
     }
-    for (int u = n + tid; u < width; u += kThreads) emit(u, kNone, (I)-1);     // fewer elements than that
+    for (int u = n + ties + tid; u < width; u += kThreads) emit(u, kNone, (I)-1);     // fewer elements than that
     return;
   }
   Entry<V, I> last{INFINITY, -1};                            // one by one
@@ -96,7 +126,7 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, V mine, con
     auto better = [&](const Entry<V, I>& o) {
       if (o.index >= 0 && (best.index < 0 || before(o, best))) best = o;
     };
-    reach(bound, [&](V x, I i) {
+    one([&](V x, I i) {
       const Entry<V, I> e{x, i};
       if (w == 0 || before(last, e)) better(e);
     });
@@ -156,6 +186,7 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
   __shared__ uint64_t arrived[kParts];
   __shared__ Shared<float, int> sh;
   __shared__ float red[2][kThreads / 32];
+  __shared__ int sums_s[kThreads / 32];
   const int n = blockIdx.x / chunks, chunk = blockIdx.x - n * chunks;      // n: beam over all groups
   const int g = n / beams;
   const T* row = logits + g * group_stride + (int64_t)(n - g * beams) * beam_stride;
@@ -226,9 +257,7 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
     take(u);
   }
   for (; part < kParts; ++part) tc::mbar_wait(&arrived[part], 0, status, 700);
-  float top = mine;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  float top = warp_max(mine);
   if ((tid & 31) == 0) red[0][tid >> 5] = top;
   __syncthreads();
 #pragma unroll
@@ -242,31 +271,69 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
     for (int u = 1; u < kThreads / 32; ++u) sum += red[1][u];
     sums[blockIdx.x] = make_float2(top, sum);
   }
-  // Few threads have anything to give: each one's units are looked through by its whole warp.
-  auto reach = [&](float bound, auto f) {
-    for (unsigned left = __ballot_sync(0xffffffffu, mine >= bound); left != 0u; left &= left - 1u) {
-      const int first = (tid & ~31) + __ffs(left) - 1;
-      for (int u = first + (tid & 31) * kThreads; u < count; u += 32 * kThreads) {
-        const uint4 raw = run[u];
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float most = -INFINITY;
+  auto hits_of = [&](int u, auto wanted) {                     // which elements of a unit, a bit each (a NaN is never chosen)
+    const uint4 raw = run[u];
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const int64_t v = (int64_t)(unit0 + u) * kPer - lead;
+    unsigned hits = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) most = fmaxf(most, W::at(w[i / W::kPer], i % W::kPer));
-        if (most < bound) continue;
-        const int64_t v = (int64_t)(unit0 + u) * kPer - lead;
-#pragma unroll 1
-        for (int i = 0; i < kPer; ++i) {
-          if (v + i < 0 || v + i >= vocab) continue;
-          const float x = fmaxf(to_float<T>(reinterpret_cast<const T*>(run)[u * kPer + i]), -INFINITY);      // a NaN is never chosen
-          if (x >= bound) f(x, (int)(v + i));
-        }
+    for (int i = 0; i < kPer; ++i)
+      if (wanted(fmaxf(W::at(w[i / W::kPer], i % W::kPer), -INFINITY)) && v + i >= 0 && v + i < vocab) hits |= 1u << i;
+    return hits;
+  };
+  // Few threads have anything to give: where they have many units, each one's are looked through by its whole warp.
+  auto reach = [&](float bound, bool above, auto f) {
+    bool more = true;
+    auto take_unit = [&](int u) {
+      for (unsigned hits = hits_of(u, [&](float x) { return above ? x > bound : x >= bound; }); hits != 0u && more; hits &= hits - 1u) {
+        const int i = __ffs(hits) - 1;
+        more = f(fmaxf(to_float<T>(reinterpret_cast<const T*>(run)[u * kPer + i]), -INFINITY), (int)((int64_t)(unit0 + u) * kPer - lead + i));
       }
+    };
+    const bool any = above ? mine > bound : mine >= bound;
+    if (count <= 2 * kThreads) {
+      for (int u = tid; u < count && any && more; u += kThreads) take_unit(u);
+      return;
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, any); left != 0u; left &= left - 1u) {
+      for (int u = (tid & ~31) + __ffs(left) - 1 + (tid & 31) * kThreads; u < count && more; u += 32 * kThreads) take_unit(u);
       __syncwarp();
     }
   };
+  auto one = [&](auto f) {
+    for (int u = tid; u < count; u += kThreads)
+      for (unsigned hits = hits_of(u, [](float) { return true; }); hits != 0u; hits &= hits - 1u) {
+        const int i = __ffs(hits) - 1;
+        f(fmaxf(to_float<T>(reinterpret_cast<const T*>(run)[u * kPer + i]), -INFINITY), (int)((int64_t)(unit0 + u) * kPer - lead + i));
+      }
+  };
+  auto equal = [&](float x, int need, auto f) {                // 256 units at a time, a prefix sum over the threads
+    int found = 0;
+    for (int base = 0; base < count && found < need; base += kThreads) {
+      const int u = base + tid;
+      const int64_t v = (int64_t)(unit0 + u) * kPer - lead;
+      unsigned hits = u < count ? hits_of(u, [&](float y) { return y == x; }) : 0u;
+      int upto = __popc(hits);
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, s);
+        if ((tid & 31) >= s) upto += y;
+      }
+      if ((tid & 31) == 31) sums_s[tid >> 5] = upto;
+      __syncthreads();
+      int at = found + upto - __popc(hits);
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < (tid >> 5)) at += sums_s[w];
+        found += sums_s[w];
+      }
+      for (; hits != 0u && at < need; hits &= hits - 1u, ++at) f(at, (int)(v + __ffs(hits) - 1));
+      __syncthreads();
+    }
+    return true;
+  };
   float* out_v = values + (int64_t)blockIdx.x * width;
   int* out_t = tokens + (int64_t)blockIdx.x * width;
-  largest(sh, width, mine, reach, [&](int at, float v, int i) {
+  largest(sh, width, max(1, min(kThreads / 32, (count + 31) / 32)), mine, reach, one, equal, [&](int at, float v, int i) {
     out_v[at] = v;
     out_t[at] = i;
   });
@@ -330,12 +397,14 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
   };
   double mine = -INFINITY;
   each([&](double x, long long) { mine = x > mine ? x : mine; });
-  auto reach = [&](double bound, auto f) {
+  auto reach = [&](double bound, bool above, auto f) {
+    bool more = true;
     each([&](double x, long long i) {
-      if (x >= bound) f(x, i);
+      if (more && (above ? x > bound : x >= bound)) more = f(x, i);
     });
   };
-  largest(sh, width, mine, reach, [&](int at, double v, long long i) {
+  auto equal = [](double, int, auto) { return false; };        // (places are not in order of their index)
+  largest(sh, width, kThreads / 32, mine, reach, each, equal, [&](int at, double v, long long i) {
     const int64_t o = (int64_t)g * width + at;
     out_scores[o] = (float)v;
     out_rows[o] = g * beams + (int)(i >> 32);

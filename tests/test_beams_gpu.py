@@ -23,7 +23,8 @@ def _check(logits, scores, width):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("groups,n,vocab,width", [(1, 1, 1, 1), (1, 1, 7, 5), (2, 3, 33, 32), (1, 4, 50257, 4), (3, 5, 8191, 11), (40, 8, 5003, 8),
-                                                  (1, 1, 50304, 32), (2, 256, 300, 9), (70, 12, 2049, 32)])
+                                                  (1, 1, 50304, 32), (2, 256, 300, 9), (70, 12, 2049, 32), (13, 2, 388, 5),
+                                                  (13, 7, 244, 10), (3, 1, 257, 32), (2, 2, 2056, 31)])
 def test_selection(dtype, groups, n, vocab, width):
     gen = torch.Generator().manual_seed(vocab + width)
     logits = (torch.randn(groups, n, vocab, generator=gen) * 3).to(dtype).cuda()
