@@ -138,37 +138,69 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
     auto next = [](Ring& x) {
       if (++x.slot == kRing) { x.slot = 0; x.par ^= 1u; }
     };
-    if (warp == 13) {
-      // ============================================ TMA loads =============================================
-      if (PAGED || lane == 0) {
-        // PAGED: a lane a box of the tile; its page of the tile after is fetched with each load (`page`: of the next tile of K
-        // or V, which two heads share), so that no load waits for the table.
-        const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
-        int page_k = -1, page_v = -1;
-        if constexpr (PAGED) page_k = page_v = boxes.page(i0, seq, lane);
-        auto load = [&](int off, const CUtensorMap* map, int id, int row, int head, int page) {
-          if constexpr (PAGED) {
-            const int used = boxes.count(row, seq);
-            __syncwarp();
-            if (lane == 0) mbar_expect_tx(&bars[id], used * paged.box_rows * 128);
-            __syncwarp();
-            if (lane < used) tma_load_4d(smem + off + lane * paged.box_rows * 128, map, &bars[id], 0, boxes.at(row, lane), head, page);
-          } else {
-            mbar_expect_tx(&bars[id], kRowTile);
-            tma_load_4d(smem + off, map, &bars[id], 0, row, head, b);
-          }
-        };
-        auto next_page = [&](int& page, int nj) {
-          if constexpr (PAGED) page = boxes.page(nj * kTile, seq, lane);
-        };
-        if (lane == 0) {
-          mbar_expect_tx(&bars[QF], 3 * kRowTile);
-          const int q_row = item.token + i0 - q_offset;
-          tma_load_4d(smem + L::q + 2 * kRowTile, &map_q0, &bars[QF], 0, q_row, 0, b);
-          tma_load_4d(smem + L::q, &map_q, &bars[QF], 0, q_row, h0, b);
-          tma_load_4d(smem + L::q + kRowTile, &map_q, &bars[QF], 0, q_row, h0 + 1, b);
+    // PAGED: a lane a box of a tile; its page of the tile after is fetched with each load (by the caller), so that no load waits
+    // for the table.
+    const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
+    auto load_boxes = [&](int off, const CUtensorMap* map, int id, int j0, int head, int page) {
+      const int used = boxes.count(j0, seq);
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(&bars[id], used * paged.box_rows * 128);
+      __syncwarp();
+      if (lane < used) tma_load_4d(smem + off + lane * paged.box_rows * 128, map, &bars[id], 0, boxes.at(j0, lane), head, page);
+    };
+    if (PAGED && warp == 13) {
+      // ======================================== Q, and K in pages ==========================================
+      if (lane == 0) {
+        mbar_expect_tx(&bars[QF], 3 * kRowTile);
+        const int q_row = item.token + i0 - q_offset;
+        tma_load_4d(smem + L::q + 2 * kRowTile, &map_q0, &bars[QF], 0, q_row, 0, b);
+        tma_load_4d(smem + L::q, &map_q, &bars[QF], 0, q_row, h0, b);
+        tma_load_4d(smem + L::q + kRowTile, &map_q, &bars[QF], 0, q_row, h0 + 1, b);
+      }
+      Ring rk{0, 1};
+      int page = boxes.page(i0, seq, lane);
+#pragma unroll 1
+      for (int n = 0; n < 2 * steps; ++n) {                    // tile n of the ring: step n / 2 of head n & 1
+        const int j0 = i0 - (n >> 1) * kTile;
+        if (n >= kRing) wait(bar(FREEK + (int)rk.slot), rk.par, 501);
+        load_boxes(L::k + rk.slot * kRowTile, &map_k, LDK + (int)rk.slot, j0, h0 + (n & 1), page);
+        next(rk);
+        if (n & 1) page = boxes.page(j0 - kTile, seq, lane);
+      }
+    } else if (PAGED && warp == 15) {
+      // ================== K0 and V in pages: two warps issue (with one, pages of 16 took 5.3 k cycles a step) ==================
+      Ring rv{0, 1};
+      int page_k0 = boxes.page(i0, seq, lane), page_v = page_k0;
+      load_boxes(L::k0, &map_k0, LDK0, i0, 0, page_k0);
+      page_k0 = boxes.page(i0 - kTile, seq, lane);
+#pragma unroll 1
+      for (int t = 0; t < steps; ++t) {
+        const int j0 = i0 - t * kTile;
+        if (t + 1 < steps) {                                   // K0 of the next step, once this step's L0 is done
+          wait(bar(L0F), (uint32_t)(t & 1), 503);
+          load_boxes(L::k0, &map_k0, LDK0, j0 - kTile, 0, page_k0);
+          page_k0 = boxes.page(j0 - 2 * kTile, seq, lane);
         }
-        if (!PAGED) load(L::k0, &map_k0, LDK0, i0, 0, -1);
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          if (2 * t + x >= kRing) wait(bar(FREEV + (int)rv.slot), rv.par, 502);
+          load_boxes(L::v + rv.slot * kRowTile, &map_v, LDV + (int)rv.slot, j0, h0 + x, page_v);
+          next(rv);
+        }
+        page_v = boxes.page(j0 - kTile, seq, lane);
+      }
+    } else if (warp == 13) {
+      // ============================================ TMA loads =============================================
+      if (lane == 0) {
+        auto load = [&](int off, const CUtensorMap* map, int id, int row, int head) {
+          mbar_expect_tx(&bars[id], kRowTile);
+          tma_load_4d(smem + off, map, &bars[id], 0, row, head, b);
+        };
+        mbar_expect_tx(&bars[QF], 3 * kRowTile);
+        tma_load_4d(smem + L::q + 2 * kRowTile, &map_q0, &bars[QF], 0, i0 - q_offset, 0, b);
+        tma_load_4d(smem + L::q, &map_q, &bars[QF], 0, i0 - q_offset, h0, b);
+        tma_load_4d(smem + L::q + kRowTile, &map_q, &bars[QF], 0, i0 - q_offset, h0 + 1, b);
+        load(L::k0, &map_k0, LDK0, i0, 0);
         // Tile n of the K and V rings: step n / 2 of head n & 1.  K runs one tile ahead of V.
         const int tiles = 2 * steps;
         int nj_k = mi, nj_v = mi, nj_k0 = mi;
@@ -177,26 +209,20 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
         for (int n = 0; n <= tiles; ++n) {
           if (n < tiles) {
             if (n >= kRing) wait(bar(FREEK + (int)rk.slot), rk.par, 501);
-            load(L::k + rk.slot * kRowTile, &map_k, LDK + (int)rk.slot, nj_k * kTile, h0 + (n & 1), page_k);
+            load(L::k + rk.slot * kRowTile, &map_k, LDK + (int)rk.slot, nj_k * kTile, h0 + (n & 1));
             next(rk);
-            if (n & 1) {
-              nj_k = step_back(nj_k);
-              next_page(page_k, nj_k);
-            }
+            if (n & 1) nj_k = step_back(nj_k);
           }
           if (n > 0) {
             if (n - 1 >= kRing) wait(bar(FREEV + (int)rv.slot), rv.par, 502);
-            load(L::v + rv.slot * kRowTile, &map_v, LDV + (int)rv.slot, nj_v * kTile, h0 + ((n - 1) & 1), page_v);
+            load(L::v + rv.slot * kRowTile, &map_v, LDV + (int)rv.slot, nj_v * kTile, h0 + ((n - 1) & 1));
             next(rv);
-            if (!(n & 1)) {
-              nj_v = step_back(nj_v);
-              next_page(page_v, nj_v);
-            }
+            if (!(n & 1)) nj_v = step_back(nj_v);
           }
-          if (!PAGED && (n & 1) && (n >> 1) + 1 < steps) {     // K0 of the next step, once this step's L0 is done
+          if ((n & 1) && (n >> 1) + 1 < steps) {               // K0 of the next step, once this step's L0 is done
             wait(bar(L0F), (uint32_t)((n >> 1) & 1), 503);
             nj_k0 = step_back(nj_k0);
-            load(L::k0, &map_k0, LDK0, nj_k0 * kTile, 0, -1);
+            load(L::k0, &map_k0, LDK0, nj_k0 * kTile, 0);
           }
         }
       }
@@ -266,20 +292,6 @@ __global__ void __launch_bounds__(kThreads, 1) forward_pair_kernel(
           mma_commit(bar(FF));
         }
         __syncwarp();
-      }
-    } else if (PAGED && warp == 15) {
-      // ===================== K0 in pages: not behind the boxes of K and V, which a step waits for less ===================
-      const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
-      int page = boxes.page(i0, seq, lane);
-#pragma unroll 1
-      for (int t = 0; t < steps; ++t) {
-        const int j0 = i0 - t * kTile, used = boxes.count(j0, seq);
-        if (t > 0) wait(bar(L0F), (uint32_t)((t - 1) & 1), 504);     // L0 of the step before is done
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(&bars[LDK0], used * paged.box_rows * 128);
-        __syncwarp();
-        if (lane < used) tma_load_4d(smem + L::k0 + lane * paged.box_rows * 128, &map_k0, &bars[LDK0], 0, boxes.at(j0, lane), 0, page);
-        page = boxes.page(j0 - kTile, seq, lane);
       }
     } else if (warp < 12) {
       // ================================= selection: relu(L0) under the mask, the carry ========================

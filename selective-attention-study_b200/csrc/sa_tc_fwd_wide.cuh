@@ -58,6 +58,7 @@ struct WideSmem {
 };
 constexpr int kWideCompute = 512;                      // four warpgroups: 32 of a step's 128 key columns, D / 4 of the d each
 constexpr int kWideThreads = kWideCompute + 32;        // + the control warp: one lane issues every TMA load and MMA
+constexpr int kWidePagedThreads = kWideThreads + 64;   // PAGED: + two warps for the boxes of the pages
 constexpr int kWideBarrier = 1;                        // hardware barrier id of the arithmetic warps
 
 // With pieces > 1 a CTA walks one piece of its query tile's key tiles (nothing goes from key tile to key tile but the softmax
@@ -72,7 +73,7 @@ struct SplitWalk {
 // a kernel without the other code, which took 5 % longer with it (15 heads of T = 16384, head_dim 64: 1.41 -> 1.37 ms).
 // PAGED: `paged` says what a CTA has (seq, ntiles, q_offset, out and lse2 are not looked at).
 template <int D, bool SELF, bool LIVE, bool SPLIT, bool PAGED = false>
-__global__ void __launch_bounds__(kWideThreads, 1)
+__global__ void __launch_bounds__(PAGED ? kWidePagedThreads : kWideThreads, 1)
     forward_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q0,
                         const __grid_constant__ CUtensorMap map_k0, const float* __restrict__ carry,
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   // P V of a step; bar_fin the last P V.  Arrival barriers (one arrival per arithmetic warp and step): bar_sel
   // selection tile written and the previous step's logits read; bar_p P written and O rescaled.
   __shared__ uint64_t bar_q, bar_k[2], bar_k0[2], bar_v[2], bar_l0, bar_tri, bar_pv, bar_fin, bar_sel, bar_p, bar_setup;
+  __shared__ uint64_t free_k[2], free_k0[2], free_v[2];       // PAGED: the products that read a tile (that will be refilled) are done
   __shared__ uint32_t tmem_base_s;
   __shared__ __align__(16) float carry_s[2][kTile];
   __shared__ float rmax_s[4][kTile];
@@ -141,6 +143,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       mbar_init(&bar_k[u], 1);
       mbar_init(&bar_k0[u], 1);
       mbar_init(&bar_v[u], 1);
+      if (PAGED) {
+        mbar_init(&free_k[u], 1);
+        mbar_init(&free_k0[u], 1);
+        mbar_init(&free_v[u], 1);
+      }
     }
     mbar_init(&bar_l0, 1);
     mbar_init(&bar_tri, 1);
@@ -200,35 +207,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       converge();
     };
-    // PAGED: a lane a box; its page of the tile after is fetched with each load, so that no load waits for the table.
-    const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
-    int page_k = -1, page_k0 = -1, page_v = -1;
-    if constexpr (PAGED) page_k = page_k0 = page_v = boxes.page(key_tile(0) * kTile, seq, lane);
-    auto load_boxes = [&](int off, const CUtensorMap* map, uint64_t* bars, int it, int head, int& page) {
-      const int j0 = key_tile(it) * kTile, used = boxes.count(j0, seq);
-      uint64_t* bar = &bars[slot(it)];
-      if (elected()) mbar_expect_tx(bar, DK * used * paged.box_rows * 128);
-      converge();
-      if (lane < used)
-        for (int s2 = 0; s2 < DK; ++s2)
-          tma_load_4d(smem + off + slot(it) * L::kTileBytes + s2 * kRowTile + lane * paged.box_rows * 128, map, bar, s2 * 64,
-                      boxes.at(j0, lane), head, page);
-      converge();
-      page = boxes.page(j0 - kTile, seq, lane);
-    };
-    auto load_k = [&](int it) {
-      if constexpr (PAGED) load_boxes(L::k, &map_k, bar_k, it, h, page_k);
-      else load_tile(L::k, &map_k, bar_k, it, h);
-    };
-    auto load_k0 = [&](int it) {                               // SELF: K0 is K
-      if (SELF) return;
-      if constexpr (PAGED) load_boxes(L::k0, &map_k0, bar_k0, it, 0, page_k0);
-      else load_tile(L::k0, &map_k0, bar_k0, it, 0);
-    };
-    auto load_v = [&](int it) {
-      if constexpr (PAGED) load_boxes(L::v, &map_v, bar_v, it, h, page_v);
-      else load_tile(L::v, &map_v, bar_v, it, h);
-    };
+    auto load_k = [&](int it) { if (!PAGED) load_tile(L::k, &map_k, bar_k, it, h); };
+    auto load_k0 = [&](int it) { if (!PAGED && !SELF) load_tile(L::k0, &map_k0, bar_k0, it, 0); };   // SELF: K0 is K
+    auto load_v = [&](int it) { if (!PAGED) load_tile(L::v, &map_v, bar_v, it, h); };
     const uint32_t idesc_s = instr_desc_bf16(128, 128, false, false);
     const uint32_t idesc_tri = instr_desc_bf16(128, 128, false, true, /*negate_a=*/true);
     const uint32_t idesc_pv = instr_desc_bf16(128, D, false, true);
@@ -243,6 +224,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll
         for (int ks = 0; ks < 4 * DK; ++ks)
           mma_ts_low(tmem + kColL, tmem + (SELF ? kColQ : kColQ0) + ks * 8, at(tile, kstep(ks)), idesc_s, ks > 0);
+        if (PAGED && !SELF && it + ST < steps) mma_commit(&free_k0[slot(it)]);
         mma_commit(&bar_l0);
       }
       converge();
@@ -253,6 +235,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t tile = at(kBase, L::k + slot(it) * L::kTileBytes);
 #pragma unroll
         for (int ks = 0; ks < 4 * DK; ++ks) mma_ts_low(tmem + kColS, tmem + kColQ + ks * 8, at(tile, kstep(ks)), idesc_s, ks > 0);
+        if (PAGED && it + ST < steps) mma_commit(&free_k[slot(it)]);         // (SELF: L0 of the step came before)
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           if (kTmemAB) mma_ts_low(tmem + kColS, tmem + kColTri + ks * 8, at(mBase, L::sel + ks * 2048), idesc_tri, 1u);
@@ -274,6 +257,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           else if (it > 0) mma_ss_low<true>(tmem + kColO, at(kBase, L::p), v, idesc_pv);
           else mma_ss_low<false>(tmem + kColO, at(kBase, L::p), v, idesc_pv);
         }
+        if (PAGED && it + ST < steps) mma_commit(&free_v[slot(it)]);
         mma_commit(bar);
       }
       converge();
@@ -306,11 +290,15 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       if (l0_now && it + 1 < steps) issue_l0(it + 1);
       if (it > 0) {
         await(&bar_p, (it - 1) & 1, 320);                      // P of step it - 1 written, O rescaled
-        if (ST == 2 && it >= 2) {                              // before this barrier's next commit: P V of it - 2 done,
+        if (!PAGED && ST == 2 && it >= 2) {                    // before this barrier's next commit: P V of it - 2 done,
           await(&bar_pv, it & 1, 321);                         //   so its V tile may be refilled
           load_v(it);
         }
         issue_pv(it - 1, &bar_pv);
+      }
+      if (PAGED) {                                             // (tiles are refilled by the loading warp)
+        if (!l0_now && it + 1 < steps) issue_l0(it + 1);
+        continue;
       }
       await(&bar_tri, it & 1, 319);                            // S of step it done: its K tile is free
       if (it + ST < steps) load_k(it + ST);
@@ -325,6 +313,38 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if (!kOneLane && lane == 0) wait.end(status);
     }
     __syncwarp();
+  } else if (PAGED && warp > kWideCompute / 32) {
+    // ====== loading warps, one for K0 and K, one for V: a lane a box; its page of the tile after is fetched meanwhile ======
+    // (Issued by the control warp between its products, the boxes of pages of 16 made a step of head_dim 64 2.2 k cycles longer, of
+    // 128 tokens 1.1 k; by one warp for all three, pages of 16 cost a fifth.)
+    Waiter wait;
+    wait.begin(status);
+    const PageBoxes boxes{paged.tables + (int64_t)item.row * paged.max_pages, paged.page_shift, paged.box_rows};
+    int page = boxes.page(last * kTile, seq, lane);
+    auto load = [&](int off, const CUtensorMap* map, uint64_t* bars, uint64_t* freed, int it, int head) {
+      const int u = ST == 2 ? (it & 1) : 0, j0 = (last - it) * kTile, used = boxes.count(j0, seq);
+      if (it >= ST) wait(smem_u32(&freed[u]), (uint32_t)(((ST == 2 ? it >> 1 : it) & 1) ^ 1), 325);
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(&bars[u], DK * used * paged.box_rows * 128);
+      __syncwarp();
+      if (lane < used)
+        for (int s2 = 0; s2 < DK; ++s2)
+          tma_load_4d(smem + off + u * L::kTileBytes + s2 * kRowTile + lane * paged.box_rows * 128, map, &bars[u], s2 * 64, boxes.at(j0, lane),
+                      head, page);
+    };
+    const bool values = warp > kWideCompute / 32 + 1;
+#pragma unroll 1
+    for (int n = 0; n < steps; ++n) {
+      const int page_next = boxes.page((last - n - 1) * kTile, seq, lane);
+      if (values) {
+        load(L::v, &map_v, bar_v, free_v, n, h);
+      } else {
+        if (!SELF) load(L::k0, &map_k0, bar_k0, free_k0, n, 0);
+        load(L::k, &map_k, bar_k, free_k, n, h);
+      }
+      page = page_next;
+    }
+    if (lane == 0) wait.end(status);
   } else {
     // ======================================= arithmetic warps ============================================
     const int row = tid & 127, wg = tid >> 7;

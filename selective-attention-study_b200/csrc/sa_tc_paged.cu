@@ -327,7 +327,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   }
   const dim3 grid((unsigned)l.tile_items_max * a.heads);
   auto wide = [&](auto kernel) {
-    return launch(kernel, grid, kWideThreads, WideSmem<D>::total + 1024, true, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
+    return launch(kernel, grid, kWidePagedThreads, WideSmem<D>::total + 1024, true, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
                   (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
                   SplitWalk{}, walk);
   };
