@@ -455,19 +455,8 @@ int select(const Select& p, cudaStream_t s) {
     default: return SA_ERR_BAD_ARGUMENT;
   }
   if (st != SA_OK) return st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(p.groups);
-  config.blockDim = dim3(kThreads);
-  config.stream = s;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  count_launch();
-  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, choose_kernel, p.scores, p.beams, p.vocab, p.width, r.chunks, (const float2*)sums,
-                                   (const float*)values, (const int*)tokens, p.out_scores, p.out_rows, p.out_tokens));
-  return SA_OK;
+  return launch_after(choose_kernel, dim3(p.groups), kThreads, 0, s, p.scores, p.beams, p.vocab, p.width, r.chunks, (const float2*)sums,
+                      (const float*)values, (const int*)tokens, p.out_scores, p.out_rows, p.out_tokens);
 }
 
 }  // namespace beam

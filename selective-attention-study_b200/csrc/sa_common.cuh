@@ -175,4 +175,24 @@ struct ProfileScope {
     }                                                         \
   } while (0)
 
+// Launches a kernel that may begin while the one before it in the stream still runs (programmatic stream serialization); the
+// kernel waits for that one's results itself.
+template <typename... Args>
+int launch_after(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+  SA_CUDA_CHECK(allow_smem(kernel, smem));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  count_launch();
+  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+  return SA_OK;
+}
+
 }  // namespace sa

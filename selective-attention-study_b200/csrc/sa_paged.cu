@@ -503,23 +503,6 @@ __global__ void __launch_bounds__(256) move_kernel(const int4* __restrict__ move
   }
 }
 
-template <typename... Args>
-int launch_after(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = s;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  count_launch();
-  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
-  return SA_OK;
-}
-
 }  // namespace
 
 int append(const Tables& t, const int* counts, int total, int max_length, int max_count, int* query_start, int* cached, int64_t* slots,
@@ -556,7 +539,6 @@ int append(const Tables& t, const int* counts, int total, int max_length, int ma
                                                : by_width(std::integral_constant<int, kMaxRows / 1024>{}, 1024);
   if (st != SA_OK || a.inside) return st;
   const unsigned blocks = (unsigned)min((total + 255) / 256, 2 * kSms);
-  SA_CUDA_CHECK(allow_smem(spread_kernel, smem));
   return launch_after(spread_kernel, dim3(blocks), 256, smem, s, a);
 }
 
@@ -579,7 +561,6 @@ int move_rows(const Tables& t, const int* copies, const int* work, int groups, i
   // 32 keys a CTA (a line of every row), or 8 where the rows would not fit the shared memory
   auto move = [&](auto kernel, int units) -> int {
     const size_t smem = (size_t)t.rows * units * sizeof(float4);
-    SA_CUDA_CHECK(allow_smem(kernel, smem));
     const int chunks = (int)((capacity + 4 * units - 1) / (4 * units));
     const unsigned history = (unsigned)chunks * groups, pages = (unsigned)min(t.rows, 256) * 2 * kPagePieces;
     return launch_after(kernel, dim3(history + pages), 256, smem, s, reinterpret_cast<const int4*>(work), reinterpret_cast<const int2*>(copies),

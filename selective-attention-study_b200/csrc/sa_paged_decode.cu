@@ -341,29 +341,15 @@ int decode_impl(const Attention& a, bool beside, cudaStream_t s) {
   if (st != SA_OK) return st;
   int* tickets = a.plan_tickets ? a.work + l.tickets : reinterpret_cast<int*>(a.workspace + w.own_tickets);
   if (!a.plan_tickets && !beside) SA_CUDA_CHECK(cudaMemsetAsync(tickets, 0, (size_t)l.tickets_count * 4, s));
-  auto kernel = decode_pages_kernel<D>;
-  SA_CUDA_CHECK(allow_smem(kernel, smem_bytes<D>()));
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)l.decode_items_max * a.heads + (beside ? 1 : 0));
-  config.blockDim = dim3(kAllThreads);
-  config.dynamicSmemBytes = smem_bytes<D>();
-  config.stream = s;
-  config.attrs = &attr;
-  config.numAttrs = 1;
   ProfileScope prof(SA_KERNEL_DECODE, s);
-  count_launch();
   using bf16 = __nv_bfloat16;
-  SA_CUDA_CHECK(cudaLaunchKernelEx(
-      &config, kernel, map_k, map_v, static_cast<const bf16*>(a.q), Strides{a.q_stride[0], a.q_stride[1]}, static_cast<const bf16*>(a.k),
+  return launch_after(
+      decode_pages_kernel<D>, dim3((unsigned)l.decode_items_max * a.heads + (beside ? 1 : 0)), kAllThreads, smem_bytes<D>(), s, map_k, map_v, static_cast<const bf16*>(a.q), Strides{a.q_stride[0], a.q_stride[1]}, static_cast<const bf16*>(a.k),
       Strides{a.k_stride[0], a.k_stride[1]}, static_cast<const bf16*>(a.v), Strides{a.v_stride[0], a.v_stride[1]},
       static_cast<bf16*>(a.k_pages), static_cast<bf16*>(a.v_pages), a.selected, a.sel_stride, a.block_tables, a.max_pages, a.num_pages,
       a.page_shift, box_rows, (const int*)a.work, reinterpret_cast<const DecodeItem*>(a.work + l.decode_items), l.decode_items_max,
       a.workspace + w.partial, a.workspace + w.sel_new, w.key_stride, reinterpret_cast<unsigned*>(tickets), a.heads, a.groups, a.exempt,
-      1.0f / sqrtf((float)D), a.slots, a.total, static_cast<bf16*>(a.y), status, beside));
-  return SA_OK;
+      1.0f / sqrtf((float)D), a.slots, a.total, static_cast<bf16*>(a.y), status, beside);
 }
 
 }  // namespace

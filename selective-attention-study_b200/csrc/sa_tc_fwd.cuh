@@ -18,7 +18,7 @@ struct PagedWalk {
   const int* header;                 // of the step's plan
   const paged::TileItem* items;
   const int* tables;                 // pages of a row
-  int max_pages, page_shift, box_rows;
+  int heads, max_pages, page_shift, box_rows;
   int64_t key_stride;
   unsigned int* tickets;             // one a tile and head, zero
   float *part, *lse;                 // rows of pieces, by item and head
@@ -46,6 +46,10 @@ int forward_pair(const Problem& p, const ForwardMaps& m, const float* carry, flo
 // Two rows a CTA (sa_tc_fwd_self.cu): head_dim 64, one head per selector, an even number of rows.
 int forward_self(const Problem& p, const ForwardMaps& m, const float* carry, float* out, float* lse2, const WaitCtx& status,
                  const uint8_t* alive, cudaStream_t s);
+
+// The same over pages (sa_tc_paged_self.cu): head_dim 64, every head its own selector, an even number of heads.
+int forward_self_pages(const PagedWalk& walk, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const float* carry,
+                       int items_max, int exempt, float scale, const WaitCtx& status, __nv_bfloat16* y, const RowLayout& y_rows, cudaStream_t s);
 
 }  // namespace tc
 }  // namespace sa

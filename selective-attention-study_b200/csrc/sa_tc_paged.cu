@@ -4,7 +4,7 @@
 //   colsum_pages_kernel   selection pass: column sums of a query tile's relu'd, masked logits, key tile by key tile
 //   scan_pages_kernel     their running sum over the tiles of a row, from the row's history on (-> what the tiles start from), and
 //                         the history moved on
-//   forward_pair_kernel, forward_wide_kernel (PAGED)   sa_tc_fwd_pair.cuh, sa_tc_fwd_wide.cuh
+//   forward_pair_kernel, forward_self_kernel, forward_wide_kernel (PAGED)   sa_tc_fwd_pair.cuh, sa_tc_fwd_self.cuh, sa_tc_fwd_wide.cuh
 //
 // The plan of the step (sa_paged.cu) says which tiles there are; the host knows bounds, so a grid covers those and CTAs without
 // a tile return at once.  A query tile is 128 positions of one row, counted from its token 0, as the key tiles are: the
@@ -236,24 +236,6 @@ __global__ void __launch_bounds__(256) restore_kernel(const float* __restrict__ 
   selected[((int64_t)r * groups + g) * sel_stride + j] = carry[((int64_t)t0 * groups + g) * key_stride + j];
 }
 
-template <typename... Args>
-int launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t s, Args... args) {
-  SA_CUDA_CHECK(allow_smem(kernel, smem));
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = s;
-  config.attrs = &attr;
-  config.numAttrs = overlap ? 1 : 0;
-  count_launch();
-  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
-  return SA_OK;
-}
-
 template <int D>
 int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   constexpr int DK = D / 64;
@@ -280,7 +262,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
     const TokenRows v{static_cast<const uint4*>(a.v), a.v_stride[0] / 8, a.v_stride[1] / 8};
     const int64_t units = (int64_t)a.total * a.heads * (D / 8);
     const unsigned blocks = (unsigned)max((int64_t)1, min((units + 255) / 256, (int64_t)8 * kSms));
-    st = launch(store_kernel, dim3(blocks), 256, 0, true, s, k, v, static_cast<uint4*>(a.k_pages), static_cast<uint4*>(a.v_pages),
+    st = launch_after(store_kernel, dim3(blocks), 256, 0, s, k, v, static_cast<uint4*>(a.k_pages), static_cast<uint4*>(a.v_pages),
                 static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk,
                 reinterpret_cast<unsigned int*>(a.workspace + w.own_tickets), a.plan_tickets ? 0 : l.tickets_count);
     if (st != SA_OK) return st;
@@ -289,7 +271,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   walk.header = a.work;
   walk.items = reinterpret_cast<const TileItem*>(a.work + l.tile_items);
   walk.tables = a.block_tables;
-  walk.max_pages = a.max_pages; walk.page_shift = a.page_shift; walk.box_rows = box_rows;
+  walk.heads = a.heads; walk.max_pages = a.max_pages; walk.page_shift = a.page_shift; walk.box_rows = box_rows;
   walk.key_stride = w.key_stride;
   walk.tickets = walk_tickets;
   walk.part = a.workspace + w.part;
@@ -302,13 +284,13 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
     // key tiles per CTA: 8, or 32 where that still gives every SM several CTAs (the query tile and the set-up are paid per CTA)
     const int chunk = (int64_t)l.tiles_max * key_tiles * a.groups >= 32 * 16 * kSms ? 32 : 8;
     ProfileScope prof(SA_KERNEL_TC_COLSUM, s);
-    st = launch(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, true, s,
+    st = launch_after(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, s,
                 map_q, map_k, carry, a.exempt, scale, status, chunk, tiles, walk);
     if (st != SA_OK) return st;
   }
   {
     ProfileScope prof(SA_KERNEL_TC_SCAN, s);
-    st = launch(scan_pages_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, true, s, carry, w.key_stride,
+    st = launch_after(scan_pages_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, s, carry, w.key_stride,
                 (const int*)(a.work + l.tile_start), tiles, a.groups, a.selected, a.sel_stride);
     if (st != SA_OK) return st;
     *moved = true;
@@ -321,13 +303,15 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   const RowLayout y_rows{0, D, (int64_t)a.heads * D};
   if constexpr (D == 64) {
     if (!self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
-      return launch(forward_pair_kernel<false, true>, dim3((unsigned)l.tile_items_max * (a.heads / 2)), kThreads, PairSmem::total, true, s,
+      return launch_after(forward_pair_kernel<false, true>, dim3((unsigned)l.tile_items_max * (a.heads / 2)), kThreads, PairSmem::total, s,
                     map_q, map_k, map_v, map_q, map_k, (const float*)carry, (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale,
                     status, y, y_rows, 0, (const uint8_t*)nullptr, walk);
   }
+  if (D == 64 && self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
+    return forward_self_pages(walk, map_q, map_k, map_v, carry, l.tile_items_max, a.exempt, scale, status, y, y_rows, s);
   const dim3 grid((unsigned)l.tile_items_max * a.heads);
   auto wide = [&](auto kernel) {
-    return launch(kernel, grid, kWidePagedThreads, WideSmem<D>::total + 1024, true, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
+    return launch_after(kernel, grid, kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
                   (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
                   SplitWalk{}, walk);
   };
@@ -370,9 +354,12 @@ int tiles(const Attention& a, bool* moved, cudaStream_t s) {
 int restore_histories(const Attention& a, cudaStream_t s) {
   const StepLayout l = step_layout(a.rows, a.total, a.heads);
   const AttentionScratch w = attention_scratch(a);
-  return tc::launch(tc::restore_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, false, s,
-                    (const float*)(a.workspace + w.carry), w.key_stride, (const int*)(a.work + l.tile_start),
-                    reinterpret_cast<const TileItem*>(a.work + l.tiles), a.groups, a.selected, a.sel_stride);
+  count_launch();
+  tc::restore_kernel<<<dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, s>>>(
+      a.workspace + w.carry, w.key_stride, a.work + l.tile_start, reinterpret_cast<const TileItem*>(a.work + l.tiles), a.groups, a.selected,
+      a.sel_stride);
+  SA_CUDA_CHECK(cudaGetLastError());
+  return SA_OK;
 }
 
 }  // namespace paged
