@@ -301,11 +301,11 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // Row r becomes a copy of row parents[r] (outside [0, rows): an empty row).  Full pages are shared.  The page that is being
 // filled stays with the lowest child; the others get a page of their own, and `copies` says what has to be copied into it.
 //
-// One cluster of eight CTAs, in four passes with a cluster barrier between: (1) the new tables into scratch, a reference more
-// for each page of a new row (a page that old and new row have at the same place counts for neither); (2) a reference less for
-// each page of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first,
-// and takes the pages for the copies off its end, in row order; (4) the tables.  A row for which there is none becomes empty (its
-// full pages are shared with the lowest child, so nothing else is freed).
+// One cluster of eight CTAs, in passes with a cluster barrier between: (1) the new tables into scratch, a reference more for each
+// page of a new row (a page that old and new row have at the same place counts for neither); (2) a reference less for each page
+// of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first, and takes the
+// pages for the copies off its end, in row order, while (4) the others write the tables.  A row for which there is none becomes
+// empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes.
 constexpr int kCluster = 8, kReorderThreads = 1024;
 
 // The work of a reordering, int32 words: how many rows change, then (row, parent, tokens, tokens of the page being filled) of
@@ -384,16 +384,27 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
   }
   __threadfence();
   cluster.sync();
-  // (3)
-  if (cta == 0) {
+  // (3), and (4) by the other CTAs meanwhile: all of the new tables but the pages that (3) takes
+  __shared__ int dropped_s;                                       // rows for which there was no page
+  if (cta != 0) {
+    for (int r = warp - kReorderThreads / 32; r < t.rows; r += warps - kReorderThreads / 32) {
+      const int p = parent_s[r], full = p >= 0 ? length_s[p] >> t.page_shift : 0;
+      const bool fresh = __ldcg(info + r) != 0;
+      int* to = t.block_tables + (int64_t)r * t.max_pages;
+      const int* now = scratch + (int64_t)r * t.max_pages;
+      for (int b = lane; b < t.max_pages; b += 32)
+        if (!(fresh && b == full)) to[b] = __ldcg(now + b);
+    }
+  } else {
+    if (tid == 0) dropped_s = 0;
     int count = min(max(*t.free_count, 0), t.num_pages);
     for (int w0 = 0; w0 < words; w0 += kReorderThreads) {
       const int w = w0 + tid;
       unsigned bits = w < words ? __ldcg(marks + w) : 0u;
       int n[1] = {__popc(bits)}, total[1];
       block_scan(n, total, warp_sums);
-      for (int at = count + (int)n[0]; bits != 0u && at < t.num_pages; bits &= bits - 1u, ++at) t.free_pages[at] = w * 32 + __ffs(bits) - 1;
-      count = min(count + (int)total[0], t.num_pages);
+      for (int at = count + n[0]; bits != 0u && at < t.num_pages; bits &= bits - 1u, ++at) t.free_pages[at] = w * 32 + __ffs(bits) - 1;
+      count = min(count + total[0], t.num_pages);
     }
     __syncthreads();                                              // the list
     int used = 0, n_moved = 0;
@@ -408,43 +419,42 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
       int src = -1, dst = -1;
       bool dropped = false;
       if (fresh) {
-        const int k = used + (int)n[0];
-        int* to = scratch + (int64_t)r * t.max_pages;
+        const int k = used + n[0];
+        const int* now = scratch + (int64_t)r * t.max_pages;
         if (k < count) {
-          src = __ldcg(to + full);
+          src = __ldcg(now + full);
           dst = t.free_pages[count - 1 - k];
-          to[full] = dst;
+          t.block_tables[(int64_t)r * t.max_pages + full] = dst;
           if (real(dst)) atomicAdd(t.page_refs + dst, 1);
         } else {                                                  // out of pages: the row becomes empty
           dropped = true;
-          for (int b = 0; b <= full; ++b) {
-            const int page = __ldcg(to + b);
-            if (b < full && real(page)) atomicSub(t.page_refs + page, 1);
-            to[b] = -1;
-          }
+          dropped_s = 1;
+          for (int b = 0; b < full; ++b)
+            if (real(__ldcg(now + b))) atomicSub(t.page_refs + __ldcg(now + b), 1);
         }
       }
       if (r < t.rows) {
         copies[2 * r] = src;
         copies[2 * r + 1] = dst;
-        info[r] = dropped ? 0 : len;                              // the row's new length
+        t.lengths[r] = dropped ? 0 : len;
         if (changes)
           reinterpret_cast<int4*>(moved)[1 + n_moved + n[1]] = make_int4(r, p, dropped ? 0 : len, fresh && !dropped ? len & page_mask : 0);
       }
-      used += (int)total[0];
-      n_moved += (int)total[1];
+      used += total[0];
+      n_moved += total[1];
     }
     if (tid == 0) {
       *t.free_count = count - min(used, count);
       moved[0] = n_moved;
     }
   }
-  __threadfence();
   cluster.sync();
-  // (4)
-  for (int r = me; r < t.rows; r += all) t.lengths[r] = __ldcg(info + r);
-  const int64_t n = (int64_t)t.rows * t.max_pages;
-  for (int64_t i = me; i < n; i += all) t.block_tables[i] = __ldcg(scratch + i);
+  if (cta == 0 && dropped_s != 0) {
+    for (int r = warp; r < t.rows; r += kReorderThreads / 32) {
+      if (__ldcg(info + r) == 0 || copies[2 * r + 1] >= 0) continue;
+      for (int b = lane; b < t.max_pages; b += 32) t.block_tables[(int64_t)r * t.max_pages + b] = -1;
+    }
+  }
 }
 
 // The rows of `moved` in one layer.  The first history_ctas CTAs gather the history, 4 UNITS keys of one group over all rows, through shared
