@@ -281,8 +281,10 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   const float scale = 1.0f / sqrtf((float)D);
   const int key_tiles = (a.max_length + kTile - 1) / kTile;
   {
-    // key tiles per CTA: 8, or 32 where that still gives every SM several CTAs (the query tile and the set-up are paid per CTA)
-    const int chunk = (int64_t)l.tiles_max * key_tiles * a.groups >= 32 * 16 * kSms ? 32 : 8;
+    // key tiles per CTA (the query tile and the set-up are paid per CTA): 32 where that still gives every SM several CTAs, else 8,
+    // or 4 where that would be fewer than two an SM (in 2, 4, 8: 1,024 tokens after 8,000 12, 12, 14 us, 2,048 after 30,000 31, 27, 26)
+    const int64_t products = (int64_t)l.tiles_max * key_tiles * a.groups;
+    const int chunk = products >= 32 * 16 * kSms ? 32 : products >= 8 * 2 * kSms ? 8 : 4;
     ProfileScope prof(SA_KERNEL_TC_COLSUM, s);
     st = launch_after(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, s,
                 map_q, map_k, carry, a.exempt, scale, status, chunk, tiles, walk);
