@@ -150,8 +150,9 @@ template <int PER, typename S>
 __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Append a) {
   const Tables& t = a.t;
   extern __shared__ int rows_s[];
-  __shared__ S warp_sums[5][32];
+  __shared__ S warp_sums[4][32];
   __shared__ int header[kHeaderWords];
+  __shared__ int mi_s[kSms];                     // tiles whose walks are cut
   const RowSums sums(rows_s, t.rows);
   const int tid = threadIdx.x;
   const int r0 = tid * PER;
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
     }
   }
   block_scan(pages, pages_total, warp_sums);
-  S next[5] = {0, 0, 0, 0, 0}, next_total[5];    // tiles, key tiles of their walks, single tokens, their keys, pages taken
+  S next[4] = {0, 0, 0, 0}, next_total[4];       // tiles, single tokens, their keys, pages taken
   {
     S upto = pages[0];
 #pragma unroll
@@ -200,24 +201,22 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
         a.cached[r] = fits[u] ? before[u] : -1;
       }
       if (!fits[u]) count[u] = 0;
-      else next[4] += need[u];
+      else next[3] += need[u];
       if (count[u] > 0 && count[u] < a.least_tokens) {
-        next[2] += 1;
-        next[3] += before[u] + 1;
+        next[1] += 1;
+        next[2] += before[u] + 1;
       } else if (count[u] > 0) {
-        const S first = before[u] / kTile, last = (before[u] + count[u] - 1) / kTile;
-        next[0] += last - first + 1;
-        next[1] += (last - first + 1) * (first + last + 2) / 2;
+        next[0] += (before[u] + count[u] - 1) / kTile - before[u] / kTile + 1;
       }
     }
   }
   block_scan(next, next_total, warp_sums);
-  const int n_tiles = (int)next_total[0], singles = (int)next_total[2];
+  const int n_tiles = (int)next_total[0], singles = (int)next_total[1];
   // pieces of single tokens: about one wave of CTAs over all heads, or several where rows alone are more than that
   int piece_keys = kTile;
   if (singles > 0) {
     const int spread_over = 2 * singles <= a.wave_decode ? a.wave_decode - singles : kDecodeWaves * a.wave_decode;
-    const S keys = (next_total[3] + spread_over - 1) / spread_over;
+    const S keys = (next_total[2] + spread_over - 1) / spread_over;
     piece_keys = (int)max((S)kTile, (keys + kTile - 1) / kTile * kTile);
   }
   S pieces[1] = {0}, pieces_total[1] = {0};
@@ -227,8 +226,8 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       if (count[u] > 0 && count[u] < a.least_tokens) pieces[0] += before[u] / piece_keys + 1;
     block_scan(pieces, pieces_total, warp_sums);
   }
-  // Few tiles: their walks are cut so that all heads together fill the GPU.
-  const bool cut = n_tiles > 0 && 2 * n_tiles <= a.wave_tiles;
+  // Few tiles: their walks are cut so that all heads together are one wave of CTAs.
+  const bool cut = n_tiles > 0 && n_tiles < a.wave_tiles;
   {
     int tile_at = (int)next[0], piece_at = (int)pieces[0];
 #pragma unroll
@@ -254,21 +253,38 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       header[kPieceKeys] = piece_keys;
       header[kPagesWanted] = min(sums.page[t.rows], free_count);     // of the rows that are served: those up to the first that is not
       header[kFreeBefore] = free_count;
-      header[kFreeAfter] = free_count - (int)next_total[4];
+      header[kFreeAfter] = free_count - (int)next_total[3];
       header[kCut] = cut;
     }
   }
   __syncthreads();                                               // the sums, and who is served
-  if (cut) {                                                     // at most half a wave of 148 tiles; a piece takes at least four key tiles
-    const S per = (next_total[1] + (a.wave_tiles - n_tiles) - 1) / (a.wave_tiles - n_tiles);
-    const int piece_tiles = (int)max((S)4, per);
+  if (cut) {                                                     // a thread a tile, fewer than 148
     TileItem x{};
-    S parts[1] = {0}, parts_total[1];
     if (tid < n_tiles) {
       const int r = row_of(sums.tile, t.rows, tid);
       x = TileItem{r, sums.start[r], sums.before[r] / kTile + tid - sums.tile[r], tid, 0, 1, sums.before[r],
                    sums.before[r] + sums.start[r + 1] - sums.start[r]};
       reinterpret_cast<TileItem*>(a.work + a.layout.tiles)[tid] = x;
+      mi_s[tid] = x.mi;
+    }
+    __syncthreads();
+    if (tid < 32) {                                               // the shortest pieces, of four key tiles at least, that are one wave
+      int low = 4, high = 4;
+      for (int u = tid; u < n_tiles; u += 32) high = max(high, mi_s[u] + 1);
+      high = __reduce_max_sync(0xffffffffu, high);
+      while (low < high) {
+        const int middle = (low + high) >> 1;
+        int n = 0;
+        for (int u = tid; u < n_tiles; u += 32) n += (mi_s[u] + middle) / middle;
+        if (__reduce_add_sync(0xffffffffu, n) <= a.wave_tiles) high = middle;
+        else low = middle + 1;
+      }
+      if (tid == 0) header[kTileItems] = low;
+    }
+    __syncthreads();
+    const int piece_tiles = header[kTileItems];
+    S parts[1] = {0}, parts_total[1];
+    if (tid < n_tiles) {
       x.pieces = (x.mi + piece_tiles) / piece_tiles;
       parts[0] = x.pieces;
     }
@@ -536,8 +552,7 @@ int append(const Tables& t, const int* counts, int total, int max_length, int ma
     return SA_OK;
   };
   const int64_t most = (int64_t)t.rows * max(total + 1, min(max_length, t.max_pages << t.page_shift) + 1);
-  const int64_t walks = ((int64_t)total / kTile + 2 * t.rows) * (((int64_t)t.max_pages << t.page_shift) / kTile + 2);
-  const bool narrow = most < (1LL << 31) && 2 * walks < (1LL << 31);
+  const bool narrow = most < (1LL << 31);
   auto by_width = [&](auto per, int threads) {
     constexpr int kPer = decltype(per)::value;
     return narrow ? launch(append_kernel<kPer, int>, threads) : launch(append_kernel<kPer, long long>, threads);

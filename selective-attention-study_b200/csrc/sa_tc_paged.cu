@@ -317,7 +317,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
                   (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
                   SplitWalk{}, walk);
   };
-  const bool whole = (int64_t)2 * tiles_min > paged::tile_wave(a.heads);
+  const bool whole = tiles_min >= paged::tile_wave(a.heads);
   if (self) return whole ? wide(forward_wide_kernel<D, true, false, false, true>) : wide(forward_wide_kernel<D, true, false, true, true>);
   return whole ? wide(forward_wide_kernel<D, false, false, false, true>) : wide(forward_wide_kernel<D, false, false, true, true>);
 }
