@@ -7,7 +7,8 @@
 // sum of exponentials and its WIDTH largest logits.  choose_kernel (a CTA a group) makes the
 // beams' log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
-// Bound by memory where there are many beams, else by the latency of the two launches.
+// 256 beams of 50,304 bf16 logits (25.7 MB): 15 + 7 us, the first at 27 % of the copy rate: bound by issue (about 60 instructions for
+// 8 logits, two thirds of them for the exponentials) and by the start and end of its one wave; 4 beams 6 + 6 us, latency.
 //
 // The largest of a set, without sorting it: each warp that has elements gives the largest of its lanes' own maxima, about two times
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among

@@ -144,8 +144,8 @@ __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const 
 }
 
 // One CTA: PER rows a thread and four prefix sums over the rows; what is per page, tile or token (spread) here too where that is
-// little, else in a second kernel of many CTAs (a quarter of a million slots and 16,800 pages: 48 us in one CTA).  What a small
-// step takes is the chain of dependent loads, sums and barriers.  S: 32 bits where no sum can pass them.
+// little, else in a second kernel of many CTAs (512 rows with 264,000 tokens and 16,800 pages: 6 + 13 us; in one CTA 48).  Bound by
+// the chain of dependent loads, sums and barriers: 64 rows of one token 7 us.  S: 32 bits where no sum can pass them.
 template <int PER, typename S>
 __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Append a) {
   const Tables& t = a.t;
@@ -321,7 +321,8 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // page of a new row (a page that old and new row have at the same place counts for neither); (2) a reference less for each page
 // of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first, and takes the
 // pages for the copies off its end, in row order, while (4) the others write the tables.  A row for which there is none becomes
-// empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes.
+// empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes: 4 rows 10 us,
+// 256 rows of up to 47 pages 14 us.
 constexpr int kCluster = 8, kReorderThreads = 1024;
 
 // The work of a reordering, int32 words: how many rows change, then (row, parent, tokens, tokens of the page being filled) of
@@ -476,7 +477,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
 // The rows of `moved` in one layer.  The first history_ctas CTAs gather the history, 4 UNITS keys of one group over all rows, through shared
 // memory, since a row can be read and written: first everything is read, then everything is written.  The others copy the tokens
 // of the pages that are being filled into the pages that the copies got: kPagePieces CTAs a row and pool.
-// Bound by memory: 256 rows, half of them with a page of 64 tokens x 16 heads, two thirds with 16 histories of 1,500 keys.
+// Bound by memory, 65 MB in 20 us for 256 rows of which half get a page of 64 tokens of 16 heads, and two thirds 16 histories of 1,500
+// keys: half of the copy rate.  (A row of a warp in flight at a time, in two launches, took 28 us.)
 constexpr int kPagePieces = 4;
 template <int UNITS>
 __global__ void __launch_bounds__(256) move_kernel(const int4* __restrict__ moved, const int2* __restrict__ copies, float* selected, int groups,

