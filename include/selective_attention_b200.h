@@ -375,7 +375,8 @@ int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int tota
  * or every head its own).  Stores k and v in their pages, moves the histories on.
  *   k_pages, v_pages  (num_pages, heads, page_size, head_dim)
  *   selected          (rows, groups, max_pages * page_size) fp32
- *   q, k, v           (total, heads, head_dim) with token and head strides, multiples of 8 elements
+ *   total, max_length, max_count   as sa_page_append was given them for this plan
+ *   q, k, v           (total, heads, head_dim) with token and head strides, multiples of 8 elements, not 0
  *   y                 (total, heads, head_dim) contiguous; zeros for tokens without a slot
  *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream); 0: the call
  *                     clears tickets of its own

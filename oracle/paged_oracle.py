@@ -117,7 +117,7 @@ def attend(q, k, v, history, cached, exempt, per_head):
         # relative error of a probability: the logit's own (32-bit sums of D products and of the history), its rounding, and the
         # selection's; y = sum p v / sum p has it once above and once below the line
         small = 2.0 ** -23 * ((d + 4) * sizes[x] + 4 * before[s]) + 2.0 ** -20
-        rel = torch.expm1(2.0 ** -8 * inside[s] + small).masked_fill(j > i, 0.0)
+        rel = torch.expm1(2.0 ** -8 * inside[s] + small).masked_fill((j > i) | torch.isinf(before[s]), 0.0)      # (no weight at all)
         y_off[:, x] = (p * (rel + 2.0 ** -8 * (1 + rel))) @ v[:, x].abs() + (p * rel).sum(-1, keepdim=True) * y[:, x].abs()
     y_off = 2.0 ** -8 * y.abs() + (1 + 2.0 ** -8) * y_off + 1e-30             # the output's own rounding
     return y, after, y_off, after_off

@@ -115,7 +115,7 @@ int sa_paged_run(const sa_paged_attention* in) {
     if (!aligned(p, 16)) return SA_ERR_ALIGNMENT;
   if (!aligned(in->workspace, 256) || !aligned(in->selected, 4)) return SA_ERR_ALIGNMENT;
   for (const int64_t* s : {in->q_stride, in->k_stride, in->v_stride})
-    if (s[0] % 8 != 0 || s[1] % 8 != 0) return SA_ERR_ALIGNMENT;
+    if (s[0] % 8 != 0 || s[1] % 8 != 0 || s[0] <= 0 || s[1] <= 0) return SA_ERR_ALIGNMENT;
   if (in->workspace_bytes < paged::attention_scratch(a).floats * 4) return SA_ERR_WORKSPACE;
   if (tc::timeout_pending()) return SA_ERR_DEVICE_TIMEOUT;
   a.query_start = in->query_start; a.cached = in->cached; a.slots = in->slots; a.work = in->work;

@@ -483,7 +483,9 @@ Tensor paged_attention(const PageTables& t, const PageStep& step, const Tensor& 
   if (total == 0) return y;
   auto prepare = [&](const Tensor& x) {
     const Tensor c = x.scalar_type() == at::kBFloat16 ? x : x.to(at::kBFloat16);
-    const bool ok = c.stride(2) == 1 && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 && c.stride(0) % 8 == 0 && c.stride(1) % 8 == 0;
+    // rows at multiples of 16 bytes, none broadcast (a tensor map has no stride of 0)
+    const bool ok = c.stride(2) == 1 && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 && c.stride(0) > 0 && c.stride(0) % 8 == 0 &&
+                    c.stride(1) > 0 && c.stride(1) % 8 == 0;
     return ok ? c : c.clone(at::MemoryFormat::Contiguous);
   };
   const Tensor q = prepare(q_in), k = prepare(k_in), v = prepare(v_in);

@@ -132,3 +132,51 @@ def test_beam_search_over_the_paged_cache():
         for page in t["block_tables"][r, :-(-length // 16)].tolist():
             refs[page] += 1
     assert torch.equal(refs, t["page_refs"].cpu()) and int((refs == 0).sum()) == int(t["free_count"])
+
+
+def test_a_captured_search_step_is_replayed():
+    """Selection, reordering, moves, tables and attention of a step in one graph, against the same calls one by one."""
+    gen = torch.Generator().manual_seed(12)
+    vocab, h, d, n, groups = 211, 4, 64, 3, 2
+    table = torch.randn(vocab, 3, h, d, generator=gen).bfloat16().cuda()
+    head = (torch.randn(h * d, vocab, generator=gen) * 0.2).cuda()
+    rows = n * groups
+
+    class Search:
+        def __init__(self):
+            self.t = paged.begin_tables(rows, 80, 16, 10, h)
+            self.cache = paged.begin_pages(self.t, d)
+            counts = torch.tensor([30, 0, 0, 47, 0, 0], dtype=torch.int32).cuda()
+            step = paged.append_tokens(self.t, counts, 77)
+            qkv = table[torch.arange(77, device="cuda")]
+            y = paged.paged_attention(self.cache, self.t, step, *(qkv[:, i] for i in range(3)))
+            self.y = y[(step["query_start"][1:].long() - 1).clamp_min(0)].float().reshape(rows, -1)
+            self.scores = torch.tensor([[0.0] + [-float("inf")] * (n - 1)] * groups).cuda()
+            self.ones = torch.ones(rows, dtype=torch.int32).cuda()
+
+        def step(self):
+            scores, parents, tokens = beams.beam_select((self.y @ head).view(groups, n, vocab), self.scores, n)
+            paged.move_rows(self.cache, paged.reorder_rows(self.t, parents.reshape(-1)))
+            step = paged.append_tokens(self.t, self.ones, rows, max_count=1)
+            qkv = table[tokens.reshape(-1)]
+            y = paged.paged_attention(self.cache, self.t, step, *(qkv[:, i] for i in range(3)))
+            self.scores.copy_(scores)
+            self.y.copy_(y.float().reshape(rows, -1))
+            return tokens, parents
+
+    eager, captured = Search(), Search()
+    want = [[x.clone() for x in eager.step()] for _ in range(20)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        warm = Search()
+        warm.step()                                                # the library's set-up calls come before a capture
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = captured.step()
+    for tokens, parents in want:
+        graph.replay()
+        assert torch.equal(out[0], tokens) and torch.equal(out[1], parents)
+    assert torch.equal(captured.y, eager.y) and torch.equal(captured.scores, eager.scores)
+    for name in ("block_tables", "lengths", "page_refs", "free_count"):
+        assert torch.equal(captured.t[name], eager.t[name])

@@ -245,6 +245,78 @@ def test_outputs_equal_the_dense_cache():
     torch.testing.assert_close(cache["selected"][:, :, :n], dense["selected"][:, :, :n], atol=1e-4, rtol=1e-5)
 
 
+def test_tokens_of_any_strides():
+    """Broadcast heads and tokens, rows at odd addresses, other types: as their contiguous bf16 form."""
+    s = _prefix(4, 64, False, [70, 300])
+    caches = [{name: x.clone() for name, x in s.cache.items()} for _ in range(6)]
+    step = paged.append_tokens(s.t, _ints([33, 1]), 34)
+    q, k, v = (x.cuda() for x in s.tokens(34))
+    k, v = k[:, :1].expand(-1, 4, -1), v[:1].expand(34, -1, -1)
+    wide = torch.zeros(34, 4, 67, device="cuda", dtype=torch.bfloat16)
+    wide[:, :, 3:] = q
+    forms = [(q, k.contiguous(), v.contiguous()), (q, k, v), (wide[:, :, 3:], k, v), (q.float(), k.float(), v.half()),
+             (q.transpose(1, 2).contiguous().transpose(1, 2), k, v), (q[:, :1].expand(-1, 4, -1), k, v)]
+    ys = [paged.paged_attention(cache, s.t, step, *x) for cache, x in zip(caches, forms)]
+    for y, cache in zip(ys[1:5], caches[1:5]):
+        assert torch.equal(y, ys[0])
+        for name in ("k", "v", "selected"):
+            assert torch.equal(torch.nan_to_num(cache[name]), torch.nan_to_num(caches[0][name]))
+    assert torch.isfinite(ys[5].float()).all()
+
+
+@pytest.mark.parametrize("heads,per_head", [(2, False), (16, False), (4, True)])
+def test_keys_that_were_taken_out(heads, per_head):
+    """Keys whose history their owner has made infinite have no weight: as if they were not there."""
+    lengths = [500, 200, 64]
+    s = _prefix(heads, 64, per_head, lengths)
+    gone = slice(16, 400)                                          # whole tiles and pages of row 0, a part of the others'
+    for r, n in enumerate(lengths):
+        s.cache["selected"][r, :, gone.start:min(gone.stop, n)] = float("inf")
+        keys, values, history = s.rows[r]
+        s.rows[r] = (keys, values, torch.cat([history[:, :16], torch.full_like(history[:, gone], float("inf")), history[:, 400:]], 1))
+    for counts in ([1, 1, 1], [130, 40, 500], [1, 1, 1]):
+        n = sum(counts)
+        step = _append(s.t, s.want, counts, n)
+        q, k, v = s.tokens(n)
+        y = s.slot.attend_pages(q.cuda(), k.cuda(), v.cuda(), s.cache, s.t, step)
+        s.expect(counts, step["query_start"].tolist(), step["cached"].tolist(), q, k, v, y)
+        got = s.cache["selected"].cpu()
+        for r, (_, _, history) in enumerate(s.rows):
+            assert torch.equal(torch.isinf(got[r, :, :history.shape[1]]), torch.isinf(history))
+
+
+def test_many_rows():
+    """More rows than a thread has in the plan's sums, and more walks and pieces than CTAs that are resident."""
+    rows, rng = 1100, random.Random(8)
+    s = Served(rows, 2, 64, 16, 10, 5 * rows, scale=0.7, seed=9)
+    s.step([rng.choice([0, 1, 2, 3, 40]) for _ in range(rows)])
+    s.step([rng.choice([0, 1]) for _ in range(rows)], max_count=1)
+    s.step([rng.choice([0, 1, 1, 5]) for _ in range(rows)])
+
+
+def test_pools_beyond_32_bit_offsets():
+    """Pages whose elements lie beyond 2^31: the same numbers as in a small pool."""
+    h, d, page = 16, 64, 32
+    outs = []
+    for num_pages in (80, 70000):                                  # 70,000 pages of 32 x 1,024 elements
+        t = paged.begin_tables(2, num_pages, page, 40, h)
+        t["free_pages"].copy_(torch.arange(num_pages, dtype=torch.int32))          # the last pages first
+        cache = paged.begin_pages(t, d)
+        gen = torch.Generator().manual_seed(4)
+        got = []
+        for counts in ([500, 77], [1, 1], [200, 40], [1, 1]):
+            step = paged.append_tokens(t, _ints(counts), sum(counts))
+            x = [torch.randn(sum(counts), h, d, generator=gen).bfloat16().cuda() for _ in range(3)]
+            got.append(paged.paged_attention(cache, t, step, *x))
+        moves = paged.reorder_rows(t, _ints([0, 0]))
+        paged.move_rows(cache, moves)
+        step = paged.append_tokens(t, _ints([1, 1]), 2)
+        got.append(paged.paged_attention(cache, t, step, *(torch.randn(1, h, d, generator=gen).bfloat16().cuda().repeat(2, 1, 1) for _ in range(3))))
+        assert torch.equal(got[-1][0], got[-1][1]) and (num_pages == 80 or int(t["block_tables"].max()) == num_pages - 1)
+        outs.append(got + [cache["selected"]])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_pages_outside_the_pool_read_as_zeros():
     """A table that its owner has damaged: nothing outside the pools is read or written."""
     h, d = 2, 64

@@ -112,7 +112,7 @@ def test_bad_attention_is_refused_before_any_launch():
     assert status()[0] == 4 and status()[1] > 0                    # workspace_bytes 0
     assert status(struct_bytes=8) == (1, 0) and status(exempt=0)[0] == 1 and status(total=0)[0] == 1 and status(max_length=129)[0] == 1
     assert status(head_dim=32)[0] == 2 and status(groups=3)[0] == 2 and status(q=None)[0] == 1 and status(y=None)[0] == 1
-    assert status(k_pages=4104)[0] == 3 and status(q_stride=[128, 68])[0] == 3 and status(workspace=4112)[0] == 3
+    assert status(k_pages=4104)[0] == 3 and status(q_stride=[128, 68])[0] == 3 and status(v_stride=[128, 0])[0] == 3 and status(workspace=4112)[0] == 3
 
 
 def test_bad_selections_are_refused_before_any_launch():
