@@ -386,10 +386,48 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
+// Several tensors in one allocation: `bytes` of each, from 256-byte boundaries on.
+struct Carved {
+  Tensor base;
+  int64_t at = 0;
+  static int64_t room(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+  Carved(int64_t bytes, const Tensor& like) : base(fresh({bytes}, at::kByte, like)) {}
+  Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    at += room((int64_t)t.nbytes());
+    return t;
+  }
+};
+
 struct PageTables {                               // paged.begin_tables
   Tensor block_tables, lengths, free_pages, free_count, page_refs;
   int64_t page_size, heads;
 };
+
+// The tables out of their dict; what is missing is a KeyError, as in Python.
+PageTables tables_in(const pybind11::dict& d) {
+  static PyObject* const keys[7] = {PyUnicode_InternFromString("block_tables"), PyUnicode_InternFromString("lengths"),
+                                    PyUnicode_InternFromString("free_pages"),   PyUnicode_InternFromString("free_count"),
+                                    PyUnicode_InternFromString("page_refs"),    PyUnicode_InternFromString("page_size"),
+                                    PyUnicode_InternFromString("heads")};
+  PyObject* found[7];
+  for (int i = 0; i < 7; ++i) {
+    found[i] = PyDict_GetItemWithError(d.ptr(), keys[i]);
+    if (found[i] == nullptr) {
+      if (!PyErr_Occurred()) PyErr_SetObject(PyExc_KeyError, keys[i]);
+      throw pybind11::error_already_set();
+    }
+    TORCH_CHECK_TYPE(i >= 5 || THPVariable_Check(found[i]), "page tables must be tensors");
+  }
+  PageTables t;
+  Tensor* const to[5] = {&t.block_tables, &t.lengths, &t.free_pages, &t.free_count, &t.page_refs};
+  for (int i = 0; i < 5; ++i) *to[i] = THPVariable_Unpack(found[i]);
+  t.page_size = pybind11::cast<int64_t>(pybind11::handle(found[5]));
+  t.heads = pybind11::cast<int64_t>(pybind11::handle(found[6]));
+  return t;
+}
 
 sa_page_tables tables_of(const PageTables& t) {
   TORCH_CHECK_VALUE(t.block_tables.dim() == 2 && t.lengths.dim() == 1 && t.free_pages.dim() == 1 && t.page_refs.dim() == 1 &&
@@ -429,7 +467,8 @@ struct PageStep {
   uint64_t stream, capture;
 };
 
-pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t total, int64_t max_length, int64_t max_count) {
+pybind11::tuple append_tokens(const pybind11::dict& tables, const Tensor& counts, int64_t total, int64_t max_length, int64_t max_count) {
+  const PageTables t = tables_in(tables);
   const sa_page_tables p = tables_of(t);
   check_int32(counts, t, p.rows, "counts");
   TORCH_CHECK_VALUE(total >= 0 && total <= (1 << 30), "total must be the number of the step's tokens; got ", total);
@@ -439,8 +478,9 @@ pybind11::tuple append_tokens(const PageTables& t, const Tensor& counts, int64_t
   max_length = std::min(max_length, capacity);
   max_count = std::min({max_count, max_length, std::max<int64_t>(total, 1)});
   const int64_t words = (int64_t)sa_page_step_words(p.rows, (int)total, p.heads);
-  const Tensor work = fresh({words}, at::kInt, t.lengths), query_start = fresh({p.rows + 1}, at::kInt, t.lengths),
-               cached = fresh({p.rows}, at::kInt, t.lengths), slots = fresh({total}, at::kLong, t.lengths);
+  Carved all(Carved::room(4 * words) + Carved::room(4 * (p.rows + 1)) + Carved::room(4 * p.rows) + Carved::room(8 * total), t.lengths);
+  const Tensor work = all.take({words}, at::kInt), query_start = all.take({p.rows + 1}, at::kInt), cached = all.take({p.rows}, at::kInt),
+               slots = all.take({total}, at::kLong);
   void* const stream = stream_of(t.lengths);
   check("sa_page_append", sa_page_append(&p, counts.data_ptr<int32_t>(), (int)total, (int)max_length, (int)max_count,
                                          query_start.data_ptr<int32_t>(), cached.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
@@ -463,8 +503,10 @@ void check_pools(const PageTables& t, const sa_page_tables& p, const Tensor& kc,
   TORCH_CHECK_VALUE(kc.size(3) == 64 || kc.size(3) == 128, "head_dim must be 64 or 128 in a paged cache; got ", kc.size(3));
 }
 
-Tensor paged_attention(const PageTables& t, const PageStep& step, const Tensor& kc, const Tensor& vc, const Tensor& selected, const Tensor& q_in,
-                       const Tensor& k_in, const Tensor& v_in, int64_t exempt) {
+Tensor paged_attention(const pybind11::dict& tables, const PageStep& step, const Tensor& kc, const Tensor& vc, const Tensor& selected,
+                       const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, int64_t exempt) {
+  const PageTables t = tables_in(tables);
+  const pybind11::gil_scoped_release release;
   const sa_page_tables p = tables_of(t);
   check_pools(t, p, kc, vc, selected);
   const int64_t total = step.slots.numel(), h = p.heads, d = kc.size(3);
@@ -515,17 +557,21 @@ Tensor paged_attention(const PageTables& t, const PageStep& step, const Tensor& 
   return y;
 }
 
-pybind11::tuple reorder_rows(const PageTables& t, const Tensor& parents) {
+pybind11::tuple reorder_rows(const pybind11::dict& tables, const Tensor& parents) {
+  const PageTables t = tables_in(tables);
   const sa_page_tables p = tables_of(t);
   check_int32(parents, t, p.rows, "parents");
   const c10::cuda::CUDAGuard guard(t.block_tables.device());
-  const Tensor copies = fresh({p.rows, 2}, at::kInt, parents);
-  const Tensor work = fresh({(int64_t)sa_page_reorder_words(p.rows, p.max_pages, p.num_pages)}, at::kInt, parents);
+  const int64_t words = (int64_t)sa_page_reorder_words(p.rows, p.max_pages, p.num_pages);
+  Carved all(Carved::room(8 * p.rows) + Carved::room(4 * words), parents);
+  const Tensor copies = all.take({p.rows, 2}, at::kInt), work = all.take({words}, at::kInt);
   check("sa_page_reorder", sa_page_reorder(&p, parents.data_ptr<int32_t>(), copies.data_ptr<int32_t>(), work.data_ptr<int32_t>(), stream_of(t.lengths)));
   return pybind11::make_tuple(copies, work);
 }
 
-void move_rows(const PageTables& t, const Tensor& copies, const Tensor& work, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
+void move_rows(const pybind11::dict& tables, const Tensor& copies, const Tensor& work, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
+  const PageTables t = tables_in(tables);
+  const pybind11::gil_scoped_release release;
   const sa_page_tables p = tables_of(t);
   check_pools(t, p, kc, vc, selected);
   check_int32(copies, t, 2 * (int64_t)p.rows, "the moves' copies");
@@ -547,7 +593,8 @@ pybind11::tuple beam_select(const Tensor& logits_in, const Tensor& scores_in, in
   const c10::cuda::CUDAGuard guard(logits_in.device());
   const Tensor logits = logits_in.stride(2) == 1 || vocab == 1 ? logits_in : logits_in.contiguous();
   const Tensor scores = (scores_in.scalar_type() == at::kFloat ? scores_in : scores_in.to(at::kFloat)).contiguous();
-  const Tensor out = fresh({g, width}, at::kFloat, scores), rows = fresh({g, width}, at::kInt, scores), tokens = fresh({g, width}, at::kLong, scores);
+  Carved all(2 * Carved::room(4 * g * width) + Carved::room(8 * g * width), scores);
+  const Tensor out = all.take({g, width}, at::kFloat), rows = all.take({g, width}, at::kInt), tokens = all.take({g, width}, at::kLong);
   sa_beam a{};
   a.struct_bytes = sizeof(sa_beam);
   a.dtype = code_of(logits); a.groups = (int32_t)g; a.beams = (int32_t)k; a.vocab = (int32_t)vocab; a.width = (int32_t)width;
@@ -572,12 +619,10 @@ PYBIND11_MODULE(_native, m) {
   m.def("prefill_rows", &prefill_rows, nogil());
   m.def("store_rows", &store_rows, nogil());
   m.def("decode", &decode);
-  pybind11::class_<PageTables>(m, "PageTables")
-      .def(pybind11::init<Tensor, Tensor, Tensor, Tensor, Tensor, int64_t, int64_t>());
   pybind11::class_<PageStep>(m, "PageStep");
   m.def("append_tokens", &append_tokens);
-  m.def("paged_attention", &paged_attention, nogil());
+  m.def("paged_attention", &paged_attention);
   m.def("reorder_rows", &reorder_rows);
-  m.def("move_rows", &move_rows, nogil());
+  m.def("move_rows", &move_rows);
   m.def("beam_select", &beam_select);
 }

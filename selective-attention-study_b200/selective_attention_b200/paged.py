@@ -54,11 +54,6 @@ def begin_pages(tables: dict, head_dim: int, per_head: bool = False) -> dict:
             "selected": torch.zeros(rows, heads if per_head else 1, max_pages * page, dtype=torch.float32, device=device)}
 
 
-def _tables(tables: dict):
-    return _lib.native().PageTables(tables["block_tables"], tables["lengths"], tables["free_pages"], tables["free_count"],
-                                    tables["page_refs"], tables["page_size"], tables["heads"])
-
-
 def append_tokens(tables: dict, counts: torch.Tensor, total: int, max_length: int | None = None, max_count: int | None = None) -> dict:
     """Row r gets ``counts[r]`` (int32, on the GPU) new tokens; the tables have their pages afterwards.  ``total``: how many tokens the
     step has; q, k, v of its attention hold them row after row.
@@ -73,7 +68,7 @@ def append_tokens(tables: dict, counts: torch.Tensor, total: int, max_length: in
     native = _lib.native()
     most = tables["block_tables"].shape[1] * tables["page_size"]
     max_length = most if max_length is None else int(max_length)
-    made = native.append_tokens(_tables(tables), counts, int(total), max_length, most if max_count is None else int(max_count))
+    made = native.append_tokens(tables, counts, int(total), max_length, most if max_count is None else int(max_count))
     return {"query_start": made[0], "cached": made[1], "slots": made[2], "_plan": made[3]}
 
 
@@ -84,7 +79,7 @@ def paged_attention(cache: dict, tables: dict, step: dict, q: torch.Tensor, k: t
 
     One call per layer and step; calls of one step on one stream share its plan.  Nothing behind a row's last token is read
     into a result or written."""
-    return _lib.native().paged_attention(_tables(tables), step["_plan"], cache["k"], cache["v"], cache["selected"], q, k, v,
+    return _lib.native().paged_attention(tables, step["_plan"], cache["k"], cache["v"], cache["selected"], q, k, v,
                                          kernels._check_exempt(exempt))
 
 
@@ -96,10 +91,10 @@ def reorder_rows(tables: dict, parents: torch.Tensor) -> dict:
     parent; the others get a page of their own, and ``move_rows`` copies its tokens in every layer: "copies" (rows, 2) int32
     holds source and target, or -1, -1.  Pages that nobody holds any more go back first, lowest first.  A row that needs a page
     when there is none becomes empty."""
-    copies, work = _lib.native().reorder_rows(_tables(tables), parents)
+    copies, work = _lib.native().reorder_rows(tables, parents)
     return {"copies": copies, "tables": tables, "_work": work}
 
 
 def move_rows(cache: dict, moves: dict) -> None:
     """Carries out ``moves`` in one layer: the tokens of the copied pages, and the histories of the rows."""
-    _lib.native().move_rows(_tables(moves["tables"]), moves["copies"], moves["_work"], cache["k"], cache["v"], cache["selected"])
+    _lib.native().move_rows(moves["tables"], moves["copies"], moves["_work"], cache["k"], cache["v"], cache["selected"])
