@@ -14,6 +14,8 @@
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among
 // themselves.  Where more than kList reach it, because many are equal to it (masked logits, most often), those above it are ranked
 // and the first of the equal ones are found in order; where that is not so either, they are taken one by one.
+#include <type_traits>
+
 #include "sa_common.cuh"
 #include "sa_beam.cuh"
 #include "sa_tc_ptx.cuh"
@@ -39,7 +41,6 @@ __device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& 
 template <typename V, typename I>
 struct Shared {
   V tops[2 * kMaxWidth];
-  V bound;
   Entry<V, I> list[kList];
   int count;
   Entry<V, I> warp_best[kThreads / 32];
@@ -50,13 +51,13 @@ __device__ __forceinline__ float warp_max(float x) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(x));
   return top;
 }
+// (no NaN) by the bits, as a whole number whose order is the values': its upper half, then the lower one of those that have that
 __device__ __forceinline__ double warp_max(double x) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    const double o = __shfl_xor_sync(0xffffffffu, x, s);
-    x = o > x ? o : x;
-  }
-  return x;
+  const long long bits = __double_as_longlong(x), key = bits ^ ((bits >> 63) & 0x7fffffffffffffffLL);
+  const int high = (int)(key >> 32), top = __reduce_max_sync(0xffffffffu, high);
+  const unsigned low = __reduce_max_sync(0xffffffffu, high == top ? (unsigned)key : 0u);
+  const long long best = ((long long)top << 32) | low;
+  return __longlong_as_double(best ^ ((best >> 63) & 0x7fffffffffffffffLL));
 }
 
 // Calls emit(rank, value, index) for the `width` first of the CTA's elements, which the first `warps` warps have.  `mine` is the
@@ -78,14 +79,20 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, 
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  if (tid < given) {
-    const V own = sh.tops[tid];
-    int rank = 0;
-    for (int u = 0; u < given; ++u) rank += sh.tops[u] > own || (sh.tops[u] == own && u < tid) ? 1 : 0;
-    if (rank == width - 1) sh.bound = own;
+  V bound;                                                  // the `width`-th of them: every warp finds it for itself
+  {
+    const V own[2] = {lane < given ? sh.tops[lane] : kNone, lane + 32 < given ? sh.tops[lane + 32] : kNone};
+    int rank[2] = {0, 0};
+#pragma unroll 8
+    for (int u = 0; u < given; ++u) {
+      const V other = sh.tops[u];
+      rank[0] += other > own[0] || (other == own[0] && u < lane) ? 1 : 0;
+      if (given > 32) rank[1] += other > own[1] || (other == own[1] && u < lane + 32) ? 1 : 0;
+    }
+    const unsigned first = __ballot_sync(0xffffffffu, lane < given && rank[0] == width - 1);
+    const unsigned second = __ballot_sync(0xffffffffu, lane + 32 < given && rank[1] == width - 1);
+    bound = first != 0u ? __shfl_sync(0xffffffffu, own[0], __ffs(first) - 1) : __shfl_sync(0xffffffffu, own[1], __ffs(second) - 1);
   }
-  __syncthreads();
-  const V bound = sh.bound;
   reach(bound, false, [&](V x, I i) {
     const int at = atomicAdd(&sh.count, 1);
     if (at < kList) sh.list[at] = Entry<V, I>{x, i};
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
   extern __shared__ __align__(128) uint4 run[];
   __shared__ uint64_t arrived[kParts];
   __shared__ Shared<float, int> sh;
-  __shared__ float red[2][kThreads / 32];
+  __shared__ float2 red[kThreads / 32];
   __shared__ int sums_s[kThreads / 32];
   const int n = blockIdx.x / chunks, chunk = blockIdx.x - n * chunks;      // n: beam over all groups
   const int g = n / beams;
@@ -231,58 +238,67 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
   // The run's maximum (NaNs aside) and its sum of exponentials (with them), by thread with a maximum of its own.
   // +inf: inf - inf, a NaN as a NaN among the logits: the beam has no finite sum.
   float mine = -INFINITY, sum = 0.f;
-  auto take = [&](int u) {
-    const uint4 raw = run[u];
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[kPer], top = mine;
+  auto take = [&](int u, auto n_units) {                       // n_units of them, kThreads apart
+    constexpr int kUnits = decltype(n_units)::value;
+    float x[kUnits][kPer], top = mine;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      x[i] = W::at(w[i / W::kPer], i % W::kPer);
-      top = fmaxf(top, x[i]);
+    for (int o = 0; o < kUnits; ++o) {
+      const uint4 raw = run[u + o * kThreads];
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[o][i] = W::at(w[i / W::kPer], i % W::kPer);
     }
+#pragma unroll
+    for (int o = 0; o < kUnits; ++o)
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) top = fmaxf(top, fmaxf(x[o][i], x[o][i + 1]));
     const float from = top == -INFINITY ? 0.f : top;
     if (top > mine) sum *= tc::ex2((mine - from) * kLog2e);
     mine = top;
     const float2 shift = make_float2(-from, -from), scale = make_float2(kLog2e, kLog2e);
-    float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kPer; i += 2) {
-      const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), shift), scale);
-      part = __fadd2_rn(part, make_float2(tc::ex2(d.x), tc::ex2(d.y)));
+    for (int o = 0; o < kUnits; ++o) {
+      float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[o][i], x[o][i + 1]), shift), scale);
+        part = __fadd2_rn(part, make_float2(tc::ex2(d.x), tc::ex2(d.y)));
+      }
+      sum += part.x + part.y;
     }
-    sum += part.x + part.y;
   };
   int here = whole0, part = 0;                              // units below `here` have arrived
-  for (int u = tid; u < count; u += kThreads) {
+  auto arrive = [&](int u) {
     for (; u >= here && part < kParts; here = min(here + part_units, whole1)) tc::mbar_wait(&arrived[part++], 0, status, 700);
-    take(u);
+  };
+  int u = tid;
+  for (; u + kThreads < count; u += 2 * kThreads) {
+    arrive(u + kThreads);
+    take(u, std::integral_constant<int, 2>{});
+  }
+  if (u < count) {
+    arrive(u);
+    take(u, std::integral_constant<int, 1>{});
   }
   for (; part < kParts; ++part) tc::mbar_wait(&arrived[part], 0, status, 700);
-  float top = warp_max(mine);
-  if ((tid & 31) == 0) red[0][tid >> 5] = top;
-  __syncthreads();
+  {
+    const float top = warp_max(mine);
+    if (top != -INFINITY) sum *= tc::ex2((mine - top) * kLog2e);
 #pragma unroll
-  for (int u = 0; u < kThreads / 32; ++u) top = fmaxf(top, red[0][u]);
-  if (top != -INFINITY) sum *= tc::ex2((mine - top) * kLog2e);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  if ((tid & 31) == 0) red[1][tid >> 5] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    for (int u = 1; u < kThreads / 32; ++u) sum += red[1][u];
-    sums[blockIdx.x] = make_float2(top, sum);
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    if ((tid & 31) == 0) red[tid >> 5] = make_float2(top, sum);
   }
   auto hits_of = [&](int u, auto wanted) {                     // which elements of a unit, a bit each (a NaN is never chosen)
     const uint4 raw = run[u];
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    const int64_t v = (int64_t)(unit0 + u) * kPer - lead;
+    const unsigned v = (unsigned)(unit0 + u) * kPer - lead;     // (of an element before the row: above every place)
     unsigned hits = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (wanted(fmaxf(W::at(w[i / W::kPer], i % W::kPer), -INFINITY)) && v + i >= 0 && v + i < vocab) hits |= 1u << i;
+      if (wanted(fmaxf(W::at(w[i / W::kPer], i % W::kPer), -INFINITY)) && v + i < (unsigned)vocab) hits |= 1u << i;
     return hits;
   };
-  // Few threads have anything to give: where they have many units, each one's are looked through by its whole warp.
+  // Few threads have anything to give: where they have many units, each one's are looked through by half of its warp.
   auto reach = [&](float bound, bool above, auto f) {
     bool more = true;
     auto take_unit = [&](int u) {
@@ -296,8 +312,12 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
       for (int u = tid; u < count && any && more; u += kThreads) take_unit(u);
       return;
     }
-    for (unsigned left = __ballot_sync(0xffffffffu, any); left != 0u; left &= left - 1u) {
-      for (int u = (tid & ~31) + __ffs(left) - 1 + (tid & 31) * kThreads; u < count && more; u += 32 * kThreads) take_unit(u);
+    for (unsigned left = __ballot_sync(0xffffffffu, any); left != 0u;) {
+      const unsigned rest = left & (left - 1u);
+      const unsigned whose = (tid & 16) == 0 ? left : rest;
+      if (whose != 0u)
+        for (int u = (tid & ~31) + __ffs(whose) - 1 + (tid & 15) * kThreads; u < count && more; u += 16 * kThreads) take_unit(u);
+      left = rest & (rest - 1u);
       __syncwarp();
     }
   };
@@ -338,51 +358,73 @@ __global__ void __launch_bounds__(kThreads, 4) candidates_kernel(const T* __rest
     out_v[at] = v;
     out_t[at] = i;
   });
+  if (tid == kThreads - 32) {                                  // (barriers are behind it; the first warps are still ranking)
+    float top = red[0].x, all = 0.f;
+#pragma unroll
+    for (int u = 1; u < kThreads / 32; ++u) top = fmaxf(top, red[u].x);
+    const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < kThreads / 32; ++u) all += red[u].y * (red[u].x == top ? 1.f : tc::ex2((red[u].x - from) * kLog2e));
+    sums[blockIdx.x] = make_float2(top, all);
+  }
 }
 
-__global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restrict__ scores, int beams, int vocab, int width, int chunks,
+constexpr int kKept = 4;               // candidates of a thread of choose_kernel that are on their way while the sums are made
+
+// MANY: more candidates than the threads keep at hand.  They are lists in order, WIDTH of each run, so the first of a list is its
+// largest, and a list is read until it falls below the bound.  A run's list counts as 2^split of them, of every 2^split-th entry.
+// (32 beams of 50,304, 13,312 candidates to a group, choose_kernel alone: 68 us with every candidate looked at, CHOOSE_MANY so.)
+template <bool MANY>
+__global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restrict__ scores, int beams, int vocab, int width, int chunks, int split,
                                                           const float2* __restrict__ sums, const float* __restrict__ values,
                                                           const int* __restrict__ tokens, float* __restrict__ out_scores,
                                                           int* __restrict__ out_rows, long long* __restrict__ out_tokens) {
-  tc::after_previous_kernel();
   __shared__ Shared<double, long long> sh;
   __shared__ double base[kMaxBeams];                         // score - log-sum-exp of a beam; NaN: all of its scores are -inf
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  // candidate of this thread in every 256: a warp has every eighth, of all beams (of a poor beam alone, its maximum would let
-  // all of the others' candidates pass)
+  // element (a candidate, or a list of MANY) of this thread in every 256: a warp has every eighth, of all beams (of a poor beam alone,
+  // its maximum would let all of the others' candidates pass)
   const int place = lane * (kThreads / 32) + (tid >> 5);
   const int per_beam = chunks * width, n = beams * per_beam;
   const int64_t first = (int64_t)g * n;
-  constexpr int kKept = 4;                                   // candidates of a thread that are on their way meanwhile
   float kept_v[kKept];
-  int kept_t[kKept];
+  int kept_t[kKept], kept_k[kKept];
+  if constexpr (!MANY) {
 #pragma unroll
-  for (int u = 0; u < kKept; ++u) {
-    const int i = place + u * kThreads;
-    kept_v[u] = i < n ? values[first + i] : 0.f;
-    kept_t[u] = i < n ? tokens[first + i] : -1;
+    for (int u = 0; u < kKept; ++u) kept_k[u] = (place + u * kThreads) / per_beam;
   }
-  for (int k = tid >> 5; k < beams; k += kThreads / 32) {
-    const float2* part = sums + ((int64_t)g * beams + k) * chunks;
-    float top = -INFINITY;
-    for (int c = lane; c < chunks; c += 32) top = fmaxf(top, part[c].x);
+  if (tid < beams) base[tid] = (double)scores[(int64_t)g * beams + tid];      // (there before the logits are)
+  tc::after_previous_kernel();
+  if constexpr (!MANY) {
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    for (int u = 0; u < kKept; ++u) {
+      const int i = place + u * kThreads;
+      kept_v[u] = i < n ? values[first + i] : 0.f;
+      kept_t[u] = i < n ? tokens[first + i] : -1;
+    }
+  }
+  __syncthreads();                                           // the scores
+  int lanes = 32;                                            // of a beam
+  while (lanes > 1 && lanes / 2 >= chunks && kThreads / lanes < beams) lanes /= 2;
+  for (int k0 = 0; k0 < beams; k0 += kThreads / lanes) {
+    const int k = k0 + tid / lanes;
+    const float2* part = sums + ((int64_t)g * beams + min(k, beams - 1)) * chunks;
+    float top = -INFINITY;
+    for (int c = tid & (lanes - 1); c < chunks; c += lanes) top = fmaxf(top, part[c].x);
+    for (int s = lanes / 2; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
     double sum = 0.0;
-    for (int c = lane; c < chunks; c += 32) {
+    for (int c = tid & (lanes - 1); c < chunks; c += lanes) {
       const float2 p = part[c];
       if (p.y != 0.f) sum += (double)p.y * exp2f((p.x - top) * kLog2e);         // 0: nothing but -inf; a NaN stays
     }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    if (lane == 0) {
-      const double b = (double)scores[(int64_t)g * beams + k] - ((double)top + log(sum));
+    for (int s = lanes / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    if ((tid & (lanes - 1)) == 0 && k < beams) {
+      const double b = base[k] - ((double)top + log(sum));
       base[k] = isfinite(b) ? b : nan("");
     }
   }
   __syncthreads();
-  auto one = [&](int i, float value, int token, auto f) {    // f(score, place): beam in the upper half of the place, token in the lower
-    const int k = i / per_beam;
+  auto one = [&](int i, int k, float value, int token, auto f) {    // f(score, place): beam in the upper half of the place, token in the lower
     if (isnan(base[k])) {                                     // equal ones: the lowest tokens stand for all
       const int v = i - k * per_beam;
       if (v < width && v < vocab) f(-(double)INFINITY, ((long long)k << 32) | v);
@@ -391,18 +433,46 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
     }
   };
   auto each = [&](auto f) {
+    if constexpr (!MANY) {
 #pragma unroll
-    for (int u = 0; u < kKept; ++u)
-      if (place + u * kThreads < n) one(place + u * kThreads, kept_v[u], kept_t[u], f);
-    for (int i = place + kKept * kThreads; i < n; i += kThreads) one(i, values[first + i], tokens[first + i], f);
+      for (int u = 0; u < kKept; ++u)
+        if (place + u * kThreads < n) one(place + u * kThreads, kept_k[u], kept_v[u], kept_t[u], f);
+    } else {
+      for (int i = place; i < n; i += kThreads) one(i, i / per_beam, values[first + i], tokens[first + i], f);
+    }
+  };
+  // f(score, place) for the candidates of this thread's lists, of each until that says no
+  auto lists = [&](auto f) {
+    const int step = 1 << split, n_lists = (beams * chunks) << split;
+#pragma unroll 4
+    for (int l = place; l < n_lists; l += kThreads) {
+      const int at = (l >> split) * width, k = (l >> split) / chunks;
+      bool on = true;
+      for (int e = l & (step - 1); e < width && on; e += step)
+        one(at + e, k, values[first + at + e], tokens[first + at + e], [&](double x, long long i) { on = f(x, i); });
+    }
   };
   double mine = -INFINITY;
-  each([&](double x, long long) { mine = x > mine ? x : mine; });
+  if constexpr (MANY) {
+    lists([&](double x, long long) {
+      mine = x > mine ? x : mine;
+      return false;
+    });
+  } else {
+    each([&](double x, long long) { mine = x > mine ? x : mine; });
+  }
   auto reach = [&](double bound, bool above, auto f) {
     bool more = true;
-    each([&](double x, long long i) {
-      if (more && (above ? x > bound : x >= bound)) more = f(x, i);
-    });
+    auto take = [&](double x, long long i) {
+      const bool in = above ? x > bound : x >= bound;
+      if (more && in) more = f(x, i);
+      return more && in;
+    };
+    if constexpr (MANY) {
+      if (above ? mine > bound : mine >= bound) lists(take);
+    } else {
+      each(take);
+    }
   };
   auto equal = [](double, int, auto) { return false; };        // (places are not in order of their index)
   largest(sh, width, kThreads / 32, mine, reach, each, equal, [&](int at, double v, long long i) {
@@ -456,8 +526,15 @@ int select(const Select& p, cudaStream_t s) {
     default: return SA_ERR_BAD_ARGUMENT;
   }
   if (st != SA_OK) return st;
-  return launch_after(choose_kernel, dim3(p.groups), kThreads, 0, s, p.scores, p.beams, p.vocab, p.width, r.chunks, (const float2*)sums,
-                      (const float*)values, (const int*)tokens, p.out_scores, p.out_rows, p.out_tokens);
+  auto choose = [&](auto kernel, int split) {
+    return launch_after(kernel, dim3(p.groups), kThreads, 0, s, p.scores, p.beams, p.vocab, p.width, r.chunks, split, (const float2*)sums,
+                        (const float*)values, (const int*)tokens, p.out_scores, p.out_rows, p.out_tokens);
+  };
+  const int lists = p.beams * r.chunks;
+  if (lists * p.width <= kKept * kThreads) return choose(choose_kernel<false>, 0);
+  int split = 0;                                             // a list or more a thread, where that makes enough of them
+  while ((lists << (split + 1)) <= kThreads && (2 << split) <= p.width) ++split;
+  return choose(choose_kernel<true>, split);
 }
 
 }  // namespace beam

@@ -66,6 +66,23 @@ def test_first_step_and_values_that_are_not_finite():
         _check(logits.cuda(), scores.cuda(), width)
 
 
+@pytest.mark.parametrize("groups,n,vocab,width", [(1, 32, 50304, 32), (3, 16, 20011, 32), (2, 256, 9000, 32), (1, 256, 6000, 5), (2, 33, 300, 32),
+                                                  (1, 5, 200000, 32)])
+def test_many_candidates(groups, n, vocab, width):
+    """Where a group has more candidates than its threads keep at hand: ordinary beams; then with masked, poor and equal ones among them."""
+    gen = torch.Generator().manual_seed(n + width)
+    logits = (torch.randn(groups, n, vocab, generator=gen) * 3).bfloat16()
+    scores = -5 * torch.rand(groups, n, generator=gen)
+    _check(logits.cuda(), scores.cuda(), width)
+    scores[:, 1::3] = -float("inf")
+    logits[:, 0, 7:], logits[:, 2::4] = -float("inf"), logits[:, :1, :1]
+    logits[:, 3, vocab // 2], logits[:, 4, 1] = float("nan"), float("inf")
+    _check(logits.cuda(), scores.cuda(), width)
+    scores[:, 1:] = -float("inf")                                 # a search's first step
+    _check(logits.cuda(), scores.cuda(), width)
+    _check(torch.zeros_like(logits).cuda(), torch.zeros_like(scores).cuda(), width)
+
+
 def test_arguments_that_are_refused():
     x, s = torch.zeros(2, 3, 10, device="cuda"), torch.zeros(2, 3, device="cuda")
     for bad in ((x, s, 0), (x, s, 31), (x, s, 33), (x.long(), s, 2), (x, s.cpu(), 2), (x[:, :0], s[:, :0], 1), (x, s[:, :2], 2)):
