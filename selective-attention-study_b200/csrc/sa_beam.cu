@@ -373,11 +373,10 @@ constexpr int kKept = 4;               // candidates of a thread of choose_kerne
 
 // MANY: more candidates than the threads keep at hand.  They are lists in order, WIDTH of each run, so the first of a list is its
 // largest, and a list is read until it falls below the bound.  A run's list counts as 2^split of them, of every 2^split-th entry.
-// (32 beams of 50,304, 13,312 candidates to a group, choose_kernel alone: 68 us with every candidate looked at, CHOOSE_MANY so.)
+// (32 beams of 50,304, 13,312 candidates to a group, choose_kernel alone: 68 us with every candidate looked at, 14 us so.)
 template <bool MANY>
 __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restrict__ scores, int beams, int vocab, int width, int chunks, int split,
-                                                          const float2* __restrict__ sums, const float* __restrict__ values,
-                                                          const int* __restrict__ tokens, float* __restrict__ out_scores,
+                                                          const float2* sums, const float* values, const int* tokens, float* __restrict__ out_scores,
                                                           int* __restrict__ out_rows, long long* __restrict__ out_tokens) {
   __shared__ Shared<double, long long> sh;
   __shared__ double base[kMaxBeams];                         // score - log-sum-exp of a beam; NaN: all of its scores are -inf
@@ -393,8 +392,13 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
 #pragma unroll
     for (int u = 0; u < kKept; ++u) kept_k[u] = (place + u * kThreads) / per_beam;
   }
-  if (tid < beams) base[tid] = (double)scores[(int64_t)g * beams + tid];      // (there before the logits are)
+  int lanes = 32;                                            // of a beam
+  while (lanes > 1 && lanes / 2 >= chunks && kThreads / lanes < beams) lanes /= 2;
+  const int c0 = tid & (lanes - 1), k_first = tid / lanes;
+  float score = k_first < beams ? scores[(int64_t)g * beams + k_first] : 0.f;      // (there before the logits are)
   tc::after_previous_kernel();
+  const float2* all = sums + (int64_t)g * beams * chunks;
+  float2 own = k_first < beams && c0 < chunks ? all[k_first * chunks + c0] : make_float2(-INFINITY, 0.f);
   if constexpr (!MANY) {
 #pragma unroll
     for (int u = 0; u < kKept; ++u) {
@@ -403,23 +407,22 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
       kept_t[u] = i < n ? tokens[first + i] : -1;
     }
   }
-  __syncthreads();                                           // the scores
-  int lanes = 32;                                            // of a beam
-  while (lanes > 1 && lanes / 2 >= chunks && kThreads / lanes < beams) lanes /= 2;
   for (int k0 = 0; k0 < beams; k0 += kThreads / lanes) {
-    const int k = k0 + tid / lanes;
-    const float2* part = sums + ((int64_t)g * beams + min(k, beams - 1)) * chunks;
-    float top = -INFINITY;
-    for (int c = tid & (lanes - 1); c < chunks; c += lanes) top = fmaxf(top, part[c].x);
-    for (int s = lanes / 2; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    double sum = 0.0;
-    for (int c = tid & (lanes - 1); c < chunks; c += lanes) {
-      const float2 p = part[c];
-      if (p.y != 0.f) sum += (double)p.y * exp2f((p.x - top) * kLog2e);         // 0: nothing but -inf; a NaN stays
+    const int k = k0 + k_first;
+    const float2* part = all + (int64_t)min(k, beams - 1) * chunks;
+    if (k0 > 0) {
+      score = scores[(int64_t)g * beams + min(k, beams - 1)];
+      own = c0 < chunks ? part[c0] : make_float2(-INFINITY, 0.f);
     }
+    float top = own.x;
+    for (int c = c0 + lanes; c < chunks; c += lanes) top = fmaxf(top, part[c].x);
+    for (int s = lanes / 2; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    auto term = [&](const float2& p) { return p.y != 0.f ? (double)p.y * exp2f((p.x - top) * kLog2e) : 0.0; };   // 0: nothing but -inf; a NaN stays
+    double sum = term(own);
+    for (int c = c0 + lanes; c < chunks; c += lanes) sum += term(part[c]);
     for (int s = lanes / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    if ((tid & (lanes - 1)) == 0 && k < beams) {
-      const double b = base[k] - ((double)top + log(sum));
+    if (c0 == 0 && k < beams) {
+      const double b = (double)score - ((double)top + log(sum));
       base[k] = isfinite(b) ? b : nan("");
     }
   }

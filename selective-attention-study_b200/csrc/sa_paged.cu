@@ -481,7 +481,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
 // keys: half of the copy rate.  (A row of a warp in flight at a time, in two launches, took 28 us.)
 constexpr int kPagePieces = 4;
 template <int UNITS>
-__global__ void __launch_bounds__(256) move_kernel(const int4* __restrict__ moved, const int2* __restrict__ copies, float* selected, int groups,
+__global__ void __launch_bounds__(256) move_kernel(const int4* moved, const int2* copies, float* selected, int groups,
                                                    int64_t capacity, int chunks, int history_ctas, uint4* k_pages, uint4* v_pages, int heads,
                                                    int num_pages, int64_t head_units, int row_units) {
   tc::after_previous_kernel();

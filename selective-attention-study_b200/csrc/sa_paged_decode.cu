@@ -55,12 +55,12 @@ __device__ __forceinline__ uint32_t split(float p) {
 
 template <int D>
 __global__ void __launch_bounds__(kAllThreads) decode_pages_kernel(
-    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* __restrict__ q,
-    Strides q_str, const __nv_bfloat16* __restrict__ k_new, Strides k_str, const __nv_bfloat16* __restrict__ v_new, Strides v_str,
-    __nv_bfloat16* k_pages, __nv_bfloat16* v_pages, float* selected, int64_t sel_stride, const int* __restrict__ tables, int max_pages,
-    int num_pages, int page_shift, int box_rows, const int* __restrict__ header, const DecodeItem* __restrict__ items, int items_max,
-    float* __restrict__ partial, float* __restrict__ sel_new, int64_t new_stride, unsigned int* tickets, int heads, int groups, int exempt,
-    float scale, const int64_t* __restrict__ slots, int total, __nv_bfloat16* __restrict__ y, tc::WaitCtx status, bool beside) {
+    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* q,
+    Strides q_str, const __nv_bfloat16* k_new, Strides k_str, const __nv_bfloat16* v_new, Strides v_str,
+    __nv_bfloat16* k_pages, __nv_bfloat16* v_pages, float* selected, int64_t sel_stride, const int* tables, int max_pages,
+    int num_pages, int page_shift, int box_rows, const int* header, const DecodeItem* items, int items_max,
+    float* partial, float* sel_new, int64_t new_stride, unsigned int* tickets, int heads, int groups, int exempt,
+    float scale, const int64_t* slots, int total, __nv_bfloat16* y, tc::WaitCtx status, bool beside) {
   constexpr int DK = D / 64, KB = D / 16;
   constexpr int kStageBytes = 2 * DK * kTileBytes;                // K, then V
   if (!beside) {

@@ -32,7 +32,7 @@ struct TokenRows {
 };
 // A unit is 16 bytes of one token's K or V; heads * units of a token are neighbours.
 __global__ void __launch_bounds__(256) store_kernel(TokenRows k, TokenRows v, uint4* k_pages, uint4* v_pages, uint4* y,
-                                                    const int64_t* __restrict__ slots, int total, int heads, int row_units, int num_pages,
+                                                    const int64_t* slots, int total, int heads, int row_units, int num_pages,
                                                     int page_shift, unsigned int* tickets, int n_tickets, unsigned int* more_tickets,
                                                     int n_more) {
   after_previous_kernel();
@@ -58,8 +58,8 @@ __global__ void __launch_bounds__(256) store_kernel(TokenRows k, TokenRows v, ui
 // and issue as that one: 17 query tiles x 251 key tiles of head_dim 64 25 us, 16 heads each for itself 17 x 63 64 us.
 template <int D>
 __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                           float* __restrict__ carry, int exempt, float scale, WaitCtx status, int chunk,
-                                                           const TileItem* __restrict__ tiles, const __grid_constant__ PagedWalk paged) {
+                                                           float* carry, int exempt, float scale, WaitCtx status, int chunk,
+                                                           const TileItem* tiles, const __grid_constant__ PagedWalk paged) {
   constexpr int DK = D / 64;
   after_previous_kernel();
   if ((int)blockIdx.x >= paged.header[paged::kTiles]) return;
@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
 
 // One thread per key and group of a row that has tiles (8 us for 17 tiles of 32,000 keys): carry[tile][group][j] = what the key has received before the tile, in
 // place, and `selected` moved on.  A new key has received nothing before the step, whatever an earlier row left there.
-__global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t key_stride, const int* __restrict__ tile_start,
-                                                         const TileItem* __restrict__ tiles, int groups, float* selected,
+__global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t key_stride, const int* tile_start,
+                                                         const TileItem* tiles, int groups, float* selected,
                                                          int64_t sel_stride) {
   after_previous_kernel();
   const int r = blockIdx.z, g = blockIdx.y;

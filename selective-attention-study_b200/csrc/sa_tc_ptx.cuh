@@ -149,7 +149,8 @@ __device__ __forceinline__ float load_ahead(const float* p) {
 }
 
 // First in a kernel that is launched while the one before it still runs (programmatic stream serialization): the next one may be
-// launched, and everything that the kernels before have written is there.
+// launched, and everything that the kernels before have written is there.  What they write (or read, where this one writes it) comes
+// through pointers without __restrict__: a load through one that is const __restrict__ may be moved to before the wait.
 __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
