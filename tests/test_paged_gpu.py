@@ -86,6 +86,19 @@ def test_rows_become_copies_as_in_the_oracle(rows, page, num_pages):
         assert all((row[len(held):] == [-1] * (8 - len(held))) for row, held in zip(t["block_tables"].tolist(), want.blocks))
 
 
+@pytest.mark.parametrize("rows,max_pages", [(1, 33), (3, 64), (5, 1000), (100, 70), (129, 65)])
+def test_copies_of_rows_of_many_pages(rows, max_pages):
+    rng = random.Random(rows)
+    t, want = _both(rows, rows * max_pages, 16, max_pages)
+    counts = [rng.randint(1, 16 * max_pages) for _ in range(rows - 1)] + [16 * max_pages - 1]
+    _append(t, want, counts, sum(counts))
+    for _ in range(3):
+        parents = [rng.randint(-1, rows - 1) for _ in range(rows - 1)] + [rows - 1]
+        moves = paged.reorder_rows(t, _ints(parents))
+        assert [tuple(x) for x in moves["copies"].tolist()] == want.reorder(parents)
+        _same_tables(t, want)
+
+
 def test_copies_in_a_full_pool():
     t, want = _both(6, 8, 16, 4)
     _append(t, want, [20, 20, 40, 0, 0, 0], 80)                    # 7 of 8 pages
