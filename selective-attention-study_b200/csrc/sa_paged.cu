@@ -100,16 +100,27 @@ __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const 
     t.block_tables[(int64_t)r * t.max_pages + block] = page;
     if (page >= 0 && page < t.num_pages) atomicAdd(t.page_refs + page, 1);
   }
-  for (int i = first; i < a.total; i += step) {
-    const int r = row_of(s.start, t.rows, i);
-    int64_t slot = -1;
-    if (i < s.start[t.rows] && s.before[r] >= 0) {
-      const int position = s.before[r] + i - s.start[r], block = position >> t.page_shift;
-      const int fresh = block - ((s.before[r] + page_mask) >> t.page_shift);    // of the row's new pages
-      const int page = fresh >= 0 ? t.free_pages[free_before - 1 - (s.page[r] + fresh)] : t.block_tables[(int64_t)r * t.max_pages + block];
-      slot = ((int64_t)page << t.page_shift) + (position & page_mask);
+  const int run = a.total > step ? 4 : 1;                          // of tokens: one search, and most often one page (512 rows: 22.5 -> 20.5 us)
+  for (int i0 = run * first; i0 < a.total; i0 += run * step) {
+    int r = row_of(s.start, t.rows, i0), block_was = -1, page = -1;
+    const int i1 = min(i0 + run, a.total);
+    for (int i = i0; i < i1; ++i) {
+      if (i >= s.start[r + 1]) {
+        r = row_of(s.start, t.rows, i);                            // (there may be many empty rows between)
+        block_was = -1;
+      }
+      int64_t slot = -1;
+      if (i < s.start[t.rows] && s.before[r] >= 0) {
+        const int position = s.before[r] + i - s.start[r], block = position >> t.page_shift;
+        if (block != block_was) {
+          const int fresh = block - ((s.before[r] + page_mask) >> t.page_shift);  // of the row's new pages
+          page = fresh >= 0 ? t.free_pages[free_before - 1 - (s.page[r] + fresh)] : t.block_tables[(int64_t)r * t.max_pages + block];
+          block_was = block;
+        }
+        slot = ((int64_t)page << t.page_shift) + (position & page_mask);
+      }
+      a.slots[i] = slot;
     }
-    a.slots[i] = slot;
   }
   // tiles (a row's first tile first), and walks over their keys, the longest of all rows first: a CTA each, taken in this order
   // (a warp a tile: its place is the number of longer walks, and of equal ones of earlier rows)
@@ -304,9 +315,10 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
 
 __global__ void __launch_bounds__(256) spread_kernel(const __grid_constant__ Append a) {
   tc::after_previous_kernel();
-  extern __shared__ int rows_s[];
+  extern __shared__ __align__(16) int rows_s[];
   __shared__ int header[kHeaderWords];
-  for (int i = threadIdx.x; i < 5 * (a.t.rows + 1) - 1; i += blockDim.x) rows_s[i] = __ldcg(a.work + a.layout.sums + i);
+  const int4* sums = reinterpret_cast<const int4*>(a.work + a.layout.sums);      // (in eights of words, as the layout leaves them)
+  for (int i = threadIdx.x; i < (5 * (a.t.rows + 1) + 3) / 4; i += blockDim.x) reinterpret_cast<int4*>(rows_s)[i] = __ldcg(sums + i);
   if (threadIdx.x < kHeaderWords) header[threadIdx.x] = __ldcg(a.work + threadIdx.x);
   __syncthreads();
   spread(a, RowSums(rows_s, a.t.rows), header, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
@@ -572,7 +584,7 @@ int append(const Tables& t, const int* counts, int total, int max_length, int ma
                                                : by_width(std::integral_constant<int, kMaxRows / 1024>{}, 1024);
   if (st != SA_OK || a.inside) return st;
   const unsigned blocks = (unsigned)min((total + 255) / 256, 2 * kSms);
-  return launch_after(spread_kernel, dim3(blocks), 256, smem, s, a);
+  return launch_after(spread_kernel, dim3(blocks), 256, smem + 16, s, a);
 }
 
 size_t reorder_work_words(int rows, int max_pages, int num_pages) { return ReorderWork(rows, max_pages, num_pages).words; }
