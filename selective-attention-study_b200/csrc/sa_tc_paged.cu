@@ -52,14 +52,50 @@ __global__ void __launch_bounds__(256) store_kernel(TokenRows k, TokenRows v, ui
   }
 }
 
+// ---- what the keys have received before each tile ------------------------------------------------------------------------------
+// col[t pitch] = what key j has received before tile t of its row, in place of what it receives from it, for tiles [t, n); returns
+// the sum after the last.  The loads go past the L1 cache: other CTAs of the same launch may have written them.
+__device__ __forceinline__ float scan_key(float* col, int64_t pitch, int t, int n, float run) {
+  for (; t + 8 <= n; t += 8) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = __ldcg(col + (t + u) * pitch);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      col[(t + u) * pitch] = run;
+      run += x[u];
+    }
+  }
+  for (; t < n; ++t) {
+    const float x = __ldcg(col + t * pitch);
+    col[t * pitch] = run;
+    run += x;
+  }
+  return run;
+}
+// The scan of the keys of one row and group (`first`: its first tile): `selected` moved on.  A new key has received nothing before
+// the step, whatever an earlier row left there.
+struct History {
+  float* selected;
+  int64_t stride;                    // keys of a row
+  unsigned int* tickets;             // colsum_pages_kernel scans: one a row (at its first tile), group and key tile; else null
+};
+__device__ __forceinline__ void scan_row_key(float* carry, int64_t key_stride, int groups, int t0, int n, int g, int j, const TileItem& w,
+                                             const History& history) {
+  float* sel = history.selected + ((int64_t)w.row * groups + g) * history.stride + j;
+  const float run = j < w.cached ? *sel : 0.f;
+  *sel = scan_key(carry + ((int64_t)t0 * groups + g) * key_stride + j, groups * key_stride, max(j / kTile - w.cached / kTile, 0), n, run);
+}
+
 // ---- selection column sums --------------------------------------------------------------------------------------------------
 // As colsum_kernel (sa_tc_fwd.cu), with the loops the other way round: a CTA keeps one query tile and takes a run of `chunk` key
 // tiles, since rows have few query tiles.  128 threads own a key each, a fifth warp loads and issues, one tile ahead.  Bound by latency
 // and issue as that one: 17 query tiles x 251 key tiles of head_dim 64 25 us, 16 heads each for itself 17 x 63 64 us.
+// With a key tile a CTA, the last of a row's CTAs to finish it also scans it (scan_pages_kernel's work): a launch fewer.
 template <int D>
 __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                            float* carry, int exempt, float scale, WaitCtx status, int chunk,
-                                                           const TileItem* tiles, const __grid_constant__ PagedWalk paged) {
+                                                           const TileItem* tiles, const __grid_constant__ PagedWalk paged, History history) {
   constexpr int DK = D / 64;
   after_previous_kernel();
   if ((int)blockIdx.x >= paged.header[paged::kTiles]) return;
@@ -190,46 +226,36 @@ __global__ void __launch_bounds__(160) colsum_pages_kernel(const __grid_constant
     }
   }
   tc_fence_before_sync();
+  if (history.tickets != nullptr) __threadfence();                         // the sums, before the ticket
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 256);
+  if (history.tickets == nullptr) return;
+  __shared__ bool last_s;
+  const int first = w.cached / kTile, n = (w.length - 1) / kTile + 1 - first, t0 = w.tile - (w.mi - first);      // the row's tiles
+  if (tid == 0) {
+    const unsigned all = n - max(nj0 - first, 0);                          // of its tiles reach these keys
+    last_s = atomicAdd(history.tickets + ((int64_t)t0 * gridDim.z + h) * gridDim.y + blockIdx.y, 1u) == all - 1u;
+  }
+  __syncthreads();
+  if (!last_s || tid >= kTile) return;
+  __threadfence();
+  const int j = nj0 * kTile + tid;
+  if (j < w.length) scan_row_key(carry, paged.key_stride, gridDim.z, t0, n, h, j, w, history);
 }
 
-// One thread per key and group of a row that has tiles (8 us for 17 tiles of 32,000 keys): carry[tile][group][j] = what the key has received before the tile, in
-// place, and `selected` moved on.  A new key has received nothing before the step, whatever an earlier row left there.
-__global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t key_stride, const int* tile_start,
-                                                         const TileItem* tiles, int groups, float* selected,
-                                                         int64_t sel_stride) {
+// One thread per key and group of a row that has tiles (8 us for 17 tiles of 32,000 keys).
+__global__ void __launch_bounds__(256) scan_pages_kernel(float* carry, int64_t key_stride, const int* tile_start, const TileItem* tiles,
+                                                         int groups, History history) {
   after_previous_kernel();
   const int r = blockIdx.z, g = blockIdx.y;
   const int t0 = tile_start[r], n = tile_start[r + 1] - t0;
   if (n == 0) return;
   const TileItem w = tiles[t0];                                 // the row's first tile
   const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= w.length) return;
-  const int64_t pitch = groups * key_stride;
-  float* col = carry + ((int64_t)t0 * groups + g) * key_stride + j;
-  float* sel = selected + ((int64_t)r * groups + g) * sel_stride + j;
-  float run = j < w.cached ? *sel : 0.f;
-  int t = max(j / kTile - w.mi, 0);
-  for (; t + 8 <= n; t += 8) {
-    float x[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) x[u] = col[(t + u) * pitch];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      col[(t + u) * pitch] = run;
-      run += x[u];
-    }
-  }
-  for (; t < n; ++t) {
-    const float x = col[t * pitch];
-    col[t * pitch] = run;
-    run += x;
-  }
-  *sel = run;
+  if (j < w.length) scan_row_key(carry, key_stride, groups, t0, n, g, j, w, history);
 }
 
-// The histories of the rows that have tiles as they were before scan_pages_kernel: what their first tile starts from.
+// The histories of the rows that have tiles as they were before the scan: what their first tile starts from.
 __global__ void __launch_bounds__(256) restore_kernel(const float* __restrict__ carry, int64_t key_stride, const int* __restrict__ tile_start,
                                                       const TileItem* __restrict__ tiles, int groups, float* selected, int64_t sel_stride) {
   const int r = blockIdx.z, g = blockIdx.y, t0 = tile_start[r];
@@ -257,15 +283,23 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   if (st != SA_OK) return st;
 
   unsigned int* const walk_tickets = reinterpret_cast<unsigned int*>(a.workspace + w.tickets);
-  // store: also clears the tickets of this call, the walks' and (where they are not the plan's) the single tokens'
-  const int n_walk = l.tiles_max * a.heads;
+  // key tiles per CTA of the selection (the query tile and the set-up are paid per CTA): 32 where that still gives every SM several
+  // CTAs, else 8, or 4 where that would be fewer than two an SM (in 2, 4, 8: 1,024 tokens after 8,000 12, 12, 14 us, 2,048 after 30,000
+  // 31, 27, 26).  One where all of them are few, and then the scan too.  Calls in 4 with a scan of its own, in one with it, in one
+  // without: a prompt of 300 21.5, 20.9, 20.1 us, of 1,000 32.7, 31.2, 30.5, of 2,000 58.8, 58.3, 56.5; 1,024 after 8,000 127.5 in 4, 130 so.
+  const int key_tiles = (a.max_length + kTile - 1) / kTile;
+  const int64_t products = (int64_t)l.tiles_max * key_tiles * a.groups;
+  const int chunk = products >= 32 * 16 * kSms ? 32 : products >= 8 * 2 * kSms ? 8 : products >= 4 * kSms ? 4 : 1;
+  const bool scans = chunk == 1;
+  // store: also clears the tickets of this call, the walks', the scans' and (where they are not the plan's) the single tokens'
+  const int n_walk = l.tiles_max * a.heads, n_scan = scans ? l.tiles_max * a.groups * key_tiles : 0;
   {
     const TokenRows k{static_cast<const uint4*>(a.k), a.k_stride[0] / 8, a.k_stride[1] / 8};
     const TokenRows v{static_cast<const uint4*>(a.v), a.v_stride[0] / 8, a.v_stride[1] / 8};
     const int64_t units = (int64_t)a.total * a.heads * (D / 8);
     const unsigned blocks = (unsigned)max((int64_t)1, min((units + 255) / 256, (int64_t)8 * kSms));
     st = launch_after(store_kernel, dim3(blocks), 256, 0, s, k, v, static_cast<uint4*>(a.k_pages), static_cast<uint4*>(a.v_pages),
-                static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk,
+                static_cast<uint4*>(a.y), a.slots, a.total, a.heads, D / 8, a.num_pages, a.page_shift, walk_tickets, n_walk + n_scan,
                 reinterpret_cast<unsigned int*>(a.workspace + w.own_tickets), a.plan_tickets ? 0 : l.tickets_count);
     if (st != SA_OK) return st;
   }
@@ -281,21 +315,18 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   const TileItem* tiles = reinterpret_cast<const TileItem*>(a.work + l.tiles);
   float* carry = a.workspace + w.carry;
   const float scale = 1.0f / sqrtf((float)D);
-  const int key_tiles = (a.max_length + kTile - 1) / kTile;
+  const History history{a.selected, a.sel_stride, scans ? walk_tickets + n_walk : nullptr};
   {
-    // key tiles per CTA (the query tile and the set-up are paid per CTA): 32 where that still gives every SM several CTAs, else 8,
-    // or 4 where that would be fewer than two an SM (in 2, 4, 8: 1,024 tokens after 8,000 12, 12, 14 us, 2,048 after 30,000 31, 27, 26)
-    const int64_t products = (int64_t)l.tiles_max * key_tiles * a.groups;
-    const int chunk = products >= 32 * 16 * kSms ? 32 : products >= 8 * 2 * kSms ? 8 : 4;
     ProfileScope prof(SA_KERNEL_TC_COLSUM, s);
-    st = launch_after(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, s,
-                map_q, map_k, carry, a.exempt, scale, status, chunk, tiles, walk);
+    st = launch_after(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, s, map_q, map_k, carry, a.exempt,
+                      scale, status, chunk, tiles, walk, history);
     if (st != SA_OK) return st;
+    *moved = scans;
   }
-  {
+  if (!scans) {
     ProfileScope prof(SA_KERNEL_TC_SCAN, s);
     st = launch_after(scan_pages_kernel, dim3((a.max_length + 255) / 256, a.groups, a.rows), 256, 0, s, carry, w.key_stride,
-                (const int*)(a.work + l.tile_start), tiles, a.groups, a.selected, a.sel_stride);
+                      (const int*)(a.work + l.tile_start), tiles, a.groups, history);
     if (st != SA_OK) return st;
     *moved = true;
   }
@@ -346,7 +377,7 @@ AttentionScratch attention_scratch(const Attention& a) {
     const size_t cut = (size_t)tile_wave(a.heads) * a.heads * kTile;        // the plan cuts no more than a wave of walks
     w.part = take(cut * a.head_dim);
     w.lse = take(cut);
-    w.tickets = take((size_t)l.tiles_max * a.heads);
+    w.tickets = take((size_t)l.tiles_max * a.heads + (size_t)l.tiles_max * a.groups * (w.key_stride / kTile));      // the walks', the scans'
   }
   return w;
 }

@@ -571,7 +571,8 @@ for counts in ([200, 1, 1], [1, 1, 1], [3000, 1, 1]):
     y = paged.paged_attention(want, t, step, *x)
     got, launches = tried(lambda: paged.paged_attention(cache, t, step, *x), same_history)
     assert torch.equal(got, y) and torch.equal(cache["selected"], want["selected"]), counts
-    assert launches == (1 if most == 1 else 5), launches
+    few = most == 200 and sys.argv[2] == "shared"              # selection of few tiles scans them, too
+    assert launches == (1 if most == 1 else 4 if few else 5), launches
 print("all tried")
 """
 
