@@ -7,8 +7,10 @@
 // sum of exponentials and its WIDTH largest logits.  choose_kernel (a CTA a group) makes the
 // beams' log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
-// 256 beams of 50,304 bf16 logits (25.7 MB): 15 + 7 us, the first at 27 % of the copy rate: bound by issue (about 60 instructions for
-// 8 logits, two thirds of them for the exponentials) and by the start and end of its one wave; 4 beams 6 + 6 us, latency.
+// 256 beams of 50,304 bf16 logits (25.7 MB): 13 + 6 us.  Where the first goes, in cycles of a CTA that ends last: 1,500 until its loads
+// are issued, 12,000 until its first part is there (behind the three other CTAs of its SM), 19,000 until it has looked at the run,
+// 24,000 with the ranking.  From L2 the first part takes 4,600 and the rest as long, so the exponentials (8 cycles of a warp each) and
+// the loads share the blame.  4 beams: 6 + 6 us, latency.
 //
 // The largest of a set, without sorting it: each warp that has elements gives the largest of its lanes' own maxima, about two times
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among
@@ -178,8 +180,9 @@ template <> struct Word<__half> {
 
 // Elements are taken in units of 16 bytes from a 16-byte boundary on: a row that begins elsewhere has `lead` elements fewer in
 // its first unit.  A unit that sticks out of the row is put together element by element; the others come by bulk copies in
-// kParts parts, so that the first is worked on while the last is on its way.
-constexpr int kParts = 4;
+// kParts parts, so that the first is worked on while the last is on its way (in 1, 2, 3, 4, 12: 14.0, 13.4, 12.7, 13.6, 16.3 us for 256
+// beams of 50,304: every wait costs some 250 cycles).
+constexpr int kParts = 3;
 constexpr int kMostUnits = 3328;     // of a CTA: 52 KB, four CTAs an SM
 
 template <typename T>
