@@ -143,11 +143,12 @@ __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const 
   for (int i = first; i < n_single; i += step) {
     const int r = row_of(s.piece, t.rows, i);
     DecodeItem x;
-    x.row = r; x.token = s.start[r];
+    const int count = s.start[r + 1] - s.start[r];
+    x.row = (short)r; x.count = (short)count; x.token = s.start[r];
     x.first = s.piece[r];
     x.piece = i - x.first;
     x.pieces = s.piece[r + 1] - x.first;
-    x.length = s.before[r] + 1;
+    x.length = s.before[r] + count;
     x.c0 = x.piece * piece_keys;
     x.c1 = min(x.c0 + piece_keys, x.length);
     reinterpret_cast<DecodeItem*>(a.work + a.layout.decode_items)[i] = x;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
     }
   }
   block_scan(pages, pages_total, warp_sums);
-  S next[4] = {0, 0, 0, 0}, next_total[4];       // tiles, single tokens, their keys, pages taken
+  S next[4] = {0, 0, 0, 0}, next_total[4];       // tiles, rows of few tokens, their keys, pages taken
   {
     S upto = pages[0];
 #pragma unroll
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       else next[3] += need[u];
       if (count[u] > 0 && count[u] < a.least_tokens) {
         next[1] += 1;
-        next[2] += before[u] + 1;
+        next[2] += before[u] + count[u];
       } else if (count[u] > 0) {
         next[0] += (before[u] + count[u] - 1) / kTile - before[u] / kTile + 1;
       }
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
   }
   block_scan(next, next_total, warp_sums);
   const int n_tiles = (int)next_total[0], singles = (int)next_total[1];
-  // pieces of single tokens: about one wave of CTAs over all heads, or several where rows alone are more than that
+  // pieces of rows of few tokens: about one wave of CTAs over all heads, or several where rows alone are more than that
   int piece_keys = kTile;
   if (singles > 0) {
     const int spread_over = 2 * singles <= a.wave_decode ? a.wave_decode - singles : kDecodeWaves * a.wave_decode;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
   if (singles > 0) {
 #pragma unroll
     for (int u = 0; u < PER; ++u)
-      if (count[u] > 0 && count[u] < a.least_tokens) pieces[0] += before[u] / piece_keys + 1;
+      if (count[u] > 0 && count[u] < a.least_tokens) pieces[0] += (before[u] + count[u] - 1) / piece_keys + 1;
     block_scan(pieces, pieces_total, warp_sums);
   }
   // Few tiles: their walks are cut so that all heads together are one wave of CTAs.
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
         a.query_start[r] = sums.start[r];
       }
       if (count[u] >= a.least_tokens) tile_at += (before[u] + count[u] - 1) / kTile - before[u] / kTile + 1;
-      else if (count[u] > 0) piece_at += before[u] / piece_keys + 1;
+      else if (count[u] > 0) piece_at += (before[u] + count[u] - 1) / piece_keys + 1;
     }
     if (tid == 0) {
       sums.start[t.rows] = a.query_start[t.rows] = (int)min(total[0], (S)a.total);

@@ -27,17 +27,20 @@ struct TileItem {
   int piece, pieces;
   int cached, length;      // tokens of the row before and after the step
 };
-// Keys [c0, c1) of a row that gets a single token.
+// Keys [c0, c1) of a row that gets one token, or a few.
 struct DecodeItem {
-  int row, token;
+  short row, count;           // rows are at most kMaxRows; new tokens
+  int token;
   int c0, c1;
   int piece, pieces, first;   // `first`: the row's first item
-  int length;                 // with the new token
+  int length;                 // with the new tokens
 };
 
-// Rows of this many new tokens go through the tile kernels, rows of fewer (one) through the single-token kernel.  A step of one
-// row that may get several takes the tile kernels whatever it gets: the other launch would find nothing, for 2 us.
-inline int tile_tokens(int rows, int total, int max_count) { return rows == 1 && min(total, max_count) > 1 ? 1 : 2; }
+// Rows of this many new tokens go through the tile kernels, rows of fewer through the kernel of few tokens.  A step of one row
+// that may get more takes the tile kernels whatever it gets: the other launch would find nothing, for 2 us.
+constexpr int kFewTokens = 8;
+inline bool few_only(int total, int max_count) { return min(total, max_count) <= kFewTokens; }
+inline int tile_tokens(int rows, int total, int max_count) { return rows == 1 && !few_only(total, max_count) ? 1 : kFewTokens + 1; }
 
 struct StepLayout {
   int tiles_max, tile_items_max, decode_items_max;
@@ -49,7 +52,7 @@ inline int tile_wave(int heads) { const int w = kSms / heads; return w > 1 ? w :
 constexpr int kDecodeWaves = 4;
 inline StepLayout step_layout(int rows, int total, int heads) {
   StepLayout l{};
-  const int64_t with_tiles = min(rows, total / 2);            // rows of two tokens or more; n of them touch (n + 254) / 128 tiles
+  const int64_t with_tiles = min(rows, total / (rows == 1 ? 1 : kFewTokens + 1));   // n tokens of one touch (n + 254) / 128 tiles
   l.tiles_max = (int)(((int64_t)total + 254 * with_tiles) / kTile);
   l.tile_items_max = l.tiles_max > 0 ? l.tiles_max + tile_wave(heads) : 0;
   const int singles = min(rows, total), wave = decode_wave(heads);      // as the plan spreads them (append_kernel)

@@ -129,9 +129,9 @@ int sa_paged_run(const sa_paged_attention* in) {
   }
   a.workspace = static_cast<float*>(in->workspace);
   cudaStream_t s = static_cast<cudaStream_t>(in->stream);
-  // Rows of two tokens or more go through the tile kernels, rows of one through the single-token kernel; the step's bounds say
-  // where there can be none of either.
-  if (a.max_count == 1) return paged::decode(a, false, s);
+  // Rows of few tokens go through a kernel of their own, the others through the tile kernels; the step's bounds say where there can
+  // be none of either.
+  if (paged::few_only(a.total, a.max_count)) return paged::decode(a, false, s);
   bool moved = false;
   st = paged::tiles(a, &moved, s);
   if (st == SA_OK && paged::tile_tokens(a.rows, a.total, a.max_count) > 1) st = paged::decode(a, true, s);

@@ -370,9 +370,9 @@ AttentionScratch attention_scratch(const Attention& a) {
     return at;
   };
   w.own_tickets = take((size_t)l.tickets_count);
-  w.partial = take((size_t)l.decode_items_max * a.heads * (a.head_dim + 2));
+  w.partial = take((size_t)l.decode_items_max * a.heads * min(a.max_count, paged::kFewTokens) * (a.head_dim + 2));
   w.sel_new = take(a.groups < a.heads ? (size_t)a.rows * a.groups * w.key_stride : 0);
-  if (a.max_count > 1 && l.tiles_max > 0) {
+  if (!few_only(a.total, a.max_count) && l.tiles_max > 0) {
     w.carry = take((size_t)l.tiles_max * a.groups * w.key_stride);
     const size_t cut = (size_t)tile_wave(a.heads) * a.heads * kTile;        // the plan cuts no more than a wave of walks
     w.part = take(cut * a.head_dim);
