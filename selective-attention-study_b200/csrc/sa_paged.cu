@@ -280,18 +280,24 @@ __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Ap
       mi_s[tid] = x.mi;
     }
     __syncthreads();
-    if (tid < 32) {                                               // the shortest pieces, of four key tiles at least, that are one wave
-      int low = 4, high = 4;
-      for (int u = tid; u < n_tiles; u += 32) high = max(high, mi_s[u] + 1);
-      high = __reduce_max_sync(0xffffffffu, high);
-      while (low < high) {
-        const int middle = (low + high) >> 1;
-        int n = 0;
-        for (int u = tid; u < n_tiles; u += 32) n += (mi_s[u] + middle) / middle;
-        if (__reduce_add_sync(0xffffffffu, n) <= a.wave_tiles) high = middle;
-        else low = middle + 1;
-      }
-      if (tid == 0) header[kTileItems] = low;
+    if (tid < 32) {
+      int longest = kPieceTiles;
+      for (int u = tid; u < n_tiles; u += 32) longest = max(longest, mi_s[u] + 1);
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      auto shortest = [&](int most) {                             // pieces, of so many items at most
+        int low = kPieceTiles, high = longest;
+        while (low < high) {
+          const int middle = (low + high) >> 1;
+          int n = 0;
+          for (int u = tid; u < n_tiles; u += 32) n += (mi_s[u] + middle) / middle;
+          if (__reduce_add_sync(0xffffffffu, n) <= most) high = middle;
+          else low = middle + 1;
+        }
+        return low;
+      };
+      // One wave of CTAs, or two where tiles of one length leave many SMs without a piece.  A CTA's set-up takes as long as three steps.
+      const int one = shortest(a.wave_tiles), two = shortest(kTileWaves * a.wave_tiles);
+      if (tid == 0) header[kTileItems] = two < one && 2 * (two + 4) < one + 3 ? two : one;
     }
     __syncthreads();
     const int piece_tiles = header[kTileItems];

@@ -50,11 +50,12 @@ struct StepLayout {
 inline int decode_wave(int heads) { const int w = kSms * kDecodeCtas / heads; return w > 1 ? w : 1; }
 inline int tile_wave(int heads) { const int w = kSms / heads; return w > 1 ? w : 1; }
 constexpr int kDecodeWaves = 4;
+constexpr int kTileWaves = 2, kPieceTiles = 4;                  // waves of pieces at most; key tiles of a piece at least
 inline StepLayout step_layout(int rows, int total, int heads) {
   StepLayout l{};
   const int64_t with_tiles = min(rows, total / (rows == 1 ? 1 : kFewTokens + 1));   // n tokens of one touch (n + 254) / 128 tiles
   l.tiles_max = (int)(((int64_t)total + 254 * with_tiles) / kTile);
-  l.tile_items_max = l.tiles_max > 0 ? l.tiles_max + tile_wave(heads) : 0;
+  l.tile_items_max = l.tiles_max > 0 ? l.tiles_max + kTileWaves * tile_wave(heads) : 0;
   const int singles = min(rows, total), wave = decode_wave(heads);      // as the plan spreads them (append_kernel)
   l.decode_items_max = 2 * singles <= wave ? wave : singles + kDecodeWaves * wave;
   size_t at = kHeaderWords;

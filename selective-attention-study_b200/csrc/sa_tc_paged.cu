@@ -332,21 +332,22 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   }
   // Two heads a CTA, or one: as over contiguous caches (sa_tc_fwd.cu), by the tiles that there are at least, since the plan's
   // number is on the device.  Where there may be few, the plan may have cut their walks.
+  // (A CTA without an item takes an SM for a microsecond.)
+  const int items_max = (int)min((int64_t)l.tile_items_max, (int64_t)l.tiles_max * ((key_tiles + paged::kPieceTiles - 1) / paged::kPieceTiles));
   const int tiles_min = (a.total - (a.rows - 1) + kTile - 1) / kTile;
   ProfileScope prof(SA_KERNEL_TC_FORWARD, s);
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
   const RowLayout y_rows{0, D, (int64_t)a.heads * D};
   if constexpr (D == 64) {
     if (!self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
-      return launch_after(forward_pair_kernel<false, true>, dim3((unsigned)l.tile_items_max * (a.heads / 2)), kThreads, PairSmem::total, s,
+      return launch_after(forward_pair_kernel<false, true>, dim3((unsigned)items_max * (a.heads / 2)), kThreads, PairSmem::total, s,
                     map_q, map_k, map_v, map_q, map_k, (const float*)carry, (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale,
                     status, y, y_rows, 0, (const uint8_t*)nullptr, walk);
   }
   if (D == 64 && self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
-    return forward_self_pages(walk, map_q, map_k, map_v, carry, l.tile_items_max, a.exempt, scale, status, y, y_rows, s);
-  const dim3 grid((unsigned)l.tile_items_max * a.heads);
+    return forward_self_pages(walk, map_q, map_k, map_v, carry, items_max, a.exempt, scale, status, y, y_rows, s);
   auto wide = [&](auto kernel) {
-    return launch_after(kernel, grid, kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
+    return launch_after(kernel, dim3((unsigned)items_max * a.heads), kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
                   (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
                   SplitWalk{}, walk);
   };
@@ -374,7 +375,7 @@ AttentionScratch attention_scratch(const Attention& a) {
   w.sel_new = take(a.groups < a.heads ? (size_t)a.rows * a.groups * w.key_stride : 0);
   if (!few_only(a.total, a.max_count) && l.tiles_max > 0) {
     w.carry = take((size_t)l.tiles_max * a.groups * w.key_stride);
-    const size_t cut = (size_t)tile_wave(a.heads) * a.heads * kTile;        // the plan cuts no more than a wave of walks
+    const size_t cut = (size_t)kTileWaves * tile_wave(a.heads) * a.heads * kTile;      // the plan cuts walks into no more pieces than that
     w.part = take(cut * a.head_dim);
     w.lse = take(cut);
     w.tickets = take((size_t)l.tiles_max * a.heads + (size_t)l.tiles_max * a.groups * (w.key_stride / kTile));      // the walks', the scans'
