@@ -264,6 +264,20 @@ __global__ void __launch_bounds__(256) restore_kernel(const float* __restrict__ 
   selected[((int64_t)r * groups + g) * sel_stride + j] = carry[((int64_t)t0 * groups + g) * key_stride + j];
 }
 
+// Two heads a CTA (10 units of time a step) or one (7)?  Of one row the walks are known: `tiles` of them, up to `longest` key tiles, with
+// a set-up of three steps each.  Either kernel takes as long as its longest walk, or as all of them over the SMs; of one head a CTA the walks
+// that find no SM at first come after the shortest of the others.  Several rows: by the number of CTAs, as over contiguous caches.
+// Two heads and one, in us: 16 heads, a prompt of 1,300 46, 34, of 2,000 57, 48, of 3,000 81, 89, of 8,000 314, 400; 2,000 after 2,000 98,
+// 99, after 8,000 207, 239; 8 heads, a prompt of 4,000 97, 73, of 8,000 179, 214; 12 heads, 1,300 after 20,000 402, 283; 32 heads, a
+// prompt of 1,300 48, 54, 1,300 after 8,000 327, 328.
+bool two_heads(int rows, int tiles, int longest, int heads) {
+  if (rows > 1) return (int64_t)tiles * heads > kSms;
+  const double steps = tiles * (longest - 0.5 * (tiles - 1) + 3), top = longest + 3, waiting = top - (double)kSms / heads;
+  const double two = 10 * max(top, steps * heads / 2 / kSms);
+  const double one = 7 * max(max(top, steps * heads / kSms), tiles * heads > kSms ? 2 * waiting : 0.0);
+  return two < one;
+}
+
 template <int D>
 int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   constexpr int DK = D / 64;
@@ -330,8 +344,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
     if (st != SA_OK) return st;
     *moved = true;
   }
-  // Two heads a CTA, or one: as over contiguous caches (sa_tc_fwd.cu), by the tiles that there are at least, since the plan's
-  // number is on the device.  Where there may be few, the plan may have cut their walks.
+  // The plan's numbers are on the device: the host goes by the tiles that there are at least, and by the items that there can be.
   // (A CTA without an item takes an SM for a microsecond.)
   const int items_max = (int)min((int64_t)l.tile_items_max, (int64_t)l.tiles_max * ((key_tiles + paged::kPieceTiles - 1) / paged::kPieceTiles));
   const int tiles_min = (a.total - (a.rows - 1) + kTile - 1) / kTile;
@@ -339,12 +352,12 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
   const RowLayout y_rows{0, D, (int64_t)a.heads * D};
   if constexpr (D == 64) {
-    if (!self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
+    if (!self && a.heads % 2 == 0 && two_heads(a.rows, tiles_min, key_tiles, a.heads))
       return launch_after(forward_pair_kernel<false, true>, dim3((unsigned)items_max * (a.heads / 2)), kThreads, PairSmem::total, s,
                     map_q, map_k, map_v, map_q, map_k, (const float*)carry, (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale,
                     status, y, y_rows, 0, (const uint8_t*)nullptr, walk);
   }
-  if (D == 64 && self && a.heads % 2 == 0 && (int64_t)tiles_min * a.heads > kSms)
+  if (D == 64 && self && a.heads % 2 == 0 && two_heads(a.rows, tiles_min, key_tiles, a.heads))
     return forward_self_pages(walk, map_q, map_k, map_v, carry, items_max, a.exempt, scale, status, y, y_rows, s);
   auto wide = [&](auto kernel) {
     return launch_after(kernel, dim3((unsigned)items_max * a.heads), kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,

@@ -239,13 +239,23 @@ def test_few_tokens_after_many(heads, dim, per_head, rows, achieved):
 
 @pytest.mark.parametrize("heads,dim,per_head,first,chunk", [
     (2, 64, False, 5000, 40),                                     # few tiles after many keys: pieces of a walk
-    (16, 64, False, 300, 1500),                                   # many tiles: two heads a CTA
+    (16, 64, False, 300, 1500), (32, 64, False, 100, 1450), (32, 64, True, 100, 1300),      # many tiles: one head a CTA, and two
+    (16, 64, False, 2000, 500), (16, 64, True, 2300, 500),        # walks in pieces of which there are two waves
     (12, 64, False, 1, 1700), (5, 64, False, 777, 1601), (8, 128, False, 500, 1300), (16, 64, True, 129, 1200), (3, 128, True, 3000, 129)])
 def test_one_row_prompt_and_chunk(heads, dim, per_head, first, chunk, achieved):
     s = Served(1, heads, dim, 64, -(-(first + chunk + 3) // 64), 120, per_head, exempt=16, scale=0.3, seed=2)
     worst = max(s.step([first]), s.step([chunk]), s.step([1], total=3), s.step([1]))
     s.pools()
     achieved(f"paged prompt and chunk H={heads} D={dim} {first}+{chunk}", share_of_bound=worst)
+
+
+@pytest.mark.parametrize("per_head", [False, True])
+def test_chunks_of_many_tiles(per_head, achieved):
+    """Several rows whose tiles are more than the SMs: two heads a CTA."""
+    s = Served(3, 16, 64, 32, 60, 150, per_head, exempt=3, scale=0.4, seed=8)
+    worst = max(s.step([900, 33, 700]), s.step([700, 1, 810]), s.step([640, 500, 200]))
+    s.pools()
+    achieved(f"paged chunks of many tiles per_head={per_head}", share_of_bound=worst)
 
 
 def test_rows_that_are_not_served():
