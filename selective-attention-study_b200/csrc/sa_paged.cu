@@ -70,7 +70,7 @@ struct Append {
   int* work;
   StepLayout layout;
 };
-// Sums over the rows before a row (rows + 1 each): tokens, pages that they take, tiles, pieces of single tokens; and the tokens that
+// Sums over the rows before a row (rows + 1 each): tokens, pages that they take, tiles, pieces of rows of few tokens; and the tokens that
 // a row has (-1: it is left as it is).
 struct RowSums {
   int *start, *page, *tile, *piece, *before;
@@ -156,7 +156,7 @@ __device__ __forceinline__ void spread(const Append& a, const RowSums& s, const 
 }
 
 // One CTA: PER rows a thread and four prefix sums over the rows; what is per page, tile or token (spread) here too where that is
-// little, else in a second kernel of many CTAs (512 rows with 264,000 tokens and 16,800 pages: 6 + 13 us; in one CTA 48).  Bound by
+// little, else in a second kernel of many CTAs (512 rows with 264,000 tokens and 16,800 pages: 6 + 12 us; in one CTA 48).  Bound by
 // the chain of dependent loads, sums and barriers: 64 rows of one token 7 us.  S: 32 bits where no sum can pass them.
 template <int PER, typename S>
 __global__ void __launch_bounds__(1024) append_kernel(const __grid_constant__ Append a) {
@@ -340,8 +340,8 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // page of a new row (a page that old and new row have at the same place counts for neither); (2) a reference less for each page
 // of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first, and takes the
 // pages for the copies off its end, in row order, while (4) the others write the tables.  A row for which there is none becomes
-// empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes: 4 rows 10 us,
-// 256 rows of up to 47 pages 14 us.
+// empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes: 4 rows of 26
+// or of 500 pages 8 us, 256 rows of 24 10 us.
 constexpr int kCluster = 8, kReorderThreads = 1024;
 
 // The work of a reordering, int32 words: how many rows change, then (row, parent, tokens, tokens of the page being filled) of

@@ -8,7 +8,7 @@ namespace paged {
 
 constexpr int kMaxRows = 4096;       // requests of one set of tables (the table kernel keeps five numbers a row in shared memory)
 constexpr int kTile = 128;           // query rows and keys of a tile of the tensor-core kernels
-constexpr int kDecodeCtas = 4;       // CTAs of the single-token kernel that an SM holds
+constexpr int kDecodeCtas = 4;       // CTAs of the kernel of few tokens that an SM holds
 
 struct Tables {
   int rows, max_pages, num_pages, page_shift, heads;
@@ -91,7 +91,7 @@ struct Attention {
   void* y;                            // (total, heads, head_dim)
   float* workspace;
 };
-// Floats of scratch: the single-token kernel's partial sums and new selection; the tile kernels' checkpoints and pieces.
+// Floats of scratch: the partial sums of the kernel of few tokens and new selection; the tile kernels' checkpoints and pieces.
 struct AttentionScratch {
   size_t own_tickets, partial, sel_new, carry, part, lse, tickets, floats;
   int64_t key_stride;                 // keys of a checkpoint row

@@ -305,7 +305,7 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   const int64_t products = (int64_t)l.tiles_max * key_tiles * a.groups;
   const int chunk = products >= 32 * 16 * kSms ? 32 : products >= 8 * 2 * kSms ? 8 : products >= 4 * kSms ? 4 : 1;
   const bool scans = chunk == 1;
-  // store: also clears the tickets of this call, the walks', the scans' and (where they are not the plan's) the single tokens'
+  // store: also clears the tickets of this call, the walks', the scans' and (where they are not the plan's) the few tokens'
   const int n_walk = l.tiles_max * a.heads, n_scan = scans ? l.tiles_max * a.groups * key_tiles : 0;
   {
     const TokenRows k{static_cast<const uint4*>(a.k), a.k_stride[0] / 8, a.k_stride[1] / 8};

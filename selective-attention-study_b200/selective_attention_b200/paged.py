@@ -59,7 +59,8 @@ def append_tokens(tables: dict, counts: torch.Tensor, total: int, max_length: in
     step has; q, k, v of its attention hold them row after row.
 
     ``max_length`` and ``max_count`` are bounds that the host knows: no row is longer after the step, no row gets more tokens.  They
-    set scratch and launches (a step with max_count 1 is a decode step); by default they are what the tables allow.
+    set scratch and launches (a step with a max_count of up to 8 is a decode step: one launch a layer); by default they are what
+    the tables allow.
 
     Returns "query_start" (rows + 1,) int32, where each row's tokens start (cut at ``total``); "cached" (rows,) int32, the tokens
     before the step; "slots" (total,) int64, page * page_size + offset of every token.  A row that does not fit -- its table, the
