@@ -418,7 +418,8 @@ int sa_page_move(const sa_page_tables* tables, const int32_t* copies, const int3
 
 /* The `width` (at most 32) best continuations of every group of beams (at most 256): scores[k] + logits[k][v] - log sum_u
  * exp(logits[k][u]), largest first, equal ones by the lowest k * vocab + v.  A score that is not finite (a beam whose score is
- * -inf, or whose logits hold a NaN or +inf or nothing but -inf) counts as -inf.
+ * -inf, or whose logits hold a NaN or +inf or nothing but -inf) counts as -inf.  Scores of two beams that are nearer to one another
+ * than the rounding of a log-sum-exp of 32-bit exponentials (2^-20 at most) may stand in either order.
  *   logits      (groups, beams, vocab) at group and beam strides, contiguous along the vocabulary
  *   scores      (groups, beams) fp32
  *   out_scores, out_rows, out_tokens   (groups, width): fp32; int32 group * beams + beam; int64 */
