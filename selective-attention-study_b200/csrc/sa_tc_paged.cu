@@ -347,7 +347,9 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   // The plan's numbers are on the device: the host goes by the tiles that there are at least, and by the items that there can be.
   // (A CTA without an item takes an SM for a microsecond.)
   const int items_max = (int)min((int64_t)l.tile_items_max, (int64_t)l.tiles_max * ((key_tiles + paged::kPieceTiles - 1) / paged::kPieceTiles));
-  const int tiles_min = (a.total - (a.rows - 1) + kTile - 1) / kTile;
+  // (Either kernel is right whatever the plan has: one that knows no pieces takes a whole walk for each of them.)  At least: all tokens
+  // in full tiles, or one for each row of more than a few, of which none has more than max_count.
+  const int tiles_min = max((a.total - (a.rows - 1) + kTile - 1) / kTile, (a.total - paged::kFewTokens * a.rows) / (a.max_count - paged::kFewTokens));
   ProfileScope prof(SA_KERNEL_TC_FORWARD, s);
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
   const RowLayout y_rows{0, D, (int64_t)a.heads * D};

@@ -258,6 +258,22 @@ def test_chunks_of_many_tiles(per_head, achieved):
     achieved(f"paged chunks of many tiles per_head={per_head}", share_of_bound=worst)
 
 
+@pytest.mark.parametrize("heads,dim,per_head", [(16, 64, False), (32, 64, False), (16, 64, True), (16, 128, False), (8, 128, True)])
+def test_a_step_with_room_for_more_tokens(heads, dim, per_head):
+    """The kernels are chosen for `total` tokens, the plan is made for those that there are."""
+    s = Served(2, heads, dim, 64, 45, 70, per_head, exempt=2, scale=0.4, seed=10)
+    s.step([1200, 30])
+    s.step([150, 0], total=2600)
+    s.step([0, 40], total=2000, max_count=1300)
+    s.step([5, 9], total=1900)
+    s.pools()
+    s = Served(1, heads, dim, 64, 45, 45, per_head, exempt=2, scale=0.4, seed=11)
+    s.step([1200])
+    s.step([150], total=1650)
+    s.step([3], total=1400)
+    s.pools()
+
+
 def test_rows_that_are_not_served():
     s = Served(5, 4, 64, 16, 12, 16, scale=0.5)
     s.step([100, 20, 0, 5, 1])
