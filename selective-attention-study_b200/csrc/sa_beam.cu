@@ -64,8 +64,9 @@ __device__ __forceinline__ double warp_max(double x) {
 
 // Calls emit(rank, value, index) for the `width` first of the CTA's elements, which the first `warps` warps have.  `mine` is the
 // largest value of the calling thread's (-inf: none).  reach(bound, above, f) calls f(value, index) for the CTA's elements that are
-// not below `bound` (`above`: that are above it), until that says no, one(f) for the calling thread's (no value a NaN).  equal(x, n, f) calls f(k, index) for the first n
-// of the elements that are x, or returns false.  All threads call this; emit is called by any.
+// not below `bound` (`above`: that are above it), until that says no, one(f) for the calling thread's (no value a NaN).
+// equal(x, n, f) calls f(k, index) for the first n of the elements that are x, or returns false.  All threads call this; emit is
+// called by any.
 template <typename V, typename I, typename Reach, typename One, typename Equal, typename Emit>
 __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, V mine, const Reach& reach, const One& one, const Equal& equal,
                                         const Emit& emit) {

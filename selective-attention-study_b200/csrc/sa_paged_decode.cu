@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(kAllThreads, D == 64 ? 4 : 2) decode_pages_ker
           for (int u = tid; u < rows * (other ? 3 : 2) * DK * 8; u += kThreads) {
             const int col = u % (DK * 8), which = u / (DK * 8) % (other ? 3 : 2), row = row0 + u / (DK * 8 * (other ? 3 : 2));
             const int64_t token = w.token + (j0 + row - a0), token_slot = slots[token];
-            const __nv_bfloat16* from = which == 1 ? v_new + token * v_str.token + h * v_str.head : k_new + token * k_str.token + (which == 0 ? h : h0) * k_str.head;
+            const __nv_bfloat16* from = which == 1 ? v_new + token * v_str.token + h * v_str.head
+                                                   : k_new + token * k_str.token + (which == 0 ? h : h0) * k_str.head;
             const uint4 x = reinterpret_cast<const uint4*>(from)[col];
             *reinterpret_cast<uint4*>(stage + (which * DK + (col >> 3)) * kTileBytes + tc::swz_off(row, col & 7)) = x;
             if (which < 2 && token_slot >= 0 && token_slot < ((int64_t)num_pages << page_shift)) {

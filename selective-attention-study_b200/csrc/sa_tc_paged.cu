@@ -332,8 +332,9 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   const History history{a.selected, a.sel_stride, scans ? walk_tickets + n_walk : nullptr};
   {
     ProfileScope prof(SA_KERNEL_TC_COLSUM, s);
-    st = launch_after(colsum_pages_kernel<D>, dim3(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups), 160, 3 * DK * kRowTile + 1024, s, map_q, map_k, carry, a.exempt,
-                      scale, status, chunk, tiles, walk, history);
+    const dim3 grid(l.tiles_max, (key_tiles + chunk - 1) / chunk, a.groups);
+    st = launch_after(colsum_pages_kernel<D>, grid, 160, 3 * DK * kRowTile + 1024, s, map_q, map_k, carry, a.exempt, scale, status, chunk,
+                      tiles, walk, history);
     if (st != SA_OK) return st;
     *moved = scans;
   }
@@ -362,7 +363,8 @@ int tiles_impl(const Attention& a, bool* moved, cudaStream_t s) {
   if (D == 64 && self && a.heads % 2 == 0 && two_heads(a.rows, tiles_min, key_tiles, a.heads))
     return forward_self_pages(walk, map_q, map_k, map_v, carry, items_max, a.exempt, scale, status, y, y_rows, s);
   auto wide = [&](auto kernel) {
-    return launch_after(kernel, dim3((unsigned)items_max * a.heads), kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
+    const dim3 grid((unsigned)items_max * a.heads);
+    return launch_after(kernel, grid, kWidePagedThreads, WideSmem<D>::total + 1024, s, map_q, map_k, map_v, map_q, map_k, (const float*)carry,
                   (float*)nullptr, (float*)nullptr, a.heads, 0, 0, a.exempt, scale, status, y, y_rows, 0, (const uint8_t*)nullptr,
                   SplitWalk{}, walk);
   };
