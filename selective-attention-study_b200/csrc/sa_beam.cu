@@ -14,8 +14,9 @@
 //
 // The largest of a set, without sorting it: each warp that has elements gives the largest of its lanes' own maxima, about two times
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among
-// themselves.  Where more than kList reach it, because many are equal to it (masked logits, most often), those above it are ranked
-// and the first of the equal ones are found in order; where that is not so either, they are taken one by one.
+// themselves.  Where more than kList reach it (one beam far above the others, most often), the WIDTH-th of the first kList of them is a
+// better bound; where that does not help because many are equal to it (masked logits, most often), those above it are ranked and the
+// first of the equal ones are found in order; where that is not so either, they are taken one by one.
 #include <type_traits>
 
 #include "sa_common.cuh"
@@ -27,7 +28,7 @@ namespace beam {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kList = 256;
+constexpr int kList = kThreads;
 
 template <typename V, typename I>
 struct Entry {
@@ -43,6 +44,7 @@ __device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& 
 template <typename V, typename I>
 struct Shared {
   V tops[2 * kMaxWidth];
+  V bound;
   Entry<V, I> list[kList];
   int count;
   Entry<V, I> warp_best[kThreads / 32];
@@ -103,6 +105,26 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, 
   });
   __syncthreads();
   int n = sh.count;
+  while (n > kList) {                                        // of those that are on the list the `width`-th is a better bound
+    const V own = sh.list[tid].value;
+    int rank = 0;
+#pragma unroll 8
+    for (int u = 0; u < kList; ++u) rank += sh.list[u].value > own || (sh.list[u].value == own && u < tid) ? 1 : 0;
+    if (rank == width - 1) sh.bound = own;
+    __syncthreads();
+    const V better = sh.bound;
+    if (!(better > bound)) break;
+    bound = better;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    reach(bound, false, [&](V x, I i) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kList) sh.list[at] = Entry<V, I>{x, i};
+      return at <= kList;
+    });
+    __syncthreads();
+    n = sh.count;
+  }
   int ties = 0;                                              // of the first `width`, those that are equal to the bound
   if (n > kList) {
     __syncthreads();

@@ -81,6 +81,11 @@ def test_many_candidates(groups, n, vocab, width):
     scores[:, 1:] = -float("inf")                                 # a search's first step
     _check(logits.cuda(), scores.cuda(), width)
     _check(torch.zeros_like(logits).cuda(), torch.zeros_like(scores).cuda(), width)
+    logits = (torch.randn(groups, n, vocab, generator=gen) * 3).bfloat16()
+    for far in (3.0, 100.0):                                      # one beam far above the others
+        scores = -far - torch.rand(groups, n, generator=gen)
+        scores[:, n // 2] = 0.0
+        _check(logits.cuda(), scores.cuda(), width)
 
 
 def test_arguments_that_are_refused():
