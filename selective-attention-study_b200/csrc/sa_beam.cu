@@ -66,7 +66,8 @@ __device__ __forceinline__ double warp_max(double x) {
 
 // Calls emit(rank, value, index) for the `width` first of the CTA's elements, which the first `warps` warps have.  `mine` is the
 // largest value of the calling thread's (-inf: none).  reach(bound, above, f) calls f(value, index) for the CTA's elements that are
-// not below `bound` (`above`: that are above it), until that says no, one(f) for the calling thread's (no value a NaN).
+// not below `bound` (`above`: that are above it), until that says no, one(f) for the calling thread's (no value a NaN), of a list in
+// order up to the first that f says yes to at least.
 // equal(x, n, f) calls f(k, index) for the first n of the elements that are x, or returns false.  All threads call this; emit is
 // called by any.
 template <typename V, typename I, typename Reach, typename One, typename Equal, typename Emit>
@@ -161,7 +162,9 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, 
     };
     one([&](V x, I i) {
       const Entry<V, I> e{x, i};
-      if (w == 0 || before(last, e)) better(e);
+      const bool left = w == 0 || before(last, e);
+      if (left) better(e);
+      return left;
     });
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
@@ -462,13 +465,9 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
     }
   };
   auto each = [&](auto f) {
-    if constexpr (!MANY) {
 #pragma unroll
-      for (int u = 0; u < kKept; ++u)
-        if (place + u * kThreads < n) one(place + u * kThreads, kept_k[u], kept_v[u], kept_t[u], f);
-    } else {
-      for (int i = place; i < n; i += kThreads) one(i, i / per_beam, values[first + i], tokens[first + i], f);
-    }
+    for (int u = 0; u < kKept; ++u)
+      if (place + u * kThreads < n) one(place + u * kThreads, kept_k[u], kept_v[u], kept_t[u], f);
   };
   // f(score, place) for the candidates of this thread's lists, of each until that says no
   auto lists = [&](auto f) {
@@ -504,7 +503,11 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const float* __restric
     }
   };
   auto equal = [](double, int, auto) { return false; };        // (places are not in order of their index)
-  largest(sh, width, kThreads / 32, mine, reach, each, equal, [&](int at, double v, long long i) {
+  auto rest = [&](auto f) {
+    if constexpr (MANY) lists([&](double x, long long i) { return !f(x, i); });
+    else each(f);
+  };
+  largest(sh, width, kThreads / 32, mine, reach, rest, equal, [&](int at, double v, long long i) {
     const int64_t o = (int64_t)g * width + at;
     out_scores[o] = (float)v;
     out_rows[o] = g * beams + (int)(i >> 32);
