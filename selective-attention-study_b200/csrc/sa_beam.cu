@@ -29,6 +29,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kList = kThreads;
+constexpr int kTops = 64;              // maxima that make the first bound: a lane of every warp ranks two
+constexpr bool tops_are_enough(int warps) { return warps == 0 || (kTops / warps >= (kMaxWidth + warps - 1) / warps && tops_are_enough(warps - 1)); }
+static_assert(tops_are_enough(kThreads / 32), "the maxima of any number of warps are as many as the widest selection");
 
 template <typename V, typename I>
 struct Entry {
@@ -43,7 +46,7 @@ __device__ __forceinline__ bool before(const Entry<V, I>& a, const Entry<V, I>& 
 
 template <typename V, typename I>
 struct Shared {
-  V tops[2 * kMaxWidth];
+  V tops[kTops];
   V bound;
   Entry<V, I> list[kList];
   int count;
@@ -75,8 +78,9 @@ __device__ __forceinline__ void largest(Shared<V, I>& sh, int width, int warps, 
                                         const Emit& emit) {
   const int tid = threadIdx.x, lane = tid & 31;
   constexpr V kNone = -INFINITY;
-  // of w warps all but the last have 32 lanes' elements (or every lane of all has one): 2 ceil(width / w) of each are enough
-  const int each = min(32, 2 * ((width + warps - 1) / warps)), given = each * warps;      // at most 64 in all
+  // of w warps all but the last have 32 lanes' elements (or every lane of all has one): 2 ceil(width / w) of each are enough, and
+  // so is what kTops has room for (where w does not divide the width twice as many would be up to 72)
+  const int each = min(32, min(2 * ((width + warps - 1) / warps), kTops / warps)), given = each * warps;
   for (int u = 0; u < each && (tid >> 5) < warps; ++u) {
     const V top = warp_max(mine);
     const unsigned at = __ballot_sync(0xffffffffu, mine == top);

@@ -88,6 +88,51 @@ def test_many_candidates(groups, n, vocab, width):
         _check(logits.cuda(), scores.cuda(), width)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("warps", [3, 5, 6, 7])
+@pytest.mark.parametrize("width", [29, 30, 31, 32])
+def test_runs_whose_warps_do_not_divide_the_width(dtype, warps, width):
+    """A run of 3, 5, 6 or 7 warps of 16-byte units: twice as many maxima a warp as an even share are more than 64 in all.  Drawn
+    logits, and maxima gathered in two or three warps so that the last of the first `width` lies far down in one of them."""
+    gen = torch.Generator().manual_seed(100 * warps + width)
+    per = 4 if dtype == torch.float32 else 8
+    for units in (32 * warps, 32 * warps - 31, 32 * warps - 9):
+        logits = torch.randn(40, 1, units * per, generator=gen)
+        scores = -torch.rand(40, 1, generator=gen)
+        _check(logits.to(dtype).cuda(), scores.cuda(), width)
+        _check(logits[:39].view(13, 3, units * per).to(dtype).cuda(), scores[:39].view(13, 3).cuda(), width)
+        each = 2 * -(-width // warps)
+        for g in range(40):
+            # `each` high units in one warp, the lowest of them; as many in the next as reach maximum 63; the others wherever there is room
+            order = [63 % warps] + [w for w in torch.randperm(warps, generator=gen).tolist() if w != 63 % warps]
+            low = order.pop(1 + g % (warps - 1))
+            room = [min(32, units - 32 * w) for w in order]
+            left, takes = width - min(each, min(32, units - 32 * low)), []
+            for w, n in zip(order, room):
+                takes.append((w, min(left, n, 63 // warps + 1)))
+                left -= takes[-1][1]
+            value = 16.0 + 0.125 * width                          # downwards in steps that every type has
+            for w, n in takes + [(low, width - sum(n for _, n in takes))]:
+                for u in torch.randperm(min(32, units - 32 * w), generator=gen)[:n].tolist():
+                    logits[g, 0, (32 * w + u) * per + (u + g) % per] = value
+                    value -= 0.125
+        _check(logits.to(dtype).cuda(), scores.cuda(), width)
+
+
+@pytest.mark.parametrize("dtype,per", [(torch.float32, 4), (torch.bfloat16, 8)])
+def test_a_long_vocabulary_with_a_short_last_run(dtype, per):
+    """488 runs of 512 units and one of 160 (five warps), which holds the best."""
+    gen = torch.Generator().manual_seed(per)
+    vocab = (488 * 512 + 160) * per
+    logits = torch.randn(1, 1, vocab, generator=gen)
+    for _ in range(6):
+        logits[0, 0, -160 * per:] = torch.randn(160 * per, generator=gen)
+        for w, n in ((3, 13), (1, 5), (0, 14)):                   # the 14th of warp 0 is the last of 32
+            units = torch.randperm(32, generator=gen)[:n] + 32 * w
+            logits[0, 0, (488 * 512 + units) * per + 1] = 16.0 + 0.125 * torch.arange(n) + 4 * (w > 0) + 2 * (w > 1)
+        _check(logits.to(dtype).cuda(), torch.zeros(1, 1).cuda(), 32)
+
+
 def test_arguments_that_are_refused():
     x, s = torch.zeros(2, 3, 10, device="cuda"), torch.zeros(2, 3, device="cuda")
     for bad in ((x, s, 0), (x, s, 31), (x, s, 33), (x.long(), s, 2), (x, s.cpu(), 2), (x[:, :0], s[:, :0], 1), (x, s[:, :2], 2)):
