@@ -81,9 +81,12 @@ __global__ void __launch_bounds__(kAllThreads, D == 64 ? 4 : 2) decode_pages_ker
   if (!beside) {
     tc::after_previous_kernel();
   } else {
-    // The kernel before is that of the same call's tiles, which this one needs nothing of: it has let this one begin once
-    // everything before it was there.  One block more waits for its end, so that what comes after both waits for both.
+    // The kernel before is that of the same call's tiles, which this one needs nothing of: each of its blocks has let this one
+    // begin after its own wait, when the plan, the pages and the histories that earlier kernels wrote were performed in device
+    // memory.  This grid has not waited for those itself, so every thread fences before its first load: none of them is served by
+    // a line that was read before.  One block more waits for the tiles' end, so that what comes after both waits for both.
     asm volatile("griddepcontrol.launch_dependents;");
+    __threadfence();
     if (blockIdx.x == (unsigned)items_max * heads) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       return;
