@@ -385,7 +385,7 @@ typedef struct sa_paged_attention {
   int32_t struct_bytes;   /* sizeof(sa_paged_attention) */
   int32_t groups, head_dim, exempt, total, max_length, max_count, plan_tickets;
   const sa_page_tables* tables;
-  const int32_t *query_start, *cached;
+  const int32_t *query_start, *cached;   /* not read, may be NULL: `work` has what they say */
   const int64_t* slots;
   int32_t* work;
   void *k_pages, *v_pages;

@@ -79,7 +79,7 @@ inline StepLayout step_layout(int rows, int total, int heads) {
 struct Attention {
   int rows, max_pages, num_pages, page_shift, heads, groups, head_dim, exempt;
   int total, max_length, max_count;
-  const int *block_tables, *query_start, *cached;
+  const int* block_tables;
   const int64_t* slots;
   int* work;                          // the step's plan, with its tickets
   bool plan_tickets;                  // the plan's tickets are this call's alone while it runs; false: the call clears its own

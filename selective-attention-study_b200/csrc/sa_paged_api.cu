@@ -108,8 +108,7 @@ int sa_paged_run(const sa_paged_attention* in) {
   paged::Attention a;
   int st = to_attention(in, &a);
   if (st != SA_OK) return st;
-  if (!in->query_start || !in->cached || !in->slots || !in->work || !in->q || !in->k || !in->v || !in->k_pages || !in->v_pages ||
-      !in->selected || !in->y || !in->workspace)
+  if (!in->slots || !in->work || !in->q || !in->k || !in->v || !in->k_pages || !in->v_pages || !in->selected || !in->y || !in->workspace)
     return SA_ERR_BAD_ARGUMENT;
   for (const void* p : {in->q, in->k, in->v, (const void*)in->k_pages, (const void*)in->v_pages, (const void*)in->y, (const void*)in->work})
     if (!aligned(p, 16)) return SA_ERR_ALIGNMENT;
@@ -118,7 +117,7 @@ int sa_paged_run(const sa_paged_attention* in) {
     if (s[0] % 8 != 0 || s[1] % 8 != 0 || s[0] <= 0 || s[1] <= 0) return SA_ERR_ALIGNMENT;
   if (in->workspace_bytes < paged::attention_scratch(a).floats * 4) return SA_ERR_WORKSPACE;
   if (tc::timeout_pending()) return SA_ERR_DEVICE_TIMEOUT;
-  a.query_start = in->query_start; a.cached = in->cached; a.slots = in->slots; a.work = in->work;
+  a.slots = in->slots; a.work = in->work;
   a.plan_tickets = in->plan_tickets != 0;
   a.k_pages = in->k_pages; a.v_pages = in->v_pages; a.selected = in->selected;
   a.q = in->q; a.k = in->k; a.v = in->v; a.y = in->y;

@@ -462,7 +462,7 @@ void check_int32(const Tensor& x, const PageTables& t, int64_t n, const char* wh
 
 // A step as paged.append_tokens made it: its plan, its bounds, and the stream and capture that it was made on.
 struct PageStep {
-  Tensor query_start, cached, slots, work;
+  Tensor cached, slots, work;
   int64_t max_pages, num_pages, page_size, max_length, max_count;
   uint64_t stream, capture;
 };
@@ -486,8 +486,8 @@ pybind11::tuple append_tokens(const pybind11::dict& tables, const Tensor& counts
                                          query_start.data_ptr<int32_t>(), cached.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
                                          work.data_ptr<int32_t>(), stream));
   return pybind11::make_tuple(query_start, cached, slots,
-                              PageStep{query_start, cached, slots, work, p.max_pages, p.num_pages, p.page_size, max_length, max_count, reinterpret_cast<uint64_t>(stream),
-                                       (uint64_t)sa_stream_capture(stream)});
+                              PageStep{cached, slots, work, p.max_pages, p.num_pages, p.page_size, max_length, max_count,
+                                       reinterpret_cast<uint64_t>(stream), (uint64_t)sa_stream_capture(stream)});
 }
 
 void check_pools(const PageTables& t, const sa_page_tables& p, const Tensor& kc, const Tensor& vc, const Tensor& selected) {
@@ -539,7 +539,6 @@ Tensor paged_attention(const pybind11::dict& tables, const PageStep& step, const
   // calls on the stream that made the plan, outside any capture or in the same one, run one after the other
   a.plan_tickets = step.stream == reinterpret_cast<uint64_t>(stream) && step.capture == (uint64_t)sa_stream_capture(stream);
   a.tables = &p;
-  a.query_start = step.query_start.data_ptr<int32_t>(); a.cached = step.cached.data_ptr<int32_t>();
   a.slots = step.slots.data_ptr<int64_t>(); a.work = step.work.data_ptr<int32_t>();
   a.k_pages = kc.data_ptr(); a.v_pages = vc.data_ptr(); a.selected = selected.data_ptr<float>();
   a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();

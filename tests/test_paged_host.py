@@ -115,6 +115,24 @@ def test_bad_attention_is_refused_before_any_launch():
     assert status(k_pages=4104)[0] == 3 and status(q_stride=[128, 68])[0] == 3 and status(v_stride=[128, 0])[0] == 3 and status(workspace=4112)[0] == 3
 
 
+def test_attention_takes_rows_from_the_plan_alone():
+    """What the plan holds already need not be given a second time: a call without it gets as far as its workspace."""
+    lib, t = _lib.load(), _c_tables()
+    p = _lib.PagedAttention()
+    p.struct_bytes = ctypes.sizeof(_lib.PagedAttention)
+    p.tables = ctypes.pointer(t)
+    p.groups, p.head_dim, p.exempt, p.total, p.max_length, p.max_count = 1, 64, 1, 4, 64, 4
+    for name in ("slots", "work", "k_pages", "v_pages", "selected", "q", "k", "v", "y", "workspace"):
+        setattr(p, name, 4096)
+    for name in ("q_stride", "k_stride", "v_stride"):
+        getattr(p, name)[:] = [128, 64]
+    assert lib.sa_paged_run(ctypes.byref(p)) == 4                  # workspace_bytes 0
+    for name in ("slots", "work"):
+        setattr(p, name, None)
+        assert lib.sa_paged_run(ctypes.byref(p)) == 1
+        setattr(p, name, 4096)
+
+
 def test_bad_selections_are_refused_before_any_launch():
     lib = _lib.load()
 
