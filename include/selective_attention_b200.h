@@ -408,7 +408,7 @@ int sa_paged_run(const sa_paged_attention* p);
  *   copies   (rows, 2): the page to copy and the one that receives it, or -1 -1
  *   work     sa_page_reorder_words() int32 words, 16-byte aligned; sa_page_move reads it
  * Pages that no row holds any more go to the end of the free list, lowest first, before the new ones are taken off it.  A row for
- * which there is none becomes empty.
+ * which there is none becomes empty, and work[1] is how many did.
  * sa_page_move: the tokens of those pages and the histories of the rows, for one layer.  Behind a row's last token everything is
  * left as it was. */
 size_t sa_page_reorder_words(int rows, int max_pages, int num_pages);

@@ -344,8 +344,8 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // or of 500 pages 8 us, 256 rows of 24 10 us.
 constexpr int kCluster = 8, kReorderThreads = 1024;
 
-// The work of a reordering, int32 words: how many rows change, then (row, parent, tokens, tokens of the page being filled) of
-// each | a word a row | a bit a page | the new tables.
+// The work of a reordering, int32 words: how many rows change, how many were lost for want of a page, then (row, parent, tokens,
+// tokens of the page being filled) of each that changes | a word a row | a bit a page | the new tables.
 struct ReorderWork {
   size_t moved, info, marks, scratch, words;
   ReorderWork(int rows, int max_pages, int num_pages) {
@@ -470,7 +470,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
           if (real(dst)) atomicAdd(t.page_refs + dst, 1);
         } else {                                                  // out of pages: the row becomes empty
           dropped = true;
-          dropped_s = 1;
+          atomicAdd(&dropped_s, 1);
           for (int b = 0; b < full; ++b)
             if (real(__ldcg(now + b))) atomicSub(t.page_refs + __ldcg(now + b), 1);
         }
@@ -491,6 +491,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kReorderThrea
     }
   }
   cluster.sync();
+  if (me == 0) moved[1] = dropped_s;
   if (cta == 0 && dropped_s != 0) {
     for (int r = warp; r < t.rows; r += kReorderThreads / 32) {
       if (__ldcg(info + r) == 0 || copies[2 * r + 1] >= 0) continue;

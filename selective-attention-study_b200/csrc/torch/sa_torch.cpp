@@ -563,9 +563,13 @@ pybind11::tuple reorder_rows(const pybind11::dict& tables, const Tensor& parents
   const c10::cuda::CUDAGuard guard(t.block_tables.device());
   const int64_t words = (int64_t)sa_page_reorder_words(p.rows, p.max_pages, p.num_pages);
   Carved all(Carved::room(8 * p.rows) + Carved::room(4 * words), parents);
-  const Tensor copies = all.take({p.rows, 2}, at::kInt), work = all.take({words}, at::kInt);
+  const Tensor copies = all.take({p.rows, 2}, at::kInt);
+  const int64_t work_at = all.at;
+  const Tensor work = all.take({words}, at::kInt);
+  all.at = work_at + 4;                           // work[1]
+  const Tensor lost = all.take({1}, at::kInt);
   check("sa_page_reorder", sa_page_reorder(&p, parents.data_ptr<int32_t>(), copies.data_ptr<int32_t>(), work.data_ptr<int32_t>(), stream_of(t.lengths)));
-  return pybind11::make_tuple(copies, work);
+  return pybind11::make_tuple(copies, work, lost);
 }
 
 void move_rows(const pybind11::dict& tables, const Tensor& copies, const Tensor& work, const Tensor& kc, const Tensor& vc, const Tensor& selected) {

@@ -91,9 +91,10 @@ def reorder_rows(tables: dict, parents: torch.Tensor) -> dict:
     Full pages are shared between the copies.  The page that is still being filled stays with the lowest row that has the
     parent; the others get a page of their own, and ``move_rows`` copies its tokens in every layer: "copies" (rows, 2) int32
     holds source and target, or -1, -1.  Pages that nobody holds any more go back first, lowest first.  A row that needs a page
-    when there is none becomes empty."""
-    copies, work = _lib.native().reorder_rows(tables, parents)
-    return {"copies": copies, "tables": tables, "_work": work}
+    when there is none becomes empty: "lost" (1,) int32 is how many did, and their "lengths" are 0.  What they were is gone, so a
+    search that must not lose a beam keeps a free page for every row."""
+    copies, work, lost = _lib.native().reorder_rows(tables, parents)
+    return {"copies": copies, "lost": lost, "tables": tables, "_work": work}
 
 
 def move_rows(cache: dict, moves: dict) -> None:

@@ -112,6 +112,22 @@ def test_copies_in_a_full_pool():
     assert int(t["free_count"]) == 8
 
 
+@pytest.mark.parametrize("rows,free", [(6, 0), (6, 2), (40, 7), (1500, 700), (300, 299), (300, 300)])
+def test_rows_that_are_lost_are_counted(rows, free):
+    """Copies of one row that need a page each, in a pool that has `free` of them; then with nothing to copy."""
+    t, want = _both(rows, 2 + free, 16, 2)
+    _append(t, want, [21] + [0] * (rows - 1), 21)
+    moves = paged.reorder_rows(t, _ints([0] * rows))
+    assert [tuple(x) for x in moves["copies"].tolist()] == want.reorder([0] * rows)
+    _same_tables(t, want)
+    assert moves["lost"].dtype == torch.int32 and moves["lost"].tolist() == [max(rows - 1 - free, 0)]
+    assert int((t["lengths"] == 0).sum()) == max(rows - 1 - free, 0)
+    moves = paged.reorder_rows(t, _ints(list(range(rows))))
+    assert moves["lost"].tolist() == [0] and (moves["copies"] == -1).all()
+    moves = paged.reorder_rows(t, _ints([-1] * rows))             # given back, not lost
+    assert moves["lost"].tolist() == [0] and int(t["free_count"]) == 2 + free
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 
 class Served:
