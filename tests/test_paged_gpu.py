@@ -342,6 +342,26 @@ def test_tokens_of_any_strides():
     assert torch.isfinite(ys[5].float()).all()
 
 
+@pytest.mark.parametrize("counts", [[33, 1], [1, 1], [5, 1]])
+def test_tokens_of_heads_that_share_them(counts):
+    """q, k, v of one head for all of them (a stride of 0 over heads), or of one token for all: as when every head has its copy."""
+    s = _prefix(4, 64, False, [70, 300])
+    n = sum(counts)
+    step = paged.append_tokens(s.t, _ints(counts), n, max_count=max(counts))
+    q, k, v = (x.cuda() for x in s.tokens(n))
+    head = lambda x: x[:, :1].expand(-1, 4, -1)                    # noqa: E731
+    token = lambda x: x[:1].expand(n, -1, -1)                      # noqa: E731
+    both = lambda x: x[:1, :1].expand(n, 4, -1)                    # noqa: E731
+    for form in ((head(q), k, v), (q, head(k), v), (q, k, head(v)), (token(q), token(k), token(v)), (both(q), both(k), both(v)),
+                 (head(q).float(), head(k).half(), token(v).float())):
+        shared, own = ({name: x.clone() for name, x in s.cache.items()} for _ in range(2))
+        y = paged.paged_attention(shared, s.t, step, *form)
+        want = paged.paged_attention(own, s.t, step, *(x.bfloat16().contiguous().clone() for x in form))
+        assert torch.equal(y, want) and torch.isfinite(y.float()).all() and (y != 0).any()
+        for name in ("k", "v", "selected"):
+            assert torch.equal(torch.nan_to_num(shared[name]), torch.nan_to_num(own[name])), name
+
+
 @pytest.mark.parametrize("heads,per_head", [(2, False), (16, False), (4, True)])
 def test_keys_that_were_taken_out(heads, per_head):
     """Keys whose history their owner has made infinite have no weight: as if they were not there."""
