@@ -378,8 +378,8 @@ int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int tota
  *   total, max_length, max_count   as sa_page_append was given them for this plan
  *   q, k, v           (total, heads, head_dim) with token and head strides, multiples of 8 elements, not 0
  *   y                 (total, heads, head_dim) contiguous; zeros for tokens without a slot
- *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream); 0: the call
- *                     clears tickets of its own
+ *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream, by any
+ *                     thread); 0: the call clears tickets of its own
  * A page outside the pool reads as zeros.  A call that returns an error leaves the histories as they were. */
 typedef struct sa_paged_attention {
   int32_t struct_bytes;   /* sizeof(sa_paged_attention) */

@@ -1,5 +1,7 @@
 // extern "C" boundary of the paged cache and of beam selection: argument checks.  Declarations are in
 // include/selective_attention_b200.h.
+#include <mutex>
+
 #include "sa_beam.cuh"
 #include "sa_paged.cuh"
 #include "sa_tc_host.cuh"
@@ -128,6 +130,10 @@ int sa_paged_run(const sa_paged_attention* in) {
   }
   a.workspace = static_cast<float*>(in->workspace);
   cudaStream_t s = static_cast<cudaStream_t>(in->stream);
+  // A call's launches stand together in its stream: with another thread's between them, the few tokens of two calls could run at
+  // once, and calls of one plan and stream share its tickets.
+  static std::mutex launches;
+  const std::lock_guard<std::mutex> guard(launches);
   // Rows of few tokens go through a kernel of their own, the others through the tile kernels; the step's bounds say where there can
   // be none of either.
   if (paged::few_only(a.total, a.max_count)) return paged::decode(a, false, s);

@@ -536,6 +536,37 @@ def test_layers_share_a_step_on_two_streams_and_in_two_graphs(counts):
         assert torch.equal(torch.nan_to_num(cache["selected"]), torch.nan_to_num(layers[0]["selected"]))
 
 
+@pytest.mark.parametrize("counts", [[1, 1, 200, 1], [5, 1, 1, 8]])
+def test_layers_of_a_step_from_two_threads(counts):
+    """Calls of one step on one stream by several threads at once: as one after the other."""
+    import threading
+
+    s = _prefix(4, 64, False, [600, 500, 30, 640])
+    n, layers = sum(counts), 24
+    caches = [{name: x.clone() for name, x in s.cache.items()} for _ in range(layers + 1)]
+    step = paged.append_tokens(s.t, _ints(counts), n, max_count=max(counts))
+    q, k, v = (x.cuda() for x in s.tokens(n))
+    want = paged.paged_attention(caches[layers], s.t, step, q, k, v)
+    torch.cuda.synchronize()
+    ys, start = [None] * layers, threading.Barrier(4)
+
+    def work(first):
+        start.wait()
+        for i in range(first, layers, 4):
+            ys[i] = paged.paged_attention(caches[i], s.t, step, q, k, v)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for y, cache in zip(ys, caches):
+        assert torch.equal(y, want)
+        for name in ("k", "v", "selected"):
+            assert torch.equal(torch.nan_to_num(cache[name]), torch.nan_to_num(caches[layers][name]))
+
+
 def test_the_same_step_gives_the_same_bits():
     s = _prefix(4, 64, False, [3000 % 600, 9, 600])
     saved = [{name: x.clone() for name, x in s.cache.items()} for _ in range(3)]
