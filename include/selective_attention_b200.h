@@ -375,7 +375,7 @@ int sa_page_append(const sa_page_tables* tables, const int32_t* counts, int tota
  * or every head its own).  Stores k and v in their pages, moves the histories on.
  *   k_pages, v_pages  (num_pages, heads, page_size, head_dim)
  *   selected          (rows, groups, max_pages * page_size) fp32
- *   total, max_length, max_count   as sa_page_append was given them for this plan
+ *   total, max_length, max_count   as sa_page_append was given them for this plan (max_length: at most max_pages * page_size)
  *   q, k, v           (total, heads, head_dim) with token and head strides, multiples of 8 elements, not 0
  *   y                 (total, heads, head_dim) contiguous; zeros for tokens without a slot
  *   plan_tickets      1: no other call that uses this plan's tickets runs at the same time (calls of one stream, by any
@@ -419,7 +419,8 @@ int sa_page_move(const sa_page_tables* tables, const int32_t* copies, const int3
 /* The `width` (at most 32) best continuations of every group of beams (at most 256): scores[k] + logits[k][v] - log sum_u
  * exp(logits[k][u]), largest first, equal ones by the lowest k * vocab + v.  A score that is not finite (a beam whose score is
  * -inf, or whose logits hold a NaN or +inf or nothing but -inf) counts as -inf.  Scores of two beams that are nearer to one another
- * than the rounding of a log-sum-exp of 32-bit exponentials (2^-20 at most) may stand in either order.
+ * than the rounding of a log-sum-exp of 32-bit exponentials (2^-20 at most) may stand in either order, and so may those of one beam
+ * that 64 bits do not tell apart.
  *   logits      (groups, beams, vocab) at group and beam strides, contiguous along the vocabulary
  *   scores      (groups, beams) fp32
  *   out_scores, out_rows, out_tokens   (groups, width): fp32; int32 group * beams + beam; int64 */

@@ -7,10 +7,10 @@
 // sum of exponentials and its WIDTH largest logits.  choose_kernel (a CTA a group) makes the
 // beams' log-sum-exp of those and takes the best of all candidates, in 64 bits: two beams' scores can be as near to one another as
 // the rounding of a 32-bit sum, and which one comes first is a whole number.
-// 256 beams of 50,304 bf16 logits (25.7 MB): 13 + 6 us.  Where the first goes, in cycles of a CTA that ends last: 1,500 until its loads
-// are issued, 12,000 until its first part is there (behind the three other CTAs of its SM), 19,000 until it has looked at the run,
-// 24,000 with the ranking.  From L2 the first part takes 4,600 and the rest as long, so the exponentials (8 cycles of a warp each) and
-// the loads share the blame.  4 beams: 6 + 6 us, latency.
+// 256 beams of 50,304 bf16 logits (25.7 MB): 16.2 us both, each alone with cold caches 14.6 and 6.2.  Where the first goes, in cycles
+// of a CTA that ends last: 1,500 until its loads are issued, 12,000 until its first part is there (behind the three other CTAs of its
+// SM), 19,000 until it has looked at the run, 24,000 with the ranking.  From L2 the first part takes 4,600 and the rest as long, so the
+// exponentials (8 cycles of a warp each) and the loads share the blame.  4 beams: 7.6 us both, alone 6 to 7 and 5 to 6: latency.
 //
 // The largest of a set, without sorting it: each warp that has elements gives the largest of its lanes' own maxima, about two times
 // WIDTH of them in all.  WIDTH elements at least reach the WIDTH-th of those, and not many more do.  They are ranked among

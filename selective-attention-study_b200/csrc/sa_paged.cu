@@ -341,7 +341,7 @@ constexpr int kInside = 2048;         // tokens of a step that one CTA writes by
 // of an old row, marking those that nobody holds; (3) one CTA puts the marked pages on the free list, lowest first, and takes the
 // pages for the copies off its end, in row order, while (4) the others write the tables.  A row for which there is none becomes
 // empty (its full pages are shared with the lowest child, so nothing else is freed).  Bound by the latency of the passes: 4 rows of 26
-// or of 500 pages 8 us, 256 rows of 24 10 us.
+// or of 500 pages 8 to 9 us, 256 rows of 24 11 us; with cold caches 10, 12 and 13 to 14.
 constexpr int kCluster = 8, kReorderThreads = 1024;
 
 // The work of a reordering, int32 words: how many rows change, how many were lost for want of a page, then (row, parent, tokens,
@@ -603,7 +603,7 @@ int reorder(const Tables& t, const int* parents, int* copies, int* work, cudaStr
   const size_t smem = 2 * (size_t)t.rows * 4;
   SA_CUDA_CHECK(allow_smem(reorder_kernel, smem));
   // where there are more warps than rows, a row's pages are cut into parts of a warp's width or more, a power of two of them
-  // (4 rows of 500 pages: 28.8 us with a warp a row, 8.6 us so; 256 rows of 24 pages: no parts)
+  // (4 rows of 500 pages: 28.8 us with a warp a row, 8.2 us so; 256 rows of 24 pages: no parts)
   int shift = 0;
   while ((t.rows << (shift + 1)) <= kCluster * kReorderThreads / 32 && (32 << shift) < t.max_pages) ++shift;
   const int span = (t.max_pages + (1 << shift) - 1) >> shift;

@@ -20,7 +20,8 @@
 // copy rate (89 in pages of 16); 64 rows of 1 to 7,000 tokens 142 us, 93 %.  With p in 32 bits on the CUDA cores and a lane
 // group a key, which is 28 instructions a key, they took 105 and 190 us.  Several tokens of each of the 64 rows: 2, 4, 8 163, 166, 172 us
 // (as tiles of 128 queries 383, 384, 391), 5 after 131,000 97 us (207); 16 rows of 1 to 6,000 66 us, 40 % more instructions than for
-// one token and a second K through L2.
+// one token and a second K through L2.  8 heads of head_dim 128 (as many bytes as 16 of 64): a row of 131,000 91 us, 102 with four
+// tokens; 64 rows of 226,000 tokens in all 145 us (16 heads of 64: 145), 168 with four tokens of each.
 // Pieces: one wave of CTAs over all heads, or four where the rows alone fill half of one.  131,000 tokens in 1, 1.5, 2, 4 waves:
 // 86.5, 91.7, 90.6, 99.7 us; the 64 rows in 1, 2, 4, 8: 159, 159, 139, 140; 16 rows of 1 to 6,000 in 1, 2, 4: 37, 39, 43.
 #include <float.h>

@@ -18,5 +18,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int) -> tuple
     a beam that does not take part.  Returns the new scores (groups, width) fp32, the row that each comes from (int32, counted
     over all groups: ``parents`` of ``paged.reorder_rows`` where every group has ``width`` rows), and its token (int64).
     Compared in 64 bits, over log-sum-exps of 32-bit exponentials (2^-20 at most): continuations of two beams that are nearer to one
-    another than that may come in either order.  Where a beam's logits hold a NaN or +inf, or nothing above -inf, its continuations count as -inf."""
+    another than that may come in either order, and so may those of one beam that 64 bits do not tell apart (a score of -1e30, say).
+    Where a beam's logits hold a NaN or +inf, or nothing above -inf, its continuations count as -inf."""
     return _lib.native().beam_select(logits, scores, int(width))

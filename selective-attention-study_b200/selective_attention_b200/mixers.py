@@ -114,7 +114,9 @@ class SelectiveAttentionSlot:
 
     def attend_pages(self, q, k, v, cache: dict, tables: dict, step: dict):
         """The new tokens of a step (``paged.append_tokens``), (total, H, D), row after row: prompts, chunks of them and single
-        tokens of many requests at once.  (total, H, D) outputs in v's dtype; the pages and histories move on."""
+        tokens of many requests at once.  (total, H, D) outputs in v's dtype; the pages and histories move on.  A paged cache is
+        bf16: fp16 and fp32 are rounded to it, and outputs have its precision in whatever dtype they come (``begin_cache`` keeps
+        fp16 and fp32)."""
         if cache["selected"].shape[1] != self.groups:
             raise ValueError(f"the cache has {cache['selected'].shape[1]} histories a row, the layer {self.groups} selectors")
         y = paged.paged_attention(cache, tables, step, q, k, v, exempt=self.exempt)

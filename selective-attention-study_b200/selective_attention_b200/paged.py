@@ -76,7 +76,8 @@ def append_tokens(tables: dict, counts: torch.Tensor, total: int, max_length: in
 def paged_attention(cache: dict, tables: dict, step: dict, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, exempt: int = 1) -> torch.Tensor:
     """Selective Attention of the step's tokens: q, k, v (total, H, D), any token and head strides.  Stores k and v in the pages, returns
     (total, H, D) bf16 -- row r's tokens get what ``selective_attention`` over all tokens of the row gives its last ones -- and
-    moves ``cache["selected"]`` on.  Tokens without a slot get zeros.
+    moves ``cache["selected"]`` on.  Tokens without a slot get zeros.  The cache is bf16 and so are its products: q, k, v in fp16 or
+    fp32 are rounded to it first (2^-8, where a dense cache keeps their type).
 
     One call per layer and step; calls of one step on one stream share its plan.  Nothing behind a row's last token is read
     into a result or written."""
