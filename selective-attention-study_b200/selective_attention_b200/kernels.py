@@ -89,7 +89,7 @@ def supported(q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | 
 def _check_exempt(exempt: int) -> int:
     if int(exempt) != exempt or exempt < 1:
         raise ValueError(f"exempt must be an integer >= 1 (position 0, <BOS>, is always exempt); got {exempt}")
-    return int(exempt)
+    return min(int(exempt), 2 ** 31 - 1)          # positions are 32-bit numbers: beyond them everything is exempt
 
 
 def _check_blocks(*blocks) -> None:

@@ -301,6 +301,18 @@ def test_rows_that_are_not_served():
     s.pools()
 
 
+@pytest.mark.parametrize("exempt", [2 ** 31, 2 ** 32 + 1])
+def test_a_layer_in_which_nothing_is_selected(exempt):
+    """More exempt positions than 32 bits count: plain causal attention, in a prompt, a chunk and single tokens, paged and dense."""
+    s = Served(2, 4, 64, 16, 20, 40, exempt=exempt, scale=0.5)
+    for counts in ([200, 30], [1, 1], [3, 60], [5, 1]):
+        s.step(counts)
+    assert (s.cache["selected"][0, :, :209] == 0).all()
+    q, k, v = (x.transpose(0, 1)[None].cuda() for x in s.tokens(150))
+    y = kernels.selective_attention_forward(q, k, v, exempt=exempt)[0]
+    assert torch.equal(y, kernels.selective_attention_forward(q, k, v, exempt=150)[0])
+
+
 def test_outputs_equal_the_dense_cache():
     """The same numbers through the dense cache: rows of one length, a prompt, a chunk and single tokens."""
     gen = torch.Generator().manual_seed(5)

@@ -7,7 +7,7 @@ import torch
 
 import paged_oracle
 import selective_oracle as oracle
-from selective_attention_b200 import _lib, beams, mixers, paged
+from selective_attention_b200 import _lib, beams, kernels, mixers, paged
 
 
 def _cpu_tables(rows=3, num_pages=8, page=16, max_pages=4, heads=2):
@@ -131,6 +131,14 @@ def test_attention_takes_rows_from_the_plan_alone():
         setattr(p, name, None)
         assert lib.sa_paged_run(ctypes.byref(p)) == 1
         setattr(p, name, 4096)
+
+
+@pytest.mark.parametrize("exempt", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 10 ** 30])
+def test_exemptions_beyond_32_bits_exempt_everything(exempt):
+    slot = mixers.SelectiveAttentionSlot(2, 64, exempt=exempt)
+    assert ctypes.c_int32(slot.exempt).value == slot.exempt == 2 ** 31 - 1
+    q = torch.randn(1, 2, 9, 16)
+    assert kernels.selective_logits(q, q, exempt)[1].abs().max() == 0
 
 
 def test_bad_selections_are_refused_before_any_launch():
