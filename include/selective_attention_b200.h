@@ -440,6 +440,102 @@ typedef struct sa_beam {
 size_t sa_beam_workspace_bytes(int dtype, int groups, int beams, int vocab, int width);
 int sa_beam_select(const sa_beam* p);
 
+/* ---- what a decoder has around its attention ----------------------------------------------------------------------------------
+ * The reference calls library operators here (src/selective_attention/model.py:31-47,325-328,365-366,402-418).
+ *
+ * Softmax cross entropy over a vocabulary, from hidden states and the output table; the logits x W^T are never kept.
+ *   x        (tokens, width) at a token stride, weight (vocab, width) at a row stride, both contiguous along the width
+ *   product  type of the products' operands: x and weight are rounded to it first (SA_F32: three bf16 parts, 24 bits)
+ *   targets  int64; ignore_index counts for nothing, and what stands in its row of x does not matter; any other target outside the vocabulary makes
+ *            its loss and the gradients NaN
+ *   lse      (tokens,) fp32, log2 of the sum of exponentials: written by the forward, read by the backward; count (1,) fp32 likewise
+ *   loss     (tokens,) fp32 without a reduction (0 where the target is ignored), else one number
+ *   dloss    of loss's shape; dx, dweight contiguous, of x's and weight's type, either may be null
+ * sums are fp32; the gradient of the logits is rounded to `product` between the products (fp16: scaled by 2^14 over the
+ * largest |dloss|; SA_F32: three parts).  A gradient is the same from call to call. */
+enum sa_reduction { SA_REDUCTION_NONE = 0, SA_REDUCTION_SUM = 1, SA_REDUCTION_MEAN = 2 };
+typedef struct sa_linear_loss {
+  int32_t struct_bytes;   /* sizeof(sa_linear_loss) */
+  int32_t product, x_dtype, weight_dtype, reduction;
+  int32_t tokens, vocab, width;
+  int64_t ignore_index;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const int64_t* targets;
+  float *lse, *count, *loss;
+  const float* dloss;
+  void *dx, *dweight;
+  void* workspace;        /* sa_linear_loss_forward_bytes() or _backward_bytes(), 256-byte aligned */
+  uint64_t workspace_bytes;
+  void* stream;
+} sa_linear_loss;
+size_t sa_linear_loss_forward_bytes(const sa_linear_loss* p);
+int sa_linear_loss_forward(const sa_linear_loss* p);
+size_t sa_linear_loss_backward_bytes(const sa_linear_loss* p);
+int sa_linear_loss_backward(const sa_linear_loss* p);
+
+/* Layer norm over rows of `width` (at most 16,384) contiguous values at row strides, with fp32 statistics.
+ *   s = x + branch (branch may be null: s = x), rounded to x's type and written to `sum` with a branch;
+ *   y = (s - mean) / sqrt(var + eps) * weight + bias (either may be null), in y_dtype, contiguous
+ *   stats    (rows, 2) fp32, mean and 1 / sqrt(var + eps): written by the forward (may be null there), read by the backward
+ * Backward: x is s, at x_stride.  dy and (may be null) dsum, the gradient that s has from elsewhere, at row strides; dx of x's type and
+ * dbranch of branch_dtype (may be null) contiguous; dweight, dbias (may be null) of weight_dtype.
+ *   workspace  sa_norm_backward_bytes(), 16-byte aligned; parameters' sums over rows are taken in an order that the sizes alone decide */
+typedef struct sa_norm {
+  int32_t struct_bytes;   /* sizeof(sa_norm) */
+  int32_t x_dtype, branch_dtype, y_dtype, weight_dtype;
+  int32_t width;
+  int64_t rows;
+  float eps;
+  int32_t reserved;       /* 0 */
+  const void* x;
+  int64_t x_stride;
+  const void* branch;
+  int64_t branch_stride;
+  const void *weight, *bias;
+  void *sum, *y;
+  float* stats;
+  const void* dy;
+  int64_t dy_stride;
+  const void* dsum;
+  int64_t dsum_stride;
+  void *dx, *dbranch, *dweight, *dbias;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} sa_norm;
+int sa_norm_forward(const sa_norm* p);
+size_t sa_norm_backward_bytes(const sa_norm* p);
+int sa_norm_backward(const sa_norm* p);
+
+/* Rows of a table, scaled: y[n] = scale * weight[idx[n]], and the gradient of the table, dweight[v] = scale * sum of dy[n] over the n with
+ * idx[n] = v, in fp32 and in an order that idx alone decides; rows that no token names are zeros.
+ *   idx      int64; one outside the table gives a row of NaN and has no part in the gradient
+ *   weight   (vocab, width) at a row stride; y (tokens, width) contiguous; dy at a row stride; dweight contiguous, of weight's type
+ *   workspace (backward)  sa_embedding_backward_bytes(), 16-byte aligned */
+typedef struct sa_embedding {
+  int32_t struct_bytes;   /* sizeof(sa_embedding) */
+  int32_t weight_dtype, y_dtype;
+  int32_t tokens, vocab, width;
+  float scale;
+  int32_t reserved;       /* 0 */
+  const int64_t* idx;
+  const void* weight;
+  int64_t weight_stride;
+  void* y;
+  const void* dy;
+  int64_t dy_stride;
+  void* dweight;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} sa_embedding;
+int sa_embedding_forward(const sa_embedding* p);
+size_t sa_embedding_backward_bytes(const sa_embedding* p);
+int sa_embedding_backward(const sa_embedding* p);
+
 /* Per-kernel device timing for benchmarks.  sa_profile_enable(id) makes every later launch of that
  * kernel record a CUDA event pair on its stream (id 0 disables); sa_profile_collect waits for the
  * recorded pairs, writes their durations in milliseconds (launch order) to ms_host, forgets them and

@@ -1,0 +1,296 @@
+// Rows of a table, scaled, and the table's gradient by sorted tokens.
+//
+// Forward: a copy.  Backward, for vocab rows and N tokens, three launches:
+//   order   sorts the tokens by their row, tokens of a row in order.  A CTA owns a range of rows and reads all N indices: its 32
+//           warps take a run of tokens each, count theirs by row, and after a prefix sum over the warps every warp writes its own
+//           tokens' places without another barrier.  148 CTAs read N indices each out of L2, which costs less than the launches of
+//           a radix sort.
+//   sum     pieces of 32 sorted tokens: their gradients are summed row by row in that order; a row inside one piece is finished,
+//           the parts of rows that cross pieces are kept.  Rows that no token names are written as zeros beside it.
+//   join    sums the parts of each row that crossed pieces.
+// So a word that is every tenth token is summed by as many CTAs as it needs, and nothing depends on the order of threads.
+#include "sa_layers.cuh"
+
+#include <algorithm>
+
+namespace sa {
+namespace embed {
+namespace {
+
+constexpr int kPiece = 32;                 // sorted tokens that are summed in a row
+constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32;
+constexpr int kMostRows = 1600;            // of the table, a CTA of `order`: 32 counters each in shared memory
+constexpr int kThreads = 256, kJoinThreads = 512;
+constexpr int kZeroRows = 16;              // rows of the table that a CTA looks at for the ones without tokens
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const sa_embedding p, int chunks) {
+  tc::after_previous_kernel();
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (id >= (int64_t)p.tokens * chunks) return;
+  const int n = (int)(id / chunks), t = (int)(id - (int64_t)n * chunks);
+  const int64_t v = p.idx[n];
+  const bool inside = v >= 0 && v < p.vocab;
+  // one chunk a thread: with VEC eight neighbours, otherwise values `chunks` apart
+  float x[1][8];
+  if (VEC) {
+    if (inside) load_row<1, 1, true>(x, p.weight, p.weight_dtype, v * p.weight_stride + t * 8, 8, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[0][i] = inside ? x[0][i] * p.scale : NAN;
+    store_row<1, 1, true>(x, p.y, p.y_dtype, (int64_t)n * p.width + t * 8, 8, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int col = i * chunks + t;
+      if (col >= p.width) continue;
+      float one[1][8];
+      if (inside) load_row<1, 1, false>(one, p.weight, p.weight_dtype, v * p.weight_stride + col, 1, 0);
+      one[0][0] = inside ? one[0][0] * p.scale : NAN;
+      store_row<1, 1, false>(one, p.y, p.y_dtype, (int64_t)n * p.width + col, 1, 0);
+    }
+  }
+}
+
+// sorted: (token, row) by row; starts: where each row's tokens begin, and the number of all behind them.
+__global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx, int tokens, int vocab, int rows, int2* sorted, int* starts) {
+  tc::after_previous_kernel();
+  extern __shared__ int counts[];                                  // [rows][warps]
+  __shared__ int before_s[kOrderWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lo = blockIdx.x * rows, hi = min(vocab, lo + rows), mine = hi - lo;
+  for (int i = threadIdx.x; i < mine * kOrderWarps; i += kOrderThreads) counts[i] = 0;
+  __syncthreads();
+  const int run = ((tokens + kOrderWarps - 1) / kOrderWarps + 31) / 32 * 32;
+  const int from = min(tokens, warp * run), to = min(tokens, from + run);
+  int before = 0;                                                  // tokens of earlier rows
+#pragma unroll 8
+  for (int n = from + lane; n < to; n += 32) {
+    const int64_t v = idx[n];
+    if (v >= 0 && v < lo) ++before;
+    if (v >= lo && v < hi) atomicAdd(&counts[(int)(v - lo) * kOrderWarps + warp], 1);
+  }
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+  if (lane == 0) before_s[warp] = before;
+  __syncthreads();
+  before = 0;
+  for (int i = 0; i < kOrderWarps; ++i) before += before_s[i];
+  // Places: rows in order, in each the warps in order.  A warp scans a row's 32 counters; rows' totals are scanned by the CTA, as many
+  // rows at a time as it has warps.
+  __shared__ int totals[kOrderWarps];
+  for (int r0 = 0; r0 < mine; r0 += kOrderWarps) {
+    const int r = r0 + warp;
+    const int own = r < mine ? counts[r * kOrderWarps + lane] : 0;
+    int upto = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (lane == 31) totals[warp] = upto;
+    __syncthreads();
+    int all = totals[lane], earlier = lane < warp ? all : 0;
+    for (int o = 16; o > 0; o >>= 1) {
+      earlier += __shfl_xor_sync(~0u, earlier, o);
+      all += __shfl_xor_sync(~0u, all, o);
+    }
+    if (r < mine) {
+      counts[r * kOrderWarps + lane] = before + earlier + upto - own;
+      if (lane == 0) starts[lo + r] = before + earlier;
+    }
+    before += all;
+    __syncthreads();
+  }
+  if (hi == vocab && threadIdx.x == 0) starts[vocab] = before;
+  __syncthreads();
+  for (int n0 = from; n0 < to; n0 += 32) {
+    const int n = n0 + lane;
+    const int64_t v = n < to ? idx[n] : -1;
+    const int r = v >= lo && v < hi ? (int)(v - lo) : -1;
+    if (__ballot_sync(~0u, r >= 0) == 0u) continue;
+    const unsigned int same = __match_any_sync(~0u, r);
+    if (r >= 0) {
+      const int at = counts[r * kOrderWarps + warp] + __popc(same & ((1u << lane) - 1u));
+      sorted[at] = make_int2(n, (int)v);
+    }
+    __syncwarp();
+    if (r >= 0 && lane == __ffs(same) - 1) counts[r * kOrderWarps + warp] += __popc(same);
+    __syncwarp();
+  }
+}
+
+struct Sum {
+  const int2* sorted;
+  const int* starts;
+  const void* dy;
+  int dtype;                               // of dy
+  int64_t dy_stride;
+  void* dweight;
+  int weight_dtype;
+  float scale;
+  int vocab, width, chunks, groups;        // chunks of 8 values in a row; rows that a CTA works on side by side
+  float* parts;                            // [pieces][2][width]: of a row that began before the piece, of one that goes on behind it
+  int pieces;
+};
+
+// A thread's eight columns of a row: neighbours, or `chunks` apart.
+template <bool VEC> __device__ __forceinline__ int column(const Sum& p, int t, int i) { return VEC ? t * 8 + i : i * p.chunks + t; }
+
+template <bool VEC>
+__device__ __forceinline__ void read_eight(const Sum& p, const void* base, int dtype, int64_t at, int t, float (&x)[8]) {
+  if (VEC) {
+    float v[1][8];
+    load_row<1, 1, true>(v, base, dtype, at + t * 8, 8, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[0][i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int col = column<VEC>(p, t, i);
+      x[i] = 0.f;
+      if (col < p.width) {
+        if (dtype == SA_F32) x[i] = static_cast<const float*>(base)[at + col];
+        else if (dtype == SA_BF16) x[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at + col]);
+        else x[i] = __half2float(static_cast<const __half*>(base)[at + col]);
+      }
+    }
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void write_eight(const Sum& p, void* base, int dtype, int64_t at, int t, const float (&x)[8]) {
+  if (VEC) {
+    float v[1][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[0][i] = x[i];
+    store_row<1, 1, true>(v, base, dtype, at + t * 8, 8, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int col = column<VEC>(p, t, i);
+      if (col >= p.width) continue;
+      if (dtype == SA_F32) static_cast<float*>(base)[at + col] = x[i];
+      else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(base)[at + col] = __float2bfloat16_rn(x[i]);
+      else static_cast<__half*>(base)[at + col] = __float2half_rn(x[i]);
+    }
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void finish_row(const Sum& p, int row, int t, const float (&x)[8]) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x[i] * p.scale;
+  write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)row * p.width, t, y);
+}
+
+// blockIdx.y: columns, kThreads chunks at a time.  The first CTAs take pieces, the others rows without tokens.
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_blocks) {
+  tc::after_previous_kernel();
+  const int across = min(p.chunks, kThreads), group = threadIdx.x / across, t = blockIdx.y * kThreads + threadIdx.x - group * across;
+  if (group >= p.groups || t >= p.chunks) return;
+  if ((int)blockIdx.x >= piece_blocks) {
+    const int v0 = ((int)blockIdx.x - piece_blocks) * kZeroRows, v1 = min(p.vocab, v0 + kZeroRows);
+    const float none[8] = {};
+    for (int v = v0 + group; v < v1; v += p.groups)
+      if (p.starts[v] == p.starts[v + 1]) write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)v * p.width, t, none);
+    return;
+  }
+  const int piece = blockIdx.x * p.groups + group, all = p.starts[p.vocab];
+  const int from = piece * kPiece, to = min(all, from + kPiece);
+  if (from >= to) return;
+  float sum[8] = {};
+  constexpr int kAhead = 4;                                        // rows of dy in flight
+  for (int i0 = from; i0 < to; i0 += kAhead) {
+    int2 at[kAhead];
+    float x[kAhead][8];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) at[k] = i0 + k < to ? p.sorted[i0 + k] : make_int2(0, -1);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (at[k].y >= 0) read_eight<VEC>(p, p.dy, p.dtype, at[k].x * p.dy_stride, t, x[k]);
+    const int next = i0 + kAhead < to ? p.sorted[i0 + kAhead].y : -1;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (at[k].y < 0) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += x[k][i];
+      if ((k + 1 < kAhead ? at[k + 1 < kAhead ? k + 1 : k].y : next) == at[k].y) continue;
+      const int begin = p.starts[at[k].y], end = p.starts[at[k].y + 1];
+      if (begin >= from && end <= from + kPiece) finish_row<VEC>(p, at[k].y, t, sum);
+      else write_eight<VEC>(p, p.parts, SA_F32, ((int64_t)piece * 2 + (begin >= from ? 1 : 0)) * p.width, t, sum);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+    }
+  }
+}
+
+// Rows that cross pieces, by the piece in which they begin.  The CTA's groups take runs of the parts, and the first joins them.
+template <bool VEC>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
+  tc::after_previous_kernel();
+  __shared__ float by_group[kJoinThreads][9];
+  const int across = min(p.chunks, kJoinThreads), group = threadIdx.x / across, t = blockIdx.y * kJoinThreads + threadIdx.x - group * across;
+  const int groups = kJoinThreads / across;
+  const int all = p.starts[p.vocab], from = blockIdx.x * kPiece, to = from + kPiece;
+  if (to >= all) return;                                           // nothing behind this piece
+  const int row = p.sorted[to - 1].y;
+  if (p.sorted[to].y != row || p.starts[row] < from) return;       // its last row ends here, or began before
+  const int last = (p.starts[row + 1] - 1) / kPiece, parts = last - (int)blockIdx.x + 1;
+  const int per = (parts + groups - 1) / groups, k0 = min(parts, group * per), k1 = min(parts, k0 + per);
+  float sum[8] = {};
+  if (group < groups && t < p.chunks) {
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+      float x[8];
+      read_eight<VEC>(p, p.parts, SA_F32, ((int64_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * p.width, t, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += x[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) by_group[threadIdx.x][i] = sum[i];
+  __syncthreads();
+  if (group != 0 || t >= p.chunks) return;
+  for (int g = 1; g < groups; ++g)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += by_group[g * across + threadIdx.x][i];
+  finish_row<VEC>(p, row, t, sum);
+}
+
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int pieces_of(const sa_embedding& p) { return (p.tokens + kPiece - 1) / kPiece; }
+int order_rows(const sa_embedding& p) { return std::min((p.vocab + kSms - 1) / kSms, kMostRows); }
+
+}  // namespace
+
+size_t backward_bytes(const sa_embedding& p) {
+  return (size_t)(up((int64_t)p.tokens * 8, 256) + up(((int64_t)p.vocab + 1) * 4, 256) + (int64_t)pieces_of(p) * 2 * p.width * 4);
+}
+
+int forward(const sa_embedding& p, cudaStream_t s) {
+  const int chunks = (p.width + 7) / 8;
+  const dim3 grid((unsigned)(((int64_t)p.tokens * chunks + kThreads - 1) / kThreads));
+  const bool vec = p.width % 8 == 0 && eights(p.weight, p.weight_dtype, p.weight_stride, p.vocab) && eights(p.y, p.y_dtype, p.width, p.tokens);
+  return vec ? launch_after(forward_kernel<true>, grid, kThreads, 0, s, p, chunks) : launch_after(forward_kernel<false>, grid, kThreads, 0, s, p, chunks);
+}
+
+int backward(const sa_embedding& p, cudaStream_t s) {
+  char* room = static_cast<char*>(p.workspace);
+  int2* sorted = reinterpret_cast<int2*>(room);
+  int* starts = reinterpret_cast<int*>(room + up((int64_t)p.tokens * 8, 256));
+  float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(starts) + up(((int64_t)p.vocab + 1) * 4, 256));
+  const int rows = order_rows(p);
+  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * kOrderWarps * 4, s, p.idx, p.tokens, p.vocab, rows,
+                        sorted, starts);
+  if (st != SA_OK) return st;
+  Sum a{sorted, starts, p.dy, p.y_dtype, p.dy_stride, p.dweight, p.weight_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p)};
+  a.groups = a.chunks < kThreads ? kThreads / a.chunks : 1;
+  const bool vec = p.width % 8 == 0 && eights(p.dy, p.y_dtype, p.dy_stride, p.tokens) && eights(p.dweight, p.weight_dtype, p.width, p.vocab);
+  const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;
+  const dim3 grid(piece_blocks + (p.vocab + kZeroRows - 1) / kZeroRows, (a.chunks + kThreads - 1) / kThreads);
+  st = vec ? launch_after(sum_kernel<true>, grid, kThreads, 0, s, a, piece_blocks) : launch_after(sum_kernel<false>, grid, kThreads, 0, s, a, piece_blocks);
+  if (st != SA_OK || a.pieces < 2) return st;
+  const dim3 join(a.pieces - 1, (a.chunks + kJoinThreads - 1) / kJoinThreads);
+  return vec ? launch_after(join_kernel<true>, join, kJoinThreads, 0, s, a) : launch_after(join_kernel<false>, join, kJoinThreads, 0, s, a);
+}
+
+}  // namespace embed
+}  // namespace sa

@@ -1,0 +1,527 @@
+// Matrix products of the loss over a vocabulary (sa_loss.cu): D = A B^T with 16-bit operands and fp32 sums, a persistent kernel
+// with three epilogues.  A CTA, or the two CTAs of a cluster on one tile (CTAS = 2), own 128 rows each of a tile of up to
+// 128 * CTAS columns; TMA fills a ring of stages 64 deep, one thread issues the MMAs, and two accumulators in tensor memory let
+// the epilogue of a tile run under the products of the next.
+//
+// Either operand may stand with the contraction contiguous ("K-major": rows of x or W) or with its own index contiguous
+// ("MN-major": W, x and the probabilities as the gradients' products read them), so nothing is transposed in memory.
+// fp32 operands come as three bf16 parts of 8 bits each, x = hi + mid + lo, and a product is the six products of parts that reach
+// 2^-16 of it or more, smallest first: six times the work of a bf16 product.
+#pragma once
+
+#include "sa_tc_ptx.cuh"
+
+namespace sa {
+namespace product {
+
+using namespace tc;
+
+constexpr int kRows = 128;                 // of a CTA
+constexpr int kDepth = 64;                 // of a stage: 128 bytes of a 16-bit operand
+constexpr int kOperand = kRows * kDepth * 2;
+constexpr int kStages = 6;
+constexpr int kThreads = 384;              // warp 0 loads, warp 1 issues, warp 2 has the tensor memory, warps 4 to 11 read it
+constexpr int kEpilogueWarps = 8;
+constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
+constexpr int kTerms = 6;                  // of an fp32 product
+
+// The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  `split`: the walks of all
+// tiles, `ticks` each, are dealt out evenly, so a tile may be shared by neighbouring clusters, each with a sum of its own (a slab).
+// Launches with the same tiles and ticks share their tiles alike, whatever their contraction's length.
+struct Walk {
+  int m, n;                                // rows and columns of the result
+  int bn;                                  // columns of a tile, a multiple of 32
+  int m_tiles, n_tiles;
+  int depth_blocks, blocks;                // stages of one term, of all terms
+  int ticks;
+  int clusters;
+  int split;
+  int segment;                             // stages that are summed in tensor memory at a time
+  int group;                               // row tiles that are walked side by side
+  __host__ __device__ int64_t total() const { return (int64_t)m_tiles * n_tiles * ticks; }
+  __host__ __device__ int64_t begin_of(int c) const { return total() * c / clusters; }
+  __host__ __device__ int cluster_at(int64_t tick) const {        // whose share it is, with `split`
+    int c = (int)(tick * clusters / total());
+    while (c + 1 < clusters && begin_of(c + 1) <= tick) ++c;
+    while (c > 0 && begin_of(c) > tick) --c;
+    return c;
+  }
+  // Slabs of a tile: from the cluster of its first tick to that of its last.
+  __host__ __device__ int slabs_of(int64_t tile) const {
+    return split ? cluster_at((tile + 1) * ticks - 1) - cluster_at(tile * ticks) + 1 : 1;
+  }
+  int most_slabs() const { return split ? (int)((ticks - 1) / (total() / clusters)) + 2 : 1; }
+  __host__ __device__ void place(int tile, int* tm, int* tn) const {
+    const int per = group * n_tiles, g = tile / per, r = tile - g * per;
+    const int rows = m_tiles - g * group < group ? m_tiles - g * group : group;
+    *tn = r / rows;
+    *tm = g * group + (r - *tn * rows);
+  }
+  __host__ __device__ int columns(int tn) const {                 // of a tile, in 32s
+    const int left = (n - tn * bn + 31) / 32 * 32;
+    return left < bn ? left : bn;
+  }
+};
+
+// A cluster's walk, the same in every role of its CTAs: units of at most `segment` stages.
+struct Units {
+  int64_t pos, end;                        // split: ticks
+  int tile, k, share0, share1;             // the tile at hand, and the stages of it that are this cluster's
+  int tm, tn, k0, k1, slab;
+  bool first;                              // of this cluster's sums of the tile
+  __host__ __device__ void begin(const Walk& w, int c) {
+    pos = w.split ? w.begin_of(c) : 0;
+    end = w.split ? w.begin_of(c + 1) : 0;
+    tile = c - w.clusters;
+    k = share1 = 0;
+  }
+  __host__ __device__ bool next(const Walk& w, int c) {
+    while (k >= share1) {
+      slab = 0;
+      share0 = 0;
+      share1 = w.blocks;
+      if (w.split) {
+        if (pos >= end) return false;
+        tile = (int)(pos / w.ticks);
+        const int64_t from = (int64_t)tile * w.ticks, to = min(from + w.ticks, end);
+        share0 = (int)((pos - from) * w.blocks / w.ticks);
+        share1 = (int)((to - from) * w.blocks / w.ticks);
+        pos = to;
+        slab = c - w.cluster_at(from);
+      } else {
+        tile += w.clusters;
+        if (tile >= w.m_tiles * w.n_tiles) return false;
+      }
+      w.place(tile, &tm, &tn);
+      k = share0;
+    }
+    first = k == share0;
+    k0 = k;
+    k1 = k = min(share1, k + w.segment);
+    return true;
+  }
+};
+
+// Where an operand's tiles start: offsets of its own index and of the contraction, in elements.
+struct Origin {
+  int own, depth;
+};
+
+enum Kind { kStats, kProbabilities, kResult };
+
+struct Epilogue {
+  // kStats: of every row and half tile, the maximum (times log2 e) and the sum of exponentials above it; the targets' logits
+  float2* stats;                           // [2 * n_tiles][m]
+  float* at_target;                        // [m], times log2 e
+  const int64_t* targets;
+  int column0;                             // of the vocabulary, that the launch's first column is
+  unsigned int* zeroed;                    // kStats: a counter to be cleared for the kernel behind
+  // kProbabilities: (exp2(z log2 e - lse) - [target]) * factor, in `parts` 16-bit parts
+  const float* lse;
+  const float* factor;
+  uint16_t* p;
+  int64_t p_pitch, p_part;                 // elements of a row, of a part
+  int parts;
+  int half;                                // fp16, not bf16
+  // kResult
+  void* out;                               // fp32 slabs, or the result
+  int dtype;
+  int64_t out_pitch, slab_stride;
+  int accumulate;                          // onto what stands there already
+  const float* scale;                      // of the result, may be null
+};
+
+// ---- PTX of CTA pairs ---------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t address_in(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+        : "memory");
+}
+// Arrives on the barrier at this offset in every CTA of the tile once the MMAs issued so far are complete.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    mma_commit(bar);
+}
+template <int CTAS>
+__device__ __forceinline__ void tensor_memory_alloc(uint32_t* dst, uint32_t cols) {
+  if constexpr (CTAS == 2) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, cols);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void tensor_memory_free(uint32_t addr, uint32_t cols) {
+  if constexpr (CTAS == 2) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  } else {
+    tmem_dealloc(addr, cols);
+  }
+}
+// 32 bytes a thread: a whole sector of memory.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// ---- epilogues: 32 columns of a row in registers ----------------------------------------------------------------------------------
+
+// Running maximum and sum, in log2 units.
+struct RowStats {
+  float top = -INFINITY, sum = 0.f;
+  __device__ __forceinline__ void add(const uint32_t (&r)[32], int valid) {
+    float z[32], best = top;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      z[i] = __uint_as_float(r[i]) * kLog2e;
+      if (i >= valid) z[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) best = fmaxf(best, z[i]);
+    const float from = best == -INFINITY ? 0.f : best;      // nothing above -inf yet: exp2(-inf - 0) is what is meant
+    sum *= ex2(top - from);
+    top = best;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) part[i & 3] += ex2(z[i] - from);
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+};
+
+__device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
+  float v = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v = j == i ? __uint_as_float(r[j]) : v;
+  return v;
+}
+
+// (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
+__device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int64_t at, float lse, float factor, int target) {
+  float p[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    p[i] = ex2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse));
+    p[i] = factor == 0.f ? 0.f : (i == target ? p[i] - 1.f : p[i]) * factor;   // a token that does not count: exactly nothing
+  }
+  for (int part = 0; part < e.parts; ++part) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = e.half ? pack_half(p[2 * i], p[2 * i + 1]) : pack_bf16(p[2 * i], p[2 * i + 1]);
+    uint16_t* dst = e.p + part * e.p_part + at;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
+      store32(dst + 16 * h, v);
+    }
+    if (part + 1 < e.parts) {                                                // what is left for the next part: exact
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[2 * i] -= __uint_as_float(w[i] << 16);
+        p[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+// 32 columns of a row of the result, `valid` of them inside.
+__device__ __forceinline__ void store_result(const Epilogue& e, uint32_t (&r)[32], int64_t at, int valid, bool add, float scale) {
+  if (e.scale != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale);
+  }
+  if (e.dtype == SA_F32) {
+    float* dst = static_cast<float*>(e.out) + at;
+    const bool whole = valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+    if (whole) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        uint32_t v[8];
+        if (add) {
+          load32(dst + 8 * h, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(r[8 * h + i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = r[8 * h + i];
+        }
+        store32(dst + 8 * h, v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < valid) dst[i] = (add ? dst[i] : 0.f) + __uint_as_float(r[i]);
+    }
+    return;
+  }
+  uint16_t* dst = static_cast<uint16_t*>(e.out) + at;
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    w[i] = e.dtype == SA_F16 ? pack_half(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]))
+                             : pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  if (valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
+      store32(dst + 16 * h, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < valid) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
+// ---- the kernel ---------------------------------------------------------------------------------------------------------------
+
+template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Walk w, const Origin at_a,
+               const Origin at_b, const Epilogue e, const WaitCtx status) {
+  constexpr int kColumns = kRows * CTAS;                            // of an accumulator
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[2 * kStages + 4];
+  __shared__ uint32_t tmem_base_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CTAS == 2 ? cluster_rank() : 0u;
+  const int c = blockIdx.x / CTAS;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, read = done + 16;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * kStages; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars[2 * kStages + i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars[2 * kStages + 2 + i], kEpilogueWarps * CTAS);
+    mbar_init_fence();
+  }
+  if (warp == 2) tensor_memory_alloc<CTAS>(&tmem_base_s, 2 * kColumns);
+  tc_fence_before_sync();
+  if constexpr (CTAS == 2) cluster_barrier();
+  else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_base_s;
+  after_previous_kernel();
+  Waiter wait;
+  wait.begin(status);
+  Units u;
+  u.begin(w, c);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- loads.  Both CTAs count on the first one's barrier: its thread issues the MMAs of both.
+      const uint32_t full_there = CTAS == 2 ? address_in(full, 0) : full;
+      const uint32_t ring = smem_u32(smem);
+      int stage = 0, round = 0;
+      while (u.next(w, c)) {
+        const int a0 = at_a.own + u.tm * kColumns + (int)rank * kRows;
+        const int b0 = at_b.own + u.tn * w.bn + (int)rank * (w.columns(u.tn) / CTAS);
+        int term = u.k0 / w.depth_blocks, block = u.k0 - term * w.depth_blocks;
+        for (int k = u.k0; k < u.k1; ++k) {
+          if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1000);
+          if (rank == 0) expect_tx(full + 8 * stage, 2 * kOperand * CTAS);
+          // parts of the terms: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+          const int pa = w.blocks == w.depth_blocks ? 0 : (0x001012 >> (4 * term)) & 3;
+          const int pb = w.blocks == w.depth_blocks ? 0 : (0x010210 >> (4 * term)) & 3;
+          const uint32_t a = ring + stage * 2 * kOperand, b = a + kOperand, bar = full_there + 8 * stage;
+          const int ka = at_a.depth + block * kDepth, kb = at_b.depth + block * kDepth;
+          if constexpr (A_MN) {
+            load_3d<CTAS>(a, &map_a, bar, a0, ka, pa);
+            load_3d<CTAS>(a + kOperand / 2, &map_a, bar, a0 + 64, ka, pa);
+          } else {
+            load_3d<CTAS>(a, &map_a, bar, ka, a0, pa);
+          }
+          if constexpr (B_MN) {
+            load_3d<CTAS>(b, &map_b, bar, b0, kb, pb);
+            load_3d<CTAS>(b + kOperand / 2, &map_b, bar, b0 + 64, kb, pb);
+          } else {
+            load_3d<CTAS>(b, &map_b, bar, kb, b0, pb);
+          }
+          if (++block == w.depth_blocks) {
+            block = 0;
+            ++term;
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            ++round;
+          }
+        }
+      }
+      for (int i = 0; i < kStages; ++i) {                            // what was loaded has been read
+        if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1001);
+        if (++stage == kStages) {
+          stage = 0;
+          ++round;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      // ---- products.  The whole warp walks: an MMA issued in a divergent branch takes longer.
+      const uint32_t format = e.half ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t a_low = desc_low(smem_u32(smem), A_MN ? kOperand / 2 : 16), b_low = desc_low(smem_u32(smem) + kOperand, B_MN ? kOperand / 2 : 16);
+      constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
+      int stage = 0, round = 0, n = 0;
+      while (u.next(w, c)) {
+        const uint32_t idesc = (1u << 4) | format | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                               ((uint32_t)(w.columns(u.tn) >> 3) << 17) | ((uint32_t)(kColumns >> 4) << 24);
+        const uint32_t acc = tmem + (n & 1) * kColumns;
+        if (n >= 2) wait(read + 8 * (n & 1), ((n >> 1) - 1) & 1, 1002);
+        for (int k = u.k0; k < u.k1; ++k) {
+          wait(full + 8 * stage, round & 1, 1003);
+          __syncwarp();
+          tc_fence_after_sync();
+          const uint32_t at = (uint32_t)(stage * 2 * kOperand) >> 4;
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < kDepth / 16; ++s) mma<CTAS>(acc, a_low + at + s * kStepA, b_low + at + s * kStepB, idesc, k > u.k0 || s > 0);
+            commit<CTAS>(empty + 8 * stage);
+            if (k + 1 == u.k1) commit<CTAS>(done + 8 * (n & 1));
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            ++round;
+          }
+        }
+        ++n;
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogues: a warp reads the 32 rows that its place in the CTA allows, two warps share their columns
+    const int half = (warp - 4) >> 2;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;              // 32 lanes, in bits 16 on
+    const uint32_t read_there = CTAS == 2 ? address_in(read, 0) : read;
+    if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 128 && e.zeroed != nullptr) *e.zeroed = 0u;
+    int n = 0;
+    while (u.next(w, c)) {
+      const int row = u.tm * kColumns + (int)rank * kRows + (warp & 3) * 32 + lane;
+      const bool inside = row < w.m;
+      const int columns = w.columns(u.tn), chunks = columns >> 5;
+      const int from = half == 0 ? 0 : (chunks + 1) >> 1, to = half == 0 ? (chunks + 1) >> 1 : chunks;
+      const uint32_t acc = tmem + (n & 1) * kColumns + lanes;
+      wait(done + 8 * (n & 1), (n >> 1) & 1, 1004);
+      __syncwarp();
+      tc_fence_after_sync();
+      if constexpr (KIND == kStats) {
+        const int64_t target = inside ? e.targets[row] : -1;
+        RowStats stats;
+        for (int i = from; i < to; ++i) {
+          uint32_t r[32];
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          const int col = u.tn * w.bn + i * 32;
+          stats.add(r, w.n - col);
+          const int64_t mine = target - e.column0 - col;
+          if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = select(r, (int)mine) * kLog2e;
+        }
+        if (inside) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(stats.top, stats.sum);
+      } else if constexpr (KIND == kProbabilities) {
+        const float lse = inside ? e.lse[row] : 0.f, factor = inside ? e.factor[row] : 0.f;
+        const int64_t target = inside ? e.targets[row] : -1;
+        for (int i = from; i < to; ++i) {
+          uint32_t r[32];
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          const int col = u.tn * w.bn + i * 32;
+          const int64_t mine = target - e.column0 - col;
+          if (inside) store_probabilities(e, r, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
+        }
+      } else {
+        const bool add = !u.first || e.accumulate;
+        const float scale = e.scale != nullptr ? *e.scale : 1.f;
+        for (int i = from; i < to; ++i) {
+          uint32_t r[32];
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          const int col = u.tn * w.bn + i * 32;
+          if (inside && col < w.n) store_result(e, r, u.slab * e.slab_stride + (int64_t)row * e.out_pitch + col, w.n - col, add, scale);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTAS == 2) arrive_cluster(read_there + 8 * (n & 1));
+        else mbar_arrive(read + 8 * (n & 1));
+      }
+      ++n;
+    }
+  }
+  wait.end(status);
+  tc_fence_before_sync();
+  __syncwarp();
+  if constexpr (CTAS == 2) cluster_barrier();
+  else __syncthreads();
+  if (warp == 2) tensor_memory_free<CTAS>(tmem, 2 * kColumns);
+}
+
+}  // namespace product
+}  // namespace sa

@@ -27,7 +27,9 @@ EXPORTS = ("sa_abi_version", "sa_status_string", "sa_last_cuda_error", "sa_engin
            "sa_tile_table_bytes", "sa_forward_live_tiles", "sa_backward_live_tiles", "sa_prefill_extend_live_tiles", "sa_decode_step_live_keys",
            "sa_decode_run", "sa_prefill_scratch_bytes", "sa_prefill_rows", "sa_cache_store", "sa_page_step_words", "sa_page_append",
            "sa_paged_workspace_bytes", "sa_paged_run", "sa_page_reorder_words", "sa_page_reorder", "sa_page_move", "sa_stream_capture",
-           "sa_beam_workspace_bytes", "sa_beam_select")
+           "sa_beam_workspace_bytes", "sa_beam_select", "sa_norm_forward", "sa_norm_backward_bytes", "sa_norm_backward", "sa_embedding_forward",
+           "sa_embedding_backward_bytes", "sa_embedding_backward", "sa_linear_loss_forward_bytes", "sa_linear_loss_forward",
+           "sa_linear_loss_backward_bytes", "sa_linear_loss_backward")
 
 
 class Problem(ctypes.Structure):
@@ -71,6 +73,34 @@ class Beam(ctypes.Structure):
                [("logits", ctypes.c_void_p), ("group_stride", ctypes.c_int64), ("beam_stride", ctypes.c_int64)] + \
                [(n, ctypes.c_void_p) for n in ("scores", "out_scores", "out_rows", "out_tokens", "workspace")] + \
                [("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
+
+
+class LinearLoss(ctypes.Structure):
+    """sa_linear_loss"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "product", "x_dtype", "weight_dtype", "reduction", "tokens", "vocab", "width")] + \
+               [("ignore_index", ctypes.c_int64), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("weight_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("targets", "lse", "count", "loss", "dloss", "dx", "dweight", "workspace")] + \
+               [("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
+
+
+class Norm(ctypes.Structure):
+    """sa_norm"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "x_dtype", "branch_dtype", "y_dtype", "weight_dtype", "width")] + \
+               [("rows", ctypes.c_int64), ("eps", ctypes.c_float), ("reserved", ctypes.c_int32), ("x", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("branch", ctypes.c_void_p), ("branch_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("weight", "bias", "sum", "y", "stats", "dy")] + \
+               [("dy_stride", ctypes.c_int64), ("dsum", ctypes.c_void_p), ("dsum_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("dx", "dbranch", "dweight", "dbias", "workspace")] + \
+               [("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
+
+
+class Embedding(ctypes.Structure):
+    """sa_embedding"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_bytes", "weight_dtype", "y_dtype", "tokens", "vocab", "width")] + \
+               [("scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("idx", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("weight_stride", ctypes.c_int64), ("y", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64),
+                ("dweight", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("stream", ctypes.c_void_p)]
 
 
 class LibraryError(RuntimeError):
@@ -190,6 +220,10 @@ def load() -> ctypes.CDLL:
     lib.sa_beam_workspace_bytes.argtypes = [i32] * 5
     lib.sa_beam_select.restype = i32
     lib.sa_beam_select.argtypes = [ctypes.POINTER(Beam)]
+    for name, struct in (("sa_norm", Norm), ("sa_embedding", Embedding), ("sa_linear_loss", LinearLoss)):
+        for fn in ("_forward", "_backward", "_backward_bytes") + (("_forward_bytes",) if struct is LinearLoss else ()):
+            getattr(lib, name + fn).restype = sz if fn.endswith("bytes") else i32
+            getattr(lib, name + fn).argtypes = [ctypes.POINTER(struct)]
     lib.sa_device_status.restype = i32
     lib.sa_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint), i32]
     lib.sa_selftest_tcgen05.restype = i32
