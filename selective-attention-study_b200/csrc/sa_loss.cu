@@ -208,22 +208,24 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* stats, int slot
   }
 }
 
-// A tile of a result from its slabs, in order.
-__global__ void __launch_bounds__(256) finish_kernel(const float* slabs, int64_t slab_stride, int64_t pitch, const Walk w, int rows_of_tile,
-                                                     const float* scale, void* out, int dtype, int64_t out_pitch) {
+// Two rows of a dealt tile from its slabs, in order.
+__global__ void __launch_bounds__(256) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, void* out, int dtype,
+                                                     int64_t out_pitch) {
   after_previous_kernel();
-  const int tile = blockIdx.x;
+  const int tile = w.whole + blockIdx.x;
   int tm, tn;
   w.place(tile, &tm, &tn);
   const int n = w.slabs_of(tile), columns = min(w.bn, w.n - tn * w.bn);
   const float by = scale != nullptr ? *scale : 1.f;
-  for (int i = threadIdx.x; i < 8 * columns; i += 256) {
-    const int r = i / columns, in_tile = blockIdx.y * 8 + r, row = tm * rows_of_tile + in_tile, col = tn * w.bn + (i - r * columns);
-    if (in_tile >= rows_of_tile || row >= w.m) continue;
+  const float* base = slabs + (int64_t)blockIdx.x * w.slabs * tile_rows * w.bn;
+  for (int i = threadIdx.x; i < 2 * w.bn; i += 256) {
+    const int in_tile = blockIdx.y * 2 + i / w.bn, c = i % w.bn, row = tm * tile_rows + in_tile;
+    if (row >= w.m || c >= columns) continue;
     float v = 0.f;
-    for (int k = 0; k < n; ++k) v += slabs[k * slab_stride + (int64_t)row * pitch + col];
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) v += base[((int64_t)k * tile_rows + in_tile) * w.bn + c];
     v *= by;
-    const int64_t at = (int64_t)row * out_pitch + col;
+    const int64_t at = (int64_t)row * out_pitch + tn * w.bn + c;
     if (dtype == SA_F32) static_cast<float*>(out)[at] = v;
     else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(out)[at] = __float2half_rn(v);
@@ -261,8 +263,9 @@ struct Operand {
   int map(CUtensorMap* m, bool mn_major) const { return make_map(m, base, width, rows, parts, pitch, part, mn_major ? 64 : kRows); }
 };
 
-// The walk over an m x n result of contraction `depth`.  `shared`: tiles may be split over clusters where whole ones would leave
-// many of them idle in the last round; `ticks`: as in the launch whose slabs this one adds to (0: the first).
+// The walk over an m x n result of contraction `depth`.  `shared`: what is left over of whole rounds is dealt out where it would
+// leave clusters idle, which costs slabs; then a row's tiles stand side by side, since their left operand, dz, comes from
+// memory and is to be read once.  `ticks`: as in the launch whose slabs this one adds to (0: the first).
 Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool shared, int segment, int ticks = 0) {
   Walk w{};
   w.m = m;
@@ -273,20 +276,25 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool shared, int 
   w.depth_blocks = (int)over(depth, kDepth);
   w.blocks = w.depth_blocks * terms;
   w.ticks = ticks > 0 ? ticks : w.blocks;
-  const int64_t tiles = (int64_t)w.m_tiles * w.n_tiles, most = kSms / ctas;
-  w.clusters = (int)std::min(tiles, most);
+  w.whole = w.tiles();
+  w.slabs = 1;
+  const int most = kSms / ctas;
+  w.clusters = std::min(w.tiles(), most);
   w.segment = segment > 0 ? std::min(segment, w.blocks) : w.blocks;
-  w.group = std::min(w.m_tiles, 8);
-  if (shared) {
-    const int64_t rounds = over(tiles, most);
-    const int64_t c = std::min(most, std::max<int64_t>(1, w.total() / 8));      // at least eight stages each
-    if (tiles * 100 < 88 * rounds * most && c >= w.clusters) {
-      w.split = 1;
-      w.clusters = (int)c;
+  w.group = shared ? 1 : std::min(w.m_tiles, 8);
+  const int left = w.tiles() % most;
+  if (shared && left * 100 < 88 * most && left > 0) {
+    const int64_t stages = (int64_t)left * w.ticks;
+    const int c = (int)std::min<int64_t>(most, stages / 8);                                // at least eight stages each
+    if (c > left && (c == most || w.tiles() < most)) {
+      w.whole -= left;
+      w.clusters = c;
+      w.slabs = (int)((w.ticks - 1) / (stages / c)) + 2;
     }
   }
   return w;
 }
+int64_t slab_floats(const Walk& w, int ctas) { return (int64_t)(w.tiles() - w.whole) * w.slabs * kRows * ctas * w.bn; }
 
 template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_a, Origin at_b, const Epilogue& e, const WaitCtx& status,
@@ -321,6 +329,9 @@ int run(int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a
   return ctas == 2 ? launch<2, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, e, status, s)
                    : launch<1, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, e, status, s);
 }
+
+// CTAs of a tile: two where there are rows for both.
+int ctas_of(int rows) { return rows > kRows ? 2 : 1; }
 
 int parts_of(const Problem& p) { return p.product == SA_F32 ? 3 : 1; }
 int terms_of(const Problem& p) { return p.product == SA_F32 ? kTerms : 1; }
@@ -388,7 +399,7 @@ struct Forward {
   Forward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
-    ctas = 1;
+    ctas = ctas_of(p.tokens);
     walk = walk_of(p.tokens, p.vocab, p.width, terms_of(p), ctas, false, 0);
     stats = room.take<float2>((int64_t)2 * walk.n_tiles * p.tokens);
     sums = room.take<float2>(over(p.tokens, 32));
@@ -400,41 +411,63 @@ struct Forward {
 struct Backward {
   Room room;
   Operand x, weight, dz;
-  float *factor, *scale, *largest, *dx_slabs = nullptr, *dw_slabs = nullptr;
+  float *factor, *scale, *largest, *dx_sums = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr;
   int ctas, piece;
-  bool direct;                   // dx is written by its product
-  int64_t pitch;                 // of slabs
+  int64_t pitch;                 // of dx_sums
   Backward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
-    ctas = 1;
+    ctas = ctas_of(p.tokens);
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, true, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
     factor = room.take<float>(p.tokens);
     scale = room.take<float>(1);
     largest = room.take<float>(1);
-    // Pieces of the vocabulary, of equal size: dz of one takes 256 MB, or 4,096 columns where that is more.
-    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p);
-    const int64_t columns = std::max<int64_t>(4096, (256ll << 20) / column / 256 * 256);
-    piece = (int)std::min<int64_t>(p.vocab, up(over(p.vocab, over(p.vocab, columns)), 256));
+    piece = piece_of(p);
     dz.rows = p.tokens;
     dz.parts = parts_of(p);
     dz.pitch = up(piece, 64);
     dz.part = dz.pitch * p.tokens;
     dz.base = room.take<uint16_t>(dz.part * dz.parts);
     pitch = up(p.width, 8);
-    const Walk dx = dx_walk(p, piece);
-    direct = piece == p.vocab && !dx.split && (dx.segment == dx.blocks || p.x_dtype == SA_F32);
-    if (p.dx != nullptr && !direct) dx_slabs = room.take<float>((int64_t)dx.most_slabs() * p.tokens * pitch);
-    int64_t rows = 0;
-    for (const int n : {piece, p.vocab % piece})
-      if (p.dweight != nullptr && n > 0 && dw_walk(p, n).split) rows = std::max(rows, (int64_t)dw_walk(p, n).most_slabs() * n);
-    if (rows > 0) dw_slabs = room.take<float>(rows * pitch);
+    if (p.dx != nullptr) {
+      if (piece < p.vocab) dx_sums = room.take<float>(p.tokens * pitch);
+      dx_slabs = room.take<float>(slab_floats(dx_walk(p, piece), ctas));
+    }
+    if (p.dweight != nullptr) {
+      int64_t most = slab_floats(dw_walk(p, piece), ctas_of(piece));
+      if (p.vocab % piece != 0) most = std::max(most, slab_floats(dw_walk(p, p.vocab % piece), ctas_of(p.vocab % piece)));
+      dw_slabs = room.take<float>(most);
+    }
+  }
+  // Columns of a piece of the vocabulary: its dz takes up to 320 MB (16,384 tokens: 37 tiles of 256 columns, with four tiles across
+  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more; of the sizes down to half of that, the one that
+  // leaves the fewest clusters idle in dW.
+  static int piece_of(const Problem& p) {
+    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>(4096, (320ll << 20) / column / 256 * 256);
+    if (p.vocab <= most) return p.vocab;
+    const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
+    int64_t best = 0, at = blocks;
+    for (int64_t b = blocks; 2 * b > blocks; --b) {
+      const int64_t tiles = b * across, used = tiles * 1000 / (over(tiles, clusters) * clusters);
+      if (used > best) {
+        best = used;
+        at = b;
+      }
+    }
+    return (int)(at * 256);
   }
   Walk dx_walk(const Problem& p, int columns) const {
     const int terms = terms_of(p);
     return walk_of(p.tokens, p.width, columns, terms, ctas, true, segment_of(p), (int)over(piece, kDepth) * terms);
   }
-  Walk dw_walk(const Problem& p, int columns) const { return walk_of(columns, p.width, p.tokens, terms_of(p), ctas, true, segment_of(p)); }
+  Walk dw_walk(const Problem& p, int columns) const {
+    return walk_of(columns, p.width, p.tokens, terms_of(p), ctas_of(columns), true, segment_of(p));
+  }
 };
+
+int finish(const float* slabs, const Walk& w, int ctas, const float* scale, void* out, int dtype, int64_t pitch, cudaStream_t s) {
+  if (w.whole == w.tiles()) return SA_OK;
+  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / 2), 256, 0, s, slabs, w, kRows * ctas, scale, out, dtype, pitch);
+}
 
 }  // namespace
 
@@ -501,48 +534,35 @@ int backward(const Problem& p, cudaStream_t s) {
     if (st != SA_OK) return st;
     Operand dz = b.dz;
     dz.width = columns;
+    const bool first = v0 == 0, last = v0 + columns == p.vocab;
     if (p.dx != nullptr) {
       const Walk w = b.dx_walk(p, columns);
       Epilogue r{};
       r.half = half;
-      if (b.direct) {
-        r.out = p.dx;
-        r.dtype = p.x_dtype;
-        r.out_pitch = p.width;
-        r.scale = scale;
-      } else {
-        r.out = b.dx_slabs;
-        r.dtype = SA_F32;
-        r.out_pitch = b.pitch;
-        r.slab_stride = (int64_t)p.tokens * b.pitch;
-        r.accumulate = v0 > 0;
-      }
+      r.out = last ? p.dx : b.dx_sums;
+      r.dtype = last ? p.x_dtype : SA_F32;
+      r.out_pitch = last ? p.width : b.pitch;
+      r.addend = first ? nullptr : b.dx_sums;
+      r.addend_pitch = b.pitch;
+      r.scale = last ? scale : nullptr;
+      r.slabs = b.dx_slabs;
+      r.later = !first;
       st = run<kResult, false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
-      if (st == SA_OK && !b.direct && v0 + columns == p.vocab)
-        st = launch_after(finish_kernel, dim3(w.m_tiles * w.n_tiles, kRows * b.ctas / 8), 256, 0, s, (const float*)b.dx_slabs, r.slab_stride, b.pitch,
-                          w, kRows * b.ctas, scale, p.dx, p.x_dtype, (int64_t)p.width);
+      if (st == SA_OK && last) st = finish(b.dx_slabs, w, b.ctas, scale, p.dx, p.x_dtype, p.width, s);
       if (st != SA_OK) return st;
     }
     if (p.dweight != nullptr) {
+      const int ctas = ctas_of(columns);
       const Walk w = b.dw_walk(p, columns);
-      void* out = static_cast<char*>(p.dweight) + (size_t)v0 * p.width * bytes_of(p.weight_dtype);
       Epilogue r{};
       r.half = half;
-      if (w.split) {
-        r.out = b.dw_slabs;
-        r.dtype = SA_F32;
-        r.out_pitch = b.pitch;
-        r.slab_stride = (int64_t)columns * b.pitch;
-      } else {
-        r.out = out;
-        r.dtype = p.weight_dtype;
-        r.out_pitch = p.width;
-        r.scale = scale;
-      }
-      st = run<kResult, true, true>(b.ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
-      if (st == SA_OK && w.split)
-        st = launch_after(finish_kernel, dim3(w.m_tiles * w.n_tiles, kRows * b.ctas / 8), 256, 0, s, (const float*)b.dw_slabs, r.slab_stride, b.pitch,
-                          w, kRows * b.ctas, scale, out, p.weight_dtype, (int64_t)p.width);
+      r.out = static_cast<char*>(p.dweight) + (size_t)v0 * p.width * bytes_of(p.weight_dtype);
+      r.dtype = p.weight_dtype;
+      r.out_pitch = p.width;
+      r.scale = scale;
+      r.slabs = b.dw_slabs;
+      st = run<kResult, true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
+      if (st == SA_OK) st = finish(b.dw_slabs, w, ctas, scale, r.out, p.weight_dtype, p.width, s);
     }
   }
   return st;

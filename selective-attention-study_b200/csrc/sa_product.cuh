@@ -25,32 +25,34 @@ constexpr int kEpilogueWarps = 8;
 constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
 constexpr int kTerms = 6;                  // of an fp32 product
 
-// The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  `split`: the walks of all
-// tiles, `ticks` each, are dealt out evenly, so a tile may be shared by neighbouring clusters, each with a sum of its own (a slab).
-// Launches with the same tiles and ticks share their tiles alike, whatever their contraction's length.
+// The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  The first `whole` tiles are
+// walked by one cluster each, round by round; what is left, less than a round, is dealt out evenly, `ticks` to a tile, so that such a
+// tile is shared by neighbouring clusters, each with a sum of its own (a slab).  Launches with the same tiles and ticks share
+// their tiles alike, whatever their contraction's length.
 struct Walk {
   int m, n;                                // rows and columns of the result
   int bn;                                  // columns of a tile, a multiple of 32
-  int m_tiles, n_tiles;
+  int m_tiles, n_tiles, whole;
   int depth_blocks, blocks;                // stages of one term, of all terms
   int ticks;
   int clusters;
-  int split;
+  int slabs;                               // that a dealt tile has room for
   int segment;                             // stages that are summed in tensor memory at a time
   int group;                               // row tiles that are walked side by side
-  __host__ __device__ int64_t total() const { return (int64_t)m_tiles * n_tiles * ticks; }
-  __host__ __device__ int64_t begin_of(int c) const { return total() * c / clusters; }
-  __host__ __device__ int cluster_at(int64_t tick) const {        // whose share it is, with `split`
-    int c = (int)(tick * clusters / total());
+  __host__ __device__ int tiles() const { return m_tiles * n_tiles; }
+  __host__ __device__ int64_t dealt() const { return (int64_t)(tiles() - whole) * ticks; }
+  __host__ __device__ int64_t begin_of(int c) const { return dealt() * c / clusters; }
+  __host__ __device__ int cluster_at(int64_t tick) const {        // whose share it is
+    int c = (int)(tick * clusters / dealt());
     while (c + 1 < clusters && begin_of(c + 1) <= tick) ++c;
     while (c > 0 && begin_of(c) > tick) --c;
     return c;
   }
-  // Slabs of a tile: from the cluster of its first tick to that of its last.
-  __host__ __device__ int slabs_of(int64_t tile) const {
-    return split ? cluster_at((tile + 1) * ticks - 1) - cluster_at(tile * ticks) + 1 : 1;
+  // Slabs of a dealt tile: from the cluster of its first tick to that of its last.
+  __host__ __device__ int slabs_of(int tile) const {
+    const int64_t at = (int64_t)(tile - whole) * ticks;
+    return cluster_at(at + ticks - 1) - cluster_at(at) + 1;
   }
-  int most_slabs() const { return split ? (int)((ticks - 1) / (total() / clusters)) + 2 : 1; }
   __host__ __device__ void place(int tile, int* tm, int* tn) const {
     const int per = group * n_tiles, g = tile / per, r = tile - g * per;
     const int rows = m_tiles - g * group < group ? m_tiles - g * group : group;
@@ -65,32 +67,34 @@ struct Walk {
 
 // A cluster's walk, the same in every role of its CTAs: units of at most `segment` stages.
 struct Units {
-  int64_t pos, end;                        // split: ticks
-  int tile, k, share0, share1;             // the tile at hand, and the stages of it that are this cluster's
+  int64_t pos, end;                        // of the dealt tiles, in ticks
+  int tile, at, k, share0, share1;         // the tile at hand, the next whole one, and the stages that are this cluster's
   int tm, tn, k0, k1, slab;
   bool first;                              // of this cluster's sums of the tile
   __host__ __device__ void begin(const Walk& w, int c) {
-    pos = w.split ? w.begin_of(c) : 0;
-    end = w.split ? w.begin_of(c + 1) : 0;
-    tile = c - w.clusters;
+    const bool some = w.whole < w.tiles();
+    pos = some ? w.begin_of(c) : 0;
+    end = some ? w.begin_of(c + 1) : 0;
+    at = c;
     k = share1 = 0;
   }
   __host__ __device__ bool next(const Walk& w, int c) {
     while (k >= share1) {
-      slab = 0;
-      share0 = 0;
-      share1 = w.blocks;
-      if (w.split) {
+      if (at < w.whole) {
+        tile = at;
+        at += w.clusters;
+        slab = 0;
+        share0 = 0;
+        share1 = w.blocks;
+      } else {
         if (pos >= end) return false;
-        tile = (int)(pos / w.ticks);
-        const int64_t from = (int64_t)tile * w.ticks, to = min(from + w.ticks, end);
+        const int t = (int)(pos / w.ticks);
+        const int64_t from = (int64_t)t * w.ticks, to = min(from + w.ticks, end);
+        tile = w.whole + t;
         share0 = (int)((pos - from) * w.blocks / w.ticks);
         share1 = (int)((to - from) * w.blocks / w.ticks);
         pos = to;
         slab = c - w.cluster_at(from);
-      } else {
-        tile += w.clusters;
-        if (tile >= w.m_tiles * w.n_tiles) return false;
       }
       w.place(tile, &tm, &tn);
       k = share0;
@@ -123,12 +127,15 @@ struct Epilogue {
   int64_t p_pitch, p_part;                 // elements of a row, of a part
   int parts;
   int half;                                // fp16, not bf16
-  // kResult
-  void* out;                               // fp32 slabs, or the result
+  // kResult: of whole tiles (sums + addend) * scale; dealt tiles keep their sums in slabs of a tile each
+  void* out;
   int dtype;
-  int64_t out_pitch, slab_stride;
-  int accumulate;                          // onto what stands there already
-  const float* scale;                      // of the result, may be null
+  int64_t out_pitch;
+  const float* addend;                     // fp32, may be null
+  int64_t addend_pitch;
+  const float* scale;                      // may be null
+  float* slabs;
+  int later;                               // dealt tiles add to what their slabs hold
 };
 
 // ---- PTX of CTA pairs ---------------------------------------------------------------------------------------------------------
@@ -291,54 +298,54 @@ __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uin
   }
 }
 
-// 32 columns of a row of the result, `valid` of them inside.
-__device__ __forceinline__ void store_result(const Epilogue& e, uint32_t (&r)[32], int64_t at, int valid, bool add, float scale) {
-  if (e.scale != nullptr) {
+// 32 columns of a row in fp32, `valid` of them inside.
+__device__ __forceinline__ void add_row(const float* p, uint32_t (&r)[32], int valid) {
+  if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale);
-  }
-  if (e.dtype == SA_F32) {
-    float* dst = static_cast<float*>(e.out) + at;
-    const bool whole = valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
-    if (whole) {
+    for (int h = 0; h < 4; ++h) {
+      uint32_t v[8];
+      load32(p + 8 * h, v);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t v[8];
-        if (add) {
-          load32(dst + 8 * h, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(r[8 * h + i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = r[8 * h + i];
-        }
-        store32(dst + 8 * h, v);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < valid) dst[i] = (add ? dst[i] : 0.f) + __uint_as_float(r[i]);
+      for (int i = 0; i < 8; ++i) r[8 * h + i] = __float_as_uint(__uint_as_float(r[8 * h + i]) + __uint_as_float(v[i]));
     }
-    return;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < valid) r[i] = __float_as_uint(__uint_as_float(r[i]) + p[i]);
   }
-  uint16_t* dst = static_cast<uint16_t*>(e.out) + at;
+}
+__device__ __forceinline__ void store_row(float* p, const uint32_t (&r)[32], int valid) {
+  if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = r[8 * h + i];
+      store32(p + 8 * h, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < valid) p[i] = __uint_as_float(r[i]);
+  }
+}
+__device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&r)[32], int valid, bool half) {
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    w[i] = e.dtype == SA_F16 ? pack_half(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]))
-                             : pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-  if (valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+    w[i] = half ? pack_half(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])) : pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
-      store32(dst + 16 * h, v);
+      store32(p + 16 * h, v);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (i < valid) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      if (i < valid) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
   }
 }
 
@@ -496,14 +503,30 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (inside) store_probabilities(e, r, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
         }
       } else {
-        const bool add = !u.first || e.accumulate;
+        const bool dealt = u.tile >= w.whole;
+        const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
+        float* const slab = dealt ? e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * kColumns + in_tile) * w.bn : nullptr;
         const float scale = e.scale != nullptr ? *e.scale : 1.f;
         for (int i = from; i < to; ++i) {
           uint32_t r[32];
           tmem_ld32(acc + i * 32, r);
           tmem_ld_wait();
-          const int col = u.tn * w.bn + i * 32;
-          if (inside && col < w.n) store_result(e, r, u.slab * e.slab_stride + (int64_t)row * e.out_pitch + col, w.n - col, add, scale);
+          const int col = u.tn * w.bn + i * 32, valid = w.n - col;
+          if (!inside || valid <= 0) continue;
+          if (dealt) {
+            if (!u.first || e.later) add_row(slab + i * 32, r, 32);
+            store_row(slab + i * 32, r, 32);
+            continue;
+          }
+          const int64_t at = (int64_t)row * e.out_pitch + col;
+          if (!u.first) add_row(static_cast<const float*>(e.out) + at, r, valid);      // fp32 operands alone have more segments
+          else if (e.addend != nullptr) add_row(e.addend + (int64_t)row * e.addend_pitch + col, r, valid);
+          if (e.scale != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+          }
+          if (e.dtype == SA_F32) store_row(static_cast<float*>(e.out) + at, r, valid);
+          else store_row(static_cast<uint16_t*>(e.out) + at, r, valid, e.dtype == SA_F16);
         }
       }
       tc_fence_before_sync();
