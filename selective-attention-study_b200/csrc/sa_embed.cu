@@ -19,8 +19,8 @@ namespace {
 
 constexpr int kPiece = 32;                 // sorted tokens that are summed in a row
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32;
-constexpr int kMostRows = 1600;            // of the table, a CTA of `order`: 32 counters each in shared memory
-constexpr int kThreads = 256, kJoinThreads = 512;
+constexpr int kMostRows = 1600;            // of the table, a CTA of `order`: 32 counters and a place each in shared memory
+constexpr int kThreads = 256, kJoinThreads = 1024;
 constexpr int kZeroRows = 16;              // rows of the table that a CTA looks at for the ones without tokens
 
 template <bool VEC>
@@ -74,46 +74,72 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx
   __syncthreads();
   before = 0;
   for (int i = 0; i < kOrderWarps; ++i) before += before_s[i];
-  // Places: rows in order, in each the warps in order.  A warp scans a row's 32 counters; rows' totals are scanned by the CTA, as many
-  // rows at a time as it has warps.
-  __shared__ int totals[kOrderWarps];
-  for (int r0 = 0; r0 < mine; r0 += kOrderWarps) {
-    const int r = r0 + warp;
-    const int own = r < mine ? counts[r * kOrderWarps + lane] : 0;
+  // Places: rows in order, in each the warps in order.  A warp turns a row's 32 counters into sums of the earlier ones; then the
+  // rows' totals are added up, a run of rows a warp.
+  int* const totals = counts + rows * kOrderWarps;                 // [rows]
+  for (int r = warp; r < mine; r += kOrderWarps) {
+    const int own = counts[r * kOrderWarps + lane];
     int upto = own;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int other = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += other;
     }
-    if (lane == 31) totals[warp] = upto;
-    __syncthreads();
-    int all = totals[lane], earlier = lane < warp ? all : 0;
-    for (int o = 16; o > 0; o >>= 1) {
-      earlier += __shfl_xor_sync(~0u, earlier, o);
-      all += __shfl_xor_sync(~0u, all, o);
+    counts[r * kOrderWarps + lane] = upto - own;
+    if (lane == 31) totals[r] = upto;
+  }
+  __syncthreads();
+  const int per = (mine + kOrderWarps - 1) / kOrderWarps, r0 = min(mine, warp * per), r1 = min(mine, r0 + per);
+  int all = 0;
+  for (int r = r0 + lane; r < r1; r += 32) all += totals[r];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+  __syncthreads();                                                 // before_s has been read by all
+  if (lane == 0) before_s[warp] = all;
+  __syncthreads();
+  int upto = before;
+  for (int i = 0; i < kOrderWarps; ++i) {
+    if (i < warp) upto += before_s[i];
+    before += before_s[i];
+  }
+  for (int r = r0; r < r1; r += 32) {
+    const int own = r + lane < r1 ? totals[r + lane] : 0;
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(~0u, sum, o);
+      if (lane >= o) sum += other;
     }
-    if (r < mine) {
-      counts[r * kOrderWarps + lane] = before + earlier + upto - own;
-      if (lane == 0) starts[lo + r] = before + earlier;
+    if (r + lane < r1) {
+      totals[r + lane] = upto + sum - own;
+      starts[lo + r + lane] = upto + sum - own;
     }
-    before += all;
-    __syncthreads();
+    upto += __shfl_sync(~0u, sum, 31);
   }
   if (hi == vocab && threadIdx.x == 0) starts[vocab] = before;
   __syncthreads();
-  for (int n0 = from; n0 < to; n0 += 32) {
-    const int n = n0 + lane;
-    const int64_t v = n < to ? idx[n] : -1;
-    const int r = v >= lo && v < hi ? (int)(v - lo) : -1;
-    if (__ballot_sync(~0u, r >= 0) == 0u) continue;
-    const unsigned int same = __match_any_sync(~0u, r);
-    if (r >= 0) {
-      const int at = counts[r * kOrderWarps + warp] + __popc(same & ((1u << lane) - 1u));
-      sorted[at] = make_int2(n, (int)v);
+  constexpr int kAhead = 8;                                        // indices in flight
+  for (int n0 = from; n0 < to; n0 += 32 * kAhead) {
+    int row[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int n = n0 + 32 * k + lane;
+      const int64_t v = n < to ? idx[n] : -1;
+      row[k] = v >= lo && v < hi ? (int)(v - lo) : -1;
     }
-    __syncwarp();
-    if (r >= 0 && lane == __ffs(same) - 1) counts[r * kOrderWarps + warp] += __popc(same);
-    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = row[k];
+      if (__ballot_sync(~0u, r >= 0) == 0u) continue;
+      const unsigned int same = __match_any_sync(~0u, r);
+      if (r >= 0) {
+        const int at = totals[r] + counts[r * kOrderWarps + warp] + __popc(same & ((1u << lane) - 1u));
+        sorted[at] = make_int2(n0 + 32 * k + lane, lo + r);
+      }
+      __syncwarp();
+      if (r >= 0 && lane == __ffs(same) - 1) counts[r * kOrderWarps + warp] += __popc(same);
+      __syncwarp();
+    }
   }
 }
 
@@ -197,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
   const int from = piece * kPiece, to = min(all, from + kPiece);
   if (from >= to) return;
   float sum[8] = {};
-  constexpr int kAhead = 4;                                        // rows of dy in flight
+  constexpr int kAhead = 4;                                        // rows of dy in flight (8: fewer CTAs an SM, 39 -> 45 us)
   for (int i0 = from; i0 < to; i0 += kAhead) {
     int2 at[kAhead];
     float x[kAhead][8];
@@ -237,7 +263,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
   const int per = (parts + groups - 1) / groups, k0 = min(parts, group * per), k1 = min(parts, k0 + per);
   float sum[8] = {};
   if (group < groups && t < p.chunks) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = k0; k < k1; ++k) {
       float x[8];
       read_eight<VEC>(p, p.parts, SA_F32, ((int64_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * p.width, t, x);
@@ -278,7 +304,7 @@ int backward(const sa_embedding& p, cudaStream_t s) {
   int* starts = reinterpret_cast<int*>(room + up((int64_t)p.tokens * 8, 256));
   float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(starts) + up(((int64_t)p.vocab + 1) * 4, 256));
   const int rows = order_rows(p);
-  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * kOrderWarps * 4, s, p.idx, p.tokens, p.vocab, rows,
+  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.tokens, p.vocab, rows,
                         sorted, starts);
   if (st != SA_OK) return st;
   Sum a{sorted, starts, p.dy, p.y_dtype, p.dy_stride, p.dweight, p.weight_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p)};

@@ -27,9 +27,11 @@ __device__ __forceinline__ int column_of(int chunk, int i, int t) {
   return VEC ? (chunk * T + t) * 8 + i : (chunk * 8 + i) * T + t;
 }
 
-struct Eight {
-  float v[8];
-};
+// Whether a value lies in the row: with VEC one question for the eight.
+template <int T, bool VEC>
+__device__ __forceinline__ bool in_row(int chunk, int i, int t, int width) {
+  return column_of<T, VEC>(chunk, VEC ? 0 : i, t) < width;
+}
 
 __device__ __forceinline__ void unpack_pair(uint32_t w, bool half, float* to) {
   if (half) {
@@ -60,14 +62,22 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi, bool half) {
 }
 
 // The branch on the type is around all loads of a row, so that they are in flight together.
-template <int NV, int T, bool VEC>
+// SHARED: from shared memory, at a multiple of 16 bytes.
+template <int NV, int T, bool VEC, bool SHARED = false>
 __device__ __forceinline__ void load_row(float (&v)[NV][8], const void* base, int dtype, int64_t at, int width, int t) {
   if (dtype == SA_F32) {
     const float* p = static_cast<const float*>(base) + at;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       if (VEC) {
-        if (column_of<T, VEC>(c, 0, t) < width) load_eight(p + column_of<T, VEC>(c, 0, t), v[c]);
+        if (column_of<T, VEC>(c, 0, t) >= width) continue;
+        if (SHARED) {
+          const float4* q = reinterpret_cast<const float4*>(p + column_of<T, VEC>(c, 0, t));
+          const float4 a = q[0], b = q[1];
+          v[c][0] = a.x; v[c][1] = a.y; v[c][2] = a.z; v[c][3] = a.w; v[c][4] = b.x; v[c][5] = b.y; v[c][6] = b.z; v[c][7] = b.w;
+        } else {
+          load_eight(p + column_of<T, VEC>(c, 0, t), v[c]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)

@@ -137,29 +137,48 @@ __global__ void __launch_bounds__(1024) largest_kernel(const float* dloss, const
   }
 }
 
-// Joins the half tiles of 32 tokens: a warp takes every eighth, a lane a token.  The last CTA to end sums all tokens, in order.
-__global__ void __launch_bounds__(256) join_kernel(const float2* stats, int slots, const float* at_target, const int64_t* targets,
-                                                   int64_t ignore_index, int tokens, int vocab, int reduction, float* lse, float* loss,
-                                                   float* count, float2* sums, unsigned int* ticket) {
+// Joins the half tiles of 32 tokens: a lane has a token, the 32 warps take the half tiles in turn, eight loads in flight.  The last CTA
+// to end sums all tokens, in order.
+constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32, kJoinAhead = 8;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats, int slots, const float* at_target, const int64_t* targets,
+                                                            int64_t ignore_index, int tokens, int vocab, int reduction, float* lse, float* loss,
+                                                            float* count, float2* sums, unsigned int* ticket) {
   after_previous_kernel();
-  __shared__ float2 parts[8][32];
+  __shared__ float2 parts[kJoinWarps][32];
   __shared__ bool last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
-  auto add = [&](float2 v) {
-    const float most = fmaxf(top, v.x), from = most == -INFINITY ? 0.f : most;
-    sum = sum * ex2(top - from) + v.y * ex2(v.x - from);
+  auto add = [&](const float2* v, int n) {
+    float most = top;
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+      if (i < n) most = fmaxf(most, v[i].x);
+    const float from = most == -INFINITY ? 0.f : most;
+    sum *= ex2(top - from);
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+      if (i < n) sum += v[i].y * ex2(v[i].x - from);
     top = most;
   };
-  if (row < tokens) {
-#pragma unroll 4
-    for (int i = warp; i < slots; i += 8) add(stats[(int64_t)i * tokens + row]);
+  for (int i = warp; i < slots; i += kJoinWarps * kJoinAhead) {
+    float2 v[kJoinAhead];
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k)
+      v[k] = i + k * kJoinWarps < slots && row < tokens ? stats[(int64_t)(i + k * kJoinWarps) * tokens + row] : make_float2(-INFINITY, 0.f);
+    add(v, kJoinAhead);
   }
   parts[warp][lane] = make_float2(top, sum);
   __syncthreads();
   if (warp == 0) {
-    for (int i = 1; i < 8; ++i) add(parts[i][lane]);
+    top = -INFINITY;
+    sum = 0.f;
+    for (int i = 0; i < kJoinWarps; i += kJoinAhead) {
+      float2 v[kJoinAhead];
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) v[k] = parts[i + k][lane];
+      add(v, kJoinAhead);
+    }
     float mine = 0.f, counts = 0.f;
     if (row < tokens) {
       const float all = top + log2f(sum);
@@ -185,50 +204,55 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* stats, int slot
   }
   if (reduction == SA_REDUCTION_NONE) return;
   __syncthreads();
-  if (!last) return;
+  if (!last || warp > 0) return;
   __threadfence();
   double a = 0.0, b = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) {
+  for (int i = lane; i < (int)gridDim.x; i += 32) {
     const volatile float2* v = sums + i;
     a += (double)v->x;
     b += (double)v->y;
   }
-  __shared__ double2 all[256];
-  all[threadIdx.x] = make_double2(a, b);
-  for (int o = 128; o > 0; o >>= 1) {
-    __syncthreads();
-    if (threadIdx.x < o) {
-      all[threadIdx.x].x += all[threadIdx.x + o].x;
-      all[threadIdx.x].y += all[threadIdx.x + o].y;
-    }
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(~0u, a, o);
+    b += __shfl_xor_sync(~0u, b, o);
   }
-  if (threadIdx.x == 0) {
-    *count = (float)all[0].y;
-    *loss = (float)(reduction == SA_REDUCTION_MEAN ? all[0].x / all[0].y : all[0].x);
+  if (lane == 0) {
+    *count = (float)b;
+    *loss = (float)(reduction == SA_REDUCTION_MEAN ? a / b : a);
   }
 }
 
-// Two rows of a dealt tile from its slabs, in order.
-__global__ void __launch_bounds__(256) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, void* out, int dtype,
-                                                     int64_t out_pitch) {
+// Rows of a dealt tile from its slabs, in order: a thread has four columns of a row, four slabs in flight.
+constexpr int kFinishThreads = 256;
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, void* out,
+                                                                int dtype, int64_t out_pitch) {
   after_previous_kernel();
   const int tile = w.whole + blockIdx.x;
   int tm, tn;
   w.place(tile, &tm, &tn);
-  const int n = w.slabs_of(tile), columns = min(w.bn, w.n - tn * w.bn);
+  const int n = w.slabs_of(tile), columns = min(w.bn, w.n - tn * w.bn), across = w.bn >> 2;
+  const int in_tile = blockIdx.y * (kFinishThreads / across) + threadIdx.x / across, c = (threadIdx.x % across) * 4, row = tm * tile_rows + in_tile;
+  if (row >= w.m || c >= columns) return;
   const float by = scale != nullptr ? *scale : 1.f;
-  const float* base = slabs + (int64_t)blockIdx.x * w.slabs * tile_rows * w.bn;
-  for (int i = threadIdx.x; i < 2 * w.bn; i += 256) {
-    const int in_tile = blockIdx.y * 2 + i / w.bn, c = i % w.bn, row = tm * tile_rows + in_tile;
-    if (row >= w.m || c >= columns) continue;
-    float v = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) v += base[((int64_t)k * tile_rows + in_tile) * w.bn + c];
-    v *= by;
-    const int64_t at = (int64_t)row * out_pitch + tn * w.bn + c;
-    if (dtype == SA_F32) static_cast<float*>(out)[at] = v;
-    else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(out)[at] = __float2half_rn(v);
+  const float4* from = reinterpret_cast<const float4*>(slabs + ((int64_t)blockIdx.x * w.slabs * tile_rows + in_tile) * w.bn + c);
+  const int64_t stride = (int64_t)tile_rows * w.bn / 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const float4 x = from[k * stride];
+    v.x += x.x;
+    v.y += x.y;
+    v.z += x.z;
+    v.w += x.w;
+  }
+  const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+  const int64_t at = (int64_t)row * out_pitch + tn * w.bn + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (c + i >= columns) break;
+    if (dtype == SA_F32) static_cast<float*>(out)[at + i] = f[i];
+    else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(out)[at + i] = __float2bfloat16_rn(f[i]);
+    else static_cast<__half*>(out)[at + i] = __float2half_rn(f[i]);
   }
 }
 
@@ -466,7 +490,8 @@ struct Backward {
 
 int finish(const float* slabs, const Walk& w, int ctas, const float* scale, void* out, int dtype, int64_t pitch, cudaStream_t s) {
   if (w.whole == w.tiles()) return SA_OK;
-  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / 2), 256, 0, s, slabs, w, kRows * ctas, scale, out, dtype, pitch);
+  const int rows = kFinishThreads / (w.bn >> 2);                  // bn: 128 or 256
+  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, slabs, w, kRows * ctas, scale, out, dtype, pitch);
 }
 
 }  // namespace
@@ -490,7 +515,7 @@ int forward(const Problem& p, cudaStream_t s) {
   e.half = p.product == SA_F16;
   st = run<kStats, false, false>(f.ctas, f.x, f.weight, f.walk, Origin{0, 0}, Origin{0, 0}, e, status, s);
   if (st != SA_OK) return st;
-  return launch_after(join_kernel, dim3((unsigned)over(p.tokens, 32)), 256, 0, s, (const float2*)f.stats, 2 * f.walk.n_tiles,
+  return launch_after(join_kernel, dim3((unsigned)over(p.tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * f.walk.n_tiles,
                       (const float*)f.at_target, p.targets, p.ignore_index, p.tokens, p.vocab, p.reduction, p.lse, p.loss, p.count, f.sums, f.ticket);
 }
 

@@ -12,121 +12,144 @@ namespace sa {
 namespace norm {
 namespace {
 
-// Sums of two values over the T threads of a row: a warp, or the CTA.  `buffer` is one of two that rows take in turn, so one barrier
-// a sum is enough.
-template <int T>
-__device__ __forceinline__ float2 row_sum(float2 v, float2 (*buffer)[32], int& turn) {
+// Sums of N values over the T threads of a row: part of a warp, a warp, or the CTA.  `buffer` is one of two that rows take in turn, so
+// one barrier a sum is enough.
+template <int T, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float2 (*buffer)[32], int& turn) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(~0u, v.x, o);
-    v.y += __shfl_xor_sync(~0u, v.y, o);
-  }
+  for (int o = T < 32 ? T / 2 : 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(~0u, v[k], o);
   if constexpr (T > 32) {
     float2* b = buffer[turn];
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = make_float2(v[0], N > 1 ? v[N - 1] : 0.f);
     __syncthreads();
-    v = make_float2(0.f, 0.f);
+    float2 all = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
-      v.x += b[i].x;
-      v.y += b[i].y;
+      all.x += b[i].x;
+      all.y += b[i].y;
     }
+    v[0] = all.x;
+    if (N > 1) v[N - 1] = all.y;
   }
-  return v;
 }
 
 template <int T> constexpr int kBlock = T < 128 ? 128 : T;
 template <int T> constexpr int kRowsOf = kBlock<T> / T;
 
+// Rows of which a team has the loads in flight together: narrow ones are too short to keep memory busy by themselves.
+template <int T, int NV> constexpr int kTogether = T <= 32 && NV == 1 ? 2 : 1;
+
 template <int T, int NV, bool VEC>
 __global__ void __launch_bounds__(kBlock<T>) forward_kernel(const sa_norm p) {
   tc::after_previous_kernel();
+  constexpr int R = kTogether<T, NV>;
   __shared__ float2 buffer[2][32];
   const int t = threadIdx.x % T;
-  const int64_t row = (int64_t)blockIdx.x * kRowsOf<T> + threadIdx.x / T;
-  if (row >= p.rows) return;                                     // a whole warp, or the whole CTA
   int turn = 0;
-  float s[NV][8];
-  load_row<NV, T, VEC>(s, p.x, p.x_dtype, row * p.x_stride, p.width, t);
+  float s[R][NV][8];
+  int64_t row[R];
+  int width[R];                                                  // threads of a warp that have no row go through the sums with the others
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    row[q] = ((int64_t)blockIdx.x * R + q) * kRowsOf<T> + threadIdx.x / T;
+    width[q] = row[q] < p.rows ? p.width : 0;
+    load_row<NV, T, VEC>(s[q], p.x, p.x_dtype, row[q] * p.x_stride, width[q], t);
+  }
   if (p.branch != nullptr) {
-    float b[NV][8];
-    load_row<NV, T, VEC>(b, p.branch, p.branch_dtype, row * p.branch_stride, p.width, t);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      float b[NV][8];
+      load_row<NV, T, VEC>(b, p.branch, p.branch_dtype, row[q] * p.branch_stride, width[q], t);
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[q][c][i] = rounded_to(s[q][c][i] + b[c][i], p.x_dtype);
+      store_row<NV, T, VEC>(s[q], p.sum, p.x_dtype, row[q] * p.width, width[q], t);
+    }
+  }
+  const float over = 1.f / (float)p.width;
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    float sum[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] = rounded_to(s[c][i] + b[c][i], p.x_dtype);
-    store_row<NV, T, VEC>(s, p.sum, p.x_dtype, row * p.width, p.width, t);
-  }
-  float2 sum = make_float2(0.f, 0.f);
+      for (int i = 0; i < 8; ++i)
+        if (in_row<T, VEC>(c, i, t, width[q])) sum[0] += s[q][c][i];
+    row_sum<T>(sum, buffer, turn);
+    const float mean = sum[0] * over;
+    sum[0] = 0.f;
 #pragma unroll
-  for (int c = 0; c < NV; ++c)
+    for (int c = 0; c < NV; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (column_of<T, VEC>(c, i, t) < p.width) sum.x += s[c][i];
-  const float mean = row_sum<T>(sum, buffer, turn).x / (float)p.width;
-  sum = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[c][i] -= mean;
-      if (column_of<T, VEC>(c, i, t) < p.width) sum.x += s[c][i] * s[c][i];
+      for (int i = 0; i < 8; ++i) {
+        s[q][c][i] -= mean;
+        if (in_row<T, VEC>(c, i, t, width[q])) sum[0] += s[q][c][i] * s[q][c][i];
+      }
+    row_sum<T>(sum, buffer, turn);
+    const float r = rsqrtf(sum[0] * over + p.eps);
+    if (t == 0 && width[q] > 0 && p.stats != nullptr) {
+      p.stats[2 * row[q]] = mean;
+      p.stats[2 * row[q] + 1] = r;
     }
-  const float r = 1.f / sqrtf(row_sum<T>(sum, buffer, turn).x / (float)p.width + p.eps);
-  if (t == 0 && p.stats != nullptr) {
-    p.stats[2 * row] = mean;
-    p.stats[2 * row + 1] = r;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[q][c][i] *= r;
   }
   if (p.weight != nullptr) {
     float w[NV][8];
     load_row<NV, T, VEC>(w, p.weight, p.weight_dtype, 0, p.width, t);
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+    for (int q = 0; q < R; ++q)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] = s[c][i] * r * w[c][i];
-  } else {
+      for (int c = 0; c < NV; ++c)
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] *= r;
+        for (int i = 0; i < 8; ++i) s[q][c][i] *= w[c][i];
   }
   if (p.bias != nullptr) {
     float b[NV][8];
     load_row<NV, T, VEC>(b, p.bias, p.weight_dtype, 0, p.width, t);
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+    for (int q = 0; q < R; ++q)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] += b[c][i];
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[q][c][i] += b[c][i];
   }
-  store_row<NV, T, VEC>(s, p.y, p.y_dtype, row * p.width, p.width, t);
+#pragma unroll
+  for (int q = 0; q < R; ++q) store_row<NV, T, VEC>(s[q], p.y, p.y_dtype, row[q] * p.width, width[q], t);
 }
 
-// `sums`: (CTAs, 2, width), the parts of dw and db; null when neither is asked for.
+// ---- backward -------------------------------------------------------------------------------------------------------------------
+
+// A thread's part of the gradient: of rows, h and g = dy in and dx out, and its columns' sums for dw and db.
 template <int T, int NV, bool VEC, bool BIAS>
-__global__ void __launch_bounds__(kBlock<T>) backward_kernel(const sa_norm p, float* sums) {
-  tc::after_previous_kernel();
-  __shared__ float2 buffer[2][32];
-  const int t = threadIdx.x % T, lane_row = threadIdx.x / T;
-  int turn = 0;
+struct Gradient {
   float dw[NV][8], db[BIAS ? NV : 1][8];
-#pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      dw[c][i] = 0.f;
-      if (BIAS) db[c][i] = 0.f;
-    }
-  for (int64_t row = (int64_t)blockIdx.x * kRowsOf<T> + lane_row; row < p.rows; row += (int64_t)gridDim.x * kRowsOf<T>) {
-    float h[NV][8], g[NV][8];
-    load_row<NV, T, VEC>(h, p.x, p.x_dtype, row * p.x_stride, p.width, t);
-    load_row<NV, T, VEC>(g, p.dy, p.y_dtype, row * p.dy_stride, p.width, t);
-    const float2 stats = make_float2(p.stats[2 * row], p.stats[2 * row + 1]);
+  __device__ __forceinline__ Gradient() {
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        h[c][i] = (h[c][i] - stats.x) * stats.y;
+        dw[c][i] = 0.f;
+        if (BIAS) db[c][i] = 0.f;
+      }
+  }
+  // `width` is 0 in threads that have no row but go through the sums with the others.
+  __device__ __forceinline__ void row(const sa_norm& p, float (&h)[NV][8], float (&g)[NV][8], float2 stats, int width, int t, float2 (*buffer)[32],
+                                      int& turn) {
+    const float over = 1.f / (float)p.width;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool inside = in_row<T, VEC>(c, i, t, width);
+        h[c][i] = inside ? (h[c][i] - stats.x) * stats.y : 0.f;
+        g[c][i] = inside ? g[c][i] : 0.f;
         dw[c][i] += g[c][i] * h[c][i];
         if (BIAS) db[c][i] += g[c][i];
       }
@@ -136,82 +159,213 @@ __global__ void __launch_bounds__(kBlock<T>) backward_kernel(const sa_norm p, fl
 #pragma unroll
       for (int c = 0; c < NV; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] *= w[c][i];
+        for (int i = 0; i < 8; ++i)
+          if (in_row<T, VEC>(c, i, t, p.width)) g[c][i] *= w[c][i];
     }
-    float2 m = make_float2(0.f, 0.f);
+    float m[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (column_of<T, VEC>(c, i, t) < p.width) {
-          m.x += g[c][i];
-          m.y += g[c][i] * h[c][i];
-        }
-    m = row_sum<T>(m, buffer, turn);
-    m.x /= (float)p.width;
-    m.y /= (float)p.width;
+      for (int i = 0; i < 8; ++i) {
+        m[0] += g[c][i];
+        m[1] += g[c][i] * h[c][i];
+      }
+    row_sum<T>(m, buffer, turn);
+    const float mean_g = m[0] * over, mean_gh = m[1] * over;
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[c][i] = stats.y * (g[c][i] - m.x - h[c][i] * m.y);
+      for (int i = 0; i < 8; ++i) g[c][i] = stats.y * (g[c][i] - mean_g - h[c][i] * mean_gh);
+  }
+  // The CTA's sums into its part, its teams in their order.
+  __device__ __forceinline__ void finish(const sa_norm& p, float* sums, float* shared, int t, int team) {
+    if constexpr (kRowsOf<T> > 1) {
+      constexpr int kTeam = T * NV * 8 * (BIAS ? 2 : 1);
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (team > 0) {
+            shared[(team - 1) * kTeam + (c * 8 + i) * T + t] = dw[c][i];
+            if (BIAS) shared[(team - 1) * kTeam + ((NV + c) * 8 + i) * T + t] = db[c][i];
+          }
+      __syncthreads();
+      if (team > 0) return;
+      for (int k = 0; k < kRowsOf<T> - 1; ++k)
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dw[c][i] += shared[k * kTeam + (c * 8 + i) * T + t];
+            if (BIAS) db[c][i] += shared[k * kTeam + ((NV + c) * 8 + i) * T + t];
+          }
+    }
+    float* mine = sums + (int64_t)blockIdx.x * (BIAS ? 2 : 1) * p.width;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = column_of<T, VEC>(c, i, t);
+        if (col >= p.width) continue;
+        mine[col] = dw[c][i];
+        if (BIAS) mine[p.width + col] = db[c][i];
+      }
+  }
+};
+template <int T, int NV, bool BIAS> constexpr size_t kTeamBytes = kRowsOf<T> > 1 ? (kRowsOf<T> - 1) * T * NV * 8 * (BIAS ? 2 : 1) * 4 : 0;
+
+// Rows as they lie, by plain loads: strides and addresses that the copies below do not take, or rows too long for them.
+// `sums`: (CTAs, 1 or 2, width), the parts of dw and db; null when neither is asked for.
+template <int T, int NV, bool VEC, bool BIAS>
+__global__ void __launch_bounds__(kBlock<T>) backward_kernel(const sa_norm p, float* sums) {
+  tc::after_previous_kernel();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 buffer[2][32];
+  const int t = threadIdx.x % T, team = threadIdx.x / T;
+  int turn = 0;
+  Gradient<T, NV, VEC, BIAS> gradient;
+  const int64_t rounds = (p.rows + kRowsOf<T> - 1) / kRowsOf<T>;
+  for (int64_t i0 = blockIdx.x; i0 < rounds; i0 += gridDim.x) {
+    const int64_t row = i0 * kRowsOf<T> + team;
+    const int width = row < p.rows ? p.width : 0;
+    float h[NV][8], g[NV][8];
+    load_row<NV, T, VEC>(h, p.x, p.x_dtype, row * p.x_stride, width, t);
+    load_row<NV, T, VEC>(g, p.dy, p.y_dtype, row * p.dy_stride, width, t);
+    const float2 stats = width > 0 ? make_float2(p.stats[2 * row], p.stats[2 * row + 1]) : make_float2(0.f, 0.f);
+    gradient.row(p, h, g, stats, width, t, buffer, turn);
     if (p.dsum != nullptr) {
-      load_row<NV, T, VEC>(h, p.dsum, p.x_dtype, row * p.dsum_stride, p.width, t);
+      load_row<NV, T, VEC>(h, p.dsum, p.x_dtype, row * p.dsum_stride, width, t);
 #pragma unroll
       for (int c = 0; c < NV; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[c][i] += h[c][i];
     }
-    store_row<NV, T, VEC>(g, p.dx, p.x_dtype, row * p.width, p.width, t);
-    if (p.dbranch != nullptr) store_row<NV, T, VEC>(g, p.dbranch, p.branch_dtype, row * p.width, p.width, t);
+    store_row<NV, T, VEC>(g, p.dx, p.x_dtype, row * p.width, width, t);
+    if (p.dbranch != nullptr) store_row<NV, T, VEC>(g, p.dbranch, p.branch_dtype, row * p.width, width, t);
   }
-  if (sums == nullptr) return;
-  if constexpr (kRowsOf<T> > 1) {                                // the CTA's warps, in their order
-    __shared__ float part[kRowsOf<T> - 1][T * NV * 8 * (BIAS ? 2 : 1)];
-#pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane_row > 0) {
-          part[lane_row - 1][(c * 8 + i) * T + t] = dw[c][i];
-          if (BIAS) part[lane_row - 1][((NV + c) * 8 + i) * T + t] = db[c][i];
-        }
-    __syncthreads();
-    if (lane_row > 0) return;
-    for (int k = 0; k < kRowsOf<T> - 1; ++k)
-#pragma unroll
-      for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dw[c][i] += part[k][(c * 8 + i) * T + t];
-          if (BIAS) db[c][i] += part[k][((NV + c) * 8 + i) * T + t];
-        }
-  }
-  float* mine = sums + (int64_t)blockIdx.x * (BIAS ? 2 : 1) * p.width;
-#pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int col = column_of<T, VEC>(c, i, t);
-      if (col >= p.width) continue;
-      mine[col] = dw[c][i];
-      if (BIAS) mine[p.width + col] = db[c][i];
-    }
+  if (sums != nullptr) gradient.finish(p, sums, reinterpret_cast<float*>(smem), t, team);
 }
 
-// Columns of the parameters' gradients: 32 a CTA, whose 16 warps take the parts in turn.
+// Rows copied ahead into shared memory by bulk copies: what is in flight takes no registers, so the few CTAs that a thread's 60
+// to 100 registers allow keep memory busy.  A stage has `rows` rows of x, dy and dsum with their statistics; contiguous rows of any
+// width come in one copy a tensor (a multiple of 8 rows begins on 16 bytes), others row by row.
+constexpr int kRing = 3;
+struct Copies {
+  int rows;                                // of a stage, even and a multiple of the rows that a CTA works on at a time
+  int bytes[3];                            // of a row of x, dy, dsum (0: none)
+  int at[4];                               // of x, dy, dsum and the statistics in a stage
+  int stage;                               // bytes
+  int64_t stride[3];                       // of rows, in bytes
+  bool together[3];                        // contiguous
+};
+template <int T, int NV, bool VEC, bool BIAS>
+__global__ void __launch_bounds__(kBlock<T>) backward_copied_kernel(const sa_norm p, float* sums, const Copies c, const tc::WaitCtx status) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 buffer[2][32];
+  __shared__ uint64_t full[kRing];
+  const int t = threadIdx.x % T, team = threadIdx.x / T;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) tc::mbar_init(&full[i], 1);
+    tc::mbar_init_fence();
+  }
+  __syncthreads();
+  tc::after_previous_kernel();
+  tc::Waiter wait;
+  wait.begin(status);
+  const int64_t stages = (p.rows + c.rows - 1) / c.rows;
+  const char* const from[3] = {static_cast<const char*>(p.x), static_cast<const char*>(p.dy), static_cast<const char*>(p.dsum)};
+  auto load = [&](int64_t i, int slot) {                          // by one thread
+    const int64_t row = i * c.rows;
+    const int n = (int)min((int64_t)c.rows, p.rows - row);
+    uint8_t* to = smem + slot * c.stage;
+    const uint32_t stats = (uint32_t)(n * 8) & ~15u;
+    uint32_t all = stats;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) all += (uint32_t)(n * c.bytes[k]) & ~15u;
+    tc::mbar_expect_tx(&full[slot], all);
+    if (stats > 0) tc::bulk_load(to + c.at[3], p.stats + 2 * row, stats, &full[slot]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (c.bytes[k] == 0) continue;
+      const char* src = from[k] + row * c.stride[k];
+      if (c.together[k]) {
+        const uint32_t size = (uint32_t)(n * c.bytes[k]) & ~15u;
+        if (size > 0) tc::bulk_load(to + c.at[k], src, size, &full[slot]);
+      } else {
+        for (int r = 0; r < n; ++r) tc::bulk_load(to + c.at[k] + r * c.bytes[k], src + r * c.stride[k], (uint32_t)c.bytes[k], &full[slot]);
+      }
+    }
+  };
+  if (threadIdx.x == 0)
+    for (int k = 0; k < kRing; ++k)
+      if (blockIdx.x + (int64_t)k * gridDim.x < stages) load(blockIdx.x + (int64_t)k * gridDim.x, k);
+  int turn = 0, slot = 0, round = 0;
+  Gradient<T, NV, VEC, BIAS> gradient;
+  for (int64_t i = blockIdx.x; i < stages; i += gridDim.x) {
+    const int64_t row0 = i * c.rows;
+    const int n = (int)min((int64_t)c.rows, p.rows - row0);
+    uint8_t* const at = smem + slot * c.stage;
+    wait(tc::smem_u32(&full[slot]), round & 1, 1100);
+    if (n < c.rows) {                                             // the last stage: what is left of 16 bytes
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const int done = (n * c.bytes[k]) & ~15, rest = n * c.bytes[k] - done;
+        if ((int)threadIdx.x < rest / 2)
+          reinterpret_cast<uint16_t*>(at + c.at[k] + done)[threadIdx.x] =
+              reinterpret_cast<const uint16_t*>(from[k] + row0 * c.stride[k] + done)[threadIdx.x];
+      }
+      if (threadIdx.x < 2 && n % 2 != 0) reinterpret_cast<float*>(at + c.at[3])[2 * (n - 1) + threadIdx.x] = p.stats[2 * (row0 + n - 1) + threadIdx.x];
+      __syncthreads();
+    }
+    for (int r0 = 0; r0 < n; r0 += kRowsOf<T>) {
+      const int r = r0 + team;
+      const int width = r < n ? p.width : 0;
+      float h[NV][8], g[NV][8];
+      load_row<NV, T, VEC, true>(h, at + c.at[0] + r * c.bytes[0], p.x_dtype, 0, width, t);
+      load_row<NV, T, VEC, true>(g, at + c.at[1] + r * c.bytes[1], p.y_dtype, 0, width, t);
+      const float2 stats = reinterpret_cast<const float2*>(at + c.at[3])[r];
+      gradient.row(p, h, g, stats, width, t, buffer, turn);
+      if (c.bytes[2] != 0) {
+        load_row<NV, T, VEC, true>(h, at + c.at[2] + r * c.bytes[2], p.x_dtype, 0, width, t);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[k][e] += h[k][e];
+      }
+      store_row<NV, T, VEC>(g, p.dx, p.x_dtype, (row0 + r) * p.width, width, t);
+      if (p.dbranch != nullptr) store_row<NV, T, VEC>(g, p.dbranch, p.branch_dtype, (row0 + r) * p.width, width, t);
+    }
+    __syncthreads();                                              // the stage has been read
+    if (threadIdx.x == 0 && i + (int64_t)kRing * gridDim.x < stages) load(i + (int64_t)kRing * gridDim.x, slot);
+    if (++slot == kRing) {
+      slot = 0;
+      ++round;
+    }
+  }
+  wait.end(status);
+  if (sums != nullptr) gradient.finish(p, sums, reinterpret_cast<float*>(smem), t, team);
+}
+
+// Columns of the parameters' gradients: 8 a CTA (a sector of each part), whose 64 groups of 8 threads take the parts in turn.
 __global__ void __launch_bounds__(512) parameters_kernel(const float* sums, int parts, int width, int columns, int dtype, void* dweight, void* dbias) {
   tc::after_previous_kernel();
-  __shared__ float by_warp[16][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  __shared__ float by_group[64][9];
+  const int c = threadIdx.x & 7, group = threadIdx.x >> 3, col = blockIdx.x * 8 + c;
   float v = 0.f;
   if (col < columns) {
 #pragma unroll 8
-    for (int i = warp; i < parts; i += 16) v += sums[(int64_t)i * columns + col];
+    for (int i = group; i < parts; i += 64) v += sums[(int64_t)i * columns + col];
   }
-  by_warp[warp][lane] = v;
+  by_group[group][c] = v;
   __syncthreads();
-  if (warp != 0 || col >= columns) return;
-  for (int i = 1; i < 16; ++i) v += by_warp[i][lane];
+  if (group >= 8) return;
+  for (int i = group + 8; i < 64; i += 8) v += by_group[i][c];
+  __syncwarp();
+  by_group[group][c] = v;
+  asm volatile("bar.sync 1, 64;" ::: "memory");
+  if (group != 0 || col >= columns) return;
+  for (int i = 1; i < 8; ++i) v += by_group[i][c];
   void* out = col < width ? dweight : dbias;
   if (out == nullptr) return;
   const int at = col < width ? col : col - width;
@@ -236,6 +390,8 @@ int by_width(int width, F f) {
   using std::integral_constant;
 #define SA_NORM_CASE(most, threads, chunks) \
   if (width <= most) return f(integral_constant<int, threads>(), integral_constant<int, chunks>())
+  SA_NORM_CASE(64, 8, 1);
+  SA_NORM_CASE(128, 16, 1);
   SA_NORM_CASE(256, 32, 1);
   SA_NORM_CASE(512, 32, 2);
   SA_NORM_CASE(1024, 128, 1);
@@ -247,13 +403,64 @@ int by_width(int width, F f) {
   return SA_ERR_UNSUPPORTED;
 }
 
-int threads_of(int width) { return width <= 512 ? 32 : width <= 2048 ? 128 : width <= 4096 ? 256 : width <= 8192 ? 512 : 1024; }
-// CTAs of the backward: about 1,024 threads an SM.
+// What the backward's copies look like; false where rows do not take them.
+bool copies_of(const sa_norm& p, int rows_at_a_time, Copies* c) {
+  const void* const from[3] = {p.x, p.dy, p.dsum};
+  const int types[3] = {p.x_dtype, p.y_dtype, p.x_dtype};
+  const int64_t strides[3] = {p.x_stride, p.dy_stride, p.dsum_stride};
+  bool odd = false;                        // rows that are no multiple of 16 bytes
+  int row = 8;
+  for (int k = 0; k < 3; ++k) {
+    const int size = types[k] == SA_F32 ? 4 : 2;
+    c->bytes[k] = from[k] != nullptr ? p.width * size : 0;
+    c->stride[k] = strides[k] * size;
+    c->together[k] = p.rows == 1 || strides[k] == p.width;
+    if (from[k] == nullptr) continue;
+    if (reinterpret_cast<uintptr_t>(from[k]) % 16 != 0) return false;
+    if (!c->together[k] && (c->bytes[k] % 16 != 0 || c->stride[k] % 16 != 0)) return false;
+    odd = odd || c->bytes[k] % 16 != 0;
+    row += c->bytes[k];
+  }
+  if (reinterpret_cast<uintptr_t>(p.stats) % 16 != 0) return false;
+  // stages of about 8 KB, of whole rounds of the CTA's teams
+  const int step = std::max(rows_at_a_time, odd ? 8 : 2);
+  c->rows = std::max(step, 8192 / row / step * step);
+  int at = 0;
+  for (int k = 0; k < 3; ++k) {
+    c->at[k] = at;
+    at += (c->rows * c->bytes[k] + 15) / 16 * 16;
+  }
+  c->at[3] = at;
+  c->stage = (at + c->rows * 8 + 127) / 128 * 128;
+  return c->stage * kRing <= 104 * 1024;        // two CTAs an SM
+}
+
+// CTAs of the backward: at most 768 threads an SM, or as many as their stages leave room for.
 int blocks_of(const sa_norm& p) {
-  const int t = threads_of(p.width), block = std::max(t, 128), rows = block / t;
-  return (int)std::min<int64_t>((p.rows + rows - 1) / rows, (int64_t)kSms * (1024 / block));
+  int blocks = 0;
+  by_width(p.width, [&](auto threads, auto chunks) {
+    constexpr int T = decltype(threads)::value;
+    Copies c;
+    const bool copied = copies_of(p, kRowsOf<T>, &c);
+    const int64_t rows = copied ? c.rows : kRowsOf<T>;
+    const int here = copied ? std::min(768 / kBlock<T>, 200 * 1024 / (c.stage * kRing + 2048)) : 512 / kBlock<T>;
+    blocks = (int)std::min<int64_t>((p.rows + rows - 1) / rows, (int64_t)kSms * std::max(1, here));
+    return SA_OK;
+  });
+  return blocks;
 }
 int columns_of(const sa_norm& p) { return p.width * (p.dbias != nullptr ? 2 : 1); }
+
+template <int T, int NV, bool VEC, bool BIAS>
+int launch_backward(const sa_norm& p, int blocks, float* sums, cudaStream_t s) {
+  Copies c;
+  if (!copies_of(p, kRowsOf<T>, &c)) return launch_after(backward_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, kTeamBytes<T, NV, BIAS>, s, p, sums);
+  tc::WaitCtx status;
+  const int st = tc::wait_ctx(&status);
+  if (st != SA_OK) return st;
+  const size_t smem = std::max((size_t)c.stage * kRing, kTeamBytes<T, NV, BIAS>);
+  return launch_after(backward_copied_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, smem, s, p, sums, (const Copies)c, (const tc::WaitCtx)status);
+}
 
 }  // namespace
 
@@ -264,7 +471,8 @@ size_t backward_bytes(const sa_norm& p) {
 int forward(const sa_norm& p, cudaStream_t s) {
   return by_width(p.width, [&](auto threads, auto chunks) {
     constexpr int T = decltype(threads)::value, NV = decltype(chunks)::value;
-    const dim3 grid((unsigned)((p.rows + kRowsOf<T> - 1) / kRowsOf<T>));
+    constexpr int kRows = kRowsOf<T> * kTogether<T, NV>;
+    const dim3 grid((unsigned)((p.rows + kRows - 1) / kRows));
     return vectors(p, false) ? launch_after(forward_kernel<T, NV, true>, grid, kBlock<T>, 0, s, p)
                              : launch_after(forward_kernel<T, NV, false>, grid, kBlock<T>, 0, s, p);
   });
@@ -273,17 +481,13 @@ int forward(const sa_norm& p, cudaStream_t s) {
 int backward(const sa_norm& p, cudaStream_t s) {
   const int blocks = blocks_of(p);
   float* sums = p.dweight == nullptr && p.dbias == nullptr ? nullptr : static_cast<float*>(p.workspace);
-  int st = by_width(p.width, [&](auto threads, auto chunks) {
+  const int st = by_width(p.width, [&](auto threads, auto chunks) {
     constexpr int T = decltype(threads)::value, NV = decltype(chunks)::value;
-    const dim3 grid(blocks);
-    if (p.dbias != nullptr)
-      return vectors(p, true) ? launch_after(backward_kernel<T, NV, true, true>, grid, kBlock<T>, 0, s, p, sums)
-                              : launch_after(backward_kernel<T, NV, false, true>, grid, kBlock<T>, 0, s, p, sums);
-    return vectors(p, true) ? launch_after(backward_kernel<T, NV, true, false>, grid, kBlock<T>, 0, s, p, sums)
-                            : launch_after(backward_kernel<T, NV, false, false>, grid, kBlock<T>, 0, s, p, sums);
+    if (p.dbias != nullptr) return vectors(p, true) ? launch_backward<T, NV, true, true>(p, blocks, sums, s) : launch_backward<T, NV, false, true>(p, blocks, sums, s);
+    return vectors(p, true) ? launch_backward<T, NV, true, false>(p, blocks, sums, s) : launch_backward<T, NV, false, false>(p, blocks, sums, s);
   });
   if (st != SA_OK || sums == nullptr) return st;
-  return launch_after(parameters_kernel, dim3((columns_of(p) + 31) / 32), 512, 0, s, (const float*)sums, blocks, p.width, columns_of(p), p.weight_dtype,
+  return launch_after(parameters_kernel, dim3((columns_of(p) + 7) / 8), 512, 0, s, (const float*)sums, blocks, p.width, columns_of(p), p.weight_dtype,
                       p.dweight, p.dbias);
 }
 

@@ -342,6 +342,9 @@ __device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&r)[32], 
       for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
       store32(p + 16 * h, v);
     }
+  } else if (valid >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) reinterpret_cast<uint4*>(p)[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)

@@ -621,9 +621,20 @@ const char* name_of(at::ScalarType t) { return c10::toString(t); }
 
 // (..., d) as rows of d contiguous values at one stride: a view where the layout allows it.
 Tensor rows_in(const Tensor& t) {
+  if (t.dim() == 2 && t.stride(0) >= 0 && (t.stride(1) == 1 || t.size(1) == 1)) return t;
   const Tensor r = t.reshape({t.numel() / std::max<int64_t>(t.size(-1), 1), t.size(-1)});
   return (r.stride(1) == 1 || r.size(1) == 1) && r.stride(0) >= 0 ? r : r.contiguous();
 }
+Tensor in_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+Tensor in_order(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+// Small numbers of a node in one: a list of them takes longer to make than a kernel to launch.
+int64_t packed(std::initializer_list<int64_t> values) {         // each -1 .. 254
+  int64_t all = 0;
+  int at = 0;
+  for (const int64_t v : values) all |= (v + 1) << (8 * at++);
+  return all;
+}
+int64_t packed_at(int64_t all, int i) { return ((all >> (8 * i)) & 255) - 1; }
 void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor given(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 
@@ -655,13 +666,13 @@ sa_norm norm_of(const Tensor& x, const Tensor& weight, const Tensor& bias, doubl
 variable_list run_norm(const Tensor& x_in, const Tensor& branch_in, const Tensor& weight, const Tensor& bias, double eps, at::ScalarType type,
                        Tensor* rows, Tensor* stats) {
   const Tensor x = rows_in(x_in);
-  const Tensor y = at::empty(x_in.sizes(), x_in.options().dtype(type));
+  const Tensor y = fresh(x_in.sizes(), type, x_in);
   Tensor sum, branch;
   if (branch_in.defined()) {
     branch = rows_in(branch_in);
-    sum = at::empty(x_in.sizes(), x_in.options());
+    sum = fresh(x_in.sizes(), x_in.scalar_type(), x_in);
   }
-  if (stats != nullptr) *stats = at::empty({x.size(0), 2}, x.options().dtype(at::kFloat));
+  if (stats != nullptr) *stats = fresh({x.size(0), 2}, at::kFloat, x);
   if (rows != nullptr) *rows = x;
   if (x.numel() > 0) {
     sa_norm p = norm_of(x, weight, bias, eps);
@@ -690,13 +701,14 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     ctx->save_for_backward({branch ? out[0] : x, given(weight), given(bias), stats});
     ctx->saved_data["eps"] = eps;
     auto wants = [](const std::optional<Tensor>& t) { return (int64_t)(t && t->requires_grad()); };
-    ctx->saved_data["args"] = c10::List<int64_t>({type, branch ? (int64_t)branch->scalar_type() : -1, wants(branch), wants(weight), wants(bias)});
+    ctx->saved_data["args"] = packed({type, branch ? (int64_t)branch->scalar_type() : -1, wants(branch), wants(weight), wants(bias)});
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad_out) {
     const auto saved = ctx->get_saved_variables();
-    const auto args = ctx->saved_data["args"].toIntVector();
+    const int64_t all = ctx->saved_data["args"].toInt();
+    const int64_t args[5] = {packed_at(all, 0), packed_at(all, 1), packed_at(all, 2), packed_at(all, 3), packed_at(all, 4)};
     variable_list grads(6);
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -706,16 +718,16 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
       const bool added = args[1] >= 0;
       const Tensor x = rows_in(s);
       const Tensor dy_in = grad_out[added ? 1 : 0], dsum_in = added ? grad_out[0] : Tensor();
-      const Tensor dy = rows_in(dy_in.defined() ? dy_in.to(type) : at::zeros(s.sizes(), s.options().dtype(type)));
-      const Tensor dsum = dsum_in.defined() ? rows_in(dsum_in.to(s.scalar_type())) : Tensor();
-      Tensor dx = at::empty(s.sizes(), s.options().memory_format(at::MemoryFormat::Contiguous)), dbranch, dweight, dbias;
-      if (args[2]) dbranch = (at::ScalarType)args[1] == s.scalar_type() ? dx : at::empty(s.sizes(), s.options().dtype((at::ScalarType)args[1]).memory_format(at::MemoryFormat::Contiguous));
-      const Tensor w = weight.defined() ? weight.contiguous() : weight;
-      if (args[3]) dweight = at::empty(w.sizes(), w.options());
-      if (args[4]) dbias = at::empty(bias.sizes(), bias.options());
+      const Tensor dy = rows_in(dy_in.defined() ? in_type(dy_in, type) : at::zeros(s.sizes(), s.options().dtype(type)));
+      const Tensor dsum = dsum_in.defined() ? rows_in(in_type(dsum_in, s.scalar_type())) : Tensor();
+      Tensor dx = fresh(s.sizes(), s.scalar_type(), s), dbranch, dweight, dbias;
+      if (args[2]) dbranch = (at::ScalarType)args[1] == s.scalar_type() ? dx : fresh(s.sizes(), (at::ScalarType)args[1], s);
+      const Tensor w = weight.defined() ? in_order(weight) : weight;
+      if (args[3]) dweight = fresh(w.sizes(), w.scalar_type(), w);
+      if (args[4]) dbias = fresh(bias.sizes(), bias.scalar_type(), bias);
       if (x.numel() > 0) {
         sa_norm p = norm_of(x, w, bias, ctx->saved_data["eps"].toDouble());
-        const Tensor stats = saved[3].contiguous();
+        const Tensor stats = in_order(saved[3]);
         p.bias = nullptr;
         p.y_dtype = code_of(dy);
         p.stats = stats.data_ptr<float>();
@@ -731,7 +743,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         p.dweight = pointer(dweight);
         p.dbias = pointer(dbias);
         p.workspace_bytes = sa_norm_backward_bytes(&p);
-        const Tensor workspace = bytes_on(x, p.workspace_bytes);
+        const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
         p.workspace = workspace.data_ptr();
         check("sa_norm_backward", sa_norm_backward(&p), true);
       } else {
@@ -766,7 +778,7 @@ variable_list layer_norm(const Tensor& x, const std::optional<Tensor>& branch, c
   TORCH_CHECK_VALUE(eps >= 0.0, fn, ": eps must not be negative; got ", eps);
   const at::ScalarType type = dtype ? *dtype : x.scalar_type();
   TORCH_CHECK_VALUE(code_of(type) >= 0, fn, ": dtype must be float32, bfloat16 or float16; got ", name_of(type));
-  auto contiguous = [](const std::optional<Tensor>& t) { return t ? std::optional<Tensor>(t->contiguous()) : t; };
+  auto contiguous = [](const std::optional<Tensor>& t) { return t ? std::optional<Tensor>(in_order(*t)) : t; };
   const auto w = contiguous(weight), b = contiguous(bias);
   auto wants = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
   if (c10::GradMode::is_enabled() && (x.requires_grad() || wants(branch) || wants(weight) || wants(bias)))
@@ -789,7 +801,7 @@ sa_embedding embedding_of(const Tensor& idx, int64_t vocab, int64_t width, doubl
 
 Tensor run_embedding(const Tensor& idx, const Tensor& weight_in, double scale, at::ScalarType type, at::IntArrayRef shape) {
   const Tensor weight = rows_in(weight_in);
-  const Tensor y = at::empty(shape, weight.options().dtype(type));
+  const Tensor y = fresh(shape, type, weight);
   if (y.numel() > 0) {
     sa_embedding p = embedding_of(idx, weight.size(0), weight.size(1), scale);
     p.weight_dtype = code_of(weight);
@@ -818,9 +830,9 @@ struct Embedding : public torch::autograd::Function<Embedding> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::cuda::CUDAGuard guard(saved[0].device());
-      const Tensor idx = saved[0].contiguous();
-      const Tensor dy = rows_in(grad_out[0].to((at::ScalarType)args[3]));
-      const Tensor dweight = at::empty({args[0], args[1]}, dy.options().dtype((at::ScalarType)args[2]));
+      const Tensor idx = in_order(saved[0]);
+      const Tensor dy = rows_in(in_type(grad_out[0], (at::ScalarType)args[3]));
+      const Tensor dweight = fresh({args[0], args[1]}, (at::ScalarType)args[2], dy);
       if (idx.numel() == 0) {
         dweight.zero_();
       } else {
@@ -831,7 +843,7 @@ struct Embedding : public torch::autograd::Function<Embedding> {
         p.dy_stride = dy.stride(0);
         p.dweight = dweight.data_ptr();
         p.workspace_bytes = sa_embedding_backward_bytes(&p);
-        const Tensor workspace = bytes_on(dy, p.workspace_bytes);
+        const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, dy);
         p.workspace = workspace.data_ptr();
         check("sa_embedding_backward", sa_embedding_backward(&p), true);
       }
@@ -841,7 +853,7 @@ struct Embedding : public torch::autograd::Function<Embedding> {
   }
 };
 
-Tensor indices_in(const Tensor& t) { return (t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous(); }
+Tensor indices_in(const Tensor& t) { return in_order(in_type(t, at::kLong)); }
 
 Tensor embedding(const Tensor& idx_in, const Tensor& weight, double scale, const std::optional<at::ScalarType>& dtype) {
   const char* fn = "embedding";
@@ -885,9 +897,8 @@ sa_linear_loss loss_of(const Tensor& x, const Tensor& weight, const Tensor& targ
 Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore_index, int64_t reduction, int64_t product,
                 at::IntArrayRef shape, Tensor* lse) {
   const int64_t n = x.size(0);
-  const auto fp32 = x.options().dtype(at::kFloat);
-  *lse = at::empty({n + 1}, fp32);
-  const Tensor loss = reduction == SA_REDUCTION_NONE ? at::empty(shape, fp32) : at::empty({}, fp32);
+  *lse = fresh({n + 1}, at::kFloat, x);
+  const Tensor loss = fresh(reduction == SA_REDUCTION_NONE ? shape : at::IntArrayRef(), at::kFloat, x);
   if (n == 0) {                                     // a mean over nothing is no number
     if (reduction != SA_REDUCTION_NONE) loss.fill_(reduction == SA_REDUCTION_MEAN ? std::nan("") : 0.0);
     return loss;
@@ -897,7 +908,7 @@ Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, in
   p.count = p.lse + n;
   p.loss = loss.data_ptr<float>();
   p.workspace_bytes = sa_linear_loss_forward_bytes(&p);
-  const Tensor workspace = bytes_on(x, p.workspace_bytes);
+  const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
   p.workspace = workspace.data_ptr();
   check("sa_linear_loss_forward", sa_linear_loss_forward(&p));
   return loss;
@@ -920,10 +931,10 @@ struct LinearLoss : public torch::autograd::Function<LinearLoss> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::cuda::CUDAGuard guard(saved[0].device());
-      const Tensor x = rows_in(saved[0]), weight = rows_in(saved[1]), targets = saved[2].contiguous(), lse = saved[3].contiguous();
-      const Tensor dloss = grad_out[0].to(at::kFloat).contiguous();
-      if (ctx->needs_input_grad(0)) grads[0] = at::empty(saved[0].sizes(), saved[0].options().memory_format(at::MemoryFormat::Contiguous));
-      if (ctx->needs_input_grad(1)) grads[1] = at::empty(saved[1].sizes(), saved[1].options().memory_format(at::MemoryFormat::Contiguous));
+      const Tensor x = rows_in(saved[0]), weight = rows_in(saved[1]), targets = in_order(saved[2]), lse = in_order(saved[3]);
+      const Tensor dloss = in_order(in_type(grad_out[0], at::kFloat));
+      if (ctx->needs_input_grad(0)) grads[0] = fresh(saved[0].sizes(), saved[0].scalar_type(), saved[0]);
+      if (ctx->needs_input_grad(1)) grads[1] = fresh(saved[1].sizes(), saved[1].scalar_type(), saved[1]);
       if (x.size(0) == 0) {
         if (grads[1].defined()) grads[1].zero_();
       } else if (grads[0].defined() || grads[1].defined()) {
@@ -934,7 +945,7 @@ struct LinearLoss : public torch::autograd::Function<LinearLoss> {
         p.dx = pointer(grads[0]);
         p.dweight = pointer(grads[1]);
         p.workspace_bytes = sa_linear_loss_backward_bytes(&p);
-        const Tensor workspace = bytes_on(x, p.workspace_bytes);
+        const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
         p.workspace = workspace.data_ptr();
         check("sa_linear_loss_backward", sa_linear_loss_backward(&p), true);
       }
