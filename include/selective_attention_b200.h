@@ -448,7 +448,8 @@ int sa_beam_select(const sa_beam* p);
  *   product  type of the products' operands: x and weight are rounded to it first (SA_F32: three bf16 parts, 24 bits)
  *   targets  int64; ignore_index counts for nothing, and what stands in its row of x does not matter; any other target outside the vocabulary makes
  *            its loss and the gradients NaN
- *   lse      (tokens,) fp32, log2 of the sum of exponentials: written by the forward, read by the backward; count (1,) fp32 likewise
+ *   lse      (tokens, 2) fp32, log2 of the sum of exponentials in two parts: written by the forward, read by the backward; count (1,) fp32
+ *            likewise
  *   loss     (tokens,) fp32 without a reduction (0 where the target is ignored), else one number
  *   dloss    of loss's shape; dx, dweight contiguous, of x's and weight's type, either may be null
  * sums are fp32; the gradient of the logits is rounded to `product` between the products (fp16: scaled by 2^14 over the
@@ -467,14 +468,21 @@ typedef struct sa_linear_loss {
   float *lse, *count, *loss;
   const float* dloss;
   void *dx, *dweight;
-  void* workspace;        /* sa_linear_loss_forward_bytes() or _backward_bytes(), 256-byte aligned */
+  void* workspace;        /* as many bytes as the call's _bytes() says, 256-byte aligned; none for sa_linear_loss_scale */
   uint64_t workspace_bytes;
   void* stream;
+  float *dx_sums, *dweight_sums;   /* (tokens, width) and (vocab, width) fp32, contiguous, for the two calls below; either may be null */
 } sa_linear_loss;
 size_t sa_linear_loss_forward_bytes(const sa_linear_loss* p);
 int sa_linear_loss_forward(const sa_linear_loss* p);
 size_t sa_linear_loss_backward_bytes(const sa_linear_loss* p);
 int sa_linear_loss_backward(const sa_linear_loss* p);
+/* The same with a product less, where there is a reduction and product is SA_BF16 or SA_F32: _train writes loss and count, and the
+ * gradients' sums for a sum's cotangent of 1; _scale makes dx and dweight of them (those that are not null) for dloss and count.
+ * lse is not used.  In products of SA_BF16 the softmax enters as exponentials of 8 bits, and x over their sum rounded to 8 bits. */
+size_t sa_linear_loss_train_bytes(const sa_linear_loss* p);
+int sa_linear_loss_train(const sa_linear_loss* p);
+int sa_linear_loss_scale(const sa_linear_loss* p);
 
 /* Layer norm over rows of `width` (at most 16,384) contiguous values at row strides, with fp32 statistics.
  *   s = x + branch (branch may be null: s = x), rounded to x's type and written to `sum` with a branch;

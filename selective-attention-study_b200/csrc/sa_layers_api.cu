@@ -48,7 +48,7 @@ int check_embedding(const sa_embedding* p, bool backward) {
   return ok ? SA_OK : SA_ERR_ALIGNMENT;
 }
 
-int to_loss(const sa_linear_loss* in, bool backward, loss::Problem* p) {
+int to_loss(const sa_linear_loss* in, loss::Problem* p) {
   if (in == nullptr || in->struct_bytes != (int32_t)sizeof(sa_linear_loss)) return SA_ERR_BAD_ARGUMENT;
   if (!type_ok(in->product) || !type_ok(in->x_dtype) || !type_ok(in->weight_dtype)) return SA_ERR_BAD_ARGUMENT;
   if (in->reduction < SA_REDUCTION_NONE || in->reduction > SA_REDUCTION_MEAN) return SA_ERR_BAD_ARGUMENT;
@@ -57,15 +57,23 @@ int to_loss(const sa_linear_loss* in, bool backward, loss::Problem* p) {
   // sums of 24-bit products are kept in fp32 only where results are
   if (in->product == SA_F32 && (in->x_dtype != SA_F32 || in->weight_dtype != SA_F32)) return SA_ERR_UNSUPPORTED;
   *p = loss::Problem{in->product, in->x_dtype, in->weight_dtype, in->reduction, in->tokens, in->vocab, in->width, in->ignore_index, in->x, in->x_stride,
-                     in->weight, in->weight_stride, in->targets, in->lse, in->count, in->loss, in->dloss, in->dx, in->dweight, in->workspace};
+                     in->weight, in->weight_stride, in->targets, in->lse, in->count, in->loss, in->dloss, in->dx, in->dweight, in->dx_sums, in->dweight_sums,
+                     in->workspace};
   return SA_OK;
+}
+
+// The form that computes the gradients with the loss: one cotangent, and operands whose exponents hold e^44.
+int check_train(const sa_linear_loss* in) {
+  if (in->reduction == SA_REDUCTION_NONE || in->product == SA_F16) return SA_ERR_UNSUPPORTED;
+  if (!in->dx_sums && !in->dweight_sums) return SA_ERR_BAD_ARGUMENT;
+  return aligned(in->dx_sums, 4) && aligned(in->dweight_sums, 4) ? SA_OK : SA_ERR_ALIGNMENT;
 }
 
 int check_loss(const sa_linear_loss* in, bool backward, size_t need) {
   if (!in->x || !in->weight || !in->targets || !in->lse || !in->workspace) return SA_ERR_BAD_ARGUMENT;
   if (in->reduction != SA_REDUCTION_NONE && !in->count) return SA_ERR_BAD_ARGUMENT;
   if (backward ? !in->dloss || (!in->dx && !in->dweight) : !in->loss) return SA_ERR_BAD_ARGUMENT;
-  if (!fits(in->x, in->x_dtype) || !fits(in->weight, in->weight_dtype) || !aligned(in->targets, 8) || !aligned(in->lse, 4) || !aligned(in->count, 4) ||
+  if (!fits(in->x, in->x_dtype) || !fits(in->weight, in->weight_dtype) || !aligned(in->targets, 8) || !aligned(in->lse, 8) || !aligned(in->count, 4) ||
       !aligned(in->loss, 4) || !aligned(in->dloss, 4) || !fits(in->dx, in->x_dtype) || !fits(in->dweight, in->weight_dtype) ||
       !aligned(in->workspace, 256))
     return SA_ERR_ALIGNMENT;
@@ -121,26 +129,54 @@ int sa_embedding_backward(const sa_embedding* p) {
 
 size_t sa_linear_loss_forward_bytes(const sa_linear_loss* in) {
   loss::Problem p;
-  return to_loss(in, false, &p) == SA_OK ? loss::forward_bytes(p) : 0;
+  return to_loss(in, &p) == SA_OK ? loss::forward_bytes(p) : 0;
 }
 
 int sa_linear_loss_forward(const sa_linear_loss* in) {
   loss::Problem p;
-  int st = to_loss(in, false, &p);
+  int st = to_loss(in, &p);
   if (st == SA_OK) st = check_loss(in, false, loss::forward_bytes(p));
   return st != SA_OK ? st : loss::forward(p, static_cast<cudaStream_t>(in->stream));
 }
 
 size_t sa_linear_loss_backward_bytes(const sa_linear_loss* in) {
   loss::Problem p;
-  return to_loss(in, true, &p) == SA_OK ? loss::backward_bytes(p) : 0;
+  return to_loss(in, &p) == SA_OK ? loss::backward_bytes(p) : 0;
 }
 
 int sa_linear_loss_backward(const sa_linear_loss* in) {
   loss::Problem p;
-  int st = to_loss(in, true, &p);
+  int st = to_loss(in, &p);
   if (st == SA_OK) st = check_loss(in, true, loss::backward_bytes(p));
   return st != SA_OK ? st : loss::backward(p, static_cast<cudaStream_t>(in->stream));
+}
+
+size_t sa_linear_loss_train_bytes(const sa_linear_loss* in) {
+  loss::Problem p;
+  return to_loss(in, &p) == SA_OK && check_train(in) == SA_OK ? loss::train_bytes(p) : 0;
+}
+
+int sa_linear_loss_train(const sa_linear_loss* in) {
+  loss::Problem p;
+  int st = to_loss(in, &p);
+  if (st == SA_OK) st = check_train(in);
+  if (st != SA_OK) return st;
+  if (!in->x || !in->weight || !in->targets || !in->count || !in->loss || !in->workspace) return SA_ERR_BAD_ARGUMENT;
+  if (!fits(in->x, in->x_dtype) || !fits(in->weight, in->weight_dtype) || !aligned(in->targets, 8) || !aligned(in->count, 4) ||
+      !aligned(in->loss, 4) || !aligned(in->workspace, 256))
+    return SA_ERR_ALIGNMENT;
+  if (in->workspace_bytes < loss::train_bytes(p)) return SA_ERR_WORKSPACE;
+  return tc::timeout_pending() ? SA_ERR_DEVICE_TIMEOUT : loss::train(p, static_cast<cudaStream_t>(in->stream));
+}
+
+int sa_linear_loss_scale(const sa_linear_loss* in) {
+  loss::Problem p;
+  int st = to_loss(in, &p);
+  if (st == SA_OK) st = check_train(in);
+  if (st != SA_OK) return st;
+  if (!in->dloss || !in->count || (!in->dx && !in->dweight) || (in->dx && !in->dx_sums) || (in->dweight && !in->dweight_sums)) return SA_ERR_BAD_ARGUMENT;
+  if (!aligned(in->dloss, 4) || !aligned(in->count, 4) || !fits(in->dx, in->x_dtype) || !fits(in->dweight, in->weight_dtype)) return SA_ERR_ALIGNMENT;
+  return loss::scale(p, static_cast<cudaStream_t>(in->stream));
 }
 
 }  // extern "C"

@@ -2,10 +2,19 @@
 //
 //   z = x W^T,  loss_n = log sum_v exp z_nv - z_n,t(n),  dz = (softmax(z) - [v = t]) g_n,  dx = dz W,  dW = dz^T x.
 //
-// Forward: one product whose epilogue reduces every half tile of logits to its rows' maxima and sums, and a kernel that joins
-// them.  Backward: the vocabulary in pieces; a piece's logits are computed again (the same product), turned into dz in 16 bits,
-// and read by the two products of the gradients.  Four products of 2 N V d operations in all, one of them for not keeping N V
-// logits; the sums of dx over the pieces stay in fp32.
+// Forward alone: one product whose epilogue reduces every half tile of logits to its rows' maxima and sums, and a kernel that joins
+// them.
+//
+// Training with a sum or a mean (bf16 and fp32 products): the cotangent is one number, so the gradients are computed with the loss,
+// up to that number, and no logit twice.  Tokens come in runs; of a run, the product's epilogue keeps e = exp(z - ref) in 16 bits
+// beside the rows' sums s.  softmax(z) = e / s, so the rest is a scale of rows: of the result in dx = (1 / s) e W, and of the
+// right operand in dW = e^T (x / s).  ref is the target's logit, a dot product beforehand: e = 1 at the target and at most
+// e^loss elsewhere, which 8 bits of exponent hold with room for 1 / s up to a loss of 44.  Rows beyond that are found by the sums
+// and go through the product once more with their maximum for ref.  Three products of 2 N V d operations; the sums of dW over the runs stay in fp32.
+//
+// Otherwise (a cotangent for every token; fp16, whose five bits of exponent do not hold e): the backward computes the logits again
+// in pieces of the vocabulary, turns a piece's into dz in 16 bits, and reads them with the two products of the gradients.  Four products
+// in all; the sums of dx over the pieces stay in fp32.
 #include "sa_loss.cuh"
 
 #include <algorithm>
@@ -45,6 +54,54 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t
   return __half2float(static_cast<const __half*>(p)[at]);
 }
 
+// Eight values of a row from column `col` on, zeros behind the width.
+__device__ __forceinline__ void load_columns(const void* base, int dtype, int64_t row_at, int col, int width, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  const int64_t at = row_at + col;
+  const char* src = static_cast<const char*>(base) + at * (dtype == SA_F32 ? 4 : 2);
+  if (col + 8 <= width && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    if (dtype == SA_F32) {
+      const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
+    const uint4 a = *reinterpret_cast<const uint4*>(src);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (dtype == SA_BF16) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (col + i < width) v[i] = load_as_float(base, dtype, at + i);
+}
+// Eight values in `parts` parts of 16 bits, each what the ones before it leave.
+__device__ __forceinline__ void store_columns(uint16_t* dst, int64_t part_stride, int parts, int half, float (&v)[8]) {
+  for (int part = 0; part < parts; ++part) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = half ? pack_half(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst + part * part_stride) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (part + 1 < parts) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float first = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        v[i] = first == INFINITY || first == -INFINITY ? 0.f : v[i] - first;
+      }
+    }
+  }
+}
+
 __global__ void __launch_bounds__(256) convert_kernel(const Convert c) {
   after_previous_kernel();
   const int chunks = c.pitch >> 3;
@@ -67,52 +124,9 @@ __global__ void __launch_bounds__(256) convert_kernel(const Convert c) {
       c.factor[row] = !counts ? 0.f : t < 0 || t >= c.vocab ? NAN : factor;
     }
   }
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  const int64_t at = row * c.src_stride + col;
-  const int bytes = c.dtype == SA_F32 ? 4 : 2;
-  if (counts) {
-    const char* src = static_cast<const char*>(c.src) + at * bytes;
-    if (col + 8 <= c.width && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-      if (c.dtype == SA_F32) {
-        const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(src);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (c.dtype == SA_BF16) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-          } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < c.width) v[i] = load_as_float(c.src, c.dtype, at + i);
-    }
-  }
-  for (int part = 0; part < c.parts; ++part) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = c.half ? pack_half(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(c.dst + part * c.part + (int64_t)row * c.pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (part + 1 < c.parts) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16) == INFINITY || __uint_as_float(w[i] << 16) == -INFINITY ? 0.f : v[2 * i] - __uint_as_float(w[i] << 16);
-        const float high = __uint_as_float(w[i] & 0xFFFF0000u);
-        v[2 * i + 1] = high == INFINITY || high == -INFINITY ? 0.f : v[2 * i + 1] - high;
-      }
-    }
-  }
+  float v[8] = {};
+  if (counts) load_columns(c.src, c.dtype, row * c.src_stride, col, c.width, v);
+  store_columns(c.dst + (int64_t)row * c.pitch + col, c.part, c.parts, c.half, v);
 }
 
 // The largest |dloss| of the tokens that count.
@@ -140,8 +154,8 @@ __global__ void __launch_bounds__(1024) largest_kernel(const float* dloss, const
 // Joins the half tiles of 32 tokens: a lane has a token, the 32 warps take the half tiles in turn, eight loads in flight.  The last CTA
 // to end sums all tokens, in order.
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32, kJoinAhead = 8;
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats, int slots, const float* at_target, const int64_t* targets,
-                                                            int64_t ignore_index, int tokens, int vocab, int reduction, float* lse, float* loss,
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats, int slots, const float2* at_target, const int64_t* targets,
+                                                            int64_t ignore_index, int tokens, int vocab, int reduction, float2* lse, float* loss,
                                                             float* count, float2* sums, unsigned int* ticket) {
   after_previous_kernel();
   __shared__ float2 parts[kJoinWarps][32];
@@ -181,11 +195,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
     }
     float mine = 0.f, counts = 0.f;
     if (row < tokens) {
-      const float all = top + log2f(sum);
-      lse[row] = all;
+      const float rest = log2f(sum), all = top + rest, back = all - top;
+      lse[row] = make_float2(all, fabsf(all) < INFINITY ? (top - (all - back)) + (rest - back) : 0.f);
       const int64_t t = targets[row];
       if (t != ignore_index) {
-        mine = t < 0 || t >= vocab ? NAN : (all - at_target[row]) * kLn2;
+        const float2 here = at_target[row];
+        mine = t < 0 || t >= vocab ? NAN : ((lse[row].x - here.x) + (lse[row].y - here.y)) * kLn2;
         counts = 1.f;
       }
       if (reduction == SA_REDUCTION_NONE) loss[row] = mine;
@@ -222,10 +237,204 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
   }
 }
 
+// ---- training: what stands between the products -----------------------------------------------------------------------------------
+
+// What e is relative to, in log2 units: the target's logit; +inf for a token that does not count, NaN for a target outside the
+// vocabulary.  A warp a token.
+__global__ void __launch_bounds__(256) reference_kernel(const void* x, int x_dtype, int64_t x_stride, const void* weight, int weight_dtype,
+                                                        int64_t weight_stride, const int64_t* targets, int64_t ignore_index, int tokens, int vocab,
+                                                        int width, float* ref, int* any) {
+  after_previous_kernel();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *any = 0;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= tokens) return;
+  const int64_t t = targets[row];
+  float sum = 0.f;
+  if (t != ignore_index && t >= 0 && t < vocab) {
+    for (int col = lane * 8; col < width; col += 256) {
+      float a[8], b[8];
+      load_columns(x, x_dtype, row * x_stride, col, width, a);
+      load_columns(weight, weight_dtype, t * weight_stride, col, width, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(a[i], b[i], sum);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (lane == 0) ref[row] = t == ignore_index ? INFINITY : t < 0 || t >= vocab ? NAN : sum * kLog2e;
+}
+
+struct Rows {                              // of a run of tokens
+  const float2* stats;                     // (maximum, sum) of every half tile, [slots][tokens]
+  int slots;
+  const float2* at_target;
+  const float* e_target;
+  const int64_t* targets;
+  int64_t ignore_index;
+  int tokens, vocab, width;
+  float* ref;
+  int* far;                                // rows whose sums left the range
+  int* any;                                // whether there is one
+  int again;                               // they have been through the product once more
+  float* loss;
+  float* inverse;                          // 1 / s, 0 for a token that does not count
+  uint16_t* e;
+  int64_t e_pitch, e_part;
+  const void* x;
+  int x_dtype;
+  int64_t x_stride;
+  uint16_t* scaled;                        // x / s
+  int64_t scaled_pitch, scaled_part;
+  int parts;
+};
+constexpr float kFarthest = 18446744073709551616.f;      // 2^64
+
+// Sums of 32 tokens; their losses, e at the target less s (e - s is s times softmax - 1), and x / s.
+__global__ void __launch_bounds__(kJoinThreads) rows_kernel(const Rows r) {
+  after_previous_kernel();
+  if (r.again && *r.any == 0) return;
+  __shared__ float2 parts[kJoinWarps][32];
+  __shared__ float inverse_s[32];
+  __shared__ int now_s[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.x * 32, row = row0 + lane;
+  const bool inside = row < r.tokens;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = warp; i < r.slots; i += kJoinWarps * kJoinAhead) {
+    float2 v[kJoinAhead];
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k)
+      v[k] = i + k * kJoinWarps < r.slots && inside ? r.stats[(int64_t)(i + k * kJoinWarps) * r.tokens + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k) {
+      top = fmaxf(top, v[k].x);
+      sum += v[k].y;
+    }
+  }
+  parts[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (warp == 0) {
+    for (int i = 1; i < kJoinWarps; ++i) {
+      top = fmaxf(top, parts[i][lane].x);
+      sum += parts[i][lane].y;
+    }
+    const int64_t t = inside ? r.targets[row] : r.ignore_index;
+    const bool counts = inside && t != r.ignore_index, good = t >= 0 && t < r.vocab;
+    bool now = inside;                                             // finished here
+    if (r.again) {
+      now = inside && r.far[row] != 0;
+    } else if (inside) {
+      const bool far = counts && good && !(sum < kFarthest);
+      r.far[row] = far;
+      if (far) {
+        r.ref[row] = top;
+        *r.any = 1;
+        now = false;
+      }
+    }
+    float inverse = 0.f;
+    if (now) {
+      float loss = 0.f;
+      if (counts) {
+        const float ref = r.ref[row];
+        inverse = good ? 1.f / sum : NAN;
+        const float e = r.e_target[row];
+        loss = !good ? NAN : (e > 1.f / kFarthest ? log2f(sum / e) : (ref - r.at_target[row].x) + log2f(sum)) * kLn2;
+        if (good) {
+          float at = e - sum;
+          for (int part = 0; part < r.parts; ++part) {
+            const __nv_bfloat16 b = __float2bfloat16_rn(at);
+            r.e[part * r.e_part + (int64_t)row * r.e_pitch + t] = __bfloat16_as_ushort(b);
+            at -= __bfloat162float(b);
+          }
+        }
+      }
+      r.loss[row] = loss;
+      r.inverse[row] = inverse;
+    }
+    inverse_s[lane] = inverse;
+    now_s[lane] = now;
+  }
+  __syncthreads();
+  if (r.scaled == nullptr) return;
+  const int chunks = (int)(r.scaled_pitch >> 3);
+  for (int i = threadIdx.x; i < 32 * chunks; i += kJoinThreads) {
+    const int k = i / chunks, col = (i - k * chunks) * 8;
+    if (!now_s[k]) continue;
+    float v[8] = {};
+    if (inverse_s[k] != 0.f) {
+      load_columns(r.x, r.x_dtype, (row0 + k) * r.x_stride, col, r.width, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= inverse_s[k];
+    }
+    store_columns(r.scaled + (int64_t)(row0 + k) * r.scaled_pitch + col, r.scaled_part, r.parts, 0, v);
+  }
+}
+
+// The loss of all tokens, summed in an order that their number alone decides.
+__global__ void __launch_bounds__(1024) total_kernel(const float* losses, const int64_t* targets, int64_t ignore_index, int tokens, int reduction,
+                                                     float* loss, float* count) {
+  after_previous_kernel();
+  __shared__ double2 warps[32];
+  double a = 0.0, b = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < tokens; i += 1024) {
+    a += (double)losses[i];
+    b += targets[i] != ignore_index ? 1.0 : 0.0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(~0u, a, o);
+    b += __shfl_xor_sync(~0u, b, o);
+  }
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_double2(a, b);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 32; ++i) {
+    a += warps[i].x;
+    b += warps[i].y;
+  }
+  *count = (float)b;
+  *loss = (float)(reduction == SA_REDUCTION_MEAN ? a / b : a);
+}
+
+// Gradients from their sums: times the cotangent, over the tokens that count for a mean.  Eight values a thread.
+__global__ void __launch_bounds__(256) scale_kernel(const float* sums, int64_t n, const float* dloss, const float* count, int reduction, void* out,
+                                                    int dtype) {
+  after_previous_kernel();
+  float by = *dloss;
+  if (reduction == SA_REDUCTION_MEAN) by = *count == 0.f ? 0.f : by / *count;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= n) return;
+  const bool whole = at + 8 <= n && (reinterpret_cast<uintptr_t>(out) & 31) == 0 && (reinterpret_cast<uintptr_t>(sums) & 31) == 0;
+  float v[8];
+  if (whole) {
+    uint32_t r[8];
+    load32(sums + at, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]) * by;
+    if (dtype == SA_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[i]);
+      store32(static_cast<float*>(out) + at, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = dtype == SA_F16 ? pack_half(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    return;
+  }
+  for (int i = 0; i < 8 && at + i < n; ++i) {
+    const float f = sums[at + i] * by;
+    if (dtype == SA_F32) static_cast<float*>(out)[at + i] = f;
+    else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(out)[at + i] = __float2bfloat16_rn(f);
+    else static_cast<__half*>(out)[at + i] = __float2half_rn(f);
+  }
+}
+
 // Rows of a dealt tile from its slabs, in order: a thread has four columns of a row, four slabs in flight.
 constexpr int kFinishThreads = 256;
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, void* out,
-                                                                int dtype, int64_t out_pitch) {
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, int scale_rows,
+                                                                void* out, int dtype, int64_t out_pitch) {
   after_previous_kernel();
   const int tile = w.whole + blockIdx.x;
   int tm, tn;
@@ -233,7 +442,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const float* sla
   const int n = w.slabs_of(tile), columns = min(w.bn, w.n - tn * w.bn), across = w.bn >> 2;
   const int in_tile = blockIdx.y * (kFinishThreads / across) + threadIdx.x / across, c = (threadIdx.x % across) * 4, row = tm * tile_rows + in_tile;
   if (row >= w.m || c >= columns) return;
-  const float by = scale != nullptr ? *scale : 1.f;
+  const float by = scale != nullptr ? scale[scale_rows ? row : 0] : 1.f;
   const float4* from = reinterpret_cast<const float4*>(slabs + ((int64_t)blockIdx.x * w.slabs * tile_rows + in_tile) * w.bn + c);
   const int64_t stride = (int64_t)tile_rows * w.bn / 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -281,9 +490,9 @@ int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, in
 
 // A matrix of rows as the products read it.
 struct Operand {
-  const uint16_t* base;
-  int64_t rows, width, pitch, part;
-  int parts;
+  const uint16_t* base = nullptr;
+  int64_t rows = 0, width = 0, pitch = 0, part = 0;
+  int parts = 0;
   int map(CUtensorMap* m, bool mn_major) const { return make_map(m, base, width, rows, parts, pitch, part, mn_major ? 64 : kRows); }
 };
 
@@ -417,8 +626,7 @@ struct Forward {
   Operand x, weight;
   int ctas;
   Walk walk;
-  float2 *stats, *sums;
-  float* at_target;
+  float2 *stats, *sums, *at_target;
   unsigned int* ticket;
   Forward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
@@ -427,10 +635,24 @@ struct Forward {
     walk = walk_of(p.tokens, p.vocab, p.width, terms_of(p), ctas, false, 0);
     stats = room.take<float2>((int64_t)2 * walk.n_tiles * p.tokens);
     sums = room.take<float2>(over(p.tokens, 32));
-    at_target = room.take<float>(p.tokens);
+    at_target = room.take<float2>(p.tokens);
     ticket = room.take<unsigned int>(1);
   }
 };
+
+// Of `most` row tiles down to half as many, with `across` tiles a row: how many leave the fewest clusters idle.
+int64_t best_blocks(int64_t most, int64_t across) {
+  const int64_t clusters = kSms / 2;
+  int64_t best = 0, at = most;
+  for (int64_t b = most; 2 * b > most; --b) {
+    const int64_t tiles = b * across, used = tiles * 1000 / (over(tiles, clusters) * clusters);
+    if (used > best) {
+      best = used;
+      at = b;
+    }
+  }
+  return at;
+}
 
 struct Backward {
   Room room;
@@ -468,16 +690,7 @@ struct Backward {
   static int piece_of(const Problem& p) {
     const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>(4096, (320ll << 20) / column / 256 * 256);
     if (p.vocab <= most) return p.vocab;
-    const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
-    int64_t best = 0, at = blocks;
-    for (int64_t b = blocks; 2 * b > blocks; --b) {
-      const int64_t tiles = b * across, used = tiles * 1000 / (over(tiles, clusters) * clusters);
-      if (used > best) {
-        best = used;
-        at = b;
-      }
-    }
-    return (int)(at * 256);
+    return (int)(256 * best_blocks(most / 256, over(p.width, 2 * kRows)));
   }
   Walk dx_walk(const Problem& p, int columns) const {
     const int terms = terms_of(p);
@@ -488,16 +701,72 @@ struct Backward {
   }
 };
 
-int finish(const float* slabs, const Walk& w, int ctas, const float* scale, void* out, int dtype, int64_t pitch, cudaStream_t s) {
+int finish(const float* slabs, const Walk& w, int ctas, const float* scale, int scale_rows, void* out, int dtype, int64_t pitch, cudaStream_t s) {
   if (w.whole == w.tiles()) return SA_OK;
   const int rows = kFinishThreads / (w.bn >> 2);                  // bn: 128 or 256
-  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, slabs, w, kRows * ctas, scale, out, dtype, pitch);
+  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, slabs, w, kRows * ctas, scale, scale_rows, out, dtype,
+                      pitch);
 }
+
+struct Train {
+  Room room;
+  Operand x, weight, e, scaled;
+  int run;                       // tokens of a run
+  float *ref, *losses, *e_target, *inverse, *dx_slabs = nullptr, *dw_slabs = nullptr;
+  int *far, *any;
+  float2 *stats, *at_target;
+  Train(const Problem& p, void* base) : room{static_cast<char*>(base)} {
+    x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
+    weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
+    run = run_of(p);
+    ref = room.take<float>(p.tokens);
+    losses = room.take<float>(p.tokens);
+    far = room.take<int>(p.tokens);
+    any = room.take<int>(1);
+    at_target = room.take<float2>(run);
+    e_target = room.take<float>(run);
+    inverse = room.take<float>(run);
+    stats = room.take<float2>((int64_t)2 * logits_walk(p, run).n_tiles * run);
+    e.parts = scaled.parts = parts_of(p);
+    e.rows = scaled.rows = run;
+    e.width = p.vocab;
+    e.pitch = up(p.vocab, 64);
+    e.part = e.pitch * run;
+    e.base = room.take<uint16_t>(e.part * e.parts);
+    scaled.width = p.width;
+    scaled.pitch = up(p.width, 8);
+    scaled.part = scaled.pitch * run;
+    if (p.dweight_sums != nullptr) {
+      scaled.base = room.take<uint16_t>(scaled.part * scaled.parts);
+      dw_slabs = room.take<float>(slab_floats(dw_walk(p, run), ctas_of(p.vocab)));
+    }
+    if (p.dx_sums != nullptr) {
+      int64_t most = slab_floats(dx_walk(p, run), ctas_of(run));
+      if (p.tokens % run != 0) most = std::max(most, slab_floats(dx_walk(p, p.tokens % run), ctas_of(p.tokens % run)));
+      dx_slabs = room.take<float>(most);
+    }
+  }
+  // Tokens of a run: e takes up to 480 MB (50,304 words: 18 tiles of 256 tokens, with four across one round of 72 clusters in dx), or 512
+  // tokens where that is more; of the sizes down to half of that, the one that leaves the fewest clusters idle in dx.
+  static int run_of(const Problem& p) {
+    const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(512, (480ll << 20) / row / 256 * 256);
+    return p.tokens <= most ? p.tokens : (int)(256 * best_blocks(most / 256, over(p.width, 2 * kRows)));
+  }
+  Walk logits_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.vocab, p.width, terms_of(p), ctas_of(run), false, 0); }
+  Walk dx_walk(const Problem& p, int tokens) const {
+    return walk_of(tokens, p.width, p.vocab, terms_of(p), ctas_of(tokens), true, segment_of(p));
+  }
+  Walk dw_walk(const Problem& p, int tokens) const {
+    const int terms = terms_of(p);
+    return walk_of(p.vocab, p.width, tokens, terms, ctas_of(p.vocab), true, segment_of(p), (int)over(run, kDepth) * terms);
+  }
+};
 
 }  // namespace
 
 size_t forward_bytes(const Problem& p) { return Forward(p, nullptr).room.used; }
 size_t backward_bytes(const Problem& p) { return Backward(p, nullptr).room.used; }
+size_t train_bytes(const Problem& p) { return Train(p, nullptr).room.used; }
 
 int forward(const Problem& p, cudaStream_t s) {
   WaitCtx status;
@@ -516,7 +785,112 @@ int forward(const Problem& p, cudaStream_t s) {
   st = run<kStats, false, false>(f.ctas, f.x, f.weight, f.walk, Origin{0, 0}, Origin{0, 0}, e, status, s);
   if (st != SA_OK) return st;
   return launch_after(join_kernel, dim3((unsigned)over(p.tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * f.walk.n_tiles,
-                      (const float*)f.at_target, p.targets, p.ignore_index, p.tokens, p.vocab, p.reduction, p.lse, p.loss, p.count, f.sums, f.ticket);
+                      (const float2*)f.at_target, p.targets, p.ignore_index, p.tokens, p.vocab, p.reduction,
+                      reinterpret_cast<float2*>(p.lse), p.loss, p.count, f.sums, f.ticket);
+}
+
+int train(const Problem& p, cudaStream_t s) {
+  WaitCtx status;
+  int st = wait_ctx(&status);
+  if (st != SA_OK) return st;
+  const Train t(p, p.workspace);
+  if (t.x.part != 0) st = run_convert(convert_of(p, t.x, p.x, p.x_dtype, p.x_stride), s);
+  if (st == SA_OK && t.weight.part != 0) st = run_convert(convert_of(p, t.weight, p.weight, p.weight_dtype, p.weight_stride), s);
+  if (st == SA_OK)
+    st = launch_after(reference_kernel, dim3((unsigned)over(p.tokens, 8)), 256, 0, s, p.x, p.x_dtype, p.x_stride, p.weight, p.weight_dtype,
+                      p.weight_stride, p.targets, p.ignore_index, p.tokens, p.vocab, p.width, t.ref, t.any);
+  const size_t x_bytes = bytes_of(p.x_dtype);
+  for (int n0 = 0; n0 < p.tokens && st == SA_OK; n0 += t.run) {
+    const int tokens = std::min(t.run, p.tokens - n0);
+    const bool first = n0 == 0, last = n0 + tokens == p.tokens;
+    const Walk logits = t.logits_walk(p, tokens);
+    Epilogue e{};
+    e.stats = t.stats;
+    e.at_target = t.at_target;
+    e.e_target = t.e_target;
+    e.targets = p.targets + n0;
+    e.ref = t.ref + n0;
+    e.p = const_cast<uint16_t*>(t.e.base);
+    e.p_pitch = t.e.pitch;
+    e.p_part = t.e.part;
+    e.parts = t.e.parts;
+    Rows r{};
+    r.stats = t.stats;
+    r.slots = 2 * logits.n_tiles;
+    r.at_target = t.at_target;
+    r.e_target = t.e_target;
+    r.targets = e.targets;
+    r.ignore_index = p.ignore_index;
+    r.tokens = tokens;
+    r.vocab = p.vocab;
+    r.width = p.width;
+    r.ref = t.ref + n0;
+    r.far = t.far + n0;
+    r.any = t.any;
+    r.loss = t.losses + n0;
+    r.inverse = t.inverse;
+    r.e = e.p;
+    r.e_pitch = e.p_pitch;
+    r.e_part = e.p_part;
+    r.x = static_cast<const char*>(p.x) + (size_t)n0 * p.x_stride * x_bytes;
+    r.x_dtype = p.x_dtype;
+    r.x_stride = p.x_stride;
+    r.scaled = const_cast<uint16_t*>(t.scaled.base);
+    r.scaled_pitch = t.scaled.pitch;
+    r.scaled_part = t.scaled.part;
+    r.parts = e.parts;
+    for (int again = 0; again < 2 && st == SA_OK; ++again) {       // the second time for rows that are far, where there are any
+      e.only = again ? r.far : nullptr;
+      e.any = again ? t.any : nullptr;
+      r.again = again;
+      st = run<kBoth, false, false>(ctas_of(t.run), t.x, t.weight, logits, Origin{n0, 0}, Origin{0, 0}, e, status, s);
+      if (st == SA_OK) st = launch_after(rows_kernel, dim3((unsigned)over(tokens, 32)), kJoinThreads, 0, s, (const Rows)r);
+    }
+    Operand left = t.e, right = t.scaled;
+    left.rows = right.rows = tokens;
+    if (p.dx_sums != nullptr && st == SA_OK) {
+      const int ctas = ctas_of(tokens);
+      const Walk w = t.dx_walk(p, tokens);
+      Epilogue o{};
+      o.out = p.dx_sums + (int64_t)n0 * p.width;
+      o.dtype = SA_F32;
+      o.out_pitch = p.width;
+      o.scale = t.inverse;
+      o.scale_rows = 1;
+      o.slabs = t.dx_slabs;
+      st = run<kResult, false, true>(ctas, left, t.weight, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      if (st == SA_OK) st = finish(t.dx_slabs, w, ctas, t.inverse, 1, o.out, SA_F32, p.width, s);
+    }
+    if (p.dweight_sums != nullptr && st == SA_OK) {
+      const int ctas = ctas_of(p.vocab);
+      const Walk w = t.dw_walk(p, tokens);
+      Epilogue o{};
+      o.out = p.dweight_sums;
+      o.dtype = SA_F32;
+      o.out_pitch = p.width;
+      o.addend = first ? nullptr : p.dweight_sums;
+      o.addend_pitch = p.width;
+      o.slabs = t.dw_slabs;
+      o.later = !first;
+      st = run<kResult, true, true>(ctas, left, right, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      if (st == SA_OK && last) st = finish(t.dw_slabs, w, ctas, nullptr, 0, p.dweight_sums, SA_F32, p.width, s);
+    }
+  }
+  if (st != SA_OK) return st;
+  return launch_after(total_kernel, dim3(1), 1024, 0, s, (const float*)t.losses, p.targets, p.ignore_index, p.tokens, p.reduction, p.loss, p.count);
+}
+
+int scale(const Problem& p, cudaStream_t s) {
+  int st = SA_OK;
+  const int64_t n[2] = {(int64_t)p.tokens * p.width, (int64_t)p.vocab * p.width};
+  const float* const from[2] = {p.dx_sums, p.dweight_sums};
+  void* const to[2] = {p.dx, p.dweight};
+  const int types[2] = {p.x_dtype, p.weight_dtype};
+  for (int i = 0; i < 2 && st == SA_OK; ++i)
+    if (to[i] != nullptr)
+      st = launch_after(scale_kernel, dim3((unsigned)over(over(n[i], 8), 256)), 256, 0, s, from[i], n[i], p.dloss, (const float*)p.count, p.reduction,
+                        to[i], types[i]);
+  return st;
 }
 
 int backward(const Problem& p, cudaStream_t s) {
@@ -547,7 +921,7 @@ int backward(const Problem& p, cudaStream_t s) {
     Epilogue e{};
     e.targets = p.targets;
     e.column0 = v0;
-    e.lse = p.lse;
+    e.lse = reinterpret_cast<const float2*>(p.lse);
     e.factor = b.factor;
     e.p = const_cast<uint16_t*>(b.dz.base);
     e.p_pitch = b.dz.pitch;
@@ -573,7 +947,7 @@ int backward(const Problem& p, cudaStream_t s) {
       r.slabs = b.dx_slabs;
       r.later = !first;
       st = run<kResult, false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
-      if (st == SA_OK && last) st = finish(b.dx_slabs, w, b.ctas, scale, p.dx, p.x_dtype, p.width, s);
+      if (st == SA_OK && last) st = finish(b.dx_slabs, w, b.ctas, scale, 0, p.dx, p.x_dtype, p.width, s);
       if (st != SA_OK) return st;
     }
     if (p.dweight != nullptr) {
@@ -587,7 +961,7 @@ int backward(const Problem& p, cudaStream_t s) {
       r.scale = scale;
       r.slabs = b.dw_slabs;
       st = run<kResult, true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
-      if (st == SA_OK) st = finish(b.dw_slabs, w, ctas, scale, r.out, p.weight_dtype, p.width, s);
+      if (st == SA_OK) st = finish(b.dw_slabs, w, ctas, scale, 0, r.out, p.weight_dtype, p.width, s);
     }
   }
   return st;

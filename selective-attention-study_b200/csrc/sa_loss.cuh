@@ -20,10 +20,15 @@ struct Problem {
   float *lse, *count, *loss;
   const float* dloss;
   void *dx, *dweight;           // contiguous, of x's and weight's type; either may be null
+  float *dx_sums, *dweight_sums;
   void* workspace;
 };
 size_t forward_bytes(const Problem& p);
 int forward(const Problem& p, cudaStream_t s);
+// Loss and gradients together, for one cotangent that is not known yet: sums in fp32 that `scale` turns into the gradients.
+size_t train_bytes(const Problem& p);
+int train(const Problem& p, cudaStream_t s);
+int scale(const Problem& p, cudaStream_t s);
 size_t backward_bytes(const Problem& p);
 int backward(const Problem& p, cudaStream_t s);
 

@@ -111,17 +111,23 @@ struct Origin {
   int own, depth;
 };
 
-enum Kind { kStats, kProbabilities, kResult };
+enum Kind { kStats, kProbabilities, kBoth, kResult };
 
 struct Epilogue {
   // kStats: of every row and half tile, the maximum (times log2 e) and the sum of exponentials above it; the targets' logits
   float2* stats;                           // [2 * n_tiles][m]
-  float* at_target;                        // [m], times log2 e
+  float2* at_target;                       // [m], times log2 e, in two parts
+  float* e_target;                         // kBoth: [m], the exponential
   const int64_t* targets;
   int column0;                             // of the vocabulary, that the launch's first column is
   unsigned int* zeroed;                    // kStats: a counter to be cleared for the kernel behind
+  // kBoth: exp2(z log2 e - ref) in `parts` parts, with their sum (and the maximum of z log2 e) in the place of the others'; 0 where
+  // ref is +inf
+  const float* ref;
+  const int* only;                         // rows that are not marked stay as they are; null: all are meant
+  const int* any;                          // nothing is done where this is 0; null: it is done
   // kProbabilities: (exp2(z log2 e - lse) - [target]) * factor, in `parts` 16-bit parts
-  const float* lse;
+  const float2* lse;                       // in two parts
   const float* factor;
   uint16_t* p;
   int64_t p_pitch, p_part;                 // elements of a row, of a part
@@ -134,6 +140,7 @@ struct Epilogue {
   const float* addend;                     // fp32, may be null
   int64_t addend_pitch;
   const float* scale;                      // may be null
+  int scale_rows;                          // one for every row
   float* slabs;
   int later;                               // dealt tiles add to what their slabs hold
 };
@@ -239,43 +246,34 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 
 // ---- epilogues: 32 columns of a row in registers ----------------------------------------------------------------------------------
 
-// Running maximum and sum, in log2 units.
+// Running maximum, in log2 units and rounded, and sum of exponentials above it.  The differences are taken before they are rounded:
+// a rounded logit of 100 would move its exponential by 2^-18.
 struct RowStats {
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY, from = 0.f, sum = 0.f;             // from: top * log2 e, or 0 while nothing is above -inf
   __device__ __forceinline__ void add(const uint32_t (&r)[32], int valid) {
     float z[32], best = top;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      z[i] = __uint_as_float(r[i]) * kLog2e;
-      if (i >= valid) z[i] = -INFINITY;
-    }
+    for (int i = 0; i < 32; ++i) z[i] = i < valid ? __uint_as_float(r[i]) : -INFINITY;
 #pragma unroll
     for (int i = 0; i < 32; ++i) best = fmaxf(best, z[i]);
-    const float from = best == -INFINITY ? 0.f : best;      // nothing above -inf yet: exp2(-inf - 0) is what is meant
-    sum *= ex2(top - from);
+    const float to = best == -INFINITY ? 0.f : best * kLog2e;
+    sum *= top == -INFINITY ? 0.f : ex2(from - to);
     top = best;
+    from = to;
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) part[i & 3] += ex2(z[i] - from);
+    for (int i = 0; i < 32; ++i) part[i & 3] += ex2(__fmaf_rn(z[i], kLog2e, -from));
     sum += (part[0] + part[1]) + (part[2] + part[3]);
   }
+  __device__ __forceinline__ float2 result() const { return make_float2(top == -INFINITY ? top : from, sum); }
 };
-
-__device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
-  float v = 0.f;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) v = j == i ? __uint_as_float(r[j]) : v;
-  return v;
+__device__ __forceinline__ float2 in_log2(float z) {         // z * log2 e in two parts
+  const float hi = z * kLog2e;
+  return make_float2(hi, fabsf(hi) < INFINITY ? __fmaf_rn(z, kLog2e, -hi) : 0.f);
 }
 
-// (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
-__device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int64_t at, float lse, float factor, int target) {
-  float p[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    p[i] = ex2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse));
-    p[i] = factor == 0.f ? 0.f : (i == target ? p[i] - 1.f : p[i]) * factor;   // a token that does not count: exactly nothing
-  }
+// 32 columns rounded to the parts.
+__device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], int64_t at) {
   for (int part = 0; part < e.parts; ++part) {
     uint32_t w[16];
 #pragma unroll
@@ -296,6 +294,24 @@ __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uin
       }
     }
   }
+}
+
+__device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
+  float v = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v = j == i ? __uint_as_float(r[j]) : v;
+  return v;
+}
+
+// (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
+__device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int64_t at, float2 lse, float factor, int target) {
+  float p[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    p[i] = ex2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse.x) - lse.y);
+    p[i] = factor == 0.f ? 0.f : (i == target ? p[i] - 1.f : p[i]) * factor;   // a token that does not count: exactly nothing
+  }
+  store_parts(e, p, at);
 }
 
 // 32 columns of a row in fp32, `valid` of them inside.
@@ -385,6 +401,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   wait.begin(status);
   Units u;
   u.begin(w, c);
+  if (KIND == kBoth && e.any != nullptr && *e.any == 0) u.at = w.whole;     // tiles are all whole here: nothing to do
 
   if (warp == 0) {
     if (lane == 0) {
@@ -491,11 +508,41 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int col = u.tn * w.bn + i * 32;
           stats.add(r, w.n - col);
           const int64_t mine = target - e.column0 - col;
-          if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = select(r, (int)mine) * kLog2e;
+          if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = in_log2(select(r, (int)mine));
         }
-        if (inside) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(stats.top, stats.sum);
+        if (inside) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = stats.result();
+      } else if constexpr (KIND == kBoth) {
+        const int64_t target = inside ? e.targets[row] : -1;
+        const float ref = inside ? e.ref[row] : INFINITY;
+        const bool store = inside && (e.only == nullptr || e.only[row] != 0);
+        float top = -INFINITY, sum = 0.f;
+        for (int i = from; i < to; ++i) {
+          uint32_t r[32];
+          tmem_ld32(acc + i * 32, r);
+          tmem_ld_wait();
+          const int col = u.tn * w.bn + i * 32, valid = w.n - col;
+          const int64_t mine = target - e.column0 - col;
+          float p[32], part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const bool counts = j < valid && ref != INFINITY;
+            top = j < valid ? fmaxf(top, __uint_as_float(r[j])) : top;
+            p[j] = ex2(__fmaf_rn(__uint_as_float(r[j]), kLog2e, -ref));
+            p[j] = counts ? p[j] : 0.f;
+            part[j & 3] += p[j];
+          }
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          if (store && mine >= 0 && mine < 32 && mine < valid) {
+            const float z = select(r, (int)mine);
+            e.at_target[row] = in_log2(z);
+            e.e_target[row] = ex2(__fmaf_rn(z, kLog2e, -ref));        // as it stands in the sum
+          }
+          if (store) store_parts(e, p, (int64_t)row * e.p_pitch + col);
+        }
+        if (store) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(top * kLog2e, sum);
       } else if constexpr (KIND == kProbabilities) {
-        const float lse = inside ? e.lse[row] : 0.f, factor = inside ? e.factor[row] : 0.f;
+        const float2 lse = inside ? e.lse[row] : make_float2(0.f, 0.f);
+        const float factor = inside ? e.factor[row] : 0.f;
         const int64_t target = inside ? e.targets[row] : -1;
         for (int i = from; i < to; ++i) {
           uint32_t r[32];
@@ -509,7 +556,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const bool dealt = u.tile >= w.whole;
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
         float* const slab = dealt ? e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * kColumns + in_tile) * w.bn : nullptr;
-        const float scale = e.scale != nullptr ? *e.scale : 1.f;
+        const float scale = e.scale != nullptr && inside ? e.scale[e.scale_rows ? row : 0] : 1.f;
         for (int i = from; i < to; ++i) {
           uint32_t r[32];
           tmem_ld32(acc + i * 32, r);

@@ -893,11 +893,11 @@ sa_linear_loss loss_of(const Tensor& x, const Tensor& weight, const Tensor& targ
   return p;
 }
 
-// The loss; `lse`: (tokens + 1,) what the backward needs, the last number the tokens that count.
+// The loss; `lse`: (2 tokens + 2,) what the backward needs, the last but one the number of tokens that count.
 Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore_index, int64_t reduction, int64_t product,
                 at::IntArrayRef shape, Tensor* lse) {
   const int64_t n = x.size(0);
-  *lse = fresh({n + 1}, at::kFloat, x);
+  *lse = fresh({2 * n + 2}, at::kFloat, x);
   const Tensor loss = fresh(reduction == SA_REDUCTION_NONE ? shape : at::IntArrayRef(), at::kFloat, x);
   if (n == 0) {                                     // a mean over nothing is no number
     if (reduction != SA_REDUCTION_NONE) loss.fill_(reduction == SA_REDUCTION_MEAN ? std::nan("") : 0.0);
@@ -905,7 +905,7 @@ Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, in
   }
   sa_linear_loss p = loss_of(x, weight, targets, ignore_index, reduction, product);
   p.lse = lse->data_ptr<float>();
-  p.count = p.lse + n;
+  p.count = p.lse + 2 * n;
   p.loss = loss.data_ptr<float>();
   p.workspace_bytes = sa_linear_loss_forward_bytes(&p);
   const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
@@ -913,6 +913,80 @@ Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, in
   check("sa_linear_loss_forward", sa_linear_loss_forward(&p));
   return loss;
 }
+
+// The loss with its gradients up to the cotangent, where that is one number and the operands' exponents allow it: a product less than
+// computing the logits again.
+bool gradients_with_loss(int64_t reduction, int64_t product) { return reduction != SA_REDUCTION_NONE && product != SA_F16; }
+
+struct LinearLossTrained : public torch::autograd::Function<LinearLossTrained> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& targets, int64_t ignore_index, int64_t reduction,
+                        int64_t product) {
+    const c10::cuda::CUDAGuard guard(x_in.device());
+    const Tensor x = rows_in(x_in), weight = rows_in(weight_in);
+    const Tensor loss = fresh({}, at::kFloat, x), count = fresh({1}, at::kFloat, x);
+    Tensor dx, dweight;
+    if (x_in.requires_grad()) dx = fresh(x_in.sizes(), at::kFloat, x);
+    if (weight_in.requires_grad()) dweight = fresh(weight_in.sizes(), at::kFloat, x);
+    if (x.size(0) == 0) {                             // a mean over nothing is no number
+      loss.fill_(reduction == SA_REDUCTION_MEAN ? std::nan("") : 0.0);
+      count.zero_();
+      if (dweight.defined()) dweight.zero_();
+    } else {
+      sa_linear_loss p = loss_of(x, weight, targets, ignore_index, reduction, product);
+      p.loss = loss.data_ptr<float>();
+      p.count = count.data_ptr<float>();
+      p.dx_sums = static_cast<float*>(pointer(dx));
+      p.dweight_sums = static_cast<float*>(pointer(dweight));
+      p.workspace_bytes = sa_linear_loss_train_bytes(&p);
+      const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
+      p.workspace = workspace.data_ptr();
+      check("sa_linear_loss_train", sa_linear_loss_train(&p));
+    }
+    ctx->save_for_backward({dx, dweight, count});
+    ctx->saved_data["args"] = packed({reduction, product, (int64_t)x.scalar_type(), (int64_t)weight.scalar_type()});
+    ctx->saved_data["tokens"] = x.size(0);
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["width"] = weight.size(1);
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad_out) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t all = ctx->saved_data["args"].toInt();
+    variable_list grads(6);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor dx_sums = saved[0].defined() ? in_order(saved[0]) : saved[0], dweight_sums = saved[1].defined() ? in_order(saved[1]) : saved[1];
+      const Tensor count = in_order(saved[2]);
+      const c10::cuda::CUDAGuard guard(count.device());
+      const Tensor dloss = in_order(in_type(grad_out[0], at::kFloat));
+      const auto x_type = (at::ScalarType)packed_at(all, 2), weight_type = (at::ScalarType)packed_at(all, 3);
+      if (dx_sums.defined() && ctx->needs_input_grad(0)) grads[0] = fresh(dx_sums.sizes(), x_type, dx_sums);
+      if (dweight_sums.defined() && ctx->needs_input_grad(1)) grads[1] = fresh(dweight_sums.sizes(), weight_type, dweight_sums);
+      sa_linear_loss p{};
+      p.struct_bytes = sizeof(sa_linear_loss);
+      p.reduction = (int32_t)packed_at(all, 0);
+      p.product = (int32_t)packed_at(all, 1);
+      p.x_dtype = code_of(x_type);
+      p.weight_dtype = code_of(weight_type);
+      p.tokens = (int32_t)ctx->saved_data["tokens"].toInt();
+      p.vocab = (int32_t)ctx->saved_data["vocab"].toInt();
+      p.width = (int32_t)ctx->saved_data["width"].toInt();
+      if (p.tokens == 0) {
+        if (grads[1].defined()) grads[1].zero_();
+      } else if (grads[0].defined() || grads[1].defined()) {
+        p.count = count.data_ptr<float>();
+        p.dloss = dloss.data_ptr<float>();
+        p.dx_sums = static_cast<float*>(pointer(dx_sums));
+        p.dweight_sums = static_cast<float*>(pointer(dweight_sums));
+        p.dx = pointer(grads[0]);
+        p.dweight = pointer(grads[1]);
+        p.stream = stream_of(count);
+        check("sa_linear_loss_scale", sa_linear_loss_scale(&p), true);
+      }
+    }
+    return once_differentiable(grad_out, std::move(grads));
+  }
+};
 
 struct LinearLoss : public torch::autograd::Function<LinearLoss> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore_index, int64_t reduction,
@@ -931,7 +1005,9 @@ struct LinearLoss : public torch::autograd::Function<LinearLoss> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::cuda::CUDAGuard guard(saved[0].device());
-      const Tensor x = rows_in(saved[0]), weight = rows_in(saved[1]), targets = in_order(saved[2]), lse = in_order(saved[3]);
+      const Tensor x = rows_in(saved[0]), weight = rows_in(saved[1]), targets = in_order(saved[2]);
+      Tensor lse = in_order(saved[3]);
+      if (reinterpret_cast<uintptr_t>(lse.data_ptr()) % 8 != 0) lse = lse.clone();        // from a hook on saved tensors
       const Tensor dloss = in_order(in_type(grad_out[0], at::kFloat));
       if (ctx->needs_input_grad(0)) grads[0] = fresh(saved[0].sizes(), saved[0].scalar_type(), saved[0]);
       if (ctx->needs_input_grad(1)) grads[1] = fresh(saved[1].sizes(), saved[1].scalar_type(), saved[1]);
@@ -940,7 +1016,7 @@ struct LinearLoss : public torch::autograd::Function<LinearLoss> {
       } else if (grads[0].defined() || grads[1].defined()) {
         sa_linear_loss p = loss_of(x, weight, targets, args[0], args[1], args[2]);
         p.lse = lse.data_ptr<float>();
-        p.count = p.lse + x.size(0);
+        p.count = p.lse + 2 * x.size(0);
         p.dloss = dloss.data_ptr<float>();
         p.dx = pointer(grads[0]);
         p.dweight = pointer(grads[1]);
@@ -975,7 +1051,10 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
                     ": autocast to ", name_of(product), " needs x and weight in that dtype");
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor targets = indices_in(targets_in);
-  if (c10::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
+  const bool train = c10::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad());
+  if (train && gradients_with_loss(reduction, code_of(product)))
+    return LinearLossTrained::apply(x, weight, targets, ignore_index, reduction, (int64_t)code_of(product));
+  if (train)
     return LinearLoss::apply(x, weight, targets, ignore_index, reduction, (int64_t)code_of(product), targets_in.sizes());
   Tensor lse;
   return run_loss(rows_in(x), rows_in(weight), targets, ignore_index, reduction, code_of(product), targets_in.sizes(), &lse);

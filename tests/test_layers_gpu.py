@@ -267,9 +267,12 @@ def _check_loss(x, w, targets, reduction, ignore=-100, product=None, seed=0):
         _check("loss", loss.detach(), total, off_loss.sum() / (counts if reduction == "mean" else 1))
     ok = _half_step(product) if product != F32 else 2.0 ** -22                      # the rounding of dz
     g_max = float(g.abs().max())
-    lost = 2.0 ** -39 * g_max if product == F16 else 0.0                            # fp16: half the smallest step, over 2^14
-    each = dz.abs() * (ok + 2 * off[:, None] + 2.0 ** -20) + g.abs()[:, None] * (targets.flatten() != ignore)[:, None] * \
-        torch.zeros_like(dz).scatter_(1, torch.where(targets.flatten() != ignore, targets.flatten(), 0)[:, None], 2.0 ** -23) + lost
+    lost = (2.0 ** -39 if product == F16 else 2.0 ** -126) * g_max                  # fp16: half the smallest step, over 2^14; exponentials below 2^-126 are 0
+    # beside what is relative to dz: at the target, p - 1 of a p near 1 has the whole error of p, which is an exponential of 2^-22 (the
+    # instruction's bound is 2^-22.5) over a sum of such exponentials: 2^-21
+    counts = targets.flatten() != ignore
+    at_target = torch.zeros_like(dz).scatter_(1, torch.where(counts, targets.flatten(), 0)[:, None], 2.0 ** -21)
+    each = dz.abs() * (ok + 2 * off[:, None] + 2.0 ** -20) + (g.abs() * counts)[:, None] * at_target + lost
 
     def around(a, abs_a, e, b, k):
         many = (-(-k // 64) * 4 + 70) if product != F32 else 32 * 4 + 200           # groups in one sum; fp32 leaves tensor memory every 2,048
@@ -277,6 +280,8 @@ def _check_loss(x, w, targets, reduction, ignore=-100, product=None, seed=0):
 
     want, slack = around(dz, dz.abs(), each, rw.detach().double(), vocab)
     _check("dx", dx.reshape(-1, width), want, slack)
+    if reduction != "none" and product != F16:              # one cotangent: x over the sum of exponentials is rounded too
+        each = each + dz.abs() * ok
     want, slack = around(dz.T, dz.T.abs(), each.T, rx.detach().double(), n)
     _check("dw", dw, want, slack)
     assert _lib.device_status() == 0
@@ -303,14 +308,35 @@ def test_loss_and_its_gradients(tokens, vocab, width, reduction, dtype):
     _check_loss(x, w, targets, reduction)
 
 
-def test_loss_in_several_pieces_of_the_vocabulary():
-    """More than 256 MB of logits' gradients in 16 bits."""
+@pytest.mark.parametrize("dtype,tokens,vocab,width,reduction", [
+    (BF16, 9000, 40000, 64, "none"), (F32, 5000, 12000, 72, "none"), (F16, 9000, 40000, 64, "mean"),      # pieces of the vocabulary
+    (BF16, 9000, 40000, 64, "mean"), (F32, 5000, 12000, 72, "sum"), (BF16, 1500, 262144, 16, "mean")])    # runs of tokens
+def test_loss_in_several_parts(dtype, tokens, vocab, width, reduction):
+    """More logits than the workspace holds at a time: 320 to 480 MB in 16 bits."""
     gen = _gen(11)
-    for dtype, tokens, vocab, width in ((BF16, 9000, 40000, 64), (F32, 5000, 12000, 72)):
-        x = torch.randn(tokens, width, device="cuda").to(dtype)
-        w = (torch.randn(vocab, width, device="cuda") * 0.3).to(dtype)
-        targets = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
-        _check_loss(x, w, targets, "mean")
+    x = torch.randn(tokens, width, device="cuda").to(dtype)
+    w = (torch.randn(vocab, width, device="cuda") * 0.3).to(dtype)
+    targets = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
+    targets[5::11] = -100
+    _check_loss(x, w, targets, reduction)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_targets_that_are_all_but_impossible(dtype):
+    """Losses beyond 44, where exponentials over the target's leave their range: the rows go through the product once more."""
+    gen = _gen(31)
+    x, w = _randn(gen, 300, 72, dtype=dtype), _randn(gen, 900, 72, dtype=dtype, scale=4.0)
+    targets = torch.randint(0, 900, (300,), generator=gen).cuda()
+    targets[::9] = -100
+    z = x.double() @ w.double().T
+    targets[1::9] = z[1::9].argmin(1)                       # up to 200
+    targets[2::9] = z[2::9].argmax(1)
+    losses = layers.linear_cross_entropy(x, w, targets, reduction="none")
+    assert float(losses.max()) > 100 and int((losses > 44).sum()) > 30 and int((losses < 1).sum()) > 30
+    for reduction in ("sum", "none"):
+        _check_loss(x, w, targets, reduction)
+    far = torch.full_like(targets[:1], int(z[1].argmin()))
+    _check_loss(x[1:2], w, far, "mean")
 
 
 def test_loss_of_batches_strides_and_padding():
@@ -544,7 +570,7 @@ def test_saved_tensors_may_be_moved_and_hooks_see_them():
 def test_a_tensor_that_was_changed_since_is_noticed_and_a_second_derivative_is_refused():
     idx, table, weight, targets = _step_inputs(27)
     table.requires_grad_(True)
-    loss = layers.linear_cross_entropy(layers.embedding(idx, table), table, targets)
+    loss = layers.linear_cross_entropy(layers.embedding(idx, table), table, targets, reduction="none").sum()
     with torch.no_grad():
         table.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
