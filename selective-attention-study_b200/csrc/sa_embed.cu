@@ -52,7 +52,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const sa_embedding p,
 }
 
 // sorted: (token, row) by row; starts: where each row's tokens begin, and the number of all behind them.
-__global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx, int tokens, int vocab, int rows, int2* sorted, int* starts) {
+__global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx, int64_t skip, int tokens, int vocab, int rows, int2* sorted,
+                                                              int* starts) {
   tc::after_previous_kernel();
   extern __shared__ int counts[];                                  // [rows][warps]
   __shared__ int before_s[kOrderWarps];
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx
   int before = 0;                                                  // tokens of earlier rows
 #pragma unroll 8
   for (int n = from + lane; n < to; n += 32) {
-    const int64_t v = idx[n];
+    const int64_t v = idx[n] == skip ? -1 : idx[n];
     if (v >= 0 && v < lo) ++before;
     if (v >= lo && v < hi) atomicAdd(&counts[(int)(v - lo) * kOrderWarps + warp], 1);
   }
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx
     for (int k = 0; k < kAhead; ++k) {
       const int n = n0 + 32 * k + lane;
       const int64_t v = n < to ? idx[n] : -1;
-      row[k] = v >= lo && v < hi ? (int)(v - lo) : -1;
+      row[k] = v >= lo && v < hi && v != skip ? (int)(v - lo) : -1;
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -149,10 +150,12 @@ struct Sum {
   const void* dy;
   int dtype;                               // of dy
   int64_t dy_stride;
+  const float* factor;                     // of its rows, or null
   void* dweight;
   int weight_dtype;
   float scale;
   int vocab, width, chunks, groups;        // chunks of 8 values in a row; rows that a CTA works on side by side
+  bool add;                                // to what stands in dweight, fp32
   float* parts;                            // [pieces][2][width]: of a row that began before the piece, of one that goes on behind it
   int pieces;
 };
@@ -203,6 +206,12 @@ __device__ __forceinline__ void finish_row(const Sum& p, int row, int t, const f
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = x[i] * p.scale;
+  if (p.add) {
+    float old[8];
+    read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)row * p.width, t, old);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] += old[i];
+  }
   write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)row * p.width, t, y);
 }
 
@@ -236,8 +245,9 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (at[k].y < 0) continue;
+      const float factor = p.factor != nullptr ? p.factor[at[k].x] : 1.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += x[k][i];
+      for (int i = 0; i < 8; ++i) sum[i] = fmaf(factor, x[k][i], sum[i]);
       if ((k + 1 < kAhead ? at[k + 1 < kAhead ? k + 1 : k].y : next) == at[k].y) continue;
       const int begin = p.starts[at[k].y], end = p.starts[at[k].y + 1];
       if (begin >= from && end <= from + kPiece) finish_row<VEC>(p, at[k].y, t, sum);
@@ -282,14 +292,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
 }
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-int pieces_of(const sa_embedding& p) { return (p.tokens + kPiece - 1) / kPiece; }
-int order_rows(const sa_embedding& p) { return std::min((p.vocab + kSms - 1) / kSms, kMostRows); }
+int pieces_of(int tokens) { return (tokens + kPiece - 1) / kPiece; }
 
 }  // namespace
 
-size_t backward_bytes(const sa_embedding& p) {
-  return (size_t)(up((int64_t)p.tokens * 8, 256) + up(((int64_t)p.vocab + 1) * 4, 256) + (int64_t)pieces_of(p) * 2 * p.width * 4);
+size_t sum_rows_bytes(int tokens, int vocab, int width) {
+  return (size_t)(up((int64_t)tokens * 8, 256) + up(((int64_t)vocab + 1) * 4, 256) + (int64_t)pieces_of(tokens) * 2 * width * 4);
 }
+size_t backward_bytes(const sa_embedding& p) { return sum_rows_bytes(p.tokens, p.vocab, p.width); }
 
 int forward(const sa_embedding& p, cudaStream_t s) {
   const int chunks = (p.width + 7) / 8;
@@ -298,24 +308,28 @@ int forward(const sa_embedding& p, cudaStream_t s) {
   return vec ? launch_after(forward_kernel<true>, grid, kThreads, 0, s, p, chunks) : launch_after(forward_kernel<false>, grid, kThreads, 0, s, p, chunks);
 }
 
-int backward(const sa_embedding& p, cudaStream_t s) {
+int sum_rows(const RowSums& p, cudaStream_t s) {
   char* room = static_cast<char*>(p.workspace);
   int2* sorted = reinterpret_cast<int2*>(room);
   int* starts = reinterpret_cast<int*>(room + up((int64_t)p.tokens * 8, 256));
   float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(starts) + up(((int64_t)p.vocab + 1) * 4, 256));
-  const int rows = order_rows(p);
-  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.tokens, p.vocab, rows,
-                        sorted, starts);
+  const int rows = std::min((p.vocab + kSms - 1) / kSms, kMostRows);
+  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.skip, p.tokens,
+                        p.vocab, rows, sorted, starts);
   if (st != SA_OK) return st;
-  Sum a{sorted, starts, p.dy, p.y_dtype, p.dy_stride, p.dweight, p.weight_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p)};
+  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, p.add, parts, pieces_of(p.tokens)};
   a.groups = a.chunks < kThreads ? kThreads / a.chunks : 1;
-  const bool vec = p.width % 8 == 0 && eights(p.dy, p.y_dtype, p.dy_stride, p.tokens) && eights(p.dweight, p.weight_dtype, p.width, p.vocab);
+  const bool vec = p.width % 8 == 0 && eights(p.dy, p.dtype, p.dy_stride, p.tokens) && eights(p.out, p.out_dtype, p.width, p.vocab);
   const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;
-  const dim3 grid(piece_blocks + (p.vocab + kZeroRows - 1) / kZeroRows, (a.chunks + kThreads - 1) / kThreads);
+  const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + kZeroRows - 1) / kZeroRows), (a.chunks + kThreads - 1) / kThreads);
   st = vec ? launch_after(sum_kernel<true>, grid, kThreads, 0, s, a, piece_blocks) : launch_after(sum_kernel<false>, grid, kThreads, 0, s, a, piece_blocks);
   if (st != SA_OK || a.pieces < 2) return st;
   const dim3 join(a.pieces - 1, (a.chunks + kJoinThreads - 1) / kJoinThreads);
   return vec ? launch_after(join_kernel<true>, join, kJoinThreads, 0, s, a) : launch_after(join_kernel<false>, join, kJoinThreads, 0, s, a);
+}
+
+int backward(const sa_embedding& p, cudaStream_t s) {
+  return sum_rows(RowSums{p.idx, INT64_MIN, p.tokens, p.vocab, p.width, p.dy, p.y_dtype, p.dy_stride, nullptr, p.scale, p.dweight, p.weight_dtype, false, p.workspace}, s);
 }
 
 }  // namespace embed

@@ -14,6 +14,23 @@ int backward(const sa_norm& p, cudaStream_t s);
 }  // namespace norm
 
 namespace embed {
+// out[v] = scale * the sum of factor[n] * dy[n] over the n with idx[n] = v, in their order, or that added to fp32 rows.
+struct RowSums {
+  const int64_t* idx;           // those outside [0, vocab), and `skip`, have no part
+  int64_t skip;
+  int tokens, vocab, width;
+  const void* dy;
+  int dtype;
+  int64_t dy_stride;
+  const float* factor;          // null: 1
+  float scale;
+  void* out;                    // (vocab, width), contiguous
+  int out_dtype;
+  bool add;
+  void* workspace;              // sum_rows_bytes(), 16-byte aligned
+};
+size_t sum_rows_bytes(int tokens, int vocab, int width);
+int sum_rows(const RowSums& r, cudaStream_t s);
 size_t backward_bytes(const sa_embedding& p);
 int forward(const sa_embedding& p, cudaStream_t s);
 int backward(const sa_embedding& p, cudaStream_t s);

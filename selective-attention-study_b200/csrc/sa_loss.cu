@@ -7,8 +7,9 @@
 //
 // Training with a sum or a mean (bf16 and fp32 products): the cotangent is one number, so the gradients are computed with the loss,
 // up to that number, and no logit twice.  Tokens come in runs; of a run, the product's epilogue keeps e = exp(z - ref) in 16 bits
-// beside the rows' sums s.  softmax(z) = e / s, so the rest is a scale of rows: of the result in dx = (1 / s) e W, and of the
-// right operand in dW = e^T (x / s).  ref is the target's logit, a dot product beforehand: e = 1 at the target and at most
+// beside the rows' sums s.  softmax(z) = e / s, so the rest is a scale of rows, of the result in dx = (1 / s) e W and of the
+// right operand in dW = e^T (x / s).  e is 0 at the target: its part, c = softmax - 1, is added in fp32, dx_n += c W_t and dW_t +=
+// the sum of c x_n over its tokens, sorted as in an embedding's gradient.  ref is the target's logit, a dot product beforehand: exp(z - ref) is 1 at the target and at most
 // e^loss elsewhere, which 8 bits of exponent hold with room for 1 / s up to a loss of 44.  Rows beyond that are found by the sums
 // and go through the product once more with their maximum for ref.  Three products of 2 N V d operations; the sums of dW over the runs stay in fp32.
 //
@@ -19,6 +20,7 @@
 
 #include <algorithm>
 
+#include "sa_layers.cuh"
 #include "sa_product.cuh"
 
 namespace sa {
@@ -48,43 +50,6 @@ struct Convert {
   float *factor, *scale;
 };
 
-__device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t at) {
-  if (dtype == SA_F32) return static_cast<const float*>(p)[at];
-  if (dtype == SA_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
-  return __half2float(static_cast<const __half*>(p)[at]);
-}
-
-// Eight values of a row from column `col` on, zeros behind the width.
-__device__ __forceinline__ void load_columns(const void* base, int dtype, int64_t row_at, int col, int width, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  const int64_t at = row_at + col;
-  const char* src = static_cast<const char*>(base) + at * (dtype == SA_F32 ? 4 : 2);
-  if (col + 8 <= width && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    if (dtype == SA_F32) {
-      const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      return;
-    }
-    const uint4 a = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (dtype == SA_BF16) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < width) v[i] = load_as_float(base, dtype, at + i);
-}
 // Eight values in `parts` parts of 16 bits, each what the ones before it leave.
 __device__ __forceinline__ void store_columns(uint16_t* dst, int64_t part_stride, int parts, int half, float (&v)[8]) {
   for (int part = 0; part < parts; ++part) {
@@ -278,6 +243,7 @@ struct Rows {                              // of a run of tokens
   int again;                               // they have been through the product once more
   float* loss;
   float* inverse;                          // 1 / s, 0 for a token that does not count
+  float* less;                             // softmax - 1 at the target, in fp32; e is 0 there
   uint16_t* e;
   int64_t e_pitch, e_part;
   const void* x;
@@ -289,7 +255,7 @@ struct Rows {                              // of a run of tokens
 };
 constexpr float kFarthest = 18446744073709551616.f;      // 2^64
 
-// Sums of 32 tokens; their losses, e at the target less s (e - s is s times softmax - 1), and x / s.
+// Sums of 32 tokens, their losses, and x / s.
 __global__ void __launch_bounds__(kJoinThreads) rows_kernel(const Rows r) {
   after_previous_kernel();
   if (r.again && *r.any == 0) return;
@@ -333,22 +299,18 @@ __global__ void __launch_bounds__(kJoinThreads) rows_kernel(const Rows r) {
     }
     float inverse = 0.f;
     if (now) {
-      float loss = 0.f;
+      float loss = 0.f, at_target = 0.f;
       if (counts) {
         const float ref = r.ref[row];
         inverse = good ? 1.f / sum : NAN;
         const float e = r.e_target[row];
         loss = !good ? NAN : (e > 1.f / kFarthest ? log2f(sum / e) : (ref - r.at_target[row].x) + log2f(sum)) * kLn2;
-        if (good) {
-          float at = e - sum;
-          for (int part = 0; part < r.parts; ++part) {
-            const __nv_bfloat16 b = __float2bfloat16_rn(at);
-            r.e[part * r.e_part + (int64_t)row * r.e_pitch + t] = __bfloat16_as_ushort(b);
-            at -= __bfloat162float(b);
-          }
-        }
+        at_target = good ? (e - sum) * inverse : NAN;
+        if (good)
+          for (int part = 0; part < r.parts; ++part) r.e[part * r.e_part + (int64_t)row * r.e_pitch + t] = 0;
       }
       r.loss[row] = loss;
+      r.less[row] = at_target;
       r.inverse[row] = inverse;
     }
     inverse_s[lane] = inverse;
@@ -431,37 +393,45 @@ __global__ void __launch_bounds__(256) scale_kernel(const float* sums, int64_t n
   }
 }
 
-// Rows of a dealt tile from its slabs, in order: a thread has four columns of a row, four slabs in flight.
+// Rows of a cut tile from its slabs, in order: a thread has four columns of a row, four slabs in flight.
 constexpr int kFinishThreads = 256;
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const float* slabs, const Walk w, int tile_rows, const float* scale, int scale_rows,
-                                                                void* out, int dtype, int64_t out_pitch) {
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Epilogue e, const Walk w, int tile_rows) {
   after_previous_kernel();
-  const int tile = w.whole + blockIdx.x;
   int tm, tn;
-  w.place(tile, &tm, &tn);
-  const int n = w.slabs_of(tile), columns = min(w.bn, w.n - tn * w.bn), across = w.bn >> 2;
+  w.place(w.whole + blockIdx.x, &tm, &tn);
+  const int columns = min(w.bn, w.n - tn * w.bn), across = w.bn >> 2;
   const int in_tile = blockIdx.y * (kFinishThreads / across) + threadIdx.x / across, c = (threadIdx.x % across) * 4, row = tm * tile_rows + in_tile;
   if (row >= w.m || c >= columns) return;
-  const float by = scale != nullptr ? scale[scale_rows ? row : 0] : 1.f;
-  const float4* from = reinterpret_cast<const float4*>(slabs + ((int64_t)blockIdx.x * w.slabs * tile_rows + in_tile) * w.bn + c);
+  const float by = e.scale != nullptr ? e.scale[e.scale_rows ? row : 0] : 1.f;
+  const float4* from = reinterpret_cast<const float4*>(e.slabs + ((int64_t)blockIdx.x * w.slabs * tile_rows + in_tile) * w.bn + c);
   const int64_t stride = (int64_t)tile_rows * w.bn / 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = 0; k < n; ++k) {
+  for (int k = 0; k < w.slabs; ++k) {
     const float4 x = from[k * stride];
     v.x += x.x;
     v.y += x.y;
     v.z += x.z;
     v.w += x.w;
   }
-  const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
-  const int64_t at = (int64_t)row * out_pitch + tn * w.bn + c;
+  float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+  const int col = tn * w.bn + c;
+  if (e.table != nullptr && e.table_factor[row] != 0.f) {
+    const int64_t t = e.targets[row];
+    if (t >= 0 && t < e.vocab) {
+      float x[8];
+      load_columns(e.table, e.table_dtype, t * e.table_stride, col, w.n, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = fmaf(e.table_factor[row], x[i], f[i]);
+    }
+  }
+  const int64_t at = (int64_t)row * e.out_pitch + col;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (c + i >= columns) break;
-    if (dtype == SA_F32) static_cast<float*>(out)[at + i] = f[i];
-    else if (dtype == SA_BF16) static_cast<__nv_bfloat16*>(out)[at + i] = __float2bfloat16_rn(f[i]);
-    else static_cast<__half*>(out)[at + i] = __float2half_rn(f[i]);
+    if (e.dtype == SA_F32) static_cast<float*>(e.out)[at + i] = f[i];
+    else if (e.dtype == SA_BF16) static_cast<__nv_bfloat16*>(e.out)[at + i] = __float2bfloat16_rn(f[i]);
+    else static_cast<__half*>(e.out)[at + i] = __float2half_rn(f[i]);
   }
 }
 
@@ -496,33 +466,32 @@ struct Operand {
   int map(CUtensorMap* m, bool mn_major) const { return make_map(m, base, width, rows, parts, pitch, part, mn_major ? 64 : kRows); }
 };
 
-// The walk over an m x n result of contraction `depth`.  `shared`: what is left over of whole rounds is dealt out where it would
-// leave clusters idle, which costs slabs; then a row's tiles stand side by side, since their left operand, dz, comes from
-// memory and is to be read once.  `ticks`: as in the launch whose slabs this one adds to (0: the first).
-Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool shared, int segment, int ticks = 0) {
+// The walk over an m x n result of contraction `depth`.  `result`: a product of dz, which comes from memory: a row's tiles stand side by
+// side, so that it is read once, and what is left of whole rounds may be cut, in parts of at least eight stages of `longest`, the
+// longest contraction of the launches that add to the same slabs.  (Dealing all stages out evenly, without regard to depth,
+// kept 72 clusters busy where 40 whole tiles keep 40, and took 237 us instead of 215: every tile read dz for itself.)
+Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int64_t longest = 0) {
   Walk w{};
   w.m = m;
   w.n = n;
-  w.bn = kRows * ctas;
+  w.bn = kRows * (result && terms > 1 ? 1 : ctas);                 // kSegments: as many sums as a thread's registers hold
   w.m_tiles = (int)over(m, kRows * ctas);
   w.n_tiles = (int)over(n, w.bn);
   w.depth_blocks = (int)over(depth, kDepth);
   w.blocks = w.depth_blocks * terms;
-  w.ticks = ticks > 0 ? ticks : w.blocks;
   w.whole = w.tiles();
   w.slabs = 1;
   const int most = kSms / ctas;
   w.clusters = std::min(w.tiles(), most);
-  w.segment = segment > 0 ? std::min(segment, w.blocks) : w.blocks;
-  w.group = shared ? 1 : std::min(w.m_tiles, 8);
+  w.segment = result && terms > 1 ? kSegment : w.blocks;
+  w.group = result ? 1 : std::min(w.m_tiles, 8);
   const int left = w.tiles() % most;
-  if (shared && left * 100 < 88 * most && left > 0) {
-    const int64_t stages = (int64_t)left * w.ticks;
-    const int c = (int)std::min<int64_t>(most, stages / 8);                                // at least eight stages each
-    if (c > left && (c == most || w.tiles() < most)) {
+  if (result && left > 0) {
+    const int parts = (int)std::min<int64_t>(most / left, over(longest, kDepth) * terms / 8);
+    if (parts > 1) {
       w.whole -= left;
-      w.clusters = c;
-      w.slabs = (int)((w.ticks - 1) / (stages / c)) + 2;
+      w.slabs = parts;
+      w.clusters = std::max(w.clusters, std::min(most, left * parts));
     }
   }
   return w;
@@ -569,8 +538,6 @@ int ctas_of(int rows) { return rows > kRows ? 2 : 1; }
 int parts_of(const Problem& p) { return p.product == SA_F32 ? 3 : 1; }
 int terms_of(const Problem& p) { return p.product == SA_F32 ? kTerms : 1; }
 size_t bytes_of(int dtype) { return dtype == SA_F32 ? 4 : 2; }
-// Sums of fp32 operands leave tensor memory every 2,048 of the contraction: its additions round towards zero.
-int segment_of(const Problem& p) { return p.product == SA_F32 ? 32 : 0; }
 
 bool in_place(int dtype, int product, const void* base, int64_t stride, int64_t rows, int64_t width) {
   return product != SA_F32 && dtype == product && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && stride % 8 == 0 && (stride >= width || rows == 1);
@@ -617,6 +584,15 @@ Convert convert_of(const Problem& p, const Operand& o, const void* src, int dtyp
   c.dst = const_cast<uint16_t*>(o.base);
   return c;
 }
+// The same values as one matrix of a plain type: as the products have them, or, of three parts, as they were given.
+struct Matrix {
+  const void* base;
+  int dtype;
+  int64_t stride;
+};
+Matrix matrix_of(const Problem& p, const Operand& o, const void* given, int dtype, int64_t stride) {
+  return o.parts == 1 ? Matrix{o.base, p.product, o.pitch} : Matrix{given, dtype, stride};
+}
 int run_convert(const Convert& c, cudaStream_t s) {
   return launch_after(convert_kernel, dim3((unsigned)over((int64_t)c.rows * (c.pitch >> 3), 256)), 256, 0, s, c);
 }
@@ -632,27 +608,13 @@ struct Forward {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
     ctas = ctas_of(p.tokens);
-    walk = walk_of(p.tokens, p.vocab, p.width, terms_of(p), ctas, false, 0);
+    walk = walk_of(p.tokens, p.vocab, p.width, terms_of(p), ctas, false);
     stats = room.take<float2>((int64_t)2 * walk.n_tiles * p.tokens);
     sums = room.take<float2>(over(p.tokens, 32));
     at_target = room.take<float2>(p.tokens);
     ticket = room.take<unsigned int>(1);
   }
 };
-
-// Of `most` row tiles down to half as many, with `across` tiles a row: how many leave the fewest clusters idle.
-int64_t best_blocks(int64_t most, int64_t across) {
-  const int64_t clusters = kSms / 2;
-  int64_t best = 0, at = most;
-  for (int64_t b = most; 2 * b > most; --b) {
-    const int64_t tiles = b * across, used = tiles * 1000 / (over(tiles, clusters) * clusters);
-    if (used > best) {
-      best = used;
-      at = b;
-    }
-  }
-  return at;
-}
 
 struct Backward {
   Room room;
@@ -690,30 +652,44 @@ struct Backward {
   static int piece_of(const Problem& p) {
     const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>(4096, (320ll << 20) / column / 256 * 256);
     if (p.vocab <= most) return p.vocab;
-    return (int)(256 * best_blocks(most / 256, over(p.width, 2 * kRows)));
+    const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
+    int64_t best = 0, at = blocks;
+    for (int64_t b = blocks; 2 * b > blocks; --b) {
+      const int64_t tiles = b * across, used = tiles * 1000 / (over(tiles, clusters) * clusters);
+      if (used > best) {
+        best = used;
+        at = b;
+      }
+    }
+    return (int)(at * 256);
   }
-  Walk dx_walk(const Problem& p, int columns) const {
-    const int terms = terms_of(p);
-    return walk_of(p.tokens, p.width, columns, terms, ctas, true, segment_of(p), (int)over(piece, kDepth) * terms);
-  }
+  Walk dx_walk(const Problem& p, int columns) const { return walk_of(p.tokens, p.width, columns, terms_of(p), ctas, true, piece); }
   Walk dw_walk(const Problem& p, int columns) const {
-    return walk_of(columns, p.width, p.tokens, terms_of(p), ctas_of(columns), true, segment_of(p));
+    return walk_of(columns, p.width, p.tokens, terms_of(p), ctas_of(columns), true, p.tokens);
   }
 };
 
-int finish(const float* slabs, const Walk& w, int ctas, const float* scale, int scale_rows, void* out, int dtype, int64_t pitch, cudaStream_t s) {
+int finish(const Epilogue& e, const Walk& w, int ctas, cudaStream_t s) {
   if (w.whole == w.tiles()) return SA_OK;
   const int rows = kFinishThreads / (w.bn >> 2);                  // bn: 128 or 256
-  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, slabs, w, kRows * ctas, scale, scale_rows, out, dtype,
-                      pitch);
+  return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, (const Epilogue)e, (const Walk)w, kRows * ctas);
+}
+
+// A product into a result, by kResult or, for fp32 operands, kSegments.
+template <bool A_MN, bool B_MN>
+int run_result(const Problem& p, int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, const Epilogue& e,
+               const WaitCtx& status, cudaStream_t s) {
+  return p.product == SA_F32 ? run<kSegments, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s)
+                             : run<kResult, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s);
 }
 
 struct Train {
   Room room;
   Operand x, weight, e, scaled;
   int run;                       // tokens of a run
-  float *ref, *losses, *e_target, *inverse, *dx_slabs = nullptr, *dw_slabs = nullptr;
+  float *ref, *losses, *less, *e_target, *inverse, *dx_slabs = nullptr, *dw_slabs = nullptr;
   int *far, *any;
+  void* sorted = nullptr;        // of the targets
   float2 *stats, *at_target;
   Train(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
@@ -721,6 +697,7 @@ struct Train {
     run = run_of(p);
     ref = room.take<float>(p.tokens);
     losses = room.take<float>(p.tokens);
+    less = room.take<float>(p.tokens);
     far = room.take<int>(p.tokens);
     any = room.take<int>(1);
     at_target = room.take<float2>(run);
@@ -739,6 +716,7 @@ struct Train {
     if (p.dweight_sums != nullptr) {
       scaled.base = room.take<uint16_t>(scaled.part * scaled.parts);
       dw_slabs = room.take<float>(slab_floats(dw_walk(p, run), ctas_of(p.vocab)));
+      sorted = room.take<char>((int64_t)embed::sum_rows_bytes(p.tokens, p.vocab, p.width));
     }
     if (p.dx_sums != nullptr) {
       int64_t most = slab_floats(dx_walk(p, run), ctas_of(run));
@@ -746,20 +724,15 @@ struct Train {
       dx_slabs = room.take<float>(most);
     }
   }
-  // Tokens of a run: e takes up to 480 MB (50,304 words: 18 tiles of 256 tokens, with four across one round of 72 clusters in dx), or 512
-  // tokens where that is more; of the sizes down to half of that, the one that leaves the fewest clusters idle in dx.
+  // Tokens of a run, of equal size: e takes up to 480 MB, or 512 tokens' where that is more (50,304 words: 4,608 tokens at most, so 16,384 go
+  // in four runs of 4,096).
   static int run_of(const Problem& p) {
     const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(512, (480ll << 20) / row / 256 * 256);
-    return p.tokens <= most ? p.tokens : (int)(256 * best_blocks(most / 256, over(p.width, 2 * kRows)));
+    return (int)std::min<int64_t>(p.tokens, up(over(p.tokens, over(p.tokens, most)), 256));
   }
-  Walk logits_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.vocab, p.width, terms_of(p), ctas_of(run), false, 0); }
-  Walk dx_walk(const Problem& p, int tokens) const {
-    return walk_of(tokens, p.width, p.vocab, terms_of(p), ctas_of(tokens), true, segment_of(p));
-  }
-  Walk dw_walk(const Problem& p, int tokens) const {
-    const int terms = terms_of(p);
-    return walk_of(p.vocab, p.width, tokens, terms, ctas_of(p.vocab), true, segment_of(p), (int)over(run, kDepth) * terms);
-  }
+  Walk logits_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.vocab, p.width, terms_of(p), ctas_of(run), false); }
+  Walk dx_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.width, p.vocab, terms_of(p), ctas_of(tokens), true, p.vocab); }
+  Walk dw_walk(const Problem& p, int tokens) const { return walk_of(p.vocab, p.width, tokens, terms_of(p), ctas_of(p.vocab), true, run); }
 };
 
 }  // namespace
@@ -796,10 +769,10 @@ int train(const Problem& p, cudaStream_t s) {
   const Train t(p, p.workspace);
   if (t.x.part != 0) st = run_convert(convert_of(p, t.x, p.x, p.x_dtype, p.x_stride), s);
   if (st == SA_OK && t.weight.part != 0) st = run_convert(convert_of(p, t.weight, p.weight, p.weight_dtype, p.weight_stride), s);
+  const Matrix x = matrix_of(p, t.x, p.x, p.x_dtype, p.x_stride), weight = matrix_of(p, t.weight, p.weight, p.weight_dtype, p.weight_stride);
   if (st == SA_OK)
-    st = launch_after(reference_kernel, dim3((unsigned)over(p.tokens, 8)), 256, 0, s, p.x, p.x_dtype, p.x_stride, p.weight, p.weight_dtype,
-                      p.weight_stride, p.targets, p.ignore_index, p.tokens, p.vocab, p.width, t.ref, t.any);
-  const size_t x_bytes = bytes_of(p.x_dtype);
+    st = launch_after(reference_kernel, dim3((unsigned)over(p.tokens, 8)), 256, 0, s, x.base, x.dtype, x.stride, weight.base, weight.dtype, weight.stride,
+                      p.targets, p.ignore_index, p.tokens, p.vocab, p.width, t.ref, t.any);
   for (int n0 = 0; n0 < p.tokens && st == SA_OK; n0 += t.run) {
     const int tokens = std::min(t.run, p.tokens - n0);
     const bool first = n0 == 0, last = n0 + tokens == p.tokens;
@@ -829,12 +802,13 @@ int train(const Problem& p, cudaStream_t s) {
     r.any = t.any;
     r.loss = t.losses + n0;
     r.inverse = t.inverse;
+    r.less = t.less + n0;
     r.e = e.p;
     r.e_pitch = e.p_pitch;
     r.e_part = e.p_part;
-    r.x = static_cast<const char*>(p.x) + (size_t)n0 * p.x_stride * x_bytes;
-    r.x_dtype = p.x_dtype;
-    r.x_stride = p.x_stride;
+    r.x = static_cast<const char*>(x.base) + (size_t)n0 * x.stride * bytes_of(x.dtype);
+    r.x_dtype = x.dtype;
+    r.x_stride = x.stride;
     r.scaled = const_cast<uint16_t*>(t.scaled.base);
     r.scaled_pitch = t.scaled.pitch;
     r.scaled_part = t.scaled.part;
@@ -858,8 +832,14 @@ int train(const Problem& p, cudaStream_t s) {
       o.scale = t.inverse;
       o.scale_rows = 1;
       o.slabs = t.dx_slabs;
-      st = run<kResult, false, true>(ctas, left, t.weight, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
-      if (st == SA_OK) st = finish(t.dx_slabs, w, ctas, t.inverse, 1, o.out, SA_F32, p.width, s);
+      o.table = weight.base;
+      o.table_dtype = weight.dtype;
+      o.table_stride = weight.stride;
+      o.table_factor = t.less + n0;
+      o.targets = e.targets;
+      o.vocab = p.vocab;
+      st = run_result<false, true>(p, ctas, left, t.weight, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      if (st == SA_OK) st = finish(o, w, ctas, s);
     }
     if (p.dweight_sums != nullptr && st == SA_OK) {
       const int ctas = ctas_of(p.vocab);
@@ -872,9 +852,27 @@ int train(const Problem& p, cudaStream_t s) {
       o.addend_pitch = p.width;
       o.slabs = t.dw_slabs;
       o.later = !first;
-      st = run<kResult, true, true>(ctas, left, right, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
-      if (st == SA_OK && last) st = finish(t.dw_slabs, w, ctas, nullptr, 0, p.dweight_sums, SA_F32, p.width, s);
+      st = run_result<true, true>(p, ctas, left, right, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      if (st == SA_OK && last) st = finish(o, w, ctas, s);
     }
+  }
+  if (p.dweight_sums != nullptr && st == SA_OK) {
+    embed::RowSums o{};
+    o.idx = p.targets;
+    o.skip = p.ignore_index;
+    o.tokens = p.tokens;
+    o.vocab = p.vocab;
+    o.width = p.width;
+    o.dy = x.base;
+    o.dtype = x.dtype;
+    o.dy_stride = x.stride;
+    o.factor = t.less;
+    o.scale = 1.f;
+    o.out = p.dweight_sums;
+    o.out_dtype = SA_F32;
+    o.add = true;
+    o.workspace = t.sorted;
+    st = embed::sum_rows(o, s);
   }
   if (st != SA_OK) return st;
   return launch_after(total_kernel, dim3(1), 1024, 0, s, (const float*)t.losses, p.targets, p.ignore_index, p.tokens, p.reduction, p.loss, p.count);
@@ -928,7 +926,7 @@ int backward(const Problem& p, cudaStream_t s) {
     e.p_part = b.dz.part;
     e.parts = b.dz.parts;
     e.half = half;
-    const Walk logits = walk_of(p.tokens, columns, p.width, terms_of(p), b.ctas, false, 0);
+    const Walk logits = walk_of(p.tokens, columns, p.width, terms_of(p), b.ctas, false);
     st = run<kProbabilities, false, false>(b.ctas, b.x, b.weight, logits, Origin{0, 0}, Origin{v0, 0}, e, status, s);
     if (st != SA_OK) return st;
     Operand dz = b.dz;
@@ -946,8 +944,8 @@ int backward(const Problem& p, cudaStream_t s) {
       r.scale = last ? scale : nullptr;
       r.slabs = b.dx_slabs;
       r.later = !first;
-      st = run<kResult, false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
-      if (st == SA_OK && last) st = finish(b.dx_slabs, w, b.ctas, scale, 0, p.dx, p.x_dtype, p.width, s);
+      st = run_result<false, true>(p, b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
+      if (st == SA_OK && last) st = finish(r, w, b.ctas, s);
       if (st != SA_OK) return st;
     }
     if (p.dweight != nullptr) {
@@ -960,8 +958,8 @@ int backward(const Problem& p, cudaStream_t s) {
       r.out_pitch = p.width;
       r.scale = scale;
       r.slabs = b.dw_slabs;
-      st = run<kResult, true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
-      if (st == SA_OK) st = finish(b.dw_slabs, w, ctas, scale, 0, r.out, p.weight_dtype, p.width, s);
+      st = run_result<true, true>(p, ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
+      if (st == SA_OK) st = finish(r, w, ctas, s);
     }
   }
   return st;

@@ -24,35 +24,23 @@ constexpr int kThreads = 384;              // warp 0 loads, warp 1 issues, warp 
 constexpr int kEpilogueWarps = 8;
 constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
 constexpr int kTerms = 6;                  // of an fp32 product
+constexpr int kSegment = 4;                // stages, with kSegments: 256 of the contraction
+constexpr int kSegmentChunks = 2;          // chunks of 32 columns that a thread of an epilogue has of such a tile of 128
 
 // The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  The first `whole` tiles are
-// walked by one cluster each, round by round; what is left, less than a round, is dealt out evenly, `ticks` to a tile, so that such a
-// tile is shared by neighbouring clusters, each with a sum of its own (a slab).  Launches with the same tiles and ticks share
-// their tiles alike, whatever their contraction's length.
+// walked by one cluster each, round by round.  Of what is left, less than half a round, every tile is cut into `slabs` equal parts of
+// the contraction with a cluster and a sum (a slab) each; the parts of all tiles at one depth are walked side by side, so what tiles
+// share is still read once.
 struct Walk {
   int m, n;                                // rows and columns of the result
   int bn;                                  // columns of a tile, a multiple of 32
   int m_tiles, n_tiles, whole;
   int depth_blocks, blocks;                // stages of one term, of all terms
-  int ticks;
   int clusters;
-  int slabs;                               // that a dealt tile has room for
+  int slabs;                               // of a cut tile
   int segment;                             // stages that are summed in tensor memory at a time
   int group;                               // row tiles that are walked side by side
   __host__ __device__ int tiles() const { return m_tiles * n_tiles; }
-  __host__ __device__ int64_t dealt() const { return (int64_t)(tiles() - whole) * ticks; }
-  __host__ __device__ int64_t begin_of(int c) const { return dealt() * c / clusters; }
-  __host__ __device__ int cluster_at(int64_t tick) const {        // whose share it is
-    int c = (int)(tick * clusters / dealt());
-    while (c + 1 < clusters && begin_of(c + 1) <= tick) ++c;
-    while (c > 0 && begin_of(c) > tick) --c;
-    return c;
-  }
-  // Slabs of a dealt tile: from the cluster of its first tick to that of its last.
-  __host__ __device__ int slabs_of(int tile) const {
-    const int64_t at = (int64_t)(tile - whole) * ticks;
-    return cluster_at(at + ticks - 1) - cluster_at(at) + 1;
-  }
   __host__ __device__ void place(int tile, int* tm, int* tn) const {
     const int per = group * n_tiles, g = tile / per, r = tile - g * per;
     const int rows = m_tiles - g * group < group ? m_tiles - g * group : group;
@@ -67,41 +55,34 @@ struct Walk {
 
 // A cluster's walk, the same in every role of its CTAs: units of at most `segment` stages.
 struct Units {
-  int64_t pos, end;                        // of the dealt tiles, in ticks
-  int tile, at, k, share0, share1;         // the tile at hand, the next whole one, and the stages that are this cluster's
-  int tm, tn, k0, k1, slab;
-  bool first;                              // of this cluster's sums of the tile
-  __host__ __device__ void begin(const Walk& w, int c) {
-    const bool some = w.whole < w.tiles();
-    pos = some ? w.begin_of(c) : 0;
-    end = some ? w.begin_of(c + 1) : 0;
+  int at, k, share1;                       // the next item: a whole tile, or a part of one behind them
+  int tile, tm, tn, k0, k1, slab;
+  bool first, last;                        // of this cluster's sums of the tile
+  __host__ __device__ void begin(int c) {
     at = c;
     k = share1 = 0;
   }
-  __host__ __device__ bool next(const Walk& w, int c) {
+  __host__ __device__ bool next(const Walk& w) {
+    first = k >= share1;
     while (k >= share1) {
-      if (at < w.whole) {
-        tile = at;
-        at += w.clusters;
-        slab = 0;
-        share0 = 0;
-        share1 = w.blocks;
-      } else {
-        if (pos >= end) return false;
-        const int t = (int)(pos / w.ticks);
-        const int64_t from = (int64_t)t * w.ticks, to = min(from + w.ticks, end);
-        tile = w.whole + t;
-        share0 = (int)((pos - from) * w.blocks / w.ticks);
-        share1 = (int)((to - from) * w.blocks / w.ticks);
-        pos = to;
-        slab = c - w.cluster_at(from);
+      const int left = w.tiles() - w.whole;
+      if (at >= w.whole + left * w.slabs) return false;
+      tile = at;
+      slab = 0;
+      k = 0;
+      share1 = w.blocks;
+      if (at >= w.whole && w.slabs > 1) {
+        slab = (at - w.whole) / left;
+        tile = at - slab * left;
+        k = (int)((int64_t)w.blocks * slab / w.slabs);
+        share1 = (int)((int64_t)w.blocks * (slab + 1) / w.slabs);
       }
+      at += w.clusters;
       w.place(tile, &tm, &tn);
-      k = share0;
     }
-    first = k == share0;
     k0 = k;
-    k1 = k = min(share1, k + w.segment);
+    k1 = k = k + w.segment < share1 ? k + w.segment : share1;
+    last = k == share1;
     return true;
   }
 };
@@ -111,7 +92,9 @@ struct Origin {
   int own, depth;
 };
 
-enum Kind { kStats, kProbabilities, kBoth, kResult };
+// kSegments: kResult whose sums leave tensor memory every `segment` stages, into registers: the tensor cores' additions round towards zero,
+// which fp32 results would show.
+enum Kind { kStats, kProbabilities, kBoth, kResult, kSegments };
 
 struct Epilogue {
   // kStats: of every row and half tile, the maximum (times log2 e) and the sum of exponentials above it; the targets' logits
@@ -133,7 +116,7 @@ struct Epilogue {
   int64_t p_pitch, p_part;                 // elements of a row, of a part
   int parts;
   int half;                                // fp16, not bf16
-  // kResult: of whole tiles (sums + addend) * scale; dealt tiles keep their sums in slabs of a tile each
+  // kResult: of whole tiles (sums + addend) * scale + table_factor * [a row of `table`]; cut tiles keep their sums in slabs of a tile each
   void* out;
   int dtype;
   int64_t out_pitch;
@@ -142,7 +125,12 @@ struct Epilogue {
   const float* scale;                      // may be null
   int scale_rows;                          // one for every row
   float* slabs;
-  int later;                               // dealt tiles add to what their slabs hold
+  int later;                               // cut tiles add to what their slabs hold
+  const void* table;                       // whose rows that `targets` names are added, `table_factor` times; may be null
+  int table_dtype;
+  int64_t table_stride;
+  const float* table_factor;               // of a row of the result
+  int vocab;
 };
 
 // ---- PTX of CTA pairs ---------------------------------------------------------------------------------------------------------
@@ -368,6 +356,77 @@ __device__ __forceinline__ void store_row(uint16_t* p, const uint32_t (&r)[32], 
   }
 }
 
+// Eight values of a row of any type from column `col` on, zeros behind the width.
+__device__ __forceinline__ void load_columns(const void* base, int dtype, int64_t row_at, int col, int width, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  const int64_t at = row_at + col;
+  const char* src = static_cast<const char*>(base) + at * (dtype == SA_F32 ? 4 : 2);
+  if (col + 8 <= width && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    if (dtype == SA_F32) {
+      const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
+    const uint4 a = *reinterpret_cast<const uint4*>(src);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (dtype == SA_BF16) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (col + i < width) {
+      if (dtype == SA_F32) v[i] = static_cast<const float*>(base)[at + i];
+      else if (dtype == SA_BF16) v[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at + i]);
+      else v[i] = __half2float(static_cast<const __half*>(base)[at + i]);
+    }
+}
+
+// 32 columns of a row of the result, or of a slab.
+__device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, const Units& u, uint32_t (&r)[32], int row, int in_tile, int tile_rows,
+                                             int chunk) {
+  const int col = u.tn * w.bn + chunk * 32, valid = w.n - col;
+  if (valid <= 0) return;
+  if (u.tile >= w.whole) {
+    float* const slab = e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * tile_rows + in_tile) * w.bn + chunk * 32;
+    if (e.later) add_row(slab, r, 32);
+    store_row(slab, r, 32);
+    return;
+  }
+  if (e.addend != nullptr) add_row(e.addend + (int64_t)row * e.addend_pitch + col, r, valid);
+  if (e.scale != nullptr) {
+    const float scale = e.scale[e.scale_rows ? row : 0];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+  }
+  if (e.table != nullptr && e.table_factor[row] != 0.f) {
+    const int64_t t = e.targets[row];
+    const float factor = e.table_factor[row];
+    if (t >= 0 && t < e.vocab) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v[8];
+        load_columns(e.table, e.table_dtype, t * e.table_stride, col + 8 * k, w.n, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[8 * k + j] = __float_as_uint(fmaf(factor, v[j], __uint_as_float(r[8 * k + j])));
+      }
+    }
+  }
+  const int64_t at = (int64_t)row * e.out_pitch + col;
+  if (e.dtype == SA_F32) store_row(static_cast<float*>(e.out) + at, r, valid);
+  else store_row(static_cast<uint16_t*>(e.out) + at, r, valid, e.dtype == SA_F16);
+}
+
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
 template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
@@ -400,22 +459,23 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   Waiter wait;
   wait.begin(status);
   Units u;
-  u.begin(w, c);
-  if (KIND == kBoth && e.any != nullptr && *e.any == 0) u.at = w.whole;     // tiles are all whole here: nothing to do
+  u.begin(c);
+  if (KIND == kBoth && e.any != nullptr && *e.any == 0) u.at = w.tiles();    // nothing to do: tiles are all whole here
 
   if (warp == 0) {
     if (lane == 0) {
       // ---- loads.  Both CTAs count on the first one's barrier: its thread issues the MMAs of both.
       const uint32_t full_there = CTAS == 2 ? address_in(full, 0) : full;
       const uint32_t ring = smem_u32(smem);
+      const bool both = !B_MN || w.bn > 64 * CTAS;              // of a CTA's 64s of columns
       int stage = 0, round = 0;
-      while (u.next(w, c)) {
+      while (u.next(w)) {
         const int a0 = at_a.own + u.tm * kColumns + (int)rank * kRows;
         const int b0 = at_b.own + u.tn * w.bn + (int)rank * (w.columns(u.tn) / CTAS);
         int term = u.k0 / w.depth_blocks, block = u.k0 - term * w.depth_blocks;
         for (int k = u.k0; k < u.k1; ++k) {
           if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1000);
-          if (rank == 0) expect_tx(full + 8 * stage, 2 * kOperand * CTAS);
+          if (rank == 0) expect_tx(full + 8 * stage, (both ? 2 * kOperand : kOperand + kOperand / 2) * CTAS);
           // parts of the terms: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
           const int pa = w.blocks == w.depth_blocks ? 0 : (0x001012 >> (4 * term)) & 3;
           const int pb = w.blocks == w.depth_blocks ? 0 : (0x010210 >> (4 * term)) & 3;
@@ -429,7 +489,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           if constexpr (B_MN) {
             load_3d<CTAS>(b, &map_b, bar, b0, kb, pb);
-            load_3d<CTAS>(b + kOperand / 2, &map_b, bar, b0 + 64, kb, pb);
+            if (both) load_3d<CTAS>(b + kOperand / 2, &map_b, bar, b0 + 64, kb, pb);
           } else {
             load_3d<CTAS>(b, &map_b, bar, kb, b0, pb);
           }
@@ -458,7 +518,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const uint32_t a_low = desc_low(smem_u32(smem), A_MN ? kOperand / 2 : 16), b_low = desc_low(smem_u32(smem) + kOperand, B_MN ? kOperand / 2 : 16);
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
       int stage = 0, round = 0, n = 0;
-      while (u.next(w, c)) {
+      while (u.next(w)) {
         const uint32_t idesc = (1u << 4) | format | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
                                ((uint32_t)(w.columns(u.tn) >> 3) << 17) | ((uint32_t)(kColumns >> 4) << 24);
         const uint32_t acc = tmem + (n & 1) * kColumns;
@@ -488,8 +548,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;              // 32 lanes, in bits 16 on
     const uint32_t read_there = CTAS == 2 ? address_in(read, 0) : read;
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 128 && e.zeroed != nullptr) *e.zeroed = 0u;
+    float sums[KIND == kSegments ? kSegmentChunks : 1][32];
     int n = 0;
-    while (u.next(w, c)) {
+    while (u.next(w)) {
       const int row = u.tm * kColumns + (int)rank * kRows + (warp & 3) * 32 + lane;
       const bool inside = row < w.m;
       const int columns = w.columns(u.tn), chunks = columns >> 5;
@@ -552,31 +613,30 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int64_t mine = target - e.column0 - col;
           if (inside) store_probabilities(e, r, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
         }
-      } else {
-        const bool dealt = u.tile >= w.whole;
+      } else if constexpr (KIND == kResult) {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
-        float* const slab = dealt ? e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * kColumns + in_tile) * w.bn : nullptr;
-        const float scale = e.scale != nullptr && inside ? e.scale[e.scale_rows ? row : 0] : 1.f;
         for (int i = from; i < to; ++i) {
           uint32_t r[32];
           tmem_ld32(acc + i * 32, r);
           tmem_ld_wait();
-          const int col = u.tn * w.bn + i * 32, valid = w.n - col;
-          if (!inside || valid <= 0) continue;
-          if (dealt) {
-            if (!u.first || e.later) add_row(slab + i * 32, r, 32);
-            store_row(slab + i * 32, r, 32);
-            continue;
-          }
-          const int64_t at = (int64_t)row * e.out_pitch + col;
-          if (!u.first) add_row(static_cast<const float*>(e.out) + at, r, valid);      // fp32 operands alone have more segments
-          else if (e.addend != nullptr) add_row(e.addend + (int64_t)row * e.addend_pitch + col, r, valid);
-          if (e.scale != nullptr) {
+          if (inside) store_result(e, w, u, r, row, in_tile, kColumns, i);
+        }
+      } else {
+        const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+        for (int i = 0; i < kSegmentChunks; ++i) {
+          uint32_t r[32];
+          if (from + i < to) {
+            tmem_ld32(acc + (from + i) * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sums[i][j] = (u.first ? 0.f : sums[i][j]) + __uint_as_float(r[j]);
+            if (u.last && inside) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(sums[i][j]);
+              store_result(e, w, u, r, row, in_tile, kColumns, from + i);
+            }
           }
-          if (e.dtype == SA_F32) store_row(static_cast<float*>(e.out) + at, r, valid);
-          else store_row(static_cast<uint16_t*>(e.out) + at, r, valid, e.dtype == SA_F16);
         }
       }
       tc_fence_before_sync();
