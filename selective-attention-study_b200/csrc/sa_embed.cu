@@ -5,19 +5,19 @@
 //           warps take a run of tokens each, count theirs by row, and after a prefix sum over the warps every warp writes its own
 //           tokens' places without another barrier.  148 CTAs read N indices each out of L2, which costs less than the launches of
 //           a radix sort.
-//   sum     pieces of 32 sorted tokens: their gradients are summed row by row in that order; a row inside one piece is finished,
+//   sum     pieces of 4 to 32 sorted tokens: their gradients are summed row by row in that order; a row inside one piece is finished,
 //           the parts of rows that cross pieces are kept.  Rows that no token names are written as zeros beside it.
 //   join    sums the parts of each row that crossed pieces.
 // So a word that is every tenth token is summed by as many CTAs as it needs, and nothing depends on the order of threads.
 #include "sa_layers.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sa {
 namespace embed {
 namespace {
 
-constexpr int kPiece = 32;                 // sorted tokens that are summed in a row
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32;
 constexpr int kMostRows = 1600;            // of the table, a CTA of `order`: 32 counters and a place each in shared memory
 constexpr int kThreads = 256, kJoinThreads = 1024;
@@ -155,9 +155,8 @@ struct Sum {
   int weight_dtype;
   float scale;
   int vocab, width, chunks, groups;        // chunks of 8 values in a row; rows that a CTA works on side by side
-  bool add;                                // to what stands in dweight, fp32
   float* parts;                            // [pieces][2][width]: of a row that began before the piece, of one that goes on behind it
-  int pieces;
+  int pieces, piece;                       // tokens of one
 };
 
 // A thread's eight columns of a row: neighbours, or `chunks` apart.
@@ -201,22 +200,17 @@ __device__ __forceinline__ void write_eight(const Sum& p, void* base, int dtype,
     }
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void finish_row(const Sum& p, int row, int t, const float (&x)[8]) {
+// `old`: what stands there, which ADD adds to.
+template <bool VEC, bool ADD>
+__device__ __forceinline__ void finish_row(const Sum& p, int row, int t, const float (&x)[8], const float (&old)[8]) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = x[i] * p.scale;
-  if (p.add) {
-    float old[8];
-    read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)row * p.width, t, old);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] += old[i];
-  }
+  for (int i = 0; i < 8; ++i) y[i] = ADD ? fmaf(x[i], p.scale, old[i]) : x[i] * p.scale;
   write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)row * p.width, t, y);
 }
 
 // blockIdx.y: columns, kThreads chunks at a time.  The first CTAs take pieces, the others rows without tokens.
-template <bool VEC>
+template <bool VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_blocks) {
   tc::after_previous_kernel();
   const int across = min(p.chunks, kThreads), group = threadIdx.x / across, t = blockIdx.y * kThreads + threadIdx.x - group * across;
@@ -229,19 +223,28 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
     return;
   }
   const int piece = blockIdx.x * p.groups + group, all = p.starts[p.vocab];
-  const int from = piece * kPiece, to = min(all, from + kPiece);
+  const int from = piece * p.piece, to = min(all, from + p.piece);
   if (from >= to) return;
   float sum[8] = {};
   constexpr int kAhead = 4;                                        // rows of dy in flight (8: fewer CTAs an SM, 39 -> 45 us)
   for (int i0 = from; i0 < to; i0 += kAhead) {
     int2 at[kAhead];
-    float x[kAhead][8];
+    float x[kAhead][8], old[ADD ? kAhead : 1][8];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) at[k] = i0 + k < to ? p.sorted[i0 + k] : make_int2(0, -1);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (at[k].y >= 0) read_eight<VEC>(p, p.dy, p.dtype, at[k].x * p.dy_stride, t, x[k]);
+      if (at[k].y >= 0) {
+        read_eight<VEC>(p, p.dy, p.dtype, at[k].x * p.dy_stride, t, x[k]);
+        if (ADD) read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)at[k].y * p.width, t, old[k]);
+      }
     const int next = i0 + kAhead < to ? p.sorted[i0 + kAhead].y : -1;
+    int begin[kAhead], end[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      begin[k] = at[k].y >= 0 ? p.starts[at[k].y] : 0;
+      end[k] = at[k].y >= 0 ? p.starts[at[k].y + 1] : 0;
+    }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (at[k].y < 0) continue;
@@ -249,9 +252,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] = fmaf(factor, x[k][i], sum[i]);
       if ((k + 1 < kAhead ? at[k + 1 < kAhead ? k + 1 : k].y : next) == at[k].y) continue;
-      const int begin = p.starts[at[k].y], end = p.starts[at[k].y + 1];
-      if (begin >= from && end <= from + kPiece) finish_row<VEC>(p, at[k].y, t, sum);
-      else write_eight<VEC>(p, p.parts, SA_F32, ((int64_t)piece * 2 + (begin >= from ? 1 : 0)) * p.width, t, sum);
+      if (begin[k] >= from && end[k] <= from + p.piece) finish_row<VEC, ADD>(p, at[k].y, t, sum, old[ADD ? k : 0]);
+      else write_eight<VEC>(p, p.parts, SA_F32, ((int64_t)piece * 2 + (begin[k] >= from ? 1 : 0)) * p.width, t, sum);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] = 0.f;
     }
@@ -259,17 +261,17 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
 }
 
 // Rows that cross pieces, by the piece in which they begin.  The CTA's groups take runs of the parts, and the first joins them.
-template <bool VEC>
+template <bool VEC, bool ADD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
   tc::after_previous_kernel();
   __shared__ float by_group[kJoinThreads][9];
   const int across = min(p.chunks, kJoinThreads), group = threadIdx.x / across, t = blockIdx.y * kJoinThreads + threadIdx.x - group * across;
   const int groups = kJoinThreads / across;
-  const int all = p.starts[p.vocab], from = blockIdx.x * kPiece, to = from + kPiece;
+  const int all = p.starts[p.vocab], from = blockIdx.x * p.piece, to = from + p.piece;
   if (to >= all) return;                                           // nothing behind this piece
   const int row = p.sorted[to - 1].y;
   if (p.sorted[to].y != row || p.starts[row] < from) return;       // its last row ends here, or began before
-  const int last = (p.starts[row + 1] - 1) / kPiece, parts = last - (int)blockIdx.x + 1;
+  const int last = (p.starts[row + 1] - 1) / p.piece, parts = last - (int)blockIdx.x + 1;
   const int per = (parts + groups - 1) / groups, k0 = min(parts, group * per), k1 = min(parts, k0 + per);
   float sum[8] = {};
   if (group < groups && t < p.chunks) {
@@ -288,11 +290,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
   for (int g = 1; g < groups; ++g)
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += by_group[g * across + threadIdx.x][i];
-  finish_row<VEC>(p, row, t, sum);
+  float old[8] = {};
+  if (ADD) read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)row * p.width, t, old);
+  finish_row<VEC, ADD>(p, row, t, sum, old);
 }
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-int pieces_of(int tokens) { return (tokens + kPiece - 1) / kPiece; }
+// Sorted tokens that are summed in a row: 32, and fewer where that would leave an SM less than two pieces (2,048 tokens: 56 us with 32, 10 with
+// 4; but 16,384 with words as often as words are 47 with 32 and 60 with 8, whose parts of rows take longer to join).
+int piece_of(int tokens) {
+  int piece = 32;
+  while (piece > 4 && tokens / piece < 2 * kSms) piece /= 2;
+  return piece;
+}
+int pieces_of(int tokens) { return (tokens + piece_of(tokens) - 1) / piece_of(tokens); }
 
 }  // namespace
 
@@ -314,18 +325,24 @@ int sum_rows(const RowSums& p, cudaStream_t s) {
   int* starts = reinterpret_cast<int*>(room + up((int64_t)p.tokens * 8, 256));
   float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(starts) + up(((int64_t)p.vocab + 1) * 4, 256));
   const int rows = std::min((p.vocab + kSms - 1) / kSms, kMostRows);
-  int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.skip, p.tokens,
+  const int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.skip, p.tokens,
                         p.vocab, rows, sorted, starts);
   if (st != SA_OK) return st;
-  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, p.add, parts, pieces_of(p.tokens)};
+  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p.tokens), piece_of(p.tokens)};
   a.groups = a.chunks < kThreads ? kThreads / a.chunks : 1;
   const bool vec = p.width % 8 == 0 && eights(p.dy, p.dtype, p.dy_stride, p.tokens) && eights(p.out, p.out_dtype, p.width, p.vocab);
   const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;
   const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + kZeroRows - 1) / kZeroRows), (a.chunks + kThreads - 1) / kThreads);
-  st = vec ? launch_after(sum_kernel<true>, grid, kThreads, 0, s, a, piece_blocks) : launch_after(sum_kernel<false>, grid, kThreads, 0, s, a, piece_blocks);
-  if (st != SA_OK || a.pieces < 2) return st;
-  const dim3 join(a.pieces - 1, (a.chunks + kJoinThreads - 1) / kJoinThreads);
-  return vec ? launch_after(join_kernel<true>, join, kJoinThreads, 0, s, a) : launch_after(join_kernel<false>, join, kJoinThreads, 0, s, a);
+  auto launch = [&](auto vec_, auto add) {
+    constexpr bool VEC = decltype(vec_)::value, ADD = decltype(add)::value;
+    const int status = launch_after(sum_kernel<VEC, ADD>, grid, kThreads, 0, s, a, piece_blocks);
+    if (status != SA_OK || a.pieces < 2) return status;
+    return launch_after(join_kernel<VEC, ADD>, dim3(a.pieces - 1, (a.chunks + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s, a);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if (p.add) return vec ? launch(yes, yes) : launch(no, yes);
+  return vec ? launch(yes, no) : launch(no, no);
 }
 
 int backward(const sa_embedding& p, cudaStream_t s) {

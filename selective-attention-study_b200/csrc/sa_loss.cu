@@ -463,7 +463,7 @@ struct Operand {
   const uint16_t* base = nullptr;
   int64_t rows = 0, width = 0, pitch = 0, part = 0;
   int parts = 0;
-  int map(CUtensorMap* m, bool mn_major) const { return make_map(m, base, width, rows, parts, pitch, part, mn_major ? 64 : kRows); }
+  int map(CUtensorMap* m, bool mn_major, int box) const { return make_map(m, base, width, rows, parts, pitch, part, mn_major ? 64 : box); }
 };
 
 // The walk over an m x n result of contraction `depth`.  `result`: a product of dz, which comes from memory: a row's tiles stand side by
@@ -474,7 +474,7 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
   Walk w{};
   w.m = m;
   w.n = n;
-  w.bn = kRows * (result && terms > 1 ? 1 : ctas);                 // kSegments: as many sums as a thread's registers hold
+  w.bn = kRows * ctas;
   w.m_tiles = (int)over(m, kRows * ctas);
   w.n_tiles = (int)over(n, w.bn);
   w.depth_blocks = (int)over(depth, kDepth);
@@ -499,7 +499,7 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
 int64_t slab_floats(const Walk& w, int ctas) { return (int64_t)(w.tiles() - w.whole) * w.slabs * kRows * ctas * w.bn; }
 
 template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_a, Origin at_b, const Epilogue& e, const WaitCtx& status,
+int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_a, Origin at_b, int a_bytes, const Epilogue& e, const WaitCtx& status,
            cudaStream_t s) {
   auto kernel = product_kernel<CTAS, KIND, A_MN, B_MN>;
   SA_CUDA_CHECK(allow_smem(kernel, kSmem));
@@ -518,18 +518,21 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_
   config.attrs = attrs;
   config.numAttrs = 2;
   count_launch();
-  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, b, w, at_a, at_b, e, status));
+  SA_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, b, w, at_a, at_b, a_bytes, e, status));
   return SA_OK;
 }
 template <Kind KIND, bool A_MN, bool B_MN>
 int run(int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, const Epilogue& e, const WaitCtx& status,
         cudaStream_t s) {
   CUtensorMap map_a, map_b;
-  int st = a.map(&map_a, A_MN);
-  if (st == SA_OK) st = b.map(&map_b, B_MN);
+  // few tokens: a copy takes as long for a row outside the tensor as for one inside (16 tokens of 50,304 words: 33 us with 128 rows)
+  const int box = ctas == 1 ? std::min(kRows, (int)up(w.m, 8)) : kRows;
+  int st = a.map(&map_a, A_MN, box);
+  if (st == SA_OK) st = b.map(&map_b, B_MN, kRows);
   if (st != SA_OK) return st;
-  return ctas == 2 ? launch<2, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, e, status, s)
-                   : launch<1, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, e, status, s);
+  const int a_bytes = A_MN ? kOperand : box * kDepth * 2;
+  return ctas == 2 ? launch<2, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s)
+                   : launch<1, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s);
 }
 
 // CTAs of a tile: two where there are rows for both.
@@ -724,11 +727,26 @@ struct Train {
       dx_slabs = room.take<float>(most);
     }
   }
-  // Tokens of a run, of equal size: e takes up to 480 MB, or 512 tokens' where that is more (50,304 words: 4,608 tokens at most, so 16,384 go
-  // in four runs of 4,096).
+  // Tokens of a run: e takes up to 512 MB, or 512 tokens' where that is more; of the sizes down to half of that, the one whose dx takes
+  // the fewest rounds of the clusters (16,384 tokens of 50,304 words, four tiles across: three runs of 20 tiles of tokens and one of
+  // 4 take 3.5 rounds, four runs of 16 take 4).
   static int run_of(const Problem& p) {
-    const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(512, (480ll << 20) / row / 256 * 256);
-    return (int)std::min<int64_t>(p.tokens, up(over(p.tokens, over(p.tokens, most)), 256));
+    const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(512, (512ll << 20) / row / 256 * 256) / 256;
+    if (p.tokens <= most * 256) return p.tokens;
+    const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, all = over(p.tokens, 256);
+    auto rounds = [&](int64_t blocks) {                          // in thousandths, as walk_of cuts what is left of whole ones
+      const int64_t tiles = blocks * across, left = tiles % clusters;
+      return tiles / clusters * 1000 + (left > 0 ? 1000 / (clusters / left) : 0) + (blocks > 0 ? 50 : 0);
+    };
+    int64_t best = INT64_MAX, at = most;
+    for (int64_t b = most; 2 * b > most; --b) {
+      const int64_t cost = all / b * rounds(b) + rounds(all % b);
+      if (cost < best) {
+        best = cost;
+        at = b;
+      }
+    }
+    return (int)(at * 256);
   }
   Walk logits_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.vocab, p.width, terms_of(p), ctas_of(run), false); }
   Walk dx_walk(const Problem& p, int tokens) const { return walk_of(tokens, p.width, p.vocab, terms_of(p), ctas_of(tokens), true, p.vocab); }

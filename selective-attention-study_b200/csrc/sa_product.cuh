@@ -25,7 +25,7 @@ constexpr int kEpilogueWarps = 8;
 constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
 constexpr int kTerms = 6;                  // of an fp32 product
 constexpr int kSegment = 4;                // stages, with kSegments: 256 of the contraction
-constexpr int kSegmentChunks = 2;          // chunks of 32 columns that a thread of an epilogue has of such a tile of 128
+constexpr int kSegmentChunks = 4;          // chunks of 32 columns of a tile that a thread of an epilogue has, at most
 
 // The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  The first `whole` tiles are
 // walked by one cluster each, round by round.  Of what is left, less than half a round, every tile is cut into `slabs` equal parts of
@@ -429,10 +429,12 @@ __device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, c
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
+// `a_bytes`: of the left operand in a stage, less than a whole one where its box has fewer rows; what stands in the others' place makes
+// rows of the tile that nothing reads.
 template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Walk w, const Origin at_a,
-               const Origin at_b, const Epilogue e, const WaitCtx status) {
+               const Origin at_b, const int a_bytes, const Epilogue e, const WaitCtx status) {
   constexpr int kColumns = kRows * CTAS;                            // of an accumulator
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -467,7 +469,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       // ---- loads.  Both CTAs count on the first one's barrier: its thread issues the MMAs of both.
       const uint32_t full_there = CTAS == 2 ? address_in(full, 0) : full;
       const uint32_t ring = smem_u32(smem);
-      const bool both = !B_MN || w.bn > 64 * CTAS;              // of a CTA's 64s of columns
       int stage = 0, round = 0;
       while (u.next(w)) {
         const int a0 = at_a.own + u.tm * kColumns + (int)rank * kRows;
@@ -475,7 +476,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         int term = u.k0 / w.depth_blocks, block = u.k0 - term * w.depth_blocks;
         for (int k = u.k0; k < u.k1; ++k) {
           if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1000);
-          if (rank == 0) expect_tx(full + 8 * stage, (both ? 2 * kOperand : kOperand + kOperand / 2) * CTAS);
+          if (rank == 0) expect_tx(full + 8 * stage, (a_bytes + kOperand) * CTAS);
           // parts of the terms: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
           const int pa = w.blocks == w.depth_blocks ? 0 : (0x001012 >> (4 * term)) & 3;
           const int pb = w.blocks == w.depth_blocks ? 0 : (0x010210 >> (4 * term)) & 3;
@@ -489,7 +490,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           if constexpr (B_MN) {
             load_3d<CTAS>(b, &map_b, bar, b0, kb, pb);
-            if (both) load_3d<CTAS>(b + kOperand / 2, &map_b, bar, b0 + 64, kb, pb);
+            load_3d<CTAS>(b + kOperand / 2, &map_b, bar, b0 + 64, kb, pb);
           } else {
             load_3d<CTAS>(b, &map_b, bar, kb, b0, pb);
           }
@@ -548,7 +549,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;              // 32 lanes, in bits 16 on
     const uint32_t read_there = CTAS == 2 ? address_in(read, 0) : read;
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 128 && e.zeroed != nullptr) *e.zeroed = 0u;
-    float sums[KIND == kSegments ? kSegmentChunks : 1][32];
+    uint32_t sums[KIND == kSegments ? kSegmentChunks : 1][32];
     int n = 0;
     while (u.next(w)) {
       const int row = u.tm * kColumns + (int)rank * kRows + (warp & 3) * 32 + lane;
@@ -625,18 +626,21 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
 #pragma unroll
         for (int i = 0; i < kSegmentChunks; ++i) {
-          uint32_t r[32];
-          if (from + i < to) {
-            tmem_ld32(acc + (from + i) * 32, r);
+          if (from + i >= to) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[16];
+            tmem_ld16(acc + (from + i) * 32 + 16 * h, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sums[i][j] = (u.first ? 0.f : sums[i][j]) + __uint_as_float(r[j]);
-            if (u.last && inside) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(sums[i][j]);
-              store_result(e, w, u, r, row, in_tile, kColumns, from + i);
-            }
+            for (int j = 0; j < 16; ++j)
+              sums[i][16 * h + j] = __float_as_uint((u.first ? 0.f : __uint_as_float(sums[i][16 * h + j])) + __uint_as_float(r[j]));
           }
+        }
+        if (u.last && inside) {
+#pragma unroll
+          for (int i = 0; i < kSegmentChunks; ++i)
+            if (from + i < to) store_result(e, w, u, sums[i], row, in_tile, kColumns, from + i);
         }
       }
       tc_fence_before_sync();
