@@ -664,7 +664,7 @@ def run_decoder(args, w, rank, world, device):
 
     torch.manual_seed(0)
     model = SelectiveDecoder(vocab_size=50304, n_layers=w["layers"], d_model=w["heads"] * w["dim"],
-                             n_heads=w["heads"]).to(device)
+                             n_heads=w["heads"], own_layers=args.own_layers).to(device)
     params = sum(p.numel() for p in model.parameters())
     net = model
     if world > 1:
@@ -721,7 +721,8 @@ def run_decoder(args, w, rank, world, device):
             "config": {"workload": f"c5: decoder training step, {w['layers']} layers, d_model {w['heads'] * w['dim']}, "
                                    f"{w['heads']} heads x {w['dim']}, GELU MLP x4, pre-LN, no position signal, vocab 50304, "
                                    f"T={w['seq']}, {w['batch']} sequence(s) per GPU, AdamW, grad clip 1.0",
-                       "parameters": params, "parallelism": f"dp{world}", "loss": last_loss,
+                       "parameters": params, "parallelism": f"dp{world}", "loss": last_loss, "own_layers": args.own_layers,
+                       "peak_gib": torch.cuda.max_memory_allocated(device) / 2**30,
                        "l2": "activations and weights far exceed the 126 MB L2"},
             "e2e": {"value": whole_job_tokens_per_second(tokens * world, times[True]), "unit": "tokens/s",
                     "ms_per_step": times[True], "h2d_bytes_per_step": 2 * tokens * 8, "d2h_bytes_per_step": 4},
@@ -889,6 +890,8 @@ def main():
     ap.add_argument("--seq", type=int, default=None, help="override T (profiling on a small case)")
     ap.add_argument("--batch", type=int, default=None, help="override B (profiling on a small case)")
     ap.add_argument("--layers", type=int, default=None, help="override the layer count of the c5 decoder")
+    ap.add_argument("--own-layers", action="store_true",
+                    help="c5, a separate row: embedding, norms and loss by the library's kernels too, not by torch's operators")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--e2e-call", default="packed", choices=["packed", "plain"],
                     help="end-to-end arm: the layer-facing packed call (default where it applies) or the (B, H, T, D) call")

@@ -8,7 +8,11 @@ initialisation (``:379-385``), no position signal.  The loss is computed over th
 The attention layer hands the operator the fused QKV projection output as it is (the tensor-core engine
 reads strided (B, T, H, D) data through TMA descriptors), gets the merged (B, T, H * D) activation written by
 the forward kernel, and gets dq, dk, dv written straight into the projection's gradient: nothing is copied
-on either side of the kernels in either pass (bf16; fp32 runs take the unfused call)."""
+on either side of the kernels in either pass (bf16; fp32 runs take the unfused call).
+
+With ``own_layers=True`` what stands around the attention goes through the library too (``layers.py``): the embedding, every residual
+sum with the norm behind it, and the loss, whose logits are then never there at all (``loss_chunk`` has no part in it).  Parameters and
+their names are the same either way; results differ by roundings."""
 
 from __future__ import annotations
 
@@ -16,7 +20,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import kernels
+from . import kernels, layers
 
 
 class SelectiveSelfAttention(nn.Module):
@@ -45,15 +49,29 @@ class Block(nn.Module):
         self.c_fc = nn.Linear(d_model, 4 * d_model, bias=False)
         self.c_proj = nn.Linear(4 * d_model, d_model, bias=False)
 
+    def mlp(self, x: torch.Tensor) -> torch.Tensor:
+        return self.c_proj(F.gelu(self.c_fc(x)))
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = x + self.attn(self.ln_1(x))
-        return x + self.c_proj(F.gelu(self.c_fc(self.ln_2(x))))
+        return x + self.mlp(self.ln_2(x))
+
+    def forward_own(self, x: torch.Tensor, branch: torch.Tensor | None, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        """The block by ``layers``: the residual stream and the branch of the block before that is still to be added to it, and the
+        same behind this block.  ``dtype``: of the norms' results, as the projections will take them."""
+        if branch is None:
+            y = layers.layer_norm(x, self.ln_1.weight, eps=self.ln_1.eps, dtype=dtype)
+        else:
+            x, y = layers.add_layer_norm(x, branch, self.ln_1.weight, eps=self.ln_1.eps, dtype=dtype)
+        x, y = layers.add_layer_norm(x, self.attn(y), self.ln_2.weight, eps=self.ln_2.eps, dtype=dtype)
+        return x, self.mlp(y)
 
 
 class SelectiveDecoder(nn.Module):
     def __init__(self, vocab_size: int = 50304, n_layers: int = 24, d_model: int = 1024, n_heads: int = 16,
-                 loss_chunk: int = 4096):
+                 loss_chunk: int = 4096, own_layers: bool = False):
         super().__init__()
+        self.own_layers = own_layers
         self.wte = nn.Embedding(vocab_size, d_model)
         self.h = nn.ModuleList([Block(d_model, n_heads) for _ in range(n_layers)])
         self.ln_f = nn.LayerNorm(d_model, bias=False)
@@ -62,7 +80,20 @@ class SelectiveDecoder(nn.Module):
             if isinstance(module, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
+    def _forward_own(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        x, branch = layers.embedding(idx, self.wte.weight), None
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        for block in self.h:
+            x, branch = block.forward_own(x, branch, dtype)
+        if branch is None:
+            y = layers.layer_norm(x, self.ln_f.weight, eps=self.ln_f.eps, dtype=dtype)
+        else:
+            y = layers.add_layer_norm(x, branch, self.ln_f.weight, eps=self.ln_f.eps, dtype=dtype)[1]
+        return layers.linear_cross_entropy(y, self.wte.weight, targets)
+
     def forward(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        if self.own_layers:
+            return self._forward_own(idx, targets)
         x = self.wte(idx)
         for block in self.h:
             x = block(x)
