@@ -479,7 +479,9 @@ size_t sa_linear_loss_backward_bytes(const sa_linear_loss* p);
 int sa_linear_loss_backward(const sa_linear_loss* p);
 /* The same with a product less, where there is a reduction and product is SA_BF16 or SA_F32: _train writes loss and count, and the
  * gradients' sums for a sum's cotangent of 1; _scale makes dx and dweight of them (those that are not null) for dloss and count.
- * lse is not used.  In products of SA_BF16 the softmax enters as exponentials of 8 bits, and x over their sum rounded to 8 bits. */
+ * lse is not used.  In products of SA_BF16 the softmax enters as exponentials of 8 bits, and x over their sum rounded to 8 bits; the
+ * targets' part is added in fp32.  _prefers_train: 1 where that is the faster way, by an estimate (small problems are not). */
+int sa_linear_loss_prefers_train(const sa_linear_loss* p);
 size_t sa_linear_loss_train_bytes(const sa_linear_loss* p);
 int sa_linear_loss_train(const sa_linear_loss* p);
 int sa_linear_loss_scale(const sa_linear_loss* p);

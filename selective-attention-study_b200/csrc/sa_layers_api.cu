@@ -151,6 +151,11 @@ int sa_linear_loss_backward(const sa_linear_loss* in) {
   return st != SA_OK ? st : loss::backward(p, static_cast<cudaStream_t>(in->stream));
 }
 
+int sa_linear_loss_prefers_train(const sa_linear_loss* in) {
+  loss::Problem p;
+  return to_loss(in, &p) == SA_OK && loss::prefers_train(p);
+}
+
 size_t sa_linear_loss_train_bytes(const sa_linear_loss* in) {
   loss::Problem p;
   return to_loss(in, &p) == SA_OK && check_train(in) == SA_OK ? loss::train_bytes(p) : 0;

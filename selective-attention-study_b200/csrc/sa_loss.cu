@@ -780,6 +780,18 @@ int forward(const Problem& p, cudaStream_t s) {
                       reinterpret_cast<float2*>(p.lse), p.loss, p.count, f.sums, f.ticket);
 }
 
+// A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, written, read and written again, and
+// eight more launches: the smaller of both estimates, in us at 1.4 PFLOP/s (fp32: 0.75) and 6.4 TB/s.  Measured, bf16: 4,096 tokens of 8,000 words
+// of 1,024 202 us by computing the logits again and 232 with the loss, 64 of 50,304 136 and 224, 2,048 of 50,304 of 768 600 and 519; fp32: 1,024 of 8,000
+// of 512 216 and 212, 512 of 32,000 of 768 634 and 588.
+bool prefers_train(const Problem& p) {
+  if (p.reduction == SA_REDUCTION_NONE || p.product == SA_F16) return false;
+  const double values = (double)p.vocab * p.width, tokens = (double)up(p.tokens, kRows);
+  double saved = 2.0 * tokens * values * terms_of(p) / (p.product == SA_F32 ? 0.75e9 : 1.4e9);
+  if (!in_place(p.weight_dtype, p.product, p.weight, p.weight_stride, p.vocab, p.width)) saved += values * (bytes_of(p.weight_dtype) + 2 * parts_of(p)) / 6.4e6;
+  return saved > 8.0 * (values + tokens * p.width) / 6.4e6 + 50.0;
+}
+
 int train(const Problem& p, cudaStream_t s) {
   WaitCtx status;
   int st = wait_ctx(&status);

@@ -26,6 +26,7 @@ struct Problem {
 size_t forward_bytes(const Problem& p);
 int forward(const Problem& p, cudaStream_t s);
 // Loss and gradients together, for one cotangent that is not known yet: sums in fp32 that `scale` turns into the gradients.
+bool prefers_train(const Problem& p);         // whether that takes less time than forward and backward
 size_t train_bytes(const Problem& p);
 int train(const Problem& p, cudaStream_t s);
 int scale(const Problem& p, cudaStream_t s);

@@ -914,10 +914,7 @@ Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, in
   return loss;
 }
 
-// The loss with its gradients up to the cotangent, where that is one number and the operands' exponents allow it: a product less than
-// computing the logits again.
-bool gradients_with_loss(int64_t reduction, int64_t product) { return reduction != SA_REDUCTION_NONE && product != SA_F16; }
-
+// The loss with its gradients up to the cotangent, which is one number: a product less than computing the logits again.
 struct LinearLossTrained : public torch::autograd::Function<LinearLossTrained> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& targets, int64_t ignore_index, int64_t reduction,
                         int64_t product) {
@@ -1030,7 +1027,19 @@ struct LinearLoss : public torch::autograd::Function<LinearLoss> {
   }
 };
 
-Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets_in, int64_t ignore_index, int64_t reduction) {
+// Whether rows_in is a view.
+bool rows_viewable(const Tensor& t) {
+  if (t.stride(-1) != 1 && t.size(-1) != 1) return false;
+  int64_t expected = -1;                            // stride of the axis before
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (expected >= 0 && t.stride(i) != expected) return false;
+    expected = t.stride(i) * t.size(i);
+  }
+  return true;
+}
+
+Tensor linear_cross_entropy(Tensor x, Tensor weight, const Tensor& targets_in, int64_t ignore_index, int64_t reduction) {
   const char* fn = "linear_cross_entropy";
   check_not_traced(fn);
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1 && weight.size(1) >= 1, fn,
@@ -1050,10 +1059,16 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   TORCH_CHECK_VALUE(code_of(product) >= 0 && (product != at::kFloat || (x.scalar_type() == at::kFloat && weight.scalar_type() == at::kFloat)), fn,
                     ": autocast to ", name_of(product), " needs x and weight in that dtype");
   const c10::cuda::CUDAGuard guard(x.device());
+  if (!rows_viewable(x)) x = x.contiguous();        // here, where autograd sees it, and once
+  if (!rows_viewable(weight)) weight = weight.contiguous();
   const Tensor targets = indices_in(targets_in);
   const bool train = c10::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad());
-  if (train && gradients_with_loss(reduction, code_of(product)))
-    return LinearLossTrained::apply(x, weight, targets, ignore_index, reduction, (int64_t)code_of(product));
+  if (train && reduction != SA_REDUCTION_NONE) {
+    const Tensor x_rows = rows_in(x), weight_rows = rows_in(weight);
+    const sa_linear_loss p = loss_of(x_rows, weight_rows, targets, ignore_index, reduction, code_of(product));
+    if (sa_linear_loss_prefers_train(&p))
+      return LinearLossTrained::apply(x, weight, targets, ignore_index, reduction, (int64_t)code_of(product));
+  }
   if (train)
     return LinearLoss::apply(x, weight, targets, ignore_index, reduction, (int64_t)code_of(product), targets_in.sizes());
   Tensor lse;

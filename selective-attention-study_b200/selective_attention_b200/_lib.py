@@ -29,7 +29,8 @@ EXPORTS = ("sa_abi_version", "sa_status_string", "sa_last_cuda_error", "sa_engin
            "sa_paged_workspace_bytes", "sa_paged_run", "sa_page_reorder_words", "sa_page_reorder", "sa_page_move", "sa_stream_capture",
            "sa_beam_workspace_bytes", "sa_beam_select", "sa_norm_forward", "sa_norm_backward_bytes", "sa_norm_backward", "sa_embedding_forward",
            "sa_embedding_backward_bytes", "sa_embedding_backward", "sa_linear_loss_forward_bytes", "sa_linear_loss_forward",
-           "sa_linear_loss_backward_bytes", "sa_linear_loss_backward", "sa_linear_loss_train_bytes", "sa_linear_loss_train", "sa_linear_loss_scale")
+           "sa_linear_loss_backward_bytes", "sa_linear_loss_backward", "sa_linear_loss_train_bytes", "sa_linear_loss_train", "sa_linear_loss_scale",
+           "sa_linear_loss_prefers_train")
 
 
 class Problem(ctypes.Structure):
@@ -221,7 +222,7 @@ def load() -> ctypes.CDLL:
     lib.sa_beam_select.restype = i32
     lib.sa_beam_select.argtypes = [ctypes.POINTER(Beam)]
     for name, struct in (("sa_norm", Norm), ("sa_embedding", Embedding), ("sa_linear_loss", LinearLoss)):
-        for fn in ("_forward", "_backward", "_backward_bytes") + (("_forward_bytes", "_train_bytes", "_train", "_scale") if struct is LinearLoss else ()):
+        for fn in ("_forward", "_backward", "_backward_bytes") + (("_forward_bytes", "_train_bytes", "_train", "_scale", "_prefers_train") if struct is LinearLoss else ()):
             getattr(lib, name + fn).restype = sz if fn.endswith("bytes") else i32
             getattr(lib, name + fn).argtypes = [ctypes.POINTER(struct)]
     lib.sa_device_status.restype = i32

@@ -3,6 +3,7 @@
 Tolerances count roundings: half a step of the result's type relative to the value, and steps of 2^-24 (2^-22 for a group of 16 products
 that a tensor core adds, which truncates) relative to the sum of the magnitudes that were added."""
 
+import ctypes
 import math
 
 import pytest
@@ -238,22 +239,61 @@ def _loss_reference(x, w, targets, ignore, g):
     return losses, dz, x.abs() @ w.abs().T
 
 
-def _check_loss(x, w, targets, reduction, ignore=-100, product=None, seed=0):
+CODES = {F32: _lib.DTYPE_F32, BF16: _lib.DTYPE_BF16, F16: _lib.DTYPE_F16}
+
+
+def _loss_struct(x, w, targets, ignore, reduction, product):
+    p = _lib.LinearLoss()
+    p.struct_bytes, p.product, p.x_dtype, p.weight_dtype = ctypes.sizeof(p), CODES[product], CODES[x.dtype], CODES[w.dtype]
+    p.reduction, p.tokens, p.vocab, p.width = layers.REDUCTIONS[reduction], x.shape[0], w.shape[0], x.shape[1]
+    p.ignore_index, p.x, p.x_stride, p.weight, p.weight_stride = ignore, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0)
+    p.targets, p.stream = targets.data_ptr(), torch.cuda.current_stream().cuda_stream
+    return p
+
+
+def _with_the_loss(x, w, targets, ignore, reduction, product, dloss):
+    """Loss and gradients by sa_linear_loss_train and _scale, which the Python call takes where they are the faster way."""
+    lib, x, w, targets = _lib.load(), x.detach().reshape(-1, x.shape[-1]), w.detach(), targets.reshape(-1)
+    p = _loss_struct(x, w, targets, ignore, reduction, product)
+    loss, count = torch.empty((), device="cuda"), torch.empty(1, device="cuda")
+    sums = [torch.full(t.shape, float("nan"), device="cuda") for t in (x, w)]
+    p.loss, p.count, p.dx_sums, p.dweight_sums = (t.data_ptr() for t in (loss, count, *sums))
+    p.workspace_bytes = lib.sa_linear_loss_train_bytes(ctypes.byref(p))
+    workspace = torch.full((p.workspace_bytes,), 255, dtype=torch.uint8, device="cuda")
+    p.workspace = workspace.data_ptr()
+    _lib.check("sa_linear_loss_train", lib.sa_linear_loss_train(ctypes.byref(p)))
+    dx, dw = torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty_like(w, memory_format=torch.contiguous_format)
+    p.dloss, p.dx, p.dweight = dloss.data_ptr(), dx.data_ptr(), dw.data_ptr()
+    _lib.check("sa_linear_loss_scale", lib.sa_linear_loss_scale(ctypes.byref(p)))
+    return loss, dx, dw
+
+
+def _prefers(x, w, targets, ignore, reduction, product):
+    x = x.detach().reshape(-1, x.shape[-1])
+    return bool(_lib.load().sa_linear_loss_prefers_train(ctypes.byref(_loss_struct(x, w, targets, ignore, reduction, product))))
+
+
+def _check_loss(x, w, targets, reduction, ignore=-100, product=None, seed=0, train=False):
+    """``train``: by the C entries that compute the gradients with the loss."""
     gen = _gen(seed)
     n, (vocab, width) = targets.numel(), w.shape
     x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
     product = product or x.dtype
-    loss = layers.linear_cross_entropy(x, w, targets, ignore_index=ignore, reduction=reduction)
-    assert loss.dtype == F32
     counts = int((targets != ignore).sum())
     if reduction == "none":
-        dloss = (torch.rand(loss.shape, generator=gen) + 0.25).cuda()
+        dloss = (torch.rand(targets.shape, generator=gen) + 0.25).cuda()
         g = dloss.flatten().double()
     else:
         dloss = torch.tensor(0.75 if product != F16 else 768.0, device="cuda")
         g = dloss.double().expand(n) / (counts if reduction == "mean" else 1)
-    dx, dw = torch.autograd.grad(loss, (x, w), dloss)
-    assert (dx.dtype, dw.dtype, dx.shape, dw.shape) == (x.dtype, w.dtype, x.shape, w.shape)
+    if train:
+        loss, dx, dw = _with_the_loss(x, w, targets, ignore, reduction, product, dloss)
+        dx = dx.view(x.shape)
+    else:
+        train = _prefers(x, w, targets, ignore, reduction, product)
+        loss = layers.linear_cross_entropy(x, w, targets, ignore_index=ignore, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (x, w), dloss)
+    assert loss.dtype == F32 and (dx.dtype, dw.dtype, dx.shape, dw.shape) == (x.dtype, w.dtype, x.shape, w.shape)
     rx, rw = x.reshape(-1, width).to(product), w.to(product)
     losses, dz, sizes = _loss_reference(rx, rw, targets.flatten(), ignore, g)
     # a logit: width / 16 groups of products (in 3 parts: 6 times as many, of which the dropped ones are 2^-22), each truncated
@@ -280,7 +320,7 @@ def _check_loss(x, w, targets, reduction, ignore=-100, product=None, seed=0):
 
     want, slack = around(dz, dz.abs(), each, rw.detach().double(), vocab)
     _check("dx", dx.reshape(-1, width), want, slack)
-    if reduction != "none" and product != F16:              # one cotangent: x over the sum of exponentials is rounded too
+    if train:                                               # x over the sum of exponentials is rounded too
         each = each + dz.abs() * ok
     want, slack = around(dz.T, dz.T.abs(), each.T, rx.detach().double(), n)
     _check("dw", dw, want, slack)
@@ -306,6 +346,8 @@ def test_loss_and_its_gradients(tokens, vocab, width, reduction, dtype):
     if tokens > 2:
         targets[1::7] = -100
     _check_loss(x, w, targets, reduction)
+    if dtype != F16:
+        _check_loss(x, w, targets, "mean" if reduction == "none" else reduction, train=True)
 
 
 @pytest.mark.parametrize("dtype,tokens,vocab,width,reduction", [
@@ -319,6 +361,8 @@ def test_loss_in_several_parts(dtype, tokens, vocab, width, reduction):
     targets = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
     targets[5::11] = -100
     _check_loss(x, w, targets, reduction)
+    if reduction != "none" and dtype != F16:
+        _check_loss(x, w, targets, reduction, train=True)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -333,10 +377,11 @@ def test_targets_that_are_all_but_impossible(dtype):
     targets[2::9] = z[2::9].argmax(1)
     losses = layers.linear_cross_entropy(x, w, targets, reduction="none")
     assert float(losses.max()) > 100 and int((losses > 44).sum()) > 30 and int((losses < 1).sum()) > 30
-    for reduction in ("sum", "none"):
-        _check_loss(x, w, targets, reduction)
+    for reduction, train in (("sum", True), ("sum", False), ("none", False)):
+        _check_loss(x, w, targets, reduction, train=train)
     far = torch.full_like(targets[:1], int(z[1].argmin()))
-    _check_loss(x[1:2], w, far, "mean")
+    for train in (False, True):
+        _check_loss(x[1:2], w, far, "mean", train=train)
 
 
 def test_loss_of_batches_strides_and_padding():
@@ -347,8 +392,11 @@ def test_loss_of_batches_strides_and_padding():
     targets[2] = -7                                         # a sequence of padding
     targets[0, 50:] = -7
     for x, w in ((base[..., 128:], table[:, 16:144]), (base[..., 1:129], table[:, 3:131]), (base[..., ::2], table[:, 16:144].t().contiguous().t())):
-        loss, dx, dw = _check_loss(x, w, targets, "mean", ignore=-7)
-        assert (dx[2] == 0).all() and (dx[0, 50:] == 0).all()
+        for train in (False, True):
+            if train and (x.stride(-1) != 1 or w.stride(-1) != 1):
+                continue                                    # the C entries take rows
+            loss, dx, dw = _check_loss(x, w, targets, "mean", ignore=-7, train=train)
+            assert (dx[2] == 0).all() and (dx[0, 50:] == 0).all()
     same = _check_loss(base[:1, :1, 128:].expand(4, 60, 128), table[:, 16:144], targets, "none", ignore=-7)[0]
     assert (same[2] == 0).all()
 
@@ -360,12 +408,15 @@ def test_what_is_ignored_may_be_anything():
     targets = torch.randint(0, 300, (90,), generator=gen).cuda()
     targets[::3] = 5                                        # an index of the vocabulary that counts for nothing
     clean = _check_loss(x, w, targets, "mean", ignore=5)
+    clean_c = _check_loss(x, w, targets, "mean", ignore=5, train=True)
     x[::3] = float("nan")
     x[3], x[6] = float("inf"), -float("inf")
     a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
     loss = layers.linear_cross_entropy(a, b, targets, ignore_index=5)
-    dx, dw = torch.autograd.grad(loss, (a, b), torch.tensor(0.75, device="cuda"))
+    dloss = torch.tensor(0.75, device="cuda")
+    dx, dw = torch.autograd.grad(loss, (a, b), dloss)
     assert torch.equal(loss, clean[0]) and torch.equal(dx, clean[1]) and torch.equal(dw, clean[2])
+    assert all(torch.equal(p, q) for p, q in zip(_with_the_loss(x, w, targets, 5, "mean", BF16, dloss), clean_c))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -378,6 +429,9 @@ def test_no_token_counts(dtype):
         assert torch.isnan(loss).all() if reduction == "mean" else (loss == 0).all()
         for grad in torch.autograd.grad(loss.sum(), (x, w)):
             assert (grad == 0).all()
+        if reduction != "none" and dtype != F16:
+            loss, dx, dw = _with_the_loss(x, w, targets, -100, reduction, dtype, torch.ones((), device="cuda"))
+            assert (torch.isnan(loss) if reduction == "mean" else loss == 0) and (dx == 0).all() and (dw == 0).all()
     empty = layers.linear_cross_entropy(x[:0], w, targets[:0], reduction="none")
     assert empty.shape == (0,)
     assert float(layers.linear_cross_entropy(x[:0], w, targets[:0], reduction="sum").detach()) == 0.0
@@ -399,6 +453,8 @@ def test_targets_outside_the_vocabulary_and_values_that_are_not_finite():
     assert torch.isnan(got[bad]).all() and torch.equal(got[~bad].detach(), want[~bad])
     (dx,) = torch.autograd.grad(got, (a,), torch.ones_like(got))
     assert torch.isnan(dx[bad]).all() and torch.isfinite(dx[~bad]).all()
+    loss, dx, dw = _with_the_loss(x, w, targets, -100, "sum", BF16, torch.ones((), device="cuda"))
+    assert torch.isnan(loss) and torch.isnan(dx[bad]).all() and torch.isfinite(dx[~bad]).all() and torch.isnan(dw).all()
     targets = torch.randint(0, 30, (10,), generator=gen).cuda()
     a = x.clone()
     a[2, 5], a[7, 1] = float("nan"), float("inf")
@@ -462,6 +518,9 @@ def test_autocast_rounds_the_operands_and_keeps_the_gradients_types(product):
     with torch.autocast("cuda", dtype=product):
         _check_loss(x, w, targets, "mean", product=product)
         _check_loss(x.float(), w.bfloat16(), targets, "sum", product=product)
+    if product == BF16:
+        _check_loss(x, w, targets, "mean", product=product, train=True)
+        _check_loss(x.float(), w.bfloat16(), targets, "sum", product=product, train=True)
 
 
 def test_only_one_gradient_is_asked_for():
@@ -473,6 +532,48 @@ def test_only_one_gradient_is_asked_for():
     assert torch.equal(torch.autograd.grad(layers.linear_cross_entropy(x.detach(), w, targets), (w,))[0], both[1])
     loss = layers.linear_cross_entropy(x, w, targets)
     assert torch.equal(torch.autograd.grad(loss, (x,), retain_graph=True)[0], both[0]) and torch.equal(torch.autograd.grad(loss, (w,))[0], both[1])
+
+
+def test_large_problems_of_one_cotangent():
+    """Large enough that the Python call computes the gradients with the loss: one gradient or both, one cotangent or another, twice, an
+    empty rest of a batch, a captured step, other memory beneath the saved sums."""
+    gen = _gen(32)
+    x = torch.randn(6100, 256, device="cuda").bfloat16().requires_grad_(True)
+    w = (torch.randn(50000, 256, device="cuda") * 0.2).bfloat16().requires_grad_(True)
+    targets = torch.randint(0, 50000, (6100,), generator=gen).cuda()
+    assert _prefers(x, w, targets, -100, "mean", BF16)
+    loss = layers.linear_cross_entropy(x, w, targets)
+    both = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    _check_loss(x, w, targets, "mean")
+    assert all(torch.equal(2 * a, b) for a, b in zip(both, torch.autograd.grad(loss, (x, w), torch.tensor(2.0, device="cuda"))))
+    assert torch.equal(torch.autograd.grad(layers.linear_cross_entropy(x, w.detach(), targets), (x,))[0], both[0])
+    assert torch.equal(torch.autograd.grad(layers.linear_cross_entropy(x.detach(), w, targets), (w,))[0], both[1])
+    with torch.no_grad():
+        assert abs(float(layers.linear_cross_entropy(x, w, targets)) - float(loss.detach())) < 1e-5
+    with torch.autograd.graph.save_on_cpu():
+        loss = layers.linear_cross_entropy(x, w, targets)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), both))
+    odd = lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, odd):
+        loss = layers.linear_cross_entropy(x, w, targets)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), both))
+    (g,) = torch.autograd.grad(layers.linear_cross_entropy(x, w, targets), x, torch.ones((), device="cuda", requires_grad=True), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(layers.linear_cross_entropy(x, w, targets), (x, w))
+    torch.cuda.current_stream().wait_stream(side)
+    del loss, g
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = torch.autograd.grad(layers.linear_cross_entropy(x, w, targets), (x, w))
+    targets[100:400] = -100
+    graph.replay()
+    want = torch.autograd.grad(layers.linear_cross_entropy(x, w, targets), (x, w))
+    assert all(torch.equal(a, b) for a, b in zip(captured, want)) and (want[0][100:400] == 0).all()
+    assert _lib.device_status() == 0
 
 
 # ---- as the rest of torch uses them ------------------------------------------------------------------------------------------------

@@ -25,7 +25,7 @@ def _of(struct, ok, **changes):
 def test_structs_match_the_header_layout():
     assert ctypes.sizeof(_lib.Norm) == 200 and _lib.Norm.x.offset == 40 and _lib.Norm.stream.offset == 192
     assert ctypes.sizeof(_lib.Embedding) == 112 and _lib.Embedding.idx.offset == 32
-    assert ctypes.sizeof(_lib.LinearLoss) == 152 and _lib.LinearLoss.ignore_index.offset == 32 and _lib.LinearLoss.targets.offset == 72
+    assert ctypes.sizeof(_lib.LinearLoss) == 168 and _lib.LinearLoss.ignore_index.offset == 32 and _lib.LinearLoss.targets.offset == 72
 
 
 @pytest.mark.parametrize("status,changes", [
@@ -77,9 +77,24 @@ def test_loss_backward_refuses():
     assert lib.sa_linear_loss_backward_bytes(_of(_lib.LinearLoss, ok, struct_bytes=0)) == 0
 
 
+def test_loss_with_its_gradients_refuses():
+    lib, ok = _lib.load(), {**OK_LOSS, "dx_sums": 256, "dweight_sums": 256, "dloss": 256, "dx": 256}
+    for status, changes in ((2, dict(reduction=0)), (2, dict(product=2)), (1, dict(dx_sums=None, dweight_sums=None)), (3, dict(dx_sums=258)), (1, dict(loss=None)),
+                            (1, dict(count=None)), (4, dict(workspace_bytes=16)), (1, dict(targets=None))):
+        assert lib.sa_linear_loss_train(_of(_lib.LinearLoss, ok, **changes)) == status, changes
+    for status, changes in ((2, dict(reduction=0)), (1, dict(dloss=None)), (1, dict(dx=None)), (1, dict(dx_sums=None)), (1, dict(dweight=256, dweight_sums=None)),
+                            (3, dict(dx=257))):
+        assert lib.sa_linear_loss_scale(_of(_lib.LinearLoss, ok, **changes)) == status, changes
+    large = {**ok, "tokens": 16384, "vocab": 50304, "width": 1024, "x_stride": 1024, "weight_stride": 1024}
+    assert lib.sa_linear_loss_prefers_train(_of(_lib.LinearLoss, large)) == 1
+    for changes in (dict(tokens=64), dict(reduction=0), dict(product=2, x_dtype=2, weight_dtype=2), dict(struct_bytes=0)):
+        assert lib.sa_linear_loss_prefers_train(_of(_lib.LinearLoss, large, **changes)) == 0, changes
+
+
 def test_the_loss_takes_less_room_than_its_logits():
     """At 16,384 tokens of 50,304 words the logits are 1.6 GB in 16 bits."""
-    lib, big = _lib.load(), {**OK_LOSS, "tokens": 16384, "vocab": 50304, "width": 1024, "x_stride": 1024, "weight_stride": 1024, "dx": 256, "dweight": 256}
+    lib, big = _lib.load(), {**OK_LOSS, "tokens": 16384, "vocab": 50304, "width": 1024, "x_stride": 1024, "weight_stride": 1024, "dx": 256, "dweight": 256, "dx_sums": 256, "dweight_sums": 256}
+    assert 0 < lib.sa_linear_loss_train_bytes(_of(_lib.LinearLoss, big)) < 800e6
     assert 0 < lib.sa_linear_loss_forward_bytes(_of(_lib.LinearLoss, big)) < 120e6
     assert 0 < lib.sa_linear_loss_backward_bytes(_of(_lib.LinearLoss, big)) < 700e6
 
