@@ -105,6 +105,7 @@ int sa_norm_backward(const sa_norm* p) {
   if (need > 0 && p->workspace == nullptr) return SA_ERR_BAD_ARGUMENT;
   if (need > 0 && !aligned(p->workspace, 16)) return SA_ERR_ALIGNMENT;
   if (p->workspace_bytes < need) return SA_ERR_WORKSPACE;
+  if (tc::timeout_pending()) return SA_ERR_DEVICE_TIMEOUT;
   return norm::backward(*p, static_cast<cudaStream_t>(p->stream));
 }
 

@@ -600,21 +600,24 @@ int run_convert(const Convert& c, cudaStream_t s) {
   return launch_after(convert_kernel, dim3((unsigned)over((int64_t)c.rows * (c.pitch >> 3), 256)), 256, 0, s, c);
 }
 
+constexpr int kForwardRun = 65536;         // tokens whose half tiles are kept at a time: 200 MB of 50,304 words
+
 struct Forward {
   Room room;
   Operand x, weight;
-  int ctas;
-  Walk walk;
+  int ctas, run;
   float2 *stats, *sums, *at_target;
+  float* losses = nullptr;       // of several runs
   unsigned int* ticket;
   Forward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
     ctas = ctas_of(p.tokens);
-    walk = walk_of(p.tokens, p.vocab, p.width, terms_of(p), ctas, false);
-    stats = room.take<float2>((int64_t)2 * walk.n_tiles * p.tokens);
-    sums = room.take<float2>(over(p.tokens, 32));
-    at_target = room.take<float2>(p.tokens);
+    run = std::min(p.tokens, kForwardRun);
+    stats = room.take<float2>((int64_t)2 * walk_of(run, p.vocab, p.width, terms_of(p), ctas, false).n_tiles * run);
+    sums = room.take<float2>(over(run, 32));
+    at_target = room.take<float2>(run);
+    if (run < p.tokens && p.reduction != SA_REDUCTION_NONE) losses = room.take<float>(p.tokens);
     ticket = room.take<unsigned int>(1);
   }
 };
@@ -650,10 +653,10 @@ struct Backward {
     }
   }
   // Columns of a piece of the vocabulary: its dz takes up to 320 MB (16,384 tokens: 37 tiles of 256 columns, with four tiles across
-  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more; of the sizes down to half of that, the one that
+  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more, but no more than 8 GB; of the sizes down to half of that, the one that
   // leaves the fewest clusters idle in dW.
   static int piece_of(const Problem& p) {
-    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>(4096, (320ll << 20) / column / 256 * 256);
+    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>({256, std::min<int64_t>(4096, (8ll << 30) / column / 256 * 256), (320ll << 20) / column / 256 * 256});
     if (p.vocab <= most) return p.vocab;
     const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
     int64_t best = 0, at = blocks;
@@ -767,17 +770,24 @@ int forward(const Problem& p, cudaStream_t s) {
   if (f.x.part != 0) st = run_convert(convert_of(p, f.x, p.x, p.x_dtype, p.x_stride), s);
   if (st == SA_OK && f.weight.part != 0) st = run_convert(convert_of(p, f.weight, p.weight, p.weight_dtype, p.weight_stride), s);
   if (st != SA_OK) return st;
-  Epilogue e{};
-  e.stats = f.stats;
-  e.at_target = f.at_target;
-  e.targets = p.targets;
-  e.zeroed = f.ticket;
-  e.half = p.product == SA_F16;
-  st = run<kStats, false, false>(f.ctas, f.x, f.weight, f.walk, Origin{0, 0}, Origin{0, 0}, e, status, s);
-  if (st != SA_OK) return st;
-  return launch_after(join_kernel, dim3((unsigned)over(p.tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * f.walk.n_tiles,
-                      (const float2*)f.at_target, p.targets, p.ignore_index, p.tokens, p.vocab, p.reduction,
-                      reinterpret_cast<float2*>(p.lse), p.loss, p.count, f.sums, f.ticket);
+  for (int n0 = 0; n0 < p.tokens && st == SA_OK; n0 += f.run) {
+    const int tokens = std::min(f.run, p.tokens - n0);
+    const Walk walk = walk_of(tokens, p.vocab, p.width, terms_of(p), f.ctas, false);
+    Epilogue e{};
+    e.stats = f.stats;
+    e.at_target = f.at_target;
+    e.targets = p.targets + n0;
+    e.zeroed = f.ticket;
+    e.half = p.product == SA_F16;
+    st = run<kStats, false, false>(f.ctas, f.x, f.weight, walk, Origin{n0, 0}, Origin{0, 0}, e, status, s);
+    if (st != SA_OK) return st;
+    const bool each = f.losses != nullptr || p.reduction == SA_REDUCTION_NONE;
+    st = launch_after(join_kernel, dim3((unsigned)over(tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * walk.n_tiles, (const float2*)f.at_target,
+                      e.targets, p.ignore_index, tokens, p.vocab, each ? (int)SA_REDUCTION_NONE : p.reduction, reinterpret_cast<float2*>(p.lse) + n0,
+                      each ? (f.losses != nullptr ? f.losses : p.loss) + n0 : p.loss, p.count, f.sums, f.ticket);
+  }
+  if (st != SA_OK || f.losses == nullptr) return st;
+  return launch_after(total_kernel, dim3(1), 1024, 0, s, (const float*)f.losses, p.targets, p.ignore_index, p.tokens, p.reduction, p.loss, p.count);
 }
 
 // A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, written, read and written again, and

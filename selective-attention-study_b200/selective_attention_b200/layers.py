@@ -46,7 +46,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     """``cross_entropy(x @ weight.T, targets)`` in fp32 without the logits, for x (..., width), weight (vocab, width) and targets (...)
     int64 or int32: one number, or with ``reduction="none"`` a loss for every target (0 where it is ignored).
 
-    The forward keeps a log-sum-exp for every token; the backward computes the logits again, a piece of the vocabulary at a time.
+    The forward keeps a log-sum-exp for every token; the backward computes the logits again, a piece of the vocabulary at a time.  Where
+    ``reduction`` leaves one cotangent and the problem is large (bf16 and fp32 products), the gradients are computed with the loss
+    instead, up to the cotangent, a product less: their sums, of x's and weight's shapes in fp32, are kept for the backward, which scales
+    them.  Either way up to half a GB of what stands for logits is there at a time.
+
     x and weight have one dtype, or under autocast are rounded to its; their gradients have their own.  bf16 and fp16 products are
     exact with fp32 sums, and the gradient of the logits is rounded to that dtype between its products (fp16: scaled by the
     largest cotangent, so tokens whose cotangent is 2^-19 of it or less lose bits).  fp32 operands are split into three bf16

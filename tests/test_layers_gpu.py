@@ -365,6 +365,20 @@ def test_loss_in_several_parts(dtype, tokens, vocab, width, reduction):
         _check_loss(x, w, targets, reduction, train=True)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_of_more_tokens_than_a_run(reduction):
+    """65,536 tokens' half tiles are kept at a time."""
+    gen = _gen(33)
+    x, w = torch.randn(70001, 24, device="cuda").bfloat16(), (torch.randn(300, 24, device="cuda") * 0.4).bfloat16()
+    targets = torch.randint(0, 300, (70001,), generator=gen).cuda()
+    targets[65000:66000] = -100
+    _check_loss(x, w, targets, reduction)
+    with torch.no_grad():
+        got = layers.linear_cross_entropy(x, w, targets, reduction=reduction)
+    want = torch.nn.functional.cross_entropy((x.double() @ w.double().T), targets, reduction=reduction)
+    assert (got.double() - want).abs().max() < 1e-5
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_targets_that_are_all_but_impossible(dtype):
     """Losses beyond 44, where exponentials over the target's leave their range: the rows go through the product once more."""
