@@ -484,7 +484,7 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
   const int most = kSms / ctas;
   w.clusters = std::min(w.tiles(), most);
   w.segment = result && terms > 1 ? kSegment : w.blocks;
-  w.group = result ? 1 : std::min(w.m_tiles, 8);
+  w.group = result ? 1 : std::min(w.m_tiles, 32);
   const int left = w.tiles() % most;
   if (result && left > 0) {
     const int parts = (int)std::min<int64_t>(most / left, over(longest, kDepth) * terms / 8);

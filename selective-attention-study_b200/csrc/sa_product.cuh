@@ -220,6 +220,12 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
                "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
+// The same of what is not read again before much else has been written: it leaves L2 first.
+__device__ __forceinline__ void store32_once(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void load32(const void* p, uint32_t (&v)[8]) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
@@ -272,7 +278,7 @@ __device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], i
       uint32_t v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
-      store32(dst + 16 * h, v);
+      store32_once(dst + 16 * h, v);
     }
     if (part + 1 < e.parts) {                                                // what is left for the next part: exact
 #pragma unroll
