@@ -259,8 +259,9 @@ struct Copies {
   int64_t stride[3];                       // of rows, in bytes
   bool together[3];                        // contiguous
 };
+template <int T, int NV> constexpr int kResident = NV == 1 && T <= 32 ? 6 : 1;    // 85 registers a thread
 template <int T, int NV, bool VEC, bool BIAS>
-__global__ void __launch_bounds__(kBlock<T>) backward_copied_kernel(const sa_norm p, float* sums, const Copies c, const tc::WaitCtx status) {
+__global__ void __launch_bounds__(kBlock<T>, kResident<T, NV>) backward_copied_kernel(const sa_norm p, float* sums, const Copies c, const tc::WaitCtx status) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 buffer[2][32];
   __shared__ uint64_t full[kRing];
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kBlock<T>) backward_copied_kernel(const sa_nor
       if (threadIdx.x < 2 && n % 2 != 0) reinterpret_cast<float*>(at + c.at[3])[2 * (n - 1) + threadIdx.x] = p.stats[2 * (row0 + n - 1) + threadIdx.x];
       __syncthreads();
     }
-    for (int r0 = 0; r0 < n; r0 += kRowsOf<T>) {
+    auto rows = [&](int r0) {
       const int r = r0 + team;
       const int width = r < n ? p.width : 0;
       float h[NV][8], g[NV][8];
@@ -335,6 +336,12 @@ __global__ void __launch_bounds__(kBlock<T>) backward_copied_kernel(const sa_nor
       }
       store_row<NV, T, VEC>(g, p.dx, p.x_dtype, (row0 + r) * p.width, width, t);
       if (p.dbranch != nullptr) store_row<NV, T, VEC>(g, p.dbranch, p.branch_dtype, (row0 + r) * p.width, width, t);
+    };
+    if constexpr (T <= 32) {                                      // several rows in a turn of the loop would take too many registers
+#pragma unroll 1
+      for (int r0 = 0; r0 < n; r0 += kRowsOf<T>) rows(r0);
+    } else {
+      for (int r0 = 0; r0 < n; r0 += kRowsOf<T>) rows(r0);
     }
     __syncthreads();                                              // the stage has been read
     if (threadIdx.x == 0 && i + (int64_t)kRing * gridDim.x < stages) load(i + (int64_t)kRing * gridDim.x, slot);
@@ -395,9 +402,9 @@ int by_width(int width, F f) {
   SA_NORM_CASE(256, 32, 1);
   SA_NORM_CASE(512, 32, 2);
   SA_NORM_CASE(1024, 128, 1);
-  SA_NORM_CASE(2048, 128, 2);
-  SA_NORM_CASE(4096, 256, 2);
-  SA_NORM_CASE(8192, 512, 2);
+  SA_NORM_CASE(2048, 256, 1);
+  SA_NORM_CASE(4096, 512, 1);
+  SA_NORM_CASE(8192, 1024, 1);
   SA_NORM_CASE(16384, 1024, 2);
 #undef SA_NORM_CASE
   return SA_ERR_UNSUPPORTED;
