@@ -20,8 +20,9 @@ namespace {
 
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32;
 constexpr int kMostRows = 1600;            // of the table, a CTA of `order`: 32 counters and a place each in shared memory
-constexpr int kThreads = 256, kJoinThreads = 1024;
-constexpr int kZeroRows = 16;              // rows of the table that a CTA looks at for the ones without tokens
+constexpr int kThreads = 256, kJoinThreads = 512;
+// Rows of the table that a CTA looks at for the ones without tokens, with `groups` of them side by side.
+__host__ __device__ constexpr int zero_rows(int groups) { return groups * 4 > 16 ? groups * 4 : 16; }
 
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const sa_embedding p, int chunks) {
@@ -64,11 +65,36 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx
   const int run = ((tokens + kOrderWarps - 1) / kOrderWarps + 31) / 32 * 32;
   const int from = min(tokens, warp * run), to = min(tokens, from + run);
   int before = 0;                                                  // tokens of earlier rows
+  // A run of up to kKept groups of 32 is looked at once: a token's row and its place among its warp's tokens of the row are kept.
+  constexpr int kKept = 16;
+  const bool kept = run <= 32 * kKept;
+  int row[kKept], place[kKept];
+  if (kept) {
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+      const int n = from + 32 * k + lane;
+      const int64_t v = n < to ? idx[n] : -1;
+      before += v >= 0 && v < lo && v != skip;
+      row[k] = v >= lo && v < hi && v != skip ? (int)(v - lo) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+      place[k] = 0;
+      if (__ballot_sync(~0u, row[k] >= 0) == 0u) continue;
+      // a warp's counters are its own: of the lanes that have a row's tokens the first moves its counter on
+      const unsigned int same = __match_any_sync(~0u, row[k]);
+      if (row[k] >= 0) place[k] = counts[row[k] * kOrderWarps + warp] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (row[k] >= 0 && lane == __ffs(same) - 1) counts[row[k] * kOrderWarps + warp] += __popc(same);
+      __syncwarp();
+    }
+  } else {
 #pragma unroll 8
-  for (int n = from + lane; n < to; n += 32) {
-    const int64_t v = idx[n] == skip ? -1 : idx[n];
-    if (v >= 0 && v < lo) ++before;
-    if (v >= lo && v < hi) atomicAdd(&counts[(int)(v - lo) * kOrderWarps + warp], 1);
+    for (int n = from + lane; n < to; n += 32) {
+      const int64_t v = idx[n] == skip ? -1 : idx[n];
+      if (v >= 0 && v < lo) ++before;
+      if (v >= lo && v < hi) atomicAdd(&counts[(int)(v - lo) * kOrderWarps + warp], 1);
+    }
   }
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
   if (lane == 0) before_s[warp] = before;
@@ -119,9 +145,14 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const int64_t* idx
   }
   if (hi == vocab && threadIdx.x == 0) starts[vocab] = before;
   __syncthreads();
+  if (kept) {
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+      if (row[k] >= 0) sorted[totals[row[k]] + counts[row[k] * kOrderWarps + warp] + place[k]] = make_int2(from + 32 * k + lane, lo + row[k]);
+    return;
+  }
   constexpr int kAhead = 8;                                        // indices in flight
   for (int n0 = from; n0 < to; n0 += 32 * kAhead) {
-    int row[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int n = n0 + 32 * k + lane;
@@ -214,14 +245,15 @@ template <bool VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_blocks) {
   tc::after_previous_kernel();
   const int across = min(p.chunks, kThreads), group = threadIdx.x / across, t = blockIdx.y * kThreads + threadIdx.x - group * across;
-  if (group >= p.groups || t >= p.chunks) return;
+  if (group >= kThreads / across || t >= p.chunks) return;
   if ((int)blockIdx.x >= piece_blocks) {
-    const int v0 = ((int)blockIdx.x - piece_blocks) * kZeroRows, v1 = min(p.vocab, v0 + kZeroRows);
+    const int groups = kThreads / across, v0 = ((int)blockIdx.x - piece_blocks) * zero_rows(groups), v1 = min(p.vocab, v0 + zero_rows(groups));
     const float none[8] = {};
-    for (int v = v0 + group; v < v1; v += p.groups)
+    for (int v = v0 + group; v < v1; v += groups)
       if (p.starts[v] == p.starts[v + 1]) write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)v * p.width, t, none);
     return;
   }
+  if (group >= p.groups) return;
   const int piece = blockIdx.x * p.groups + group, all = p.starts[p.vocab];
   const int from = piece * p.piece, to = min(all, from + p.piece);
   if (from >= to) return;
@@ -260,55 +292,95 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_bl
   }
 }
 
-// Rows that cross pieces, by the piece in which they begin.  The CTA's groups take runs of the parts, and the first joins them.
+// Rows that cross pieces, by the piece in which they begin: a CTA looks at `some` pieces, a thread at one.  Groups of threads take a row
+// of few parts each; the parts of a longer one are dealt to all groups, whose sums are joined in a tree.
+constexpr int kJoinPieces = 64, kFewParts = 8;
 template <bool VEC, bool ADD>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Sum p, int some) {
   tc::after_previous_kernel();
   __shared__ float by_group[kJoinThreads][9];
+  __shared__ int2 found[kJoinPieces];                              // row, its last piece
+  __shared__ int first[kJoinPieces];
+  __shared__ int count;
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  const int all = p.starts[p.vocab];
+  if ((int)threadIdx.x < some) {
+    const int piece = blockIdx.x * some + threadIdx.x, from = piece * p.piece, to = from + p.piece;
+    if (to < all) {
+      const int row = p.sorted[to - 1].y;
+      // its last row goes on behind it, and did not begin before
+      if (p.sorted[to].y == row && p.starts[row] >= from) {
+        const int i = atomicAdd(&count, 1);                        // rows in any order
+        found[i] = make_int2(row, (p.starts[row + 1] - 1) / p.piece);
+        first[i] = piece;
+      }
+    }
+  }
+  __syncthreads();
   const int across = min(p.chunks, kJoinThreads), group = threadIdx.x / across, t = blockIdx.y * kJoinThreads + threadIdx.x - group * across;
-  const int groups = kJoinThreads / across;
-  const int all = p.starts[p.vocab], from = blockIdx.x * p.piece, to = from + p.piece;
-  if (to >= all) return;                                           // nothing behind this piece
-  const int row = p.sorted[to - 1].y;
-  if (p.sorted[to].y != row || p.starts[row] < from) return;       // its last row ends here, or began before
-  const int last = (p.starts[row + 1] - 1) / p.piece, parts = last - (int)blockIdx.x + 1;
-  const int per = (parts + groups - 1) / groups, k0 = min(parts, group * per), k1 = min(parts, k0 + per);
-  float sum[8] = {};
-  if (group < groups && t < p.chunks) {
+  int groups = kJoinThreads / across;
+  while (groups & (groups - 1)) groups &= groups - 1;              // a power of two
+  auto sum_of = [&](int piece, int k0, int k1, float (&sum)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = 0.f;
 #pragma unroll 8
     for (int k = k0; k < k1; ++k) {
       float x[8];
-      read_eight<VEC>(p, p.parts, SA_F32, ((int64_t)(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * p.width, t, x);
+      read_eight<VEC>(p, p.parts, SA_F32, ((int64_t)(piece + k) * 2 + (k == 0 ? 1 : 0)) * p.width, t, x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += x[i];
     }
+  };
+  auto finish = [&](int row, const float (&sum)[8]) {
+    float old[8] = {};
+    if (ADD) read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)row * p.width, t, old);
+    finish_row<VEC, ADD>(p, row, t, sum, old);
+  };
+  float sum[8];
+  if (group < groups && t < p.chunks)
+    for (int i = group; i < count; i += groups) {
+      const int parts = found[i].y - first[i] + 1;
+      if (parts > kFewParts) continue;
+      sum_of(first[i], 0, parts, sum);
+      finish(found[i].x, sum);
+    }
+  for (int i = 0; i < count; ++i) {
+    const int parts = found[i].y - first[i] + 1;
+    if (parts <= kFewParts) continue;
+    const int per = (parts + groups - 1) / groups, k0 = min(parts, group * per), k1 = min(parts, k0 + per);
+    const bool mine = group < groups && t < p.chunks;
+    if (mine) sum_of(first[i], k0, k1, sum);
+    for (int half = groups >> 1; half > 0; half >>= 1) {
+      __syncthreads();
+      if (mine && group >= half && group < 2 * half)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) by_group[threadIdx.x][e] = sum[e];
+      __syncthreads();
+      if (mine && group < half)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += by_group[threadIdx.x + half * across][e];
+    }
+    if (mine && group == 0) finish(found[i].x, sum);
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) by_group[threadIdx.x][i] = sum[i];
-  __syncthreads();
-  if (group != 0 || t >= p.chunks) return;
-  for (int g = 1; g < groups; ++g)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += by_group[g * across + threadIdx.x][i];
-  float old[8] = {};
-  if (ADD) read_eight<VEC>(p, p.dweight, SA_F32, (int64_t)row * p.width, t, old);
-  finish_row<VEC, ADD>(p, row, t, sum, old);
 }
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-// Sorted tokens that are summed in a row: 32, and fewer where that would leave an SM less than two pieces (2,048 tokens: 56 us with 32, 10 with
-// 4; but 16,384 with words as often as words are 47 with 32 and 60 with 8, whose parts of rows take longer to join).
-int piece_of(int tokens) {
+// Sorted tokens that are summed in a row: 32, and fewer where that would leave an SM less than two CTAs of threads with a chunk of a piece each
+// (2,048 tokens of 768: 56 us with 32, 10 with 4; but 16,384 of 1,024 with words as often as words are 47 with 32 and 60 with 8, whose
+// parts of rows take longer to join).
+int piece_of(int tokens, int width) {
+  const int64_t chunks = (width + 7) / 8;
   int piece = 32;
-  while (piece > 4 && tokens / piece < 2 * kSms) piece /= 2;
+  while (piece > 4 && tokens / piece * chunks < 2 * kSms * 128) piece /= 2;
   return piece;
 }
-int pieces_of(int tokens) { return (tokens + piece_of(tokens) - 1) / piece_of(tokens); }
+int pieces_of(int tokens, int width) { return (tokens + piece_of(tokens, width) - 1) / piece_of(tokens, width); }
 
 }  // namespace
 
 size_t sum_rows_bytes(int tokens, int vocab, int width) {
-  return (size_t)(up((int64_t)tokens * 8, 256) + up(((int64_t)vocab + 1) * 4, 256) + (int64_t)pieces_of(tokens) * 2 * width * 4);
+  return (size_t)(up((int64_t)tokens * 8, 256) + up(((int64_t)vocab + 1) * 4, 256) + (int64_t)pieces_of(tokens, width) * 2 * width * 4);
 }
 size_t backward_bytes(const sa_embedding& p) { return sum_rows_bytes(p.tokens, p.vocab, p.width); }
 
@@ -328,16 +400,18 @@ int sum_rows(const RowSums& p, cudaStream_t s) {
   const int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.skip, p.tokens,
                         p.vocab, rows, sorted, starts);
   if (st != SA_OK) return st;
-  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p.tokens), piece_of(p.tokens)};
-  a.groups = a.chunks < kThreads ? kThreads / a.chunks : 1;
+  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p.tokens, p.width), piece_of(p.tokens, p.width)};
+  a.groups = a.chunks < kThreads ? std::min(kThreads / a.chunks, std::max(1, a.pieces / (2 * kSms))) : 1;
   const bool vec = p.width % 8 == 0 && eights(p.dy, p.dtype, p.dy_stride, p.tokens) && eights(p.out, p.out_dtype, p.width, p.vocab);
   const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;
-  const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + kZeroRows - 1) / kZeroRows), (a.chunks + kThreads - 1) / kThreads);
+  const int across = kThreads / std::min(a.chunks, kThreads);           // rows side by side
+  const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + zero_rows(across) - 1) / zero_rows(across)), (a.chunks + kThreads - 1) / kThreads);
   auto launch = [&](auto vec_, auto add) {
     constexpr bool VEC = decltype(vec_)::value, ADD = decltype(add)::value;
     const int status = launch_after(sum_kernel<VEC, ADD>, grid, kThreads, 0, s, a, piece_blocks);
     if (status != SA_OK || a.pieces < 2) return status;
-    return launch_after(join_kernel<VEC, ADD>, dim3(a.pieces - 1, (a.chunks + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s, a);
+    const int some = std::min(kJoinPieces, std::max(1, a.pieces / (4 * kSms)));
+    return launch_after(join_kernel<VEC, ADD>, dim3((a.pieces - 2) / some + 1, (a.chunks + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s, a, some);
   };
   const std::true_type yes;
   const std::false_type no;
