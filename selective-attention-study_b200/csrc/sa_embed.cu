@@ -245,9 +245,9 @@ template <bool VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum p, int piece_blocks) {
   tc::after_previous_kernel();
   const int across = min(p.chunks, kThreads), group = threadIdx.x / across, t = blockIdx.y * kThreads + threadIdx.x - group * across;
-  if (group >= kThreads / across || t >= p.chunks) return;
+  if (group >= (int)blockDim.x / across || t >= p.chunks) return;
   if ((int)blockIdx.x >= piece_blocks) {
-    const int groups = kThreads / across, v0 = ((int)blockIdx.x - piece_blocks) * zero_rows(groups), v1 = min(p.vocab, v0 + zero_rows(groups));
+    const int groups = (int)blockDim.x / across, v0 = ((int)blockIdx.x - piece_blocks) * zero_rows(groups), v1 = min(p.vocab, v0 + zero_rows(groups));
     const float none[8] = {};
     for (int v = v0 + group; v < v1; v += groups)
       if (p.starts[v] == p.starts[v + 1]) write_eight<VEC>(p, p.dweight, p.weight_dtype, (int64_t)v * p.width, t, none);
@@ -404,11 +404,12 @@ int sum_rows(const RowSums& p, cudaStream_t s) {
   a.groups = a.chunks < kThreads ? std::min(kThreads / a.chunks, std::max(1, a.pieces / (2 * kSms))) : 1;
   const bool vec = p.width % 8 == 0 && eights(p.dy, p.dtype, p.dy_stride, p.tokens) && eights(p.out, p.out_dtype, p.width, p.vocab);
   const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;
-  const int across = kThreads / std::min(a.chunks, kThreads);           // rows side by side
-  const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + zero_rows(across) - 1) / zero_rows(across)), (a.chunks + kThreads - 1) / kThreads);
+  // as many threads as the groups need: a thread takes 80 to 128 registers
+  const int across = std::min(a.chunks, kThreads), threads = (int)up(a.groups * across, 32), side = threads / across;
+  const dim3 grid(piece_blocks + (p.add ? 0 : (p.vocab + zero_rows(side) - 1) / zero_rows(side)), (a.chunks + kThreads - 1) / kThreads);
   auto launch = [&](auto vec_, auto add) {
     constexpr bool VEC = decltype(vec_)::value, ADD = decltype(add)::value;
-    const int status = launch_after(sum_kernel<VEC, ADD>, grid, kThreads, 0, s, a, piece_blocks);
+    const int status = launch_after(sum_kernel<VEC, ADD>, grid, threads, 0, s, a, piece_blocks);
     if (status != SA_OK || a.pieces < 2) return status;
     const int some = std::min(kJoinPieces, std::max(1, a.pieces / (4 * kSms)));
     return launch_after(join_kernel<VEC, ADD>, dim3((a.pieces - 2) / some + 1, (a.chunks + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s, a, some);
