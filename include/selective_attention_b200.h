@@ -492,7 +492,7 @@ int sa_linear_loss_scale(const sa_linear_loss* p);
  *   stats    (rows, 2) fp32, mean and 1 / sqrt(var + eps): written by the forward (may be null there), read by the backward
  * Backward: x is s, at x_stride.  dy and (may be null) dsum, the gradient that s has from elsewhere, at row strides; dx of x's type and
  * dbranch of branch_dtype (may be null) contiguous; dweight, dbias (may be null) of weight_dtype.
- *   workspace  sa_norm_backward_bytes(), 16-byte aligned; parameters' sums over rows are taken in an order that the sizes alone decide */
+ *   workspace  sa_norm_backward_bytes(), 16-byte aligned; parameters' sums over rows are taken in an order that sizes and alignment alone decide */
 typedef struct sa_norm {
   int32_t struct_bytes;   /* sizeof(sa_norm) */
   int32_t x_dtype, branch_dtype, y_dtype, weight_dtype;
