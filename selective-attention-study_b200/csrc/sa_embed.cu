@@ -400,7 +400,8 @@ int sum_rows(const RowSums& p, cudaStream_t s) {
   const int st = launch_after(order_kernel, dim3((p.vocab + rows - 1) / rows), kOrderThreads, (size_t)rows * (kOrderWarps + 1) * 4, s, p.idx, p.skip, p.tokens,
                         p.vocab, rows, sorted, starts);
   if (st != SA_OK) return st;
-  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p.tokens, p.width), piece_of(p.tokens, p.width)};
+  Sum a{sorted, starts, p.dy, p.dtype, p.dy_stride, p.factor, p.out, p.out_dtype, p.scale, p.vocab, p.width, (p.width + 7) / 8, 0, parts, pieces_of(p.tokens, p.width),
+        piece_of(p.tokens, p.width)};
   a.groups = a.chunks < kThreads ? std::min(kThreads / a.chunks, std::max(1, a.pieces / (2 * kSms))) : 1;
   const bool vec = p.width % 8 == 0 && eights(p.dy, p.dtype, p.dy_stride, p.tokens) && eights(p.out, p.out_dtype, p.width, p.vocab);
   const int piece_blocks = (a.pieces + a.groups - 1) / a.groups;

@@ -9,13 +9,15 @@
 // up to that number, and no logit twice.  Tokens come in runs; of a run, the product's epilogue keeps e = exp(z - ref) in 16 bits
 // beside the rows' sums s.  softmax(z) = e / s, so the rest is a scale of rows, of the result in dx = (1 / s) e W and of the
 // right operand in dW = e^T (x / s).  e is 0 at the target: its part, c = softmax - 1, is added in fp32, dx_n += c W_t and dW_t +=
-// the sum of c x_n over its tokens, sorted as in an embedding's gradient.  ref is the target's logit, a dot product beforehand: exp(z - ref) is 1 at the target and at most
-// e^loss elsewhere, which 8 bits of exponent hold with room for 1 / s up to a loss of 44.  Rows beyond that are found by the sums
-// and go through the product once more with their maximum for ref.  Three products of 2 N V d operations; the sums of dW over the runs stay in fp32.
+// the sum of c x_n over its tokens, sorted as in an embedding's gradient.  ref is the target's logit, a dot product beforehand:
+// exp(z - ref) is 1 at the target and at most e^loss elsewhere, which 8 bits of exponent hold with room for 1 / s up to a loss of
+// 44.  Rows beyond that are found by the sums and go through the product once more with their maximum for ref.  Three products of
+// 2 N V d operations; the sums of dW over the runs stay in fp32.
 //
-// Otherwise (a cotangent for every token; fp16, whose five bits of exponent do not hold e): the backward computes the logits again
-// in pieces of the vocabulary, turns a piece's into dz in 16 bits, and reads them with the two products of the gradients.  Four products
-// in all; the sums of dx over the pieces stay in fp32.
+// Otherwise (a cotangent for every token; fp16, whose five bits of exponent do not hold e; problems so small that a product costs
+// less than the sums of the gradients, written and read): the backward computes the logits again in pieces of the vocabulary, turns
+// a piece's into dz in 16 bits, and reads them with the two products of the gradients.  Four products in all; the sums of dx over
+// the pieces stay in fp32.
 #include "sa_loss.cuh"
 
 #include <algorithm>
@@ -502,7 +504,8 @@ template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_a, Origin at_b, int a_bytes, const Epilogue& e, const WaitCtx& status,
            cudaStream_t s) {
   auto kernel = product_kernel<CTAS, KIND, A_MN, B_MN>;
-  SA_CUDA_CHECK(allow_smem(kernel, kSmem));
+  constexpr size_t kBytes = KIND == kResult ? kSmemResult : kSmem;
+  SA_CUDA_CHECK(allow_smem(kernel, kBytes));
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
@@ -513,7 +516,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(w.clusters * CTAS);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = kSmem;
+  config.dynamicSmemBytes = kBytes;
   config.stream = s;
   config.attrs = attrs;
   config.numAttrs = 2;
@@ -653,10 +656,11 @@ struct Backward {
     }
   }
   // Columns of a piece of the vocabulary: its dz takes up to 320 MB (16,384 tokens: 37 tiles of 256 columns, with four tiles across
-  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more, but no more than 8 GB; of the sizes down to half of that, the one that
-  // leaves the fewest clusters idle in dW.
+  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more, but no more than 8 GB; of the sizes down to half of
+  // that, the one that leaves the fewest clusters idle in dW.
   static int piece_of(const Problem& p) {
-    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), most = std::max<int64_t>({256, std::min<int64_t>(4096, (8ll << 30) / column / 256 * 256), (320ll << 20) / column / 256 * 256});
+    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), in_320mb = (320ll << 20) / column / 256 * 256;
+    const int64_t in_8gb = (8ll << 30) / column / 256 * 256, most = std::max<int64_t>({256, std::min<int64_t>(4096, in_8gb), in_320mb});
     if (p.vocab <= most) return p.vocab;
     const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
     int64_t best = 0, at = blocks;
@@ -683,8 +687,10 @@ int finish(const Epilogue& e, const Walk& w, int ctas, cudaStream_t s) {
 
 // A product into a result, by kResult or, for fp32 operands, kSegments.
 template <bool A_MN, bool B_MN>
-int run_result(const Problem& p, int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, const Epilogue& e,
+int run_result(const Problem& p, int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, Epilogue e,
                const WaitCtx& status, cudaStream_t s) {
+  e.aligned = ((reinterpret_cast<uintptr_t>(e.out) | (uintptr_t)e.out_pitch * bytes_of(e.dtype)) & (e.dtype == SA_F32 ? 31 : 15)) == 0;
+  e.addend_first = ((reinterpret_cast<uintptr_t>(e.addend) | (uintptr_t)e.addend_pitch * 4) & 31) == 0;
   return p.product == SA_F32 ? run<kSegments, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s)
                              : run<kResult, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s);
 }
@@ -790,10 +796,10 @@ int forward(const Problem& p, cudaStream_t s) {
   return launch_after(total_kernel, dim3(1), 1024, 0, s, (const float*)f.losses, p.targets, p.ignore_index, p.tokens, p.reduction, p.loss, p.count);
 }
 
-// A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, written, read and written again, and
-// eight more launches: the smaller of both estimates, in us at 1.4 PFLOP/s (fp32: 0.75) and 6.4 TB/s.  Measured, bf16: 4,096 tokens of 8,000 words
-// of 1,024 202 us by computing the logits again and 232 with the loss, 64 of 50,304 136 and 224, 2,048 of 50,304 of 768 600 and 519; fp32: 1,024 of 8,000
-// of 512 216 and 212, 512 of 32,000 of 768 634 and 588.
+// A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, written, read and written
+// again, and eight more launches: the smaller of both estimates, in us at 1.4 PFLOP/s (fp32: 0.75) and 6.4 TB/s.  Measured, bf16:
+// 4,096 tokens of 8,000 words of 1,024 202 us by computing the logits again and 232 with the loss, 64 of 50,304 136 and 224, 2,048 of
+// 50,304 of 768 600 and 519; fp32: 1,024 of 8,000 of 512 216 and 212, 512 of 32,000 of 768 634 and 588.
 bool prefers_train(const Problem& p) {
   if (p.reduction == SA_REDUCTION_NONE || p.product == SA_F16) return false;
   const double values = (double)p.vocab * p.width, tokens = (double)up(p.tokens, kRows);

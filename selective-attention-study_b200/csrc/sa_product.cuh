@@ -23,6 +23,8 @@ constexpr int kStages = 6;
 constexpr int kThreads = 384;              // warp 0 loads, warp 1 issues, warp 2 has the tensor memory, warps 4 to 11 read it
 constexpr int kEpilogueWarps = 8;
 constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
+constexpr int kTurnPitch = 33;               // words of 32 columns that a warp turns
+constexpr size_t kSmemResult = kSmem + (size_t)kEpilogueWarps * 32 * kTurnPitch * 4;
 constexpr int kTerms = 6;                  // of an fp32 product
 constexpr int kSegment = 4;                // stages, with kSegments: 256 of the contraction
 constexpr int kSegmentChunks = 4;          // chunks of 32 columns of a tile that a thread of an epilogue has, at most
@@ -120,8 +122,10 @@ struct Epilogue {
   void* out;
   int dtype;
   int64_t out_pitch;
+  int aligned;                             // its rows start where whole vectors are stored: set with the launch
   const float* addend;                     // fp32, may be null
   int64_t addend_pitch;
+  int addend_first;                        // its rows start at 32 bytes; others have no scale and no table beside them.  Set with the launch
   const float* scale;                      // may be null
   int scale_rows;                          // one for every row
   float* slabs;
@@ -398,39 +402,88 @@ __device__ __forceinline__ void load_columns(const void* base, int dtype, int64_
     }
 }
 
-// 32 columns of a row of the result, or of a slab.
-__device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, const Units& u, uint32_t (&r)[32], int row, int in_tile, int tile_rows,
-                                             int chunk) {
-  const int col = u.tn * w.bn + chunk * 32, valid = w.n - col;
-  if (valid <= 0) return;
+// Stores 32 columns of a warp's `rows` rows, `valid` of them inside, where rows start anywhere: turned in shared memory, so that a store runs
+// along a row (two tokens' gradient of 93,968 words of 2,926, in bf16: 352 us, a row a thread 2,140).
+template <typename T>
+__device__ __forceinline__ void store_across(T* out, int64_t pitch, const float* addend, int64_t addend_pitch, const uint32_t (&r)[32], int rows,
+                                             int valid, int lane, float* turn) {
+  constexpr int kBatch = 8;                // rows whose values and addends are in flight
+#pragma unroll
+  for (int j = 0; j < 32; ++j) turn[lane * kTurnPitch + j] = __uint_as_float(r[j]);
+  __syncwarp();
+  if (lane < valid) {
+    out += lane;
+    for (int i0 = 0; i0 < rows; i0 += kBatch) {
+      float v[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) v[k] = turn[(i0 + k) * kTurnPitch + lane];
+      if (addend != nullptr) {
+        float also[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) also[k] = i0 + k < rows ? addend[(i0 + k) * addend_pitch + lane] : 0.f;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) v[k] += also[k];
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (i0 + k < rows) {
+          if constexpr (sizeof(T) == 4) *out = v[k];
+          else if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(v[k]);
+          else *out = __float2bfloat16_rn(v[k]);
+        }
+        out += pitch;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// 32 columns of a warp's 32 rows of the result, or of a slab; a thread's row is `row0` and its lane.  With `turn`, rows that start anywhere
+// go across: the fp32 products' sums leave no registers for that, and their stores wait for the tensor cores anyway.
+__device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, const Units& u, uint32_t (&r)[32], int row0, int lane, int in_tile,
+                                             int tile_rows, int chunk, float* turn) {
+  const int col = u.tn * w.bn + chunk * 32, valid = w.n - col, row = row0 + lane;
+  const bool across = turn != nullptr && !e.aligned && u.tile < w.whole, inside = row < w.m;
+  if (valid <= 0 || row0 >= w.m || (!inside && !across)) return;
   if (u.tile >= w.whole) {
     float* const slab = e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * tile_rows + in_tile) * w.bn + chunk * 32;
     if (e.later) add_row(slab, r, 32);
     store_row(slab, r, 32);
     return;
   }
-  if (e.addend != nullptr) add_row(e.addend + (int64_t)row * e.addend_pitch + col, r, valid);
-  if (e.scale != nullptr) {
-    const float scale = e.scale[e.scale_rows ? row : 0];
+  if (inside) {
+    if (e.addend != nullptr && (!across || e.addend_first)) add_row(e.addend + (int64_t)row * e.addend_pitch + col, r, valid);
+    if (e.scale != nullptr) {
+      const float scale = e.scale[e.scale_rows ? row : 0];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
-  }
-  if (e.table != nullptr && e.table_factor[row] != 0.f) {
-    const int64_t t = e.targets[row];
-    const float factor = e.table_factor[row];
-    if (t >= 0 && t < e.vocab) {
+      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+    }
+    if (e.table != nullptr && e.table_factor[row] != 0.f) {
+      const int64_t t = e.targets[row];
+      const float factor = e.table_factor[row];
+      if (t >= 0 && t < e.vocab) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v[8];
-        load_columns(e.table, e.table_dtype, t * e.table_stride, col + 8 * k, w.n, v);
+        for (int k = 0; k < 4; ++k) {
+          float v[8];
+          load_columns(e.table, e.table_dtype, t * e.table_stride, col + 8 * k, w.n, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[8 * k + j] = __float_as_uint(fmaf(factor, v[j], __uint_as_float(r[8 * k + j])));
+          for (int j = 0; j < 8; ++j) r[8 * k + j] = __float_as_uint(fmaf(factor, v[j], __uint_as_float(r[8 * k + j])));
+        }
       }
     }
   }
-  const int64_t at = (int64_t)row * e.out_pitch + col;
-  if (e.dtype == SA_F32) store_row(static_cast<float*>(e.out) + at, r, valid);
-  else store_row(static_cast<uint16_t*>(e.out) + at, r, valid, e.dtype == SA_F16);
+  if (!across) {
+    const int64_t at = (int64_t)row * e.out_pitch + col;
+    if (e.dtype == SA_F32) store_row(static_cast<float*>(e.out) + at, r, valid);
+    else store_row(static_cast<uint16_t*>(e.out) + at, r, valid, e.dtype == SA_F16);
+    return;
+  }
+  const int64_t at = (int64_t)row0 * e.out_pitch + col;
+  const float* const addend = e.addend != nullptr && !e.addend_first ? e.addend + (int64_t)row0 * e.addend_pitch + col : nullptr;
+  const int rows = min(32, w.m - row0);
+  if (e.dtype == SA_F32) store_across(static_cast<float*>(e.out) + at, e.out_pitch, addend, e.addend_pitch, r, rows, valid, lane, turn);
+  else if (e.dtype == SA_BF16) store_across(static_cast<__nv_bfloat16*>(e.out) + at, e.out_pitch, addend, e.addend_pitch, r, rows, valid, lane, turn);
+  else store_across(static_cast<__half*>(e.out) + at, e.out_pitch, addend, e.addend_pitch, r, rows, valid, lane, turn);
 }
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
@@ -555,6 +608,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;              // 32 lanes, in bits 16 on
     const uint32_t read_there = CTAS == 2 ? address_in(read, 0) : read;
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 128 && e.zeroed != nullptr) *e.zeroed = 0u;
+    float* const turn = reinterpret_cast<float*>(smem + kStages * 2 * kOperand) + (warp - 4) * 32 * kTurnPitch;    // kResult
     uint32_t sums[KIND == kSegments ? kSegmentChunks : 1][32];
     int n = 0;
     while (u.next(w)) {
@@ -626,7 +680,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           uint32_t r[32];
           tmem_ld32(acc + i * 32, r);
           tmem_ld_wait();
-          if (inside) store_result(e, w, u, r, row, in_tile, kColumns, i);
+          store_result(e, w, u, r, row - lane, lane, in_tile, kColumns, i, turn);
         }
       } else {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
@@ -646,7 +700,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (u.last && inside) {
 #pragma unroll
           for (int i = 0; i < kSegmentChunks; ++i)
-            if (from + i < to) store_result(e, w, u, sums[i], row, in_tile, kColumns, from + i);
+            if (from + i < to) store_result(e, w, u, sums[i], row - lane, lane, in_tile, kColumns, from + i, nullptr);
         }
       }
       tc_fence_before_sync();

@@ -365,6 +365,21 @@ def test_loss_in_several_parts(dtype, tokens, vocab, width, reduction):
         _check_loss(x, w, targets, reduction, train=True)
 
 
+@pytest.mark.parametrize("dtype,width,reduction", [
+    (BF16, 259, "none"), (F16, 262, "sum"), (BF16, 261, "mean"), (BF16, 264, "none"), (F32, 65, "mean")])
+def test_rows_of_gradients_that_start_anywhere(dtype, width, reduction):
+    """Tiles enough that most are stored whole, in several pieces or runs, into rows that start at 2, 4, 8 or 16 bytes."""
+    gen = _gen(12)
+    tokens, vocab = (19500, 19201) if dtype != F32 else (5000, 19201)
+    x = torch.randn(tokens, width, device="cuda").to(dtype)
+    w = (torch.randn(vocab, width, device="cuda") * 0.2).to(dtype)
+    targets = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
+    targets[5::11] = -100
+    _check_loss(x, w, targets, reduction)
+    if dtype != F16:
+        _check_loss(x, w, targets, "sum", train=True)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_loss_of_more_tokens_than_a_run(reduction):
     """65,536 tokens' half tiles are kept at a time."""
