@@ -391,12 +391,16 @@ bool vectors(const sa_norm& p, bool backward) {
          eights(p.dbranch, p.branch_dtype, w, 1);
 }
 
-// Threads and values of a row by its width: f(threads, chunks of 8 a thread).
+// Threads and values of a row by its width: f(threads, chunks of 8 a thread).  As few threads as hold it: with eight, 5,333,333 rows of 3
+// bf16 values took 335 us forward and 936 with the gradients, with one 41 and 139; 500,000 of 32 25 and 80, with four 14 and 76.
 template <typename F>
 int by_width(int width, F f) {
   using std::integral_constant;
 #define SA_NORM_CASE(most, threads, chunks) \
   if (width <= most) return f(integral_constant<int, threads>(), integral_constant<int, chunks>())
+  SA_NORM_CASE(8, 1, 1);
+  SA_NORM_CASE(16, 2, 1);
+  SA_NORM_CASE(32, 4, 1);
   SA_NORM_CASE(64, 8, 1);
   SA_NORM_CASE(128, 16, 1);
   SA_NORM_CASE(256, 32, 1);

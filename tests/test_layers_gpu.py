@@ -102,6 +102,15 @@ def test_layer_norm_and_its_gradients(shape, xt, bt, wt, yt, bias):
         _check("dbias", grads[at + 1], dy.double().sum(rows), many * step * dy.double().abs().sum(rows))
 
 
+@pytest.mark.parametrize("shape,xt,bt,yt,bias", [
+    ((1, 5), F32, None, F32, True), ((50001, 3), BF16, None, BF16, True), ((9999, 7), F32, BF16, BF16, True), ((257, 1), F32, None, BF16, True),
+    ((5000, 8), BF16, BF16, BF16, False), ((129, 8), F32, None, F32, True), ((4097, 9), F16, F16, F16, True), ((3, 700, 16), BF16, None, F32, False),
+    ((2049, 15), F16, None, F32, True), ((63, 31), F32, F16, F32, True), ((30011, 32), BF16, BF16, BF16, True), ((2, 24), F16, None, F16, False)])
+def test_rows_of_a_few_values(shape, xt, bt, yt, bias):
+    """One, two or four threads a row."""
+    test_layer_norm_and_its_gradients(shape, xt, bt, F32 if xt == F32 else xt, yt, bias)
+
+
 def test_layer_norm_without_parameters_and_without_gradients():
     gen = _gen(1)
     x = _randn(gen, 12, 100, dtype=BF16)
