@@ -151,8 +151,10 @@ __device__ __forceinline__ uint32_t address_in(uint32_t addr, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// Relaxed: what it tells of are loads from tensor memory whose values are there.  A release to the cluster would also wait for the warp's
+// stores to global memory.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -242,26 +244,87 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Waits for the loads from tensor memory; the values are there behind it, for the compiler too.
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 // ---- epilogues: 32 columns of a row in registers ----------------------------------------------------------------------------------
+
+// Two values in a register pair: one instruction for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 both(Pair x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float most_of(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The largest of 32 columns and of `than`, by four chains.
+__device__ __forceinline__ float most_of(const uint32_t (&r)[32], float than) {
+  float m[4] = {than, __uint_as_float(r[1]), __uint_as_float(r[2]), __uint_as_float(r[3])};
+  m[0] = fmaxf(m[0], __uint_as_float(r[0]));
+#pragma unroll
+  for (int i = 4; i < 32; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      m[k] = i + 4 + k < 32 ? most_of(m[k], __uint_as_float(r[i + k]), __uint_as_float(r[i + 4 + k])) : fmaxf(m[k], __uint_as_float(r[i + k]));
+  return fmaxf(most_of(m[0], m[1], m[2]), m[3]);
+}
+// exp2(z log2 e - from) of 32 columns, and their sum.
+__device__ __forceinline__ float exponentials(const uint32_t (&r)[32], float from, float (&p)[32]) {
+  const Pair by = pair(kLog2e, kLog2e), less = pair(-from, -from);
+  Pair sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const float2 x = both(fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), by, less));
+    p[i] = ex2(x.x);
+    p[i + 1] = ex2(x.y);
+    sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], pair(p[i], p[i + 1]));
+  }
+  const float2 a = both(sums[0]), b = both(sums[1]);
+  return (a.x + a.y) + (b.x + b.y);
+}
 
 // Running maximum, in log2 units and rounded, and sum of exponentials above it.  The differences are taken before they are rounded:
 // a rounded logit of 100 would move its exponential by 2^-18.
 struct RowStats {
   float top = -INFINITY, from = 0.f, sum = 0.f;             // from: top * log2 e, or 0 while nothing is above -inf
-  __device__ __forceinline__ void add(const uint32_t (&r)[32], int valid) {
-    float z[32], best = top;
+  __device__ __forceinline__ void add(uint32_t (&r)[32], int valid) {
+    if (valid < 32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] = i < valid ? __uint_as_float(r[i]) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) best = fmaxf(best, z[i]);
-    const float to = best == -INFINITY ? 0.f : best * kLog2e;
+      for (int i = 0; i < 32; ++i) r[i] = i < valid ? r[i] : __float_as_uint(-INFINITY);
+    }
+    const float best = most_of(r, top), to = best == -INFINITY ? 0.f : best * kLog2e;
     sum *= top == -INFINITY ? 0.f : ex2(from - to);
     top = best;
     from = to;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) part[i & 3] += ex2(__fmaf_rn(z[i], kLog2e, -from));
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
+    float p[32];
+    sum += exponentials(r, from, p);
   }
   __device__ __forceinline__ float2 result() const { return make_float2(top == -INFINITY ? top : from, sum); }
 };
@@ -270,8 +333,8 @@ __device__ __forceinline__ float2 in_log2(float z) {         // z * log2 e in tw
   return make_float2(hi, fabsf(hi) < INFINITY ? __fmaf_rn(z, kLog2e, -hi) : 0.f);
 }
 
-// 32 columns rounded to the parts.
-__device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], int64_t at) {
+// 32 columns rounded to the parts; exactly nothing of a token that does not count, whatever they are.
+__device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], bool counts, int64_t at) {
   for (int part = 0; part < e.parts; ++part) {
     uint32_t w[16];
 #pragma unroll
@@ -281,7 +344,7 @@ __device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], i
     for (int h = 0; h < 2; ++h) {
       uint32_t v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = w[8 * h + i];
+      for (int i = 0; i < 8; ++i) v[i] = counts ? w[8 * h + i] : 0u;
       store32_once(dst + 16 * h, v);
     }
     if (part + 1 < e.parts) {                                                // what is left for the next part: exact
@@ -303,13 +366,21 @@ __device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
 
 // (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
 __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int64_t at, float2 lse, float factor, int target) {
+  const Pair by = pair(kLog2e, kLog2e), less = pair(-lse.x, -lse.x), less_still = pair(-lse.y, -lse.y);
   float p[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    p[i] = ex2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse.x) - lse.y);
-    p[i] = factor == 0.f ? 0.f : (i == target ? p[i] - 1.f : p[i]) * factor;   // a token that does not count: exactly nothing
+  for (int i = 0; i < 32; i += 2) {
+    const float2 x = both(add2(fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), by, less), less_still));
+    p[i] = ex2(x.x);
+    p[i + 1] = ex2(x.y);
   }
-  store_parts(e, p, at);
+  if (target >= 0) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) p[i] = i == target ? p[i] - 1.f : p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) p[i] *= factor;
+  store_parts(e, p, factor != 0.f, at);
 }
 
 // 32 columns of a row in fp32, `valid` of them inside.
@@ -620,68 +691,77 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       wait(done + 8 * (n & 1), (n >> 1) & 1, 1004);
       __syncwarp();
       tc_fence_after_sync();
+      auto release = [&] {                                           // all that this warp reads of the accumulator has been read
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CTAS == 2) arrive_cluster(read_there + 8 * (n & 1));
+          else mbar_arrive(read + 8 * (n & 1));
+        }
+      };
+      // The chunks in turn, the next one's load on its way meanwhile; the accumulator goes back before the last one's arithmetic.
+      auto each_chunk = [&](auto f) {
+        uint32_t r[2][32];
+        if (from < to) tmem_ld32(acc + from * 32, r[0]);
+        else release();
+        for (int i = from; i < to; i += 2) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (i + h >= to) break;
+            tmem_loaded(r[h]);
+            if (i + h + 1 < to) tmem_ld32(acc + (i + h + 1) * 32, r[h ^ 1]);
+            else release();
+            f(i + h, r[h]);
+          }
+        }
+      };
       if constexpr (KIND == kStats) {
         const int64_t target = inside ? e.targets[row] : -1;
         RowStats stats;
-        for (int i = from; i < to; ++i) {
-          uint32_t r[32];
-          tmem_ld32(acc + i * 32, r);
-          tmem_ld_wait();
+        each_chunk([&](int i, uint32_t (&r)[32]) {
           const int col = u.tn * w.bn + i * 32;
           stats.add(r, w.n - col);
           const int64_t mine = target - e.column0 - col;
           if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = in_log2(select(r, (int)mine));
-        }
+        });
         if (inside) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = stats.result();
       } else if constexpr (KIND == kBoth) {
         const int64_t target = inside ? e.targets[row] : -1;
         const float ref = inside ? e.ref[row] : INFINITY;
         const bool store = inside && (e.only == nullptr || e.only[row] != 0);
         float top = -INFINITY, sum = 0.f;
-        for (int i = from; i < to; ++i) {
-          uint32_t r[32];
-          tmem_ld32(acc + i * 32, r);
-          tmem_ld_wait();
+        each_chunk([&](int i, uint32_t (&r)[32]) {
           const int col = u.tn * w.bn + i * 32, valid = w.n - col;
           const int64_t mine = target - e.column0 - col;
-          float p[32], part[4] = {0.f, 0.f, 0.f, 0.f};
+          float p[32];
+          if (valid < 32) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const bool counts = j < valid && ref != INFINITY;
-            top = j < valid ? fmaxf(top, __uint_as_float(r[j])) : top;
-            p[j] = ex2(__fmaf_rn(__uint_as_float(r[j]), kLog2e, -ref));
-            p[j] = counts ? p[j] : 0.f;
-            part[j & 3] += p[j];
+            for (int j = 0; j < 32; ++j) r[j] = j < valid ? r[j] : __float_as_uint(-INFINITY);
           }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          top = most_of(r, top);
+          sum += exponentials(r, ref, p);
           if (store && mine >= 0 && mine < 32 && mine < valid) {
             const float z = select(r, (int)mine);
             e.at_target[row] = in_log2(z);
             e.e_target[row] = ex2(__fmaf_rn(z, kLog2e, -ref));        // as it stands in the sum
           }
-          if (store) store_parts(e, p, (int64_t)row * e.p_pitch + col);
-        }
-        if (store) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(top * kLog2e, sum);
+          if (store) store_parts(e, p, ref != INFINITY, (int64_t)row * e.p_pitch + col);
+        });
+        if (store) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(top * kLog2e, ref != INFINITY ? sum : 0.f);
       } else if constexpr (KIND == kProbabilities) {
         const float2 lse = inside ? e.lse[row] : make_float2(0.f, 0.f);
         const float factor = inside ? e.factor[row] : 0.f;
         const int64_t target = inside ? e.targets[row] : -1;
-        for (int i = from; i < to; ++i) {
-          uint32_t r[32];
-          tmem_ld32(acc + i * 32, r);
-          tmem_ld_wait();
+        each_chunk([&](int i, uint32_t (&r)[32]) {
           const int col = u.tn * w.bn + i * 32;
           const int64_t mine = target - e.column0 - col;
           if (inside) store_probabilities(e, r, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
-        }
+        });
       } else if constexpr (KIND == kResult) {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
-        for (int i = from; i < to; ++i) {
-          uint32_t r[32];
-          tmem_ld32(acc + i * 32, r);
-          tmem_ld_wait();
+        each_chunk([&](int i, uint32_t (&r)[32]) {
           store_result(e, w, u, r, row - lane, lane, in_tile, kColumns, i, turn);
-        }
+        });
       } else {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
 #pragma unroll
@@ -703,12 +783,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (from + i < to) store_result(e, w, u, sums[i], row - lane, lane, in_tile, kColumns, from + i, nullptr);
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CTAS == 2) arrive_cluster(read_there + 8 * (n & 1));
-        else mbar_arrive(read + 8 * (n & 1));
-      }
+      if constexpr (KIND == kSegments) release();
       ++n;
     }
   }
