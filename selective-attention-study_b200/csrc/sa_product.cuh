@@ -699,20 +699,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           else mbar_arrive(read + 8 * (n & 1));
         }
       };
-      // The chunks in turn, the next one's load on its way meanwhile; the accumulator goes back before the last one's arithmetic.
+      // The chunks in turn; the accumulator goes back before the last one's arithmetic.  (The next chunk's load before a chunk's arithmetic:
+      // +4 to +10 % at widths up to 512.  Sixteen warps: -8 % at 64, +2 % from 768 on.)
       auto each_chunk = [&](auto f) {
-        uint32_t r[2][32];
-        if (from < to) tmem_ld32(acc + from * 32, r[0]);
-        else release();
-        for (int i = from; i < to; i += 2) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (i + h >= to) break;
-            tmem_loaded(r[h]);
-            if (i + h + 1 < to) tmem_ld32(acc + (i + h + 1) * 32, r[h ^ 1]);
-            else release();
-            f(i + h, r[h]);
-          }
+        if (from == to) release();
+        for (int i = from; i < to; ++i) {
+          uint32_t r[32];
+          tmem_ld32(acc + i * 32, r);
+          tmem_loaded(r);
+          if (i + 1 == to) release();
+          f(i, r);
         }
       };
       if constexpr (KIND == kStats) {
