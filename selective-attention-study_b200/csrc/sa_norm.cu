@@ -1,9 +1,10 @@
 // Layer norm, after a residual sum or alone, and its gradient.  s = x + branch, h = (s - mean) / sqrt(var + eps), y = h w + b;
 //   ds = r (g - mean(g) - h mean(g h)) + ds_out,  g = dy w;   dw = sum over rows of dy h,   db = sum over rows of dy.
 //
-// Both directions are bound by memory: a row stays in the registers of one warp (up to 512 values) or of one CTA between its only
-// load and its only store; mean and variance are two sums over the registers, the second about the mean.  The backward's CTAs walk
-// over rows and keep their columns' sums for dw and db in registers; a second kernel joins the CTAs' sums in their order.
+// Both directions are bound by memory: a row stays in the registers of a warp or a part of one (up to 512 values) or of one CTA between
+// its only load and its only store; mean and variance are two sums over the registers, the second about the mean.  The backward's CTAs
+// walk over rows and keep their columns' sums for dw and db, in registers up to 8,192 columns; a second kernel joins the CTAs' sums in
+// their order.
 #include "sa_layers.cuh"
 
 #include <algorithm>
@@ -43,7 +44,7 @@ template <int T> constexpr int kRowsOf = kBlock<T> / T;
 template <int T, int NV> constexpr int kTogether = T <= 32 && NV == 1 ? 2 : 1;
 
 template <int T, int NV, bool VEC>
-__global__ void __launch_bounds__(kBlock<T>) forward_kernel(const sa_norm p) {
+__global__ void __launch_bounds__(kBlock<T>, T == 512 ? 2 : 1) forward_kernel(const sa_norm p) {
   tc::after_previous_kernel();
   constexpr int R = kTogether<T, NV>;
   __shared__ float2 buffer[2][32];
@@ -126,18 +127,31 @@ __global__ void __launch_bounds__(kBlock<T>) forward_kernel(const sa_norm p) {
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 
+// Rows of more than 8,192 values leave no registers for their columns' sums: those are in shared memory, a thread's apart by the threads
+// (4,000 rows of 12,288 in bf16 with a bias: 340 us with spilled registers, 230 this way; rows of 4,096 and 8,192 gain nothing from it).
+template <int T, int NV> constexpr bool kSumsShared = T * NV * 8 > 8192;
+
 // A thread's part of the gradient: of rows, h and g = dy in and dx out, and its columns' sums for dw and db.
 template <int T, int NV, bool VEC, bool BIAS>
 struct Gradient {
-  float dw[NV][8], db[BIAS ? NV : 1][8];
-  __device__ __forceinline__ Gradient() {
+  static constexpr bool kShared = kSumsShared<T, NV>;
+  float dw[kShared ? 1 : NV][8], db[BIAS && !kShared ? NV : 1][8];
+  float* const mine;                       // in shared memory: dw, then db
+  __device__ __forceinline__ Gradient(uint8_t* smem, int t) : mine(reinterpret_cast<float*>(smem) + t) {
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dw[c][i] = 0.f;
-        if (BIAS) db[c][i] = 0.f;
-      }
+      for (int i = 0; i < 8; ++i) add(c, i, 0.f, 0.f, true);
+  }
+  __device__ __forceinline__ void add(int c, int i, float w, float b, bool first = false) {
+    if constexpr (kShared) {
+      float* const at = mine + (c * 8 + i) * T;
+      *at = first ? w : *at + w;
+      if (BIAS) at[NV * 8 * T] = first ? b : at[NV * 8 * T] + b;
+    } else {
+      dw[c][i] = first ? w : dw[c][i] + w;
+      if (BIAS) db[c][i] = first ? b : db[c][i] + b;
+    }
   }
   // `width` is 0 in threads that have no row but go through the sums with the others.
   __device__ __forceinline__ void row(const sa_norm& p, float (&h)[NV][8], float (&g)[NV][8], float2 stats, int width, int t, float2 (*buffer)[32],
@@ -150,8 +164,7 @@ struct Gradient {
         const bool inside = in_row<T, VEC>(c, i, t, width);
         h[c][i] = inside ? (h[c][i] - stats.x) * stats.y : 0.f;
         g[c][i] = inside ? g[c][i] : 0.f;
-        dw[c][i] += g[c][i] * h[c][i];
-        if (BIAS) db[c][i] += g[c][i];
+        add(c, i, g[c][i] * h[c][i], g[c][i]);
       }
     if (p.weight != nullptr) {
       float w[NV][8];
@@ -201,19 +214,20 @@ struct Gradient {
             if (BIAS) db[c][i] += shared[k * kTeam + ((NV + c) * 8 + i) * T + t];
           }
     }
-    float* mine = sums + (int64_t)blockIdx.x * (BIAS ? 2 : 1) * p.width;
+    float* out = sums + (int64_t)blockIdx.x * (BIAS ? 2 : 1) * p.width;
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int col = column_of<T, VEC>(c, i, t);
         if (col >= p.width) continue;
-        mine[col] = dw[c][i];
-        if (BIAS) mine[p.width + col] = db[c][i];
+        out[col] = kShared ? mine[(c * 8 + i) * T] : dw[kShared ? 0 : c][i];
+        if (BIAS) out[p.width + col] = kShared ? mine[(NV * 8 + c * 8 + i) * T] : db[kShared ? 0 : c][i];
       }
   }
 };
-template <int T, int NV, bool BIAS> constexpr size_t kTeamBytes = kRowsOf<T> > 1 ? (kRowsOf<T> - 1) * T * NV * 8 * (BIAS ? 2 : 1) * 4 : 0;
+template <int T, int NV, bool BIAS>
+constexpr size_t kTeamBytes = (kSumsShared<T, NV> ? 1 : kRowsOf<T> - 1) * (size_t)T * NV * 8 * (BIAS ? 2 : 1) * 4;
 
 // Rows as they lie, by plain loads: strides and addresses that the copies below do not take, or rows too long for them.
 // `sums`: (CTAs, 1 or 2, width), the parts of dw and db; null when neither is asked for.
@@ -224,7 +238,7 @@ __global__ void __launch_bounds__(kBlock<T>) backward_kernel(const sa_norm p, fl
   __shared__ float2 buffer[2][32];
   const int t = threadIdx.x % T, team = threadIdx.x / T;
   int turn = 0;
-  Gradient<T, NV, VEC, BIAS> gradient;
+  Gradient<T, NV, VEC, BIAS> gradient(smem, t);
   const int64_t rounds = (p.rows + kRowsOf<T> - 1) / kRowsOf<T>;
   for (int64_t i0 = blockIdx.x; i0 < rounds; i0 += gridDim.x) {
     const int64_t row = i0 * kRowsOf<T> + team;
@@ -302,7 +316,7 @@ __global__ void __launch_bounds__(kBlock<T>, kResident<T, NV>) backward_copied_k
     for (int k = 0; k < kRing; ++k)
       if (blockIdx.x + (int64_t)k * gridDim.x < stages) load(blockIdx.x + (int64_t)k * gridDim.x, k);
   int turn = 0, slot = 0, round = 0;
-  Gradient<T, NV, VEC, BIAS> gradient;
+  Gradient<T, NV, VEC, BIAS> gradient(smem, t);
   for (int64_t i = blockIdx.x; i < stages; i += gridDim.x) {
     const int64_t row0 = i * c.rows;
     const int n = (int)min((int64_t)c.rows, p.rows - row0);
@@ -391,9 +405,10 @@ bool vectors(const sa_norm& p, bool backward) {
          eights(p.dbranch, p.branch_dtype, w, 1);
 }
 
-// Threads and values of a row by its width: f(threads, chunks of 8 a thread).  As few threads as hold it: with eight, 5,333,333 rows of 3
-// bf16 values took 335 us forward and 936 with the gradients, with one 41 and 139; 500,000 of 32 25 and 80, with four 14 and 76.
-template <typename F>
+// Threads and values of a row by its width: f(threads, chunks of 8 a thread).  Of narrow rows, as few threads as hold them: with eight,
+// 5,333,333 rows of 3 bf16 values took 335 us forward and 936 with the gradients, with one 41 and 139; 500,000 of 32 25 and 80, with four
+// 14 and 76.
+template <bool FORWARD, typename F>
 int by_width(int width, F f) {
   using std::integral_constant;
 #define SA_NORM_CASE(most, threads, chunks) \
@@ -406,16 +421,24 @@ int by_width(int width, F f) {
   SA_NORM_CASE(256, 32, 1);
   SA_NORM_CASE(512, 32, 2);
   SA_NORM_CASE(1024, 128, 1);
-  SA_NORM_CASE(2048, 256, 1);
-  SA_NORM_CASE(4096, 512, 1);
-  SA_NORM_CASE(8192, 1024, 1);
-  SA_NORM_CASE(16384, 1024, 2);
+  // wide ones: the forward has many CTAs an SM of few threads, each with 32 values (8,000 rows of 8,192 in bf16: 61 us, with 1,024
+  // threads of 8 values 119; 8,000 of 2,048: 14 and 19); the backward's sums of columns leave room for 8 values
+  if constexpr (FORWARD) {
+    SA_NORM_CASE(2048, 128, 2);
+    SA_NORM_CASE(4096, 128, 4);
+    SA_NORM_CASE(8192, 256, 4);
+  } else {
+    SA_NORM_CASE(2048, 256, 1);
+    SA_NORM_CASE(4096, 512, 1);
+    SA_NORM_CASE(8192, 1024, 1);
+  }
+  SA_NORM_CASE(16384, 512, 4);
 #undef SA_NORM_CASE
   return SA_ERR_UNSUPPORTED;
 }
 
 // What the backward's copies look like; false where rows do not take them.
-bool copies_of(const sa_norm& p, int rows_at_a_time, Copies* c) {
+bool copies_of(const sa_norm& p, int threads, int rows_at_a_time, Copies* c) {
   const void* const from[3] = {p.x, p.dy, p.dsum};
   const int types[3] = {p.x_dtype, p.y_dtype, p.x_dtype};
   const int64_t strides[3] = {p.x_stride, p.dy_stride, p.dsum_stride};
@@ -443,16 +466,16 @@ bool copies_of(const sa_norm& p, int rows_at_a_time, Copies* c) {
   }
   c->at[3] = at;
   c->stage = (at + c->rows * 8 + 127) / 128 * 128;
-  return c->stage * kRing <= 104 * 1024;        // two CTAs an SM
+  return c->stage * kRing <= (threads < 1024 ? 104 : 212) * 1024;        // two CTAs an SM, or the one that has all registers
 }
 
 // CTAs of the backward: at most 768 threads an SM, or as many as their stages leave room for.
 int blocks_of(const sa_norm& p) {
   int blocks = 0;
-  by_width(p.width, [&](auto threads, auto chunks) {
+  by_width<false>(p.width, [&](auto threads, auto chunks) {
     constexpr int T = decltype(threads)::value;
     Copies c;
-    const bool copied = copies_of(p, kRowsOf<T>, &c);
+    const bool copied = copies_of(p, kBlock<T>, kRowsOf<T>, &c);
     const int64_t rows = copied ? c.rows : kRowsOf<T>;
     const int here = copied ? std::min(768 / kBlock<T>, 200 * 1024 / (c.stage * kRing + 2048)) : 512 / kBlock<T>;
     blocks = (int)std::min<int64_t>((p.rows + rows - 1) / rows, (int64_t)kSms * std::max(1, here));
@@ -464,13 +487,18 @@ int columns_of(const sa_norm& p) { return p.width * (p.dbias != nullptr ? 2 : 1)
 
 template <int T, int NV, bool VEC, bool BIAS>
 int launch_backward(const sa_norm& p, int blocks, float* sums, cudaStream_t s) {
-  Copies c;
-  if (!copies_of(p, kRowsOf<T>, &c)) return launch_after(backward_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, kTeamBytes<T, NV, BIAS>, s, p, sums);
-  tc::WaitCtx status;
-  const int st = tc::wait_ctx(&status);
-  if (st != SA_OK) return st;
-  const size_t smem = std::max((size_t)c.stage * kRing, kTeamBytes<T, NV, BIAS>);
-  return launch_after(backward_copied_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, smem, s, p, sums, (const Copies)c, (const tc::WaitCtx)status);
+  if constexpr (!kSumsShared<T, NV>) {     // whose stages would be too large
+    Copies c;
+    if (copies_of(p, kBlock<T>, kRowsOf<T>, &c)) {
+      tc::WaitCtx status;
+      const int st = tc::wait_ctx(&status);
+      if (st != SA_OK) return st;
+      const size_t smem = std::max((size_t)c.stage * kRing, kTeamBytes<T, NV, BIAS>);
+      return launch_after(backward_copied_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, smem, s, p, sums, (const Copies)c,
+                          (const tc::WaitCtx)status);
+    }
+  }
+  return launch_after(backward_kernel<T, NV, VEC, BIAS>, dim3(blocks), kBlock<T>, kTeamBytes<T, NV, BIAS>, s, p, sums);
 }
 
 }  // namespace
@@ -480,7 +508,7 @@ size_t backward_bytes(const sa_norm& p) {
 }
 
 int forward(const sa_norm& p, cudaStream_t s) {
-  return by_width(p.width, [&](auto threads, auto chunks) {
+  return by_width<true>(p.width, [&](auto threads, auto chunks) {
     constexpr int T = decltype(threads)::value, NV = decltype(chunks)::value;
     constexpr int kRows = kRowsOf<T> * kTogether<T, NV>;
     const dim3 grid((unsigned)((p.rows + kRows - 1) / kRows));
@@ -492,10 +520,11 @@ int forward(const sa_norm& p, cudaStream_t s) {
 int backward(const sa_norm& p, cudaStream_t s) {
   const int blocks = blocks_of(p);
   float* sums = p.dweight == nullptr && p.dbias == nullptr ? nullptr : static_cast<float*>(p.workspace);
-  const int st = by_width(p.width, [&](auto threads, auto chunks) {
+  const int st = by_width<false>(p.width, [&](auto threads, auto chunks) {
     constexpr int T = decltype(threads)::value, NV = decltype(chunks)::value;
-    if (p.dbias != nullptr) return vectors(p, true) ? launch_backward<T, NV, true, true>(p, blocks, sums, s) : launch_backward<T, NV, false, true>(p, blocks, sums, s);
-    return vectors(p, true) ? launch_backward<T, NV, true, false>(p, blocks, sums, s) : launch_backward<T, NV, false, false>(p, blocks, sums, s);
+    const bool vec = vectors(p, true);
+    if (p.dbias != nullptr) return vec ? launch_backward<T, NV, true, true>(p, blocks, sums, s) : launch_backward<T, NV, false, true>(p, blocks, sums, s);
+    return vec ? launch_backward<T, NV, true, false>(p, blocks, sums, s) : launch_backward<T, NV, false, false>(p, blocks, sums, s);
   });
   if (st != SA_OK || sums == nullptr) return st;
   return launch_after(parameters_kernel, dim3((columns_of(p) + 7) / 8), 512, 0, s, (const float*)sums, blocks, p.width, columns_of(p), p.weight_dtype,
