@@ -111,6 +111,14 @@ def test_rows_of_a_few_values(shape, xt, bt, yt, bias):
     test_layer_norm_and_its_gradients(shape, xt, bt, F32 if xt == F32 else xt, yt, bias)
 
 
+@pytest.mark.parametrize("shape,xt,bt,yt,bias", [
+    ((700, 8192), BF16, None, BF16, True), ((451, 8200), F16, None, F16, False), ((601, 12288), BF16, BF16, BF16, True), ((333, 16384), F32, None, F32, True),
+    ((449, 8191), F32, BF16, BF16, True), ((901, 4097), F16, None, F32, True), ((750, 4096), F32, BF16, F32, False)])
+def test_rows_of_many_values(shape, xt, bt, yt, bias):
+    """Several rows a CTA, whose columns' sums are in registers or in shared memory."""
+    test_layer_norm_and_its_gradients(shape, xt, bt, F32 if xt == F32 else xt, yt, bias)
+
+
 def test_layer_norm_without_parameters_and_without_gradients():
     gen = _gen(1)
     x = _randn(gen, 12, 100, dtype=BF16)
