@@ -49,7 +49,7 @@ struct Convert {
   int64_t ignore_index;
   int vocab, reduction;
   const float *dloss, *count, *largest;
-  float *factor, *scale;
+  float *factor, *scale, *less;
 };
 
 // Eight values in `parts` parts of 16 bits, each what the ones before it leave.
@@ -87,7 +87,11 @@ __global__ void __launch_bounds__(256) convert_kernel(const Convert c) {
         const float most = c.reduction == SA_REDUCTION_NONE ? *c.largest : fabsf(g);
         factor = most == 0.f ? 0.f : g / most * kHalfScale;
         if (row == 0) *c.scale = c.reduction == SA_REDUCTION_MEAN && *c.count == 0.f ? 0.f : most / kHalfScale;
+      } else if (c.reduction != SA_REDUCTION_NONE) {      // left to the results: in 8 bits it would move every token's gradient alike
+        factor = 1.f;
+        if (row == 0) *c.scale = c.reduction == SA_REDUCTION_MEAN && *c.count == 0.f ? 0.f : g;
       }
+      c.less[row] = 0.f;
       c.factor[row] = !counts ? 0.f : t < 0 || t >= c.vocab ? NAN : factor;
     }
   }
@@ -628,7 +632,7 @@ struct Forward {
 struct Backward {
   Room room;
   Operand x, weight, dz;
-  float *factor, *scale, *largest, *dx_sums = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr;
+  float *factor, *scale, *largest, *less, *dx_sums = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr;
   int ctas, piece;
   int64_t pitch;                 // of dx_sums
   Backward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
@@ -638,6 +642,7 @@ struct Backward {
     factor = room.take<float>(p.tokens);
     scale = room.take<float>(1);
     largest = room.take<float>(1);
+    less = room.take<float>(p.tokens);
     piece = piece_of(p);
     dz.rows = p.tokens;
     dz.parts = parts_of(p);
@@ -957,9 +962,11 @@ int backward(const Problem& p, cudaStream_t s) {
   c.largest = b.largest;
   c.factor = b.factor;
   c.scale = b.scale;
+  c.less = b.less;
   st = run_convert(c, s);
   if (st == SA_OK && b.weight.part != 0) st = run_convert(convert_of(p, b.weight, p.weight, p.weight_dtype, p.weight_stride), s);
-  const float* scale = half ? b.scale : nullptr;
+  const float* scale = half || p.reduction != SA_REDUCTION_NONE ? b.scale : nullptr;
+  const Matrix weight = matrix_of(p, b.weight, p.weight, p.weight_dtype, p.weight_stride);
   for (int v0 = 0; v0 < p.vocab && st == SA_OK; v0 += b.piece) {
     const int columns = std::min(b.piece, p.vocab - v0);
     Epilogue e{};
@@ -972,6 +979,8 @@ int backward(const Problem& p, cudaStream_t s) {
     e.p_part = b.dz.part;
     e.parts = b.dz.parts;
     e.half = half;
+    e.scale = scale;
+    e.less = b.less;
     const Walk logits = walk_of(p.tokens, columns, p.width, terms_of(p), b.ctas, false);
     st = run<kProbabilities, false, false>(b.ctas, b.x, b.weight, logits, Origin{0, 0}, Origin{v0, 0}, e, status, s);
     if (st != SA_OK) return st;
@@ -988,6 +997,12 @@ int backward(const Problem& p, cudaStream_t s) {
       r.addend = first ? nullptr : b.dx_sums;
       r.addend_pitch = b.pitch;
       r.scale = last ? scale : nullptr;
+      r.table = last && b.dz.parts == 1 ? weight.base : nullptr;
+      r.table_dtype = weight.dtype;
+      r.table_stride = weight.stride;
+      r.table_factor = b.less;
+      r.targets = p.targets;
+      r.vocab = p.vocab;
       r.slabs = b.dx_slabs;
       r.later = !first;
       st = run_result<false, true>(p, b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);

@@ -114,6 +114,7 @@ struct Epilogue {
   // kProbabilities: (exp2(z log2 e - lse) - [target]) * factor, in `parts` 16-bit parts
   const float2* lse;                       // in two parts
   const float* factor;
+  float* less;                             // of one part: [m], what its rounding takes from the target's column, times `scale`
   uint16_t* p;
   int64_t p_pitch, p_part;                 // elements of a row, of a part
   int parts;
@@ -365,7 +366,8 @@ __device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
 }
 
 // (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
-__device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int64_t at, float2 lse, float factor, int target) {
+__device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int row, int64_t at, float2 lse, float factor,
+                                                    int target) {
   const Pair by = pair(kLog2e, kLog2e), less = pair(-lse.x, -lse.x), less_still = pair(-lse.y, -lse.y);
   float p[32];
 #pragma unroll
@@ -377,6 +379,12 @@ __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uin
   if (target >= 0) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) p[i] = i == target ? p[i] - 1.f : p[i];
+    if (e.parts == 1 && factor != 0.f) {                                     // the largest column by far, most often
+      float d = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) d = i == target ? p[i] * factor : d;
+      e.less[row] = (d - (e.half ? __half2float(__float2half_rn(d)) : __bfloat162float(__float2bfloat16_rn(d)))) * (e.scale != nullptr ? *e.scale : 1.f);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 32; ++i) p[i] *= factor;
@@ -751,7 +759,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         each_chunk([&](int i, uint32_t (&r)[32]) {
           const int col = u.tn * w.bn + i * 32;
           const int64_t mine = target - e.column0 - col;
-          if (inside) store_probabilities(e, r, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
+          if (inside) store_probabilities(e, r, row, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
         });
       } else if constexpr (KIND == kResult) {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;

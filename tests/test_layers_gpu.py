@@ -447,6 +447,27 @@ def test_loss_of_batches_strides_and_padding():
     assert (same[2] == 0).all()
 
 
+@pytest.mark.parametrize("reduction", ["sum", "mean", "none"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_cotangents_rounding_moves_no_gradient(dtype, reduction):
+    """Targets' gradients of the logits about half a step from a number of the type: rounded, they would move every token's alike, by 0.7
+    to 1 half steps."""
+    dloss = (1 + _half_step(dtype)) / (1 - 1 / 700) * (200 if reduction == "mean" else 1)
+    gen = _gen(41)
+    x, w = _randn(gen, 200, 136, dtype=dtype).requires_grad_(True), _randn(gen, 700, 136, dtype=dtype, scale=0.05).requires_grad_(True)
+    targets = torch.randint(0, 700, (200,), generator=gen).cuda()
+    loss = layers.linear_cross_entropy(x, w, targets, reduction=reduction)
+    g = torch.full_like(loss, dloss).detach()
+    (dx,) = torch.autograd.grad(loss, x, g)
+    with torch.no_grad():
+        z = x.double() @ w.double().T
+        dz = (torch.softmax(z, 1) - torch.nn.functional.one_hot(targets, 700)) * (dloss / (200 if reduction == "mean" else 1))
+        want = dz @ w.double()
+    # 27,200 roundings of dx, spread over half a step or less each way: 3^-1/2 of one in their norm at most; of dz, those of what is not at
+    # the target, a 15th of dx's norm
+    assert float((dx.double() - want).norm() / want.norm()) < (3 ** -0.5 + 0.07) * _half_step(dtype)
+
+
 def test_what_is_ignored_may_be_anything():
     gen = _gen(13)
     x = _randn(gen, 90, 96, dtype=BF16)
