@@ -16,8 +16,8 @@
 //
 // Otherwise (a cotangent for every token; fp16, whose five bits of exponent do not hold e; problems so small that a product costs
 // less than the sums of the gradients, written and read): the backward computes the logits again in pieces of the vocabulary, turns
-// a piece's into dz in 16 bits, and reads them with the two products of the gradients.  Four products in all; the sums of dx over
-// the pieces stay in fp32.
+// a piece's into dz in 16 bits, and reads them with the two products of the gradients; what the rounding takes from dz at the target is
+// added to dx in fp32, and one cotangent scales the results.  Four products in all; the sums of dx over the pieces stay in fp32.
 #include "sa_loss.cuh"
 
 #include <algorithm>
@@ -489,7 +489,7 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
   w.slabs = 1;
   const int most = kSms / ctas;
   w.clusters = std::min(w.tiles(), most);
-  w.segment = result && terms > 1 ? kSegment : w.blocks;
+  w.segment = result && terms == kTerms ? kSegment : w.blocks;
   w.group = result ? 1 : std::min(w.m_tiles, 32);
   const int left = w.tiles() % most;
   if (result && left > 0) {
@@ -645,7 +645,7 @@ struct Backward {
     less = room.take<float>(p.tokens);
     piece = piece_of(p);
     dz.rows = p.tokens;
-    dz.parts = parts_of(p);
+    dz.parts = dz_parts(p);
     dz.pitch = up(piece, 64);
     dz.part = dz.pitch * p.tokens;
     dz.base = room.take<uint16_t>(dz.part * dz.parts);
@@ -660,11 +660,15 @@ struct Backward {
       dw_slabs = room.take<float>(most);
     }
   }
+  // Of few tokens dz is kept in two parts for dW, whose product is bound by what it writes up to here (128 tokens of 50,304 words of 768
+  // 107 us a call, with one part 105): the 8 bits of one would make most of its error (2.3e-3 to 2.9e-3 against 64 bits, 1.7e-3 with
+  // two).  dx has the first part.
+  static int dz_parts(const Problem& p) { return p.product == SA_BF16 && p.tokens <= kRows ? 2 : parts_of(p); }
   // Columns of a piece of the vocabulary: its dz takes up to 320 MB (16,384 tokens: 37 tiles of 256 columns, with four tiles across
   // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more, but no more than 8 GB; of the sizes down to half of
   // that, the one that leaves the fewest clusters idle in dW.
   static int piece_of(const Problem& p) {
-    const int64_t column = (int64_t)p.tokens * 2 * parts_of(p), in_320mb = (320ll << 20) / column / 256 * 256;
+    const int64_t column = (int64_t)p.tokens * 2 * dz_parts(p), in_320mb = (320ll << 20) / column / 256 * 256;
     const int64_t in_8gb = (8ll << 30) / column / 256 * 256, most = std::max<int64_t>({256, std::min<int64_t>(4096, in_8gb), in_320mb});
     if (p.vocab <= most) return p.vocab;
     const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
@@ -680,7 +684,7 @@ struct Backward {
   }
   Walk dx_walk(const Problem& p, int columns) const { return walk_of(p.tokens, p.width, columns, terms_of(p), ctas, true, piece); }
   Walk dw_walk(const Problem& p, int columns) const {
-    return walk_of(columns, p.width, p.tokens, terms_of(p), ctas_of(columns), true, p.tokens);
+    return walk_of(columns, p.width, p.tokens, p.product == SA_F32 ? kTerms : dz_parts(p), ctas_of(columns), true, p.tokens);
   }
 };
 
@@ -997,7 +1001,7 @@ int backward(const Problem& p, cudaStream_t s) {
       r.addend = first ? nullptr : b.dx_sums;
       r.addend_pitch = b.pitch;
       r.scale = last ? scale : nullptr;
-      r.table = last && b.dz.parts == 1 ? weight.base : nullptr;
+      r.table = last && b.dz.parts < 3 ? weight.base : nullptr;
       r.table_dtype = weight.dtype;
       r.table_stride = weight.stride;
       r.table_factor = b.less;

@@ -114,7 +114,7 @@ struct Epilogue {
   // kProbabilities: (exp2(z log2 e - lse) - [target]) * factor, in `parts` 16-bit parts
   const float2* lse;                       // in two parts
   const float* factor;
-  float* less;                             // of one part: [m], what its rounding takes from the target's column, times `scale`
+  float* less;                             // of one or two parts: [m], what the first one's rounding takes from the target's column, times `scale`
   uint16_t* p;
   int64_t p_pitch, p_part;                 // elements of a row, of a part
   int parts;
@@ -379,7 +379,7 @@ __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uin
   if (target >= 0) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) p[i] = i == target ? p[i] - 1.f : p[i];
-    if (e.parts == 1 && factor != 0.f) {                                     // the largest column by far, most often
+    if (e.parts < 3 && factor != 0.f) {                                      // the largest column by far, most often
       float d = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) d = i == target ? p[i] * factor : d;
@@ -607,6 +607,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       // ---- loads.  Both CTAs count on the first one's barrier: its thread issues the MMAs of both.
       const uint32_t full_there = CTAS == 2 ? address_in(full, 0) : full;
       const uint32_t ring = smem_u32(smem);
+      // parts of the terms: of one (0,0), of two (1,0) (0,0), of six (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+      const int terms = w.blocks / w.depth_blocks, parts_a = terms == 1 ? 0 : terms == 2 ? 0x01 : 0x001012, parts_b = terms < 6 ? 0 : 0x010210;
       int stage = 0, round = 0;
       while (u.next(w)) {
         const int a0 = at_a.own + u.tm * kColumns + (int)rank * kRows;
@@ -615,9 +617,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (int k = u.k0; k < u.k1; ++k) {
           if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1000);
           if (rank == 0) expect_tx(full + 8 * stage, (a_bytes + kOperand) * CTAS);
-          // parts of the terms: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-          const int pa = w.blocks == w.depth_blocks ? 0 : (0x001012 >> (4 * term)) & 3;
-          const int pb = w.blocks == w.depth_blocks ? 0 : (0x010210 >> (4 * term)) & 3;
+          const int pa = (parts_a >> (4 * term)) & 3, pb = (parts_b >> (4 * term)) & 3;
           const uint32_t a = ring + stage * 2 * kOperand, b = a + kOperand, bar = full_there + 8 * stage;
           const int ka = at_a.depth + block * kDepth, kb = at_b.depth + block * kDepth;
           if constexpr (A_MN) {

@@ -52,8 +52,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     them.  Either way up to half a GB of what stands for logits is there at a time.
 
     x and weight have one dtype, or under autocast are rounded to its; their gradients have their own.  bf16 and fp16 products are
-    exact with fp32 sums, and the gradient of the logits is rounded to that dtype between its products (fp16: scaled by the
-    largest cotangent, so tokens whose cotangent is 2^-19 of it or less lose bits).  fp32 operands are split into three bf16
+    exact with fp32 sums, and the gradient of the logits is rounded to that dtype between its products, but for the target's in x's
+    gradient (fp16: scaled by the largest cotangent, so tokens whose cotangent is 2^-19 of it or less lose bits).  fp32 operands are split into three bf16
     parts, which keep 24 bits.
 
     What stands in x where a target is ignored does not matter.  A target outside the vocabulary that is not ``ignore_index`` makes its

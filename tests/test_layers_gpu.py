@@ -468,6 +468,21 @@ def test_a_cotangents_rounding_moves_no_gradient(dtype, reduction):
     assert float((dx.double() - want).norm() / want.norm()) < (3 ** -0.5 + 0.07) * _half_step(dtype)
 
 
+@pytest.mark.parametrize("tokens,reduction", [(1, "sum"), (9, "mean"), (64, "none"), (65, "none"), (128, "sum")])
+def test_few_tokens_gradients_are_as_exact_as_their_type(tokens, reduction):
+    gen = _gen(42)
+    x, w = _randn(gen, tokens, 272, dtype=BF16).requires_grad_(True), _randn(gen, 300, 272, dtype=BF16, scale=0.2).requires_grad_(True)
+    targets = torch.randint(0, 300, (tokens,), generator=gen).cuda()
+    loss = layers.linear_cross_entropy(x, w, targets, reduction=reduction)
+    g = (torch.rand(loss.shape, generator=gen) + 0.5).cuda()
+    (dw,) = torch.autograd.grad(loss, w, g)
+    z = x.detach().double() @ w.detach().double().T
+    dz = torch.softmax(z, 1) - torch.nn.functional.one_hot(targets, 300)
+    want = (dz * (g if reduction == "none" else g / (tokens if reduction == "mean" else 1)).double().reshape(-1, 1)).T @ x.detach().double()
+    # dz keeps 16 bits; the 81,600 roundings of dw are spread as above
+    assert float((dw.double() - want).norm() / want.norm()) < (3 ** -0.5 + 0.01) * _half_step(BF16)
+
+
 def test_what_is_ignored_may_be_anything():
     gen = _gen(13)
     x = _randn(gen, 90, 96, dtype=BF16)
