@@ -641,6 +641,11 @@ Tensor given(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 void check_not_traced(const char* fn) {
   TORCH_CHECK(torch::jit::tracer::getTracingState() == nullptr, fn, " cannot be recorded by a trace: its result would be a constant of it");
 }
+// A tangent would be dropped without a word where no gradient is asked for.
+void check_no_tangent(const char* fn, std::initializer_list<std::optional<Tensor>> arguments) {
+  for (const auto& t : arguments)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), fn, " has no forward-mode derivative");
+}
 void check_cuda(const char* fn, const char* what, const Tensor& t, const Tensor& like) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device(), fn, ": ", what, " must be a CUDA tensor, all on one device; got ", t.device());
   TORCH_CHECK_VALUE(code_of(t) >= 0, fn, ": dtype of ", what, " must be float32, bfloat16 or float16; got ", name_of(t.scalar_type()));
@@ -763,6 +768,7 @@ variable_list layer_norm(const Tensor& x, const std::optional<Tensor>& branch, c
                          double eps, const std::optional<at::ScalarType>& dtype) {
   const char* fn = branch ? "add_layer_norm" : "layer_norm";
   check_not_traced(fn);
+  check_no_tangent(fn, {x, branch, weight, bias});
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, fn, ": x must be (..., width) of a width of 1 to 16384; got ", x.sizes());
   check_cuda(fn, "x", x, x);
   if (branch) {
@@ -858,6 +864,7 @@ Tensor indices_in(const Tensor& t) { return in_order(in_type(t, at::kLong)); }
 Tensor embedding(const Tensor& idx_in, const Tensor& weight, double scale, const std::optional<at::ScalarType>& dtype) {
   const char* fn = "embedding";
   check_not_traced(fn);
+  check_no_tangent(fn, {weight});
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, fn, ": weight must be (vocab, width); got ", weight.sizes());
   check_cuda(fn, "weight", weight, weight);
   TORCH_CHECK_VALUE(idx_in.is_cuda() && idx_in.device() == weight.device() && (idx_in.scalar_type() == at::kLong || idx_in.scalar_type() == at::kInt), fn,
@@ -1042,6 +1049,7 @@ bool rows_viewable(const Tensor& t) {
 Tensor linear_cross_entropy(Tensor x, Tensor weight, const Tensor& targets_in, int64_t ignore_index, int64_t reduction) {
   const char* fn = "linear_cross_entropy";
   check_not_traced(fn);
+  check_no_tangent(fn, {x, weight});
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1 && weight.size(1) >= 1, fn,
                     ": x must be (..., width) and weight (vocab, width); got ", x.sizes(), " and ", weight.sizes());
   check_cuda(fn, "x", x, x);

@@ -3,7 +3,8 @@
 The reference calls library operators here (``src/selective_attention/model.py:31-47,325-328,365-366,402-418``); its loss keeps the
 (tokens, vocab) logits, in pieces for evaluation (``:420-447``).  Here they are kernels of the library, differentiable once, with gradients
 that are the same from call to call.  CUDA tensors and the built library only; float32, bfloat16 and float16, any strides (a tensor whose
-last axis is not contiguous is copied).  A call cannot be recorded by ``torch.jit.trace``."""
+last axis is not contiguous is copied).  A call cannot be recorded by ``torch.jit.trace`` and has no forward-mode derivative: a tensor that
+carries a tangent is refused."""
 
 from __future__ import annotations
 
