@@ -12,7 +12,8 @@ on either side of the kernels in either pass (bf16; fp32 runs take the unfused c
 
 With ``own_layers=True`` what stands around the attention goes through the library too (``layers.py``): the embedding, every residual
 sum with the norm behind it, and the loss, whose logits are then never there at all (``loss_chunk`` has no part in it).  Parameters and
-their names are the same either way; results differ by roundings."""
+their names are the same either way; results differ by roundings.  Blocks are called as modules, with the residual stream and what is
+still to be added to it (their hooks run, and see both); norms and the embedding are not, and one that has hooks is refused."""
 
 from __future__ import annotations
 
@@ -40,6 +41,19 @@ class SelectiveSelfAttention(nn.Module):
         return self.c_proj(y.transpose(1, 2).reshape(b, t, self.d_model))
 
 
+def _check_no_hooks(module: nn.Module) -> None:
+    if module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks:
+        raise RuntimeError(f"own_layers=True reads the parameters of {type(module).__name__} and does not call it: its hooks would not run")
+
+
+def _add_norm(x: torch.Tensor, branch: torch.Tensor | None, norm: nn.LayerNorm, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """x, with ``branch`` added where there is one, and its norm."""
+    _check_no_hooks(norm)
+    if branch is None:
+        return x, layers.layer_norm(x, norm.weight, eps=norm.eps, dtype=dtype)
+    return layers.add_layer_norm(x, branch, norm.weight, eps=norm.eps, dtype=dtype)
+
+
 class Block(nn.Module):
     def __init__(self, d_model: int, n_heads: int):
         super().__init__()
@@ -52,18 +66,14 @@ class Block(nn.Module):
     def mlp(self, x: torch.Tensor) -> torch.Tensor:
         return self.c_proj(F.gelu(self.c_fc(x)))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = x + self.attn(self.ln_1(x))
-        return x + self.mlp(self.ln_2(x))
-
-    def forward_own(self, x: torch.Tensor, branch: torch.Tensor | None, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-        """The block by ``layers``: the residual stream and the branch of the block before that is still to be added to it, and the
-        same behind this block.  ``dtype``: of the norms' results, as the projections will take them."""
-        if branch is None:
-            y = layers.layer_norm(x, self.ln_1.weight, eps=self.ln_1.eps, dtype=dtype)
-        else:
-            x, y = layers.add_layer_norm(x, branch, self.ln_1.weight, eps=self.ln_1.eps, dtype=dtype)
-        x, y = layers.add_layer_norm(x, self.attn(y), self.ln_2.weight, eps=self.ln_2.eps, dtype=dtype)
+    def forward(self, x: torch.Tensor, branch: torch.Tensor | None = None, dtype: torch.dtype | None = None):
+        """The residual stream behind the block.  With ``dtype``, of the norms' results as the projections will take them, by ``layers``:
+        ``branch`` is what the block before leaves to be added to the stream, and the result is the stream and what this one leaves."""
+        if dtype is None:
+            x = x + self.attn(self.ln_1(x))
+            return x + self.mlp(self.ln_2(x))
+        x, y = _add_norm(x, branch, self.ln_1, dtype)
+        x, y = _add_norm(x, self.attn(y), self.ln_2, dtype)
         return x, self.mlp(y)
 
 
@@ -81,14 +91,12 @@ class SelectiveDecoder(nn.Module):
                 nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
     def _forward_own(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        _check_no_hooks(self.wte)
         x, branch = layers.embedding(idx, self.wte.weight), None
         dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
         for block in self.h:
-            x, branch = block.forward_own(x, branch, dtype)
-        if branch is None:
-            y = layers.layer_norm(x, self.ln_f.weight, eps=self.ln_f.eps, dtype=dtype)
-        else:
-            y = layers.add_layer_norm(x, branch, self.ln_f.weight, eps=self.ln_f.eps, dtype=dtype)[1]
+            x, branch = block(x, branch, dtype)
+        y = _add_norm(x, branch, self.ln_f, dtype)[1]
         return layers.linear_cross_entropy(y, self.wte.weight, targets)
 
     def forward(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
