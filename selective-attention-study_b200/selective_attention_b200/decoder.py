@@ -97,7 +97,7 @@ class SelectiveDecoder(nn.Module):
         for block in self.h:
             x, branch = block(x, branch, dtype)
         y = _add_norm(x, branch, self.ln_f, dtype)[1]
-        return layers.linear_cross_entropy(y, self.wte.weight, targets)
+        return layers.linear_cross_entropy(y, self.wte.weight, targets, reduction="sum") / targets.numel()
 
     def forward(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         if self.own_layers:

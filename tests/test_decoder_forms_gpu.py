@@ -51,3 +51,14 @@ def test_hooks_of_what_is_not_called_are_refused(name, kind):
         own(idx, targets)
     handle.remove()
     assert torch.isfinite(own(idx, targets))
+
+
+@pytest.mark.parametrize("ignored", [1, 100, 260])
+def test_ignored_targets_weigh_the_same_either_way(ignored):
+    plain, own, idx, targets = _pair()
+    targets.view(-1)[:ignored] = -100
+    want, wanted = _run(plain, idx, targets)
+    loss, grads = _run(own, idx, targets)
+    assert abs(loss - want) <= 1e-5 * want                  # fp32 on both sides
+    for name, grad in grads.items():
+        assert float((grad - wanted[name]).norm()) <= 2e-4 * float(wanted[name].norm()), name
