@@ -448,8 +448,8 @@ int sa_beam_select(const sa_beam* p);
  *   product  type of the products' operands: x and weight are rounded to it first (SA_F32: three bf16 parts, 24 bits)
  *   targets  int64; ignore_index counts for nothing, and what stands in its row of x does not matter; any other target outside the vocabulary makes
  *            its loss and the gradients NaN
- *   lse      (tokens, 2) fp32, log2 of the sum of exponentials in two parts: written by the forward, read by the backward; count (1,) fp32
- *            likewise
+ *   lse      (tokens, 2) fp32, the largest logit and log2 of the sum of exponentials relative to it: written by the forward, read by the
+ *            backward; count (1,) fp32 likewise
  *   loss     (tokens,) fp32 without a reduction (0 where the target is ignored), else one number
  *   dloss    of loss's shape; dx, dweight contiguous, of x's and weight's type, either may be null
  * sums are fp32; the gradient of the logits is rounded to `product` between the products (fp16: scaled by 2^14 over the

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(1024) largest_kernel(const float* dloss, const
 // Joins the half tiles of 32 tokens: a lane has a token, the 32 warps take the half tiles in turn, eight loads in flight.  The last CTA
 // to end sums all tokens, in order.
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32, kJoinAhead = 8;
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats, int slots, const float2* at_target, const int64_t* targets,
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats, int slots, const float* at_target, const int64_t* targets,
                                                             int64_t ignore_index, int tokens, int vocab, int reduction, float2* lse, float* loss,
                                                             float* count, float2* sums, unsigned int* ticket) {
   after_previous_kernel();
@@ -140,10 +140,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
     for (int i = 0; i < kJoinAhead; ++i)
       if (i < n) most = fmaxf(most, v[i].x);
     const float from = most == -INFINITY ? 0.f : most;
-    sum *= ex2(top - from);
+    sum *= ex2(between(top, from));
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i)
-      if (i < n) sum += v[i].y * ex2(v[i].x - from);
+      if (i < n) sum += v[i].y * ex2(between(v[i].x, from));
     top = most;
   };
   for (int i = warp; i < slots; i += kJoinWarps * kJoinAhead) {
@@ -166,12 +166,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
     }
     float mine = 0.f, counts = 0.f;
     if (row < tokens) {
-      const float rest = log2f(sum), all = top + rest, back = all - top;
-      lse[row] = make_float2(all, fabsf(all) < INFINITY ? (top - (all - back)) + (rest - back) : 0.f);
+      const float rest = log2_above(sum, top);
+      lse[row] = make_float2(top, rest);
       const int64_t t = targets[row];
       if (t != ignore_index) {
-        const float2 here = at_target[row];
-        mine = t < 0 || t >= vocab ? NAN : ((lse[row].x - here.x) + (lse[row].y - here.y)) * kLn2;
+        mine = t < 0 || t >= vocab ? NAN : (top - at_target[row]) + rest * kLn2;
         counts = 1.f;
       }
       if (reduction == SA_REDUCTION_NONE) loss[row] = mine;
@@ -210,8 +209,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
 
 // ---- training: what stands between the products -----------------------------------------------------------------------------------
 
-// What e is relative to, in log2 units: the target's logit; +inf for a token that does not count, NaN for a target outside the
-// vocabulary.  A warp a token.
+// What e is relative to: the target's logit; +inf for a token that does not count, NaN for a target outside the vocabulary.  A warp a token.
 __global__ void __launch_bounds__(256) reference_kernel(const void* x, int x_dtype, int64_t x_stride, const void* weight, int weight_dtype,
                                                         int64_t weight_stride, const int64_t* targets, int64_t ignore_index, int tokens, int vocab,
                                                         int width, float* ref, int* any) {
@@ -232,19 +230,20 @@ __global__ void __launch_bounds__(256) reference_kernel(const void* x, int x_dty
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (lane == 0) ref[row] = t == ignore_index ? INFINITY : t < 0 || t >= vocab ? NAN : sum * kLog2e;
+  if (lane == 0) ref[row] = t == ignore_index ? INFINITY : t < 0 || t >= vocab ? NAN : sum;
 }
 
 struct Rows {                              // of a run of tokens
   const float2* stats;                     // (maximum, sum) of every half tile, [slots][tokens]
   int slots;
-  const float2* at_target;
+  const float* at_target;
   const float* e_target;
   const int64_t* targets;
   int64_t ignore_index;
   int tokens, vocab, width;
   float* ref;
-  int* far;                                // rows whose sums left the range
+  int* far;                                // rows whose sums left the range: the target's logit is far from the largest, or, of logits
+                                           // of 10^9, from what the product makes of it
   int* any;                                // whether there is one
   int again;                               // they have been through the product once more
   float* loss;
@@ -295,7 +294,7 @@ __global__ void __launch_bounds__(kJoinThreads) rows_kernel(const Rows r) {
     if (r.again) {
       now = inside && r.far[row] != 0;
     } else if (inside) {
-      const bool far = counts && good && !(sum < kFarthest);
+      const bool far = counts && good && !(sum < kFarthest && sum > 1.f / kFarthest);
       r.far[row] = far;
       if (far) {
         r.ref[row] = top;
@@ -310,7 +309,7 @@ __global__ void __launch_bounds__(kJoinThreads) rows_kernel(const Rows r) {
         const float ref = r.ref[row];
         inverse = good ? 1.f / sum : NAN;
         const float e = r.e_target[row];
-        loss = !good ? NAN : (e > 1.f / kFarthest ? log2f(sum / e) : (ref - r.at_target[row].x) + log2f(sum)) * kLn2;
+        loss = !good ? NAN : e > 1.f / kFarthest ? log2f(sum / e) * kLn2 : (ref - r.at_target[row]) + log2_above(sum, ref) * kLn2;
         at_target = good ? (e - sum) * inverse : NAN;
         if (good)
           for (int part = 0; part < r.parts; ++part) r.e[part * r.e_part + (int64_t)row * r.e_pitch + t] = 0;
@@ -613,8 +612,8 @@ struct Forward {
   Room room;
   Operand x, weight;
   int ctas, run;
-  float2 *stats, *sums, *at_target;
-  float* losses = nullptr;       // of several runs
+  float2 *stats, *sums;
+  float *at_target, *losses = nullptr;       // losses: of several runs
   unsigned int* ticket;
   Forward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
@@ -623,7 +622,7 @@ struct Forward {
     run = std::min(p.tokens, kForwardRun);
     stats = room.take<float2>((int64_t)2 * walk_of(run, p.vocab, p.width, terms_of(p), ctas, false).n_tiles * run);
     sums = room.take<float2>(over(run, 32));
-    at_target = room.take<float2>(run);
+    at_target = room.take<float>(run);
     if (run < p.tokens && p.reduction != SA_REDUCTION_NONE) losses = room.take<float>(p.tokens);
     ticket = room.take<unsigned int>(1);
   }
@@ -711,7 +710,8 @@ struct Train {
   float *ref, *losses, *less, *e_target, *inverse, *dx_slabs = nullptr, *dw_slabs = nullptr;
   int *far, *any;
   void* sorted = nullptr;        // of the targets
-  float2 *stats, *at_target;
+  float2* stats;
+  float* at_target;
   Train(const Problem& p, void* base) : room{static_cast<char*>(base)} {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
@@ -721,7 +721,7 @@ struct Train {
     less = room.take<float>(p.tokens);
     far = room.take<int>(p.tokens);
     any = room.take<int>(1);
-    at_target = room.take<float2>(run);
+    at_target = room.take<float>(run);
     e_target = room.take<float>(run);
     inverse = room.take<float>(run);
     stats = room.take<float2>((int64_t)2 * logits_walk(p, run).n_tiles * run);
@@ -797,7 +797,7 @@ int forward(const Problem& p, cudaStream_t s) {
     st = run<kStats, false, false>(f.ctas, f.x, f.weight, walk, Origin{n0, 0}, Origin{0, 0}, e, status, s);
     if (st != SA_OK) return st;
     const bool each = f.losses != nullptr || p.reduction == SA_REDUCTION_NONE;
-    st = launch_after(join_kernel, dim3((unsigned)over(tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * walk.n_tiles, (const float2*)f.at_target,
+    st = launch_after(join_kernel, dim3((unsigned)over(tokens, 32)), kJoinThreads, 0, s, (const float2*)f.stats, 2 * walk.n_tiles, (const float*)f.at_target,
                       e.targets, p.ignore_index, tokens, p.vocab, each ? (int)SA_REDUCTION_NONE : p.reduction, reinterpret_cast<float2*>(p.lse) + n0,
                       each ? (f.losses != nullptr ? f.losses : p.loss) + n0 : p.loss, p.count, f.sums, f.ticket);
   }

@@ -99,20 +99,20 @@ struct Origin {
 enum Kind { kStats, kProbabilities, kBoth, kResult, kSegments };
 
 struct Epilogue {
-  // kStats: of every row and half tile, the maximum (times log2 e) and the sum of exponentials above it; the targets' logits
+  // kStats: of every row and half tile, the maximum and the sum of exponentials above it (see base_of); the targets' logits
   float2* stats;                           // [2 * n_tiles][m]
-  float2* at_target;                       // [m], times log2 e, in two parts
+  float* at_target;                        // [m]
   float* e_target;                         // kBoth: [m], the exponential
   const int64_t* targets;
   int column0;                             // of the vocabulary, that the launch's first column is
   unsigned int* zeroed;                    // kStats: a counter to be cleared for the kernel behind
-  // kBoth: exp2(z log2 e - ref) in `parts` parts, with their sum (and the maximum of z log2 e) in the place of the others'; 0 where
+  // kBoth: exp(z - ref) (see base_of) in `parts` parts, with their sum (and the maximum of z) in the place of the others'; 0 where
   // ref is +inf
   const float* ref;
   const int* only;                         // rows that are not marked stay as they are; null: all are meant
   const int* any;                          // nothing is done where this is 0; null: it is done
-  // kProbabilities: (exp2(z log2 e - lse) - [target]) * factor, in `parts` 16-bit parts
-  const float2* lse;                       // in two parts
+  // kProbabilities: (exp2((z - lse.x) log2 e - lse.y) - [target]) * factor, in `parts` 16-bit parts
+  const float2* lse;
   const float* factor;
   float* less;                             // of one or two parts: [m], what the first one's rounding takes from the target's column, times `scale`
   uint16_t* p;
@@ -296,43 +296,63 @@ __device__ __forceinline__ float most_of(const uint32_t (&r)[32], float than) {
       m[k] = i + 4 + k < 32 ? most_of(m[k], __uint_as_float(r[i + k]), __uint_as_float(r[i + 4 + k])) : fmaxf(m[k], __uint_as_float(r[i + k]));
   return fmaxf(most_of(m[0], m[1], m[2]), m[3]);
 }
-// exp2(z log2 e - from) of 32 columns, and their sum.
-__device__ __forceinline__ float exponentials(const uint32_t (&r)[32], float from, float (&p)[32]) {
-  const Pair by = pair(kLog2e, kLog2e), less = pair(-from, -from);
+// Exponentials of logits relative to another one, exp(z - top), are exp2(z log2 e - base) for the base of `top`: top * log2 e, rounded once
+// and taken from the exact product, so that only what the base is relative to moves (a rounded z log2 e of 100 would move its exponential
+// by 2^-18).  The rounding is up to 8 where |top| is kHuge, far less than an exponential can bear, and anything beyond, where logits
+// mask words or stand for nothing else that is useful: there the difference comes first and the base is `top` itself.
+constexpr float kHuge = 134217728.f;                        // 2^27
+__device__ __forceinline__ bool is_huge(float top) { return fabsf(top) >= kHuge; }
+__device__ __forceinline__ float base_of(float top) { return __fmul_rn(top, kLog2e); }
+// log2 of exponentials that are relative to the base of `top`, were they relative to that of `other`.
+__device__ __forceinline__ float between(float top, float other) {
+  return is_huge(top) || is_huge(other) ? (top - other) * kLog2e : base_of(top) - base_of(other);
+}
+// log2 of a sum relative to the base of `top`, above top itself.
+__device__ __forceinline__ float log2_above(float sum, float top) {
+  return log2f(sum) - (is_huge(top) ? 0.f : __fmaf_rn(top, kLog2e, -base_of(top)));
+}
+// Of 32 columns, and their sum.
+__device__ __forceinline__ float exponentials(const uint32_t (&r)[32], float top, float (&p)[32]) {
+  const Pair by = pair(kLog2e, kLog2e);
   Pair sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-#pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const float2 x = both(fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), by, less));
-    p[i] = ex2(x.x);
-    p[i + 1] = ex2(x.y);
+  auto add = [&](int i, Pair x) {
+    const float2 at = both(x);
+    p[i] = ex2(at.x);
+    p[i + 1] = ex2(at.y);
     sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], pair(p[i], p[i + 1]));
+  };
+  if (is_huge(top)) {
+    const Pair less = pair(-top, -top);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) add(i, fma2(add2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), less), by, pair(0.f, 0.f)));
+  } else {
+    const Pair less = pair(-base_of(top), -base_of(top));
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) add(i, fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), by, less));
   }
   const float2 a = both(sums[0]), b = both(sums[1]);
   return (a.x + a.y) + (b.x + b.y);
 }
+__device__ __forceinline__ float exponential(float z, float top) {           // one, as it stands in the sum
+  return ex2(is_huge(top) ? (z - top) * kLog2e : __fmaf_rn(z, kLog2e, -base_of(top)));
+}
 
-// Running maximum, in log2 units and rounded, and sum of exponentials above it.  The differences are taken before they are rounded:
-// a rounded logit of 100 would move its exponential by 2^-18.
+// Running maximum and sum of exponentials above it.
 struct RowStats {
-  float top = -INFINITY, from = 0.f, sum = 0.f;             // from: top * log2 e, or 0 while nothing is above -inf
+  float top = -INFINITY, sum = 0.f;
   __device__ __forceinline__ void add(uint32_t (&r)[32], int valid) {
     if (valid < 32) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = i < valid ? r[i] : __float_as_uint(-INFINITY);
     }
-    const float best = most_of(r, top), to = best == -INFINITY ? 0.f : best * kLog2e;
-    sum *= top == -INFINITY ? 0.f : ex2(from - to);
+    const float best = most_of(r, top), from = best == -INFINITY ? 0.f : best;
+    sum *= top == -INFINITY ? 0.f : ex2(between(top, from));
     top = best;
-    from = to;
     float p[32];
     sum += exponentials(r, from, p);
   }
-  __device__ __forceinline__ float2 result() const { return make_float2(top == -INFINITY ? top : from, sum); }
+  __device__ __forceinline__ float2 result() const { return make_float2(top, sum); }
 };
-__device__ __forceinline__ float2 in_log2(float z) {         // z * log2 e in two parts
-  const float hi = z * kLog2e;
-  return make_float2(hi, fabsf(hi) < INFINITY ? __fmaf_rn(z, kLog2e, -hi) : 0.f);
-}
 
 // 32 columns rounded to the parts; exactly nothing of a token that does not count, whatever they are.
 __device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], bool counts, int64_t at) {
@@ -365,14 +385,14 @@ __device__ __forceinline__ float select(const uint32_t (&r)[32], int i) {
   return v;
 }
 
-// (exp2(z - lse) - [target]) * factor of 32 columns, rounded to the parts.
+// (exp2((z - lse.x) log2 e - lse.y) - [target]) * factor of 32 columns, rounded to the parts.
 __device__ __forceinline__ void store_probabilities(const Epilogue& e, const uint32_t (&r)[32], int row, int64_t at, float2 lse, float factor,
                                                     int target) {
-  const Pair by = pair(kLog2e, kLog2e), less = pair(-lse.x, -lse.x), less_still = pair(-lse.y, -lse.y);
+  const Pair by = pair(kLog2e, kLog2e), top = pair(-lse.x, -lse.x), rest = pair(-lse.y, -lse.y);
   float p[32];
 #pragma unroll
   for (int i = 0; i < 32; i += 2) {
-    const float2 x = both(add2(fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), by, less), less_still));
+    const float2 x = both(fma2(add2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), top), by, rest));
     p[i] = ex2(x.x);
     p[i + 1] = ex2(x.y);
   }
@@ -726,12 +746,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int col = u.tn * w.bn + i * 32;
           stats.add(r, w.n - col);
           const int64_t mine = target - e.column0 - col;
-          if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = in_log2(select(r, (int)mine));
+          if (mine >= 0 && mine < 32 && col + mine < w.n) e.at_target[row] = select(r, (int)mine);
         });
         if (inside) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = stats.result();
       } else if constexpr (KIND == kBoth) {
         const int64_t target = inside ? e.targets[row] : -1;
-        const float ref = inside ? e.ref[row] : INFINITY;
+        const float ref = inside ? e.ref[row] : INFINITY, relative_to = ref == INFINITY ? 0.f : ref;
         const bool store = inside && (e.only == nullptr || e.only[row] != 0);
         float top = -INFINITY, sum = 0.f;
         each_chunk([&](int i, uint32_t (&r)[32]) {
@@ -743,15 +763,15 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             for (int j = 0; j < 32; ++j) r[j] = j < valid ? r[j] : __float_as_uint(-INFINITY);
           }
           top = most_of(r, top);
-          sum += exponentials(r, ref, p);
+          sum += exponentials(r, relative_to, p);
           if (store && mine >= 0 && mine < 32 && mine < valid) {
             const float z = select(r, (int)mine);
-            e.at_target[row] = in_log2(z);
-            e.e_target[row] = ex2(__fmaf_rn(z, kLog2e, -ref));        // as it stands in the sum
+            e.at_target[row] = z;
+            e.e_target[row] = exponential(z, ref);
           }
           if (store) store_parts(e, p, ref != INFINITY, (int64_t)row * e.p_pitch + col);
         });
-        if (store) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(top * kLog2e, ref != INFINITY ? sum : 0.f);
+        if (store) e.stats[(int64_t)(2 * u.tn + half) * w.m + row] = make_float2(top, ref != INFINITY ? sum : 0.f);
       } else if constexpr (KIND == kProbabilities) {
         const float2 lse = inside ? e.lse[row] : make_float2(0.f, 0.f);
         const float factor = inside ? e.factor[row] : 0.f;

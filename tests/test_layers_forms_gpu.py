@@ -42,3 +42,62 @@ def test_tangents_and_batches_of_a_transform_are_refused(name):
             torch.func.jvp(lambda a: call(*inputs[:i], a, *inputs[i + 1:]), (inputs[i],), (torch.ones_like(inputs[i]),))
         with pytest.raises(RuntimeError):
             torch.func.vmap(lambda a: call(*inputs[:i], a, *inputs[i + 1:]))(inputs[i][None])
+
+
+def _gradients(x, w, targets, reduction):
+    a, b = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    loss = layers.linear_cross_entropy(a, b, targets, reduction=reduction)
+    return [loss.detach(), *torch.autograd.grad(loss, (a, b), torch.ones_like(loss))]
+
+
+@pytest.mark.parametrize("masked", [-1e4, -1e8, -3e8, -1e10, -1e30, -2e38])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_words_masked_by_any_number_leave_the_others_alone(dtype, masked):
+    """A column of ones and a bias of the words in the table; whole tiles of nothing but masked words, before, between and behind others."""
+    gen = torch.Generator("cpu").manual_seed(51)
+    x, w = torch.randn(150, 64, generator=gen).to(dtype).cuda(), (torch.randn(1500, 64, generator=gen) * 0.2).to(dtype).cuda()
+    kept = torch.zeros(1500, dtype=torch.bool, device="cuda")
+    kept[520:700], kept[1100:1180] = True, True
+    x[:, 63] = 1
+    w[:, 63] = 0
+    w[~kept] = 0
+    w[~kept, 63] = masked
+    words = kept.nonzero()[:, 0]
+    at = torch.randint(0, len(words), (150,), generator=gen).cuda()
+    for reduction in ("none", "sum"):
+        loss, dx, dw = _gradients(x, w, words[at], reduction)
+        want, wanted, dwant = _gradients(x, w[kept], at, reduction)
+        assert torch.isfinite(loss).all() and (loss - want).abs().max() <= 2.0 ** -20 * (150 if reduction == "sum" else 1) * 8
+        half = torch.finfo(dtype).eps / 2 + 2.0 ** -20          # the same sums, of more or fewer tiles
+        assert (dx.float() - wanted.float()).abs().max() <= 2 * half * wanted.float().abs().max()
+        assert (dw[kept].float() - dwant.float()).abs().max() <= 2 * half * dwant.float().abs().max() and (dw[~kept] == 0).all()
+    # rows that the mask leaves nothing of: all words alike
+    loss, dx, _ = _gradients(x, w[~kept], at, "none")
+    assert (loss - torch.log(torch.tensor(1500.0 - len(words)))).abs().max() < 2.0 ** -18 and torch.isfinite(dx).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [30.0, 1e3, 1e4, 1e6])
+def test_logits_of_any_size(dtype, scale):
+    """Up to 10^13: losses of nothing or of about as much, as their products are rounded."""
+    gen = torch.Generator("cpu").manual_seed(52)
+    x, w = ((torch.randn(n, 64, generator=gen) * scale).to(dtype).cuda() for n in (200, 900))
+    z = x.double() @ w.double().T
+    targets = z.argmax(1)
+    targets[::2] = torch.randint(0, 900, (100,), generator=gen).cuda()
+    p = torch.softmax(z, 1)
+    off = 18 * 2.0 ** -22 * (x.double().abs() @ w.double().abs().T).amax(1)          # of any logit: 64 / 16 groups of products, in up to 3 parts
+    want = torch.logsumexp(z, 1) - z.gather(1, targets[:, None])[:, 0]
+    loss, dx, dw = _gradients(x, w, targets, "none")
+    assert ((loss.double() - want).abs() <= 2 * off + 2.0 ** -20 * (1 + want)).all()
+    # half the targets are the largest word by far: nothing is left of their gradients
+    sure = (1 - p.gather(1, targets[:, None])[:, 0] < 1e-30) & (z.topk(2).values.diff(dim=1)[:, 0].abs() > 4 * off + 100)
+    # but for exp2(r) of a rounding r of the largest logit times log2 e, of up to 8: 2^-22 of itself, its logarithm 2^-24 of up to 8 and as
+    # much again for r taken from it, so 2^-20 in the loss, and in dz, whose exponential adds 2^-22
+    assert sure.sum() > 60 and (loss[sure].abs() < 2.0 ** -20).all() and torch.isfinite(dx).all() and torch.isfinite(dw).all()
+    assert (dx[sure].abs() <= 2.0 ** -19 * w.float().abs().amax()).all()
+    import test_layers_gpu
+
+    total, dx, dw = test_layers_gpu._with_the_loss(x, w, targets, -100, "sum", dtype, torch.ones((), device="cuda"))
+    assert abs(float(total) - float(want.sum())) <= float((2 * off + 2.0 ** -20 * (1 + want)).sum()) + 2.0 ** -23 * float(want.sum())
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and (dx[sure] == 0).all()
