@@ -21,6 +21,7 @@
 #include "sa_loss.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sa_layers.cuh"
 #include "sa_product.cuh"
@@ -488,7 +489,9 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
   w.slabs = 1;
   const int most = kSms / ctas;
   w.clusters = std::min(w.tiles(), most);
-  w.segment = result && terms == kTerms ? kSegment : w.blocks;
+  const bool three = terms == kTerms;      // parts of an fp32 operand
+  const bool cut = three ? result || w.depth_blocks > kSegment : w.blocks > (result ? kSegmentResult : kUncutLogits);
+  w.segment = !cut ? w.blocks : three ? kSegment : result ? kSegmentResult : kSegmentLogits;
   w.group = result ? 1 : std::min(w.m_tiles, 32);
   const int left = w.tiles() % most;
   if (result && left > 0) {
@@ -503,10 +506,10 @@ Walk walk_of(int m, int n, int64_t depth, int terms, int ctas, bool result, int6
 }
 int64_t slab_floats(const Walk& w, int ctas) { return (int64_t)(w.tiles() - w.whole) * w.slabs * kRows * ctas * w.bn; }
 
-template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
+template <int CTAS, Kind KIND, bool A_MN, bool B_MN, bool SEGMENTS>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const Walk& w, Origin at_a, Origin at_b, int a_bytes, const Epilogue& e, const WaitCtx& status,
            cudaStream_t s) {
-  auto kernel = product_kernel<CTAS, KIND, A_MN, B_MN>;
+  auto kernel = product_kernel<CTAS, KIND, A_MN, B_MN, SEGMENTS>;
   constexpr size_t kBytes = KIND == kResult ? kSmemResult : kSmem;
   SA_CUDA_CHECK(allow_smem(kernel, kBytes));
   cudaLaunchAttribute attrs[2];
@@ -537,8 +540,12 @@ int run(int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a
   if (st == SA_OK) st = b.map(&map_b, B_MN, kRows);
   if (st != SA_OK) return st;
   const int a_bytes = A_MN ? kOperand : box * kDepth * 2;
-  return ctas == 2 ? launch<2, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s)
-                   : launch<1, KIND, A_MN, B_MN>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s);
+  auto go = [&](auto segments) {
+    constexpr bool SEGMENTS = decltype(segments)::value;
+    return ctas == 2 ? launch<2, KIND, A_MN, B_MN, SEGMENTS>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s)
+                     : launch<1, KIND, A_MN, B_MN, SEGMENTS>(map_a, map_b, w, at_a, at_b, a_bytes, e, status, s);
+  };
+  return w.segment < w.blocks ? go(std::true_type()) : go(std::false_type());
 }
 
 // CTAs of a tile: two where there are rows for both.
@@ -693,14 +700,13 @@ int finish(const Epilogue& e, const Walk& w, int ctas, cudaStream_t s) {
   return launch_after(finish_kernel, dim3(w.tiles() - w.whole, kRows * ctas / rows), kFinishThreads, 0, s, (const Epilogue)e, (const Walk)w, kRows * ctas);
 }
 
-// A product into a result, by kResult or, for fp32 operands, kSegments.
+// A product into a result.
 template <bool A_MN, bool B_MN>
-int run_result(const Problem& p, int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, Epilogue e,
+int run_result(int ctas, const Operand& a, const Operand& b, const Walk& w, Origin at_a, Origin at_b, Epilogue e,
                const WaitCtx& status, cudaStream_t s) {
   e.aligned = ((reinterpret_cast<uintptr_t>(e.out) | (uintptr_t)e.out_pitch * bytes_of(e.dtype)) & (e.dtype == SA_F32 ? 31 : 15)) == 0;
   e.addend_first = ((reinterpret_cast<uintptr_t>(e.addend) | (uintptr_t)e.addend_pitch * 4) & 31) == 0;
-  return p.product == SA_F32 ? run<kSegments, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s)
-                             : run<kResult, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s);
+  return run<kResult, A_MN, B_MN>(ctas, a, b, w, at_a, at_b, e, status, s);
 }
 
 struct Train {
@@ -893,7 +899,7 @@ int train(const Problem& p, cudaStream_t s) {
       o.table_factor = t.less + n0;
       o.targets = e.targets;
       o.vocab = p.vocab;
-      st = run_result<false, true>(p, ctas, left, t.weight, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      st = run_result<false, true>(ctas, left, t.weight, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
       if (st == SA_OK) st = finish(o, w, ctas, s);
     }
     if (p.dweight_sums != nullptr && st == SA_OK) {
@@ -907,7 +913,7 @@ int train(const Problem& p, cudaStream_t s) {
       o.addend_pitch = p.width;
       o.slabs = t.dw_slabs;
       o.later = !first;
-      st = run_result<true, true>(p, ctas, left, right, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
+      st = run_result<true, true>(ctas, left, right, w, Origin{0, 0}, Origin{0, 0}, o, status, s);
       if (st == SA_OK && last) st = finish(o, w, ctas, s);
     }
   }
@@ -1009,7 +1015,7 @@ int backward(const Problem& p, cudaStream_t s) {
       r.vocab = p.vocab;
       r.slabs = b.dx_slabs;
       r.later = !first;
-      st = run_result<false, true>(p, b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
+      st = run_result<false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
       if (st == SA_OK && last) st = finish(r, w, b.ctas, s);
       if (st != SA_OK) return st;
     }
@@ -1023,7 +1029,7 @@ int backward(const Problem& p, cudaStream_t s) {
       r.out_pitch = p.width;
       r.scale = scale;
       r.slabs = b.dw_slabs;
-      st = run_result<true, true>(p, ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
+      st = run_result<true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
       if (st == SA_OK) st = finish(r, w, ctas, s);
     }
   }

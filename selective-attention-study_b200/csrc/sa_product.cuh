@@ -1,5 +1,5 @@
 // Matrix products of the loss over a vocabulary (sa_loss.cu): D = A B^T with 16-bit operands and fp32 sums, a persistent kernel
-// with three epilogues.  A CTA, or the two CTAs of a cluster on one tile (CTAS = 2), own 128 rows each of a tile of up to
+// with four epilogues.  A CTA, or the two CTAs of a cluster on one tile (CTAS = 2), own 128 rows each of a tile of up to
 // 128 * CTAS columns; TMA fills a ring of stages 64 deep, one thread issues the MMAs, and two accumulators in tensor memory let
 // the epilogue of a tile run under the products of the next.
 //
@@ -26,7 +26,12 @@ constexpr size_t kSmem = (size_t)kStages * 2 * kOperand + 1024;
 constexpr int kTurnPitch = 33;               // words of 32 columns that a warp turns
 constexpr size_t kSmemResult = kSmem + (size_t)kEpilogueWarps * 32 * kTurnPitch * 4;
 constexpr int kTerms = 6;                  // of an fp32 product
-constexpr int kSegment = 4;                // stages, with kSegments: 256 of the contraction
+// The tensor cores' additions round towards zero: 2^-23.4 a group of 16 products of what is summed, all one way, so a long sum loses in
+// proportion to its length (logits of a width of 4,096: 2.8e-6 of the loss; the mean of 50,304 rows of a table: 2.9e-4 of it).  So an
+// epilogue adds the sums of a few stages at a time in its registers, with rounding to nearest: of fp32 operands of 256 of the contraction
+// (1.5e-7 of the loss); of 16-bit ones of 512 in logits, up to a width of 1,024 of all (3e-7, 6.9e-7), and of 8,192 in gradients, which are
+// rounded to 16 bits themselves.
+constexpr int kSegment = 4, kSegmentLogits = 8, kUncutLogits = 16, kSegmentResult = 128;
 constexpr int kSegmentChunks = 4;          // chunks of 32 columns of a tile that a thread of an epilogue has, at most
 
 // The work of a launch: tiles of rows x columns, each a walk over `blocks` stages of the contraction.  The first `whole` tiles are
@@ -40,7 +45,7 @@ struct Walk {
   int depth_blocks, blocks;                // stages of one term, of all terms
   int clusters;
   int slabs;                               // of a cut tile
-  int segment;                             // stages that are summed in tensor memory at a time
+  int segment;                             // stages that are summed in tensor memory at a time, `blocks` without SEGMENTS
   int group;                               // row tiles that are walked side by side
   __host__ __device__ int tiles() const { return m_tiles * n_tiles; }
   __host__ __device__ void place(int tile, int* tm, int* tn) const {
@@ -59,13 +64,12 @@ struct Walk {
 struct Units {
   int at, k, share1;                       // the next item: a whole tile, or a part of one behind them
   int tile, tm, tn, k0, k1, slab;
-  bool first, last;                        // of this cluster's sums of the tile
+  bool last;                               // of this cluster's sums of the tile
   __host__ __device__ void begin(int c) {
     at = c;
     k = share1 = 0;
   }
   __host__ __device__ bool next(const Walk& w) {
-    first = k >= share1;
     while (k >= share1) {
       const int left = w.tiles() - w.whole;
       if (at >= w.whole + left * w.slabs) return false;
@@ -94,9 +98,8 @@ struct Origin {
   int own, depth;
 };
 
-// kSegments: kResult whose sums leave tensor memory every `segment` stages, into registers: the tensor cores' additions round towards zero,
-// which fp32 results would show.
-enum Kind { kStats, kProbabilities, kBoth, kResult, kSegments };
+// SEGMENTS of the kernel: sums leave tensor memory every `segment` stages, of which every tile has several.
+enum Kind { kStats, kProbabilities, kBoth, kResult };
 
 struct Epilogue {
   // kStats: of every row and half tile, the maximum and the sum of exponentials above it (see base_of); the targets' logits
@@ -537,12 +540,11 @@ __device__ __forceinline__ void store_across(T* out, int64_t pitch, const float*
   __syncwarp();
 }
 
-// 32 columns of a warp's 32 rows of the result, or of a slab; a thread's row is `row0` and its lane.  With `turn`, rows that start anywhere
-// go across: the fp32 products' sums leave no registers for that, and their stores wait for the tensor cores anyway.
+// 32 columns of a warp's 32 rows of the result, or of a slab; a thread's row is `row0` and its lane.  Rows that start anywhere go across.
 __device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, const Units& u, uint32_t (&r)[32], int row0, int lane, int in_tile,
                                              int tile_rows, int chunk, float* turn) {
   const int col = u.tn * w.bn + chunk * 32, valid = w.n - col, row = row0 + lane;
-  const bool across = turn != nullptr && !e.aligned && u.tile < w.whole, inside = row < w.m;
+  const bool across = !e.aligned && u.tile < w.whole, inside = row < w.m;
   if (valid <= 0 || row0 >= w.m || (!inside && !across)) return;
   if (u.tile >= w.whole) {
     float* const slab = e.slabs + (((int64_t)(u.tile - w.whole) * w.slabs + u.slab) * tile_rows + in_tile) * w.bn + chunk * 32;
@@ -589,7 +591,7 @@ __device__ __forceinline__ void store_result(const Epilogue& e, const Walk& w, c
 
 // `a_bytes`: of the left operand in a stage, less than a whole one where its box has fewer rows; what stands in the others' place makes
 // rows of the tile that nothing reads.
-template <int CTAS, Kind KIND, bool A_MN, bool B_MN>
+template <int CTAS, Kind KIND, bool A_MN, bool B_MN, bool SEGMENTS>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Walk w, const Origin at_a,
                const Origin at_b, const int a_bytes, const Epilogue e, const WaitCtx status) {
@@ -708,7 +710,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t read_there = CTAS == 2 ? address_in(read, 0) : read;
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 128 && e.zeroed != nullptr) *e.zeroed = 0u;
     float* const turn = reinterpret_cast<float*>(smem + kStages * 2 * kOperand) + (warp - 4) * 32 * kTurnPitch;    // kResult
-    uint32_t sums[KIND == kSegments ? kSegmentChunks : 1][32];
+    uint32_t sums[SEGMENTS ? kSegmentChunks : 1][32];
+    auto clear = [&] {                                               // behind a tile, so that its epilogue has the registers
+#pragma unroll
+      for (int i = 0; i < kSegmentChunks; ++i)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sums[i][j] = 0u;
+    };
+    if constexpr (SEGMENTS) clear();
     int n = 0;
     while (u.next(w)) {
       const int row = u.tm * kColumns + (int)rank * kRows + (warp & 3) * 32 + lane;
@@ -739,6 +748,29 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           f(i, r);
         }
       };
+      if constexpr (SEGMENTS) {
+        // the last one's sums and the others' meet in tensor memory, where they take no registers of what follows
+#pragma unroll
+        for (int i = 0; i < kSegmentChunks; ++i) {
+          if (from + i >= to) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[16];
+            tmem_ld16(acc + (from + i) * 32 + 16 * h, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[i][16 * h + j] = __float_as_uint(__uint_as_float(sums[i][16 * h + j]) + __uint_as_float(r[j]));
+          }
+          if (u.last) tmem_st32(acc + (from + i) * 32, sums[i]);
+        }
+        if (u.last) {
+          tmem_st_wait();
+        } else {
+          release();
+          ++n;
+          continue;
+        }
+      }
       if constexpr (KIND == kStats) {
         const int64_t target = inside ? e.targets[row] : -1;
         RowStats stats;
@@ -781,33 +813,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int64_t mine = target - e.column0 - col;
           if (inside) store_probabilities(e, r, row, (int64_t)row * e.p_pitch + col, lse, factor, mine >= 0 && mine < 32 ? (int)mine : -1);
         });
-      } else if constexpr (KIND == kResult) {
+      } else {
         const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
         each_chunk([&](int i, uint32_t (&r)[32]) {
           store_result(e, w, u, r, row - lane, lane, in_tile, kColumns, i, turn);
         });
-      } else {
-        const int in_tile = (int)rank * kRows + (warp & 3) * 32 + lane;
-#pragma unroll
-        for (int i = 0; i < kSegmentChunks; ++i) {
-          if (from + i >= to) break;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[16];
-            tmem_ld16(acc + (from + i) * 32 + 16 * h, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              sums[i][16 * h + j] = __float_as_uint((u.first ? 0.f : __uint_as_float(sums[i][16 * h + j])) + __uint_as_float(r[j]));
-          }
-        }
-        if (u.last && inside) {
-#pragma unroll
-          for (int i = 0; i < kSegmentChunks; ++i)
-            if (from + i < to) store_result(e, w, u, sums[i], row - lane, lane, in_tile, kColumns, from + i, nullptr);
-        }
       }
-      if constexpr (KIND == kSegments) release();
+      if constexpr (SEGMENTS) clear();
       ++n;
     }
   }

@@ -101,3 +101,78 @@ def test_logits_of_any_size(dtype, scale):
     total, dx, dw = test_layers_gpu._with_the_loss(x, w, targets, -100, "sum", dtype, torch.ones((), device="cuda"))
     assert abs(float(total) - float(want.sum())) <= float((2 * off + 2.0 ** -20 * (1 + want)).sum()) + 2.0 ** -23 * float(want.sum())
     assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and (dx[sure] == 0).all()
+
+
+def _definition(x, w, targets):
+    """Losses, and the gradients of their sum, in 64 bits."""
+    x, w = x.double(), w.double()
+    z = x @ w.T
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    losses = (lse - z.gather(1, targets[:, None]))[:, 0]
+    dz = torch.exp_(z.sub_(lse)).scatter_add_(1, targets[:, None], -torch.ones_like(lse))
+    return losses, dz @ w, dz.T @ x
+
+
+def _off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("dtype,bound", [(BF16, 1e-6), (F16, 1e-6), (F32, 6e-7)])
+@pytest.mark.parametrize("tokens", [100, 300])
+@pytest.mark.parametrize("width", [2048, 4096, 16384])
+def test_a_wide_products_error_does_not_grow_with_its_width(width, tokens, dtype, bound):
+    """A group of 16 products loses up to 2^-23 of what is summed so far, towards zero: half of that over 512 of the contraction, on what
+    is half of its sum on average, is 5e-7 of the sum (of 256, 2.4e-7); several such sums have signs of their own.  Over the whole width,
+    the loss was 1.4e-6, 2.8e-6 and 1.1e-5 off; fp32 gradients 1.7e-6, 3.4e-6 and 1.2e-5."""
+    gen = torch.Generator("cuda").manual_seed(61)
+    x = torch.randn(tokens, width, generator=gen, device="cuda").to(dtype)
+    w = (torch.randn(3000, width, generator=gen, device="cuda") * 3.0 / width ** 0.5).to(dtype)
+    targets = torch.randint(0, 3000, (tokens,), generator=gen, device="cuda")
+    losses, dx, dw = _definition(x, w, targets)
+    got = _gradients(x, w, targets, "none")
+    with torch.no_grad():
+        alone = layers.linear_cross_entropy(x, w, targets, reduction="none")
+    assert _off(got[0], losses) < bound and _off(alone, losses) < bound
+    # e^z has z's error times its size, of 3 to 10 here, beside roundings to the type
+    half = torch.finfo(dtype).eps / 2
+    grads = [got[1:]]
+    if dtype != F16:
+        import test_layers_gpu
+
+        total, *with_the_loss = test_layers_gpu._with_the_loss(x, w, targets, -100, "sum", dtype, torch.ones((), device="cuda"))
+        assert abs(float(total) - float(losses.sum())) < bound * float(losses.sum())
+        grads.append(with_the_loss)
+    for a, b in grads:
+        assert _off(a, dx) < 1.2e-6 + half and _off(b, dw) < 1.2e-6 + half
+
+
+@pytest.mark.parametrize("tokens,vocab,width", [(8000, 600, 72), (70, 60000, 40), (4000, 9000, 520)])
+def test_a_long_sums_error_in_fp32_does_not_grow_with_its_length(tokens, vocab, width):
+    """Sums of the gradients over tokens and words: 2.4e-6 where 2,048 of the contraction were added towards zero."""
+    gen = torch.Generator("cuda").manual_seed(62)
+    x, w = (torch.randn(n, width, generator=gen, device="cuda") for n in (tokens, vocab))
+    w *= 3.0 / width ** 0.5
+    targets = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    losses, dx, dw = _definition(x, w, targets)
+    import test_layers_gpu
+
+    ones = torch.ones((), device="cuda")
+    for loss, a, b in (_gradients(x, w, targets, "none"), test_layers_gpu._with_the_loss(x, w, targets, -100, "sum", F32, ones)):
+        assert _off(loss, losses if loss.dim() else losses.sum()) < 6e-7 and _off(a, dx) < 1.2e-6 and _off(b, dw) < 1.2e-6
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_what_rows_of_a_table_have_in_common_keeps_its_size(reduction):
+    """dx is a mean of the table's rows less one of them; the rows' own mean of 1 enters and leaves.  Towards zero, 50,304 words lost 2.9e-4
+    of it, 1.8 times what dx is rounded by."""
+    gen = torch.Generator("cuda").manual_seed(63)
+    x = (torch.randn(4864, 1024, generator=gen, device="cuda") * 0.2).to(BF16)
+    w = (1 + torch.randn(50304, 1024, generator=gen, device="cuda") * 0.1).to(BF16)
+    targets = torch.randint(0, 50304, (4864,), generator=gen, device="cuda")
+    a = x.clone().requires_grad_(True)
+    loss = layers.linear_cross_entropy(a, w, targets, reduction=reduction)
+    (dx,) = torch.autograd.grad(loss, a, torch.ones_like(loss))
+    _, want, _ = _definition(x[:64], w, targets[:64])
+    # 8,192 words are 512 groups of 2^-23 at most; roundings of dx and of the exponentials have no sign
+    assert abs(float((dx[:64].double() - want).mean())) < 512 * 2.0 ** -23 + 2e-5
+    assert _off(dx[:64], want) < 0.55 * 2.0 ** -8                 # a rounding to 8 bits is 0.43 of its half step in the norm
