@@ -420,8 +420,13 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Epilogue e
     v.z += x.z;
     v.w += x.w;
   }
-  float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
   const int col = tn * w.bn + c;
+  float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (e.cut_addend && c + i < columns) f[i] += e.addend[(int64_t)row * e.addend_pitch + col + i];
+    f[i] *= by;
+  }
   if (e.table != nullptr && e.table_factor[row] != 0.f) {
     const int64_t t = e.targets[row];
     if (t >= 0 && t < e.vocab) {
@@ -613,7 +618,7 @@ int run_convert(const Convert& c, cudaStream_t s) {
   return launch_after(convert_kernel, dim3((unsigned)over((int64_t)c.rows * (c.pitch >> 3), 256)), 256, 0, s, c);
 }
 
-constexpr int kForwardRun = 65536;         // tokens whose half tiles are kept at a time: 200 MB of 50,304 words
+constexpr int64_t kMost = 320ll << 20;     // bytes of what stands for logits at a time, where the rest of a call does not ask for more
 
 struct Forward {
   Room room;
@@ -626,57 +631,73 @@ struct Forward {
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, false, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
     ctas = ctas_of(p.tokens);
-    run = std::min(p.tokens, kForwardRun);
+    run = run_of(p);
     stats = room.take<float2>((int64_t)2 * walk_of(run, p.vocab, p.width, terms_of(p), ctas, false).n_tiles * run);
     sums = room.take<float2>(over(run, 32));
     at_target = room.take<float>(run);
     if (run < p.tokens && p.reduction != SA_REDUCTION_NONE) losses = room.take<float>(p.tokens);
     ticket = room.take<unsigned int>(1);
   }
+  // Tokens whose half tiles are kept at a time: up to 65,536 (200 MB of 50,304 words), of many words fewer.
+  static int run_of(const Problem& p) {
+    const int64_t token = over(p.vocab, kRows * ctas_of(p.tokens)) * 2 * sizeof(float2);
+    return (int)std::min<int64_t>(p.tokens, std::max<int64_t>(256, std::min<int64_t>(65536, kMost / token / 256 * 256)));
+  }
 };
 
 struct Backward {
   Room room;
   Operand x, weight, dz;
-  float *factor, *scale, *largest, *less, *dx_sums = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr;
-  int ctas, piece;
-  int64_t pitch;                 // of dx_sums
+  float *factor, *scale, *largest, *less, *dx_sums = nullptr, *dx_slabs = nullptr, *dw_sums = nullptr, *dw_slabs = nullptr;
+  int ctas, run, piece;
+  int64_t pitch;                 // of dx_sums and dw_sums
   Backward(const Problem& p, void* base) : room{static_cast<char*>(base)} {
-    ctas = ctas_of(p.tokens);
+    run = run_of(p);
+    ctas = ctas_of(run);
     x = operand_of(p, p.x, p.x_dtype, p.x_stride, p.tokens, true, &room);
     weight = operand_of(p, p.weight, p.weight_dtype, p.weight_stride, p.vocab, false, &room);
     factor = room.take<float>(p.tokens);
     scale = room.take<float>(1);
     largest = room.take<float>(1);
     less = room.take<float>(p.tokens);
-    piece = piece_of(p);
-    dz.rows = p.tokens;
+    piece = piece_of(p, run);
     dz.parts = dz_parts(p);
     dz.pitch = up(piece, 64);
-    dz.part = dz.pitch * p.tokens;
+    dz.part = dz.pitch * run;
     dz.base = room.take<uint16_t>(dz.part * dz.parts);
     pitch = up(p.width, 8);
+    int64_t dx = 0, dw = 0;      // slabs of the largest of the products
+    for (int tokens : {run, p.tokens % run})
+      if (tokens > 0) {
+        dx = std::max(dx, slab_floats(dx_walk(p, tokens, piece), ctas));
+        for (int columns : {piece, p.vocab % piece})
+          if (columns > 0) dw = std::max(dw, slab_floats(dw_walk(p, columns, tokens), ctas_of(columns)));
+      }
     if (p.dx != nullptr) {
-      if (piece < p.vocab) dx_sums = room.take<float>(p.tokens * pitch);
-      dx_slabs = room.take<float>(slab_floats(dx_walk(p, piece), ctas));
+      if (piece < p.vocab) dx_sums = room.take<float>(run * pitch);
+      dx_slabs = room.take<float>(dx);
     }
     if (p.dweight != nullptr) {
-      int64_t most = slab_floats(dw_walk(p, piece), ctas_of(piece));
-      if (p.vocab % piece != 0) most = std::max(most, slab_floats(dw_walk(p, p.vocab % piece), ctas_of(p.vocab % piece)));
-      dw_slabs = room.take<float>(most);
+      if (run < p.tokens) dw_sums = room.take<float>(p.vocab * pitch);
+      dw_slabs = room.take<float>(dw);
     }
   }
   // Of few tokens dz is kept in two parts for dW, whose product is bound by what it writes up to here (128 tokens of 50,304 words of 768
   // 107 us a call, with one part 105): the 8 bits of one would make most of its error (2.3e-3 to 2.9e-3 against 64 bits, 1.7e-3 with
   // two).  dx has the first part.
   static int dz_parts(const Problem& p) { return p.product == SA_BF16 && p.tokens <= kRows ? 2 : parts_of(p); }
+  // Tokens of a run: as many as leave a piece of the vocabulary 4,096 columns, or all that there are.  The sums of dW over the runs are kept
+  // in fp32; fewer columns instead would have those of dx read and written more often (131,072 tokens of 50,304 words of 1,024: 42.8 ms in
+  // four runs, 43.2 with 4,096 columns of all tokens in 1.2 GB more).
+  static int run_of(const Problem& p) {
+    const int64_t row = up(std::min(p.vocab, 4096), 64) * 2 * dz_parts(p), most = kMost / row / 256 * 256;
+    return p.tokens <= most ? p.tokens : (int)up(over(p.tokens, over(p.tokens, most)), 256);
+  }
   // Columns of a piece of the vocabulary: its dz takes up to 320 MB (16,384 tokens: 37 tiles of 256 columns, with four tiles across
-  // two whole rounds of 74 clusters in dW), or 4,096 columns where that is more, but no more than 8 GB; of the sizes down to half of
-  // that, the one that leaves the fewest clusters idle in dW.
-  static int piece_of(const Problem& p) {
-    const int64_t column = (int64_t)p.tokens * 2 * dz_parts(p), in_320mb = (320ll << 20) / column / 256 * 256;
-    const int64_t in_8gb = (8ll << 30) / column / 256 * 256, most = std::max<int64_t>({256, std::min<int64_t>(4096, in_8gb), in_320mb});
-    if (p.vocab <= most) return p.vocab;
+  // two whole rounds of 74 clusters in dW); of the sizes down to half of that, the one that leaves the fewest clusters idle in dW.
+  static int piece_of(const Problem& p, int run) {
+    const int64_t column = (int64_t)run * 2 * dz_parts(p), most = kMost / column / 256 * 256;
+    if (up(p.vocab, 64) * column <= kMost) return p.vocab;
     const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, blocks = most / 256;
     int64_t best = 0, at = blocks;
     for (int64_t b = blocks; 2 * b > blocks; --b) {
@@ -688,9 +709,9 @@ struct Backward {
     }
     return (int)(at * 256);
   }
-  Walk dx_walk(const Problem& p, int columns) const { return walk_of(p.tokens, p.width, columns, terms_of(p), ctas, true, piece); }
-  Walk dw_walk(const Problem& p, int columns) const {
-    return walk_of(columns, p.width, p.tokens, p.product == SA_F32 ? kTerms : dz_parts(p), ctas_of(columns), true, p.tokens);
+  Walk dx_walk(const Problem& p, int tokens, int columns) const { return walk_of(tokens, p.width, columns, terms_of(p), ctas, true, piece); }
+  Walk dw_walk(const Problem& p, int columns, int tokens) const {
+    return walk_of(columns, p.width, tokens, p.product == SA_F32 ? kTerms : dz_parts(p), ctas_of(columns), true, tokens);
   }
 };
 
@@ -751,11 +772,12 @@ struct Train {
       dx_slabs = room.take<float>(most);
     }
   }
-  // Tokens of a run: e takes up to 512 MB, or 512 tokens' where that is more; of the sizes down to half of that, the one whose dx takes
+  // Tokens of a run: e takes up to 512 MB, or 256 tokens' where that is more (see prefers_train); of the sizes down to half of that, the one whose dx takes
   // the fewest rounds of the clusters (16,384 tokens of 50,304 words, four tiles across: three runs of 20 tiles of tokens and one of
   // 4 take 3.5 rounds, four runs of 16 take 4).
+  static constexpr int64_t kMost = 512ll << 20;
   static int run_of(const Problem& p) {
-    const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(512, (512ll << 20) / row / 256 * 256) / 256;
+    const int64_t row = up(p.vocab, 64) * 2 * parts_of(p), most = std::max<int64_t>(256, kMost / row / 256 * 256) / 256;
     if (p.tokens <= most * 256) return p.tokens;
     const int64_t across = over(p.width, 2 * kRows), clusters = kSms / 2, all = over(p.tokens, 256);
     auto rounds = [&](int64_t blocks) {                          // in thousandths, as walk_of cuts what is left of whole ones
@@ -811,16 +833,20 @@ int forward(const Problem& p, cudaStream_t s) {
   return launch_after(total_kernel, dim3(1), 1024, 0, s, (const float*)f.losses, p.targets, p.ignore_index, p.tokens, p.reduction, p.loss, p.count);
 }
 
-// A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, written, read and written
-// again, and eight more launches: the smaller of both estimates, in us at 1.4 PFLOP/s (fp32: 0.75) and 6.4 TB/s.  Measured, bf16:
-// 4,096 tokens of 8,000 words of 1,024 202 us by computing the logits again and 232 with the loss, 64 of 50,304 136 and 224, 2,048 of
-// 50,304 of 768 600 and 519; fp32: 1,024 of 8,000 of 512 216 and 212, 512 of 32,000 of 768 634 and 588.
+// A product (and a copy of the table in the products' parts) saved against the fp32 sums of the gradients, of the table's in every run of
+// tokens, and eight more launches: the smaller of both estimates, in us at 1.4 PFLOP/s (fp32: 0.75) and 6.4 TB/s.  Near the border it
+// leans to the second way, whose dW is the more exact one.  Measured, the logits computed again and the gradients with the loss, bf16: 64
+// tokens of 50,304 words of 1,024 132 and 203 us, 1,024 of 50,304 of 768 252 and 264, 2,048 462 and 481 (it takes 481), 4,096 1,181 and
+// 1,007, 16,384 of 1,024 4,480 and 4,200, 4,096 of 262,144 of 256 (four runs) 2,484 and 2,481, of 500,000 4,829 and 6,089; fp32: 1,024 of 8,000 of 512 198 and 189, 512 of
+// 32,000 of 768 559 and 472, 2,048 of 200,000 of 128 3,446 and 3,671 (it takes 3,671).
 bool prefers_train(const Problem& p) {
   if (p.reduction == SA_REDUCTION_NONE || p.product == SA_F16) return false;
   const double values = (double)p.vocab * p.width, tokens = (double)up(p.tokens, kRows);
   double saved = 2.0 * tokens * values * terms_of(p) / (p.product == SA_F32 ? 0.75e9 : 1.4e9);
   if (!in_place(p.weight_dtype, p.product, p.weight, p.weight_stride, p.vocab, p.width)) saved += values * (bytes_of(p.weight_dtype) + 2 * parts_of(p)) / 6.4e6;
-  return saved > 8.0 * (values + tokens * p.width) / 6.4e6 + 50.0;
+  const int64_t run = Train::run_of(p);
+  if (run * up(p.vocab, 64) * 2 * parts_of(p) > Train::kMost) return false;
+  return saved > 8.0 * (values * (double)over(p.tokens, run) + tokens * p.width) / 6.4e6 + 50.0;
 }
 
 int train(const Problem& p, cudaStream_t s) {
@@ -977,60 +1003,68 @@ int backward(const Problem& p, cudaStream_t s) {
   if (st == SA_OK && b.weight.part != 0) st = run_convert(convert_of(p, b.weight, p.weight, p.weight_dtype, p.weight_stride), s);
   const float* scale = half || p.reduction != SA_REDUCTION_NONE ? b.scale : nullptr;
   const Matrix weight = matrix_of(p, b.weight, p.weight, p.weight_dtype, p.weight_stride);
-  for (int v0 = 0; v0 < p.vocab && st == SA_OK; v0 += b.piece) {
-    const int columns = std::min(b.piece, p.vocab - v0);
-    Epilogue e{};
-    e.targets = p.targets;
-    e.column0 = v0;
-    e.lse = reinterpret_cast<const float2*>(p.lse);
-    e.factor = b.factor;
-    e.p = const_cast<uint16_t*>(b.dz.base);
-    e.p_pitch = b.dz.pitch;
-    e.p_part = b.dz.part;
-    e.parts = b.dz.parts;
-    e.half = half;
-    e.scale = scale;
-    e.less = b.less;
-    const Walk logits = walk_of(p.tokens, columns, p.width, terms_of(p), b.ctas, false);
-    st = run<kProbabilities, false, false>(b.ctas, b.x, b.weight, logits, Origin{0, 0}, Origin{v0, 0}, e, status, s);
-    if (st != SA_OK) return st;
-    Operand dz = b.dz;
-    dz.width = columns;
-    const bool first = v0 == 0, last = v0 + columns == p.vocab;
-    if (p.dx != nullptr) {
-      const Walk w = b.dx_walk(p, columns);
-      Epilogue r{};
-      r.half = half;
-      r.out = last ? p.dx : b.dx_sums;
-      r.dtype = last ? p.x_dtype : SA_F32;
-      r.out_pitch = last ? p.width : b.pitch;
-      r.addend = first ? nullptr : b.dx_sums;
-      r.addend_pitch = b.pitch;
-      r.scale = last ? scale : nullptr;
-      r.table = last && b.dz.parts < 3 ? weight.base : nullptr;
-      r.table_dtype = weight.dtype;
-      r.table_stride = weight.stride;
-      r.table_factor = b.less;
-      r.targets = p.targets;
-      r.vocab = p.vocab;
-      r.slabs = b.dx_slabs;
-      r.later = !first;
-      st = run_result<false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
-      if (st == SA_OK && last) st = finish(r, w, b.ctas, s);
+  for (int n0 = 0; n0 < p.tokens && st == SA_OK; n0 += b.run) {
+    const int tokens = std::min(b.run, p.tokens - n0);
+    for (int v0 = 0; v0 < p.vocab && st == SA_OK; v0 += b.piece) {
+      const int columns = std::min(b.piece, p.vocab - v0);
+      Epilogue e{};
+      e.targets = p.targets + n0;
+      e.column0 = v0;
+      e.lse = reinterpret_cast<const float2*>(p.lse) + n0;
+      e.factor = b.factor + n0;
+      e.p = const_cast<uint16_t*>(b.dz.base);
+      e.p_pitch = b.dz.pitch;
+      e.p_part = b.dz.part;
+      e.parts = b.dz.parts;
+      e.half = half;
+      e.scale = scale;
+      e.less = b.less + n0;
+      const Walk logits = walk_of(tokens, columns, p.width, terms_of(p), b.ctas, false);
+      st = run<kProbabilities, false, false>(b.ctas, b.x, b.weight, logits, Origin{n0, 0}, Origin{v0, 0}, e, status, s);
       if (st != SA_OK) return st;
-    }
-    if (p.dweight != nullptr) {
-      const int ctas = ctas_of(columns);
-      const Walk w = b.dw_walk(p, columns);
-      Epilogue r{};
-      r.half = half;
-      r.out = static_cast<char*>(p.dweight) + (size_t)v0 * p.width * bytes_of(p.weight_dtype);
-      r.dtype = p.weight_dtype;
-      r.out_pitch = p.width;
-      r.scale = scale;
-      r.slabs = b.dw_slabs;
-      st = run_result<true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, 0}, r, status, s);
-      if (st == SA_OK) st = finish(r, w, ctas, s);
+      Operand dz = b.dz;
+      dz.rows = tokens;
+      dz.width = columns;
+      if (p.dx != nullptr) {
+        const bool first = v0 == 0, last = v0 + columns == p.vocab;
+        const Walk w = b.dx_walk(p, tokens, columns);
+        Epilogue r{};
+        r.half = half;
+        r.out = last ? static_cast<char*>(p.dx) + (size_t)n0 * p.width * bytes_of(p.x_dtype) : static_cast<void*>(b.dx_sums);
+        r.dtype = last ? p.x_dtype : SA_F32;
+        r.out_pitch = last ? p.width : b.pitch;
+        r.addend = first ? nullptr : b.dx_sums;
+        r.addend_pitch = b.pitch;
+        r.scale = last ? scale : nullptr;
+        r.table = last && b.dz.parts < 3 ? weight.base : nullptr;
+        r.table_dtype = weight.dtype;
+        r.table_stride = weight.stride;
+        r.table_factor = b.less + n0;
+        r.targets = e.targets;
+        r.vocab = p.vocab;
+        r.slabs = b.dx_slabs;
+        r.later = !first;
+        st = run_result<false, true>(b.ctas, dz, b.weight, w, Origin{0, 0}, Origin{0, v0}, r, status, s);
+        if (st == SA_OK && last) st = finish(r, w, b.ctas, s);
+        if (st != SA_OK) return st;
+      }
+      if (p.dweight != nullptr) {
+        const bool first = n0 == 0, last = n0 + tokens == p.tokens;
+        const int ctas = ctas_of(columns);
+        const Walk w = b.dw_walk(p, columns, tokens);
+        Epilogue r{};
+        r.half = half;
+        r.out = last ? static_cast<char*>(p.dweight) + (size_t)v0 * p.width * bytes_of(p.weight_dtype) : static_cast<void*>(b.dw_sums + v0 * b.pitch);
+        r.dtype = last ? p.weight_dtype : SA_F32;
+        r.out_pitch = last ? p.width : b.pitch;
+        r.addend = first ? nullptr : b.dw_sums + v0 * b.pitch;
+        r.addend_pitch = b.pitch;
+        r.cut_addend = !first;
+        r.scale = last ? scale : nullptr;
+        r.slabs = b.dw_slabs;
+        st = run_result<true, true>(ctas, dz, b.x, w, Origin{0, 0}, Origin{0, n0}, r, status, s);
+        if (st == SA_OK) st = finish(r, w, ctas, s);
+      }
     }
   }
   return st;

@@ -129,6 +129,7 @@ struct Epilogue {
   int aligned;                             // its rows start where whole vectors are stored: set with the launch
   const float* addend;                     // fp32, may be null
   int64_t addend_pitch;
+  int cut_addend;                          // cut tiles have it too; otherwise what is added to them stands in their slabs
   int addend_first;                        // its rows start at 32 bytes; others have no scale and no table beside them.  Set with the launch
   const float* scale;                      // may be null
   int scale_rows;                          // one for every row

@@ -50,7 +50,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     The forward keeps a log-sum-exp for every token; the backward computes the logits again, a piece of the vocabulary at a time.  Where
     ``reduction`` leaves one cotangent and the problem is large (bf16 and fp32 products), the gradients are computed with the loss
     instead, up to the cotangent, a product less: their sums, of x's and weight's shapes in fp32, are kept for the backward, which scales
-    them.  Either way up to half a GB of what stands for logits is there at a time.
+    them.  Either way up to half a GB of what stands for logits is there at a time: more tokens go in runs, with a sum of the table's gradient in
+    fp32 beside them.
 
     x and weight have one dtype, or under autocast are rounded to its; their gradients have their own.  bf16 and fp16 products are
     exact with fp32 sums, and the gradient of the logits is rounded to that dtype between its products, but for the target's in x's

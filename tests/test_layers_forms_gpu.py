@@ -176,3 +176,42 @@ def test_what_rows_of_a_table_have_in_common_keeps_its_size(reduction):
     # 8,192 words are 512 groups of 2^-23 at most; roundings of dx and of the exponentials have no sign
     assert abs(float((dx[:64].double() - want).mean())) < 512 * 2.0 ** -23 + 2e-5
     assert _off(dx[:64], want) < 0.55 * 2.0 ** -8                 # a rounding to 8 bits is 0.43 of its half step in the norm
+
+
+@pytest.mark.parametrize("dtype,tokens,vocab,width,reduction", [
+    (BF16, 41100, 4500, 72, "none"), (F16, 50000, 4200, 40, "mean"), (F32, 15000, 5000, 65, "none"), (F16, 90001, 2500, 261, "none"),
+    (F32, 40000, 1500, 20, "sum"), (BF16, 600000, 260, 24, "mean"), (BF16, 130000, 5000, 8, "none")])
+def test_more_tokens_than_a_run_of_the_gradients(dtype, tokens, vocab, width, reduction):
+    """Runs of tokens, and in them pieces of the vocabulary, ragged both: 320 MB of what stands for logits at a time."""
+    gen = torch.Generator("cuda").manual_seed(71)
+    x = torch.randn(tokens, width, generator=gen, device="cuda").to(dtype)
+    w = (torch.randn(vocab, width, generator=gen, device="cuda") * 2.0 / width ** 0.5).to(dtype)
+    targets = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    targets[3::7] = -100
+    targets[tokens // 2:tokens // 2 + 2000] = -100
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    g = torch.rand(tokens, generator=gen, device="cuda") + 0.5 if reduction == "none" else torch.tensor(0.75 if dtype != F16 else 768.0, device="cuda")
+    loss = layers.linear_cross_entropy(a, b, targets, reduction=reduction)
+    got = torch.autograd.grad(loss, (a, b), g, retain_graph=True)
+    again = torch.autograd.grad(loss, (a, b), g)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    counts = targets != -100
+    each = torch.where(counts, g.double(), 0.0) / (int(counts.sum()) if reduction == "mean" else 1)
+    dx, dw, losses = torch.empty(tokens, width, dtype=torch.float64, device="cuda"), torch.zeros(vocab, width, dtype=torch.float64, device="cuda"), []
+    for i in range(0, tokens, 10000):
+        rows = slice(i, i + 10000)
+        z = x[rows].double() @ w.double().T
+        logp, at = torch.log_softmax(z, 1), targets[rows].clamp(min=0)[:, None]
+        losses.append(torch.where(counts[rows], -logp.gather(1, at)[:, 0], 0.0))
+        dz = logp.exp_().scatter_add_(1, at, -torch.ones(len(at), 1, dtype=torch.float64, device="cuda")) * each[rows, None]
+        dx[rows] = dz @ w.double()
+        dw += dz.T @ x[rows].double()
+    losses = torch.cat(losses)
+    want = losses if reduction == "none" else losses.sum() / (int(counts.sum()) if reduction == "mean" else 1)
+    assert _off(loss.detach(), want) < 6e-7
+    # dx: its rounding and, of 16 bits, that of what is not at the target; dw: its rounding and dz's
+    half = torch.finfo(dtype).eps / 2 if dtype != F32 else 1.2e-6
+    assert _off(got[0], dx) < 0.55 * half + 1.2e-6 and _off(got[1], dw) < 0.66 * half + 1.2e-6 and (got[0][~counts] == 0).all()
+    one = torch.autograd.grad(layers.linear_cross_entropy(a, b.detach(), targets, reduction=reduction), a, g)[0]
+    other = torch.autograd.grad(layers.linear_cross_entropy(a.detach(), b, targets, reduction=reduction), b, g)[0]
+    assert torch.equal(one, got[0]) and torch.equal(other, got[1])
