@@ -213,11 +213,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* stats,
 // What e is relative to: the target's logit; +inf for a token that does not count, NaN for a target outside the vocabulary.  A warp a token.
 __global__ void __launch_bounds__(256) reference_kernel(const void* x, int x_dtype, int64_t x_stride, const void* weight, int weight_dtype,
                                                         int64_t weight_stride, const int64_t* targets, int64_t ignore_index, int tokens, int vocab,
-                                                        int width, float* ref, int* any) {
+                                                        int width, float* ref, int* any, int run) {
   after_previous_kernel();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *any = 0;
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= tokens) return;
+  if (lane == 0 && row % run == 0) any[row / run] = 0;
   const int64_t t = targets[row];
   float sum = 0.f;
   if (t != ignore_index && t >= 0 && t < vocab) {
@@ -735,7 +735,7 @@ struct Train {
   Operand x, weight, e, scaled;
   int run;                       // tokens of a run
   float *ref, *losses, *less, *e_target, *inverse, *dx_slabs = nullptr, *dw_slabs = nullptr;
-  int *far, *any;
+  int *far, *any;                // of tokens, of runs
   void* sorted = nullptr;        // of the targets
   float2* stats;
   float* at_target;
@@ -747,7 +747,7 @@ struct Train {
     losses = room.take<float>(p.tokens);
     less = room.take<float>(p.tokens);
     far = room.take<int>(p.tokens);
-    any = room.take<int>(1);
+    any = room.take<int>(over(p.tokens, run));
     at_target = room.take<float>(run);
     e_target = room.take<float>(run);
     inverse = room.take<float>(run);
@@ -859,7 +859,7 @@ int train(const Problem& p, cudaStream_t s) {
   const Matrix x = matrix_of(p, t.x, p.x, p.x_dtype, p.x_stride), weight = matrix_of(p, t.weight, p.weight, p.weight_dtype, p.weight_stride);
   if (st == SA_OK)
     st = launch_after(reference_kernel, dim3((unsigned)over(p.tokens, 8)), 256, 0, s, x.base, x.dtype, x.stride, weight.base, weight.dtype, weight.stride,
-                      p.targets, p.ignore_index, p.tokens, p.vocab, p.width, t.ref, t.any);
+                      p.targets, p.ignore_index, p.tokens, p.vocab, p.width, t.ref, t.any, t.run);
   for (int n0 = 0; n0 < p.tokens && st == SA_OK; n0 += t.run) {
     const int tokens = std::min(t.run, p.tokens - n0);
     const bool first = n0 == 0, last = n0 + tokens == p.tokens;
@@ -886,7 +886,7 @@ int train(const Problem& p, cudaStream_t s) {
     r.width = p.width;
     r.ref = t.ref + n0;
     r.far = t.far + n0;
-    r.any = t.any;
+    r.any = t.any + n0 / t.run;
     r.loss = t.losses + n0;
     r.inverse = t.inverse;
     r.less = t.less + n0;
@@ -902,7 +902,7 @@ int train(const Problem& p, cudaStream_t s) {
     r.parts = e.parts;
     for (int again = 0; again < 2 && st == SA_OK; ++again) {       // the second time for rows that are far, where there are any
       e.only = again ? r.far : nullptr;
-      e.any = again ? t.any : nullptr;
+      e.any = again ? r.any : nullptr;
       r.again = again;
       st = run<kBoth, false, false>(ctas_of(t.run), t.x, t.weight, logits, Origin{n0, 0}, Origin{0, 0}, e, status, s);
       if (st == SA_OK) st = launch_after(rows_kernel, dim3((unsigned)over(tokens, 32)), kJoinThreads, 0, s, (const Rows)r);

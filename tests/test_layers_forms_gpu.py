@@ -215,3 +215,26 @@ def test_more_tokens_than_a_run_of_the_gradients(dtype, tokens, vocab, width, re
     one = torch.autograd.grad(layers.linear_cross_entropy(a, b.detach(), targets, reduction=reduction), a, g)[0]
     other = torch.autograd.grad(layers.linear_cross_entropy(a.detach(), b, targets, reduction=reduction), b, g)[0]
     assert torch.equal(one, got[0]) and torch.equal(other, got[1])
+
+
+def test_a_far_row_has_its_own_run_alone_gone_through_once_more():
+    """Eight runs of tokens; the product of the logits is about a quarter of a run."""
+    import test_layers_gpu
+
+    gen = torch.Generator("cuda").manual_seed(81)
+    x = torch.randn(16384, 512, generator=gen, device="cuda").to(BF16)
+    w = (torch.randn(131072, 512, generator=gen, device="cuda") * 0.05).to(BF16)
+    targets = torch.randint(0, 131072, (16384,), generator=gen, device="cuda")
+    ones, far = torch.ones((), device="cuda"), x.clone()
+    far[7] = w[(targets[7] + 1) % 131072] * 200             # the logit of another word is 256
+    times = {}
+    for _ in range(4):
+        for name, a in (("near", x), ("far", far)):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            loss, dx, _ = test_layers_gpu._with_the_loss(a, w, targets, -100, "sum", BF16, ones)
+            end.record()
+            torch.cuda.synchronize()
+            times[name] = min(times.get(name, 1e9), begin.elapsed_time(end))
+            assert torch.isfinite(loss) and torch.isfinite(dx).all()
+    assert times["far"] < 1.13 * times["near"], times       # 1.03; with every later run once more 1.25
