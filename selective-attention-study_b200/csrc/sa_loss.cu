@@ -683,9 +683,9 @@ struct Backward {
     }
   }
   // Of few tokens dz is kept in two parts for dW, whose product is bound by what it writes up to here (128 tokens of 50,304 words of 768
-  // 107 us a call, with one part 105): the 8 bits of one would make most of its error (2.3e-3 to 2.9e-3 against 64 bits, 1.7e-3 with
-  // two).  dx has the first part.
-  static int dz_parts(const Problem& p) { return p.product == SA_BF16 && p.tokens <= kRows ? 2 : parts_of(p); }
+  // 107 us a call, with one part 105): the bits of one would make most of its error (2.3e-3 to 2.9e-3 against 64 bits, 1.7e-3 with
+  // two; fp16 2.6e-4 to 4e-4 and 2.1e-4).  dx has the first part.
+  static int dz_parts(const Problem& p) { return p.product != SA_F32 && p.tokens <= kRows ? 2 : parts_of(p); }
   // Tokens of a run: as many as leave a piece of the vocabulary 4,096 columns, or all that there are.  The sums of dW over the runs are kept
   // in fp32; fewer columns instead would have those of dx read and written more often (131,072 tokens of 50,304 words of 1,024: 42.8 ms in
   // four runs, 43.2 with 4,096 columns of all tokens in 1.2 GB more).

@@ -375,8 +375,10 @@ __device__ __forceinline__ void store_parts(const Epilogue& e, float (&p)[32], b
     if (part + 1 < e.parts) {                                                // what is left for the next part: exact
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[2 * i] -= __uint_as_float(w[i] << 16);
-        p[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
+        const float2 kept = e.half ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
+                                   : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        p[2 * i] -= kept.x;
+        p[2 * i + 1] -= kept.y;
       }
     }
   }

@@ -238,3 +238,23 @@ def test_a_far_row_has_its_own_run_alone_gone_through_once_more():
             times[name] = min(times.get(name, 1e9), begin.elapsed_time(end))
             assert torch.isfinite(loss) and torch.isfinite(dx).all()
     assert times["far"] < 1.13 * times["near"], times       # 1.03; with every later run once more 1.25
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,reduction", [(1, "sum"), (2, "none"), (9, "mean"), (64, "none"), (128, "sum")])
+def test_few_tokens_dw_is_as_exact_as_its_type(tokens, reduction, dtype):
+    """dz in two parts; in one, a token's whole part of dw would be off by what its target's dz is rounded by."""
+    for seed in range(6):
+        gen = torch.Generator("cuda").manual_seed(90 + seed)
+        x = torch.randn(tokens, 1000, generator=gen, device="cuda").to(dtype)
+        w = (torch.randn(300, 1000, generator=gen, device="cuda") * 0.1).to(dtype).requires_grad_(True)
+        targets = torch.randint(0, 300, (tokens,), generator=gen, device="cuda")
+        loss = layers.linear_cross_entropy(x, w, targets, reduction=reduction)
+        g = (torch.rand(loss.shape, generator=gen, device="cuda") + 0.5) * (1024.0 if dtype == F16 else 1.0)
+        (dw,) = torch.autograd.grad(loss, w, g)
+        z = x.double() @ w.detach().double().T
+        dz = torch.softmax(z, 1) - torch.nn.functional.one_hot(targets, 300)
+        want = (dz * (g if reduction == "none" else g / (tokens if reduction == "mean" else 1)).double().reshape(-1, 1)).T @ x.double()
+        # a rounding to nearest is 0.43 of its half step in the norm, where values lie anywhere between two powers of two; of 1,000 that are
+        # most of it, give or take a tenth
+        assert _off(dw, want) < 0.48 * torch.finfo(dtype).eps / 2, seed
