@@ -669,7 +669,7 @@ sa_norm norm_of(const Tensor& x, const Tensor& weight, const Tensor& bias, doubl
 
 // {y} or {sum, y}; `stats` is what the backward needs, undefined where there will be none.
 variable_list run_norm(const Tensor& x_in, const Tensor& branch_in, const Tensor& weight, const Tensor& bias, double eps, at::ScalarType type,
-                       Tensor* rows, Tensor* stats) {
+                       Tensor* stats) {
   const Tensor x = rows_in(x_in);
   const Tensor y = fresh(x_in.sizes(), type, x_in);
   Tensor sum, branch;
@@ -678,7 +678,6 @@ variable_list run_norm(const Tensor& x_in, const Tensor& branch_in, const Tensor
     sum = fresh(x_in.sizes(), x_in.scalar_type(), x_in);
   }
   if (stats != nullptr) *stats = fresh({x.size(0), 2}, at::kFloat, x);
-  if (rows != nullptr) *rows = x;
   if (x.numel() > 0) {
     sa_norm p = norm_of(x, weight, bias, eps);
     p.y_dtype = code_of(y);
@@ -700,8 +699,8 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& branch, const std::optional<Tensor>& weight,
                                const std::optional<Tensor>& bias, double eps, int64_t type) {
     const c10::cuda::CUDAGuard guard(x.device());
-    Tensor rows, stats;
-    const variable_list out = run_norm(x, given(branch), given(weight), given(bias), eps, (at::ScalarType)type, &rows, &stats);
+    Tensor stats;
+    const variable_list out = run_norm(x, given(branch), given(weight), given(bias), eps, (at::ScalarType)type, &stats);
     // what is normalised: the sum, or x
     ctx->save_for_backward({branch ? out[0] : x, given(weight), given(bias), stats});
     ctx->saved_data["eps"] = eps;
@@ -790,7 +789,7 @@ variable_list layer_norm(const Tensor& x, const std::optional<Tensor>& branch, c
   if (c10::GradMode::is_enabled() && (x.requires_grad() || wants(branch) || wants(weight) || wants(bias)))
     return LayerNorm::apply(x, branch, w, b, eps, (int64_t)type);
   const c10::cuda::CUDAGuard guard(x.device());
-  return run_norm(x, given(branch), given(w), given(b), eps, type, nullptr, nullptr);
+  return run_norm(x, given(branch), given(w), given(b), eps, type, nullptr);
 }
 
 sa_embedding embedding_of(const Tensor& idx, int64_t vocab, int64_t width, double scale) {
@@ -921,7 +920,7 @@ Tensor run_loss(const Tensor& x, const Tensor& weight, const Tensor& targets, in
   return loss;
 }
 
-// The loss with its gradients up to the cotangent, which is one number: a product less than computing the logits again.
+// The loss with its gradients up to the cotangent, which is one number: a product less than computing the logits again.  There are tokens.
 struct LinearLossTrained : public torch::autograd::Function<LinearLossTrained> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& targets, int64_t ignore_index, int64_t reduction,
                         int64_t product) {
@@ -931,21 +930,15 @@ struct LinearLossTrained : public torch::autograd::Function<LinearLossTrained> {
     Tensor dx, dweight;
     if (x_in.requires_grad()) dx = fresh(x_in.sizes(), at::kFloat, x);
     if (weight_in.requires_grad()) dweight = fresh(weight_in.sizes(), at::kFloat, x);
-    if (x.size(0) == 0) {                             // a mean over nothing is no number
-      loss.fill_(reduction == SA_REDUCTION_MEAN ? std::nan("") : 0.0);
-      count.zero_();
-      if (dweight.defined()) dweight.zero_();
-    } else {
-      sa_linear_loss p = loss_of(x, weight, targets, ignore_index, reduction, product);
-      p.loss = loss.data_ptr<float>();
-      p.count = count.data_ptr<float>();
-      p.dx_sums = static_cast<float*>(pointer(dx));
-      p.dweight_sums = static_cast<float*>(pointer(dweight));
-      p.workspace_bytes = sa_linear_loss_train_bytes(&p);
-      const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
-      p.workspace = workspace.data_ptr();
-      check("sa_linear_loss_train", sa_linear_loss_train(&p));
-    }
+    sa_linear_loss p = loss_of(x, weight, targets, ignore_index, reduction, product);
+    p.loss = loss.data_ptr<float>();
+    p.count = count.data_ptr<float>();
+    p.dx_sums = static_cast<float*>(pointer(dx));
+    p.dweight_sums = static_cast<float*>(pointer(dweight));
+    p.workspace_bytes = sa_linear_loss_train_bytes(&p);
+    const Tensor workspace = fresh({(int64_t)p.workspace_bytes}, at::kByte, x);
+    p.workspace = workspace.data_ptr();
+    check("sa_linear_loss_train", sa_linear_loss_train(&p));
     ctx->save_for_backward({dx, dweight, count});
     ctx->saved_data["args"] = packed({reduction, product, (int64_t)x.scalar_type(), (int64_t)weight.scalar_type()});
     ctx->saved_data["tokens"] = x.size(0);
@@ -975,9 +968,7 @@ struct LinearLossTrained : public torch::autograd::Function<LinearLossTrained> {
       p.tokens = (int32_t)ctx->saved_data["tokens"].toInt();
       p.vocab = (int32_t)ctx->saved_data["vocab"].toInt();
       p.width = (int32_t)ctx->saved_data["width"].toInt();
-      if (p.tokens == 0) {
-        if (grads[1].defined()) grads[1].zero_();
-      } else if (grads[0].defined() || grads[1].defined()) {
+      if (grads[0].defined() || grads[1].defined()) {
         p.count = count.data_ptr<float>();
         p.dloss = dloss.data_ptr<float>();
         p.dx_sums = static_cast<float*>(pointer(dx_sums));
