@@ -452,8 +452,10 @@ int sa_beam_select(const sa_beam* p);
  *            backward; count (1,) fp32 likewise
  *   loss     (tokens,) fp32 without a reduction (0 where the target is ignored), else one number
  *   dloss    of loss's shape; dx, dweight contiguous, of x's and weight's type, either may be null
- * sums are fp32; the gradient of the logits is rounded to `product` between the products (fp16: scaled by 2^14 over the
- * largest |dloss|; SA_F32: three parts).  A gradient is the same from call to call. */
+ * sums are fp32; the gradient of the logits is rounded to `product` between the products (fp16: scaled by 2^14 over the largest |dloss|;
+ * SA_F32: in three parts; of up to 128 tokens in two for dweight), and what that takes from the target's is added to dx in fp32.  One
+ * dloss scales the results.  Workspaces hold up to 512 MB of what stands for logits, beside copies of x and weight where those are not of the
+ * product's type at multiples of 16 bytes, and fp32 sums of the gradients.  A gradient is the same from call to call. */
 enum sa_reduction { SA_REDUCTION_NONE = 0, SA_REDUCTION_SUM = 1, SA_REDUCTION_MEAN = 2 };
 typedef struct sa_linear_loss {
   int32_t struct_bytes;   /* sizeof(sa_linear_loss) */
@@ -479,7 +481,8 @@ size_t sa_linear_loss_backward_bytes(const sa_linear_loss* p);
 int sa_linear_loss_backward(const sa_linear_loss* p);
 /* The same with a product less, where there is a reduction and product is SA_BF16 or SA_F32: _train writes loss and count, and the
  * gradients' sums for a sum's cotangent of 1; _scale makes dx and dweight of them (those that are not null) for dloss and count.
- * lse is not used.  In products of SA_BF16 the softmax enters as exponentials of 8 bits, and x over their sum rounded to 8 bits; the
+ * lse is not used.  Exponentials of 256 tokens at least are kept at a time (with more than 2^20 words of SA_BF16, 349,504 of SA_F32, that is
+ * more than 512 MB, and _prefers_train is 0).  In products of SA_BF16 the softmax enters as exponentials of 8 bits, and x over their sum rounded to 8 bits; the
  * targets' part is added in fp32.  _prefers_train: 1 where that is the faster way, by an estimate (small problems are not). */
 int sa_linear_loss_prefers_train(const sa_linear_loss* p);
 size_t sa_linear_loss_train_bytes(const sa_linear_loss* p);

@@ -3,8 +3,8 @@
 // Forward: a copy.  Backward, for vocab rows and N tokens, three launches:
 //   order   sorts the tokens by their row, tokens of a row in order.  A CTA owns a range of rows and reads all N indices: its 32
 //           warps take a run of tokens each, count theirs by row, and after a prefix sum over the warps every warp writes its own
-//           tokens' places without another barrier.  148 CTAs read N indices each out of L2, which costs less than the launches of
-//           a radix sort.
+//           tokens' places without another barrier.  148 CTAs, or one for every 1,600 rows of a larger table, read N indices each
+//           out of L2, which costs less than the launches of a radix sort.
 //   sum     pieces of 4 to 32 sorted tokens: their gradients are summed row by row in that order; a row inside one piece is finished,
 //           the parts of rows that cross pieces are kept.  Rows that no token names are written as zeros beside it.
 //   join    sums the parts of each row that crossed pieces.

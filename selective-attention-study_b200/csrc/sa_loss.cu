@@ -17,7 +17,8 @@
 // Otherwise (a cotangent for every token; fp16, whose five bits of exponent do not hold e; problems so small that a product costs
 // less than the sums of the gradients, written and read): the backward computes the logits again in pieces of the vocabulary, turns
 // a piece's into dz in 16 bits, and reads them with the two products of the gradients; what the rounding takes from dz at the target is
-// added to dx in fp32, and one cotangent scales the results.  Four products in all; the sums of dx over the pieces stay in fp32.
+// added to dx in fp32, and one cotangent scales the results.  Four products in all; the sums of dx over the pieces stay in fp32.  Beyond
+// 40,960 tokens (fp32: 13,568) they come in runs, so that no more than 320 MB of dz is there; the sums of dW over the runs stay in fp32.
 #include "sa_loss.cuh"
 
 #include <algorithm>

@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(kBlock<T>, T == 512 ? 2 : 1) forward_kernel(co
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 
 // Rows of more than 8,192 values leave no registers for their columns' sums: those are in shared memory, a thread's apart by the threads
-// (4,000 rows of 12,288 in bf16 with a bias: 340 us with spilled registers, 230 this way; rows of 4,096 and 8,192 gain nothing from it).
+// (4,000 rows of 12,288 in bf16 with a bias: 340 us with the sums in registers, most of them spilled, 230 this way, where a thread still spills
+// 380 to 640 bytes; rows of 4,096 and 8,192, which spill 80 to 150 bytes, gain nothing from it).
 template <int T, int NV> constexpr bool kSumsShared = T * NV * 8 > 8192;
 
 // A thread's part of the gradient: of rows, h and g = dy in and dx out, and its columns' sums for dw and db.
@@ -469,7 +470,8 @@ bool copies_of(const sa_norm& p, int threads, int rows_at_a_time, Copies* c) {
   return c->stage * kRing <= (threads < 1024 ? 104 : 212) * 1024;        // two CTAs an SM, or the one that has all registers
 }
 
-// CTAs of the backward: at most 768 threads an SM, or as many as their stages leave room for.
+// CTAs of the backward: at most 768 threads an SM, one CTA at least (of 1,024 threads for rows of 4,097 to 8,192 values), or as many as
+// their stages leave room for.
 int blocks_of(const sa_norm& p) {
   int blocks = 0;
   by_width<false>(p.width, [&](auto threads, auto chunks) {

@@ -54,9 +54,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     fp32 beside them.
 
     x and weight have one dtype, or under autocast are rounded to its; their gradients have their own.  bf16 and fp16 products are
-    exact with fp32 sums, and the gradient of the logits is rounded to that dtype between its products, but for the target's in x's
-    gradient (fp16: scaled by the largest cotangent, so tokens whose cotangent is 2^-19 of it or less lose bits).  fp32 operands are split into three bf16
-    parts, which keep 24 bits.
+    exact with fp32 sums (tensor cores round towards zero: at most 1,024 products of a logit and 8,192 of a gradient are added that way), and
+    the gradient of the logits is rounded to that dtype between its products, but for the target's in x's gradient (fp16: scaled by the
+    largest cotangent, so tokens whose cotangent is 2^-19 of it or less lose bits).  weight's gradient shows that rounding beside its own
+    beyond 128 tokens: 2.4e-3 of its norm where bf16 by itself is 1.7e-3, 1.8e-3 where the gradients come with the loss.  fp32 operands
+    are split into three bf16 parts, which keep 24 bits.
 
     What stands in x where a target is ignored does not matter.  A target outside the vocabulary that is not ``ignore_index`` makes its
     loss and the gradients NaN.  The mean over no target at all is NaN, its gradients are zeros."""
