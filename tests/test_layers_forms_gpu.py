@@ -258,3 +258,45 @@ def test_few_tokens_dw_is_as_exact_as_its_type(tokens, reduction, dtype):
         # a rounding to nearest is 0.43 of its half step in the norm, where values lie anywhere between two powers of two; of 1,000 that are
         # most of it, give or take a tenth
         assert _off(dw, want) < 0.48 * torch.finfo(dtype).eps / 2, seed
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_tokens_than_a_run_of_half_tiles(dtype):
+    """Of 130,000 words 41,216 tokens' at a time: a token's loss is the same wherever it stands."""
+    gen = torch.Generator("cuda").manual_seed(101)
+    x = torch.randn(45000, 24, generator=gen, device="cuda").to(dtype)
+    w = (torch.randn(130000, 24, generator=gen, device="cuda") * 0.4).to(dtype)
+    targets = torch.randint(0, 130000, (45000,), generator=gen, device="cuda")
+    targets[41000:41500] = -100
+    losses = layers.linear_cross_entropy(x, w, targets, reduction="none")
+    halves = [layers.linear_cross_entropy(x[s], w, targets[s], reduction="none") for s in (slice(0, 20000), slice(20000, 45000))]
+    assert torch.equal(losses, torch.cat(halves)) and (losses[41000:41500] == 0).all() and torch.isfinite(losses).all()
+    for reduction in ("sum", "mean"):
+        want = losses.double().sum() / (44500 if reduction == "mean" else 1)
+        assert abs(float(layers.linear_cross_entropy(x, w, targets, reduction=reduction)) - float(want)) < 2.0 ** -22 * float(want)
+
+
+def test_captured_gradients_of_several_runs_follow_their_inputs():
+    gen = torch.Generator("cuda").manual_seed(102)
+    x = torch.randn(41100, 40, generator=gen, device="cuda").to(BF16).requires_grad_(True)
+    w = (torch.randn(4400, 40, generator=gen, device="cuda") * 0.3).to(BF16).requires_grad_(True)
+    targets, g = torch.randint(0, 4400, (41100,), generator=gen, device="cuda"), torch.rand(41100, generator=gen, device="cuda")
+
+    def step():
+        return torch.autograd.grad(layers.linear_cross_entropy(x, w, targets, reduction="none"), (x, w), g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        x.mul_(0.5)
+        w.neg_()
+        targets[::3] = -100
+        g.add_(0.25)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step())) and (got[0][::3] == 0).all()
